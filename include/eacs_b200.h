@@ -77,6 +77,86 @@ EACS_API int eacs_project(const void* x, int x_dtype, const float* gamma, const 
 /* Bytes of eacs_project's workspace for M rows (its LayerNorm statistics). */
 EACS_API size_t eacs_project_workspace_size(int64_t M);
 
+/* LayerNorm of s = x (+ residual) over the last d elements of `rows` rows:
+ * y = (s - mean) / sqrt(var + eps) * weight + bias, statistics in float32,
+ * rounded once to dtype.  It is the norm in front of an EACS layer's
+ * projections (cst_ssm/modules/eacs.py:334) and, with the blended branches as
+ * the residual, MultiScaleEACS's out_norm(x + fused)
+ * (cst_ssm/modules/multiscale.py:176-179), for training too.  x and residual
+ * have their row stride in elements (at least d); y is dense; weight and bias
+ * (d) of w_dtype may be NULL (1 and 0); residual may be NULL.  d goes up to
+ * 8192; rows that start and end on 16 bytes are read 16 bytes at a time. */
+EACS_API int eacs_layer_norm_fwd(const void* x, int64_t x_stride, const void* residual, int64_t residual_stride,
+                                 int dtype, const void* weight, const void* bias, int w_dtype, float eps, void* y,
+                                 int64_t rows, int64_t d, void* stream);
+
+/* Its backward pass.  dx (dense, dtype) is the gradient of x and of residual
+ * alike; dweight and dbias (d, w_dtype; either may be NULL) are sums over the
+ * rows in float32, added in a fixed order.  The statistics are taken again
+ * from x and residual.  The workspace (16-byte aligned) is needed when dweight
+ * or dbias is asked for. */
+EACS_API int eacs_layer_norm_bwd(const void* x, int64_t x_stride, const void* residual, int64_t residual_stride,
+                                 const void* dy, int64_t dy_stride, int dtype, const void* weight, int w_dtype,
+                                 float eps, void* dx, void* dweight, void* dbias, void* workspace,
+                                 size_t workspace_bytes, int64_t rows, int64_t d, void* stream);
+/* Bytes of its workspace (0 if the sizes are unsupported). */
+EACS_API size_t eacs_layer_norm_bwd_workspace_size(int64_t rows, int64_t d);
+
+/* The gated delta rule: a recurrence over a matrix state beside the diagonal
+ * scans.  For each head a state S (K x V, float32) and per token
+ *   S' = exp(g) S,  u = beta (v - S'^T k),  S = S' + k u^T,  o = scale S^T q.
+ * q, k (B,L,Hk,K) and v (B,L,Hv,V) of dtype, g and beta (B,L,Hv) of
+ * gate_dtype; strides are those of batch, token and head in elements, the
+ * last dimension is dense.  Hv is a multiple of Hk: value head h reads key
+ * head h / (Hv / Hk).  g <= 0 is a decay's logarithm (-inf clears the state).
+ * lengths (B) int32 or NULL: row b has min(max(lengths[b], 0), L) tokens;
+ * what lies behind is not read, its outputs and gradients are 0.
+ * initial_state (B,Hv,K,V) float32 dense or NULL (zeros).  K goes up to 128,
+ * V to 1024.  Rows of q, k, v that start on 16 bytes, with K and V multiples
+ * of 8, are read 16 bytes at a time. */
+typedef struct EacsDelta {
+    const void* q;
+    const void* k;
+    const void* v;
+    const void* g;
+    const void* beta;
+    int64_t q_stride[3];
+    int64_t k_stride[3];
+    int64_t v_stride[3];
+    int64_t g_stride[3];
+    int64_t beta_stride[3];
+    const int32_t* lengths;
+    const float* initial_state;
+    int64_t B, L, Hk, Hv, K, V;
+    float scale;
+    int32_t dtype;
+    int32_t gate_dtype;
+} EacsDelta;
+
+/* Chunked forward: o (B,L,Hv,V) dense of dtype; final_state (B,Hv,K,V)
+ * float32 or NULL.  With training != 0 the workspace holds what
+ * eacs_delta_bwd reads and is kept, unchanged, until then.  Products run on the
+ * tensor cores with operands split in two (tf32, 22 significant bits); all
+ * sums and the state are float32. */
+EACS_API int eacs_delta_fwd(const EacsDelta* p, void* o, float* final_state, void* workspace, size_t workspace_bytes,
+                            int training, void* stream);
+EACS_API size_t eacs_delta_workspace_size(const EacsDelta* p, int training);
+
+/* Backward: dout (B,L,Hv,V) of dtype with its strides, dfinal (B,Hv,K,V)
+ * float32 or NULL (the final state's gradient); dq, dk, dv dense of dtype
+ * (dq and dk summed over the value heads of a key head), dg and dbeta dense
+ * of gate_dtype, dinitial (B,Hv,K,V) float32 or NULL.  `saved` is the
+ * workspace of the training forward with the same arguments. */
+EACS_API int eacs_delta_bwd(const EacsDelta* p, const void* dout, const int64_t* dout_stride, const float* dfinal,
+                            void* dq, void* dk, void* dv, void* dg, void* dbeta, float* dinitial, const void* saved,
+                            size_t saved_bytes, void* workspace, size_t workspace_bytes, void* stream);
+EACS_API size_t eacs_delta_bwd_workspace_size(const EacsDelta* p);
+
+/* The same recurrence token by token in float32, without a workspace: for one
+ * token, or a few.  final_state may be initial_state (updated in place) or
+ * NULL. */
+EACS_API int eacs_delta_step(const EacsDelta* p, void* o, float* final_state, void* stream);
+
 /* Failure-path check (no counterpart in the reference): one CTA waits, with
  * the library's bounded waits (CTA scope and cluster scope) limited to
  * `polls` polls (1..65536), on an mbarrier phase that nothing completes.

@@ -81,6 +81,53 @@ int eacs_project(const void* x, int x_dtype, const float* gamma, const float* be
     return eacs::project_fwd(c, static_cast<cudaStream_t>(stream));
 }
 
+int eacs_layer_norm_fwd(const void* x, int64_t x_stride, const void* residual, int64_t residual_stride, int dtype,
+                        const void* weight, const void* bias, int w_dtype, float eps, void* y, int64_t rows,
+                        int64_t d, void* stream) {
+    eacs::LayerNormCall c{x, x_stride, residual, residual_stride, nullptr, 0, dtype, weight, bias, w_dtype, eps,
+                          y, nullptr, nullptr, nullptr, 0, rows, d, false};
+    return eacs::layer_norm(c, static_cast<cudaStream_t>(stream));
+}
+
+size_t eacs_layer_norm_bwd_workspace_size(int64_t rows, int64_t d) {
+    return eacs::layer_norm_bwd_workspace_size(rows, d);
+}
+
+int eacs_layer_norm_bwd(const void* x, int64_t x_stride, const void* residual, int64_t residual_stride,
+                        const void* dy, int64_t dy_stride, int dtype, const void* weight, int w_dtype, float eps,
+                        void* dx, void* dweight, void* dbias, void* workspace, size_t workspace_bytes, int64_t rows,
+                        int64_t d, void* stream) {
+    eacs::LayerNormCall c{x, x_stride, residual, residual_stride, dy, dy_stride, dtype, weight, nullptr, w_dtype, eps,
+                          dx, dweight, dbias, workspace, workspace_bytes, rows, d, true};
+    return eacs::layer_norm(c, static_cast<cudaStream_t>(stream));
+}
+
+size_t eacs_delta_workspace_size(const EacsDelta* p, int training) {
+    return p ? eacs::delta_workspace_size(*p, training != 0) : 0;
+}
+
+int eacs_delta_fwd(const EacsDelta* p, void* o, float* final_state, void* workspace, size_t workspace_bytes,
+                   int training, void* stream) {
+    if (!p) return eacs::fail(EACS_ERR_INVALID, "eacs_delta_fwd: null arguments");
+    return eacs::delta_fwd(*p, o, final_state, workspace, workspace_bytes, training != 0,
+                           static_cast<cudaStream_t>(stream));
+}
+
+size_t eacs_delta_bwd_workspace_size(const EacsDelta* p) { return p ? eacs::delta_bwd_workspace_size(*p) : 0; }
+
+int eacs_delta_bwd(const EacsDelta* p, const void* dout, const int64_t* dout_stride, const float* dfinal, void* dq,
+                   void* dk, void* dv, void* dg, void* dbeta, float* dinitial, const void* saved, size_t saved_bytes,
+                   void* workspace, size_t workspace_bytes, void* stream) {
+    if (!p || !dout_stride) return eacs::fail(EACS_ERR_INVALID, "eacs_delta_bwd: null arguments");
+    eacs::DeltaGrads d{dout, {dout_stride[0], dout_stride[1], dout_stride[2]}, dfinal, dq, dk, dv, dg, dbeta, dinitial};
+    return eacs::delta_bwd(*p, d, saved, saved_bytes, workspace, workspace_bytes, static_cast<cudaStream_t>(stream));
+}
+
+int eacs_delta_step(const EacsDelta* p, void* o, float* final_state, void* stream) {
+    if (!p) return eacs::fail(EACS_ERR_INVALID, "eacs_delta_step: null arguments");
+    return eacs::delta_step(*p, o, final_state, static_cast<cudaStream_t>(stream));
+}
+
 int eacs_wait_selftest(int polls, void* stream) {
     return eacs::wait_selftest(polls, static_cast<cudaStream_t>(stream));
 }

@@ -325,6 +325,46 @@ struct FuseCall {
 };
 int branch_fuse(const FuseCall& c, cudaStream_t stream);
 
+// layer_norm.cu: LayerNorm of x (+ residual), forward (dy null) and backward
+struct LayerNormCall {
+    const void* x;         // (rows, d) of dtype, row stride x_stride (elements)
+    int64_t x_stride;
+    const void* residual;  // or null
+    int64_t r_stride;
+    const void* dy;        // backward: upstream gradient
+    int64_t dy_stride;
+    int dtype;
+    const void* weight;    // (d) of w_dtype or null
+    const void* bias;
+    int w_dtype;
+    float eps;
+    void* out;             // (rows, d) dense: y, or the gradient of x
+    void* dweight;         // (d) of w_dtype or null
+    void* dbias;
+    void* workspace;
+    size_t workspace_bytes;
+    int64_t rows, d;
+    bool backward;
+};
+size_t layer_norm_bwd_workspace_size(int64_t rows, int64_t d);
+int layer_norm(const LayerNormCall& c, cudaStream_t stream);
+
+// delta.cu: the gated delta rule
+struct DeltaGrads {
+    const void* dout;
+    int64_t dout_stride[3];
+    const float* dfinal;  // or null
+    void *dq, *dk, *dv, *dg, *dbeta;
+    float* dinitial;      // or null
+};
+size_t delta_workspace_size(const EacsDelta& p, bool training);
+size_t delta_bwd_workspace_size(const EacsDelta& p);
+int delta_fwd(const EacsDelta& p, void* o, float* final_state, void* ws, size_t ws_bytes, bool training,
+              cudaStream_t stream);
+int delta_bwd(const EacsDelta& p, const DeltaGrads& d, const void* saved, size_t saved_bytes, void* ws, size_t ws_bytes,
+              cudaStream_t stream);
+int delta_step(const EacsDelta& p, void* o, float* final_state, cudaStream_t stream);
+
 // train.cu
 struct TrainBwdCall {
     const void* lam;

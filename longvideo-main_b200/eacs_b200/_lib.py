@@ -30,6 +30,16 @@ _F = ctypes.c_float
 _I = ctypes.c_int
 _SZ = ctypes.c_size_t
 
+
+class Delta(ctypes.Structure):
+    """EacsDelta (include/eacs_b200.h)."""
+    _fields_ = ([(n, _P) for n in ("q", "k", "v", "g", "beta")]
+                + [(n + "_stride", _I64 * 3) for n in ("q", "k", "v", "g", "beta")]
+                + [("lengths", _P), ("initial_state", _P)]
+                + [(n, _I64) for n in ("B", "L", "Hk", "Hv", "K", "V")]
+                + [("scale", _F), ("dtype", ctypes.c_int32), ("gate_dtype", ctypes.c_int32)])
+
+
 # name -> (restype, argtypes); mirrors include/eacs_b200.h
 SIGNATURES = {
     "eacs_version": (ctypes.c_char_p, []),
@@ -40,6 +50,15 @@ SIGNATURES = {
     "eacs_project": (_I, [_P, _I, _P, _P, _F, _P, _I, _I64, _P, _P, _I, _P, _P, _P, _SZ,
                           _I64, _I64, _I64, _I64, _P]),
     "eacs_project_workspace_size": (_SZ, [_I64]),
+    "eacs_layer_norm_fwd": (_I, [_P, _I64, _P, _I64, _I, _P, _P, _I, _F, _P, _I64, _I64, _P]),
+    "eacs_layer_norm_bwd": (_I, [_P, _I64, _P, _I64, _P, _I64, _I, _P, _I, _F, _P, _P, _P, _P, _SZ,
+                                 _I64, _I64, _P]),
+    "eacs_layer_norm_bwd_workspace_size": (_SZ, [_I64, _I64]),
+    "eacs_delta_fwd": (_I, [_P, _P, _P, _P, _SZ, _I, _P]),
+    "eacs_delta_workspace_size": (_SZ, [_P, _I]),
+    "eacs_delta_bwd": (_I, [_P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _SZ, _P, _SZ, _P]),
+    "eacs_delta_bwd_workspace_size": (_SZ, [_P]),
+    "eacs_delta_step": (_I, [_P, _P, _P, _P]),
     "eacs_set_kernel_events": (_I, [_P, _P]),
     "eacs_scan_fwd": (_I, [_P, _P, _P, _I64, _I64, _I64, _I64, _P]),
     "eacs_scan_bwd": (_I, [_P, _P, _P, _P, _P, _I64, _I64, _I64, _I64, _P]),

@@ -14,7 +14,7 @@ import importlib
 
 def install(package: str = "cst_ssm", fuse_ungated: bool = False,
             layer_dispatch: bool = False, queries: bool = False,
-            streaming: bool = False, multiscale: bool = False) -> dict:
+            streaming: bool = False, multiscale: bool = False, norms: bool = False) -> dict:
     """Patch `package` (already importable) and return what was replaced.
 
     fuse_ungated: also bind ContinuousSSMLayer.forward to the fused ungated
@@ -35,7 +35,10 @@ def install(package: str = "cst_ssm", fuse_ungated: bool = False,
     non-continuous discretisation.
     multiscale: also route MultiScaleEACS.forward's epilogue (fusion softmax,
     blend, LayerNorm) through the one-pass branch-fuse kernel, under the same
-    rule."""
+    rule.
+    norms: also build the LayerNorm modules of every EACSLayer,
+    ContinuousSSMLayer and MultiScaleEACS made from now on as
+    eacs_b200.ops.layer_norm.LayerNorm (forward and backward kernels)."""
     from .ops import eacs_gated_scan as ours_cell
     from .ops import scan_cuda as ours_scan
 
@@ -97,6 +100,15 @@ def install(package: str = "cst_ssm", fuse_ungated: bool = False,
         if not hasattr(current, "__wrapped__"):
             ref_ms.MultiScaleEACS.forward = ours_ms.make_forward(current)
         patched["multiscale.MultiScaleEACS.forward"] = ref_ms.MultiScaleEACS.forward
+    if norms:
+        from .ops import layer_norm as ours_norm
+
+        for mod_name, cls_name in (("modules.eacs", "EACSLayer"), ("modules.continuous_ssm", "ContinuousSSMLayer"),
+                                   ("modules.multiscale", "MultiScaleEACS")):
+            cls = getattr(importlib.import_module(f"{package}.{mod_name}"), cls_name)
+            if not hasattr(cls.__init__, "__wrapped__"):
+                cls.__init__ = ours_norm.make_init(cls.__init__)
+            patched[f"{cls_name}.__init__"] = cls.__init__
     if layer_dispatch:
         from .ops import eacs_layer as ours_layer
 

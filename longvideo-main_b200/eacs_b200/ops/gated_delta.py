@@ -1,0 +1,162 @@
+"""The gated delta rule: a recurrence over a matrix state (eacs_delta_*).
+
+For each head a state S (K x V, float32) and per token, with a decay's
+logarithm g, a rate beta, a key k, a value v and a query q:
+
+    S' = exp(g) S,  u = beta (v - S'^T k),  S = S' + k u^T,  o = scale S^T q
+
+It stands beside the diagonal scans (selective_scan, ssm_forward): the same
+role in a layer, with a state that is corrected towards v at key k instead of
+summed.  `gated_delta_rule` runs sequences 64 tokens at a time on the tensor
+cores, differentiable, from and to a state; `gated_delta_step` takes one token
+per row and updates the state in place, for streaming.
+
+Layouts: q, k (B, L, Hk, K), v (B, L, Hv, V), g and beta (B, L, Hv), states
+(B, Hv, K, V) float32.  Hv is a multiple of Hk; value head h reads key head
+h // (Hv // Hk).  Views are taken with their strides (a slice of a fused
+projection needs no copy) as long as their last dimension is dense.
+"""
+from __future__ import annotations
+
+import ctypes
+
+import torch
+from torch import Tensor
+
+from .. import _lib
+from ._check import cuda_tensors, require
+
+MAX_K = 128
+MAX_V = 1024
+
+
+def _dense_last(t: Tensor) -> Tensor:
+    if t.stride(-1) == 1 or t.shape[-1] == 1:
+        return t
+    return t.contiguous()
+
+
+def _check(name, q, k, v, g, beta, lengths, state, lead):
+    """Device of the arguments; lead: the dimensions in front of the head's."""
+    ts = [t for t in (q, k, v, g, beta, lengths, state) if t is not None]
+    dev = cuda_tensors(name, *ts)
+    require(q.dim() == lead + 2 and k.shape == q.shape, f"{name}: q and k must have one shape of {lead + 2} dimensions")
+    require(v.dim() == lead + 2 and v.shape[:lead] == q.shape[:lead], f"{name}: v must have q's leading dimensions")
+    Hk, K = q.shape[-2:]
+    Hv, V = v.shape[-2:]
+    require(Hk >= 1 and Hv >= 1 and Hv % Hk == 0, f"{name}: {Hv} value heads are not a multiple of {Hk} key heads")
+    require(1 <= K <= MAX_K and 1 <= V <= MAX_V, f"{name}: K={K}, V={V} must be 1 to {MAX_K}, 1 to {MAX_V}")
+    require(g.shape == v.shape[:-1] and beta.shape == g.shape, f"{name}: g and beta must be {tuple(v.shape[:-1])}")
+    require(q.dtype in _lib.DTYPE_CODES and k.dtype == q.dtype and v.dtype == q.dtype,
+            f"{name}: q, k and v must have one dtype, float32, float16 or bfloat16")
+    require(g.dtype == beta.dtype and g.dtype in (torch.float32, q.dtype),
+            f"{name}: g and beta must both be float32 or of q's dtype")
+    if lengths is not None:
+        require(lengths.dtype == torch.int32 and lengths.shape == q.shape[:1],
+                f"{name}: lengths must be int32 ({q.shape[0]},)")
+    if state is not None:
+        require(state.dtype == torch.float32 and state.shape == (q.shape[0], Hv, K, V),
+                f"{name}: the state must be float32 ({q.shape[0]}, {Hv}, {K}, {V})")
+    return dev
+
+
+def _args(q, k, v, g, beta, scale, lengths, state) -> _lib.Delta:
+    B, L, Hk, K = q.shape
+    Hv, V = v.shape[2:]
+    p = _lib.Delta()
+    for n, t in (("q", q), ("k", k), ("v", v), ("g", g), ("beta", beta)):
+        setattr(p, n, t.data_ptr())
+        setattr(p, n + "_stride", (ctypes.c_int64 * 3)(*t.stride()[:3]))
+    p.lengths = _lib.ptr(lengths)
+    p.initial_state = _lib.ptr(state)
+    p.B, p.L, p.Hk, p.Hv, p.K, p.V = B, L, Hk, Hv, K, V
+    p.scale = scale
+    p.dtype = _lib.DTYPE_CODES[q.dtype]
+    p.gate_dtype = _lib.DTYPE_CODES[g.dtype]
+    return p
+
+
+def _forward(args, out_state, training, dev):
+    """(o, final state or None, workspace) of (q, k, v, g, beta, scale, lengths, initial)."""
+    q, k, v = args[:3]
+    p = _args(*args)
+    L_ = _lib.lib()
+    o = torch.empty(v.shape, dtype=q.dtype, device=dev)
+    final = torch.empty(v.shape[0], v.shape[2], q.shape[3], v.shape[3], dtype=torch.float32, device=dev) if out_state else None
+    ws = torch.empty(int(L_.eacs_delta_workspace_size(ctypes.byref(p), int(training))), dtype=torch.uint8, device=dev)
+    with torch.cuda.device(dev):
+        _lib.check(L_.eacs_delta_fwd(ctypes.byref(p), o.data_ptr(), _lib.ptr(final), ws.data_ptr(), ws.numel(),
+                                     int(training), _lib.stream_ptr(dev)), "eacs_delta_fwd")
+    return o, final, ws
+
+
+class GatedDeltaFunction(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, v, g, beta, scale, lengths, initial, out_state, dev):
+        o, final, ws = _forward((q, k, v, g, beta, scale, lengths, initial), out_state, True, dev)
+        ctx.save_for_backward(q, k, v, g, beta, lengths, initial, ws)
+        ctx.scale, ctx.dev = scale, dev
+        ctx.set_materialize_grads(False)
+        return (o, final) if out_state else o
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, do, dfinal=None):
+        q, k, v, g, beta, lengths, initial, ws = ctx.saved_tensors
+        dev = ctx.dev
+        if do is None and dfinal is None:
+            return (None,) * 10
+        do = torch.zeros(v.shape, dtype=q.dtype, device=dev) if do is None else _dense_last(do)
+        dfinal = None if dfinal is None else dfinal.contiguous()
+        p = _args(q, k, v, g, beta, ctx.scale, lengths, initial)
+        L_ = _lib.lib()
+        dq, dk, dv, dg, db = (torch.empty(t.shape, dtype=t.dtype, device=dev) for t in (q, k, v, g, beta))
+        di = torch.empty(initial.shape, dtype=torch.float32, device=dev) if ctx.needs_input_grad[7] else None
+        w2 = torch.empty(int(L_.eacs_delta_bwd_workspace_size(ctypes.byref(p))), dtype=torch.uint8, device=dev)
+        with torch.cuda.device(dev):
+            _lib.check(L_.eacs_delta_bwd(
+                ctypes.byref(p), do.data_ptr(), (ctypes.c_int64 * 3)(*do.stride()[:3]), _lib.ptr(dfinal), dq.data_ptr(),
+                dk.data_ptr(), dv.data_ptr(), dg.data_ptr(), db.data_ptr(), _lib.ptr(di), ws.data_ptr(), ws.numel(),
+                w2.data_ptr(), w2.numel(), _lib.stream_ptr(dev)), "eacs_delta_bwd")
+        return dq, dk, dv, dg, db, None, None, di, None, None
+
+
+def gated_delta_rule(q: Tensor, k: Tensor, v: Tensor, g: Tensor, beta: Tensor, scale: float | None = None,
+                     initial_state: Tensor | None = None, output_final_state: bool = False,
+                     lengths: Tensor | None = None):
+    """o (B, L, Hv, V) in q's dtype; with output_final_state also the state
+    (B, Hv, K, V) float32 behind the last token.
+
+    scale defaults to K ** -0.5.  lengths (B) int32 on the device: row b has
+    lengths[b] tokens (clamped to 0..L); what lies behind is not read, its
+    outputs and gradients are 0.  Differentiable in q, k, v, g, beta and
+    initial_state, through o and the final state."""
+    dev = _check("gated_delta_rule", q, k, v, g, beta, lengths, initial_state, 2)
+    scale = q.shape[-1] ** -0.5 if scale is None else float(scale)
+    q, k, v = _dense_last(q), _dense_last(k), _dense_last(v)
+    lengths = None if lengths is None else lengths.contiguous()
+    state = None if initial_state is None else initial_state.contiguous()
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (q, k, v, g, beta, state)):
+        return GatedDeltaFunction.apply(q, k, v, g, beta, scale, lengths, state, output_final_state, dev)
+    o, final, _ = _forward((q, k, v, g, beta, scale, lengths, state), output_final_state, False, dev)
+    return (o, final) if output_final_state else o
+
+
+@torch.no_grad()
+def gated_delta_step(q: Tensor, k: Tensor, v: Tensor, g: Tensor, beta: Tensor, state: Tensor,
+                     scale: float | None = None) -> Tensor:
+    """One token per row: q, k (B, Hk, K), v (B, Hv, V), g and beta (B, Hv);
+    `state` (B, Hv, K, V) float32, contiguous, is updated in place.  Returns
+    o (B, Hv, V) in q's dtype.  No gradient."""
+    dev = _check("gated_delta_step", q, k, v, g, beta, None, state, 1)
+    require(state.is_contiguous() and not state.requires_grad,
+            "gated_delta_step: the state is updated in place: it must be contiguous and without a gradient")
+    scale = q.shape[-1] ** -0.5 if scale is None else float(scale)
+    q, k, v, g, beta = (t.unsqueeze(1) for t in (_dense_last(q), _dense_last(k), _dense_last(v), g, beta))
+    o = torch.empty(v.shape, dtype=q.dtype, device=dev)
+    p = _args(q, k, v, g, beta, scale, None, state)
+    with torch.cuda.device(dev):
+        _lib.check(_lib.lib().eacs_delta_step(ctypes.byref(p), o.data_ptr(), state.data_ptr(), _lib.stream_ptr(dev)),
+                   "eacs_delta_step")
+    torch.autograd.graph.increment_version(state)
+    return o.squeeze(1)

@@ -1,0 +1,397 @@
+"""The gated delta rule (eacs_delta_*) against its token-by-token definition in 64 bits.
+
+Tolerances are on |got - want| in the 2-norm over |want|.  Operands of the
+matrix products keep at least 16 significant bits (2^-17 each), a token's way
+from inputs to an output or gradient passes a handful of them and float32
+sums, so computed values stay under 16 * 2^-17 = 1.3e-4 of their norm in the
+worst case and, errors being of either sign, near 2^-17 * sqrt(16) = 3.1e-5:
+TOL = 6.2e-5, twice that.  One rounding to the output's type adds eps / 2.
+"""
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda:0"
+TOL = 6.2e-5
+
+if torch.cuda.is_available():
+    from eacs_b200.ops.gated_delta import gated_delta_rule, gated_delta_step
+    from eacs_b200.ops.layer_norm import layer_norm
+
+
+def tol(dtype):
+    return TOL + (torch.finfo(dtype).eps / 2 if dtype != torch.float32 else 0.0)
+
+
+def close(got, want, times=1.0, what=""):
+    assert got.shape == want.shape, what
+    want = want.to(got.device)
+    err, ref = float((got.double() - want).norm()), float(want.norm())
+    assert err <= times * tol(got.dtype) * ref + 1e-12, (what, err / max(ref, 1e-30))
+
+
+def oracle(q, k, v, g, beta, scale, initial=None, lengths=None):
+    """(o, final state), differentiable, float64."""
+    B, L, Hk, K = q.shape
+    Hv, V = v.shape[2:]
+    r = Hv // Hk
+    q, k = q.repeat_interleave(r, 2), k.repeat_interleave(r, 2)
+    S = q.new_zeros(B, Hv, K, V) if initial is None else initial
+    outs = []
+    for t in range(L):
+        Sd = S * g[:, t].exp()[..., None, None]
+        u = beta[:, t][..., None] * (v[:, t] - (Sd * k[:, t][..., None]).sum(-2))
+        Sn = Sd + k[:, t][..., None] * u[..., None, :]
+        o = (Sn * q[:, t][..., None]).sum(-2) * scale
+        if lengths is not None:
+            live = (t < lengths).view(B, 1, 1)
+            o = torch.where(live, o, torch.zeros_like(o))
+            Sn = torch.where(live[..., None], Sn, S)
+        S = Sn
+        outs.append(o)
+    return torch.stack(outs, 1) if outs else v.new_zeros(B, 0, Hv, V), S
+
+
+def make(B, L, Hk, Hv, K, V, dtype, gate=None, seed=0, initial=True):
+    gen = torch.Generator(DEV).manual_seed(seed)
+    rnd = lambda *s: torch.randn(*s, generator=gen, device=DEV)
+    k = rnd(B, L, Hk, K) + 0.8 * rnd(B, 1, Hk, K)
+    q = rnd(B, L, Hk, K)
+    gate = dtype if gate is None else gate
+    d = dict(q=(q / q.norm(dim=-1, keepdim=True)).to(dtype), k=(k / k.norm(dim=-1, keepdim=True)).to(dtype),
+             v=rnd(B, L, Hv, V).to(dtype), g=(-torch.nn.functional.softplus(rnd(B, L, Hv)) * 0.2).to(gate),
+             beta=torch.sigmoid(2 * rnd(B, L, Hv)).to(gate))
+    if initial:
+        d["initial"] = 0.5 * rnd(B, Hv, K, V)
+    return d, rnd(B, L, Hv, V).to(dtype), rnd(B, Hv, K, V)
+
+
+def both(d, do, dS, lengths=None, scale=None):
+    """Kernel and oracle: outputs, final states and gradients by name."""
+    scale = d["q"].shape[-1] ** -0.5 if scale is None else scale
+    got, want = {}, {}
+    for out, conv in ((got, lambda t: t.detach().clone()), (want, lambda t: t.detach().double().cpu())):
+        x = {n: conv(t).requires_grad_(True) for n, t in d.items()}
+        args = [x[n] for n in ("q", "k", "v", "g", "beta")]
+        if out is got:
+            o, S = gated_delta_rule(*args, scale=scale, initial_state=x.get("initial"), output_final_state=True, lengths=lengths)
+            up = [do, dS]
+        else:
+            o, S = oracle(*args, scale, x.get("initial"), None if lengths is None else lengths.cpu())
+            up = [do.double().cpu(), dS.double().cpu()]
+        grads = torch.autograd.grad([o, S], list(x.values()), up, allow_unused=True)
+        out.update(o=o.detach(), S=S.detach(), **{"d" + n: torch.zeros_like(t) if gr is None else gr
+                                                  for (n, t), gr in zip(x.items(), grads)})
+    return got, want
+
+
+def compare(got, want, times=1.0):
+    for n in want:
+        assert bool(torch.isfinite(got[n]).all()), n
+        close(got[n], want[n], times, n)
+
+
+SHAPES = [  # B, L, Hk, Hv, K, V
+    (1, 1, 1, 1, 128, 128), (2, 2, 1, 2, 64, 64), (1, 63, 2, 2, 128, 64), (2, 64, 1, 1, 64, 128), (1, 65, 2, 4, 128, 128),
+    (2, 130, 1, 3, 48, 40), (1, 257, 1, 1, 128, 200), (1, 90, 1, 2, 1, 1), (2, 70, 2, 2, 33, 17), (1, 129, 1, 1, 127, 130),
+    (1, 100, 2, 2, 72, 24)]
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("shape", SHAPES)
+def test_forward_and_backward(shape, dtype):
+    d, do, dS = make(*shape, dtype, seed=sum(shape))
+    compare(*both(d, do, dS))
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_float32_gates_and_no_initial_state(dtype):
+    d, do, dS = make(2, 150, 2, 4, 64, 96, dtype, torch.float32, seed=5, initial=False)
+    got, want = both(d, do, dS, scale=0.7)
+    assert got["dg"].dtype == torch.float32 and got["dbeta"].dtype == torch.float32
+    compare(got, want)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_lengths(dtype):
+    """Rows of no token, one token, up to a chunk's border and over L (clamped); what lies behind holds NaN and infinities."""
+    lengths = [0, 1, 64, 100, 130, 500, -3]
+    d, do, dS = make(len(lengths), 130, 1, 2, 64, 48, dtype, seed=6)
+    dev = torch.tensor(lengths, dtype=torch.int32, device=DEV)
+    clean, want = both(d, do, dS, dev)
+    compare(clean, want)
+    for i, n in enumerate(lengths):
+        n = min(max(n, 0), 130)
+        assert float(clean["o"][i, n:].abs().sum()) == 0.0
+        if n == 0:
+            assert torch.equal(clean["S"][i], d["initial"][i]) and torch.equal(clean["dinitial"][i], dS[i])
+        for name in ("q", "k", "v", "g", "beta"):
+            assert float(clean["d" + name][i, n:].abs().sum()) == 0.0
+            d[name][i, n:] = float("nan") if i % 2 else float("inf")
+        do[i, n:] = float("nan")
+    dirty, _ = both(d, do, dS, dev)
+    for n in clean:
+        assert torch.equal(clean[n], dirty[n]), n
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_resets_zero_and_double_rates(dtype):
+    """g = -inf clears the state (and leaves the precision behind it), g = 0 keeps it; beta = 0 writes nothing,
+    beta = 2 reflects."""
+    d, do, dS = make(1, 140, 1, 2, 64, 64, dtype, seed=7)
+    d["g"][0, 20], d["g"][0, 100, 0], d["g"][0, 30:60] = float("-inf"), -1e30, 0.0
+    d["beta"][0, 10:14], d["beta"][0, 50], d["beta"][0, 51] = 0.0, 2.0, -0.5
+    got, want = both(d, do, dS)
+    want["dg"] = torch.nan_to_num(want["dg"])  # 0 * inf of the definition: the state before a reset has no weight
+    for n in want:
+        if n == "dg":
+            # a reset's own gradient is a difference of terms of the size of its neighbours': of no sign, near 0
+            live = torch.isfinite(d["g"]) & (d["g"] > -100)
+            close(torch.where(live, got[n], torch.zeros_like(got[n])), torch.where(live.cpu(), want[n], torch.zeros_like(want[n])), 2.0, n)
+            assert float(got[n][~live].abs().max()) <= 2 * tol(dtype) * float(want[n].abs().max()) * 8
+        else:
+            close(got[n], want[n], 1.0, n)
+    cut = {n: t[:, 20:] for n, t in d.items() if n != "initial"}  # from the reset on nothing of before is seen
+    cut["g"] = cut["g"].clone()
+    cut["g"][0, 0] = 0.0
+    o = gated_delta_rule(*(cut[n] for n in ("q", "k", "v", "g", "beta")))
+    close(got["o"][:, 20:], o.double(), 2.0)
+
+
+def test_strong_decay_keeps_precision():
+    """Decays of e^-60 and more a token: products of decays are formed from differences, not from quotients that overflow."""
+    d, do, dS = make(1, 130, 1, 1, 64, 64, torch.float32, seed=8)
+    d["g"] = d["g"] - 60.0 * (torch.rand(1, 130, 1, device=DEV, generator=torch.Generator(DEV).manual_seed(1)) < 0.3)
+    got, want = both(d, do, dS)
+    for n in want:
+        if n != "dg":  # of decays near 0: products of numbers below 1e-26 beside rounding
+            close(got[n], want[n], 1.0, n)
+    assert float((got["dg"].double().cpu() - want["dg"]).abs().max()) <= 8 * TOL * float(want["dg"].abs().max())
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_views_of_a_fused_projection_and_broadcast(dtype):
+    """Slices of one projection (aligned and not), a transposed layout, and keys shared by expansion."""
+    B, L, H, K, V = 2, 100, 2, 64, 64
+    d, do, _ = make(B, L, H, H, K, V, dtype, seed=9, initial=False)
+    want, _ = oracle(*(d[n].double().cpu() for n in ("q", "k", "v", "g", "beta")), K ** -0.5)
+    for pad in (0, 3):
+        fused = torch.zeros(B, L, H * (2 * K + V + 2) + pad, dtype=dtype, device=DEV)
+        parts, at = {}, pad
+        for n in ("q", "k", "v", "g", "beta"):
+            w = d[n].shape[-1] if d[n].dim() == 4 else 1
+            view = fused[..., at:at + H * w].unflatten(-1, (H, w))
+            view = view if d[n].dim() == 4 else view[..., 0]
+            view.copy_(d[n])
+            parts[n], at = view, at + H * w
+        close(gated_delta_rule(*parts.values()), want)
+    heads = {n: d[n].transpose(1, 2).contiguous().transpose(1, 2) for n in d}
+    close(gated_delta_rule(*heads.values()), want)
+    k = d["k"][:, :, :1].detach().clone().requires_grad_(True)  # one key head for all, by expansion
+    args = lambda kk: (d["q"], kk.expand(B, L, H, K), d["v"], d["g"], d["beta"])
+    dk = torch.autograd.grad(gated_delta_rule(*args(k)), k, do)[0]
+    k64 = k.detach().double().cpu().requires_grad_(True)
+    d64 = {n: t.double().cpu() for n, t in d.items()}
+    o64, _ = oracle(d64["q"], k64.expand(B, L, H, K), d64["v"], d64["g"], d64["beta"], K ** -0.5)
+    close(dk, torch.autograd.grad(o64, k64, do.double().cpu())[0], 2.0)  # rounded per head, then summed and rounded
+    t = d["v"].detach().clone().transpose(-1, -2).contiguous().transpose(-1, -2)  # a value's elements apart
+    close(gated_delta_rule(d["q"], d["k"], t, d["g"], d["beta"]), want)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("shape", [(3, 7, 2, 4, 64, 40), (2, 5, 1, 1, 128, 128), (1, 6, 1, 2, 30, 37)])
+def test_steps_continue_a_sequence(shape, dtype):
+    """A prefill's state, then tokens one by one, give the whole sequence's outputs and state."""
+    B, L, Hk, Hv, K, V = shape
+    d, _, _ = make(B, 70 + L, Hk, Hv, K, V, dtype, seed=10)
+    want, S_want = oracle(*(d[n].double().cpu() for n in ("q", "k", "v", "g", "beta")), K ** -0.5, d["initial"].double().cpu())
+    head = [d[n][:, :70] for n in ("q", "k", "v", "g", "beta")]
+    o, S = gated_delta_rule(*head, initial_state=d["initial"], output_final_state=True)
+    outs, at = [o], S.data_ptr()
+    for t in range(70, 70 + L):
+        outs.append(gated_delta_step(*(d[n][:, t] for n in ("q", "k", "v", "g", "beta")), S)[:, None])
+    assert S.data_ptr() == at
+    close(torch.cat(outs, 1), want)
+    close(S, S_want)
+
+
+def test_step_state_past_32_bit_offsets():
+    B, H, K, V = 4100, 32, 128, 128  # 2^31 state values and more
+    gen = torch.Generator(DEV).manual_seed(11)
+    q, k, v = (torch.randn(B, H, n, generator=gen, device=DEV).bfloat16() for n in (K, K, V))
+    k = torch.nn.functional.normalize(k.float(), dim=-1).bfloat16()
+    g, beta = -torch.rand(B, H, generator=gen, device=DEV), torch.rand(B, H, generator=gen, device=DEV)
+    S = torch.zeros(B, H, K, V, device=DEV)
+    S[-2:] = torch.randn(2, H, K, V, generator=gen, device=DEV)
+    small = S[-2:].clone()
+    o = gated_delta_step(q, k, v, g, beta, S)
+    o2 = gated_delta_step(*(t[-2:] for t in (q, k, v, g, beta)), small)
+    assert torch.equal(o[-2:], o2) and torch.equal(S[-2:], small)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_gradient_against_differences(dtype):
+    """Directional fourth-order differences of the kernel's own forward.  h = 2^-4: truncation is h^4 = 1.5e-5 of a fifth
+    derivative, and a forward off by up to TOL of |f| moves the slope by TOL |f| / h; float32 gates and state carry the
+    directions exactly, bf16 tokens are left alone."""
+    d, do, dS = make(1, 80, 1, 2, 64, 64, dtype, torch.float32, seed=12)
+    names = ["g", "beta", "initial"] + (["q", "k", "v"] if dtype == torch.float32 else [])
+    gen = torch.Generator(DEV).manual_seed(13)
+    dirs = {n: 0.05 * torch.randn(d[n].shape, generator=gen, device=DEV) for n in names}
+    up = torch.zeros_like(dS)
+
+    def f(s):
+        x = {n: t + s * dirs[n] if n in dirs else t for n, t in d.items()}
+        S = gated_delta_rule(*(x[n] for n in ("q", "k", "v", "g", "beta")), initial_state=x["initial"], output_final_state=True)[1]
+        return float((S.double() * dS.double()).sum())
+    x = {n: t.detach().clone().requires_grad_(True) for n, t in d.items()}
+    S = gated_delta_rule(*(x[n] for n in ("q", "k", "v", "g", "beta")), initial_state=x["initial"], output_final_state=True)[1]
+    grads = torch.autograd.grad(S, [x[n] for n in names], dS)
+    slope = float(sum((a.double() * dirs[n].double()).sum() for a, n in zip(grads, names)))
+    h = 2.0 ** -4
+    num = (8 * (f(h) - f(-h)) - (f(2 * h) - f(-2 * h))) / (12 * h)
+    size = float(S.double().norm() * dS.double().norm())
+    assert abs(num - slope) <= 4 * TOL * size / (h * size ** 0.5) + 2e-3 * abs(slope), (num, slope)
+    assert up.shape == dS.shape
+
+
+def test_only_some_gradients_and_only_one_output():
+    d, do, dS = make(1, 70, 1, 1, 64, 64, torch.bfloat16, seed=14)
+    full, _ = both(d, do, torch.zeros_like(dS))
+    v = d["v"].detach().clone().requires_grad_(True)
+    o, S = gated_delta_rule(d["q"], d["k"], v, d["g"], d["beta"], initial_state=d["initial"], output_final_state=True)
+    assert torch.equal(torch.autograd.grad(o, v, do)[0], full["dv"])
+    o, S = gated_delta_rule(d["q"], d["k"], v, d["g"], d["beta"], initial_state=d["initial"], output_final_state=True)
+    gS = torch.autograd.grad(S, v, dS)[0]
+    only, _ = both(d, torch.zeros_like(do), dS)
+    assert torch.equal(gS, only["dv"])
+    odd = torch.randn(1, 70, 64, 1, device=DEV).bfloat16().transpose(2, 3).expand(1, 70, 1, 64)  # an upstream gradient in another layout
+    a = torch.autograd.grad(gated_delta_rule(d["q"], d["k"], v, d["g"], d["beta"]), v, odd)[0]
+    b = torch.autograd.grad(gated_delta_rule(d["q"], d["k"], v, d["g"], d["beta"]), v, odd.contiguous())[0]
+    assert torch.equal(a, b)
+
+
+def test_same_bits_other_stream_and_graphs():
+    d, do, dS = make(2, 200, 2, 4, 128, 128, torch.bfloat16, seed=15)
+    x = {n: t.detach().clone().requires_grad_(True) for n, t in d.items()}
+    state = torch.randn(2, 4, 128, 128, device=DEV)
+
+    def step():
+        o, S = gated_delta_rule(*(x[n] for n in ("q", "k", "v", "g", "beta")), initial_state=x["initial"], output_final_state=True)
+        return (o.detach(), S.detach(), *torch.autograd.grad([o, S], list(x.values()), [do, dS]))
+    want = step()
+    assert all(torch.equal(a, b) for a, b in zip(step(), want))
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        side = step()
+    s.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(side, want))
+    del side
+    graphs = []
+    for _ in range(2):
+        gr = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(gr):
+            out = step()
+        graphs.append((gr, out))
+    with torch.no_grad():
+        x["v"].mul_(0.5)
+    want = step()
+    for gr, _ in graphs:
+        gr.replay()
+    torch.cuda.synchronize()
+    for _, out in graphs:
+        assert all(torch.equal(a, b) for a, b in zip(out, want))
+    first = state.clone()
+    tok = [d[n][:, 0] for n in ("q", "k", "v", "g", "beta")]
+    o1 = gated_delta_step(*tok, first)
+    gr = torch.cuda.CUDAGraph()
+    cap = state.clone()
+    with torch.cuda.graph(gr):
+        o2 = gated_delta_step(*tok, cap)
+    cap.copy_(state)
+    gr.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(o1, o2) and torch.equal(first, cap)
+
+
+def test_empty():
+    q = torch.zeros(2, 0, 1, 64, device=DEV, requires_grad=True)
+    v, g = torch.zeros(2, 0, 2, 32, device=DEV), torch.zeros(2, 0, 2, device=DEV)
+    S0 = torch.randn(2, 2, 64, 32, device=DEV, requires_grad=True)
+    o, S = gated_delta_rule(q, q, v, g, g, initial_state=S0, output_final_state=True)
+    assert o.shape == (2, 0, 2, 32) and torch.equal(S, S0)
+    up = torch.randn_like(S0)
+    assert torch.equal(torch.autograd.grad(S, S0, up)[0], up)
+    with torch.no_grad():
+        assert float(gated_delta_rule(q, q, v, g, g, output_final_state=True)[1].abs().sum()) == 0.0
+    assert gated_delta_rule(q[:0], q[:0], v[:0], g[:0], g[:0]).shape == (0, 0, 2, 32)
+    assert gated_delta_step(*(torch.zeros(0, 2, 8, device=DEV) for _ in range(3)), torch.zeros(0, 2, device=DEV),
+                            torch.zeros(0, 2, device=DEV), torch.zeros(0, 2, 8, 8, device=DEV)).shape == (0, 2, 8)
+
+
+def test_norm_projection_delta_norm_together():
+    """A pre-norm block, y = norm(x + proj(delta(norm(x)))): trained end to end, then streamed frame by frame."""
+    B, L, D, H = 2, 75, 64, 2
+    K = D // H
+    gen = torch.Generator(DEV).manual_seed(16)
+    rnd = lambda *s: torch.randn(*s, generator=gen, device=DEV)
+    P = dict(w1=1 + 0.1 * rnd(D), b1=0.1 * rnd(D), win=rnd(3 * D + 2 * H, D) * D ** -0.5, wo=rnd(D, D) * D ** -0.5,
+             w2=1 + 0.1 * rnd(D), b2=0.1 * rnd(D))
+    x, dy = rnd(B, L, D), rnd(B, L, D)
+
+    def project(h, win):
+        q, k, v, a, b = (h @ win.t()).split([D, D, D, H, H], -1)
+        q, k, v = (t.unflatten(-1, (H, K)) for t in (q, k, v))
+        return (torch.nn.functional.normalize(q, dim=-1), torch.nn.functional.normalize(k, dim=-1), v,
+                torch.nn.functional.logsigmoid(a), torch.sigmoid(b))
+
+    def block(x, p, norm, rule):
+        o = rule(*project(norm(x, p["w1"], p["b1"], None), p["win"]))
+        return norm(x, p["w2"], p["b2"], o.flatten(-2) @ p["wo"].t())
+    ours = lambda x, w, b, r: layer_norm(x, w, b, 1e-5, residual=r)
+    plain = lambda x, w, b, r: torch.nn.functional.layer_norm(x if r is None else x + r, (D,), w, b, 1e-5)
+    got, want = {}, {}
+    for out, conv in ((got, lambda t: t.clone()), (want, lambda t: t.double().cpu())):
+        p = {n: conv(t).requires_grad_(True) for n, t in P.items()}
+        xx = conv(x).requires_grad_(True)
+        rule = gated_delta_rule if out is got else lambda *a: oracle(*a, K ** -0.5)[0]
+        y = block(xx, p, ours if out is got else plain, rule)
+        leaves = [xx, *p.values()]
+        out.update(y=y.detach(), **dict(zip(["x", *p], torch.autograd.grad(y, leaves, conv(dy)))))
+    for n in want:
+        close(got[n], want[n], 2.0, n)  # two norms and two products around the rule
+    with torch.no_grad():  # streaming: a prefill of 70 frames, then one frame at a time
+        q, k, v, g, b = project(layer_norm(x, P["w1"], P["b1"]), P["win"])
+        _, S = gated_delta_rule(q[:, :70], k[:, :70], v[:, :70], g[:, :70], b[:, :70], output_final_state=True)
+        for t in range(70, L):
+            q, k, v, g, b = project(layer_norm(x[:, t], P["w1"], P["b1"]), P["win"])
+            o = gated_delta_step(q, k, v, g, b, S)
+            y = layer_norm(x[:, t], P["w2"], P["b2"], residual=o.flatten(-2) @ P["wo"].t())
+            close(y, want["y"][:, t], 2.0)
+
+
+def test_refusals():
+    d, _, _ = make(2, 8, 2, 4, 16, 8, torch.bfloat16, seed=17)
+    q, k, v, g, b, S = (d[n] for n in ("q", "k", "v", "g", "beta", "initial"))
+    ok = dict(q=q, k=k, v=v, g=g, beta=b)
+    for bad in (dict(k=k[:, :7]), dict(v=v[:, :, :3]), dict(g=g[..., :2]), dict(beta=b.float()), dict(g=g.half(), beta=b.half()),
+                dict(k=k.float()), dict(q=q.double(), k=k.double(), v=v.double()), dict(initial_state=S.half()),
+                dict(initial_state=S[:1]), dict(lengths=torch.tensor([8, 8], device=DEV)),
+                dict(lengths=torch.zeros(3, dtype=torch.int32, device=DEV)), dict(lengths=torch.zeros(2, dtype=torch.int32)),
+                dict(q=q[..., :0], k=k[..., :0]), dict(v=v.cpu())):
+        with pytest.raises(RuntimeError):
+            gated_delta_rule(**{**ok, **bad})
+    wide = torch.zeros(1, 2, 1, 129, device=DEV)
+    with pytest.raises(RuntimeError, match="128"):
+        gated_delta_rule(wide, wide, wide, wide[..., 0], wide[..., 0])
+    tok = [t[:, 0] for t in (q, k, v, g, b)]
+    for bad in (S.transpose(0, 1).contiguous().transpose(0, 1), S.half(), S[:1], S.clone().requires_grad_(True)):
+        with pytest.raises(RuntimeError):
+            gated_delta_step(*tok, bad)
+    leaf = S.clone()
+    x = torch.ones(2, 4, 16, 8, device=DEV, requires_grad=True)
+    y = (x * leaf).sum()  # autograd keeps leaf for its backward
+    gated_delta_step(*tok, leaf)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.backward()
