@@ -136,7 +136,8 @@ typedef struct EacsDelta {
 /* Chunked forward: o (B,L,Hv,V) dense of dtype; final_state (B,Hv,K,V)
  * float32 or NULL.  With training != 0 the workspace holds what
  * eacs_delta_bwd reads and is kept, unchanged, until then.  Products run on the
- * tensor cores with operands split in two (tf32, 22 significant bits); all
+ * tensor cores with operands split in two (tf32, 22 significant bits; for
+ * bfloat16 inputs whose rows are read 16 bytes at a time bf16, 16 bits); all
  * sums and the state are float32. */
 EACS_API int eacs_delta_fwd(const EacsDelta* p, void* o, float* final_state, void* workspace, size_t workspace_bytes,
                             int training, void* stream);
@@ -146,7 +147,8 @@ EACS_API size_t eacs_delta_workspace_size(const EacsDelta* p, int training);
  * float32 or NULL (the final state's gradient); dq, dk, dv dense of dtype
  * (dq and dk summed over the value heads of a key head), dg and dbeta dense
  * of gate_dtype, dinitial (B,Hv,K,V) float32 or NULL.  `saved` is the
- * workspace of the training forward with the same arguments. */
+ * workspace of the training forward with the same arguments.  Where q, k and v
+ * are bfloat16 and read 16 bytes at a time, dout has to be too. */
 EACS_API int eacs_delta_bwd(const EacsDelta* p, const void* dout, const int64_t* dout_stride, const float* dfinal,
                             void* dq, void* dk, void* dv, void* dg, void* dbeta, float* dinitial, const void* saved,
                             size_t saved_bytes, void* workspace, size_t workspace_bytes, void* stream);

@@ -66,7 +66,10 @@ int eacs_device_status(int* status, void* stream) {
     if (rc) return rc;
     rc = eacs::cuda_check(eacs::query_read_status(&d, s), "eacs_device_status");
     if (rc) return rc;
-    *status = a ? a : (b ? b : (c ? c : d));
+    int e = 0;
+    rc = eacs::cuda_check(eacs::planes_read_status(&e, s), "eacs_device_status");
+    if (rc) return rc;
+    *status = a ? a : (b ? b : (c ? c : (d ? d : e)));
     return EACS_OK;
 }
 

@@ -44,101 +44,6 @@
 namespace eacs {
 namespace {
 
-// Operands are tf32 split in two (hi lo' + lo hi' + hi hi': 22 bits).  A tile is
-// float32 in shared memory and is split as it is read.  Af<P>: a 16 x 16 A
-// operand.  Tiles of B are 16 columns (two accumulators) by 16 of the summed
-// index, stored [n][k] or (TR) [k][n].
-// X: the inputs (queries, keys, upstream gradients) are exact in tf32, as
-// float16 values are: their low part is 0 and is left out.
-template <bool X>
-struct FmtF {
-    using E = float;
-    template <int P> struct Af { uint32_t h[2][4], lo[2][4]; };
-    static __device__ __forceinline__ E put(float v) { return v; }
-    static __device__ __forceinline__ void set(Af<2>& a, int s, int i, float v) { split_tf32(v, a.h[s][i], a.lo[s][i]); }
-    // the summed index runs 2t, 2t + 1 inside an accumulator tile; A and B use the same order
-    template <int P>
-    static __device__ __forceinline__ Af<P> from_acc(const float* c0, const float* c1) {
-        Af<P> a;
-#pragma unroll
-        for (int s = 0; s < 2; ++s) {
-            const float* c = s ? c1 : c0;
-            split_tf32(c[0], a.h[s][0], a.lo[s][0]);
-            split_tf32(c[2], a.h[s][1], a.lo[s][1]);
-            split_tf32(c[1], a.h[s][2], a.lo[s][2]);
-            split_tf32(c[3], a.h[s][3], a.lo[s][3]);
-        }
-        return a;
-    }
-    static __device__ __forceinline__ Af<1> from_smem(const E* s, int ld, int m0, int k0) {
-        const Lane L;
-        Af<1> a;
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            const float2 p = *reinterpret_cast<const float2*>(s + (m0 + L.g) * ld + k0 + 8 * h + 2 * L.t);
-            const float2 q = *reinterpret_cast<const float2*>(s + (m0 + L.g + 8) * ld + k0 + 8 * h + 2 * L.t);
-            split_tf32(p.x, a.h[h][0], a.lo[h][0]);
-            split_tf32(q.x, a.h[h][1], a.lo[h][1]);
-            split_tf32(p.y, a.h[h][2], a.lo[h][2]);
-            split_tf32(q.y, a.h[h][3], a.lo[h][3]);
-        }
-        return a;
-    }
-    static __device__ __forceinline__ Af<1> from_smem_t(const E* s, int ld, int m0, int k0) {
-        const Lane L;
-        Af<1> a;
-#pragma unroll
-        for (int h = 0; h < 2; ++h)
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-                split_tf32(s[(k0 + 8 * h + 2 * L.t + (i >> 1)) * ld + m0 + L.g + (i & 1) * 8], a.h[h][i], a.lo[h][i]);
-        return a;
-    }
-    static __device__ __forceinline__ void scale_k(Af<1>& a, const float* f, int k0) {
-        const int t = threadIdx.x & 3;
-#pragma unroll
-        for (int h = 0; h < 2; ++h)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const float v = __uint_as_float(a.h[h][i]) + __uint_as_float(a.lo[h][i]);
-                split_tf32(v * f[k0 + 8 * h + 2 * t + (i >> 1)], a.h[h][i], a.lo[h][i]);
-            }
-    }
-    // IN: B is a tile of inputs
-    template <int P, bool TR, bool IN = false>
-    static __device__ __forceinline__ void mma2(float* c0, float* c1, const Af<P>& a, const E* s, int ld, int n0,
-                                                int k0) {
-        const Lane L;
-#pragma unroll
-        for (int half = 0; half < 2; ++half) {
-            float* c = half ? c1 : c0;
-            const int n = n0 + 8 * half + L.g;
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                const int k = k0 + 8 * h + 2 * L.t;
-                float2 v;
-                if constexpr (TR) v = make_float2(s[k * ld + n], s[(k + 1) * ld + n]);
-                else v = *reinterpret_cast<const float2*>(s + n * ld + k);
-                uint32_t bh0, bl0, bh1, bl1;
-                split_tf32(v.x, bh0, bl0);
-                split_tf32(v.y, bh1, bl1);
-                mma_tf32(c, a.lo[h], bh0, bh1);
-                if constexpr (!(X && IN)) mma_tf32(c, a.h[h], bl0, bl1);
-                mma_tf32(c, a.h[h], bh0, bh1);
-            }
-        }
-    }
-    static __device__ __forceinline__ void load_t(float* x0, float* x1, const E* s, int ld, int r0, int c0) {
-        const Lane L;
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            float* x = h ? x1 : x0;
-#pragma unroll
-            for (int i = 0; i < 4; ++i) x[i] = s[(c0 + 8 * h + 2 * L.t + (i & 1)) * ld + r0 + L.g + (i >> 1) * 8];
-        }
-    }
-};
-
 // acc += A B with B a tile of inputs / of results
 template <class F, int P, bool TR>
 __device__ __forceinline__ void mm_in(float* c0, float* c1, const typename F::template Af<P>& a,
@@ -349,9 +254,6 @@ __device__ __forceinline__ void state_store(const float (*S)[4], float* p, int K
         }
 }
 // accumulators into a dense [row][ld] workspace tile, rows r0.., as pairs
-__device__ __forceinline__ void put2(__nv_bfloat16* p, float x, float y) {
-    *reinterpret_cast<uint32_t*>(p) = pack_bf16(x, y);
-}
 __device__ __forceinline__ void put2(float* p, float x, float y) { *reinterpret_cast<float2*>(p) = make_float2(x, y); }
 
 template <typename E, int NT>
@@ -1184,29 +1086,6 @@ int64_t pad16(int64_t v) { return (v + 15) / 16 * 16; }
 int64_t key_pad(int64_t K) { return K <= 64 ? 64 : 128; }
 size_t align256(size_t x) { return (x + 255) / 256 * 256; }
 
-struct Sizes { size_t gates, T, M, S, U, total; };
-Sizes fwd_sizes(const EacsDelta& p, bool training) {
-    const size_t ids = static_cast<size_t>(p.B) * p.Hv * chunks(p.L), e = 4;
-    Sizes z;
-    z.gates = align256(ids * kGates * sizeof(float));
-    z.T = align256(ids * kC * kC * 4);  // two bf16 planes or one float32
-    z.M = training ? align256(ids * kC * kC * e) : 0;
-    z.S = align256(ids * pad16(p.V) * key_pad(p.K) * e);
-    z.U = align256(ids * pad16(p.V) * kC * e);
-    z.total = z.gates + z.T + z.M + z.S + z.U;
-    return z;
-}
-struct BSizes { size_t dS, dV, group, total; };
-BSizes bwd_sizes(const EacsDelta& p) {
-    const size_t ids = static_cast<size_t>(p.B) * p.Hv * chunks(p.L), e = 4;
-    BSizes z;
-    z.dS = align256(ids * pad16(p.V) * key_pad(p.K) * e);
-    z.dV = align256(ids * pad16(p.V) * kC * e);
-    z.group = p.Hv > p.Hk ? align256(static_cast<size_t>(p.B) * p.Hk * chunks(p.L) * 2 * kC * key_pad(p.K) * 4) : 0;
-    z.total = z.dS + z.dV + z.group;
-    return z;
-}
-
 // EACS_OK, or the error that these sizes and types are refused with
 int check_delta(const EacsDelta& p, const char* fn) {
     if (p.B < 0 || p.L < 0 || p.Hk <= 0 || p.Hv <= 0 || p.K <= 0 || p.V <= 0)
@@ -1223,10 +1102,13 @@ int check_delta(const EacsDelta& p, const char* fn) {
     return EACS_OK;
 }
 
-bool rows16(const void* p, const int64_t* st, int64_t n, int dtype) {
-    const int e = dtype == EACS_DTYPE_F32 ? 4 : 2;
+// Whether rows of n elements start on 16 bytes (a dimension of one element has no stride).
+bool rows16(const EacsDelta& d, const void* p, const int64_t* st, int64_t H, int64_t n) {
+    const int e = d.dtype == EACS_DTYPE_F32 ? 4 : 2;
+    const int64_t size[3] = {d.B, d.L, H};
     uintptr_t bits = reinterpret_cast<uintptr_t>(p);
-    for (int i = 0; i < 3; ++i) bits |= static_cast<uintptr_t>(st[i]) * e;
+    for (int i = 0; i < 3; ++i)
+        if (size[i] > 1) bits |= static_cast<uintptr_t>(st[i]) * e;
     return (bits & 15u) == 0 && n % 8 == 0;
 }
 
@@ -1243,13 +1125,60 @@ DArgs make_args(const EacsDelta& p) {
     a.K = static_cast<int>(p.K); a.V = static_cast<int>(p.V);
     a.n = static_cast<int>(chunks(p.L)); a.Vp = static_cast<int>(pad16(p.V));
     a.gate_dtype = p.gate_dtype;
-    a.vec_qk = rows16(p.q, p.q_stride, p.K, p.dtype) && rows16(p.k, p.k_stride, p.K, p.dtype);
-    a.vec_v = rows16(p.v, p.v_stride, p.V, p.dtype);
+    a.vec_qk = rows16(p, p.q, p.q_stride, p.Hk, p.K) && rows16(p, p.k, p.k_stride, p.Hk, p.K);
+    a.vec_v = rows16(p, p.v, p.v_stride, p.Hv, p.V);
     a.scale = p.scale;
     return a;
 }
+// What a tensor map can describe: rows that start on 16 bytes, and strides above 0
+// and below 2^40 bytes (an expanded dimension has stride 0).
+bool mapped(int64_t B, int64_t L, int64_t H, const int64_t* st) {
+    const int64_t n[3] = {B, L, H};
+    for (int i = 0; i < 3; ++i)
+        if (n[i] > 1 && (st[i] <= 0 || st[i] >= int64_t{1} << 39)) return false;
+    return true;
+}
+// Whether the bfloat16 kernels take these inputs.  The backward goes by the forward's inputs alone, as it
+// reads what the forward left (an upstream gradient in another layout is
+// refused by delta_bwd then).
+bool planes(const EacsDelta& p, const DArgs& a) {
+    return p.dtype == EACS_DTYPE_BF16 && a.vec_qk && a.vec_v && mapped(p.B, p.L, p.Hk, p.q_stride) &&
+           mapped(p.B, p.L, p.Hk, p.k_stride) && mapped(p.B, p.L, p.Hv, p.v_stride);
+}
+
+struct Sizes { size_t gates, T, M, S, U, total; };
+Sizes fwd_sizes(const EacsDelta& p, const DArgs& a, bool training) {
+    const size_t ids = static_cast<size_t>(p.B) * p.Hv * chunks(p.L), e = sizeof(float);
+    Sizes z{};
+    if (planes(p, a)) {
+        z.total = planes_saved_size(a, training);
+        return z;
+    }
+    z.gates = align256(ids * kGates * e);
+    z.T = align256(ids * kC * kC * e);
+    z.M = training ? align256(ids * kC * kC * e) : 0;
+    z.S = align256(ids * pad16(p.V) * key_pad(p.K) * e);
+    z.U = align256(ids * pad16(p.V) * kC * e);
+    z.total = z.gates + z.T + z.M + z.S + z.U;
+    return z;
+}
+struct BSizes { size_t dS, dV, group, total; };
+BSizes bwd_sizes(const EacsDelta& p, const DArgs& a) {
+    const size_t ids = static_cast<size_t>(p.B) * p.Hv * chunks(p.L), e = sizeof(float);
+    BSizes z{};
+    if (planes(p, a)) {
+        z.dS = align256(planes_bwd_size(a));
+    } else {
+        z.dS = align256(ids * pad16(p.V) * key_pad(p.K) * e);
+        z.dV = align256(ids * pad16(p.V) * kC * e);
+    }
+    z.group = p.Hv > p.Hk ? align256(static_cast<size_t>(p.B) * p.Hk * chunks(p.L) * 2 * kC * key_pad(p.K) * 4) : 0;
+    z.total = z.dS + z.dV + z.group;
+    return z;
+}
+
 void set_workspace(DArgs& a, const EacsDelta& p, void* ws, bool training) {
-    const Sizes z = fwd_sizes(p, training);
+    const Sizes z = fwd_sizes(p, a, training);
     char* w = static_cast<char*>(ws);
     a.gates = reinterpret_cast<float*>(w); w += z.gates;
     a.T = w; w += z.T;
@@ -1263,11 +1192,11 @@ bool inputs_set(const EacsDelta& p) { return p.q && p.k && p.v && p.g && p.beta;
 
 size_t delta_workspace_size(const EacsDelta& p, bool training) {
     if (check_delta(p, "eacs_delta_workspace_size") != EACS_OK) return 0;
-    return fwd_sizes(p, training).total;
+    return fwd_sizes(p, make_args(p), training).total;
 }
 size_t delta_bwd_workspace_size(const EacsDelta& p) {
     if (check_delta(p, "eacs_delta_bwd_workspace_size") != EACS_OK) return 0;
-    return bwd_sizes(p).total;
+    return bwd_sizes(p, make_args(p)).total;
 }
 
 int delta_fwd(const EacsDelta& p, void* o, float* final_state, void* ws, size_t ws_bytes, bool training,
@@ -1284,15 +1213,17 @@ int delta_fwd(const EacsDelta& p, void* o, float* final_state, void* ws, size_t 
                           fn);
     }
     if (!inputs_set(p) || !o) return fail(EACS_ERR_INVALID, "%s: null pointer argument", fn);
-    const size_t need = fwd_sizes(p, training).total;
+    DArgs a = make_args(p);
+    const size_t need = fwd_sizes(p, a, training).total;
     if (!ws || ws_bytes < need) return fail(EACS_ERR_WORKSPACE, "%s: workspace of %zu bytes, %zu needed", fn, ws_bytes, need);
     if (reinterpret_cast<uintptr_t>(ws) & 15u) return fail(EACS_ERR_INVALID, "%s: workspace must be 16-byte aligned", fn);
-    DArgs a = make_args(p);
     set_workspace(a, p, ws, training);
     a.out = o;
     a.final_state = final_state;
     cudaError_t e;
-    if (p.dtype == EACS_DTYPE_BF16)
+    if (planes(p, a))
+        e = planes_fwd(a, ws, training, stream);
+    else if (p.dtype == EACS_DTYPE_BF16)
         e = p.K <= 64 ? run_fwd<FmtF<true>, __nv_bfloat16, 64>(a, stream) : run_fwd<FmtF<true>, __nv_bfloat16, 128>(a, stream);
     else if (p.dtype == EACS_DTYPE_F16)
         e = p.K <= 64 ? run_fwd<FmtF<true>, __half, 64>(a, stream) : run_fwd<FmtF<true>, __half, 128>(a, stream);
@@ -1330,27 +1261,31 @@ int delta_bwd(const EacsDelta& p, const DeltaGrads& d, const void* saved, size_t
     }
     if (!inputs_set(p) || !d.dout || !d.dq || !d.dk || !d.dv || !d.dg || !d.dbeta)
         return fail(EACS_ERR_INVALID, "%s: null pointer argument", fn);
-    const size_t need_saved = fwd_sizes(p, true).total, need = bwd_sizes(p).total;
+    DArgs a = make_args(p);
+    const size_t need_saved = fwd_sizes(p, a, true).total, need = bwd_sizes(p, a).total;
     if (!saved || saved_bytes < need_saved)
         return fail(EACS_ERR_WORKSPACE, "%s: the forward's workspace has %zu bytes, %zu needed", fn, saved_bytes, need_saved);
     if (!ws || ws_bytes < need) return fail(EACS_ERR_WORKSPACE, "%s: workspace of %zu bytes, %zu needed", fn, ws_bytes, need);
     if ((reinterpret_cast<uintptr_t>(ws) | reinterpret_cast<uintptr_t>(saved)) & 15u)
         return fail(EACS_ERR_INVALID, "%s: workspaces must be 16-byte aligned", fn);
-    DArgs a = make_args(p);
     set_workspace(a, p, const_cast<void*>(saved), true);
     a.dout = d.dout;
     a.sdo = Str{d.dout_stride[0], d.dout_stride[1], d.dout_stride[2]};
-    a.vec_do = rows16(d.dout, d.dout_stride, p.V, p.dtype);
+    a.vec_do = rows16(p, d.dout, d.dout_stride, p.Hv, p.V);
     a.dq = d.dq; a.dk = d.dk; a.dv = d.dv; a.dg = d.dg; a.dbeta = d.dbeta;
     a.dfinal = d.dfinal;
     a.dinitial = d.dinitial;
-    const BSizes z = bwd_sizes(p);
+    if (planes(p, a) && !(a.vec_do && mapped(p.B, p.L, p.Hv, d.dout_stride)))
+        return fail(EACS_ERR_INVALID, "%s: rows of dout must start on 16 bytes, with strides above 0, where those of q, k and v do", fn);
+    const BSizes z = bwd_sizes(p, a);
     char* w = static_cast<char*>(ws);
     a.dS = w; w += z.dS;
     a.dV = w; w += z.dV;
     float* group = reinterpret_cast<float*>(w);
     cudaError_t e;
-    if (p.dtype == EACS_DTYPE_BF16)
+    if (planes(p, a))
+        e = planes_bwd(a, const_cast<void*>(saved), ws, group, stream);
+    else if (p.dtype == EACS_DTYPE_BF16)
         e = p.K <= 64 ? run_bwd<FmtF<true>, __nv_bfloat16, 64>(a, group, stream) : run_bwd<FmtF<true>, __nv_bfloat16, 128>(a, group, stream);
     else if (p.dtype == EACS_DTYPE_F16)
         e = p.K <= 64 ? run_bwd<FmtF<true>, __half, 64>(a, group, stream) : run_bwd<FmtF<true>, __half, 128>(a, group, stream);

@@ -60,6 +60,101 @@ struct Lane {
     __device__ __forceinline__ Lane() : l(threadIdx.x & 31), g(l >> 2), t(l & 3) {}
 };
 
+// Operands are tf32 split in two (hi lo' + lo hi' + hi hi': 22 bits).  A tile is
+// float32 in shared memory and is split as it is read.  Af<P>: a 16 x 16 A
+// operand.  Tiles of B are 16 columns (two accumulators) by 16 of the summed
+// index, stored [n][k] or (TR) [k][n].
+// X: the inputs (queries, keys, upstream gradients) are exact in tf32, as
+// float16 values are: their low part is 0 and is left out.
+template <bool X>
+struct FmtF {
+    using E = float;
+    template <int P> struct Af { uint32_t h[2][4], lo[2][4]; };
+    static __device__ __forceinline__ E put(float v) { return v; }
+    static __device__ __forceinline__ void set(Af<2>& a, int s, int i, float v) { split_tf32(v, a.h[s][i], a.lo[s][i]); }
+    // the summed index runs 2t, 2t + 1 inside an accumulator tile; A and B use the same order
+    template <int P>
+    static __device__ __forceinline__ Af<P> from_acc(const float* c0, const float* c1) {
+        Af<P> a;
+#pragma unroll
+        for (int s = 0; s < 2; ++s) {
+            const float* c = s ? c1 : c0;
+            split_tf32(c[0], a.h[s][0], a.lo[s][0]);
+            split_tf32(c[2], a.h[s][1], a.lo[s][1]);
+            split_tf32(c[1], a.h[s][2], a.lo[s][2]);
+            split_tf32(c[3], a.h[s][3], a.lo[s][3]);
+        }
+        return a;
+    }
+    static __device__ __forceinline__ Af<1> from_smem(const E* s, int ld, int m0, int k0) {
+        const Lane L;
+        Af<1> a;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            const float2 p = *reinterpret_cast<const float2*>(s + (m0 + L.g) * ld + k0 + 8 * h + 2 * L.t);
+            const float2 q = *reinterpret_cast<const float2*>(s + (m0 + L.g + 8) * ld + k0 + 8 * h + 2 * L.t);
+            split_tf32(p.x, a.h[h][0], a.lo[h][0]);
+            split_tf32(q.x, a.h[h][1], a.lo[h][1]);
+            split_tf32(p.y, a.h[h][2], a.lo[h][2]);
+            split_tf32(q.y, a.h[h][3], a.lo[h][3]);
+        }
+        return a;
+    }
+    static __device__ __forceinline__ Af<1> from_smem_t(const E* s, int ld, int m0, int k0) {
+        const Lane L;
+        Af<1> a;
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                split_tf32(s[(k0 + 8 * h + 2 * L.t + (i >> 1)) * ld + m0 + L.g + (i & 1) * 8], a.h[h][i], a.lo[h][i]);
+        return a;
+    }
+    static __device__ __forceinline__ void scale_k(Af<1>& a, const float* f, int k0) {
+        const int t = threadIdx.x & 3;
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const float v = __uint_as_float(a.h[h][i]) + __uint_as_float(a.lo[h][i]);
+                split_tf32(v * f[k0 + 8 * h + 2 * t + (i >> 1)], a.h[h][i], a.lo[h][i]);
+            }
+    }
+    // IN: B is a tile of inputs
+    template <int P, bool TR, bool IN = false>
+    static __device__ __forceinline__ void mma2(float* c0, float* c1, const Af<P>& a, const E* s, int ld, int n0,
+                                                int k0) {
+        const Lane L;
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+            float* c = half ? c1 : c0;
+            const int n = n0 + 8 * half + L.g;
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const int k = k0 + 8 * h + 2 * L.t;
+                float2 v;
+                if constexpr (TR) v = make_float2(s[k * ld + n], s[(k + 1) * ld + n]);
+                else v = *reinterpret_cast<const float2*>(s + n * ld + k);
+                uint32_t bh0, bl0, bh1, bl1;
+                split_tf32(v.x, bh0, bl0);
+                split_tf32(v.y, bh1, bl1);
+                mma_tf32(c, a.lo[h], bh0, bh1);
+                if constexpr (!(X && IN)) mma_tf32(c, a.h[h], bl0, bl1);
+                mma_tf32(c, a.h[h], bh0, bh1);
+            }
+        }
+    }
+    static __device__ __forceinline__ void load_t(float* x0, float* x1, const E* s, int ld, int r0, int c0) {
+        const Lane L;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            float* x = h ? x1 : x0;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) x[i] = s[(c0 + 8 * h + 2 * L.t + (i & 1)) * ld + r0 + L.g + (i >> 1) * 8];
+        }
+    }
+};
+
 // ----------------------------------------------------------------------------
 // arguments and the workspace
 // ----------------------------------------------------------------------------
@@ -141,5 +236,12 @@ template <> __device__ __forceinline__ void load8<__nv_bfloat16>(const __nv_bflo
 }
 
 
+
+// delta_planes.cu: bfloat16 inputs whose rows start on 16 bytes
+size_t planes_saved_size(const DArgs& a, bool training);
+size_t planes_bwd_size(const DArgs& a);
+cudaError_t planes_fwd(DArgs a, void* ws, bool training, cudaStream_t s);
+cudaError_t planes_bwd(DArgs a, void* saved, void* ws, float* group, cudaStream_t s);
+cudaError_t planes_read_status(int* out, cudaStream_t s);
 
 }  // namespace eacs

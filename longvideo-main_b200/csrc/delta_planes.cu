@@ -1,0 +1,1557 @@
+// delta_planes.cu -- the gated delta rule on bfloat16 inputs (sm_100a).
+//
+// The formulas are those of delta.cu.  Here every product runs on bf16
+// operands: the inputs are exact in bf16, and a float32 result that goes back
+// in as an operand is split into two bf16 planes, x = hi + lo (16 significant
+// bits), or rounded to one where a term's rounding stays far below the
+// output's own (said where it is done).
+//
+// The two chains are bound by the length of one chunk's dependent products, as
+// only 16-column groups of a state run side by side (a warp each, 8 a head of
+// 128): so everything that does not depend on the state is taken out of the
+// warp that carries it.  A CTA holds G such warps, one or more helpers (the
+// forward's outputs; the reverse chain's Q^T dO) and a loading warp, which
+// copies each chunk's rows and tiles to shared memory with bulk copies, two
+// chunks deep: rows of the inputs by tensor maps (64 tokens by 64 or 16 columns,
+// swizzled so that ldmatrix meets no bank twice; a bulk copy for each row of
+// 256 bytes took 67 cycles a row and bound the chains).  Tiles that kernels hand to each other (T', M, S, U, dS, dV) lie
+// in the workspace as they lie in shared memory, padding included, so that a
+// tile is one copy.  Every wait is bounded.
+#include <cuda.h>
+#include <cudaTypedefs.h>
+
+#include <mutex>
+
+#include "delta_common.cuh"
+
+namespace eacs {
+namespace {
+
+using bf16 = __nv_bfloat16;
+
+// ----------------------------------------------------------------------------
+// barriers and bulk copies
+// ----------------------------------------------------------------------------
+__device__ __forceinline__ void mbar_arrive(uint64_t* bar) {
+    asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory");
+}
+__device__ __forceinline__ void fence_async() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+// global -> shared, 16-byte aligned, counted on `bar`
+__device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
+    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
+                     smem_u32(dst)),
+                 "l"(src), "r"(bytes), "r"(smem_u32(bar))
+                 : "memory");
+}
+__device__ __forceinline__ void bulk_store(void* dst, const void* src, uint32_t bytes) {
+    asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;" ::"l"(dst), "r"(smem_u32(src)), "r"(bytes)
+                 : "memory");
+}
+__device__ __forceinline__ void bulk_commit() { asm volatile("cp.async.bulk.commit_group;" ::: "memory"); }
+__device__ __forceinline__ void bulk_wait_read() { asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory"); }
+__device__ __forceinline__ void bulk_wait_all() { asm volatile("cp.async.bulk.wait_group 0;" ::: "memory"); }
+// a warp's wait, with one outcome for all its lanes
+__device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity) {
+    return __all_sync(0xffffffffu, mbar_wait(bar, parity));
+}
+// one arrival for a warp, after what all its lanes did
+__device__ __forceinline__ void warp_arrive(uint64_t* bar) {
+    __syncwarp();
+    if ((threadIdx.x & 31) == 0) mbar_arrive(bar);
+}
+
+// ----------------------------------------------------------------------------
+// operands
+// ----------------------------------------------------------------------------
+template <int P> struct Af { uint32_t r[P][4]; };  // 16 x 16 of A in P planes
+
+template <int P>
+__device__ __forceinline__ Af<P> from_acc(const float* c0, const float* c1) {
+    Af<P> a;
+    const float v[8] = {c0[0], c0[1], c0[2], c0[3], c1[0], c1[1], c1[2], c1[3]};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        a.r[0][i] = pack_bf16(v[2 * i], v[2 * i + 1]);
+        if constexpr (P == 2) {
+            const float2 h = unpack_bf16(a.r[0][i]);
+            a.r[1][i] = pack_bf16(v[2 * i] - h.x, v[2 * i + 1] - h.y);
+        }
+    }
+    return a;
+}
+// of a tile stored [m][k], and stored [k][m]
+__device__ __forceinline__ void ld_a(uint32_t* r, const bf16* s, int ld, int m0, int k0) {
+    const int l = threadIdx.x & 31;
+    ldsm4(r, s + (m0 + (l & 15)) * ld + k0 + (l >> 4) * 8);
+}
+__device__ __forceinline__ void ld_at(uint32_t* r, const bf16* s, int ld, int m0, int k0) {
+    const int l = threadIdx.x & 31;
+    ldsm4t(r, s + (k0 + (l & 7) + ((l >> 4) & 1) * 8) * ld + m0 + ((l >> 3) & 1) * 8);
+}
+// 16 columns of B by 16 of the summed index, stored [n][k], and (TR) [k][n]
+template <bool TR>
+__device__ __forceinline__ void ld_b(uint32_t* b, const bf16* s, int ld, int n0, int k0) {
+    const int l = threadIdx.x & 31;
+    if constexpr (TR) ldsm4t(b, s + (k0 + (l & 7) + ((l >> 3) & 1) * 8) * ld + n0 + ((l >> 4) & 1) * 8);
+    else ldsm4(b, s + (n0 + (l & 7) + ((l >> 4) & 1) * 8) * ld + k0 + ((l >> 3) & 1) * 8);
+}
+// Tiles that tensor maps bring.  Rows of 64 columns in 128-byte swizzle, 64
+// rows a box, boxes one after another (queries, keys); rows of 16 columns in
+// 32-byte swizzle (values and upstream gradients, a box a group of 16).
+__device__ __forceinline__ int at128(int row, int col) {
+    return (col >> 6) * (kC * 64) + row * 64 + ((((col >> 3) & 7) ^ (row & 7)) << 3) + (col & 7);
+}
+__device__ __forceinline__ int at32(int row, int col) { return row * 16 + (((col >> 3) ^ ((row >> 2) & 1)) << 3); }
+
+template <bool TR>
+__device__ __forceinline__ void ld_b128(uint32_t* b, const bf16* s, int n0, int k0) {
+    const int l = threadIdx.x & 31;
+    if constexpr (TR) ldsm4t(b, s + at128(k0 + (l & 7) + ((l >> 3) & 1) * 8, n0 + ((l >> 4) & 1) * 8));
+    else ldsm4(b, s + at128(n0 + (l & 7) + ((l >> 4) & 1) * 8, k0 + ((l >> 3) & 1) * 8));
+}
+// 16 rows of A: tokens m0.. of a group, and (at) its 16 columns by tokens k0..
+__device__ __forceinline__ void ld_a32(uint32_t* r, const bf16* s, int m0) {
+    const int l = threadIdx.x & 31;
+    ldsm4(r, s + at32(m0 + (l & 15), (l >> 4) * 8));
+}
+__device__ __forceinline__ void ld_at32(uint32_t* r, const bf16* s, int k0) {
+    const int l = threadIdx.x & 31;
+    ldsm4t(r, s + at32(k0 + (l & 7) + ((l >> 4) & 1) * 8, ((l >> 3) & 1) * 8));
+}
+__device__ __forceinline__ void mma_pair(float* c0, float* c1, const uint32_t* a, const uint32_t* b) {
+    mma_bf16(c0, a, b[0], b[1]);
+    mma_bf16(c1, a, b[2], b[3]);
+}
+// A in P planes times one plane of B
+template <int P, bool TR>
+__device__ __forceinline__ void mm(float* c0, float* c1, const Af<P>& a, const bf16* s, int ld, int n0, int k0) {
+    uint32_t b[4];
+    ld_b<TR>(b, s, ld, n0, k0);
+#pragma unroll
+    for (int p = P - 1; p >= 0; --p) mma_pair(c0, c1, a.r[p], b);
+}
+template <int P, bool TR>
+__device__ __forceinline__ void mm128(float* c0, float* c1, const Af<P>& a, const bf16* s, int n0, int k0) {
+    uint32_t b[4];
+    ld_b128<TR>(b, s, n0, k0);
+#pragma unroll
+    for (int p = P - 1; p >= 0; --p) mma_pair(c0, c1, a.r[p], b);
+}
+// A in P planes times B in two (the product of the low planes is left out)
+template <int P, bool TR>
+__device__ __forceinline__ void mm_hl(float* c0, float* c1, const Af<P>& a, const bf16* hi, const bf16* lo, int ld,
+                                      int n0, int k0) {
+    uint32_t b[4];
+    ld_b<TR>(b, lo, ld, n0, k0);
+    mma_pair(c0, c1, a.r[0], b);
+    mm<P, TR>(c0, c1, a, hi, ld, n0, k0);
+}
+// Steps 0..N-1 of a product: a step's tiles of B (up to four pairs) are read
+// while the step before is multiplied.
+template <int N, bool AHEAD = true, class Read, class Use>
+__device__ __forceinline__ void steps(Read read, Use use) {
+    uint32_t b[AHEAD ? 2 : 1][4][4];
+    if constexpr (AHEAD) read(0, b[0]);
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        if constexpr (AHEAD) {
+            if (i + 1 < N) read(i + 1, b[(i + 1) & 1]);
+            use(i, b[i & 1]);
+        } else {
+            read(i, b[0]);
+            use(i, b[0]);
+        }
+    }
+}
+// accumulators j0.. of `n` pairs += A (planes P-1 .. 0) B, plane by plane: eight
+// products lie between two that add to the same accumulator
+template <int P>
+__device__ __forceinline__ void mma_step(float (*c)[4], const Af<P>& a, const uint32_t (*b)[4], int from = 0, int to = 4) {
+#pragma unroll
+    for (int p = P - 1; p >= 0; --p)
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            if (i >= from && i < to) mma_pair(c[2 * i], c[2 * i + 1], a.r[p], b[i]);
+}
+// accumulators of 16 rows by 16 columns to a tile [row][col] (as ld_a reads it)
+__device__ __forceinline__ void st_tile(bf16* s, int ld, int c0, const uint32_t* r) {
+    const int l = threadIdx.x & 31;
+    asm volatile("stmatrix.sync.aligned.m8n8.x4.shared.b16 [%0], {%1,%2,%3,%4};" ::"r"(
+                     smem_u32(s + (l & 15) * ld + c0 + (l >> 4) * 8)),
+                 "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3])
+                 : "memory");
+}
+// and to a tile [col][row]
+__device__ __forceinline__ void st_tile_t(bf16* s, int ld, int c0, const uint32_t* r) {
+    const int l = threadIdx.x & 31;
+    asm volatile("stmatrix.sync.aligned.m8n8.x4.trans.shared.b16 [%0], {%1,%2,%3,%4};" ::"r"(
+                     smem_u32(s + (c0 + (l & 7) + (l >> 4) * 8) * ld + ((l >> 3) & 1) * 8)),
+                 "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3])
+                 : "memory");
+}
+
+constexpr int kCC = kC * kTld;  // elements of a 64 x 64 tile
+
+// A tensor map of (B, L, H, D) with a dense last dimension, read as (D, L, H, B).
+__device__ __forceinline__ void tma_load(void* dst, const CUtensorMap* m, uint64_t* bar, int x, int t, int h, int b) {
+    asm volatile(
+        "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6}], "
+        "[%2];" ::"r"(smem_u32(dst)),
+        "l"(m), "r"(smem_u32(bar)), "r"(x), "r"(t), "r"(h), "r"(b)
+        : "memory");
+}
+struct Maps { CUtensorMap q, k, v, d; };
+
+// Rows `rows`.. of `boxes` boxes of 64 rows x W columns become zeros; the lanes
+// of one warp.  (Rows of a padded batch behind a sequence's end: what they hold,
+// NaN as it may be, is not to reach a product.  Behind L the copy itself gives 0.)
+template <int W>
+__device__ __forceinline__ void zero_rows(bf16* s, int boxes, int rows) {
+    const int per = (kC - rows) * (W / 8);
+    for (int i = threadIdx.x & 31; i < boxes * per; i += 32)
+        *reinterpret_cast<uint4*>(s + (i / per) * kC * W + rows * W + (i % per) * 8) = make_uint4(0, 0, 0, 0);
+}
+// The aligned start of dynamic shared memory (swizzled boxes want 1024 bytes).
+__device__ __forceinline__ unsigned char* align_smem(unsigned char* p) { return p + ((1024u - (smem_u32(p) & 1023u)) & 1023u); }
+constexpr int up1024(int x) { return (x + 1023) / 1024 * 1024; }
+// e^(G_i - G_j) from G in units of log 2, high and low parts
+__device__ __forceinline__ float ratio(const float* G, int i, int j) {
+    return ex2_approx((G[i] - G[j]) + (G[kC + i] - G[kC + j]));
+}
+
+// ----------------------------------------------------------------------------
+// gates, T' and M of a chunk
+// ----------------------------------------------------------------------------
+// (I + A)^-1 by blocks, in float32: the 16 x 16 blocks on the diagonal by
+// forward substitution (a thread a column), then twice the step from blocks of
+// s to blocks of 2 s, [[P, 0], [R, Q]]^-1 = [[P^-1, 0], [-Q^-1 R P^-1, Q^-1]],
+// whose products run on the tensor cores with operands split in two tf32
+// parts.  (Forward substitution alone takes 2016 dependent multiply-adds.)
+constexpr int kAld = kC + 8;  // float32 tiles
+
+template <int KD>
+__global__ void __launch_bounds__(128) planes_prep_k(DArgs a) {
+    using F = FmtF<false>;
+    const int c = blockIdx.x, h = blockIdx.y, b = blockIdx.z;
+    const int len = row_length(a, b);
+    if (c * kC >= len) return;
+    const int rows = min(kC, len - c * kC);
+    const int hk = h / (a.Hv / a.Hk);
+    const int64_t id = (static_cast<int64_t>(b) * a.Hv + h) * a.n + c, t0 = static_cast<int64_t>(c) * kC;
+    extern __shared__ __align__(128) unsigned char smem_raw[];
+    unsigned char* smem = smem_raw;
+    constexpr int LD = KD + 8;
+    bf16* sK = reinterpret_cast<bf16*>(smem);
+    bf16* sQ = sK + kC * LD;
+    float* sA = reinterpret_cast<float*>(sQ + kC * LD);  // A, lower triangle
+    float* sT = sA + kC * kAld;                          // its inverse
+    float* sY = reinterpret_cast<float*>(smem);          // a product (K and Q are done with by then)
+    __shared__ float sG[2 * kC], sB[kC];
+    const int tid = threadIdx.x, warp = tid >> 5;
+    const Lane L;
+    {
+        const bf16* k = static_cast<const bf16*>(a.k) + b * a.sk.b + t0 * a.sk.t + hk * a.sk.h;
+        const bf16* q = static_cast<const bf16*>(a.q) + b * a.sq.b + t0 * a.sq.t + hk * a.sq.h;
+        for (int i = tid; i < kC * (KD / 8); i += 128) {
+            const int r = i / (KD / 8), col = (i % (KD / 8)) * 8;
+            const bool in = r < rows && col < a.K;
+            cp_async16(sK + r * LD + col, in ? k + r * a.sk.t + col : k, in);
+            cp_async16(sQ + r * LD + col, in ? q + r * a.sq.t + col : q, in);
+        }
+        cp_async_commit();
+    }
+    for (int i = tid; i < kC * kAld; i += 128) sT[i] = 0.f;
+    if (warp == 0) {
+        double s[2];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const int r = 2 * L.l + i;
+            float gv = 0.f, bv = 0.f;
+            if (r < rows) {
+                gv = gate_value(a.g, a.gate_dtype, b * a.sg.b + (t0 + r) * a.sg.t + h * a.sg.h);
+                bv = hold_beta(gate_value(a.beta, a.gate_dtype, b * a.sb.b + (t0 + r) * a.sb.t + h * a.sb.h));
+                gv = gv < -200.f ? -200.f : gv;  // e^-200 is 0 in float32
+            }
+            s[i] = gv * 1.4426950408889634;  // to powers of two
+            sB[r] = bv;
+        }
+        s[1] += s[0];
+        double run = s[1];
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const double up = __shfl_up_sync(0xffffffffu, run, o);
+            if (L.l >= o) run += up;
+        }
+        const double before = run - s[1], total = __shfl_sync(0xffffffffu, run, 31);
+        float* ga = a.gates + id * kGates;
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const int r = 2 * L.l + i;
+            const double G = before + s[i];
+            const float hi = static_cast<float>(G), lo = static_cast<float>(G - hi);
+            const float gam = exp2f(static_cast<float>(G));
+            sG[r] = ga[r] = hi;
+            sG[kC + r] = ga[kC + r] = lo;
+            ga[2 * kC + r] = gam;
+            ga[3 * kC + r] = exp2f(static_cast<float>(total - G));
+            ga[4 * kC + r] = a.scale * gam;
+        }
+    }
+    cp_async_wait_all();
+    __syncthreads();
+    {  // a warp 16 rows of A and of M
+        float kk[kC / 8][4] = {}, qk[kC / 8][4] = {};
+        const int m0 = warp * 16;
+#pragma unroll
+        for (int k0 = 0; k0 < KD; k0 += 16) {
+            Af<1> ak, aq;
+            ld_a(ak.r[0], sK, LD, m0, k0);
+            ld_a(aq.r[0], sQ, LD, m0, k0);
+#pragma unroll
+            for (int p = 0; p < kC / 16; ++p)
+                if (p <= warp) {
+                    uint32_t bk[4];
+                    ld_b<false>(bk, sK, LD, 16 * p, k0);
+                    mma_pair(kk[2 * p], kk[2 * p + 1], ak.r[0], bk);
+                    mma_pair(qk[2 * p], qk[2 * p + 1], aq.r[0], bk);
+                }
+        }
+        bf16* M = static_cast<bf16*>(a.M) + id * 2 * kCC;
+#pragma unroll
+        for (int j = 0; j < kC / 8; ++j) {
+            float m[4] = {};
+            if (j <= 2 * warp + 1)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const int r = m0 + L.g + (e >> 1) * 8, col = 8 * j + 2 * L.t + (e & 1);
+                    const float w = col <= r ? ratio(sG, r, col) : 0.f;
+                    m[e] = a.scale * w * qk[j][e];
+                    sA[r * kAld + col] = col < r ? sB[r] * w * kk[j][e] : 0.f;
+                }
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                const uint32_t hi = pack_bf16(m[2 * e], m[2 * e + 1]);
+                const float2 f = unpack_bf16(hi);
+                const int o = (m0 + L.g + 8 * e) * kTld + 8 * j + 2 * L.t;
+                *reinterpret_cast<uint32_t*>(M + o) = hi;
+                *reinterpret_cast<uint32_t*>(M + kCC + o) = pack_bf16(m[2 * e] - f.x, m[2 * e + 1] - f.y);
+            }
+        }
+    }
+    __syncthreads();
+    if (tid < kC) {  // column tid of its diagonal block
+        const int r0 = tid & ~15, col = tid & 15;
+        float x[16];
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+            float s0 = i == col ? 1.f : 0.f, s1 = 0.f;
+            const float* ar = sA + (r0 + i) * kAld + r0;
+#pragma unroll
+            for (int m = 0; m < i; ++m) {
+                if (m & 1) s1 = fmaf(-ar[m], x[m], s1);
+                else s0 = fmaf(-ar[m], x[m], s0);
+            }
+            x[i] = s0 + s1;
+        }
+#pragma unroll
+        for (int i = 0; i < 16; ++i) sT[(r0 + i) * kAld + tid] = x[i];
+    }
+    __syncthreads();
+    // R P^-1 into sY, then -Q^-1 of it into the inverse; warps 0, 1: a pair of 16 x 16 blocks each
+    auto put = [&](float* d, int r, int col, const float* x0, const float* x1, float sign) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const int rr = r + L.g + (e >> 1) * 8, cc = col + 2 * L.t + (e & 1);
+            d[rr * kAld + cc] = sign * x0[e];
+            d[rr * kAld + cc + 8] = sign * x1[e];
+        }
+    };
+    if (warp < 2) {
+        const int o = 32 * warp;
+        float x0[4] = {}, x1[4] = {};
+        F::template mma2<1, true>(x0, x1, F::from_smem(sA, kAld, o + 16, o), sT, kAld, o, o);
+        put(sY, o + 16, o, x0, x1, 1.f);
+        __syncwarp();
+        float z0[4] = {}, z1[4] = {};
+        F::template mma2<1, true>(z0, z1, F::from_smem(sT, kAld, o + 16, o + 16), sY, kAld, o, o + 16);
+        put(sT, o + 16, o, z0, z1, -1.f);
+    }
+    __syncthreads();
+    {  // blocks of 32: a warp one 16 x 16 tile of each product
+        const int r = 32 + 16 * (warp >> 1), col = 16 * (warp & 1);
+        float x0[4] = {}, x1[4] = {};
+#pragma unroll
+        for (int k = 0; k < 32; k += 16)
+            F::template mma2<1, true>(x0, x1, F::from_smem(sA, kAld, r, k), sT, kAld, col, k);
+        put(sY, r, col, x0, x1, 1.f);
+        __syncthreads();
+        float z0[4] = {}, z1[4] = {};
+#pragma unroll
+        for (int k = 32; k < 64; k += 16)
+            F::template mma2<1, true>(z0, z1, F::from_smem(sT, kAld, r, k), sY, kAld, col, k);
+        put(sT, r, col, z0, z1, -1.f);
+    }
+    __syncthreads();
+    bf16* T = static_cast<bf16*>(a.T) + id * 2 * kCC;
+    for (int i = tid; i < kC * 8; i += 128) {
+        const int r = i >> 3, c8 = (i & 7) * 8;
+        uint32_t hi[4], lo[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const float x = sT[r * kAld + c8 + 2 * e] * sB[c8 + 2 * e];
+            const float y = sT[r * kAld + c8 + 2 * e + 1] * sB[c8 + 2 * e + 1];
+            hi[e] = pack_bf16(x, y);
+            const float2 f = unpack_bf16(hi[e]);
+            lo[e] = pack_bf16(x - f.x, y - f.y);
+        }
+        *reinterpret_cast<uint4*>(T + r * kTld + c8) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+        *reinterpret_cast<uint4*>(T + kCC + r * kTld + c8) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+    }
+}
+
+// ----------------------------------------------------------------------------
+// the forward chain and the outputs
+// ----------------------------------------------------------------------------
+template <int KD, int G>
+struct Fwd {
+    static constexpr int LDK = KD + 8, LDO = 24;
+    // helpers: warps 0..G-1 carry states; with three of them one helper has the fourth scheduler to itself
+    static constexpr int H = G == 3 ? 1 : G, kWarps = G + H + 1;
+    static constexpr int kK = 0, kQ = kK + kC * KD, kV = kQ + kC * KD, kT = kV + kC * 16 * G, kM = kT + 2 * kCC;
+    static constexpr int kGa = kM + 2 * kCC;  // (elements) the gates, float32
+    static constexpr int kLoad = kGa * 2 + kGates * 4, kStage = up1024(kLoad);  // bytes
+    static constexpr int kS = 0, kU = 2 * 16 * LDK, kO = kU + 2 * 16 * kTld;  // a group's tiles (elements)
+    static constexpr int kGroup = (kO + kC * LDO) * 2;
+    static constexpr int kBars = 2 * kStage + G * kGroup;
+    static constexpr size_t bytes = 1024 + kBars + 8 * (5 + 4 * G);
+};
+
+// S^T (16 value rows v0.., K columns) of a (K, V) float32 state
+template <int KD>
+__device__ __forceinline__ void state_load(float (*S)[4], const float* p, int K, int V, int v0, const Lane& L) {
+#pragma unroll
+    for (int j = 0; j < KD / 8; ++j)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const int k = 8 * j + 2 * L.t + (e & 1), v = v0 + L.g + (e >> 1) * 8;
+            S[j][e] = p && k < K && v < V ? p[static_cast<int64_t>(k) * V + v] : 0.f;
+        }
+}
+template <int KD>
+__device__ __forceinline__ void state_store(const float (*S)[4], float* p, int K, int V, int v0, const Lane& L) {
+#pragma unroll
+    for (int j = 0; j < KD / 8; ++j)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const int k = 8 * j + 2 * L.t + (e & 1), v = v0 + L.g + (e >> 1) * 8;
+            if (k < K && v < V) p[static_cast<int64_t>(k) * V + v] = S[j][e];
+        }
+}
+
+template <int KD, int G>
+__global__ void __launch_bounds__(Fwd<KD, G>::kWarps * 32) planes_chain_k(DArgs a, const __grid_constant__ Maps maps) {
+    using Sm = Fwd<KD, G>;
+    const int h = blockIdx.y, b = blockIdx.z, hk = h / (a.Hv / a.Hk);
+    const int len = row_length(a, b), nc = (len + kC - 1) / kC;
+    const int warp = threadIdx.x >> 5, vb = blockIdx.x * 16 * G;
+    const Lane L;
+    extern __shared__ __align__(128) unsigned char smem_raw[];
+    unsigned char* smem = align_smem(smem_raw);
+    uint64_t* full = reinterpret_cast<uint64_t*>(smem + Sm::kBars);
+    uint64_t* empty = full + 2;
+    uint64_t* land = empty + 2;
+    uint64_t *s_full = land + 1, *s_empty = s_full + G, *u_full = s_empty + G, *u_empty = u_full + G;
+    const int64_t head = static_cast<int64_t>(b) * a.Hv + h;
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < 2; ++s) {
+            mbar_init(&full[s], 1);
+            mbar_init(&empty[s], G + Sm::H);
+        }
+        mbar_init(land, 1);
+        for (int i = 0; i < 4 * G; ++i) mbar_init(&s_full[i], 1);
+        fence_mbar_init();
+    }
+    __syncthreads();
+    bool ok = true;
+    if (warp == Sm::kWarps - 1) {
+        // ---- loads ----
+        for (int c = 0; c < nc && ok; ++c) {
+            bf16* e = reinterpret_cast<bf16*>(smem + (c & 1) * Sm::kStage);
+            const int t0 = c * kC, rows = min(kC, len - t0);
+            const bool tail = rows < min(kC, a.L - t0);
+            uint64_t* bar = tail ? land : &full[c & 1];
+            ok = warp_wait(&empty[c & 1], ((c >> 1) & 1) ^ 1);
+            if (L.l == 0) {
+                const int64_t id = head * a.n + c;
+                mbar_expect_tx(bar, Sm::kLoad);
+#pragma unroll
+                for (int x = 0; x < KD; x += 64) tma_load(e + Sm::kK + x * kC, &maps.k, bar, x, t0, hk, b);
+                bulk_load(e + Sm::kT, static_cast<const bf16*>(a.T) + id * 2 * kCC, 4 * kCC, bar);
+#pragma unroll
+                for (int g = 0; g < G; ++g) tma_load(e + Sm::kV + g * kC * 16, &maps.v, bar, vb + 16 * g, t0, h, b);
+                bulk_load(e + Sm::kGa, a.gates + id * kGates, kGates * 4, bar);
+#pragma unroll
+                for (int x = 0; x < KD; x += 64) tma_load(e + Sm::kQ + x * kC, &maps.q, bar, x, t0, hk, b);
+                bulk_load(e + Sm::kM, static_cast<const bf16*>(a.M) + id * 2 * kCC, 4 * kCC, bar);
+            }
+            __syncwarp();
+            if (tail) {
+                ok = warp_wait(land, 0) && ok;
+                zero_rows<64>(e + Sm::kK, 2 * (KD / 64), rows);  // keys and queries
+                zero_rows<16>(e + Sm::kV, G, rows);
+                warp_arrive(&full[c & 1]);
+            }
+        }
+        return;
+    }
+    if (warp < G) {
+        // ---- a state of 16 value columns ----
+        const int v0 = vb + warp * 16;
+        const bool on = v0 < a.Vp;
+        bf16* mine = reinterpret_cast<bf16*>(smem + 2 * Sm::kStage + warp * Sm::kGroup);
+        bf16 *sS = mine + Sm::kS, *sU = mine + Sm::kU;
+        float S[KD / 8][4];
+        state_load<KD>(S, a.initial ? a.initial + head * a.K * a.V : nullptr, a.K, a.V, v0, L);
+        for (int c = 0; c < nc && ok; ++c) {
+            const unsigned char* st = smem + (c & 1) * Sm::kStage;
+            const bf16* e = reinterpret_cast<const bf16*>(st);
+            const float* ga = reinterpret_cast<const float*>(e + Sm::kGa);
+            const float *gam = ga + 2 * kC, *dec = ga + 3 * kC;
+            const int64_t id = head * a.n + c;
+            ok = warp_wait(&full[c & 1], (c >> 1) & 1);
+            if (on) {
+                ok = warp_wait(&s_empty[warp], (c & 1) ^ 1) && ok;
+                if (a.S) {  // the last chunk's copies have left the tiles
+                    if (L.l == 0) bulk_wait_read();
+                    __syncwarp();
+                }
+                // (K S0)^T, S in two planes
+                float X[kC / 8][4] = {};
+                steps<KD / 16>(
+                    [&](int i, uint32_t(*f)[4]) {
+#pragma unroll
+                        for (int p = 0; p < 4; ++p) ld_b128<false>(f[p], e + Sm::kK, 16 * p, 16 * i);
+                    },
+                    [&](int i, const uint32_t(*f)[4]) {
+                        const Af<2> af = from_acc<2>(S[2 * i], S[2 * i + 1]);
+                        st_tile(sS, Sm::LDK, 16 * i, af.r[0]);
+                        if (a.S) st_tile(sS + 16 * Sm::LDK, Sm::LDK, 16 * i, af.r[1]);
+                        mma_step(X, af, f);
+                    });
+                if (a.S) fence_async();
+                warp_arrive(&s_full[warp]);
+                if (a.S && L.l == 0) {
+                    bf16* to = static_cast<bf16*>(a.S) + (id * 2 * a.Vp + v0) * Sm::LDK;
+                    bulk_store(to, sS, 32 * Sm::LDK);
+                    bulk_store(to + static_cast<int64_t>(a.Vp) * Sm::LDK, sS + 16 * Sm::LDK, 32 * Sm::LDK);
+                    bulk_commit();
+                }
+                // X = V^T - gam (K S0)^T
+#pragma unroll
+                for (int p = 0; p < kC / 16; ++p) {
+                    uint32_t r[4];
+                    ld_at32(r, e + Sm::kV + warp * kC * 16, 16 * p);
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) {
+                        const float2 f = *reinterpret_cast<const float2*>(gam + 16 * p + 8 * i + 2 * L.t);
+                        float* x = X[2 * p + i];
+                        const float2 lo = unpack_bf16(r[2 * i]), hi = unpack_bf16(r[2 * i + 1]);
+                        x[0] = fmaf(-f.x, x[0], lo.x);
+                        x[1] = fmaf(-f.y, x[1], lo.y);
+                        x[2] = fmaf(-f.x, x[2], hi.x);
+                        x[3] = fmaf(-f.y, x[3], hi.y);
+                    }
+                }
+                // U^T = X T'^T, both in two planes
+                float U[kC / 8][4] = {};
+                {
+                    Af<2> af;
+                    steps<8>(  // the low plane of T', then the high one
+                        [&](int i, uint32_t(*f)[4]) {
+#pragma unroll
+                            for (int p = 0; p < 4; ++p)
+                                if (p >= i / 2) ld_b<false>(f[p], e + Sm::kT + (i & 1 ? 0 : kCC), kTld, 16 * p, 16 * (i / 2));
+                        },
+                        [&](int i, const uint32_t(*f)[4]) {
+                            if (i & 1) {
+                                mma_step(U, af, f, i / 2);
+                            } else {
+                                af = from_acc<2>(X[i], X[i + 1]);
+                                mma_step(U, Af<1>{{{af.r[0][0], af.r[0][1], af.r[0][2], af.r[0][3]}}}, f, i / 2);
+                            }
+                        });
+                }
+                ok = warp_wait(&u_empty[warp], (c & 1) ^ 1) && ok;
+                const float gc = gam[kC - 1];
+#pragma unroll
+                for (int j = 0; j < KD / 8; ++j)
+#pragma unroll
+                    for (int x = 0; x < 4; ++x) S[j][x] *= gc;
+                // S^T = gam_63 S^T + (d U)^T K
+                {
+                    Af<2> af;
+                    constexpr int Q = KD / 64;
+                    steps<4 * Q>(
+                        [&](int i, uint32_t(*f)[4]) {
+#pragma unroll
+                            for (int p = 0; p < 4; ++p) ld_b128<true>(f[p], e + Sm::kK, 64 * (i % Q) + 16 * p, 16 * (i / Q));
+                        },
+                        [&](int i, const uint32_t(*f)[4]) {
+                            const int kk = i / Q;
+                            if (i % Q == 0) {
+                                const Af<2> au = from_acc<2>(U[2 * kk], U[2 * kk + 1]);
+                                st_tile(sU, kTld, 16 * kk, au.r[0]);
+                                st_tile(sU + 16 * kTld, kTld, 16 * kk, au.r[1]);
+                                float y[2][4];
+#pragma unroll
+                                for (int x = 0; x < 2; ++x) {
+                                    const float2 d = *reinterpret_cast<const float2*>(dec + 16 * kk + 8 * x + 2 * L.t);
+                                    const float* u = U[2 * kk + x];
+                                    y[x][0] = u[0] * d.x;
+                                    y[x][1] = u[1] * d.y;
+                                    y[x][2] = u[2] * d.x;
+                                    y[x][3] = u[3] * d.y;
+                                }
+                                af = from_acc<2>(y[0], y[1]);
+                            }
+                            mma_step(S + 8 * (i % Q), af, f);
+                        });
+                }
+                if (a.S) fence_async();
+                warp_arrive(&u_full[warp]);
+                if (a.S && L.l == 0) {
+                    bf16* to = static_cast<bf16*>(a.U) + (id * 2 * a.Vp + v0) * kTld;
+                    bulk_store(to, sU, 32 * kTld);
+                    bulk_store(to + static_cast<int64_t>(a.Vp) * kTld, sU + 16 * kTld, 32 * kTld);
+                    bulk_commit();
+                }
+            }
+            warp_arrive(&empty[c & 1]);
+        }
+        if (on && a.final_state && ok) state_store<KD>(S, a.final_state + head * a.K * a.V, a.K, a.V, v0, L);
+        if (a.S && L.l == 0) bulk_wait_all();
+        return;
+    }
+    // ---- outputs of the groups g = helper, helper + H, .. ----
+    const int helper = warp - G;
+    constexpr int NG = (G + Sm::H - 1) / Sm::H;
+    const int64_t ost = static_cast<int64_t>(a.Hv) * a.V;
+    bf16* out = static_cast<bf16*>(a.out) + static_cast<int64_t>(b) * a.L * ost + static_cast<int64_t>(h) * a.V;
+    for (int c = 0; c < nc && ok; ++c) {
+        const unsigned char* st = smem + (c & 1) * Sm::kStage;
+        const bf16* e = reinterpret_cast<const bf16*>(st);
+        const float* sgam = reinterpret_cast<const float*>(e + Sm::kGa) + 4 * kC;
+        const int rows = min(kC, len - c * kC), all = min(kC, a.L - c * kC);
+        ok = warp_wait(&full[c & 1], (c >> 1) & 1);
+        float O[NG][kC / 8][4] = {};
+#pragma unroll
+        for (int i = 0; i < NG; ++i) {
+            const int g = helper + i * Sm::H;
+            if (vb + 16 * g >= a.Vp) break;
+            const bf16* sS = reinterpret_cast<const bf16*>(smem + 2 * Sm::kStage + g * Sm::kGroup) + Sm::kS;
+            ok = warp_wait(&s_full[g], c & 1) && ok;
+            // scale gam Q S0: S in one plane (its rounding, 2^-9 of terms of any sign, against the
+            // output's own: y is off by 2.2e-3 in the norm instead of 1.7e-3, for half the products)
+            Af<1> as[2];
+            steps<KD / 16>(
+                [&](int k, uint32_t(*f)[4]) {
+                    ld_a(as[k & 1].r[0], sS, Sm::LDK, 0, 16 * k);
+#pragma unroll
+                    for (int p = 0; p < 4; ++p) ld_b128<false>(f[p], e + Sm::kQ, 16 * p, 16 * k);
+                },
+                [&](int k, const uint32_t(*f)[4]) { mma_step(O[i], as[k & 1], f); });
+            warp_arrive(&s_empty[g]);
+#pragma unroll
+            for (int j = 0; j < kC / 8; ++j) {
+                const float2 f = *reinterpret_cast<const float2*>(sgam + 8 * j + 2 * L.t);
+                O[i][j][0] *= f.x;
+                O[i][j][1] *= f.y;
+                O[i][j][2] *= f.x;
+                O[i][j][3] *= f.y;
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < NG; ++i) {
+            const int g = helper + i * Sm::H, v0 = vb + 16 * g;
+            if (v0 >= a.Vp) break;
+            bf16* theirs = reinterpret_cast<bf16*>(smem + 2 * Sm::kStage + g * Sm::kGroup);
+            ok = warp_wait(&u_full[g], c & 1) && ok;
+            Af<2> au[2];
+            steps<8>(
+                [&](int k, uint32_t(*f)[4]) {
+                    if (!(k & 1)) {
+                        ld_a(au[(k / 2) & 1].r[0], theirs + Sm::kU, kTld, 0, 8 * k);
+                        ld_a(au[(k / 2) & 1].r[1], theirs + Sm::kU + 16 * kTld, kTld, 0, 8 * k);
+                    }
+#pragma unroll
+                    for (int p = 0; p < 4; ++p)
+                        if (p >= k / 2) ld_b<false>(f[p], e + Sm::kM + (k & 1 ? 0 : kCC), kTld, 16 * p, 16 * (k / 2));
+                },
+                [&](int k, const uint32_t(*f)[4]) {
+                    const Af<2>& af = au[(k / 2) & 1];
+                    if (k & 1) mma_step(O[i], af, f, k / 2);
+                    else mma_step(O[i], Af<1>{{{af.r[0][0], af.r[0][1], af.r[0][2], af.r[0][3]}}}, f, k / 2);
+                });
+            warp_arrive(&u_empty[g]);
+            // rows of 16 values through shared memory: 32 bytes a token, two lanes each
+            bf16* sO = theirs + Sm::kO;
+#pragma unroll
+            for (int p = 0; p < kC / 16; ++p) {
+                const Af<1> o = from_acc<1>(O[i][2 * p], O[i][2 * p + 1]);
+                st_tile_t(sO, Sm::LDO, 16 * p, o.r[0]);
+            }
+            __syncwarp();
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const int r = 16 * j + (L.l >> 1), col = (L.l & 1) * 8;
+                if (r < all && v0 + col < a.V) {
+                    uint4 x = *reinterpret_cast<const uint4*>(sO + r * Sm::LDO + col);
+                    if (r >= rows) x = make_uint4(0, 0, 0, 0);
+                    *reinterpret_cast<uint4*>(out + (static_cast<int64_t>(c) * kC + r) * ost + v0 + col) = x;
+                }
+            }
+            __syncwarp();
+        }
+        warp_arrive(&empty[c & 1]);
+    }
+    for (int g = helper; g < G; g += Sm::H)  // behind the sequence
+        for (int64_t i = static_cast<int64_t>(nc) * kC * 2 + L.l; i < static_cast<int64_t>(a.L) * 2; i += 32) {
+            const int v = vb + 16 * g + (i & 1) * 8;
+            if (v < a.V) *reinterpret_cast<uint4*>(out + (i >> 1) * ost + v) = make_uint4(0, 0, 0, 0);
+        }
+}
+
+// ----------------------------------------------------------------------------
+// the reverse chain
+// ----------------------------------------------------------------------------
+// All operands in two planes but for dV in K^T (gam dV), whose rounding stays
+// below the gradients' own (measured against 64 bits: 1.7e-3 of the norm of
+// every gradient, which is the outputs' rounding alone, with either).
+template <int KD, int G>
+struct Rev {
+    static constexpr int LDK = KD + 8;
+    static constexpr int H = G == 3 ? 1 : G, kWarps = G + H + 1;
+    static constexpr int kK = 0, kQ = kK + kC * KD, kD = kQ + kC * KD, kT = kD + kC * 16 * G, kM = kT + 2 * kCC;
+    static constexpr int kGa = kM + 2 * kCC;
+    static constexpr int kLoad = kGa * 2 + kGates * 4, kStage = up1024(kLoad);
+    static constexpr int kS = 0, kX = 2 * 16 * LDK * 2, kZ = kX + 2 * 16 * kTld * 2;  // a group's tiles (bytes)
+    static constexpr int kGroup = kZ + 16 * KD * 4;
+    static constexpr int kBars = 2 * kStage + G * kGroup;
+    static constexpr size_t bytes = 1024 + kBars + 8 * (5 + 2 * G);
+};
+
+template <int KD, int G>
+__global__ void __launch_bounds__(Rev<KD, G>::kWarps * 32) planes_rchain_k(DArgs a, const __grid_constant__ Maps maps) {
+    using Sm = Rev<KD, G>;
+    const int h = blockIdx.y, b = blockIdx.z, hk = h / (a.Hv / a.Hk);
+    const int len = row_length(a, b), nc = (len + kC - 1) / kC;
+    const int warp = threadIdx.x >> 5, vb = blockIdx.x * 16 * G;
+    const Lane L;
+    extern __shared__ __align__(128) unsigned char smem_raw[];
+    unsigned char* smem = align_smem(smem_raw);
+    uint64_t* full = reinterpret_cast<uint64_t*>(smem + Sm::kBars);
+    uint64_t* empty = full + 2;
+    uint64_t* land = empty + 2;
+    uint64_t *z_full = land + 1, *z_empty = z_full + G;
+    const int64_t head = static_cast<int64_t>(b) * a.Hv + h;
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < 2; ++s) {
+            mbar_init(&full[s], 1);
+            mbar_init(&empty[s], G + Sm::H);
+        }
+        mbar_init(land, 1);
+        for (int i = 0; i < 2 * G; ++i) mbar_init(&z_full[i], 1);
+        fence_mbar_init();
+    }
+    __syncthreads();
+    bool ok = true;
+    if (warp == Sm::kWarps - 1) {
+        for (int i = 0; i < nc && ok; ++i) {
+            const int c = nc - 1 - i;
+            bf16* e = reinterpret_cast<bf16*>(smem + (i & 1) * Sm::kStage);
+            const int t0 = c * kC, rows = min(kC, len - t0);
+            const bool tail = rows < min(kC, a.L - t0);
+            uint64_t* bar = tail ? land : &full[i & 1];
+            ok = warp_wait(&empty[i & 1], ((i >> 1) & 1) ^ 1);
+            if (L.l == 0) {
+                const int64_t id = head * a.n + c;
+                mbar_expect_tx(bar, Sm::kLoad);
+#pragma unroll
+                for (int x = 0; x < KD; x += 64) tma_load(e + Sm::kK + x * kC, &maps.k, bar, x, t0, hk, b);
+#pragma unroll
+                for (int g = 0; g < G; ++g) tma_load(e + Sm::kD + g * kC * 16, &maps.d, bar, vb + 16 * g, t0, h, b);
+                bulk_load(e + Sm::kM, static_cast<const bf16*>(a.M) + id * 2 * kCC, 4 * kCC, bar);
+                bulk_load(e + Sm::kGa, a.gates + id * kGates, kGates * 4, bar);
+                bulk_load(e + Sm::kT, static_cast<const bf16*>(a.T) + id * 2 * kCC, 4 * kCC, bar);
+#pragma unroll
+                for (int x = 0; x < KD; x += 64) tma_load(e + Sm::kQ + x * kC, &maps.q, bar, x, t0, hk, b);
+            }
+            __syncwarp();
+            if (tail) {
+                ok = warp_wait(land, 0) && ok;
+                zero_rows<64>(e + Sm::kK, 2 * (KD / 64), rows);
+                zero_rows<16>(e + Sm::kD, G, rows);
+                fence_async();  // later chunks are copied over these rows
+                warp_arrive(&full[i & 1]);
+            }
+        }
+        return;
+    }
+    if (warp < G) {
+        const int v0 = vb + warp * 16;
+        const bool on = v0 < a.Vp;
+        unsigned char* mine = smem + 2 * Sm::kStage + warp * Sm::kGroup;
+        bf16 *sS = reinterpret_cast<bf16*>(mine + Sm::kS), *sX = reinterpret_cast<bf16*>(mine + Sm::kX);
+        const float4* sZ = reinterpret_cast<const float4*>(mine + Sm::kZ);
+        float S[KD / 8][4];  // dS^T
+        state_load<KD>(S, a.dfinal ? a.dfinal + head * a.K * a.V : nullptr, a.K, a.V, v0, L);
+        for (int i = 0; i < nc && ok; ++i) {
+            const int c = nc - 1 - i;
+            const bf16* e = reinterpret_cast<const bf16*>(smem + (i & 1) * Sm::kStage);
+            const float* ga = reinterpret_cast<const float*>(e + Sm::kGa);
+            const float *gam = ga + 2 * kC, *dec = ga + 3 * kC;
+            const int64_t id = head * a.n + c;
+            ok = warp_wait(&full[i & 1], (i >> 1) & 1);
+            if (on) {
+                if (L.l == 0) bulk_wait_read();  // the last chunk's copies have left the tiles
+                __syncwarp();
+                float U[kC / 8][4] = {};  // dU^T = d (K dS1)^T + dO^T M
+                steps<KD / 16>(
+                    [&](int k, uint32_t(*f)[4]) {
+#pragma unroll
+                        for (int p = 0; p < 4; ++p) ld_b128<false>(f[p], e + Sm::kK, 16 * p, 16 * k);
+                    },
+                    [&](int k, const uint32_t(*f)[4]) {
+                        const Af<2> af = from_acc<2>(S[2 * k], S[2 * k + 1]);
+                        st_tile(sS, Sm::LDK, 16 * k, af.r[0]);
+                        st_tile(sS + 16 * Sm::LDK, Sm::LDK, 16 * k, af.r[1]);
+                        mma_step(U, af, f);
+                    });
+                fence_async();
+                __syncwarp();
+                if (L.l == 0) {
+                    bf16* to = static_cast<bf16*>(a.dS) + (id * 2 * a.Vp + v0) * Sm::LDK;
+                    bulk_store(to, sS, 32 * Sm::LDK);
+                    bulk_store(to + static_cast<int64_t>(a.Vp) * Sm::LDK, sS + 16 * Sm::LDK, 32 * Sm::LDK);
+                    bulk_commit();
+                }
+#pragma unroll
+                for (int j = 0; j < kC / 8; ++j) {
+                    const float2 f = *reinterpret_cast<const float2*>(dec + 8 * j + 2 * L.t);
+                    U[j][0] *= f.x;
+                    U[j][1] *= f.y;
+                    U[j][2] *= f.x;
+                    U[j][3] *= f.y;
+                }
+                {
+                    Af<1> ad[2];
+                    steps<8>(
+                        [&](int k, uint32_t(*f)[4]) {
+                            if (!(k & 1)) ld_at32(ad[(k / 2) & 1].r[0], e + Sm::kD + warp * kC * 16, 8 * k);
+#pragma unroll
+                            for (int p = 0; p < 4; ++p)
+                                if (p <= k / 2) ld_b<true>(f[p], e + Sm::kM + (k & 1 ? 0 : kCC), kTld, 16 * p, 16 * (k / 2));
+                        },
+                        [&](int k, const uint32_t(*f)[4]) { mma_step(U, ad[(k / 2) & 1], f, 0, k / 2 + 1); });
+                }
+                float X[kC / 8][4] = {};  // dV^T = dU^T T'
+                {
+                    Af<2> af;
+                    steps<8>(
+                        [&](int k, uint32_t(*f)[4]) {
+#pragma unroll
+                            for (int p = 0; p < 4; ++p)
+                                if (p <= k / 2) ld_b<true>(f[p], e + Sm::kT + (k & 1 ? 0 : kCC), kTld, 16 * p, 16 * (k / 2));
+                        },
+                        [&](int k, const uint32_t(*f)[4]) {
+                            if (k & 1) {
+                                mma_step(X, af, f, 0, k / 2 + 1);
+                            } else {
+                                af = from_acc<2>(U[k], U[k + 1]);
+                                mma_step(X, Af<1>{{{af.r[0][0], af.r[0][1], af.r[0][2], af.r[0][3]}}}, f, 0, k / 2 + 1);
+                            }
+                        });
+                }
+                // dS^T = gam_63 dS^T + (scale gam dO)^T Q - (gam dV)^T K
+                ok = warp_wait(&z_full[warp], i & 1) && ok;
+                const float gc = gam[kC - 1];
+#pragma unroll
+                for (int j = 0; j < KD / 8; ++j) {
+                    const float4 z = sZ[j * 32 + L.l];
+                    S[j][0] = fmaf(gc, S[j][0], z.x);
+                    S[j][1] = fmaf(gc, S[j][1], z.y);
+                    S[j][2] = fmaf(gc, S[j][2], z.z);
+                    S[j][3] = fmaf(gc, S[j][3], z.w);
+                }
+                warp_arrive(&z_empty[warp]);
+                {
+                    Af<1> af;
+                    constexpr int Q = KD / 64;
+                    steps<4 * Q>(
+                        [&](int k, uint32_t(*f)[4]) {
+#pragma unroll
+                            for (int p = 0; p < 4; ++p) ld_b128<true>(f[p], e + Sm::kK, 64 * (k % Q) + 16 * p, 16 * (k / Q));
+                        },
+                        [&](int k, const uint32_t(*f)[4]) {
+                            const int kk = k / Q;
+                            if (k % Q == 0) {
+                                const Af<2> ax = from_acc<2>(X[2 * kk], X[2 * kk + 1]);
+                                st_tile(sX, kTld, 16 * kk, ax.r[0]);
+                                st_tile(sX + 16 * kTld, kTld, 16 * kk, ax.r[1]);
+                                float y[2][4];
+#pragma unroll
+                                for (int x = 0; x < 2; ++x) {
+                                    const float2 d = *reinterpret_cast<const float2*>(gam + 16 * kk + 8 * x + 2 * L.t);
+                                    const float* u = X[2 * kk + x];
+                                    y[x][0] = -u[0] * d.x;
+                                    y[x][1] = -u[1] * d.y;
+                                    y[x][2] = -u[2] * d.x;
+                                    y[x][3] = -u[3] * d.y;
+                                }
+                                af = from_acc<1>(y[0], y[1]);
+                            }
+                            mma_step(S + 8 * (k % Q), af, f);
+                        });
+                }
+                fence_async();
+                __syncwarp();
+                if (L.l == 0) {
+                    bf16* to = static_cast<bf16*>(a.dV) + (id * 2 * a.Vp + v0) * kTld;
+                    bulk_store(to, sX, 32 * kTld);
+                    bulk_store(to + static_cast<int64_t>(a.Vp) * kTld, sX + 16 * kTld, 32 * kTld);
+                    bulk_commit();
+                }
+            }
+            warp_arrive(&empty[i & 1]);
+        }
+        if (on && a.dinitial && ok) state_store<KD>(S, a.dinitial + head * a.K * a.V, a.K, a.V, v0, L);
+        if (L.l == 0) bulk_wait_all();
+        return;
+    }
+    // ---- (scale gam dO)^T Q of the groups ----
+    for (int i = 0; i < nc && ok; ++i) {
+        const bf16* e = reinterpret_cast<const bf16*>(smem + (i & 1) * Sm::kStage);
+        const float* sgam = reinterpret_cast<const float*>(e + Sm::kGa) + 4 * kC;
+        ok = warp_wait(&full[i & 1], (i >> 1) & 1);
+        for (int g = warp - G; g < G; g += Sm::H) {
+            if (vb + 16 * g >= a.Vp) break;
+            float Z[KD / 8][4] = {};
+            Af<2> af;
+            constexpr int Q = KD / 64;
+            steps<4 * Q>(
+                [&](int k, uint32_t(*f)[4]) {
+#pragma unroll
+                    for (int p = 0; p < 4; ++p) ld_b128<true>(f[p], e + Sm::kQ, 64 * (k % Q) + 16 * p, 16 * (k / Q));
+                },
+                [&](int k, const uint32_t(*f)[4]) {
+                    const int kk = k / Q;
+                    if (k % Q == 0) {
+                        uint32_t r[4];
+                        ld_at32(r, e + Sm::kD + g * kC * 16, 16 * kk);
+                        float y[2][4];
+#pragma unroll
+                        for (int x = 0; x < 2; ++x) {
+                            const float2 d = *reinterpret_cast<const float2*>(sgam + 16 * kk + 8 * x + 2 * L.t);
+                            const float2 lo = unpack_bf16(r[2 * x]), hi = unpack_bf16(r[2 * x + 1]);
+                            y[x][0] = lo.x * d.x;
+                            y[x][1] = lo.y * d.y;
+                            y[x][2] = hi.x * d.x;
+                            y[x][3] = hi.y * d.y;
+                        }
+                        af = from_acc<2>(y[0], y[1]);
+                    }
+                    mma_step(Z + 8 * (k % Q), af, f);
+                });
+            float4* sZ = reinterpret_cast<float4*>(smem + 2 * Sm::kStage + g * Sm::kGroup + Sm::kZ);
+            ok = warp_wait(&z_empty[g], (i & 1) ^ 1) && ok;
+#pragma unroll
+            for (int j = 0; j < KD / 8; ++j) sZ[j * 32 + L.l] = make_float4(Z[j][0], Z[j][1], Z[j][2], Z[j][3]);
+            warp_arrive(&z_full[g]);
+        }
+        warp_arrive(&empty[i & 1]);
+    }
+}
+
+// ----------------------------------------------------------------------------
+// dQ, dK, dV, dbeta and dg of a chunk
+// ----------------------------------------------------------------------------
+// A CTA goes through chunks (of a key head) in a grid-stride loop: a warp loads
+// ahead of eight that compute, 4 groups of 16 rows by 2 halves of the key
+// columns.  The value columns come in tiles of 32, two deep, so that the two
+// states of a chunk (in two planes 139 KB of its 260 KB) never have to be in
+// shared memory whole.  dV, whose rounding does not show in the products, goes
+// in as one plane (the output itself); U, S, dS, N and E as two.
+template <int KD>
+struct Grad {
+    static constexpr int VT = 32, LDK = KD + 8;
+    static constexpr int kD = 0, kU = kD + kC * VT, kX = kU + 2 * VT * kTld, kS = kX + 2 * VT * kTld, kR = kS + 2 * VT * LDK;
+    static constexpr int kGa = kR + 2 * VT * LDK;
+    static constexpr int kStage = up1024(kGa * 2 + kGates * 4);    // bytes
+    static constexpr int kK = 0, kQ = kC * KD, kKQ = 2 * kC * KD * 2;  // (elements, elements, bytes)
+    static constexpr int kN = 2 * kStage + 2 * kKQ;                // N and E, two planes each (bytes)
+    static constexpr int kF = kN + 4 * kCC * 2;                    // floats: beta, row sums, dbeta, totals
+    static constexpr int kBars = kF + (kC + 4 * kC + 16) * 4;
+    static constexpr size_t bytes = 1024 + kBars + 8 * 9;
+};
+
+__device__ __forceinline__ void sync_compute() { asm volatile("bar.sync 1, 256;" ::: "memory"); }
+
+__device__ __forceinline__ void split_store(bf16* s, float x, float y) {  // and its low plane kCC further
+    const uint32_t hi = pack_bf16(x, y);
+    const float2 f = unpack_bf16(hi);
+    *reinterpret_cast<uint32_t*>(s) = hi;
+    *reinterpret_cast<uint32_t*>(s + kCC) = pack_bf16(x - f.x, y - f.y);
+}
+
+// rows m0.. of accumulators to an output of row stride st: zeros from `rows` on, nothing from `all` on
+template <int NT>
+__device__ __forceinline__ void rows_out(const float (*x)[4], bf16* p, int64_t st, int m0, int rows, int all, int c0,
+                                         int cols, const Lane& L) {
+#pragma unroll
+    for (int half = 0; half < 2; ++half) {
+        const int r = m0 + L.g + 8 * half;
+        if (r >= all) continue;
+#pragma unroll
+        for (int j = 0; j < NT; ++j) {
+            const int col = c0 + 8 * j + 2 * L.t;
+            if (col < cols)
+                *reinterpret_cast<uint32_t*>(p + r * st + col) = r < rows ? pack_bf16(x[j][2 * half], x[j][2 * half + 1]) : 0u;
+        }
+    }
+}
+
+template <int KD>
+__global__ void __launch_bounds__(288) planes_grad_k(DArgs a, float* group, const __grid_constant__ Maps maps) {
+    using Sm = Grad<KD>;
+    constexpr int VT = Sm::VT, NT = KD / 16;
+    extern __shared__ __align__(128) unsigned char smem_raw[];
+    unsigned char* smem = align_smem(smem_raw);
+    uint64_t* full = reinterpret_cast<uint64_t*>(smem + Sm::kBars);
+    uint64_t *empty = full + 2, *qfull = full + 4, *qempty = full + 6, *land = full + 8;
+    const int tid = threadIdx.x, warp = tid >> 5, rep = a.Hv / a.Hk;
+    const Lane L;
+    if (tid == 0) {
+        for (int s = 0; s < 2; ++s) {
+            mbar_init(&full[s], 1);
+            mbar_init(&empty[s], 8);
+            mbar_init(&qfull[s], 1);
+            mbar_init(&qempty[s], 8);
+        }
+        mbar_init(land, 1);
+        fence_mbar_init();
+    }
+    __syncthreads();
+    const int64_t items = static_cast<int64_t>(a.B) * a.Hk * a.n;
+    bool ok = true;
+    int tile = 0, seen = 0;  // tiles and chunks so far
+    if (warp == 8) {
+        int landed = 0;
+        for (int64_t it = blockIdx.x; it < items && ok; it += gridDim.x) {
+            const int c = static_cast<int>(it % a.n), hk = static_cast<int>(it / a.n % a.Hk);
+            const int b = static_cast<int>(it / a.n / a.Hk);
+            const int t0 = c * kC, rows = min(kC, row_length(a, b) - t0);
+            if (rows <= 0) continue;
+            const bool tail = rows < min(kC, a.L - t0);
+            {
+                bf16* e = reinterpret_cast<bf16*>(smem + 2 * Sm::kStage + (seen & 1) * Sm::kKQ);
+                uint64_t* bar = tail ? land : &qfull[seen & 1];
+                ok = warp_wait(&qempty[seen & 1], ((seen >> 1) & 1) ^ 1);
+                if (L.l == 0) {
+                    mbar_expect_tx(bar, Sm::kKQ);
+#pragma unroll
+                    for (int x = 0; x < KD; x += 64) {
+                        tma_load(e + Sm::kK + x * kC, &maps.k, bar, x, t0, hk, b);
+                        tma_load(e + Sm::kQ + x * kC, &maps.q, bar, x, t0, hk, b);
+                    }
+                }
+                __syncwarp();
+                if (tail) {
+                    ok = warp_wait(land, landed++ & 1) && ok;
+                    zero_rows<64>(e + Sm::kK, 2 * (KD / 64), rows);
+                    fence_async();
+                    warp_arrive(&qfull[seen & 1]);
+                }
+                ++seen;
+            }
+            for (int h = hk * rep; h < (hk + 1) * rep; ++h) {
+                const int64_t id = (static_cast<int64_t>(b) * a.Hv + h) * a.n + c;
+                for (int v0 = 0; v0 < a.Vp && ok; v0 += VT, ++tile) {
+                    const int vn = min(VT, a.Vp - v0);
+                    bf16* e = reinterpret_cast<bf16*>(smem + (tile & 1) * Sm::kStage);
+                    uint64_t* bar = tail ? land : &full[tile & 1];
+                    ok = warp_wait(&empty[tile & 1], ((tile >> 1) & 1) ^ 1);
+                    if (L.l == 0) {
+                        mbar_expect_tx(bar, vn * (kC + 4 * kTld + 4 * Sm::LDK) * 2 + kGates * 4);
+                        for (int v = 0; v < vn; v += 16) tma_load(e + Sm::kD + v * kC, &maps.d, bar, v0 + v, t0, h, b);
+                        const bf16* U = static_cast<const bf16*>(a.U) + (id * 2 * a.Vp + v0) * kTld;
+                        const bf16* X = static_cast<const bf16*>(a.dV) + (id * 2 * a.Vp + v0) * kTld;
+                        const bf16* S = static_cast<const bf16*>(a.S) + (id * 2 * a.Vp + v0) * Sm::LDK;
+                        const bf16* R = static_cast<const bf16*>(a.dS) + (id * 2 * a.Vp + v0) * Sm::LDK;
+                        for (int p = 0; p < 2; ++p) {
+                            bulk_load(e + Sm::kS + p * VT * Sm::LDK, S + static_cast<int64_t>(p) * a.Vp * Sm::LDK,
+                                      vn * Sm::LDK * 2, bar);
+                            bulk_load(e + Sm::kR + p * VT * Sm::LDK, R + static_cast<int64_t>(p) * a.Vp * Sm::LDK,
+                                      vn * Sm::LDK * 2, bar);
+                            bulk_load(e + Sm::kU + p * VT * kTld, U + static_cast<int64_t>(p) * a.Vp * kTld, vn * kTld * 2,
+                                      bar);
+                            bulk_load(e + Sm::kX + p * VT * kTld, X + static_cast<int64_t>(p) * a.Vp * kTld, vn * kTld * 2,
+                                      bar);
+                        }
+                        bulk_load(e + Sm::kGa, a.gates + id * kGates, kGates * 4, bar);
+                    }
+                    __syncwarp();
+                    if (tail) {
+                        ok = warp_wait(land, landed++ & 1) && ok;
+                        zero_rows<16>(e + Sm::kD, vn / 16, rows);
+                        fence_async();
+                        warp_arrive(&full[tile & 1]);
+                    }
+                }
+            }
+        }
+        return;
+    }
+    const int rg = warp & 3, half = warp >> 2, m0 = rg * 16, n0 = half * (KD / 2);
+    const int r0 = m0 + L.g, r1 = r0 + 8;
+    bf16* sN = reinterpret_cast<bf16*>(smem + Sm::kN);
+    bf16* sE = sN + 2 * kCC;
+    float* sDot = reinterpret_cast<float*>(smem + Sm::kF);  // [2][64]
+    float* sDb = sDot + 2 * kC;                             // [2][64]
+    float* sTot = sDb + 2 * kC;                             // [8], [8]
+    for (int64_t it = blockIdx.x; it < items && ok; it += gridDim.x) {
+        const int c = static_cast<int>(it % a.n), hk = static_cast<int>(it / a.n % a.Hk);
+        const int b = static_cast<int>(it / a.n / a.Hk);
+        const int rows = min(kC, row_length(a, b) - c * kC), all = min(kC, a.L - c * kC);
+        const int64_t t0 = static_cast<int64_t>(c) * kC, row0 = static_cast<int64_t>(b) * a.L + t0;
+        const int64_t qst = static_cast<int64_t>(a.Hk) * a.K, vst = static_cast<int64_t>(a.Hv) * a.V;
+        bf16* dq = static_cast<bf16*>(a.dq) + row0 * qst + static_cast<int64_t>(hk) * a.K;
+        bf16* dk = static_cast<bf16*>(a.dk) + row0 * qst + static_cast<int64_t>(hk) * a.K;
+        if (rows <= 0) {  // behind the sequence
+            const uint4 z = make_uint4(0, 0, 0, 0);
+            for (int i = tid; i < all * (a.K / 8); i += 256) {
+                const int64_t o = i / (a.K / 8) * qst + i % (a.K / 8) * 8;
+                *reinterpret_cast<uint4*>(dq + o) = z;
+                *reinterpret_cast<uint4*>(dk + o) = z;
+            }
+            for (int h = hk * rep; h < (hk + 1) * rep; ++h) {
+                bf16* dv = static_cast<bf16*>(a.dv) + row0 * vst + static_cast<int64_t>(h) * a.V;
+                for (int i = tid; i < all * (a.V / 8); i += 256)
+                    *reinterpret_cast<uint4*>(dv + i / (a.V / 8) * vst + i % (a.V / 8) * 8) = z;
+                for (int i = tid; i < all; i += 256) {
+                    gate_store(a.dg, a.gate_dtype, (row0 + i) * a.Hv + h, 0.f);
+                    gate_store(a.dbeta, a.gate_dtype, (row0 + i) * a.Hv + h, 0.f);
+                }
+            }
+            continue;
+        }
+        const bf16* kq = reinterpret_cast<const bf16*>(smem + 2 * Sm::kStage + (seen & 1) * Sm::kKQ);
+        const bf16 *sK = kq + Sm::kK, *sQ = kq + Sm::kQ;
+        ok = warp_wait(&qfull[seen & 1], (seen >> 1) & 1);
+        for (int h = hk * rep; h < (hk + 1) * rep; ++h) {
+            bf16* dv = static_cast<bf16*>(a.dv) + row0 * vst + static_cast<int64_t>(h) * a.V;
+            float ib[2];
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                const int r = r0 + 8 * i;
+                ib[i] = r < rows ? 1.f / hold_beta(gate_value(a.beta, a.gate_dtype, b * a.sb.b + (t0 + r) * a.sb.t + h * a.sb.h))
+                                 : 0.f;
+            }
+            float P[kC / 8][4] = {};  // half 0: dO U^T, half 1: dV U^T
+            float aq[NT][4] = {}, ar[NT][4] = {}, aw[NT][4] = {};
+            float db0 = 0.f, db1 = 0.f, sd = 0.f;
+            float gm[2], gd[2], gc = 0.f;
+            for (int v0 = 0; v0 < a.Vp; v0 += VT, ++tile) {
+                const int vn = min(VT, a.Vp - v0);
+                const bf16* e = reinterpret_cast<const bf16*>(smem + (tile & 1) * Sm::kStage);
+                ok = warp_wait(&full[tile & 1], (tile >> 1) & 1) && ok;
+#pragma unroll
+                for (int kk = 0; kk < VT / 16; ++kk) {
+                    if (16 * kk >= vn) break;
+                    Af<1> fd, fx;
+                    Af<2> fu;
+                    ld_a32(fd.r[0], e + Sm::kD + kk * kC * 16, m0);
+                    ld_at(fx.r[0], e + Sm::kX, kTld, m0, 16 * kk);
+                    ld_at(fu.r[0], e + Sm::kU, kTld, m0, 16 * kk);
+                    ld_at(fu.r[1], e + Sm::kU + VT * kTld, kTld, m0, 16 * kk);
+                    const Af<1>& left = half ? fx : fd;
+                    constexpr int NP = NT / 2;
+                    steps<6, false>(  // (two warps a scheduler, and no registers to read ahead)
+                        [&](int i, uint32_t(*f)[4]) {
+                            const bf16* s = e + (i < 2 ? Sm::kU + (i & 1) * VT * kTld
+                                                       : (i < 4 ? Sm::kS : Sm::kR) + (i & 1) * VT * Sm::LDK);
+#pragma unroll
+                            for (int p = 0; p < 4; ++p) {
+                                if (i < 2) {
+                                    if (p <= rg) ld_b<true>(f[p], s, kTld, 16 * p, 16 * kk);
+                                } else if (p < NP) {
+                                    ld_b<true>(f[p], s, Sm::LDK, n0 + 16 * p, 16 * kk);
+                                }
+                            }
+                        },
+                        [&](int i, const uint32_t(*f)[4]) {
+                            if (i < 2) {  // dO U^T or dV U^T
+#pragma unroll
+                                for (int p = 0; p < 4; ++p)
+                                    if (p <= rg) mma_pair(P[2 * p], P[2 * p + 1], left.r[0], f[p]);
+                            } else if (i < 4) {  // dO S0^T, dV S0^T
+#pragma unroll
+                                for (int p = 0; p < NP; ++p) mma_pair(aq[2 * p], aq[2 * p + 1], fd.r[0], f[p]);
+#pragma unroll
+                                for (int p = 0; p < NP; ++p) mma_pair(ar[2 * p], ar[2 * p + 1], fx.r[0], f[p]);
+                            } else {  // U dS1^T
+                                if (i == 4) mma_step(aw, fu, f, 0, NP);
+                                else mma_step(aw, Af<1>{{{fu.r[0][0], fu.r[0][1], fu.r[0][2], fu.r[0][3]}}}, f, 0, NP);
+                            }
+                        });
+                    if ((kk & 1) == half) {  // dbeta and dv: columns dealt to the halves
+                        uint32_t xl[4];
+                        ld_at(xl, e + Sm::kX + VT * kTld, kTld, m0, 16 * kk);
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            const float2 x = unpack_bf16(fx.r[0][i]), xw = unpack_bf16(xl[i]), u = unpack_bf16(fu.r[0][i]), w = unpack_bf16(fu.r[1][i]);
+                            const float f = ib[i & 1];
+                            float& db = i & 1 ? db1 : db0;
+                            db = fmaf((x.x + xw.x) * f, (u.x + w.x) * f, db);
+                            db = fmaf((x.y + xw.y) * f, (u.y + w.y) * f, db);
+                            const int r = r0 + (i & 1) * 8, col = v0 + 16 * kk + (i >> 1) * 8 + 2 * L.t;
+                            if (r < all && col < a.V)
+                                *reinterpret_cast<uint32_t*>(dv + r * vst + col) = r < rows ? fx.r[0][i] : 0u;
+                        }
+                    }
+                }
+                for (int i = tid; i < vn * (KD / 8); i += 256) {  // <S0, dS1>
+                    const int o = i / (KD / 8) * Sm::LDK + i % (KD / 8) * 8;
+                    const uint4 sh = *reinterpret_cast<const uint4*>(e + Sm::kS + o);
+                    const uint4 sl = *reinterpret_cast<const uint4*>(e + Sm::kS + VT * Sm::LDK + o);
+                    const uint4 rh = *reinterpret_cast<const uint4*>(e + Sm::kR + o);
+                    const uint4 rl = *reinterpret_cast<const uint4*>(e + Sm::kR + VT * Sm::LDK + o);
+                    const uint32_t *s_h = &sh.x, *s_l = &sl.x, *r_h = &rh.x, *r_l = &rl.x;
+#pragma unroll
+                    for (int w = 0; w < 4; ++w) {
+                        const float2 x = unpack_bf16(s_h[w]), y = unpack_bf16(s_l[w]), u = unpack_bf16(r_h[w]), z = unpack_bf16(r_l[w]);
+                        sd = fmaf(x.x + y.x, u.x + z.x, sd);
+                        sd = fmaf(x.y + y.y, u.y + z.y, sd);
+                    }
+                }
+                if (v0 + VT >= a.Vp) {  // the gates, and N and E, before the tile is given back
+                    const float* ga = reinterpret_cast<const float*>(e + Sm::kGa);
+                    gm[0] = ga[2 * kC + r0];
+                    gm[1] = ga[2 * kC + r1];
+                    gd[0] = ga[3 * kC + r0];
+                    gd[1] = ga[3 * kC + r1];
+                    gc = ga[2 * kC + kC - 1];
+                    bf16* o = half ? sE : sN;
+                    const float f = half ? -1.f : a.scale;
+#pragma unroll
+                    for (int j = 0; j < kC / 8; ++j) {
+                        if (j > 2 * rg + 1) break;
+#pragma unroll
+                        for (int i = 0; i < 2; ++i) {
+                            const int r = i ? r1 : r0, col = 8 * j + 2 * L.t;
+                            const int last = half ? r - 1 : r;  // N with the diagonal, E without
+                            split_store(o + r * kTld + col, col <= last ? f * ratio(ga, r, col) * P[j][2 * i] : 0.f,
+                                        col + 1 <= last ? f * ratio(ga, r, col + 1) * P[j][2 * i + 1] : 0.f);
+                        }
+                    }
+                }
+                warp_arrive(&empty[tile & 1]);
+            }
+#pragma unroll
+            for (int o = 1; o < 4; o <<= 1) {
+                db0 += __shfl_xor_sync(0xffffffffu, db0, o);
+                db1 += __shfl_xor_sync(0xffffffffu, db1, o);
+            }
+            sd = warp_sum(sd);
+            float tw = 0.f;
+#pragma unroll
+            for (int j = 0; j < NT; ++j) {
+                const int col = n0 + 8 * j + 2 * L.t;
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    const float2 kv = unpack_bf16(*reinterpret_cast<const uint32_t*>(sK + at128(i ? r1 : r0, col)));
+#pragma unroll
+                    for (int x = 0; x < 2; ++x) {
+                        aq[j][2 * i + x] *= a.scale * gm[i];
+                        ar[j][2 * i + x] *= -gm[i];
+                        aw[j][2 * i + x] *= gd[i];
+                    }
+                    tw = fmaf(kv.x, aw[j][2 * i], tw);
+                    tw = fmaf(kv.y, aw[j][2 * i + 1], tw);
+                }
+            }
+            tw = warp_sum(tw);
+            if (L.t == 0) {
+                sDb[half * kC + r0] = db0;
+                sDb[half * kC + r1] = db1;
+            }
+            if (L.l == 0) {
+                sTot[warp] = sd;
+                sTot[8 + warp] = tw;
+            }
+            sync_compute();  // N, E
+#pragma unroll
+            for (int kk = 0; kk < kC / 16; ++kk) {
+                if (kk <= rg) {  // rows of N and E
+                    Af<2> fn, fe;
+#pragma unroll
+                    for (int p = 0; p < 2; ++p) {
+                        ld_a(fn.r[p], sN + p * kCC, kTld, m0, 16 * kk);
+                        ld_a(fe.r[p], sE + p * kCC, kTld, m0, 16 * kk);
+                    }
+#pragma unroll
+                    for (int p = 0; p < NT / 2; ++p) {
+                        uint32_t bk[4];
+                        ld_b128<true>(bk, sK, n0 + 16 * p, 16 * kk);
+                        mma_pair(aq[2 * p], aq[2 * p + 1], fn.r[1], bk);
+                        mma_pair(ar[2 * p], ar[2 * p + 1], fe.r[1], bk);
+                        mma_pair(aq[2 * p], aq[2 * p + 1], fn.r[0], bk);
+                        mma_pair(ar[2 * p], ar[2 * p + 1], fe.r[0], bk);
+                    }
+                }
+                if (kk >= rg) {  // columns of N and E
+                    Af<2> fn, fe;
+#pragma unroll
+                    for (int p = 0; p < 2; ++p) {
+                        ld_at(fn.r[p], sN + p * kCC, kTld, m0, 16 * kk);
+                        ld_at(fe.r[p], sE + p * kCC, kTld, m0, 16 * kk);
+                    }
+#pragma unroll
+                    for (int p = 0; p < NT / 2; ++p) {
+                        mm128<2, true>(aw[2 * p], aw[2 * p + 1], fn, sQ, n0 + 16 * p, 16 * kk);
+                        mm128<2, true>(aw[2 * p], aw[2 * p + 1], fe, sK, n0 + 16 * p, 16 * kk);
+                    }
+                }
+            }
+            float dot[2] = {};
+#pragma unroll
+            for (int j = 0; j < NT; ++j) {
+                const int col = n0 + 8 * j + 2 * L.t;
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    const int o = at128(i ? r1 : r0, col);
+                    const float2 qv = unpack_bf16(*reinterpret_cast<const uint32_t*>(sQ + o));
+                    const float2 kv = unpack_bf16(*reinterpret_cast<const uint32_t*>(sK + o));
+                    dot[i] = fmaf(qv.x, aq[j][2 * i], dot[i]);
+                    dot[i] = fmaf(qv.y, aq[j][2 * i + 1], dot[i]);
+                    dot[i] = fmaf(kv.x, ar[j][2 * i] - aw[j][2 * i], dot[i]);
+                    dot[i] = fmaf(kv.y, ar[j][2 * i + 1] - aw[j][2 * i + 1], dot[i]);
+                    ar[j][2 * i] += aw[j][2 * i];  // dK
+                    ar[j][2 * i + 1] += aw[j][2 * i + 1];
+                }
+            }
+#pragma unroll
+            for (int o = 1; o < 4; o <<= 1) {
+                dot[0] += __shfl_xor_sync(0xffffffffu, dot[0], o);
+                dot[1] += __shfl_xor_sync(0xffffffffu, dot[1], o);
+            }
+            if (L.t == 0) {
+                sDot[half * kC + r0] = dot[0];
+                sDot[half * kC + r1] = dot[1];
+            }
+            if (rep > 1) {  // the sum over the value heads of this key head; each thread its own elements
+                float* gq = group + ((static_cast<int64_t>(b) * a.Hk + hk) * a.n + c) * 2 * kC * KD;
+                float* gk = gq + kC * KD;
+#pragma unroll
+                for (int j = 0; j < NT; ++j)
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) {
+                        const int o = (i ? r1 : r0) * KD + n0 + 8 * j + 2 * L.t;
+                        float2 x = make_float2(aq[j][2 * i], aq[j][2 * i + 1]), y = make_float2(ar[j][2 * i], ar[j][2 * i + 1]);
+                        if (h > hk * rep) {
+                            const float2 p = *reinterpret_cast<const float2*>(gq + o), q = *reinterpret_cast<const float2*>(gk + o);
+                            x.x += p.x; x.y += p.y; y.x += q.x; y.y += q.y;
+                        }
+                        *reinterpret_cast<float2*>(gq + o) = x;
+                        *reinterpret_cast<float2*>(gk + o) = y;
+                        aq[j][2 * i] = x.x; aq[j][2 * i + 1] = x.y;
+                        ar[j][2 * i] = y.x; ar[j][2 * i + 1] = y.y;
+                    }
+            }
+            if (h == (hk + 1) * rep - 1) {
+                rows_out<NT>(aq, dq, qst, m0, rows, all, n0, a.K, L);
+                rows_out<NT>(ar, dk, qst, m0, rows, all, n0, a.K, L);
+            }
+            sync_compute();
+            if (warp == 0) {
+                float tot = 0.f, w = 0.f;
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    tot += sTot[i];
+                    w += sTot[8 + i];
+                }
+                tot = fmaf(gc, tot, w);  // <S1, dS1>
+                const int i0 = 2 * L.l;
+                const float y1 = sDot[i0 + 1] + sDot[kC + i0 + 1];
+                const float y0 = sDot[i0] + sDot[kC + i0] + y1;
+                float run = y0;  // sums from here to the end
+#pragma unroll
+                for (int o = 1; o < 32; o <<= 1) {
+                    const float dn = __shfl_down_sync(0xffffffffu, run, o);
+                    if (L.l + o < 32) run += dn;
+                }
+                const float behind = run - y0 + tot;
+                const int64_t o = (row0 + i0) * a.Hv + h;
+                if (i0 < all) {
+                    gate_store(a.dg, a.gate_dtype, o, i0 < rows ? y0 + behind : 0.f);
+                    gate_store(a.dbeta, a.gate_dtype, o, i0 < rows ? sDb[i0] + sDb[kC + i0] : 0.f);
+                }
+                if (i0 + 1 < all) {
+                    gate_store(a.dg, a.gate_dtype, o + a.Hv, i0 + 1 < rows ? y1 + behind : 0.f);
+                    gate_store(a.dbeta, a.gate_dtype, o + a.Hv, i0 + 1 < rows ? sDb[i0 + 1] + sDb[kC + i0 + 1] : 0.f);
+                }
+            }
+            sync_compute();  // the sums and N, E are free again
+        }
+        warp_arrive(&qempty[seen & 1]);
+        ++seen;
+    }
+}
+
+// ----------------------------------------------------------------------------
+// launches
+// ----------------------------------------------------------------------------
+template <typename K>
+cudaError_t smem_limit(K kernel, size_t bytes) {
+    return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(bytes));
+}
+
+#define PLANES_TRY(x)                         \
+    do {                                      \
+        const cudaError_t e_ = (x);           \
+        if (e_ != cudaSuccess) return e_;     \
+    } while (0)
+
+constexpr int kSms = 148;
+
+// Groups of 16 value columns per CTA of a chain, one CTA on an SM at a time:
+// the fewest rounds of CTAs, weighed with the products that a chunk's busiest
+// scheduler has to do.  (Four groups do not fit the reverse chain's tiles.)
+int chain_groups(const DArgs& a, bool reverse) {
+    const int64_t heads = static_cast<int64_t>(a.B) * a.Hv, groups = a.Vp / 16;
+    auto cost = [&](int64_t g, int64_t per) { return (heads * ((groups + g - 1) / g) + kSms - 1) / kSms * per; };
+    const int64_t x2 = cost(2, reverse ? 292 : 316), x3 = cost(3, reverse ? 384 : 372), x4 = cost(4, 440);
+    if (reverse) return x2 <= x3 ? 2 : 3;
+    return x2 <= x3 && x2 <= x4 ? 2 : x3 <= x4 ? 3 : 4;
+}
+
+template <int KD, int G>
+cudaError_t chain_launch(const DArgs& a, const Maps& m, cudaStream_t s) {
+    PLANES_TRY(smem_limit(planes_chain_k<KD, G>, Fwd<KD, G>::bytes));
+    planes_chain_k<KD, G><<<dim3((a.Vp / 16 + G - 1) / G, a.Hv, a.B), Fwd<KD, G>::kWarps * 32, Fwd<KD, G>::bytes, s>>>(a, m);
+    note_launch();
+    return cudaGetLastError();
+}
+template <int KD, int G>
+cudaError_t rchain_launch(const DArgs& a, const Maps& m, cudaStream_t s) {
+    PLANES_TRY(smem_limit(planes_rchain_k<KD, G>, Rev<KD, G>::bytes));
+    planes_rchain_k<KD, G><<<dim3((a.Vp / 16 + G - 1) / G, a.Hv, a.B), Rev<KD, G>::kWarps * 32, Rev<KD, G>::bytes, s>>>(a, m);
+    note_launch();
+    return cudaGetLastError();
+}
+
+template <int KD>
+cudaError_t chain(const DArgs& a, const Maps& m, bool reverse, cudaStream_t s) {
+    const int g = chain_groups(a, reverse);
+    if (reverse) return g == 2 ? rchain_launch<KD, 2>(a, m, s) : rchain_launch<KD, 3>(a, m, s);
+    return g == 2 ? chain_launch<KD, 2>(a, m, s) : g == 3 ? chain_launch<KD, 3>(a, m, s) : chain_launch<KD, 4>(a, m, s);
+}
+
+PFN_cuTensorMapEncodeTiled_v12000 encode_fn() {
+    static PFN_cuTensorMapEncodeTiled_v12000 fn = nullptr;
+    static std::once_flag once;
+    std::call_once(once, [] {
+        void* p = nullptr;
+        cudaDriverEntryPointQueryResult q;
+        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) == cudaSuccess &&
+            q == cudaDriverEntryPointSuccess)
+            fn = reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(p);
+    });
+    return fn;
+}
+
+// Boxes of 64 tokens by 64 columns (128-byte swizzle) or by 16 (32-byte).  A
+// dimension of one element has no stride of its own: any multiple of 16 does.
+bool make_map(CUtensorMap& m, const void* p, const Str& st, int64_t D, int64_t L, int64_t H, int64_t B, int cols) {
+    auto enc = encode_fn();
+    if (!enc) return false;
+    auto bytes = [](int64_t n, int64_t stride) { return static_cast<cuuint64_t>(n > 1 ? stride * 2 : 16); };
+    const cuuint64_t dims[4] = {static_cast<cuuint64_t>(D), static_cast<cuuint64_t>(L), static_cast<cuuint64_t>(H),
+                                static_cast<cuuint64_t>(B)};
+    const cuuint64_t strides[3] = {bytes(L, st.t), bytes(H, st.h), bytes(B, st.b)};
+    const cuuint32_t box[4] = {static_cast<cuuint32_t>(cols), kC, 1, 1}, unit[4] = {1, 1, 1, 1};
+    return enc(&m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, const_cast<void*>(p), dims, strides, box, unit,
+               CU_TENSOR_MAP_INTERLEAVE_NONE, cols == 64 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_32B,
+               CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+bool make_maps(const DArgs& a, Maps& m) {
+    return make_map(m.q, a.q, a.sq, a.K, a.L, a.Hk, a.B, 64) && make_map(m.k, a.k, a.sk, a.K, a.L, a.Hk, a.B, 64) &&
+           make_map(m.v, a.v, a.sv, a.V, a.L, a.Hv, a.B, 16) &&
+           (!a.dout || make_map(m.d, a.dout, a.sdo, a.V, a.L, a.Hv, a.B, 16));
+}
+
+template <int KD>
+cudaError_t fwd(const DArgs& a, cudaStream_t s) {
+    const size_t prep = 2 * kC * (KD + 8) * sizeof(bf16) + 2 * kC * kAld * sizeof(float);
+    PLANES_TRY(smem_limit(planes_prep_k<KD>, prep));
+    planes_prep_k<KD><<<dim3(a.n, a.Hv, a.B), 128, prep, s>>>(a);
+    note_launch();
+    PLANES_TRY(cudaGetLastError());
+    Maps m{};
+    if (!make_maps(a, m)) return cudaErrorInvalidValue;
+    return chain<KD>(a, m, false, s);
+}
+
+template <int KD>
+cudaError_t bwd(const DArgs& a, float* group, cudaStream_t s) {
+    // a runtime call first: tensor maps are not made in a thread (autograd's, say) that
+    // has not met its device yet
+    PLANES_TRY(smem_limit(planes_grad_k<KD>, Grad<KD>::bytes));
+    Maps m{};
+    if (!make_maps(a, m)) return cudaErrorInvalidValue;
+    PLANES_TRY(chain<KD>(a, m, true, s));
+    const int64_t items = static_cast<int64_t>(a.B) * a.Hk * a.n;
+    planes_grad_k<KD><<<static_cast<unsigned>(items < kSms ? items : kSms), 288, Grad<KD>::bytes, s>>>(a, group, m);
+    note_launch();
+    return cudaGetLastError();
+}
+
+size_t up256(size_t x) { return (x + 255) / 256 * 256; }
+int key_dim(const DArgs& a) { return a.K <= 64 ? 64 : 128; }
+size_t ids(const DArgs& a) { return static_cast<size_t>(a.B) * a.Hv * a.n; }
+size_t gates_bytes(const DArgs& a) { return up256(ids(a) * kGates * sizeof(float)); }
+size_t square_bytes(const DArgs& a) { return up256(ids(a) * 2 * kCC * sizeof(bf16)); }
+size_t state_bytes(const DArgs& a) { return up256(ids(a) * 2 * a.Vp * (key_dim(a) + 8) * sizeof(bf16)); }
+size_t value_bytes(const DArgs& a, int planes) { return up256(ids(a) * planes * a.Vp * kTld * sizeof(bf16)); }
+
+void set_saved(DArgs& a, void* ws, bool training) {
+    char* w = static_cast<char*>(ws);
+    a.gates = reinterpret_cast<float*>(w); w += gates_bytes(a);
+    a.T = w; w += square_bytes(a);
+    a.M = w; w += square_bytes(a);
+    a.S = training ? w : nullptr; w += state_bytes(a);
+    a.U = training ? w : nullptr;
+}
+
+}  // namespace
+
+size_t planes_saved_size(const DArgs& a, bool training) {
+    return gates_bytes(a) + 2 * square_bytes(a) + (training ? state_bytes(a) + value_bytes(a, 2) : 0);
+}
+size_t planes_bwd_size(const DArgs& a) { return state_bytes(a) + value_bytes(a, 2); }
+
+cudaError_t planes_fwd(DArgs a, void* ws, bool training, cudaStream_t s) {
+    set_saved(a, ws, training);
+    return a.K <= 64 ? fwd<64>(a, s) : fwd<128>(a, s);
+}
+
+cudaError_t planes_bwd(DArgs a, void* saved, void* ws, float* group, cudaStream_t s) {
+    set_saved(a, saved, true);
+    char* w = static_cast<char*>(ws);
+    a.dS = w;
+    a.dV = w + state_bytes(a);
+    return a.K <= 64 ? bwd<64>(a, group, s) : bwd<128>(a, group, s);
+}
+
+cudaError_t planes_read_status(int* out, cudaStream_t s) { return read_clear_status(out, s); }
+
+}  // namespace eacs

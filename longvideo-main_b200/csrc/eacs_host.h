@@ -364,6 +364,7 @@ int delta_fwd(const EacsDelta& p, void* o, float* final_state, void* ws, size_t 
 int delta_bwd(const EacsDelta& p, const DeltaGrads& d, const void* saved, size_t saved_bytes, void* ws, size_t ws_bytes,
               cudaStream_t stream);
 int delta_step(const EacsDelta& p, void* o, float* final_state, cudaStream_t stream);
+cudaError_t planes_read_status(int* out, cudaStream_t stream);
 
 // train.cu
 struct TrainBwdCall {

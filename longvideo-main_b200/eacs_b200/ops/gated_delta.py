@@ -106,7 +106,9 @@ class GatedDeltaFunction(torch.autograd.Function):
         dev = ctx.dev
         if do is None and dfinal is None:
             return (None,) * 10
-        do = torch.zeros(v.shape, dtype=q.dtype, device=dev) if do is None else _dense_last(do)
+        do = torch.zeros(v.shape, dtype=q.dtype, device=dev) if do is None else do.contiguous()
+        if do.data_ptr() % 16:  # a view that starts inside an allocation
+            do = do.clone()
         dfinal = None if dfinal is None else dfinal.contiguous()
         p = _args(q, k, v, g, beta, ctx.scale, lengths, initial)
         L_ = _lib.lib()
