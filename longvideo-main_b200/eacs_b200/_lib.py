@@ -7,6 +7,7 @@ from __future__ import annotations
 
 import ctypes
 import os
+import struct
 import threading
 
 import torch
@@ -31,13 +32,11 @@ _I = ctypes.c_int
 _SZ = ctypes.c_size_t
 
 
-class Delta(ctypes.Structure):
-    """EacsDelta (include/eacs_b200.h)."""
-    _fields_ = ([(n, _P) for n in ("q", "k", "v", "g", "beta")]
-                + [(n + "_stride", _I64 * 3) for n in ("q", "k", "v", "g", "beta")]
-                + [("lengths", _P), ("initial_state", _P)]
-                + [(n, _I64) for n in ("B", "L", "Hk", "Hv", "K", "V")]
-                + [("scale", _F), ("dtype", ctypes.c_int32), ("gate_dtype", ctypes.c_int32)])
+# EacsDelta (include/eacs_b200.h) as bytes: 5 pointers, their strides over batch,
+# token and head, lengths and initial_state, B, L, Hk, Hv, K, V, scale, types.
+# (Packed in one call: a ctypes.Structure filled field by field takes as long as
+# a short launch.)
+DELTA = struct.Struct("=5Q15q2Q6qf2i4x")
 
 
 # name -> (restype, argtypes); mirrors include/eacs_b200.h
@@ -174,6 +173,11 @@ def check(rc: int, name: str) -> None:
 
 def stream_ptr(device: torch.device | None = None) -> int:
     return torch.cuda.current_stream(device).cuda_stream
+
+
+def raw_stream(index: int) -> int:
+    """Device `index`'s current stream, as stream_ptr without a Stream object."""
+    return torch._C._cuda_getCurrentRawStream(index)
 
 
 def ptr(t: torch.Tensor | None) -> int | None:

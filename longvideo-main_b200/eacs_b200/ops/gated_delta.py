@@ -24,7 +24,7 @@ import torch
 from torch import Tensor
 
 from .. import _lib
-from ._check import cuda_tensors, require
+from ._check import on, one_device
 
 MAX_K = 128
 MAX_V = 1024
@@ -38,42 +38,47 @@ def _dense_last(t: Tensor) -> Tensor:
 
 def _check(name, q, k, v, g, beta, lengths, state, lead):
     """Device of the arguments; lead: the dimensions in front of the head's."""
-    ts = [t for t in (q, k, v, g, beta, lengths, state) if t is not None]
-    dev = cuda_tensors(name, *ts)
-    require(q.dim() == lead + 2 and k.shape == q.shape, f"{name}: q and k must have one shape of {lead + 2} dimensions")
-    require(v.dim() == lead + 2 and v.shape[:lead] == q.shape[:lead], f"{name}: v must have q's leading dimensions")
-    Hk, K = q.shape[-2:]
-    Hv, V = v.shape[-2:]
-    require(Hk >= 1 and Hv >= 1 and Hv % Hk == 0, f"{name}: {Hv} value heads are not a multiple of {Hk} key heads")
-    require(1 <= K <= MAX_K and 1 <= V <= MAX_V, f"{name}: K={K}, V={V} must be 1 to {MAX_K}, 1 to {MAX_V}")
-    require(g.shape == v.shape[:-1] and beta.shape == g.shape, f"{name}: g and beta must be {tuple(v.shape[:-1])}")
-    require(q.dtype in _lib.DTYPE_CODES and k.dtype == q.dtype and v.dtype == q.dtype,
-            f"{name}: q, k and v must have one dtype, float32, float16 or bfloat16")
-    require(g.dtype == beta.dtype and g.dtype in (torch.float32, q.dtype),
-            f"{name}: g and beta must both be float32 or of q's dtype")
-    if lengths is not None:
-        require(lengths.dtype == torch.int32 and lengths.shape == q.shape[:1],
-                f"{name}: lengths must be int32 ({q.shape[0]},)")
-    if state is not None:
-        require(state.dtype == torch.float32 and state.shape == (q.shape[0], Hv, K, V),
-                f"{name}: the state must be float32 ({q.shape[0]}, {Hv}, {K}, {V})")
+    dev = one_device(name, q, k, v, g, beta, lengths, state)
+    qs, vs, dt = q.shape, v.shape, q.dtype
+    if len(qs) != lead + 2 or k.shape != qs:
+        raise RuntimeError(f"{name}: q and k must have one shape of {lead + 2} dimensions")
+    if len(vs) != lead + 2 or vs[:lead] != qs[:lead]:
+        raise RuntimeError(f"{name}: v must have q's leading dimensions")
+    Hk, K = qs[lead:]
+    Hv, V = vs[lead:]
+    if Hk < 1 or Hv < 1 or Hv % Hk:
+        raise RuntimeError(f"{name}: {Hv} value heads are not a multiple of {Hk} key heads")
+    if not (1 <= K <= MAX_K and 1 <= V <= MAX_V):
+        raise RuntimeError(f"{name}: K={K}, V={V} must be 1 to {MAX_K}, 1 to {MAX_V}")
+    if g.shape != vs[:-1] or beta.shape != g.shape:
+        raise RuntimeError(f"{name}: g and beta must be {tuple(vs[:-1])}")
+    if dt not in _lib.DTYPE_CODES or k.dtype != dt or v.dtype != dt:
+        raise RuntimeError(f"{name}: q, k and v must have one dtype, float32, float16 or bfloat16")
+    if g.dtype != beta.dtype or (g.dtype != dt and g.dtype != torch.float32):
+        raise RuntimeError(f"{name}: g and beta must both be float32 or of q's dtype")
+    if lengths is not None and (lengths.dtype != torch.int32 or lengths.shape != qs[:1]):
+        raise RuntimeError(f"{name}: lengths must be int32 ({qs[0]},)")
+    if state is not None and (state.dtype != torch.float32 or state.shape != (qs[0], Hv, K, V)):
+        raise RuntimeError(f"{name}: the state must be float32 ({qs[0]}, {Hv}, {K}, {V})")
     return dev
 
 
-def _args(q, k, v, g, beta, scale, lengths, state) -> _lib.Delta:
-    B, L, Hk, K = q.shape
-    Hv, V = v.shape[2:]
-    p = _lib.Delta()
-    for n, t in (("q", q), ("k", k), ("v", v), ("g", g), ("beta", beta)):
-        setattr(p, n, t.data_ptr())
-        setattr(p, n + "_stride", (ctypes.c_int64 * 3)(*t.stride()[:3]))
-    p.lengths = _lib.ptr(lengths)
-    p.initial_state = _lib.ptr(state)
-    p.B, p.L, p.Hk, p.Hv, p.K, p.V = B, L, Hk, Hv, K, V
-    p.scale = scale
-    p.dtype = _lib.DTYPE_CODES[q.dtype]
-    p.gate_dtype = _lib.DTYPE_CODES[g.dtype]
-    return p
+def _args(q, k, v, g, beta, scale, lengths, state) -> bytes:
+    """EacsDelta of a sequence (B, L, H, D), or of one token a row (B, H, D)."""
+    qs, vs = q.shape, v.shape
+    if len(qs) == 4:
+        L = qs[1]
+        st = (*q.stride()[:3], *k.stride()[:3], *v.stride()[:3], *g.stride(), *beta.stride())
+    else:
+        L = 1
+        st = []
+        for t in (q, k, v, g, beta):
+            s = t.stride()
+            st += (s[0], 0, s[1])
+    return _lib.DELTA.pack(q.data_ptr(), k.data_ptr(), v.data_ptr(), g.data_ptr(), beta.data_ptr(), *st,
+                           0 if lengths is None else lengths.data_ptr(), 0 if state is None else state.data_ptr(),
+                           qs[0], L, qs[-2], vs[-2], qs[-1], vs[-1], scale, _lib.DTYPE_CODES[q.dtype],
+                           _lib.DTYPE_CODES[g.dtype])
 
 
 def _forward(args, out_state, training, dev):
@@ -83,10 +88,10 @@ def _forward(args, out_state, training, dev):
     L_ = _lib.lib()
     o = torch.empty(v.shape, dtype=q.dtype, device=dev)
     final = torch.empty(v.shape[0], v.shape[2], q.shape[3], v.shape[3], dtype=torch.float32, device=dev) if out_state else None
-    ws = torch.empty(int(L_.eacs_delta_workspace_size(ctypes.byref(p), int(training))), dtype=torch.uint8, device=dev)
-    with torch.cuda.device(dev):
-        _lib.check(L_.eacs_delta_fwd(ctypes.byref(p), o.data_ptr(), _lib.ptr(final), ws.data_ptr(), ws.numel(),
-                                     int(training), _lib.stream_ptr(dev)), "eacs_delta_fwd")
+    ws = torch.empty(int(L_.eacs_delta_workspace_size(p, int(training))), dtype=torch.uint8, device=dev)
+    with on(dev):
+        _lib.check(L_.eacs_delta_fwd(p, o.data_ptr(), _lib.ptr(final), ws.data_ptr(), ws.numel(),
+                                     int(training), _lib.raw_stream(dev.index)), "eacs_delta_fwd")
     return o, final, ws
 
 
@@ -114,12 +119,12 @@ class GatedDeltaFunction(torch.autograd.Function):
         L_ = _lib.lib()
         dq, dk, dv, dg, db = (torch.empty(t.shape, dtype=t.dtype, device=dev) for t in (q, k, v, g, beta))
         di = torch.empty(initial.shape, dtype=torch.float32, device=dev) if ctx.needs_input_grad[7] else None
-        w2 = torch.empty(int(L_.eacs_delta_bwd_workspace_size(ctypes.byref(p))), dtype=torch.uint8, device=dev)
-        with torch.cuda.device(dev):
+        w2 = torch.empty(int(L_.eacs_delta_bwd_workspace_size(p)), dtype=torch.uint8, device=dev)
+        with on(dev):
             _lib.check(L_.eacs_delta_bwd(
-                ctypes.byref(p), do.data_ptr(), (ctypes.c_int64 * 3)(*do.stride()[:3]), _lib.ptr(dfinal), dq.data_ptr(),
+                p, do.data_ptr(), (ctypes.c_int64 * 3)(*do.stride()[:3]), _lib.ptr(dfinal), dq.data_ptr(),
                 dk.data_ptr(), dv.data_ptr(), dg.data_ptr(), db.data_ptr(), _lib.ptr(di), ws.data_ptr(), ws.numel(),
-                w2.data_ptr(), w2.numel(), _lib.stream_ptr(dev)), "eacs_delta_bwd")
+                w2.data_ptr(), w2.numel(), _lib.raw_stream(dev.index)), "eacs_delta_bwd")
         return dq, dk, dv, dg, db, None, None, di, None, None
 
 
@@ -144,21 +149,20 @@ def gated_delta_rule(q: Tensor, k: Tensor, v: Tensor, g: Tensor, beta: Tensor, s
     return (o, final) if output_final_state else o
 
 
-@torch.no_grad()
 def gated_delta_step(q: Tensor, k: Tensor, v: Tensor, g: Tensor, beta: Tensor, state: Tensor,
                      scale: float | None = None) -> Tensor:
     """One token per row: q, k (B, Hk, K), v (B, Hv, V), g and beta (B, Hv);
     `state` (B, Hv, K, V) float32, contiguous, is updated in place.  Returns
     o (B, Hv, V) in q's dtype.  No gradient."""
     dev = _check("gated_delta_step", q, k, v, g, beta, None, state, 1)
-    require(state.is_contiguous() and not state.requires_grad,
-            "gated_delta_step: the state is updated in place: it must be contiguous and without a gradient")
+    if not state.is_contiguous() or state.requires_grad:
+        raise RuntimeError("gated_delta_step: the state is updated in place: it must be contiguous and without a gradient")
     scale = q.shape[-1] ** -0.5 if scale is None else float(scale)
-    q, k, v, g, beta = (t.unsqueeze(1) for t in (_dense_last(q), _dense_last(k), _dense_last(v), g, beta))
+    q, k, v = _dense_last(q), _dense_last(k), _dense_last(v)
     o = torch.empty(v.shape, dtype=q.dtype, device=dev)
     p = _args(q, k, v, g, beta, scale, None, state)
-    with torch.cuda.device(dev):
-        _lib.check(_lib.lib().eacs_delta_step(ctypes.byref(p), o.data_ptr(), state.data_ptr(), _lib.stream_ptr(dev)),
+    with on(dev):
+        _lib.check(_lib.lib().eacs_delta_step(p, o.data_ptr(), state.data_ptr(), _lib.raw_stream(dev.index)),
                    "eacs_delta_step")
     torch.autograd.graph.increment_version(state)
-    return o.squeeze(1)
+    return o

@@ -20,7 +20,7 @@ import torch
 from torch import Tensor, nn
 
 from .. import _lib
-from ._check import cuda_tensors, require
+from ._check import on, one_device
 
 MAX_D = 8192
 
@@ -46,11 +46,11 @@ def _forward(x, weight, bias, eps, residual, dev):
         xr, xs = _rows(x, d)
         rr, rs = (None, 0) if residual is None else _rows(residual, d)
         w = weight if weight is not None else bias
-        with torch.cuda.device(dev):
+        with on(dev):
             _lib.check(_lib.lib().eacs_layer_norm_fwd(
                 xr.data_ptr(), xs, _lib.ptr(rr), rs, _lib.DTYPE_CODES[x.dtype], _lib.ptr(weight), _lib.ptr(bias),
                 0 if w is None else _lib.DTYPE_CODES[w.dtype], eps, y.data_ptr(), y.numel() // d, d,
-                _lib.stream_ptr(dev)), "eacs_layer_norm_fwd")
+                _lib.raw_stream(dev.index)), "eacs_layer_norm_fwd")
     return y
 
 
@@ -80,15 +80,13 @@ class LayerNormFunction(torch.autograd.Function):
         xr, xs = _rows(x, d)
         gr, gs = _rows(dy, d)
         rr, rs = (None, 0) if residual is None else _rows(residual, d)
-        with torch.cuda.device(dev):
+        with on(dev):
             _lib.check(L.eacs_layer_norm_bwd(
                 xr.data_ptr(), xs, _lib.ptr(rr), rs, gr.data_ptr(), gs, _lib.DTYPE_CODES[x.dtype], _lib.ptr(weight),
                 0 if wd is None else _lib.DTYPE_CODES[wd], ctx.eps, dx.data_ptr(), _lib.ptr(dw), _lib.ptr(db),
-                _lib.ptr(ws), 0 if ws is None else ws.numel(), rows, d, _lib.stream_ptr(dev)), "eacs_layer_norm_bwd")
-        dr = None
-        if need_r:
-            dr = dx if not need_x else dx.clone()
-        return dx if need_x else None, dw, db, None, dr, None
+                _lib.ptr(ws), 0 if ws is None else ws.numel(), rows, d, _lib.raw_stream(dev.index)), "eacs_layer_norm_bwd")
+        # one gradient for both, as a sum's backward gives it
+        return dx if need_x else None, dw, db, None, dx if need_r else None, None
 
 
 def layer_norm(x: Tensor, weight: Tensor | None = None, bias: Tensor | None = None, eps: float = 1e-5,
@@ -97,23 +95,28 @@ def layer_norm(x: Tensor, weight: Tensor | None = None, bias: Tensor | None = No
 
     x (..., d) float32 / float16 / bfloat16, d up to 8192; residual like x;
     weight and bias (d), both of one of those dtypes, or None."""
-    ts = [t for t in (x, residual, weight, bias) if t is not None]
-    dev = cuda_tensors("layer_norm", *ts)
-    require(x.dim() >= 1 and x.dtype in _lib.DTYPE_CODES, f"layer_norm: unsupported x {x.dtype}, {x.dim()} dimensions")
+    dev = one_device("layer_norm", x, residual, weight, bias)
+    dt = x.dtype
+    if x.dim() < 1 or dt not in _lib.DTYPE_CODES:
+        raise RuntimeError(f"layer_norm: unsupported x, {dt} of {x.dim()} dimensions")
     d = x.shape[-1]
-    require(1 <= d <= MAX_D, f"layer_norm: d={d} must be 1 to {MAX_D}")
+    if not 1 <= d <= MAX_D:
+        raise RuntimeError(f"layer_norm: d={d} must be 1 to {MAX_D}")
+    grad = x.requires_grad
     if residual is not None:
-        require(residual.shape == x.shape and residual.dtype == x.dtype,
-                "layer_norm: residual must have x's shape and dtype")
-    wd = None
-    for n, t in (("weight", weight), ("bias", bias)):
+        if residual.shape != x.shape or residual.dtype != dt:
+            raise RuntimeError("layer_norm: residual must have x's shape and dtype")
+        grad = grad or residual.requires_grad
+    for t in (weight, bias):
         if t is not None:
-            require(t.shape == (d,) and t.dtype in _lib.DTYPE_CODES, f"layer_norm: {n} must be ({d},) floating")
-            require(wd is None or t.dtype == wd, "layer_norm: weight and bias must have one dtype")
-            wd = t.dtype
+            if t.dim() != 1 or t.shape[0] != d or t.dtype not in _lib.DTYPE_CODES:
+                raise RuntimeError(f"layer_norm: weight and bias must be ({d},), float32, float16 or bfloat16")
+            grad = grad or t.requires_grad
+    if weight is not None and bias is not None and weight.dtype != bias.dtype:
+        raise RuntimeError("layer_norm: weight and bias must have one dtype")
     weight = weight if weight is None else weight.contiguous()
     bias = bias if bias is None else bias.contiguous()
-    if torch.is_grad_enabled() and any(t.requires_grad for t in ts):
+    if grad and torch.is_grad_enabled():
         return LayerNormFunction.apply(x, weight, bias, float(eps), residual, dev)
     return _forward(x, weight, bias, float(eps), residual, dev)
 

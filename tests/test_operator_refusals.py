@@ -14,14 +14,9 @@ from eacs_b200 import _lib
 P = 256  # a pointer value that is never read
 
 
-def delta(B=2, L=10, Hk=2, Hv=4, K=16, V=8, dtype=2, gate=2, **kw):
-    p = _lib.Delta()
-    for n in ("q", "k", "v", "g", "beta"):
-        setattr(p, n, P)
-    p.B, p.L, p.Hk, p.Hv, p.K, p.V, p.dtype, p.gate_dtype, p.scale = B, L, Hk, Hv, K, V, dtype, gate, 1.0
-    for n, v in kw.items():
-        setattr(p, n, v)
-    return ctypes.byref(p)
+def delta(B=2, L=10, Hk=2, Hv=4, K=16, V=8, dtype=2, gate=2, **pointers):
+    p = [pointers.get(n, P) or 0 for n in ("q", "k", "v", "g", "beta")]
+    return _lib.DELTA.pack(*p, *[0] * 15, 0, 0, B, L, Hk, Hv, K, V, 1.0, dtype, gate)
 
 
 def test_layer_norm_rejects_bad_arguments_without_device():
