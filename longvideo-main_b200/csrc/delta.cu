@@ -1099,6 +1099,8 @@ int check_delta(const EacsDelta& p, const char* fn) {
     if (p.V > 1024) return fail(EACS_ERR_UNSUPPORTED, "%s: V=%lld > 1024", fn, (long long)p.V);
     if (p.B > 65535 || p.Hv > 65535 || p.L > (int64_t{1} << 30))
         return fail(EACS_ERR_UNSUPPORTED, "%s: B and Hv go to 65535, L to 2^30", fn);
+    if (p.B * p.Hv * ((p.L + kC - 1) / kC) > (int64_t{1} << 31) - 1)
+        return fail(EACS_ERR_UNSUPPORTED, "%s: more than 2^31 - 1 chunks of 64 tokens in all", fn);
     return EACS_OK;
 }
 

@@ -9,7 +9,7 @@
 namespace eacs {
 
 constexpr int kC = 64;           // tokens per chunk
-constexpr int kGates = 5 * kC;   // floats of a chunk's gates
+constexpr int kGates = 6 * kC;   // floats of a chunk's gates
 constexpr int kTld = kC + 8;     // row stride of a 64-column tile in shared memory
 constexpr float kBetaMin = 5.421010862427522e-20f;  // 2^-64
 
@@ -175,7 +175,7 @@ struct DArgs {
     int vec_qk, vec_v, vec_do;  // rows can be read 16 bytes at a time
     float scale;
     // workspace, per chunk id ((b Hv + h) n + c)
-    float* gates;  // [id][5][64]: G (high), G (low), gam, d, scale gam
+    float* gates;  // [id][6][64]: G (high), G (low), gam, d, scale gam, 1 / beta (delta_planes.cu)
     void* T;       // [id][planes][64][64]
     void* M;       // [id][64][64] or null
     void* S;       // [id][Vp][KD]: S0^T or null

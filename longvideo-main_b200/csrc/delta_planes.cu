@@ -295,6 +295,7 @@ __global__ void __launch_bounds__(128) planes_prep_k(DArgs a) {
             ga[2 * kC + r] = gam;
             ga[3 * kC + r] = exp2f(static_cast<float>(total - G));
             ga[4 * kC + r] = a.scale * gam;
+            ga[5 * kC + r] = r < rows ? 1.f / sB[r] : 0.f;
         }
     }
     cp_async_wait_all();
@@ -975,12 +976,18 @@ __global__ void __launch_bounds__(Rev<KD, G>::kWarps * 32) planes_rchain_k(DArgs
 // ----------------------------------------------------------------------------
 // dQ, dK, dV, dbeta and dg of a chunk
 // ----------------------------------------------------------------------------
-// A CTA goes through chunks (of a key head) in a grid-stride loop: a warp loads
-// ahead of eight that compute, 4 groups of 16 rows by 2 halves of the key
-// columns.  The value columns come in tiles of 32, two deep, so that the two
-// states of a chunk (in two planes 139 KB of its 260 KB) never have to be in
-// shared memory whole.  dV, whose rounding does not show in the products, goes
-// in as one plane (the output itself); U, S, dS, N and E as two.
+// A CTA goes through chunks (of a key head) in a grid-stride loop with sixteen
+// warps, of which the first also asks for the loads of the tile after next (a
+// seventeenth warp would leave 112 registers a lane).  Eight (the readers) hold dQ and dK_read, eight
+// (the writers) dK_write and N or E; of each, 4 groups of 16 rows by 2 halves of
+// the key columns.  So a lane has 64 sums and nothing spills: shared memory leaves
+// the L1 cache too small for it, and spilled sums went to L2 (1039 us for 393216
+// tokens of 128 x 128 with 16 warps of a quarter of all products each).  The value
+// columns come in tiles of 32, two deep, so that the two states of a chunk (in two
+// planes 139 KB of its 260 KB) never have to be in shared memory whole.  dV, whose
+// rounding does not show in the products, goes in as one plane (the output
+// itself); U, S, dS, N and E as two.
+constexpr int kGradWarps = 16;
 template <int KD>
 struct Grad {
     static constexpr int VT = 32, LDK = KD + 8;
@@ -989,12 +996,12 @@ struct Grad {
     static constexpr int kStage = up1024(kGa * 2 + kGates * 4);    // bytes
     static constexpr int kK = 0, kQ = kC * KD, kKQ = 2 * kC * KD * 2;  // (elements, elements, bytes)
     static constexpr int kN = 2 * kStage + 2 * kKQ;                // N and E, two planes each (bytes)
-    static constexpr int kF = kN + 4 * kCC * 2;                    // floats: beta, row sums, dbeta, totals
-    static constexpr int kBars = kF + (kC + 4 * kC + 16) * 4;
-    static constexpr size_t bytes = 1024 + kBars + 8 * 9;
+    static constexpr int kF = kN + 4 * kCC * 2;                    // floats: row sums, dbeta, totals
+    static constexpr int kBars = kF + (4 * kC + 2 * kC + 2 * kGradWarps) * 4;
+    static constexpr size_t bytes = 1024 + kBars + 8 * 9 + 8 * 4;
 };
 
-__device__ __forceinline__ void sync_compute() { asm volatile("bar.sync 1, 256;" ::: "memory"); }
+__device__ __forceinline__ void sync_compute() { __syncthreads(); }
 
 __device__ __forceinline__ void split_store(bf16* s, float x, float y) {  // and its low plane kCC further
     const uint32_t hi = pack_bf16(x, y);
@@ -1021,9 +1028,9 @@ __device__ __forceinline__ void rows_out(const float (*x)[4], bf16* p, int64_t s
 }
 
 template <int KD>
-__global__ void __launch_bounds__(288) planes_grad_k(DArgs a, float* group, const __grid_constant__ Maps maps) {
+__global__ void __launch_bounds__(32 * kGradWarps, 1) planes_grad_k(DArgs a, float* group, const __grid_constant__ Maps maps) {
     using Sm = Grad<KD>;
-    constexpr int VT = Sm::VT, NT = KD / 16;
+    constexpr int VT = Sm::VT, NT = KD / 16;  // accumulator tiles of a half of the key columns
     extern __shared__ __align__(128) unsigned char smem_raw[];
     unsigned char* smem = align_smem(smem_raw);
     uint64_t* full = reinterpret_cast<uint64_t*>(smem + Sm::kBars);
@@ -1033,111 +1040,142 @@ __global__ void __launch_bounds__(288) planes_grad_k(DArgs a, float* group, cons
     if (tid == 0) {
         for (int s = 0; s < 2; ++s) {
             mbar_init(&full[s], 1);
-            mbar_init(&empty[s], 8);
+            mbar_init(&empty[s], kGradWarps);
             mbar_init(&qfull[s], 1);
-            mbar_init(&qempty[s], 8);
+            mbar_init(&qempty[s], kGradWarps);
         }
         mbar_init(land, 1);
         fence_mbar_init();
     }
     __syncthreads();
-    const int64_t items = static_cast<int64_t>(a.B) * a.Hk * a.n;
+    const int items = a.B * a.Hk * a.n;
     bool ok = true;
     int tile = 0, seen = 0;  // tiles and chunks so far
-    if (warp == 8) {
-        int landed = 0;
-        for (int64_t it = blockIdx.x; it < items && ok; it += gridDim.x) {
-            const int c = static_cast<int>(it % a.n), hk = static_cast<int>(it / a.n % a.Hk);
-            const int b = static_cast<int>(it / a.n / a.Hk);
-            const int t0 = c * kC, rows = min(kC, row_length(a, b) - t0);
-            if (rows <= 0) continue;
-            const bool tail = rows < min(kC, a.L - t0);
-            {
-                bf16* e = reinterpret_cast<bf16*>(smem + 2 * Sm::kStage + (seen & 1) * Sm::kKQ);
-                uint64_t* bar = tail ? land : &qfull[seen & 1];
-                ok = warp_wait(&qempty[seen & 1], ((seen >> 1) & 1) ^ 1);
-                if (L.l == 0) {
-                    mbar_expect_tx(bar, Sm::kKQ);
+    // Where the loads are (warp 0 alone; in shared memory, as a lane has no registers for it):
+    // chunk, value head, first value column; tiles and chunks so far; waits for `land` so far.
+    int* at = reinterpret_cast<int*>(land + 1);
+    auto produce = [&]() {
+        int it = at[0], h = at[1], v0 = at[2];
+        if (it >= items) return;
+        const int bh = it / a.n, c = it - bh * a.n, b = bh / a.Hk, hk = bh - b * a.Hk, t0 = c * kC;
+        const int ptile = at[3], pseen = at[4];
+        int landed = at[5];
+        const int rows = min(kC, row_length(a, b) - t0);
+        const bool tail = rows < min(kC, a.L - t0);
+        if (h < 0) {  // a new chunk: its keys and queries
+            h = hk * rep;
+            bf16* e = reinterpret_cast<bf16*>(smem + 2 * Sm::kStage + (pseen & 1) * Sm::kKQ);
+            uint64_t* bar = tail ? land : &qfull[pseen & 1];
+            ok = warp_wait(&qempty[pseen & 1], ((pseen >> 1) & 1) ^ 1) && ok;
+            if (L.l == 0) {
+                mbar_expect_tx(bar, Sm::kKQ);
 #pragma unroll
-                    for (int x = 0; x < KD; x += 64) {
-                        tma_load(e + Sm::kK + x * kC, &maps.k, bar, x, t0, hk, b);
-                        tma_load(e + Sm::kQ + x * kC, &maps.q, bar, x, t0, hk, b);
-                    }
+                for (int x = 0; x < KD; x += 64) {
+                    tma_load(e + Sm::kK + x * kC, &maps.k, bar, x, t0, hk, b);
+                    tma_load(e + Sm::kQ + x * kC, &maps.q, bar, x, t0, hk, b);
                 }
-                __syncwarp();
-                if (tail) {
-                    ok = warp_wait(land, landed++ & 1) && ok;
-                    zero_rows<64>(e + Sm::kK, 2 * (KD / 64), rows);
-                    fence_async();
-                    warp_arrive(&qfull[seen & 1]);
-                }
-                ++seen;
             }
-            for (int h = hk * rep; h < (hk + 1) * rep; ++h) {
-                const int64_t id = (static_cast<int64_t>(b) * a.Hv + h) * a.n + c;
-                for (int v0 = 0; v0 < a.Vp && ok; v0 += VT, ++tile) {
-                    const int vn = min(VT, a.Vp - v0);
-                    bf16* e = reinterpret_cast<bf16*>(smem + (tile & 1) * Sm::kStage);
-                    uint64_t* bar = tail ? land : &full[tile & 1];
-                    ok = warp_wait(&empty[tile & 1], ((tile >> 1) & 1) ^ 1);
-                    if (L.l == 0) {
-                        mbar_expect_tx(bar, vn * (kC + 4 * kTld + 4 * Sm::LDK) * 2 + kGates * 4);
-                        for (int v = 0; v < vn; v += 16) tma_load(e + Sm::kD + v * kC, &maps.d, bar, v0 + v, t0, h, b);
-                        const bf16* U = static_cast<const bf16*>(a.U) + (id * 2 * a.Vp + v0) * kTld;
-                        const bf16* X = static_cast<const bf16*>(a.dV) + (id * 2 * a.Vp + v0) * kTld;
-                        const bf16* S = static_cast<const bf16*>(a.S) + (id * 2 * a.Vp + v0) * Sm::LDK;
-                        const bf16* R = static_cast<const bf16*>(a.dS) + (id * 2 * a.Vp + v0) * Sm::LDK;
-                        for (int p = 0; p < 2; ++p) {
-                            bulk_load(e + Sm::kS + p * VT * Sm::LDK, S + static_cast<int64_t>(p) * a.Vp * Sm::LDK,
-                                      vn * Sm::LDK * 2, bar);
-                            bulk_load(e + Sm::kR + p * VT * Sm::LDK, R + static_cast<int64_t>(p) * a.Vp * Sm::LDK,
-                                      vn * Sm::LDK * 2, bar);
-                            bulk_load(e + Sm::kU + p * VT * kTld, U + static_cast<int64_t>(p) * a.Vp * kTld, vn * kTld * 2,
-                                      bar);
-                            bulk_load(e + Sm::kX + p * VT * kTld, X + static_cast<int64_t>(p) * a.Vp * kTld, vn * kTld * 2,
-                                      bar);
-                        }
-                        bulk_load(e + Sm::kGa, a.gates + id * kGates, kGates * 4, bar);
-                    }
-                    __syncwarp();
-                    if (tail) {
-                        ok = warp_wait(land, landed++ & 1) && ok;
-                        zero_rows<16>(e + Sm::kD, vn / 16, rows);
-                        fence_async();
-                        warp_arrive(&full[tile & 1]);
-                    }
+            __syncwarp();
+            if (tail) {
+                ok = warp_wait(land, landed++ & 1) && ok;
+                zero_rows<64>(e + Sm::kK, 2 * (KD / 64), rows);
+                fence_async();
+                warp_arrive(&qfull[pseen & 1]);
+            }
+        }
+        const int vn = min(VT, a.Vp - v0);
+        bf16* e = reinterpret_cast<bf16*>(smem + (ptile & 1) * Sm::kStage);
+        uint64_t* bar = tail ? land : &full[ptile & 1];
+        ok = warp_wait(&empty[ptile & 1], ((ptile >> 1) & 1) ^ 1) && ok;
+        if (L.l == 0) {
+            const int64_t id = (static_cast<int64_t>(b) * a.Hv + h) * a.n + c;
+            mbar_expect_tx(bar, vn * (kC + 4 * kTld + 4 * Sm::LDK) * 2 + kGates * 4);
+            for (int v = 0; v < vn; v += 16) tma_load(e + Sm::kD + v * kC, &maps.d, bar, v0 + v, t0, h, b);
+            const bf16* U = static_cast<const bf16*>(a.U) + (id * 2 * a.Vp + v0) * kTld;
+            const bf16* X = static_cast<const bf16*>(a.dV) + (id * 2 * a.Vp + v0) * kTld;
+            const bf16* S = static_cast<const bf16*>(a.S) + (id * 2 * a.Vp + v0) * Sm::LDK;
+            const bf16* R = static_cast<const bf16*>(a.dS) + (id * 2 * a.Vp + v0) * Sm::LDK;
+            for (int p = 0; p < 2; ++p) {
+                bulk_load(e + Sm::kS + p * VT * Sm::LDK, S + static_cast<int64_t>(p) * a.Vp * Sm::LDK, vn * Sm::LDK * 2, bar);
+                bulk_load(e + Sm::kR + p * VT * Sm::LDK, R + static_cast<int64_t>(p) * a.Vp * Sm::LDK, vn * Sm::LDK * 2, bar);
+                bulk_load(e + Sm::kU + p * VT * kTld, U + static_cast<int64_t>(p) * a.Vp * kTld, vn * kTld * 2, bar);
+                bulk_load(e + Sm::kX + p * VT * kTld, X + static_cast<int64_t>(p) * a.Vp * kTld, vn * kTld * 2, bar);
+            }
+            bulk_load(e + Sm::kGa, a.gates + id * kGates, kGates * 4, bar);
+        }
+        __syncwarp();
+        if (tail) {
+            ok = warp_wait(land, landed++ & 1) && ok;
+            zero_rows<16>(e + Sm::kD, vn / 16, rows);
+            fence_async();
+            warp_arrive(&full[ptile & 1]);
+        }
+        // the next tile: of this head, of the next, or of the next chunk with a token
+        int seen_next = pseen;
+        v0 += VT;
+        if (v0 >= a.Vp) {
+            v0 = 0;
+            if (++h == (hk + 1) * rep) {
+                h = -1;
+                ++seen_next;
+                for (it += gridDim.x; it < items; it += gridDim.x) {
+                    const int nbh = it / a.n;
+                    if (row_length(a, nbh / a.Hk) > (it - nbh * a.n) * kC) break;
                 }
             }
         }
-        return;
+        if (L.l == 0) {
+            at[0] = it;
+            at[1] = h;
+            at[2] = v0;
+            at[3] = ptile + 1;
+            at[4] = seen_next;
+            at[5] = landed;
+        }
+        __syncwarp();
+    };
+    if (warp == 0) {
+        int it = blockIdx.x;
+        for (; it < items; it += gridDim.x) {
+            const int nbh = it / a.n;
+            if (row_length(a, nbh / a.Hk) > (it - nbh * a.n) * kC) break;
+        }
+        if (L.l == 0) {
+            at[0] = it;
+            at[1] = -1;
+            at[2] = at[3] = at[4] = at[5] = 0;
+        }
+        __syncwarp();
+        produce();
     }
-    const int rg = warp & 3, half = warp >> 2, m0 = rg * 16, n0 = half * (KD / 2);
+    const int rg = warp & 3, half = (warp >> 2) & 1, m0 = rg * 16, n0 = half * (KD / 2);
+    const bool writer = warp >= 8;
     const int r0 = m0 + L.g, r1 = r0 + 8;
     bf16* sN = reinterpret_cast<bf16*>(smem + Sm::kN);
     bf16* sE = sN + 2 * kCC;
-    float* sDot = reinterpret_cast<float*>(smem + Sm::kF);  // [2][64]
-    float* sDb = sDot + 2 * kC;                             // [2][64]
-    float* sTot = sDb + 2 * kC;                             // [8], [8]
-    for (int64_t it = blockIdx.x; it < items && ok; it += gridDim.x) {
-        const int c = static_cast<int>(it % a.n), hk = static_cast<int>(it / a.n % a.Hk);
-        const int b = static_cast<int>(it / a.n / a.Hk);
+    float* sW = reinterpret_cast<float*>(smem + Sm::kN);    // dK_write, once N and E are done with
+    float* sDot = reinterpret_cast<float*>(smem + Sm::kF);  // [4][64]
+    float* sDb = sDot + 4 * kC;                             // [2][64]
+    float* sTot = sDb + 2 * kC;                             // [16], [16]
+    for (int it = blockIdx.x; it < items && ok; it += gridDim.x) {
+        const int bh = it / a.n, c = it - bh * a.n, b = bh / a.Hk, hk = bh - b * a.Hk;
         const int rows = min(kC, row_length(a, b) - c * kC), all = min(kC, a.L - c * kC);
-        const int64_t t0 = static_cast<int64_t>(c) * kC, row0 = static_cast<int64_t>(b) * a.L + t0;
-        const int64_t qst = static_cast<int64_t>(a.Hk) * a.K, vst = static_cast<int64_t>(a.Hv) * a.V;
-        bf16* dq = static_cast<bf16*>(a.dq) + row0 * qst + static_cast<int64_t>(hk) * a.K;
-        bf16* dk = static_cast<bf16*>(a.dk) + row0 * qst + static_cast<int64_t>(hk) * a.K;
+        const int64_t row0 = static_cast<int64_t>(b) * a.L + static_cast<int64_t>(c) * kC;
+        const int qst = a.Hk * a.K, vst = a.Hv * a.V;
+        bf16* dq = static_cast<bf16*>(a.dq) + row0 * qst + hk * a.K;
+        bf16* dk = static_cast<bf16*>(a.dk) + row0 * qst + hk * a.K;
         if (rows <= 0) {  // behind the sequence
             const uint4 z = make_uint4(0, 0, 0, 0);
-            for (int i = tid; i < all * (a.K / 8); i += 256) {
-                const int64_t o = i / (a.K / 8) * qst + i % (a.K / 8) * 8;
+            for (int i = tid; i < all * (a.K / 8); i += 32 * kGradWarps) {
+                const int64_t o = static_cast<int64_t>(i / (a.K / 8)) * qst + i % (a.K / 8) * 8;
                 *reinterpret_cast<uint4*>(dq + o) = z;
                 *reinterpret_cast<uint4*>(dk + o) = z;
             }
             for (int h = hk * rep; h < (hk + 1) * rep; ++h) {
                 bf16* dv = static_cast<bf16*>(a.dv) + row0 * vst + static_cast<int64_t>(h) * a.V;
-                for (int i = tid; i < all * (a.V / 8); i += 256)
-                    *reinterpret_cast<uint4*>(dv + i / (a.V / 8) * vst + i % (a.V / 8) * 8) = z;
-                for (int i = tid; i < all; i += 256) {
+                for (int i = tid; i < all * (a.V / 8); i += 32 * kGradWarps)
+                    *reinterpret_cast<uint4*>(dv + static_cast<int64_t>(i / (a.V / 8)) * vst + i % (a.V / 8) * 8) = z;
+                for (int i = tid; i < all; i += 32 * kGradWarps) {
                     gate_store(a.dg, a.gate_dtype, (row0 + i) * a.Hv + h, 0.f);
                     gate_store(a.dbeta, a.gate_dtype, (row0 + i) * a.Hv + h, 0.f);
                 }
@@ -1149,77 +1187,82 @@ __global__ void __launch_bounds__(288) planes_grad_k(DArgs a, float* group, cons
         ok = warp_wait(&qfull[seen & 1], (seen >> 1) & 1);
         for (int h = hk * rep; h < (hk + 1) * rep; ++h) {
             bf16* dv = static_cast<bf16*>(a.dv) + row0 * vst + static_cast<int64_t>(h) * a.V;
-            float ib[2];
-#pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                const int r = r0 + 8 * i;
-                ib[i] = r < rows ? 1.f / hold_beta(gate_value(a.beta, a.gate_dtype, b * a.sb.b + (t0 + r) * a.sb.t + h * a.sb.h))
-                                 : 0.f;
-            }
-            float P[kC / 8][4] = {};  // half 0: dO U^T, half 1: dV U^T
-            float aq[NT][4] = {}, ar[NT][4] = {}, aw[NT][4] = {};
-            float db0 = 0.f, db1 = 0.f, sd = 0.f;
-            float gm[2], gd[2], gc = 0.f;
+            // readers: dQ and dK_read; writers: dK_write, and dO U^T (half 0) or dV U^T (half 1)
+            float x[NT][4] = {}, y[NT > 8 ? NT : 8][4] = {};
+            float db0 = 0.f, db1 = 0.f, sd = 0.f, gc = 0.f;
+            float f0[2], f1[2];  // of rows r0, r1: scale gam and gam, or d
             for (int v0 = 0; v0 < a.Vp; v0 += VT, ++tile) {
                 const int vn = min(VT, a.Vp - v0);
                 const bf16* e = reinterpret_cast<const bf16*>(smem + (tile & 1) * Sm::kStage);
+                const float* ga = reinterpret_cast<const float*>(e + Sm::kGa);
+                if (warp == 0) produce();
                 ok = warp_wait(&full[tile & 1], (tile >> 1) & 1) && ok;
 #pragma unroll
                 for (int kk = 0; kk < VT / 16; ++kk) {
                     if (16 * kk >= vn) break;
-                    Af<1> fd, fx;
-                    Af<2> fu;
-                    ld_a32(fd.r[0], e + Sm::kD + kk * kC * 16, m0);
-                    ld_at(fx.r[0], e + Sm::kX, kTld, m0, 16 * kk);
-                    ld_at(fu.r[0], e + Sm::kU, kTld, m0, 16 * kk);
-                    ld_at(fu.r[1], e + Sm::kU + VT * kTld, kTld, m0, 16 * kk);
-                    const Af<1>& left = half ? fx : fd;
-                    constexpr int NP = NT / 2;
-                    steps<6, false>(  // (two warps a scheduler, and no registers to read ahead)
-                        [&](int i, uint32_t(*f)[4]) {
-                            const bf16* s = e + (i < 2 ? Sm::kU + (i & 1) * VT * kTld
-                                                       : (i < 4 ? Sm::kS : Sm::kR) + (i & 1) * VT * Sm::LDK);
+                    if (!writer) {
+                        Af<1> fd, fx;
+                        ld_a32(fd.r[0], e + Sm::kD + kk * kC * 16, m0);
+                        ld_at(fx.r[0], e + Sm::kX, kTld, m0, 16 * kk);
 #pragma unroll
-                            for (int p = 0; p < 4; ++p) {
-                                if (i < 2) {
-                                    if (p <= rg) ld_b<true>(f[p], s, kTld, 16 * p, 16 * kk);
-                                } else if (p < NP) {
-                                    ld_b<true>(f[p], s, Sm::LDK, n0 + 16 * p, 16 * kk);
-                                }
+                        for (int p = 0; p < NT / 2; ++p) {
+                            uint32_t sh[4], sl[4];
+                            ld_b<true>(sl, e + Sm::kS + VT * Sm::LDK, Sm::LDK, n0 + 16 * p, 16 * kk);
+                            ld_b<true>(sh, e + Sm::kS, Sm::LDK, n0 + 16 * p, 16 * kk);
+                            mma_pair(x[2 * p], x[2 * p + 1], fd.r[0], sl);
+                            mma_pair(y[2 * p], y[2 * p + 1], fx.r[0], sl);
+                            mma_pair(x[2 * p], x[2 * p + 1], fd.r[0], sh);
+                            mma_pair(y[2 * p], y[2 * p + 1], fx.r[0], sh);
+                        }
+                        if ((kk & 1) == half) {  // dv
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) {
+                                const int r = r0 + (i & 1) * 8, col = v0 + 16 * kk + (i >> 1) * 8 + 2 * L.t;
+                                if (r < all && col < a.V)
+                                    *reinterpret_cast<uint32_t*>(dv + static_cast<int64_t>(r) * vst + col) =
+                                        r < rows ? fx.r[0][i] : 0u;
                             }
-                        },
-                        [&](int i, const uint32_t(*f)[4]) {
-                            if (i < 2) {  // dO U^T or dV U^T
+                        }
+                    } else {
+                        Af<1> left;
+                        Af<2> fu;
+                        ld_at(fu.r[0], e + Sm::kU, kTld, m0, 16 * kk);
+                        ld_at(fu.r[1], e + Sm::kU + VT * kTld, kTld, m0, 16 * kk);
+                        if (half) ld_at(left.r[0], e + Sm::kX, kTld, m0, 16 * kk);
+                        else ld_a32(left.r[0], e + Sm::kD + kk * kC * 16, m0);
 #pragma unroll
-                                for (int p = 0; p < 4; ++p)
-                                    if (p <= rg) mma_pair(P[2 * p], P[2 * p + 1], left.r[0], f[p]);
-                            } else if (i < 4) {  // dO S0^T, dV S0^T
+                        for (int p = 0; p < NT / 2; ++p) {
+                            uint32_t rh[4], rl[4];
+                            ld_b<true>(rl, e + Sm::kR + VT * Sm::LDK, Sm::LDK, n0 + 16 * p, 16 * kk);
+                            ld_b<true>(rh, e + Sm::kR, Sm::LDK, n0 + 16 * p, 16 * kk);
+                            mma_pair(x[2 * p], x[2 * p + 1], fu.r[0], rl);
+                            if (p <= rg)
+                                mm_hl<1, true>(y[2 * p], y[2 * p + 1], left, e + Sm::kU, e + Sm::kU + VT * kTld, kTld, 16 * p,
+                                               16 * kk);
+                            mma_pair(x[2 * p], x[2 * p + 1], fu.r[1], rh);
+                            mma_pair(x[2 * p], x[2 * p + 1], fu.r[0], rh);
+                        }
 #pragma unroll
-                                for (int p = 0; p < NP; ++p) mma_pair(aq[2 * p], aq[2 * p + 1], fd.r[0], f[p]);
+                        for (int p = NT / 2; p < kC / 16; ++p)
+                            if (p <= rg)
+                                mm_hl<1, true>(y[2 * p], y[2 * p + 1], left, e + Sm::kU, e + Sm::kU + VT * kTld, kTld, 16 * p,
+                                               16 * kk);
+                        if (half) {  // dbeta = (dV / beta).(U / beta)
+                            uint32_t xl[4];
+                            ld_at(xl, e + Sm::kX + VT * kTld, kTld, m0, 16 * kk);
 #pragma unroll
-                                for (int p = 0; p < NP; ++p) mma_pair(ar[2 * p], ar[2 * p + 1], fx.r[0], f[p]);
-                            } else {  // U dS1^T
-                                if (i == 4) mma_step(aw, fu, f, 0, NP);
-                                else mma_step(aw, Af<1>{{{fu.r[0][0], fu.r[0][1], fu.r[0][2], fu.r[0][3]}}}, f, 0, NP);
+                            for (int i = 0; i < 4; ++i) {
+                                const float2 p = unpack_bf16(left.r[0][i]), q = unpack_bf16(xl[i]);
+                                const float2 u = unpack_bf16(fu.r[0][i]), w = unpack_bf16(fu.r[1][i]);
+                                const float f = ga[5 * kC + (i & 1 ? r1 : r0)];
+                                float& db = i & 1 ? db1 : db0;
+                                db = fmaf((p.x + q.x) * f, (u.x + w.x) * f, db);
+                                db = fmaf((p.y + q.y) * f, (u.y + w.y) * f, db);
                             }
-                        });
-                    if ((kk & 1) == half) {  // dbeta and dv: columns dealt to the halves
-                        uint32_t xl[4];
-                        ld_at(xl, e + Sm::kX + VT * kTld, kTld, m0, 16 * kk);
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) {
-                            const float2 x = unpack_bf16(fx.r[0][i]), xw = unpack_bf16(xl[i]), u = unpack_bf16(fu.r[0][i]), w = unpack_bf16(fu.r[1][i]);
-                            const float f = ib[i & 1];
-                            float& db = i & 1 ? db1 : db0;
-                            db = fmaf((x.x + xw.x) * f, (u.x + w.x) * f, db);
-                            db = fmaf((x.y + xw.y) * f, (u.y + w.y) * f, db);
-                            const int r = r0 + (i & 1) * 8, col = v0 + 16 * kk + (i >> 1) * 8 + 2 * L.t;
-                            if (r < all && col < a.V)
-                                *reinterpret_cast<uint32_t*>(dv + r * vst + col) = r < rows ? fx.r[0][i] : 0u;
                         }
                     }
                 }
-                for (int i = tid; i < vn * (KD / 8); i += 256) {  // <S0, dS1>
+                for (int i = tid; i < vn * (KD / 8); i += 32 * kGradWarps) {  // <S0, dS1>
                     const int o = i / (KD / 8) * Sm::LDK + i % (KD / 8) * 8;
                     const uint4 sh = *reinterpret_cast<const uint4*>(e + Sm::kS + o);
                     const uint4 sl = *reinterpret_cast<const uint4*>(e + Sm::kS + VT * Sm::LDK + o);
@@ -1228,70 +1271,76 @@ __global__ void __launch_bounds__(288) planes_grad_k(DArgs a, float* group, cons
                     const uint32_t *s_h = &sh.x, *s_l = &sl.x, *r_h = &rh.x, *r_l = &rl.x;
 #pragma unroll
                     for (int w = 0; w < 4; ++w) {
-                        const float2 x = unpack_bf16(s_h[w]), y = unpack_bf16(s_l[w]), u = unpack_bf16(r_h[w]), z = unpack_bf16(r_l[w]);
-                        sd = fmaf(x.x + y.x, u.x + z.x, sd);
-                        sd = fmaf(x.y + y.y, u.y + z.y, sd);
+                        const float2 p = unpack_bf16(s_h[w]), q = unpack_bf16(s_l[w]), u = unpack_bf16(r_h[w]), z = unpack_bf16(r_l[w]);
+                        sd = fmaf(p.x + q.x, u.x + z.x, sd);
+                        sd = fmaf(p.y + q.y, u.y + z.y, sd);
                     }
                 }
                 if (v0 + VT >= a.Vp) {  // the gates, and N and E, before the tile is given back
-                    const float* ga = reinterpret_cast<const float*>(e + Sm::kGa);
-                    gm[0] = ga[2 * kC + r0];
-                    gm[1] = ga[2 * kC + r1];
-                    gd[0] = ga[3 * kC + r0];
-                    gd[1] = ga[3 * kC + r1];
                     gc = ga[2 * kC + kC - 1];
-                    bf16* o = half ? sE : sN;
-                    const float f = half ? -1.f : a.scale;
+                    f0[0] = ga[(writer ? 3 : 4) * kC + r0];
+                    f0[1] = ga[(writer ? 3 : 4) * kC + r1];
+                    f1[0] = ga[2 * kC + r0];
+                    f1[1] = ga[2 * kC + r1];
+                    if (writer) {
+                        bf16* o = half ? sE : sN;
+                        const float f = half ? -1.f : a.scale;
 #pragma unroll
-                    for (int j = 0; j < kC / 8; ++j) {
-                        if (j > 2 * rg + 1) break;
+                        for (int j = 0; j < kC / 8; ++j) {
+                            if (j > 2 * rg + 1) break;
+                            const int col = 8 * j + 2 * L.t;
 #pragma unroll
-                        for (int i = 0; i < 2; ++i) {
-                            const int r = i ? r1 : r0, col = 8 * j + 2 * L.t;
-                            const int last = half ? r - 1 : r;  // N with the diagonal, E without
-                            split_store(o + r * kTld + col, col <= last ? f * ratio(ga, r, col) * P[j][2 * i] : 0.f,
-                                        col + 1 <= last ? f * ratio(ga, r, col + 1) * P[j][2 * i + 1] : 0.f);
+                            for (int i = 0; i < 2; ++i) {
+                                const int r = i ? r1 : r0;
+                                const int last = half ? r - 1 : r;  // N with the diagonal, E without
+                                split_store(o + r * kTld + col, col <= last ? f * ratio(ga, r, col) * y[j][2 * i] : 0.f,
+                                            col + 1 <= last ? f * ratio(ga, r, col + 1) * y[j][2 * i + 1] : 0.f);
+                            }
                         }
                     }
                 }
                 warp_arrive(&empty[tile & 1]);
             }
-#pragma unroll
-            for (int o = 1; o < 4; o <<= 1) {
-                db0 += __shfl_xor_sync(0xffffffffu, db0, o);
-                db1 += __shfl_xor_sync(0xffffffffu, db1, o);
-            }
             sd = warp_sum(sd);
-            float tw = 0.f;
+            float tw = 0.f;  // writers: k.(d U dS1^T)
 #pragma unroll
             for (int j = 0; j < NT; ++j) {
                 const int col = n0 + 8 * j + 2 * L.t;
 #pragma unroll
                 for (int i = 0; i < 2; ++i) {
-                    const float2 kv = unpack_bf16(*reinterpret_cast<const uint32_t*>(sK + at128(i ? r1 : r0, col)));
-#pragma unroll
-                    for (int x = 0; x < 2; ++x) {
-                        aq[j][2 * i + x] *= a.scale * gm[i];
-                        ar[j][2 * i + x] *= -gm[i];
-                        aw[j][2 * i + x] *= gd[i];
+                    x[j][2 * i] *= f0[i];
+                    x[j][2 * i + 1] *= f0[i];
+                    if (writer) {
+                        const float2 kv = unpack_bf16(*reinterpret_cast<const uint32_t*>(sK + at128(i ? r1 : r0, col)));
+                        tw = fmaf(kv.x, x[j][2 * i], tw);
+                        tw = fmaf(kv.y, x[j][2 * i + 1], tw);
+                    } else {
+                        y[j][2 * i] *= -f1[i];
+                        y[j][2 * i + 1] *= -f1[i];
                     }
-                    tw = fmaf(kv.x, aw[j][2 * i], tw);
-                    tw = fmaf(kv.y, aw[j][2 * i + 1], tw);
                 }
             }
             tw = warp_sum(tw);
-            if (L.t == 0) {
-                sDb[half * kC + r0] = db0;
-                sDb[half * kC + r1] = db1;
+            if (writer && half) {
+#pragma unroll
+                for (int o = 1; o < 4; o <<= 1) {
+                    db0 += __shfl_xor_sync(0xffffffffu, db0, o);
+                    db1 += __shfl_xor_sync(0xffffffffu, db1, o);
+                }
+                if (L.t == 0) {
+                    sDb[r0] = db0;
+                    sDb[r1] = db1;
+                }
             }
             if (L.l == 0) {
                 sTot[warp] = sd;
-                sTot[8 + warp] = tw;
+                sTot[kGradWarps + warp] = tw;
             }
             sync_compute();  // N, E
+            if (!writer) {
 #pragma unroll
-            for (int kk = 0; kk < kC / 16; ++kk) {
-                if (kk <= rg) {  // rows of N and E
+                for (int kk = 0; kk < kC / 16; ++kk) {
+                    if (kk > rg) break;  // rows of N and E
                     Af<2> fn, fe;
 #pragma unroll
                     for (int p = 0; p < 2; ++p) {
@@ -1302,13 +1351,16 @@ __global__ void __launch_bounds__(288) planes_grad_k(DArgs a, float* group, cons
                     for (int p = 0; p < NT / 2; ++p) {
                         uint32_t bk[4];
                         ld_b128<true>(bk, sK, n0 + 16 * p, 16 * kk);
-                        mma_pair(aq[2 * p], aq[2 * p + 1], fn.r[1], bk);
-                        mma_pair(ar[2 * p], ar[2 * p + 1], fe.r[1], bk);
-                        mma_pair(aq[2 * p], aq[2 * p + 1], fn.r[0], bk);
-                        mma_pair(ar[2 * p], ar[2 * p + 1], fe.r[0], bk);
+                        mma_pair(x[2 * p], x[2 * p + 1], fn.r[1], bk);
+                        mma_pair(y[2 * p], y[2 * p + 1], fe.r[1], bk);
+                        mma_pair(x[2 * p], x[2 * p + 1], fn.r[0], bk);
+                        mma_pair(y[2 * p], y[2 * p + 1], fe.r[0], bk);
                     }
                 }
-                if (kk >= rg) {  // columns of N and E
+            } else {
+#pragma unroll
+                for (int kk = 0; kk < kC / 16; ++kk) {
+                    if (kk < rg) continue;  // columns of N and E
                     Af<2> fn, fe;
 #pragma unroll
                     for (int p = 0; p < 2; ++p) {
@@ -1317,26 +1369,29 @@ __global__ void __launch_bounds__(288) planes_grad_k(DArgs a, float* group, cons
                     }
 #pragma unroll
                     for (int p = 0; p < NT / 2; ++p) {
-                        mm128<2, true>(aw[2 * p], aw[2 * p + 1], fn, sQ, n0 + 16 * p, 16 * kk);
-                        mm128<2, true>(aw[2 * p], aw[2 * p + 1], fe, sK, n0 + 16 * p, 16 * kk);
+                        mm128<2, true>(x[2 * p], x[2 * p + 1], fn, sQ, n0 + 16 * p, 16 * kk);
+                        mm128<2, true>(x[2 * p], x[2 * p + 1], fe, sK, n0 + 16 * p, 16 * kk);
                     }
                 }
             }
-            float dot[2] = {};
+            float dot[2] = {};  // q.dQ + k.dK_read, or -k.dK_write
 #pragma unroll
             for (int j = 0; j < NT; ++j) {
                 const int col = n0 + 8 * j + 2 * L.t;
 #pragma unroll
                 for (int i = 0; i < 2; ++i) {
                     const int o = at128(i ? r1 : r0, col);
-                    const float2 qv = unpack_bf16(*reinterpret_cast<const uint32_t*>(sQ + o));
                     const float2 kv = unpack_bf16(*reinterpret_cast<const uint32_t*>(sK + o));
-                    dot[i] = fmaf(qv.x, aq[j][2 * i], dot[i]);
-                    dot[i] = fmaf(qv.y, aq[j][2 * i + 1], dot[i]);
-                    dot[i] = fmaf(kv.x, ar[j][2 * i] - aw[j][2 * i], dot[i]);
-                    dot[i] = fmaf(kv.y, ar[j][2 * i + 1] - aw[j][2 * i + 1], dot[i]);
-                    ar[j][2 * i] += aw[j][2 * i];  // dK
-                    ar[j][2 * i + 1] += aw[j][2 * i + 1];
+                    if (writer) {
+                        dot[i] = fmaf(-kv.x, x[j][2 * i], dot[i]);
+                        dot[i] = fmaf(-kv.y, x[j][2 * i + 1], dot[i]);
+                    } else {
+                        const float2 qv = unpack_bf16(*reinterpret_cast<const uint32_t*>(sQ + o));
+                        dot[i] = fmaf(qv.x, x[j][2 * i], dot[i]);
+                        dot[i] = fmaf(qv.y, x[j][2 * i + 1], dot[i]);
+                        dot[i] = fmaf(kv.x, y[j][2 * i], dot[i]);
+                        dot[i] = fmaf(kv.y, y[j][2 * i + 1], dot[i]);
+                    }
                 }
             }
 #pragma unroll
@@ -1345,44 +1400,56 @@ __global__ void __launch_bounds__(288) planes_grad_k(DArgs a, float* group, cons
                 dot[1] += __shfl_xor_sync(0xffffffffu, dot[1], o);
             }
             if (L.t == 0) {
-                sDot[half * kC + r0] = dot[0];
-                sDot[half * kC + r1] = dot[1];
+                sDot[(2 * writer + half) * kC + r0] = dot[0];
+                sDot[(2 * writer + half) * kC + r1] = dot[1];
             }
-            if (rep > 1) {  // the sum over the value heads of this key head; each thread its own elements
-                float* gq = group + ((static_cast<int64_t>(b) * a.Hk + hk) * a.n + c) * 2 * kC * KD;
-                float* gk = gq + kC * KD;
+            sync_compute();  // N and E are done with
+            float4* mine = reinterpret_cast<float4*>(sW) + ((rg * 2 + half) * NT) * 32 + L.l;
+            if (writer) {
 #pragma unroll
-                for (int j = 0; j < NT; ++j)
-#pragma unroll
-                    for (int i = 0; i < 2; ++i) {
-                        const int o = (i ? r1 : r0) * KD + n0 + 8 * j + 2 * L.t;
-                        float2 x = make_float2(aq[j][2 * i], aq[j][2 * i + 1]), y = make_float2(ar[j][2 * i], ar[j][2 * i + 1]);
-                        if (h > hk * rep) {
-                            const float2 p = *reinterpret_cast<const float2*>(gq + o), q = *reinterpret_cast<const float2*>(gk + o);
-                            x.x += p.x; x.y += p.y; y.x += q.x; y.y += q.y;
-                        }
-                        *reinterpret_cast<float2*>(gq + o) = x;
-                        *reinterpret_cast<float2*>(gk + o) = y;
-                        aq[j][2 * i] = x.x; aq[j][2 * i + 1] = x.y;
-                        ar[j][2 * i] = y.x; ar[j][2 * i + 1] = y.y;
-                    }
-            }
-            if (h == (hk + 1) * rep - 1) {
-                rows_out<NT>(aq, dq, qst, m0, rows, all, n0, a.K, L);
-                rows_out<NT>(ar, dk, qst, m0, rows, all, n0, a.K, L);
+                for (int j = 0; j < NT; ++j) mine[j * 32] = make_float4(x[j][0], x[j][1], x[j][2], x[j][3]);
             }
             sync_compute();
-            if (warp == 0) {
-                float tot = 0.f, w = 0.f;
+            if (!writer) {
 #pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    tot += sTot[i];
-                    w += sTot[8 + i];
+                for (int j = 0; j < NT; ++j) {
+                    const float4 w = mine[j * 32];
+                    y[j][0] += w.x;
+                    y[j][1] += w.y;
+                    y[j][2] += w.z;
+                    y[j][3] += w.w;
                 }
-                tot = fmaf(gc, tot, w);  // <S1, dS1>
+                if (rep > 1) {  // the sum over the value heads of this key head; each thread its own elements
+                    float* gq = group + static_cast<int64_t>(it) * 2 * kC * KD;
+                    float* gk = gq + kC * KD;
+#pragma unroll
+                    for (int j = 0; j < NT; ++j)
+#pragma unroll
+                        for (int i = 0; i < 2; ++i) {
+                            const int o = (i ? r1 : r0) * KD + n0 + 8 * j + 2 * L.t;
+                            if (h > hk * rep) {
+                                const float2 p = *reinterpret_cast<const float2*>(gq + o), q = *reinterpret_cast<const float2*>(gk + o);
+                                x[j][2 * i] += p.x;
+                                x[j][2 * i + 1] += p.y;
+                                y[j][2 * i] += q.x;
+                                y[j][2 * i + 1] += q.y;
+                            }
+                            if (h < (hk + 1) * rep - 1) {
+                                *reinterpret_cast<float2*>(gq + o) = make_float2(x[j][2 * i], x[j][2 * i + 1]);
+                                *reinterpret_cast<float2*>(gk + o) = make_float2(y[j][2 * i], y[j][2 * i + 1]);
+                            }
+                        }
+                }
+                if (h == (hk + 1) * rep - 1) {
+                    rows_out<NT>(x, dq, qst, m0, rows, all, n0, a.K, L);
+                    rows_out<NT>(y, dk, qst, m0, rows, all, n0, a.K, L);
+                }
+            } else if (warp == 8) {
+                float tot = L.l < kGradWarps ? gc * sTot[L.l] + sTot[kGradWarps + L.l] : 0.f;
+                tot = warp_sum(tot);  // <S1, dS1>
                 const int i0 = 2 * L.l;
-                const float y1 = sDot[i0 + 1] + sDot[kC + i0 + 1];
-                const float y0 = sDot[i0] + sDot[kC + i0] + y1;
+                const float y1 = (sDot[i0 + 1] + sDot[kC + i0 + 1]) + (sDot[2 * kC + i0 + 1] + sDot[3 * kC + i0 + 1]);
+                const float y0 = (sDot[i0] + sDot[kC + i0]) + (sDot[2 * kC + i0] + sDot[3 * kC + i0]) + y1;
                 float run = y0;  // sums from here to the end
 #pragma unroll
                 for (int o = 1; o < 32; o <<= 1) {
@@ -1393,14 +1460,14 @@ __global__ void __launch_bounds__(288) planes_grad_k(DArgs a, float* group, cons
                 const int64_t o = (row0 + i0) * a.Hv + h;
                 if (i0 < all) {
                     gate_store(a.dg, a.gate_dtype, o, i0 < rows ? y0 + behind : 0.f);
-                    gate_store(a.dbeta, a.gate_dtype, o, i0 < rows ? sDb[i0] + sDb[kC + i0] : 0.f);
+                    gate_store(a.dbeta, a.gate_dtype, o, i0 < rows ? sDb[i0] : 0.f);
                 }
                 if (i0 + 1 < all) {
                     gate_store(a.dg, a.gate_dtype, o + a.Hv, i0 + 1 < rows ? y1 + behind : 0.f);
-                    gate_store(a.dbeta, a.gate_dtype, o + a.Hv, i0 + 1 < rows ? sDb[i0 + 1] + sDb[kC + i0 + 1] : 0.f);
+                    gate_store(a.dbeta, a.gate_dtype, o + a.Hv, i0 + 1 < rows ? sDb[i0 + 1] : 0.f);
                 }
             }
-            sync_compute();  // the sums and N, E are free again
+            sync_compute();  // the sums and dK_write have been read
         }
         warp_arrive(&qempty[seen & 1]);
         ++seen;
@@ -1509,8 +1576,8 @@ cudaError_t bwd(const DArgs& a, float* group, cudaStream_t s) {
     Maps m{};
     if (!make_maps(a, m)) return cudaErrorInvalidValue;
     PLANES_TRY(chain<KD>(a, m, true, s));
-    const int64_t items = static_cast<int64_t>(a.B) * a.Hk * a.n;
-    planes_grad_k<KD><<<static_cast<unsigned>(items < kSms ? items : kSms), 288, Grad<KD>::bytes, s>>>(a, group, m);
+    const int items = a.B * a.Hk * a.n;
+    planes_grad_k<KD><<<items < kSms ? items : kSms, 32 * kGradWarps, Grad<KD>::bytes, s>>>(a, group, m);
     note_launch();
     return cudaGetLastError();
 }
