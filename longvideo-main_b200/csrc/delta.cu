@@ -1127,6 +1127,7 @@ DArgs make_args(const EacsDelta& p) {
     a.K = static_cast<int>(p.K); a.V = static_cast<int>(p.V);
     a.n = static_cast<int>(chunks(p.L)); a.Vp = static_cast<int>(pad16(p.V));
     a.gate_dtype = p.gate_dtype;
+    a.half = p.dtype == EACS_DTYPE_F16;
     a.vec_qk = rows16(p, p.q, p.q_stride, p.Hk, p.K) && rows16(p, p.k, p.k_stride, p.Hk, p.K);
     a.vec_v = rows16(p, p.v, p.v_stride, p.Hv, p.V);
     a.scale = p.scale;
@@ -1140,11 +1141,11 @@ bool mapped(int64_t B, int64_t L, int64_t H, const int64_t* st) {
         if (n[i] > 1 && (st[i] <= 0 || st[i] >= int64_t{1} << 39)) return false;
     return true;
 }
-// Whether the bfloat16 kernels take these inputs.  The backward goes by the forward's inputs alone, as it
+// Whether the 16-bit kernels take these inputs.  The backward goes by the forward's inputs alone, as it
 // reads what the forward left (an upstream gradient in another layout is
 // refused by delta_bwd then).
 bool planes(const EacsDelta& p, const DArgs& a) {
-    return p.dtype == EACS_DTYPE_BF16 && a.vec_qk && a.vec_v && mapped(p.B, p.L, p.Hk, p.q_stride) &&
+    return p.dtype != EACS_DTYPE_F32 && a.vec_qk && a.vec_v && mapped(p.B, p.L, p.Hk, p.q_stride) &&
            mapped(p.B, p.L, p.Hk, p.k_stride) && mapped(p.B, p.L, p.Hv, p.v_stride);
 }
 

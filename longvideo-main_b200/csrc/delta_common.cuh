@@ -37,6 +37,12 @@ __device__ __forceinline__ void mma_bf16(float* c, const uint32_t* a, uint32_t b
                  : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
                  : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
+__device__ __forceinline__ void mma_f16(float* c, const uint32_t* a, uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
+                 "{%0,%1,%2,%3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
 __device__ __forceinline__ void mma_tf32(float* c, const uint32_t* a, uint32_t b0, uint32_t b1) {
     asm volatile("mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
                  "{%0,%1,%2,%3};"
@@ -172,6 +178,7 @@ struct DArgs {
     float* dinitial;       // or null
     int B, L, Hk, Hv, K, V, n, Vp;  // n chunks, Vp = V rounded up to 16
     int gate_dtype;
+    int half;  // q, k, v: float16 (delta_planes.cu)
     int vec_qk, vec_v, vec_do;  // rows can be read 16 bytes at a time
     float scale;
     // workspace, per chunk id ((b Hv + h) n + c)
@@ -237,7 +244,7 @@ template <> __device__ __forceinline__ void load8<__nv_bfloat16>(const __nv_bflo
 
 
 
-// delta_planes.cu: bfloat16 inputs whose rows start on 16 bytes
+// delta_planes.cu: bfloat16 and float16 inputs whose rows start on 16 bytes
 size_t planes_saved_size(const DArgs& a, bool training);
 size_t planes_bwd_size(const DArgs& a);
 cudaError_t planes_fwd(DArgs a, void* ws, bool training, cudaStream_t s);

@@ -27,7 +27,7 @@
 namespace eacs {
 namespace {
 
-using bf16 = __nv_bfloat16;
+using e16 = uint16_t;  // a bfloat16 or float16 as it lies in memory
 
 // ----------------------------------------------------------------------------
 // barriers and bulk copies
@@ -63,34 +63,50 @@ __device__ __forceinline__ void warp_arrive(uint64_t* bar) {
 // ----------------------------------------------------------------------------
 // operands
 // ----------------------------------------------------------------------------
+// What the products are made of: pairs of a type, and its matrix instruction.
+template <typename T> struct Num;
+template <> struct Num<__nv_bfloat16> {
+    static __device__ __forceinline__ uint32_t pack(float lo, float hi) { return pack_bf16(lo, hi); }
+    static __device__ __forceinline__ float2 unpack(uint32_t v) { return unpack_bf16(v); }
+    static __device__ __forceinline__ void mma(float* c, const uint32_t* a, uint32_t b0, uint32_t b1) { mma_bf16(c, a, b0, b1); }
+};
+template <> struct Num<__half> {
+    static __device__ __forceinline__ uint32_t pack(float lo, float hi) {
+        const __half2 p = __floats2half2_rn(lo, hi);
+        return *reinterpret_cast<const uint32_t*>(&p);
+    }
+    static __device__ __forceinline__ float2 unpack(uint32_t v) { return __half22float2(*reinterpret_cast<const __half2*>(&v)); }
+    static __device__ __forceinline__ void mma(float* c, const uint32_t* a, uint32_t b0, uint32_t b1) { mma_f16(c, a, b0, b1); }
+};
+
 template <int P> struct Af { uint32_t r[P][4]; };  // 16 x 16 of A in P planes
 
-template <int P>
+template <typename T, int P>
 __device__ __forceinline__ Af<P> from_acc(const float* c0, const float* c1) {
     Af<P> a;
     const float v[8] = {c0[0], c0[1], c0[2], c0[3], c1[0], c1[1], c1[2], c1[3]};
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-        a.r[0][i] = pack_bf16(v[2 * i], v[2 * i + 1]);
+        a.r[0][i] = Num<T>::pack(v[2 * i], v[2 * i + 1]);
         if constexpr (P == 2) {
-            const float2 h = unpack_bf16(a.r[0][i]);
-            a.r[1][i] = pack_bf16(v[2 * i] - h.x, v[2 * i + 1] - h.y);
+            const float2 h = Num<T>::unpack(a.r[0][i]);
+            a.r[1][i] = Num<T>::pack(v[2 * i] - h.x, v[2 * i + 1] - h.y);
         }
     }
     return a;
 }
 // of a tile stored [m][k], and stored [k][m]
-__device__ __forceinline__ void ld_a(uint32_t* r, const bf16* s, int ld, int m0, int k0) {
+__device__ __forceinline__ void ld_a(uint32_t* r, const e16* s, int ld, int m0, int k0) {
     const int l = threadIdx.x & 31;
     ldsm4(r, s + (m0 + (l & 15)) * ld + k0 + (l >> 4) * 8);
 }
-__device__ __forceinline__ void ld_at(uint32_t* r, const bf16* s, int ld, int m0, int k0) {
+__device__ __forceinline__ void ld_at(uint32_t* r, const e16* s, int ld, int m0, int k0) {
     const int l = threadIdx.x & 31;
     ldsm4t(r, s + (k0 + (l & 7) + ((l >> 4) & 1) * 8) * ld + m0 + ((l >> 3) & 1) * 8);
 }
 // 16 columns of B by 16 of the summed index, stored [n][k], and (TR) [k][n]
 template <bool TR>
-__device__ __forceinline__ void ld_b(uint32_t* b, const bf16* s, int ld, int n0, int k0) {
+__device__ __forceinline__ void ld_b(uint32_t* b, const e16* s, int ld, int n0, int k0) {
     const int l = threadIdx.x & 31;
     if constexpr (TR) ldsm4t(b, s + (k0 + (l & 7) + ((l >> 3) & 1) * 8) * ld + n0 + ((l >> 4) & 1) * 8);
     else ldsm4(b, s + (n0 + (l & 7) + ((l >> 4) & 1) * 8) * ld + k0 + ((l >> 3) & 1) * 8);
@@ -104,47 +120,48 @@ __device__ __forceinline__ int at128(int row, int col) {
 __device__ __forceinline__ int at32(int row, int col) { return row * 16 + (((col >> 3) ^ ((row >> 2) & 1)) << 3); }
 
 template <bool TR>
-__device__ __forceinline__ void ld_b128(uint32_t* b, const bf16* s, int n0, int k0) {
+__device__ __forceinline__ void ld_b128(uint32_t* b, const e16* s, int n0, int k0) {
     const int l = threadIdx.x & 31;
     if constexpr (TR) ldsm4t(b, s + at128(k0 + (l & 7) + ((l >> 3) & 1) * 8, n0 + ((l >> 4) & 1) * 8));
     else ldsm4(b, s + at128(n0 + (l & 7) + ((l >> 4) & 1) * 8, k0 + ((l >> 3) & 1) * 8));
 }
 // 16 rows of A: tokens m0.. of a group, and (at) its 16 columns by tokens k0..
-__device__ __forceinline__ void ld_a32(uint32_t* r, const bf16* s, int m0) {
+__device__ __forceinline__ void ld_a32(uint32_t* r, const e16* s, int m0) {
     const int l = threadIdx.x & 31;
     ldsm4(r, s + at32(m0 + (l & 15), (l >> 4) * 8));
 }
-__device__ __forceinline__ void ld_at32(uint32_t* r, const bf16* s, int k0) {
+__device__ __forceinline__ void ld_at32(uint32_t* r, const e16* s, int k0) {
     const int l = threadIdx.x & 31;
     ldsm4t(r, s + at32(k0 + (l & 7) + ((l >> 4) & 1) * 8, ((l >> 3) & 1) * 8));
 }
+template <typename T>
 __device__ __forceinline__ void mma_pair(float* c0, float* c1, const uint32_t* a, const uint32_t* b) {
-    mma_bf16(c0, a, b[0], b[1]);
-    mma_bf16(c1, a, b[2], b[3]);
+    Num<T>::mma(c0, a, b[0], b[1]);
+    Num<T>::mma(c1, a, b[2], b[3]);
 }
 // A in P planes times one plane of B
-template <int P, bool TR>
-__device__ __forceinline__ void mm(float* c0, float* c1, const Af<P>& a, const bf16* s, int ld, int n0, int k0) {
+template <typename T, int P, bool TR>
+__device__ __forceinline__ void mm(float* c0, float* c1, const Af<P>& a, const e16* s, int ld, int n0, int k0) {
     uint32_t b[4];
     ld_b<TR>(b, s, ld, n0, k0);
 #pragma unroll
-    for (int p = P - 1; p >= 0; --p) mma_pair(c0, c1, a.r[p], b);
+    for (int p = P - 1; p >= 0; --p) mma_pair<T>(c0, c1, a.r[p], b);
 }
-template <int P, bool TR>
-__device__ __forceinline__ void mm128(float* c0, float* c1, const Af<P>& a, const bf16* s, int n0, int k0) {
+template <typename T, int P, bool TR>
+__device__ __forceinline__ void mm128(float* c0, float* c1, const Af<P>& a, const e16* s, int n0, int k0) {
     uint32_t b[4];
     ld_b128<TR>(b, s, n0, k0);
 #pragma unroll
-    for (int p = P - 1; p >= 0; --p) mma_pair(c0, c1, a.r[p], b);
+    for (int p = P - 1; p >= 0; --p) mma_pair<T>(c0, c1, a.r[p], b);
 }
 // A in P planes times B in two (the product of the low planes is left out)
-template <int P, bool TR>
-__device__ __forceinline__ void mm_hl(float* c0, float* c1, const Af<P>& a, const bf16* hi, const bf16* lo, int ld,
+template <typename T, int P, bool TR>
+__device__ __forceinline__ void mm_hl(float* c0, float* c1, const Af<P>& a, const e16* hi, const e16* lo, int ld,
                                       int n0, int k0) {
     uint32_t b[4];
     ld_b<TR>(b, lo, ld, n0, k0);
-    mma_pair(c0, c1, a.r[0], b);
-    mm<P, TR>(c0, c1, a, hi, ld, n0, k0);
+    mma_pair<T>(c0, c1, a.r[0], b);
+    mm<T, P, TR>(c0, c1, a, hi, ld, n0, k0);
 }
 // Steps 0..N-1 of a product: a step's tiles of B (up to four pairs) are read
 // while the step before is multiplied.
@@ -165,16 +182,16 @@ __device__ __forceinline__ void steps(Read read, Use use) {
 }
 // accumulators j0.. of `n` pairs += A (planes P-1 .. 0) B, plane by plane: eight
 // products lie between two that add to the same accumulator
-template <int P>
+template <typename T, int P>
 __device__ __forceinline__ void mma_step(float (*c)[4], const Af<P>& a, const uint32_t (*b)[4], int from = 0, int to = 4) {
 #pragma unroll
     for (int p = P - 1; p >= 0; --p)
 #pragma unroll
         for (int i = 0; i < 4; ++i)
-            if (i >= from && i < to) mma_pair(c[2 * i], c[2 * i + 1], a.r[p], b[i]);
+            if (i >= from && i < to) mma_pair<T>(c[2 * i], c[2 * i + 1], a.r[p], b[i]);
 }
 // accumulators of 16 rows by 16 columns to a tile [row][col] (as ld_a reads it)
-__device__ __forceinline__ void st_tile(bf16* s, int ld, int c0, const uint32_t* r) {
+__device__ __forceinline__ void st_tile(e16* s, int ld, int c0, const uint32_t* r) {
     const int l = threadIdx.x & 31;
     asm volatile("stmatrix.sync.aligned.m8n8.x4.shared.b16 [%0], {%1,%2,%3,%4};" ::"r"(
                      smem_u32(s + (l & 15) * ld + c0 + (l >> 4) * 8)),
@@ -182,7 +199,7 @@ __device__ __forceinline__ void st_tile(bf16* s, int ld, int c0, const uint32_t*
                  : "memory");
 }
 // and to a tile [col][row]
-__device__ __forceinline__ void st_tile_t(bf16* s, int ld, int c0, const uint32_t* r) {
+__device__ __forceinline__ void st_tile_t(e16* s, int ld, int c0, const uint32_t* r) {
     const int l = threadIdx.x & 31;
     asm volatile("stmatrix.sync.aligned.m8n8.x4.trans.shared.b16 [%0], {%1,%2,%3,%4};" ::"r"(
                      smem_u32(s + (c0 + (l & 7) + (l >> 4) * 8) * ld + ((l >> 3) & 1) * 8)),
@@ -206,7 +223,7 @@ struct Maps { CUtensorMap q, k, v, d; };
 // of one warp.  (Rows of a padded batch behind a sequence's end: what they hold,
 // NaN as it may be, is not to reach a product.  Behind L the copy itself gives 0.)
 template <int W>
-__device__ __forceinline__ void zero_rows(bf16* s, int boxes, int rows) {
+__device__ __forceinline__ void zero_rows(e16* s, int boxes, int rows) {
     const int per = (kC - rows) * (W / 8);
     for (int i = threadIdx.x & 31; i < boxes * per; i += 32)
         *reinterpret_cast<uint4*>(s + (i / per) * kC * W + rows * W + (i % per) * 8) = make_uint4(0, 0, 0, 0);
@@ -229,7 +246,7 @@ __device__ __forceinline__ float ratio(const float* G, int i, int j) {
 // parts.  (Forward substitution alone takes 2016 dependent multiply-adds.)
 constexpr int kAld = kC + 8;  // float32 tiles
 
-template <int KD>
+template <typename T, int KD>
 __global__ void __launch_bounds__(128) planes_prep_k(DArgs a) {
     using F = FmtF<false>;
     const int c = blockIdx.x, h = blockIdx.y, b = blockIdx.z;
@@ -241,8 +258,8 @@ __global__ void __launch_bounds__(128) planes_prep_k(DArgs a) {
     extern __shared__ __align__(128) unsigned char smem_raw[];
     unsigned char* smem = smem_raw;
     constexpr int LD = KD + 8;
-    bf16* sK = reinterpret_cast<bf16*>(smem);
-    bf16* sQ = sK + kC * LD;
+    e16* sK = reinterpret_cast<e16*>(smem);
+    e16* sQ = sK + kC * LD;
     float* sA = reinterpret_cast<float*>(sQ + kC * LD);  // A, lower triangle
     float* sT = sA + kC * kAld;                          // its inverse
     float* sY = reinterpret_cast<float*>(smem);          // a product (K and Q are done with by then)
@@ -250,8 +267,8 @@ __global__ void __launch_bounds__(128) planes_prep_k(DArgs a) {
     const int tid = threadIdx.x, warp = tid >> 5;
     const Lane L;
     {
-        const bf16* k = static_cast<const bf16*>(a.k) + b * a.sk.b + t0 * a.sk.t + hk * a.sk.h;
-        const bf16* q = static_cast<const bf16*>(a.q) + b * a.sq.b + t0 * a.sq.t + hk * a.sq.h;
+        const e16* k = static_cast<const e16*>(a.k) + b * a.sk.b + t0 * a.sk.t + hk * a.sk.h;
+        const e16* q = static_cast<const e16*>(a.q) + b * a.sq.b + t0 * a.sq.t + hk * a.sq.h;
         for (int i = tid; i < kC * (KD / 8); i += 128) {
             const int r = i / (KD / 8), col = (i % (KD / 8)) * 8;
             const bool in = r < rows && col < a.K;
@@ -313,11 +330,11 @@ __global__ void __launch_bounds__(128) planes_prep_k(DArgs a) {
                 if (p <= warp) {
                     uint32_t bk[4];
                     ld_b<false>(bk, sK, LD, 16 * p, k0);
-                    mma_pair(kk[2 * p], kk[2 * p + 1], ak.r[0], bk);
-                    mma_pair(qk[2 * p], qk[2 * p + 1], aq.r[0], bk);
+                    mma_pair<T>(kk[2 * p], kk[2 * p + 1], ak.r[0], bk);
+                    mma_pair<T>(qk[2 * p], qk[2 * p + 1], aq.r[0], bk);
                 }
         }
-        bf16* M = static_cast<bf16*>(a.M) + id * 2 * kCC;
+        e16* M = static_cast<e16*>(a.M) + id * 2 * kCC;
 #pragma unroll
         for (int j = 0; j < kC / 8; ++j) {
             float m[4] = {};
@@ -331,11 +348,11 @@ __global__ void __launch_bounds__(128) planes_prep_k(DArgs a) {
                 }
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
-                const uint32_t hi = pack_bf16(m[2 * e], m[2 * e + 1]);
-                const float2 f = unpack_bf16(hi);
+                const uint32_t hi = Num<T>::pack(m[2 * e], m[2 * e + 1]);
+                const float2 f = Num<T>::unpack(hi);
                 const int o = (m0 + L.g + 8 * e) * kTld + 8 * j + 2 * L.t;
                 *reinterpret_cast<uint32_t*>(M + o) = hi;
-                *reinterpret_cast<uint32_t*>(M + kCC + o) = pack_bf16(m[2 * e] - f.x, m[2 * e + 1] - f.y);
+                *reinterpret_cast<uint32_t*>(M + kCC + o) = Num<T>::pack(m[2 * e] - f.x, m[2 * e + 1] - f.y);
             }
         }
     }
@@ -393,7 +410,7 @@ __global__ void __launch_bounds__(128) planes_prep_k(DArgs a) {
         put(sT, r, col, z0, z1, -1.f);
     }
     __syncthreads();
-    bf16* T = static_cast<bf16*>(a.T) + id * 2 * kCC;
+    e16* to = static_cast<e16*>(a.T) + id * 2 * kCC;
     for (int i = tid; i < kC * 8; i += 128) {
         const int r = i >> 3, c8 = (i & 7) * 8;
         uint32_t hi[4], lo[4];
@@ -401,12 +418,12 @@ __global__ void __launch_bounds__(128) planes_prep_k(DArgs a) {
         for (int e = 0; e < 4; ++e) {
             const float x = sT[r * kAld + c8 + 2 * e] * sB[c8 + 2 * e];
             const float y = sT[r * kAld + c8 + 2 * e + 1] * sB[c8 + 2 * e + 1];
-            hi[e] = pack_bf16(x, y);
-            const float2 f = unpack_bf16(hi[e]);
-            lo[e] = pack_bf16(x - f.x, y - f.y);
+            hi[e] = Num<T>::pack(x, y);
+            const float2 f = Num<T>::unpack(hi[e]);
+            lo[e] = Num<T>::pack(x - f.x, y - f.y);
         }
-        *reinterpret_cast<uint4*>(T + r * kTld + c8) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
-        *reinterpret_cast<uint4*>(T + kCC + r * kTld + c8) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+        *reinterpret_cast<uint4*>(to + r * kTld + c8) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+        *reinterpret_cast<uint4*>(to + kCC + r * kTld + c8) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
     }
 }
 
@@ -449,7 +466,7 @@ __device__ __forceinline__ void state_store(const float (*S)[4], float* p, int K
         }
 }
 
-template <int KD, int G>
+template <typename T, int KD, int G>
 __global__ void __launch_bounds__(Fwd<KD, G>::kWarps * 32) planes_chain_k(DArgs a, const __grid_constant__ Maps maps) {
     using Sm = Fwd<KD, G>;
     const int h = blockIdx.y, b = blockIdx.z, hk = h / (a.Hv / a.Hk);
@@ -477,7 +494,7 @@ __global__ void __launch_bounds__(Fwd<KD, G>::kWarps * 32) planes_chain_k(DArgs 
     if (warp == Sm::kWarps - 1) {
         // ---- loads ----
         for (int c = 0; c < nc && ok; ++c) {
-            bf16* e = reinterpret_cast<bf16*>(smem + (c & 1) * Sm::kStage);
+            e16* e = reinterpret_cast<e16*>(smem + (c & 1) * Sm::kStage);
             const int t0 = c * kC, rows = min(kC, len - t0);
             const bool tail = rows < min(kC, a.L - t0);
             uint64_t* bar = tail ? land : &full[c & 1];
@@ -487,13 +504,13 @@ __global__ void __launch_bounds__(Fwd<KD, G>::kWarps * 32) planes_chain_k(DArgs 
                 mbar_expect_tx(bar, Sm::kLoad);
 #pragma unroll
                 for (int x = 0; x < KD; x += 64) tma_load(e + Sm::kK + x * kC, &maps.k, bar, x, t0, hk, b);
-                bulk_load(e + Sm::kT, static_cast<const bf16*>(a.T) + id * 2 * kCC, 4 * kCC, bar);
+                bulk_load(e + Sm::kT, static_cast<const e16*>(a.T) + id * 2 * kCC, 4 * kCC, bar);
 #pragma unroll
                 for (int g = 0; g < G; ++g) tma_load(e + Sm::kV + g * kC * 16, &maps.v, bar, vb + 16 * g, t0, h, b);
                 bulk_load(e + Sm::kGa, a.gates + id * kGates, kGates * 4, bar);
 #pragma unroll
                 for (int x = 0; x < KD; x += 64) tma_load(e + Sm::kQ + x * kC, &maps.q, bar, x, t0, hk, b);
-                bulk_load(e + Sm::kM, static_cast<const bf16*>(a.M) + id * 2 * kCC, 4 * kCC, bar);
+                bulk_load(e + Sm::kM, static_cast<const e16*>(a.M) + id * 2 * kCC, 4 * kCC, bar);
             }
             __syncwarp();
             if (tail) {
@@ -509,13 +526,13 @@ __global__ void __launch_bounds__(Fwd<KD, G>::kWarps * 32) planes_chain_k(DArgs 
         // ---- a state of 16 value columns ----
         const int v0 = vb + warp * 16;
         const bool on = v0 < a.Vp;
-        bf16* mine = reinterpret_cast<bf16*>(smem + 2 * Sm::kStage + warp * Sm::kGroup);
-        bf16 *sS = mine + Sm::kS, *sU = mine + Sm::kU;
+        e16* mine = reinterpret_cast<e16*>(smem + 2 * Sm::kStage + warp * Sm::kGroup);
+        e16 *sS = mine + Sm::kS, *sU = mine + Sm::kU;
         float S[KD / 8][4];
         state_load<KD>(S, a.initial ? a.initial + head * a.K * a.V : nullptr, a.K, a.V, v0, L);
         for (int c = 0; c < nc && ok; ++c) {
             const unsigned char* st = smem + (c & 1) * Sm::kStage;
-            const bf16* e = reinterpret_cast<const bf16*>(st);
+            const e16* e = reinterpret_cast<const e16*>(st);
             const float* ga = reinterpret_cast<const float*>(e + Sm::kGa);
             const float *gam = ga + 2 * kC, *dec = ga + 3 * kC;
             const int64_t id = head * a.n + c;
@@ -534,15 +551,15 @@ __global__ void __launch_bounds__(Fwd<KD, G>::kWarps * 32) planes_chain_k(DArgs 
                         for (int p = 0; p < 4; ++p) ld_b128<false>(f[p], e + Sm::kK, 16 * p, 16 * i);
                     },
                     [&](int i, const uint32_t(*f)[4]) {
-                        const Af<2> af = from_acc<2>(S[2 * i], S[2 * i + 1]);
+                        const Af<2> af = from_acc<T, 2>(S[2 * i], S[2 * i + 1]);
                         st_tile(sS, Sm::LDK, 16 * i, af.r[0]);
                         if (a.S) st_tile(sS + 16 * Sm::LDK, Sm::LDK, 16 * i, af.r[1]);
-                        mma_step(X, af, f);
+                        mma_step<T>(X, af, f);
                     });
                 if (a.S) fence_async();
                 warp_arrive(&s_full[warp]);
                 if (a.S && L.l == 0) {
-                    bf16* to = static_cast<bf16*>(a.S) + (id * 2 * a.Vp + v0) * Sm::LDK;
+                    e16* to = static_cast<e16*>(a.S) + (id * 2 * a.Vp + v0) * Sm::LDK;
                     bulk_store(to, sS, 32 * Sm::LDK);
                     bulk_store(to + static_cast<int64_t>(a.Vp) * Sm::LDK, sS + 16 * Sm::LDK, 32 * Sm::LDK);
                     bulk_commit();
@@ -556,7 +573,7 @@ __global__ void __launch_bounds__(Fwd<KD, G>::kWarps * 32) planes_chain_k(DArgs 
                     for (int i = 0; i < 2; ++i) {
                         const float2 f = *reinterpret_cast<const float2*>(gam + 16 * p + 8 * i + 2 * L.t);
                         float* x = X[2 * p + i];
-                        const float2 lo = unpack_bf16(r[2 * i]), hi = unpack_bf16(r[2 * i + 1]);
+                        const float2 lo = Num<T>::unpack(r[2 * i]), hi = Num<T>::unpack(r[2 * i + 1]);
                         x[0] = fmaf(-f.x, x[0], lo.x);
                         x[1] = fmaf(-f.y, x[1], lo.y);
                         x[2] = fmaf(-f.x, x[2], hi.x);
@@ -575,10 +592,10 @@ __global__ void __launch_bounds__(Fwd<KD, G>::kWarps * 32) planes_chain_k(DArgs 
                         },
                         [&](int i, const uint32_t(*f)[4]) {
                             if (i & 1) {
-                                mma_step(U, af, f, i / 2);
+                                mma_step<T>(U, af, f, i / 2);
                             } else {
-                                af = from_acc<2>(X[i], X[i + 1]);
-                                mma_step(U, Af<1>{{{af.r[0][0], af.r[0][1], af.r[0][2], af.r[0][3]}}}, f, i / 2);
+                                af = from_acc<T, 2>(X[i], X[i + 1]);
+                                mma_step<T>(U, Af<1>{{{af.r[0][0], af.r[0][1], af.r[0][2], af.r[0][3]}}}, f, i / 2);
                             }
                         });
                 }
@@ -600,7 +617,7 @@ __global__ void __launch_bounds__(Fwd<KD, G>::kWarps * 32) planes_chain_k(DArgs 
                         [&](int i, const uint32_t(*f)[4]) {
                             const int kk = i / Q;
                             if (i % Q == 0) {
-                                const Af<2> au = from_acc<2>(U[2 * kk], U[2 * kk + 1]);
+                                const Af<2> au = from_acc<T, 2>(U[2 * kk], U[2 * kk + 1]);
                                 st_tile(sU, kTld, 16 * kk, au.r[0]);
                                 st_tile(sU + 16 * kTld, kTld, 16 * kk, au.r[1]);
                                 float y[2][4];
@@ -613,15 +630,15 @@ __global__ void __launch_bounds__(Fwd<KD, G>::kWarps * 32) planes_chain_k(DArgs 
                                     y[x][2] = u[2] * d.x;
                                     y[x][3] = u[3] * d.y;
                                 }
-                                af = from_acc<2>(y[0], y[1]);
+                                af = from_acc<T, 2>(y[0], y[1]);
                             }
-                            mma_step(S + 8 * (i % Q), af, f);
+                            mma_step<T>(S + 8 * (i % Q), af, f);
                         });
                 }
                 if (a.S) fence_async();
                 warp_arrive(&u_full[warp]);
                 if (a.S && L.l == 0) {
-                    bf16* to = static_cast<bf16*>(a.U) + (id * 2 * a.Vp + v0) * kTld;
+                    e16* to = static_cast<e16*>(a.U) + (id * 2 * a.Vp + v0) * kTld;
                     bulk_store(to, sU, 32 * kTld);
                     bulk_store(to + static_cast<int64_t>(a.Vp) * kTld, sU + 16 * kTld, 32 * kTld);
                     bulk_commit();
@@ -637,10 +654,10 @@ __global__ void __launch_bounds__(Fwd<KD, G>::kWarps * 32) planes_chain_k(DArgs 
     const int helper = warp - G;
     constexpr int NG = (G + Sm::H - 1) / Sm::H;
     const int64_t ost = static_cast<int64_t>(a.Hv) * a.V;
-    bf16* out = static_cast<bf16*>(a.out) + static_cast<int64_t>(b) * a.L * ost + static_cast<int64_t>(h) * a.V;
+    e16* out = static_cast<e16*>(a.out) + static_cast<int64_t>(b) * a.L * ost + static_cast<int64_t>(h) * a.V;
     for (int c = 0; c < nc && ok; ++c) {
         const unsigned char* st = smem + (c & 1) * Sm::kStage;
-        const bf16* e = reinterpret_cast<const bf16*>(st);
+        const e16* e = reinterpret_cast<const e16*>(st);
         const float* sgam = reinterpret_cast<const float*>(e + Sm::kGa) + 4 * kC;
         const int rows = min(kC, len - c * kC), all = min(kC, a.L - c * kC);
         ok = warp_wait(&full[c & 1], (c >> 1) & 1);
@@ -649,7 +666,7 @@ __global__ void __launch_bounds__(Fwd<KD, G>::kWarps * 32) planes_chain_k(DArgs 
         for (int i = 0; i < NG; ++i) {
             const int g = helper + i * Sm::H;
             if (vb + 16 * g >= a.Vp) break;
-            const bf16* sS = reinterpret_cast<const bf16*>(smem + 2 * Sm::kStage + g * Sm::kGroup) + Sm::kS;
+            const e16* sS = reinterpret_cast<const e16*>(smem + 2 * Sm::kStage + g * Sm::kGroup) + Sm::kS;
             ok = warp_wait(&s_full[g], c & 1) && ok;
             // scale gam Q S0: S in one plane (its rounding, 2^-9 of terms of any sign, against the
             // output's own: y is off by 2.2e-3 in the norm instead of 1.7e-3, for half the products)
@@ -660,7 +677,7 @@ __global__ void __launch_bounds__(Fwd<KD, G>::kWarps * 32) planes_chain_k(DArgs 
 #pragma unroll
                     for (int p = 0; p < 4; ++p) ld_b128<false>(f[p], e + Sm::kQ, 16 * p, 16 * k);
                 },
-                [&](int k, const uint32_t(*f)[4]) { mma_step(O[i], as[k & 1], f); });
+                [&](int k, const uint32_t(*f)[4]) { mma_step<T>(O[i], as[k & 1], f); });
             warp_arrive(&s_empty[g]);
 #pragma unroll
             for (int j = 0; j < kC / 8; ++j) {
@@ -675,7 +692,7 @@ __global__ void __launch_bounds__(Fwd<KD, G>::kWarps * 32) planes_chain_k(DArgs 
         for (int i = 0; i < NG; ++i) {
             const int g = helper + i * Sm::H, v0 = vb + 16 * g;
             if (v0 >= a.Vp) break;
-            bf16* theirs = reinterpret_cast<bf16*>(smem + 2 * Sm::kStage + g * Sm::kGroup);
+            e16* theirs = reinterpret_cast<e16*>(smem + 2 * Sm::kStage + g * Sm::kGroup);
             ok = warp_wait(&u_full[g], c & 1) && ok;
             Af<2> au[2];
             steps<8>(
@@ -690,15 +707,15 @@ __global__ void __launch_bounds__(Fwd<KD, G>::kWarps * 32) planes_chain_k(DArgs 
                 },
                 [&](int k, const uint32_t(*f)[4]) {
                     const Af<2>& af = au[(k / 2) & 1];
-                    if (k & 1) mma_step(O[i], af, f, k / 2);
-                    else mma_step(O[i], Af<1>{{{af.r[0][0], af.r[0][1], af.r[0][2], af.r[0][3]}}}, f, k / 2);
+                    if (k & 1) mma_step<T>(O[i], af, f, k / 2);
+                    else mma_step<T>(O[i], Af<1>{{{af.r[0][0], af.r[0][1], af.r[0][2], af.r[0][3]}}}, f, k / 2);
                 });
             warp_arrive(&u_empty[g]);
             // rows of 16 values through shared memory: 32 bytes a token, two lanes each
-            bf16* sO = theirs + Sm::kO;
+            e16* sO = theirs + Sm::kO;
 #pragma unroll
             for (int p = 0; p < kC / 16; ++p) {
-                const Af<1> o = from_acc<1>(O[i][2 * p], O[i][2 * p + 1]);
+                const Af<1> o = from_acc<T, 1>(O[i][2 * p], O[i][2 * p + 1]);
                 st_tile_t(sO, Sm::LDO, 16 * p, o.r[0]);
             }
             __syncwarp();
@@ -741,7 +758,7 @@ struct Rev {
     static constexpr size_t bytes = 1024 + kBars + 8 * (5 + 2 * G);
 };
 
-template <int KD, int G>
+template <typename T, int KD, int G>
 __global__ void __launch_bounds__(Rev<KD, G>::kWarps * 32) planes_rchain_k(DArgs a, const __grid_constant__ Maps maps) {
     using Sm = Rev<KD, G>;
     const int h = blockIdx.y, b = blockIdx.z, hk = h / (a.Hv / a.Hk);
@@ -769,7 +786,7 @@ __global__ void __launch_bounds__(Rev<KD, G>::kWarps * 32) planes_rchain_k(DArgs
     if (warp == Sm::kWarps - 1) {
         for (int i = 0; i < nc && ok; ++i) {
             const int c = nc - 1 - i;
-            bf16* e = reinterpret_cast<bf16*>(smem + (i & 1) * Sm::kStage);
+            e16* e = reinterpret_cast<e16*>(smem + (i & 1) * Sm::kStage);
             const int t0 = c * kC, rows = min(kC, len - t0);
             const bool tail = rows < min(kC, a.L - t0);
             uint64_t* bar = tail ? land : &full[i & 1];
@@ -781,9 +798,9 @@ __global__ void __launch_bounds__(Rev<KD, G>::kWarps * 32) planes_rchain_k(DArgs
                 for (int x = 0; x < KD; x += 64) tma_load(e + Sm::kK + x * kC, &maps.k, bar, x, t0, hk, b);
 #pragma unroll
                 for (int g = 0; g < G; ++g) tma_load(e + Sm::kD + g * kC * 16, &maps.d, bar, vb + 16 * g, t0, h, b);
-                bulk_load(e + Sm::kM, static_cast<const bf16*>(a.M) + id * 2 * kCC, 4 * kCC, bar);
+                bulk_load(e + Sm::kM, static_cast<const e16*>(a.M) + id * 2 * kCC, 4 * kCC, bar);
                 bulk_load(e + Sm::kGa, a.gates + id * kGates, kGates * 4, bar);
-                bulk_load(e + Sm::kT, static_cast<const bf16*>(a.T) + id * 2 * kCC, 4 * kCC, bar);
+                bulk_load(e + Sm::kT, static_cast<const e16*>(a.T) + id * 2 * kCC, 4 * kCC, bar);
 #pragma unroll
                 for (int x = 0; x < KD; x += 64) tma_load(e + Sm::kQ + x * kC, &maps.q, bar, x, t0, hk, b);
             }
@@ -802,13 +819,13 @@ __global__ void __launch_bounds__(Rev<KD, G>::kWarps * 32) planes_rchain_k(DArgs
         const int v0 = vb + warp * 16;
         const bool on = v0 < a.Vp;
         unsigned char* mine = smem + 2 * Sm::kStage + warp * Sm::kGroup;
-        bf16 *sS = reinterpret_cast<bf16*>(mine + Sm::kS), *sX = reinterpret_cast<bf16*>(mine + Sm::kX);
+        e16 *sS = reinterpret_cast<e16*>(mine + Sm::kS), *sX = reinterpret_cast<e16*>(mine + Sm::kX);
         const float4* sZ = reinterpret_cast<const float4*>(mine + Sm::kZ);
         float S[KD / 8][4];  // dS^T
         state_load<KD>(S, a.dfinal ? a.dfinal + head * a.K * a.V : nullptr, a.K, a.V, v0, L);
         for (int i = 0; i < nc && ok; ++i) {
             const int c = nc - 1 - i;
-            const bf16* e = reinterpret_cast<const bf16*>(smem + (i & 1) * Sm::kStage);
+            const e16* e = reinterpret_cast<const e16*>(smem + (i & 1) * Sm::kStage);
             const float* ga = reinterpret_cast<const float*>(e + Sm::kGa);
             const float *gam = ga + 2 * kC, *dec = ga + 3 * kC;
             const int64_t id = head * a.n + c;
@@ -823,15 +840,15 @@ __global__ void __launch_bounds__(Rev<KD, G>::kWarps * 32) planes_rchain_k(DArgs
                         for (int p = 0; p < 4; ++p) ld_b128<false>(f[p], e + Sm::kK, 16 * p, 16 * k);
                     },
                     [&](int k, const uint32_t(*f)[4]) {
-                        const Af<2> af = from_acc<2>(S[2 * k], S[2 * k + 1]);
+                        const Af<2> af = from_acc<T, 2>(S[2 * k], S[2 * k + 1]);
                         st_tile(sS, Sm::LDK, 16 * k, af.r[0]);
                         st_tile(sS + 16 * Sm::LDK, Sm::LDK, 16 * k, af.r[1]);
-                        mma_step(U, af, f);
+                        mma_step<T>(U, af, f);
                     });
                 fence_async();
                 __syncwarp();
                 if (L.l == 0) {
-                    bf16* to = static_cast<bf16*>(a.dS) + (id * 2 * a.Vp + v0) * Sm::LDK;
+                    e16* to = static_cast<e16*>(a.dS) + (id * 2 * a.Vp + v0) * Sm::LDK;
                     bulk_store(to, sS, 32 * Sm::LDK);
                     bulk_store(to + static_cast<int64_t>(a.Vp) * Sm::LDK, sS + 16 * Sm::LDK, 32 * Sm::LDK);
                     bulk_commit();
@@ -853,7 +870,7 @@ __global__ void __launch_bounds__(Rev<KD, G>::kWarps * 32) planes_rchain_k(DArgs
                             for (int p = 0; p < 4; ++p)
                                 if (p <= k / 2) ld_b<true>(f[p], e + Sm::kM + (k & 1 ? 0 : kCC), kTld, 16 * p, 16 * (k / 2));
                         },
-                        [&](int k, const uint32_t(*f)[4]) { mma_step(U, ad[(k / 2) & 1], f, 0, k / 2 + 1); });
+                        [&](int k, const uint32_t(*f)[4]) { mma_step<T>(U, ad[(k / 2) & 1], f, 0, k / 2 + 1); });
                 }
                 float X[kC / 8][4] = {};  // dV^T = dU^T T'
                 {
@@ -866,10 +883,10 @@ __global__ void __launch_bounds__(Rev<KD, G>::kWarps * 32) planes_rchain_k(DArgs
                         },
                         [&](int k, const uint32_t(*f)[4]) {
                             if (k & 1) {
-                                mma_step(X, af, f, 0, k / 2 + 1);
+                                mma_step<T>(X, af, f, 0, k / 2 + 1);
                             } else {
-                                af = from_acc<2>(U[k], U[k + 1]);
-                                mma_step(X, Af<1>{{{af.r[0][0], af.r[0][1], af.r[0][2], af.r[0][3]}}}, f, 0, k / 2 + 1);
+                                af = from_acc<T, 2>(U[k], U[k + 1]);
+                                mma_step<T>(X, Af<1>{{{af.r[0][0], af.r[0][1], af.r[0][2], af.r[0][3]}}}, f, 0, k / 2 + 1);
                             }
                         });
                 }
@@ -896,7 +913,7 @@ __global__ void __launch_bounds__(Rev<KD, G>::kWarps * 32) planes_rchain_k(DArgs
                         [&](int k, const uint32_t(*f)[4]) {
                             const int kk = k / Q;
                             if (k % Q == 0) {
-                                const Af<2> ax = from_acc<2>(X[2 * kk], X[2 * kk + 1]);
+                                const Af<2> ax = from_acc<T, 2>(X[2 * kk], X[2 * kk + 1]);
                                 st_tile(sX, kTld, 16 * kk, ax.r[0]);
                                 st_tile(sX + 16 * kTld, kTld, 16 * kk, ax.r[1]);
                                 float y[2][4];
@@ -909,15 +926,15 @@ __global__ void __launch_bounds__(Rev<KD, G>::kWarps * 32) planes_rchain_k(DArgs
                                     y[x][2] = -u[2] * d.x;
                                     y[x][3] = -u[3] * d.y;
                                 }
-                                af = from_acc<1>(y[0], y[1]);
+                                af = from_acc<T, 1>(y[0], y[1]);
                             }
-                            mma_step(S + 8 * (k % Q), af, f);
+                            mma_step<T>(S + 8 * (k % Q), af, f);
                         });
                 }
                 fence_async();
                 __syncwarp();
                 if (L.l == 0) {
-                    bf16* to = static_cast<bf16*>(a.dV) + (id * 2 * a.Vp + v0) * kTld;
+                    e16* to = static_cast<e16*>(a.dV) + (id * 2 * a.Vp + v0) * kTld;
                     bulk_store(to, sX, 32 * kTld);
                     bulk_store(to + static_cast<int64_t>(a.Vp) * kTld, sX + 16 * kTld, 32 * kTld);
                     bulk_commit();
@@ -931,7 +948,7 @@ __global__ void __launch_bounds__(Rev<KD, G>::kWarps * 32) planes_rchain_k(DArgs
     }
     // ---- (scale gam dO)^T Q of the groups ----
     for (int i = 0; i < nc && ok; ++i) {
-        const bf16* e = reinterpret_cast<const bf16*>(smem + (i & 1) * Sm::kStage);
+        const e16* e = reinterpret_cast<const e16*>(smem + (i & 1) * Sm::kStage);
         const float* sgam = reinterpret_cast<const float*>(e + Sm::kGa) + 4 * kC;
         ok = warp_wait(&full[i & 1], (i >> 1) & 1);
         for (int g = warp - G; g < G; g += Sm::H) {
@@ -953,15 +970,15 @@ __global__ void __launch_bounds__(Rev<KD, G>::kWarps * 32) planes_rchain_k(DArgs
 #pragma unroll
                         for (int x = 0; x < 2; ++x) {
                             const float2 d = *reinterpret_cast<const float2*>(sgam + 16 * kk + 8 * x + 2 * L.t);
-                            const float2 lo = unpack_bf16(r[2 * x]), hi = unpack_bf16(r[2 * x + 1]);
+                            const float2 lo = Num<T>::unpack(r[2 * x]), hi = Num<T>::unpack(r[2 * x + 1]);
                             y[x][0] = lo.x * d.x;
                             y[x][1] = lo.y * d.y;
                             y[x][2] = hi.x * d.x;
                             y[x][3] = hi.y * d.y;
                         }
-                        af = from_acc<2>(y[0], y[1]);
+                        af = from_acc<T, 2>(y[0], y[1]);
                     }
-                    mma_step(Z + 8 * (k % Q), af, f);
+                    mma_step<T>(Z + 8 * (k % Q), af, f);
                 });
             float4* sZ = reinterpret_cast<float4*>(smem + 2 * Sm::kStage + g * Sm::kGroup + Sm::kZ);
             ok = warp_wait(&z_empty[g], (i & 1) ^ 1) && ok;
@@ -1003,16 +1020,17 @@ struct Grad {
 
 __device__ __forceinline__ void sync_compute() { __syncthreads(); }
 
-__device__ __forceinline__ void split_store(bf16* s, float x, float y) {  // and its low plane kCC further
-    const uint32_t hi = pack_bf16(x, y);
-    const float2 f = unpack_bf16(hi);
+template <typename T>
+__device__ __forceinline__ void split_store(e16* s, float x, float y) {  // and its low plane kCC further
+    const uint32_t hi = Num<T>::pack(x, y);
+    const float2 f = Num<T>::unpack(hi);
     *reinterpret_cast<uint32_t*>(s) = hi;
-    *reinterpret_cast<uint32_t*>(s + kCC) = pack_bf16(x - f.x, y - f.y);
+    *reinterpret_cast<uint32_t*>(s + kCC) = Num<T>::pack(x - f.x, y - f.y);
 }
 
 // rows m0.. of accumulators to an output of row stride st: zeros from `rows` on, nothing from `all` on
-template <int NT>
-__device__ __forceinline__ void rows_out(const float (*x)[4], bf16* p, int64_t st, int m0, int rows, int all, int c0,
+template <typename T, int NT>
+__device__ __forceinline__ void rows_out(const float (*x)[4], e16* p, int64_t st, int m0, int rows, int all, int c0,
                                          int cols, const Lane& L) {
 #pragma unroll
     for (int half = 0; half < 2; ++half) {
@@ -1022,12 +1040,12 @@ __device__ __forceinline__ void rows_out(const float (*x)[4], bf16* p, int64_t s
         for (int j = 0; j < NT; ++j) {
             const int col = c0 + 8 * j + 2 * L.t;
             if (col < cols)
-                *reinterpret_cast<uint32_t*>(p + r * st + col) = r < rows ? pack_bf16(x[j][2 * half], x[j][2 * half + 1]) : 0u;
+                *reinterpret_cast<uint32_t*>(p + r * st + col) = r < rows ? Num<T>::pack(x[j][2 * half], x[j][2 * half + 1]) : 0u;
         }
     }
 }
 
-template <int KD>
+template <typename T, int KD>
 __global__ void __launch_bounds__(32 * kGradWarps, 1) planes_grad_k(DArgs a, float* group, const __grid_constant__ Maps maps) {
     using Sm = Grad<KD>;
     constexpr int VT = Sm::VT, NT = KD / 16;  // accumulator tiles of a half of the key columns
@@ -1064,7 +1082,7 @@ __global__ void __launch_bounds__(32 * kGradWarps, 1) planes_grad_k(DArgs a, flo
         const bool tail = rows < min(kC, a.L - t0);
         if (h < 0) {  // a new chunk: its keys and queries
             h = hk * rep;
-            bf16* e = reinterpret_cast<bf16*>(smem + 2 * Sm::kStage + (pseen & 1) * Sm::kKQ);
+            e16* e = reinterpret_cast<e16*>(smem + 2 * Sm::kStage + (pseen & 1) * Sm::kKQ);
             uint64_t* bar = tail ? land : &qfull[pseen & 1];
             ok = warp_wait(&qempty[pseen & 1], ((pseen >> 1) & 1) ^ 1) && ok;
             if (L.l == 0) {
@@ -1084,17 +1102,17 @@ __global__ void __launch_bounds__(32 * kGradWarps, 1) planes_grad_k(DArgs a, flo
             }
         }
         const int vn = min(VT, a.Vp - v0);
-        bf16* e = reinterpret_cast<bf16*>(smem + (ptile & 1) * Sm::kStage);
+        e16* e = reinterpret_cast<e16*>(smem + (ptile & 1) * Sm::kStage);
         uint64_t* bar = tail ? land : &full[ptile & 1];
         ok = warp_wait(&empty[ptile & 1], ((ptile >> 1) & 1) ^ 1) && ok;
         if (L.l == 0) {
             const int64_t id = (static_cast<int64_t>(b) * a.Hv + h) * a.n + c;
             mbar_expect_tx(bar, vn * (kC + 4 * kTld + 4 * Sm::LDK) * 2 + kGates * 4);
             for (int v = 0; v < vn; v += 16) tma_load(e + Sm::kD + v * kC, &maps.d, bar, v0 + v, t0, h, b);
-            const bf16* U = static_cast<const bf16*>(a.U) + (id * 2 * a.Vp + v0) * kTld;
-            const bf16* X = static_cast<const bf16*>(a.dV) + (id * 2 * a.Vp + v0) * kTld;
-            const bf16* S = static_cast<const bf16*>(a.S) + (id * 2 * a.Vp + v0) * Sm::LDK;
-            const bf16* R = static_cast<const bf16*>(a.dS) + (id * 2 * a.Vp + v0) * Sm::LDK;
+            const e16* U = static_cast<const e16*>(a.U) + (id * 2 * a.Vp + v0) * kTld;
+            const e16* X = static_cast<const e16*>(a.dV) + (id * 2 * a.Vp + v0) * kTld;
+            const e16* S = static_cast<const e16*>(a.S) + (id * 2 * a.Vp + v0) * Sm::LDK;
+            const e16* R = static_cast<const e16*>(a.dS) + (id * 2 * a.Vp + v0) * Sm::LDK;
             for (int p = 0; p < 2; ++p) {
                 bulk_load(e + Sm::kS + p * VT * Sm::LDK, S + static_cast<int64_t>(p) * a.Vp * Sm::LDK, vn * Sm::LDK * 2, bar);
                 bulk_load(e + Sm::kR + p * VT * Sm::LDK, R + static_cast<int64_t>(p) * a.Vp * Sm::LDK, vn * Sm::LDK * 2, bar);
@@ -1151,8 +1169,8 @@ __global__ void __launch_bounds__(32 * kGradWarps, 1) planes_grad_k(DArgs a, flo
     const int rg = warp & 3, half = (warp >> 2) & 1, m0 = rg * 16, n0 = half * (KD / 2);
     const bool writer = warp >= 8;
     const int r0 = m0 + L.g, r1 = r0 + 8;
-    bf16* sN = reinterpret_cast<bf16*>(smem + Sm::kN);
-    bf16* sE = sN + 2 * kCC;
+    e16* sN = reinterpret_cast<e16*>(smem + Sm::kN);
+    e16* sE = sN + 2 * kCC;
     float* sW = reinterpret_cast<float*>(smem + Sm::kN);    // dK_write, once N and E are done with
     float* sDot = reinterpret_cast<float*>(smem + Sm::kF);  // [4][64]
     float* sDb = sDot + 4 * kC;                             // [2][64]
@@ -1162,8 +1180,8 @@ __global__ void __launch_bounds__(32 * kGradWarps, 1) planes_grad_k(DArgs a, flo
         const int rows = min(kC, row_length(a, b) - c * kC), all = min(kC, a.L - c * kC);
         const int64_t row0 = static_cast<int64_t>(b) * a.L + static_cast<int64_t>(c) * kC;
         const int qst = a.Hk * a.K, vst = a.Hv * a.V;
-        bf16* dq = static_cast<bf16*>(a.dq) + row0 * qst + hk * a.K;
-        bf16* dk = static_cast<bf16*>(a.dk) + row0 * qst + hk * a.K;
+        e16* dq = static_cast<e16*>(a.dq) + row0 * qst + hk * a.K;
+        e16* dk = static_cast<e16*>(a.dk) + row0 * qst + hk * a.K;
         if (rows <= 0) {  // behind the sequence
             const uint4 z = make_uint4(0, 0, 0, 0);
             for (int i = tid; i < all * (a.K / 8); i += 32 * kGradWarps) {
@@ -1172,7 +1190,7 @@ __global__ void __launch_bounds__(32 * kGradWarps, 1) planes_grad_k(DArgs a, flo
                 *reinterpret_cast<uint4*>(dk + o) = z;
             }
             for (int h = hk * rep; h < (hk + 1) * rep; ++h) {
-                bf16* dv = static_cast<bf16*>(a.dv) + row0 * vst + static_cast<int64_t>(h) * a.V;
+                e16* dv = static_cast<e16*>(a.dv) + row0 * vst + static_cast<int64_t>(h) * a.V;
                 for (int i = tid; i < all * (a.V / 8); i += 32 * kGradWarps)
                     *reinterpret_cast<uint4*>(dv + static_cast<int64_t>(i / (a.V / 8)) * vst + i % (a.V / 8) * 8) = z;
                 for (int i = tid; i < all; i += 32 * kGradWarps) {
@@ -1182,18 +1200,18 @@ __global__ void __launch_bounds__(32 * kGradWarps, 1) planes_grad_k(DArgs a, flo
             }
             continue;
         }
-        const bf16* kq = reinterpret_cast<const bf16*>(smem + 2 * Sm::kStage + (seen & 1) * Sm::kKQ);
-        const bf16 *sK = kq + Sm::kK, *sQ = kq + Sm::kQ;
+        const e16* kq = reinterpret_cast<const e16*>(smem + 2 * Sm::kStage + (seen & 1) * Sm::kKQ);
+        const e16 *sK = kq + Sm::kK, *sQ = kq + Sm::kQ;
         ok = warp_wait(&qfull[seen & 1], (seen >> 1) & 1);
         for (int h = hk * rep; h < (hk + 1) * rep; ++h) {
-            bf16* dv = static_cast<bf16*>(a.dv) + row0 * vst + static_cast<int64_t>(h) * a.V;
+            e16* dv = static_cast<e16*>(a.dv) + row0 * vst + static_cast<int64_t>(h) * a.V;
             // readers: dQ and dK_read; writers: dK_write, and dO U^T (half 0) or dV U^T (half 1)
             float x[NT][4] = {}, y[NT > 8 ? NT : 8][4] = {};
             float db0 = 0.f, db1 = 0.f, sd = 0.f, gc = 0.f;
             float f0[2], f1[2];  // of rows r0, r1: scale gam and gam, or d
             for (int v0 = 0; v0 < a.Vp; v0 += VT, ++tile) {
                 const int vn = min(VT, a.Vp - v0);
-                const bf16* e = reinterpret_cast<const bf16*>(smem + (tile & 1) * Sm::kStage);
+                const e16* e = reinterpret_cast<const e16*>(smem + (tile & 1) * Sm::kStage);
                 const float* ga = reinterpret_cast<const float*>(e + Sm::kGa);
                 if (warp == 0) produce();
                 ok = warp_wait(&full[tile & 1], (tile >> 1) & 1) && ok;
@@ -1209,10 +1227,10 @@ __global__ void __launch_bounds__(32 * kGradWarps, 1) planes_grad_k(DArgs a, flo
                             uint32_t sh[4], sl[4];
                             ld_b<true>(sl, e + Sm::kS + VT * Sm::LDK, Sm::LDK, n0 + 16 * p, 16 * kk);
                             ld_b<true>(sh, e + Sm::kS, Sm::LDK, n0 + 16 * p, 16 * kk);
-                            mma_pair(x[2 * p], x[2 * p + 1], fd.r[0], sl);
-                            mma_pair(y[2 * p], y[2 * p + 1], fx.r[0], sl);
-                            mma_pair(x[2 * p], x[2 * p + 1], fd.r[0], sh);
-                            mma_pair(y[2 * p], y[2 * p + 1], fx.r[0], sh);
+                            mma_pair<T>(x[2 * p], x[2 * p + 1], fd.r[0], sl);
+                            mma_pair<T>(y[2 * p], y[2 * p + 1], fx.r[0], sl);
+                            mma_pair<T>(x[2 * p], x[2 * p + 1], fd.r[0], sh);
+                            mma_pair<T>(y[2 * p], y[2 * p + 1], fx.r[0], sh);
                         }
                         if ((kk & 1) == half) {  // dv
 #pragma unroll
@@ -1235,25 +1253,25 @@ __global__ void __launch_bounds__(32 * kGradWarps, 1) planes_grad_k(DArgs a, flo
                             uint32_t rh[4], rl[4];
                             ld_b<true>(rl, e + Sm::kR + VT * Sm::LDK, Sm::LDK, n0 + 16 * p, 16 * kk);
                             ld_b<true>(rh, e + Sm::kR, Sm::LDK, n0 + 16 * p, 16 * kk);
-                            mma_pair(x[2 * p], x[2 * p + 1], fu.r[0], rl);
+                            mma_pair<T>(x[2 * p], x[2 * p + 1], fu.r[0], rl);
                             if (p <= rg)
-                                mm_hl<1, true>(y[2 * p], y[2 * p + 1], left, e + Sm::kU, e + Sm::kU + VT * kTld, kTld, 16 * p,
+                                mm_hl<T, 1, true>(y[2 * p], y[2 * p + 1], left, e + Sm::kU, e + Sm::kU + VT * kTld, kTld, 16 * p,
                                                16 * kk);
-                            mma_pair(x[2 * p], x[2 * p + 1], fu.r[1], rh);
-                            mma_pair(x[2 * p], x[2 * p + 1], fu.r[0], rh);
+                            mma_pair<T>(x[2 * p], x[2 * p + 1], fu.r[1], rh);
+                            mma_pair<T>(x[2 * p], x[2 * p + 1], fu.r[0], rh);
                         }
 #pragma unroll
                         for (int p = NT / 2; p < kC / 16; ++p)
                             if (p <= rg)
-                                mm_hl<1, true>(y[2 * p], y[2 * p + 1], left, e + Sm::kU, e + Sm::kU + VT * kTld, kTld, 16 * p,
+                                mm_hl<T, 1, true>(y[2 * p], y[2 * p + 1], left, e + Sm::kU, e + Sm::kU + VT * kTld, kTld, 16 * p,
                                                16 * kk);
                         if (half) {  // dbeta = (dV / beta).(U / beta)
                             uint32_t xl[4];
                             ld_at(xl, e + Sm::kX + VT * kTld, kTld, m0, 16 * kk);
 #pragma unroll
                             for (int i = 0; i < 4; ++i) {
-                                const float2 p = unpack_bf16(left.r[0][i]), q = unpack_bf16(xl[i]);
-                                const float2 u = unpack_bf16(fu.r[0][i]), w = unpack_bf16(fu.r[1][i]);
+                                const float2 p = Num<T>::unpack(left.r[0][i]), q = Num<T>::unpack(xl[i]);
+                                const float2 u = Num<T>::unpack(fu.r[0][i]), w = Num<T>::unpack(fu.r[1][i]);
                                 const float f = ga[5 * kC + (i & 1 ? r1 : r0)];
                                 float& db = i & 1 ? db1 : db0;
                                 db = fmaf((p.x + q.x) * f, (u.x + w.x) * f, db);
@@ -1271,7 +1289,7 @@ __global__ void __launch_bounds__(32 * kGradWarps, 1) planes_grad_k(DArgs a, flo
                     const uint32_t *s_h = &sh.x, *s_l = &sl.x, *r_h = &rh.x, *r_l = &rl.x;
 #pragma unroll
                     for (int w = 0; w < 4; ++w) {
-                        const float2 p = unpack_bf16(s_h[w]), q = unpack_bf16(s_l[w]), u = unpack_bf16(r_h[w]), z = unpack_bf16(r_l[w]);
+                        const float2 p = Num<T>::unpack(s_h[w]), q = Num<T>::unpack(s_l[w]), u = Num<T>::unpack(r_h[w]), z = Num<T>::unpack(r_l[w]);
                         sd = fmaf(p.x + q.x, u.x + z.x, sd);
                         sd = fmaf(p.y + q.y, u.y + z.y, sd);
                     }
@@ -1283,7 +1301,7 @@ __global__ void __launch_bounds__(32 * kGradWarps, 1) planes_grad_k(DArgs a, flo
                     f1[0] = ga[2 * kC + r0];
                     f1[1] = ga[2 * kC + r1];
                     if (writer) {
-                        bf16* o = half ? sE : sN;
+                        e16* o = half ? sE : sN;
                         const float f = half ? -1.f : a.scale;
 #pragma unroll
                         for (int j = 0; j < kC / 8; ++j) {
@@ -1293,7 +1311,7 @@ __global__ void __launch_bounds__(32 * kGradWarps, 1) planes_grad_k(DArgs a, flo
                             for (int i = 0; i < 2; ++i) {
                                 const int r = i ? r1 : r0;
                                 const int last = half ? r - 1 : r;  // N with the diagonal, E without
-                                split_store(o + r * kTld + col, col <= last ? f * ratio(ga, r, col) * y[j][2 * i] : 0.f,
+                                split_store<T>(o + r * kTld + col, col <= last ? f * ratio(ga, r, col) * y[j][2 * i] : 0.f,
                                             col + 1 <= last ? f * ratio(ga, r, col + 1) * y[j][2 * i + 1] : 0.f);
                             }
                         }
@@ -1311,7 +1329,7 @@ __global__ void __launch_bounds__(32 * kGradWarps, 1) planes_grad_k(DArgs a, flo
                     x[j][2 * i] *= f0[i];
                     x[j][2 * i + 1] *= f0[i];
                     if (writer) {
-                        const float2 kv = unpack_bf16(*reinterpret_cast<const uint32_t*>(sK + at128(i ? r1 : r0, col)));
+                        const float2 kv = Num<T>::unpack(*reinterpret_cast<const uint32_t*>(sK + at128(i ? r1 : r0, col)));
                         tw = fmaf(kv.x, x[j][2 * i], tw);
                         tw = fmaf(kv.y, x[j][2 * i + 1], tw);
                     } else {
@@ -1351,10 +1369,10 @@ __global__ void __launch_bounds__(32 * kGradWarps, 1) planes_grad_k(DArgs a, flo
                     for (int p = 0; p < NT / 2; ++p) {
                         uint32_t bk[4];
                         ld_b128<true>(bk, sK, n0 + 16 * p, 16 * kk);
-                        mma_pair(x[2 * p], x[2 * p + 1], fn.r[1], bk);
-                        mma_pair(y[2 * p], y[2 * p + 1], fe.r[1], bk);
-                        mma_pair(x[2 * p], x[2 * p + 1], fn.r[0], bk);
-                        mma_pair(y[2 * p], y[2 * p + 1], fe.r[0], bk);
+                        mma_pair<T>(x[2 * p], x[2 * p + 1], fn.r[1], bk);
+                        mma_pair<T>(y[2 * p], y[2 * p + 1], fe.r[1], bk);
+                        mma_pair<T>(x[2 * p], x[2 * p + 1], fn.r[0], bk);
+                        mma_pair<T>(y[2 * p], y[2 * p + 1], fe.r[0], bk);
                     }
                 }
             } else {
@@ -1369,8 +1387,8 @@ __global__ void __launch_bounds__(32 * kGradWarps, 1) planes_grad_k(DArgs a, flo
                     }
 #pragma unroll
                     for (int p = 0; p < NT / 2; ++p) {
-                        mm128<2, true>(x[2 * p], x[2 * p + 1], fn, sQ, n0 + 16 * p, 16 * kk);
-                        mm128<2, true>(x[2 * p], x[2 * p + 1], fe, sK, n0 + 16 * p, 16 * kk);
+                        mm128<T, 2, true>(x[2 * p], x[2 * p + 1], fn, sQ, n0 + 16 * p, 16 * kk);
+                        mm128<T, 2, true>(x[2 * p], x[2 * p + 1], fe, sK, n0 + 16 * p, 16 * kk);
                     }
                 }
             }
@@ -1381,12 +1399,12 @@ __global__ void __launch_bounds__(32 * kGradWarps, 1) planes_grad_k(DArgs a, flo
 #pragma unroll
                 for (int i = 0; i < 2; ++i) {
                     const int o = at128(i ? r1 : r0, col);
-                    const float2 kv = unpack_bf16(*reinterpret_cast<const uint32_t*>(sK + o));
+                    const float2 kv = Num<T>::unpack(*reinterpret_cast<const uint32_t*>(sK + o));
                     if (writer) {
                         dot[i] = fmaf(-kv.x, x[j][2 * i], dot[i]);
                         dot[i] = fmaf(-kv.y, x[j][2 * i + 1], dot[i]);
                     } else {
-                        const float2 qv = unpack_bf16(*reinterpret_cast<const uint32_t*>(sQ + o));
+                        const float2 qv = Num<T>::unpack(*reinterpret_cast<const uint32_t*>(sQ + o));
                         dot[i] = fmaf(qv.x, x[j][2 * i], dot[i]);
                         dot[i] = fmaf(qv.y, x[j][2 * i + 1], dot[i]);
                         dot[i] = fmaf(kv.x, y[j][2 * i], dot[i]);
@@ -1441,8 +1459,8 @@ __global__ void __launch_bounds__(32 * kGradWarps, 1) planes_grad_k(DArgs a, flo
                         }
                 }
                 if (h == (hk + 1) * rep - 1) {
-                    rows_out<NT>(x, dq, qst, m0, rows, all, n0, a.K, L);
-                    rows_out<NT>(y, dk, qst, m0, rows, all, n0, a.K, L);
+                    rows_out<T, NT>(x, dq, qst, m0, rows, all, n0, a.K, L);
+                    rows_out<T, NT>(y, dk, qst, m0, rows, all, n0, a.K, L);
                 }
             } else if (warp == 8) {
                 float tot = L.l < kGradWarps ? gc * sTot[L.l] + sTot[kGradWarps + L.l] : 0.f;
@@ -1501,26 +1519,26 @@ int chain_groups(const DArgs& a, bool reverse) {
     return x2 <= x3 && x2 <= x4 ? 2 : x3 <= x4 ? 3 : 4;
 }
 
-template <int KD, int G>
+template <typename T, int KD, int G>
 cudaError_t chain_launch(const DArgs& a, const Maps& m, cudaStream_t s) {
-    PLANES_TRY(smem_limit(planes_chain_k<KD, G>, Fwd<KD, G>::bytes));
-    planes_chain_k<KD, G><<<dim3((a.Vp / 16 + G - 1) / G, a.Hv, a.B), Fwd<KD, G>::kWarps * 32, Fwd<KD, G>::bytes, s>>>(a, m);
+    PLANES_TRY((smem_limit(planes_chain_k<T, KD, G>, Fwd<KD, G>::bytes)));
+    planes_chain_k<T, KD, G><<<dim3((a.Vp / 16 + G - 1) / G, a.Hv, a.B), Fwd<KD, G>::kWarps * 32, Fwd<KD, G>::bytes, s>>>(a, m);
     note_launch();
     return cudaGetLastError();
 }
-template <int KD, int G>
+template <typename T, int KD, int G>
 cudaError_t rchain_launch(const DArgs& a, const Maps& m, cudaStream_t s) {
-    PLANES_TRY(smem_limit(planes_rchain_k<KD, G>, Rev<KD, G>::bytes));
-    planes_rchain_k<KD, G><<<dim3((a.Vp / 16 + G - 1) / G, a.Hv, a.B), Rev<KD, G>::kWarps * 32, Rev<KD, G>::bytes, s>>>(a, m);
+    PLANES_TRY((smem_limit(planes_rchain_k<T, KD, G>, Rev<KD, G>::bytes)));
+    planes_rchain_k<T, KD, G><<<dim3((a.Vp / 16 + G - 1) / G, a.Hv, a.B), Rev<KD, G>::kWarps * 32, Rev<KD, G>::bytes, s>>>(a, m);
     note_launch();
     return cudaGetLastError();
 }
 
-template <int KD>
+template <typename T, int KD>
 cudaError_t chain(const DArgs& a, const Maps& m, bool reverse, cudaStream_t s) {
     const int g = chain_groups(a, reverse);
-    if (reverse) return g == 2 ? rchain_launch<KD, 2>(a, m, s) : rchain_launch<KD, 3>(a, m, s);
-    return g == 2 ? chain_launch<KD, 2>(a, m, s) : g == 3 ? chain_launch<KD, 3>(a, m, s) : chain_launch<KD, 4>(a, m, s);
+    if (reverse) return g == 2 ? rchain_launch<T, KD, 2>(a, m, s) : rchain_launch<T, KD, 3>(a, m, s);
+    return g == 2 ? chain_launch<T, KD, 2>(a, m, s) : g == 3 ? chain_launch<T, KD, 3>(a, m, s) : chain_launch<T, KD, 4>(a, m, s);
 }
 
 PFN_cuTensorMapEncodeTiled_v12000 encode_fn() {
@@ -1538,7 +1556,7 @@ PFN_cuTensorMapEncodeTiled_v12000 encode_fn() {
 
 // Boxes of 64 tokens by 64 columns (128-byte swizzle) or by 16 (32-byte).  A
 // dimension of one element has no stride of its own: any multiple of 16 does.
-bool make_map(CUtensorMap& m, const void* p, const Str& st, int64_t D, int64_t L, int64_t H, int64_t B, int cols) {
+bool make_map(CUtensorMap& m, const void* p, const Str& st, int64_t D, int64_t L, int64_t H, int64_t B, int cols, int half) {
     auto enc = encode_fn();
     if (!enc) return false;
     auto bytes = [](int64_t n, int64_t stride) { return static_cast<cuuint64_t>(n > 1 ? stride * 2 : 16); };
@@ -1546,38 +1564,38 @@ bool make_map(CUtensorMap& m, const void* p, const Str& st, int64_t D, int64_t L
                                 static_cast<cuuint64_t>(B)};
     const cuuint64_t strides[3] = {bytes(L, st.t), bytes(H, st.h), bytes(B, st.b)};
     const cuuint32_t box[4] = {static_cast<cuuint32_t>(cols), kC, 1, 1}, unit[4] = {1, 1, 1, 1};
-    return enc(&m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, const_cast<void*>(p), dims, strides, box, unit,
+    return enc(&m, half ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, const_cast<void*>(p), dims, strides, box, unit,
                CU_TENSOR_MAP_INTERLEAVE_NONE, cols == 64 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_32B,
                CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 bool make_maps(const DArgs& a, Maps& m) {
-    return make_map(m.q, a.q, a.sq, a.K, a.L, a.Hk, a.B, 64) && make_map(m.k, a.k, a.sk, a.K, a.L, a.Hk, a.B, 64) &&
-           make_map(m.v, a.v, a.sv, a.V, a.L, a.Hv, a.B, 16) &&
-           (!a.dout || make_map(m.d, a.dout, a.sdo, a.V, a.L, a.Hv, a.B, 16));
+    return make_map(m.q, a.q, a.sq, a.K, a.L, a.Hk, a.B, 64, a.half) && make_map(m.k, a.k, a.sk, a.K, a.L, a.Hk, a.B, 64, a.half) &&
+           make_map(m.v, a.v, a.sv, a.V, a.L, a.Hv, a.B, 16, a.half) &&
+           (!a.dout || make_map(m.d, a.dout, a.sdo, a.V, a.L, a.Hv, a.B, 16, a.half));
 }
 
-template <int KD>
+template <typename T, int KD>
 cudaError_t fwd(const DArgs& a, cudaStream_t s) {
-    const size_t prep = 2 * kC * (KD + 8) * sizeof(bf16) + 2 * kC * kAld * sizeof(float);
-    PLANES_TRY(smem_limit(planes_prep_k<KD>, prep));
-    planes_prep_k<KD><<<dim3(a.n, a.Hv, a.B), 128, prep, s>>>(a);
+    const size_t prep = 2 * kC * (KD + 8) * sizeof(e16) + 2 * kC * kAld * sizeof(float);
+    PLANES_TRY((smem_limit(planes_prep_k<T, KD>, prep)));
+    planes_prep_k<T, KD><<<dim3(a.n, a.Hv, a.B), 128, prep, s>>>(a);
     note_launch();
     PLANES_TRY(cudaGetLastError());
     Maps m{};
     if (!make_maps(a, m)) return cudaErrorInvalidValue;
-    return chain<KD>(a, m, false, s);
+    return chain<T, KD>(a, m, false, s);
 }
 
-template <int KD>
+template <typename T, int KD>
 cudaError_t bwd(const DArgs& a, float* group, cudaStream_t s) {
     // a runtime call first: tensor maps are not made in a thread (autograd's, say) that
     // has not met its device yet
-    PLANES_TRY(smem_limit(planes_grad_k<KD>, Grad<KD>::bytes));
+    PLANES_TRY((smem_limit(planes_grad_k<T, KD>, Grad<KD>::bytes)));
     Maps m{};
     if (!make_maps(a, m)) return cudaErrorInvalidValue;
-    PLANES_TRY(chain<KD>(a, m, true, s));
+    PLANES_TRY((chain<T, KD>(a, m, true, s)));
     const int items = a.B * a.Hk * a.n;
-    planes_grad_k<KD><<<items < kSms ? items : kSms, 32 * kGradWarps, Grad<KD>::bytes, s>>>(a, group, m);
+    planes_grad_k<T, KD><<<items < kSms ? items : kSms, 32 * kGradWarps, Grad<KD>::bytes, s>>>(a, group, m);
     note_launch();
     return cudaGetLastError();
 }
@@ -1586,9 +1604,9 @@ size_t up256(size_t x) { return (x + 255) / 256 * 256; }
 int key_dim(const DArgs& a) { return a.K <= 64 ? 64 : 128; }
 size_t ids(const DArgs& a) { return static_cast<size_t>(a.B) * a.Hv * a.n; }
 size_t gates_bytes(const DArgs& a) { return up256(ids(a) * kGates * sizeof(float)); }
-size_t square_bytes(const DArgs& a) { return up256(ids(a) * 2 * kCC * sizeof(bf16)); }
-size_t state_bytes(const DArgs& a) { return up256(ids(a) * 2 * a.Vp * (key_dim(a) + 8) * sizeof(bf16)); }
-size_t value_bytes(const DArgs& a, int planes) { return up256(ids(a) * planes * a.Vp * kTld * sizeof(bf16)); }
+size_t square_bytes(const DArgs& a) { return up256(ids(a) * 2 * kCC * sizeof(e16)); }
+size_t state_bytes(const DArgs& a) { return up256(ids(a) * 2 * a.Vp * (key_dim(a) + 8) * sizeof(e16)); }
+size_t value_bytes(const DArgs& a, int planes) { return up256(ids(a) * planes * a.Vp * kTld * sizeof(e16)); }
 
 void set_saved(DArgs& a, void* ws, bool training) {
     char* w = static_cast<char*>(ws);
@@ -1608,7 +1626,8 @@ size_t planes_bwd_size(const DArgs& a) { return state_bytes(a) + value_bytes(a, 
 
 cudaError_t planes_fwd(DArgs a, void* ws, bool training, cudaStream_t s) {
     set_saved(a, ws, training);
-    return a.K <= 64 ? fwd<64>(a, s) : fwd<128>(a, s);
+    if (a.half) return a.K <= 64 ? fwd<__half, 64>(a, s) : fwd<__half, 128>(a, s);
+    return a.K <= 64 ? fwd<__nv_bfloat16, 64>(a, s) : fwd<__nv_bfloat16, 128>(a, s);
 }
 
 cudaError_t planes_bwd(DArgs a, void* saved, void* ws, float* group, cudaStream_t s) {
@@ -1616,7 +1635,8 @@ cudaError_t planes_bwd(DArgs a, void* saved, void* ws, float* group, cudaStream_
     char* w = static_cast<char*>(ws);
     a.dS = w;
     a.dV = w + state_bytes(a);
-    return a.K <= 64 ? bwd<64>(a, group, s) : bwd<128>(a, group, s);
+    if (a.half) return a.K <= 64 ? bwd<__half, 64>(a, group, s) : bwd<__half, 128>(a, group, s);
+    return a.K <= 64 ? bwd<__nv_bfloat16, 64>(a, group, s) : bwd<__nv_bfloat16, 128>(a, group, s);
 }
 
 cudaError_t planes_read_status(int* out, cudaStream_t s) { return read_clear_status(out, s); }

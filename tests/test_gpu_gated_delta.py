@@ -7,12 +7,12 @@ sums, so computed values stay under 16 * 2^-17 = 1.3e-4 of their norm in the
 worst case and, errors being of either sign, near 2^-17 * sqrt(16) = 3.1e-5:
 TOL = 6.2e-5, twice that.  One rounding to the output's type adds eps / 2.
 
-In the backward of bfloat16 inputs three operands on a gradient's way (dS, dV
-and T') are rounded to one bf16 value each: off by up to 2^-9 of an element, of
-either sign and of any size below, so 2^-9 / sqrt(3) in the root of the mean
-square, and three of them sqrt(3) times that: GRAD16 = 2^-9 for gradients that
-are float32 beside bfloat16 inputs (for bfloat16 ones eps / 2 = 2^-8 holds it:
-their own rounding is 2^-8 / (2 sqrt(3)) in the mean, together 2.3e-3).
+In the backward of 16-bit inputs one operand on a gradient's way, dV, is
+rounded to one value of their type: off by up to half a step of an element,
+2^-9 for bfloat16 and 2^-12 for float16.  That is what a float32 gradient
+beside them may be off by (ONE); 16-bit ones have their own rounding, eps / 2,
+and stay under it with both (each is 1 / sqrt(3) of its half step in the mean:
+together 0.65 eps / 2).
 """
 import pytest
 import torch
@@ -20,7 +20,7 @@ import torch
 pytestmark = pytest.mark.gpu
 DEV = "cuda:0"
 TOL = 6.2e-5
-GRAD16 = 2.0 ** -9
+ONE = {torch.bfloat16: 2.0 ** -9, torch.float16: 2.0 ** -12, torch.float32: TOL}
 
 if torch.cuda.is_available():
     from eacs_b200.ops.gated_delta import gated_delta_rule, gated_delta_step
@@ -31,7 +31,7 @@ def tol(dtype, inputs=torch.float32):
     """inputs: the type of q, k and v, for gradients."""
     if dtype != torch.float32:
         return TOL + torch.finfo(dtype).eps / 2
-    return GRAD16 if inputs == torch.bfloat16 else TOL
+    return ONE[inputs]
 
 
 def close(got, want, times=1.0, what="", inputs=torch.float32):
