@@ -54,6 +54,17 @@ __device__ __forceinline__ void bulk_wait_all() { asm volatile("cp.async.bulk.wa
 __device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity) {
     return __all_sync(0xffffffffu, mbar_wait(bar, parity));
 }
+// Two barriers at once, and one that was asked earlier (a wait that is over
+// before it begins still takes some 270 cycles of a warp that has no other).
+__device__ __forceinline__ bool warp_wait2(uint64_t* a, uint32_t pa, uint64_t* b, uint32_t pb) {
+    const bool da = mbar_try_wait(a, pa), db = mbar_try_wait(b, pb);
+    if (__all_sync(0xffffffffu, da && db)) return true;
+    return warp_wait(a, pa) && warp_wait(b, pb);
+}
+__device__ __forceinline__ bool warp_wait_asked(bool done, uint64_t* bar, uint32_t parity) {
+    if (__all_sync(0xffffffffu, done)) return true;
+    return warp_wait(bar, parity);
+}
 // one arrival for a warp, after what all its lanes did
 __device__ __forceinline__ void warp_arrive(uint64_t* bar) {
     __syncwarp();
@@ -94,6 +105,15 @@ __device__ __forceinline__ Af<P> from_acc(const float* c0, const float* c1) {
         }
     }
     return a;
+}
+// Quarter i of that: registers i of both planes.
+template <typename T, int P>
+__device__ __forceinline__ void from_acc_part(Af<P>& a, int i, float x, float y) {
+    a.r[0][i] = Num<T>::pack(x, y);
+    if constexpr (P == 2) {
+        const float2 h = Num<T>::unpack(a.r[0][i]);
+        a.r[1][i] = Num<T>::pack(x - h.x, y - h.y);
+    }
 }
 // of a tile stored [m][k], and stored [k][m]
 __device__ __forceinline__ void ld_a(uint32_t* r, const e16* s, int ld, int m0, int k0) {
@@ -189,6 +209,23 @@ __device__ __forceinline__ void mma_step(float (*c)[4], const Af<P>& a, const ui
 #pragma unroll
         for (int i = 0; i < 4; ++i)
             if (i >= from && i < to) mma_pair<T>(c[2 * i], c[2 * i + 1], a.r[p], b[i]);
+}
+// The same with other work of the warp in quarters, side(0..3), between the
+// products: a warp alone on its scheduler would otherwise do it while the tensor
+// pipe stands still.
+template <typename T, int P, class Side>
+__device__ __forceinline__ void mma_step_with(float (*c)[4], const Af<P>& a, const uint32_t (*b)[4], Side side, int from = 0,
+                                              int to = 4) {
+#pragma unroll
+    for (int p = P - 1; p >= 0; --p)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            if (i >= from && i < to) mma_pair<T>(c[2 * i], c[2 * i + 1], a.r[p], b[i]);
+            if (p == P - 1) side(i);
+        }
+}
+template <int P> __device__ __forceinline__ Af<1> high(const Af<P>& a) {
+    return Af<1>{{{a.r[0][0], a.r[0][1], a.r[0][2], a.r[0][3]}}};
 }
 // accumulators of 16 rows by 16 columns to a tile [row][col] (as ld_a reads it)
 __device__ __forceinline__ void st_tile(e16* s, int ld, int c0, const uint32_t* r) {
@@ -466,7 +503,8 @@ __device__ __forceinline__ void state_store(const float (*S)[4], float* p, int K
         }
 }
 
-template <typename T, int KD, int G>
+// KEEP: S and U are written for a backward.
+template <typename T, int KD, int G, bool KEEP>
 __global__ void __launch_bounds__(Fwd<KD, G>::kWarps * 32) planes_chain_k(DArgs a, const __grid_constant__ Maps maps) {
     using Sm = Fwd<KD, G>;
     const int h = blockIdx.y, b = blockIdx.z, hk = h / (a.Hv / a.Hk);
@@ -536,34 +574,45 @@ __global__ void __launch_bounds__(Fwd<KD, G>::kWarps * 32) planes_chain_k(DArgs 
             const float* ga = reinterpret_cast<const float*>(e + Sm::kGa);
             const float *gam = ga + 2 * kC, *dec = ga + 3 * kC;
             const int64_t id = head * a.n + c;
-            ok = warp_wait(&full[c & 1], (c >> 1) & 1);
-            if (on) {
-                ok = warp_wait(&s_empty[warp], (c & 1) ^ 1) && ok;
-                if (a.S) {  // the last chunk's copies have left the tiles
+            if (!on) {
+                ok = warp_wait(&full[c & 1], (c >> 1) & 1);
+            } else {
+                ok = warp_wait2(&full[c & 1], (c >> 1) & 1, &s_empty[warp], (c & 1) ^ 1);
+                if constexpr (KEEP) {  // the last chunk's copies have left the tiles
                     if (L.l == 0) bulk_wait_read();
                     __syncwarp();
                 }
-                // (K S0)^T, S in two planes
+                // (K S0)^T, S in two planes; the next 16 columns of S are split between the products
                 float X[kC / 8][4] = {};
-                steps<KD / 16>(
-                    [&](int i, uint32_t(*f)[4]) {
+                {
+                    Af<2> as[2];
+                    as[0] = from_acc<T, 2>(S[0], S[1]);
+                    steps<KD / 16>(
+                        [&](int i, uint32_t(*f)[4]) {
 #pragma unroll
-                        for (int p = 0; p < 4; ++p) ld_b128<false>(f[p], e + Sm::kK, 16 * p, 16 * i);
-                    },
-                    [&](int i, const uint32_t(*f)[4]) {
-                        const Af<2> af = from_acc<T, 2>(S[2 * i], S[2 * i + 1]);
-                        st_tile(sS, Sm::LDK, 16 * i, af.r[0]);
-                        if (a.S) st_tile(sS + 16 * Sm::LDK, Sm::LDK, 16 * i, af.r[1]);
-                        mma_step<T>(X, af, f);
-                    });
-                if (a.S) fence_async();
+                            for (int p = 0; p < 4; ++p) ld_b128<false>(f[p], e + Sm::kK, 16 * p, 16 * i);
+                        },
+                        [&](int i, const uint32_t(*f)[4]) {
+                            Af<2>& af = as[i & 1];
+                            st_tile(sS, Sm::LDK, 16 * i, af.r[0]);
+                            if constexpr (KEEP) st_tile(sS + 16 * Sm::LDK, Sm::LDK, 16 * i, af.r[1]);
+                            mma_step_with<T>(X, af, f, [&](int q) {
+                                if (i + 1 < KD / 16) {
+                                    const float* s = S[2 * i + 2 + q / 2];
+                                    from_acc_part<T>(as[(i + 1) & 1], q, s[2 * (q & 1)], s[2 * (q & 1) + 1]);
+                                }
+                            });
+                        });
+                }
+                if constexpr (KEEP) fence_async();
                 warp_arrive(&s_full[warp]);
-                if (a.S && L.l == 0) {
+                if (KEEP && L.l == 0) {
                     e16* to = static_cast<e16*>(a.S) + (id * 2 * a.Vp + v0) * Sm::LDK;
                     bulk_store(to, sS, 32 * Sm::LDK);
                     bulk_store(to + static_cast<int64_t>(a.Vp) * Sm::LDK, sS + 16 * Sm::LDK, 32 * Sm::LDK);
                     bulk_commit();
                 }
+                const bool u_free = mbar_try_wait(&u_empty[warp], (c & 1) ^ 1);
                 // X = V^T - gam (K S0)^T
 #pragma unroll
                 for (int p = 0; p < kC / 16; ++p) {
@@ -580,10 +629,23 @@ __global__ void __launch_bounds__(Fwd<KD, G>::kWarps * 32) planes_chain_k(DArgs 
                         x[3] = fmaf(-f.y, x[3], hi.y);
                     }
                 }
-                // U^T = X T'^T, both in two planes
+                // U^T = X T'^T, both in two planes; between the products S is scaled, and the first
+                // 16 tokens of U, which are done after theirs, are split for the update
                 float U[kC / 8][4] = {};
+                const float gc = gam[kC - 1];
+                auto decayed = [&](Af<2>& to, int kk, int q) {
+                    const float2 d = *reinterpret_cast<const float2*>(dec + 16 * kk + 8 * (q / 2) + 2 * L.t);
+                    const float* u = U[2 * kk + q / 2];
+                    from_acc_part<T>(to, q, u[2 * (q & 1)] * d.x, u[2 * (q & 1) + 1] * d.y);
+                };
+                auto plain = [&](Af<2>& to, int kk, int q) {
+                    const float* u = U[2 * kk + q / 2];
+                    from_acc_part<T>(to, q, u[2 * (q & 1)], u[2 * (q & 1) + 1]);
+                };
+                Af<2> ud[2], up[2];
                 {
-                    Af<2> af;
+                    Af<2> ax[2];
+                    ax[0] = from_acc<T, 2>(X[0], X[1]);
                     steps<8>(  // the low plane of T', then the high one
                         [&](int i, uint32_t(*f)[4]) {
 #pragma unroll
@@ -591,23 +653,28 @@ __global__ void __launch_bounds__(Fwd<KD, G>::kWarps * 32) planes_chain_k(DArgs 
                                 if (p >= i / 2) ld_b<false>(f[p], e + Sm::kT + (i & 1 ? 0 : kCC), kTld, 16 * p, 16 * (i / 2));
                         },
                         [&](int i, const uint32_t(*f)[4]) {
-                            if (i & 1) {
-                                mma_step<T>(U, af, f, i / 2);
-                            } else {
-                                af = from_acc<T, 2>(X[i], X[i + 1]);
-                                mma_step<T>(U, Af<1>{{{af.r[0][0], af.r[0][1], af.r[0][2], af.r[0][3]}}}, f, i / 2);
-                            }
+                            const int kk = i / 2;
+                            const Af<2>& af = ax[kk & 1];
+                            auto side = [&](int q) {
+                                if (4 * i + q < KD / 4) {  // half a tile of S in each of 32 places
+                                    float* s = S[(4 * i + q) / 2];
+                                    s[2 * (q & 1)] *= gc;
+                                    s[2 * (q & 1) + 1] *= gc;
+                                }
+                                if ((i & 1) && kk + 1 < 4) {
+                                    const float* x = X[2 * kk + 2 + q / 2];
+                                    from_acc_part<T>(ax[(kk + 1) & 1], q, x[2 * (q & 1)], x[2 * (q & 1) + 1]);
+                                }
+                                if (i == 4) decayed(ud[0], 0, q);
+                                if (i == 5) plain(up[0], 0, q);
+                            };
+                            if (i & 1) mma_step_with<T>(U, af, f, side, kk);
+                            else mma_step_with<T>(U, high(af), f, side, kk);
                         });
                 }
-                ok = warp_wait(&u_empty[warp], (c & 1) ^ 1) && ok;
-                const float gc = gam[kC - 1];
-#pragma unroll
-                for (int j = 0; j < KD / 8; ++j)
-#pragma unroll
-                    for (int x = 0; x < 4; ++x) S[j][x] *= gc;
+                ok = warp_wait_asked(u_free, &u_empty[warp], (c & 1) ^ 1) && ok;
                 // S^T = gam_63 S^T + (d U)^T K
                 {
-                    Af<2> af;
                     constexpr int Q = KD / 64;
                     steps<4 * Q>(
                         [&](int i, uint32_t(*f)[4]) {
@@ -617,27 +684,20 @@ __global__ void __launch_bounds__(Fwd<KD, G>::kWarps * 32) planes_chain_k(DArgs 
                         [&](int i, const uint32_t(*f)[4]) {
                             const int kk = i / Q;
                             if (i % Q == 0) {
-                                const Af<2> au = from_acc<T, 2>(U[2 * kk], U[2 * kk + 1]);
-                                st_tile(sU, kTld, 16 * kk, au.r[0]);
-                                st_tile(sU + 16 * kTld, kTld, 16 * kk, au.r[1]);
-                                float y[2][4];
-#pragma unroll
-                                for (int x = 0; x < 2; ++x) {
-                                    const float2 d = *reinterpret_cast<const float2*>(dec + 16 * kk + 8 * x + 2 * L.t);
-                                    const float* u = U[2 * kk + x];
-                                    y[x][0] = u[0] * d.x;
-                                    y[x][1] = u[1] * d.y;
-                                    y[x][2] = u[2] * d.x;
-                                    y[x][3] = u[3] * d.y;
-                                }
-                                af = from_acc<T, 2>(y[0], y[1]);
+                                st_tile(sU, kTld, 16 * kk, up[kk & 1].r[0]);
+                                st_tile(sU + 16 * kTld, kTld, 16 * kk, up[kk & 1].r[1]);
                             }
-                            mma_step<T>(S + 8 * (i % Q), af, f);
+                            mma_step_with<T>(S + 8 * (i % Q), ud[kk & 1], f, [&](int q) {
+                                if (kk + 1 < 4) {
+                                    if (i % Q == 0) decayed(ud[(kk + 1) & 1], kk + 1, q);
+                                    if (i % Q == Q - 1) plain(up[(kk + 1) & 1], kk + 1, q);
+                                }
+                            });
                         });
                 }
-                if (a.S) fence_async();
+                if constexpr (KEEP) fence_async();
                 warp_arrive(&u_full[warp]);
-                if (a.S && L.l == 0) {
+                if (KEEP && L.l == 0) {
                     e16* to = static_cast<e16*>(a.U) + (id * 2 * a.Vp + v0) * kTld;
                     bulk_store(to, sU, 32 * kTld);
                     bulk_store(to + static_cast<int64_t>(a.Vp) * kTld, sU + 16 * kTld, 32 * kTld);
@@ -647,7 +707,7 @@ __global__ void __launch_bounds__(Fwd<KD, G>::kWarps * 32) planes_chain_k(DArgs 
             warp_arrive(&empty[c & 1]);
         }
         if (on && a.final_state && ok) state_store<KD>(S, a.final_state + head * a.K * a.V, a.K, a.V, v0, L);
-        if (a.S && L.l == 0) bulk_wait_all();
+        if (KEEP && L.l == 0) bulk_wait_all();
         return;
     }
     // ---- outputs of the groups g = helper, helper + H, .. ----
@@ -708,7 +768,7 @@ __global__ void __launch_bounds__(Fwd<KD, G>::kWarps * 32) planes_chain_k(DArgs 
                 [&](int k, const uint32_t(*f)[4]) {
                     const Af<2>& af = au[(k / 2) & 1];
                     if (k & 1) mma_step<T>(O[i], af, f, k / 2);
-                    else mma_step<T>(O[i], Af<1>{{{af.r[0][0], af.r[0][1], af.r[0][2], af.r[0][3]}}}, f, k / 2);
+                    else mma_step<T>(O[i], high(af), f, k / 2);
                 });
             warp_arrive(&u_empty[g]);
             // rows of 16 values through shared memory: 32 bytes a token, two lanes each
@@ -834,17 +894,26 @@ __global__ void __launch_bounds__(Rev<KD, G>::kWarps * 32) planes_rchain_k(DArgs
                 if (L.l == 0) bulk_wait_read();  // the last chunk's copies have left the tiles
                 __syncwarp();
                 float U[kC / 8][4] = {};  // dU^T = d (K dS1)^T + dO^T M
-                steps<KD / 16>(
-                    [&](int k, uint32_t(*f)[4]) {
+                {
+                    Af<2> as[2];
+                    as[0] = from_acc<T, 2>(S[0], S[1]);
+                    steps<KD / 16>(
+                        [&](int k, uint32_t(*f)[4]) {
 #pragma unroll
-                        for (int p = 0; p < 4; ++p) ld_b128<false>(f[p], e + Sm::kK, 16 * p, 16 * k);
-                    },
-                    [&](int k, const uint32_t(*f)[4]) {
-                        const Af<2> af = from_acc<T, 2>(S[2 * k], S[2 * k + 1]);
-                        st_tile(sS, Sm::LDK, 16 * k, af.r[0]);
-                        st_tile(sS + 16 * Sm::LDK, Sm::LDK, 16 * k, af.r[1]);
-                        mma_step<T>(U, af, f);
-                    });
+                            for (int p = 0; p < 4; ++p) ld_b128<false>(f[p], e + Sm::kK, 16 * p, 16 * k);
+                        },
+                        [&](int k, const uint32_t(*f)[4]) {
+                            Af<2>& af = as[k & 1];
+                            st_tile(sS, Sm::LDK, 16 * k, af.r[0]);
+                            st_tile(sS + 16 * Sm::LDK, Sm::LDK, 16 * k, af.r[1]);
+                            mma_step_with<T>(U, af, f, [&](int q) {
+                                if (k + 1 < KD / 16) {
+                                    const float* s = S[2 * k + 2 + q / 2];
+                                    from_acc_part<T>(as[(k + 1) & 1], q, s[2 * (q & 1)], s[2 * (q & 1) + 1]);
+                                }
+                            });
+                        });
+                }
                 fence_async();
                 __syncwarp();
                 if (L.l == 0) {
@@ -853,6 +922,7 @@ __global__ void __launch_bounds__(Rev<KD, G>::kWarps * 32) planes_rchain_k(DArgs
                     bulk_store(to + static_cast<int64_t>(a.Vp) * Sm::LDK, sS + 16 * Sm::LDK, 32 * Sm::LDK);
                     bulk_commit();
                 }
+                const bool z_there = mbar_try_wait(&z_full[warp], i & 1);
 #pragma unroll
                 for (int j = 0; j < kC / 8; ++j) {
                     const float2 f = *reinterpret_cast<const float2*>(dec + 8 * j + 2 * L.t);
@@ -872,63 +942,80 @@ __global__ void __launch_bounds__(Rev<KD, G>::kWarps * 32) planes_rchain_k(DArgs
                         },
                         [&](int k, const uint32_t(*f)[4]) { mma_step<T>(U, ad[(k / 2) & 1], f, 0, k / 2 + 1); });
                 }
-                float X[kC / 8][4] = {};  // dV^T = dU^T T'
+                ok = warp_wait_asked(z_there, &z_full[warp], i & 1) && ok;
+                // dV^T = dU^T T', the last 16 tokens first; between the products dS is scaled and
+                // (scale gam dO)^T Q added, and the last tokens of dV, done first, are split for the update
+                float X[kC / 8][4] = {};
+                const float gc = gam[kC - 1];
+                auto decayed = [&](Af<1>& to, int kk, int q) {
+                    const float2 d = *reinterpret_cast<const float2*>(gam + 16 * kk + 8 * (q / 2) + 2 * L.t);
+                    const float* u = X[2 * kk + q / 2];
+                    from_acc_part<T>(to, q, -u[2 * (q & 1)] * d.x, -u[2 * (q & 1) + 1] * d.y);
+                };
+                auto plain = [&](Af<2>& to, int kk, int q) {
+                    const float* u = X[2 * kk + q / 2];
+                    from_acc_part<T>(to, q, u[2 * (q & 1)], u[2 * (q & 1) + 1]);
+                };
+                Af<1> xd[2];
+                Af<2> xp[2];
                 {
-                    Af<2> af;
+                    Af<2> au[2];
+                    au[1] = from_acc<T, 2>(U[6], U[7]);
                     steps<8>(
                         [&](int k, uint32_t(*f)[4]) {
+                            const int kk = 3 - k / 2;
 #pragma unroll
                             for (int p = 0; p < 4; ++p)
-                                if (p <= k / 2) ld_b<true>(f[p], e + Sm::kT + (k & 1 ? 0 : kCC), kTld, 16 * p, 16 * (k / 2));
+                                if (p <= kk) ld_b<true>(f[p], e + Sm::kT + (k & 1 ? 0 : kCC), kTld, 16 * p, 16 * kk);
                         },
                         [&](int k, const uint32_t(*f)[4]) {
-                            if (k & 1) {
-                                mma_step<T>(X, af, f, 0, k / 2 + 1);
-                            } else {
-                                af = from_acc<T, 2>(U[k], U[k + 1]);
-                                mma_step<T>(X, Af<1>{{{af.r[0][0], af.r[0][1], af.r[0][2], af.r[0][3]}}}, f, 0, k / 2 + 1);
-                            }
+                            const int kk = 3 - k / 2;
+                            const Af<2>& af = au[kk & 1];
+                            auto side = [&](int q) {
+                                if (!(q & 1)) {  // dS: KD / 8 tiles in 8 steps of 2
+                                    constexpr int N = KD / 8;
+                                    const int j = k * 2 + q / 2;
+                                    if (j < N) {
+                                        const float4 z = sZ[j * 32 + L.l];
+                                        S[j][0] = fmaf(gc, S[j][0], z.x);
+                                        S[j][1] = fmaf(gc, S[j][1], z.y);
+                                        S[j][2] = fmaf(gc, S[j][2], z.z);
+                                        S[j][3] = fmaf(gc, S[j][3], z.w);
+                                    }
+                                }
+                                if ((k & 1) && kk > 0) {
+                                    const float* u = U[2 * kk - 2 + q / 2];
+                                    from_acc_part<T>(au[(kk - 1) & 1], q, u[2 * (q & 1)], u[2 * (q & 1) + 1]);
+                                }
+                                if (k == 4) decayed(xd[1], 3, q);
+                                if (k == 5) plain(xp[1], 3, q);
+                            };
+                            if (k & 1) mma_step_with<T>(X, af, f, side, 0, kk + 1);
+                            else mma_step_with<T>(X, high(af), f, side, 0, kk + 1);
                         });
                 }
-                // dS^T = gam_63 dS^T + (scale gam dO)^T Q - (gam dV)^T K
-                ok = warp_wait(&z_full[warp], i & 1) && ok;
-                const float gc = gam[kC - 1];
-#pragma unroll
-                for (int j = 0; j < KD / 8; ++j) {
-                    const float4 z = sZ[j * 32 + L.l];
-                    S[j][0] = fmaf(gc, S[j][0], z.x);
-                    S[j][1] = fmaf(gc, S[j][1], z.y);
-                    S[j][2] = fmaf(gc, S[j][2], z.z);
-                    S[j][3] = fmaf(gc, S[j][3], z.w);
-                }
                 warp_arrive(&z_empty[warp]);
+                // dS^T -= (gam dV)^T K
                 {
-                    Af<1> af;
                     constexpr int Q = KD / 64;
                     steps<4 * Q>(
                         [&](int k, uint32_t(*f)[4]) {
 #pragma unroll
-                            for (int p = 0; p < 4; ++p) ld_b128<true>(f[p], e + Sm::kK, 64 * (k % Q) + 16 * p, 16 * (k / Q));
+                            for (int p = 0; p < 4; ++p)
+                                ld_b128<true>(f[p], e + Sm::kK, 64 * (k % Q) + 16 * p, 16 * (3 - k / Q));
                         },
                         [&](int k, const uint32_t(*f)[4]) {
-                            const int kk = k / Q;
+                            const int kk = 3 - k / Q;
                             if (k % Q == 0) {
-                                const Af<2> ax = from_acc<T, 2>(X[2 * kk], X[2 * kk + 1]);
-                                st_tile(sX, kTld, 16 * kk, ax.r[0]);
-                                st_tile(sX + 16 * kTld, kTld, 16 * kk, ax.r[1]);
-                                float y[2][4];
-#pragma unroll
-                                for (int x = 0; x < 2; ++x) {
-                                    const float2 d = *reinterpret_cast<const float2*>(gam + 16 * kk + 8 * x + 2 * L.t);
-                                    const float* u = X[2 * kk + x];
-                                    y[x][0] = -u[0] * d.x;
-                                    y[x][1] = -u[1] * d.y;
-                                    y[x][2] = -u[2] * d.x;
-                                    y[x][3] = -u[3] * d.y;
-                                }
-                                af = from_acc<T, 1>(y[0], y[1]);
+                                st_tile(sX, kTld, 16 * kk, xp[kk & 1].r[0]);
+                                st_tile(sX + 16 * kTld, kTld, 16 * kk, xp[kk & 1].r[1]);
                             }
-                            mma_step<T>(S + 8 * (k % Q), af, f);
+                            mma_step_with<T>(S + 8 * (k % Q), xd[kk & 1], f, [&](int q) {
+                                if (kk > 0) {
+                                    if (k % Q == 0) decayed(xd[(kk - 1) & 1], kk - 1, q);
+                                    if (k % Q == Q - 1) plain(xp[(kk - 1) & 1], kk - 1, q);
+                                }
+                            });
                         });
                 }
                 fence_async();
@@ -1521,8 +1608,9 @@ int chain_groups(const DArgs& a, bool reverse) {
 
 template <typename T, int KD, int G>
 cudaError_t chain_launch(const DArgs& a, const Maps& m, cudaStream_t s) {
-    PLANES_TRY((smem_limit(planes_chain_k<T, KD, G>, Fwd<KD, G>::bytes)));
-    planes_chain_k<T, KD, G><<<dim3((a.Vp / 16 + G - 1) / G, a.Hv, a.B), Fwd<KD, G>::kWarps * 32, Fwd<KD, G>::bytes, s>>>(a, m);
+    const auto k = a.S ? planes_chain_k<T, KD, G, true> : planes_chain_k<T, KD, G, false>;
+    PLANES_TRY(smem_limit(k, Fwd<KD, G>::bytes));
+    k<<<dim3((a.Vp / 16 + G - 1) / G, a.Hv, a.B), Fwd<KD, G>::kWarps * 32, Fwd<KD, G>::bytes, s>>>(a, m);
     note_launch();
     return cudaGetLastError();
 }
