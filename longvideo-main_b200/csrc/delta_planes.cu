@@ -476,7 +476,7 @@ struct Fwd {
     static constexpr int kGa = kM + 2 * kCC;  // (elements) the gates, float32
     static constexpr int kLoad = kGa * 2 + kGates * 4, kStage = up1024(kLoad);  // bytes
     static constexpr int kS = 0, kU = 2 * 16 * LDK, kO = kU + 2 * 16 * kTld;  // a group's tiles (elements)
-    static constexpr int kGroup = (kO + kC * LDO) * 2;
+    static constexpr int kGroup = kO * 2 + 16 * kC * 4;  // (O: float32 between its two products, then rows)
     static constexpr int kBars = 2 * kStage + G * kGroup;
     static constexpr size_t bytes = 1024 + kBars + 8 * (5 + 4 * G);
 };
@@ -712,7 +712,6 @@ __global__ void __launch_bounds__(Fwd<KD, G>::kWarps * 32) planes_chain_k(DArgs 
     }
     // ---- outputs of the groups g = helper, helper + H, .. ----
     const int helper = warp - G;
-    constexpr int NG = (G + Sm::H - 1) / Sm::H;
     const int64_t ost = static_cast<int64_t>(a.Hv) * a.V;
     e16* out = static_cast<e16*>(a.out) + static_cast<int64_t>(b) * a.L * ost + static_cast<int64_t>(h) * a.V;
     for (int c = 0; c < nc && ok; ++c) {
@@ -721,15 +720,19 @@ __global__ void __launch_bounds__(Fwd<KD, G>::kWarps * 32) planes_chain_k(DArgs 
         const float* sgam = reinterpret_cast<const float*>(e + Sm::kGa) + 4 * kC;
         const int rows = min(kC, len - c * kC), all = min(kC, a.L - c * kC);
         ok = warp_wait(&full[c & 1], (c >> 1) & 1);
-        float O[NG][kC / 8][4] = {};
-#pragma unroll
-        for (int i = 0; i < NG; ++i) {
-            const int g = helper + i * Sm::H;
+        // (Loops over the groups are not unrolled: what the warps of a CTA run in a chunk has to fit
+        // the instruction cache.  O waits in shared memory between its two products.)
+#pragma unroll 1
+        for (int g = helper; g < G; g += Sm::H) {
             if (vb + 16 * g >= a.Vp) break;
-            const e16* sS = reinterpret_cast<const e16*>(smem + 2 * Sm::kStage + g * Sm::kGroup) + Sm::kS;
+            unsigned char* theirs = smem + 2 * Sm::kStage + g * Sm::kGroup;
+            const e16* sS = reinterpret_cast<const e16*>(theirs) + Sm::kS;
+            float4* sO = reinterpret_cast<float4*>(theirs + Sm::kO * 2);
             ok = warp_wait(&s_full[g], c & 1) && ok;
-            // scale gam Q S0: S in one plane (its rounding, 2^-9 of terms of any sign, against the
-            // output's own: y is off by 2.2e-3 in the norm instead of 1.7e-3, for half the products)
+            // scale gam Q S0: S in one plane (its rounding, half a step of terms of any sign, against
+            // the output's own: in bfloat16 y is off by 2.2e-3 in the norm instead of 1.7e-3, for half
+            // the products)
+            float O[kC / 8][4] = {};
             Af<1> as[2];
             steps<KD / 16>(
                 [&](int k, uint32_t(*f)[4]) {
@@ -737,22 +740,29 @@ __global__ void __launch_bounds__(Fwd<KD, G>::kWarps * 32) planes_chain_k(DArgs 
 #pragma unroll
                     for (int p = 0; p < 4; ++p) ld_b128<false>(f[p], e + Sm::kQ, 16 * p, 16 * k);
                 },
-                [&](int k, const uint32_t(*f)[4]) { mma_step<T>(O[i], as[k & 1], f); });
+                [&](int k, const uint32_t(*f)[4]) { mma_step<T>(O, as[k & 1], f); });
             warp_arrive(&s_empty[g]);
 #pragma unroll
             for (int j = 0; j < kC / 8; ++j) {
                 const float2 f = *reinterpret_cast<const float2*>(sgam + 8 * j + 2 * L.t);
-                O[i][j][0] *= f.x;
-                O[i][j][1] *= f.y;
-                O[i][j][2] *= f.x;
-                O[i][j][3] *= f.y;
+                sO[j * 32 + L.l] = make_float4(O[j][0] * f.x, O[j][1] * f.y, O[j][2] * f.x, O[j][3] * f.y);
             }
         }
-#pragma unroll
-        for (int i = 0; i < NG; ++i) {
-            const int g = helper + i * Sm::H, v0 = vb + 16 * g;
+#pragma unroll 1
+        for (int g = helper; g < G; g += Sm::H) {
+            const int v0 = vb + 16 * g;
             if (v0 >= a.Vp) break;
             e16* theirs = reinterpret_cast<e16*>(smem + 2 * Sm::kStage + g * Sm::kGroup);
+            e16* sO = theirs + Sm::kO;
+            float O[kC / 8][4];
+#pragma unroll
+            for (int j = 0; j < kC / 8; ++j) {
+                const float4 o = reinterpret_cast<const float4*>(sO)[j * 32 + L.l];
+                O[j][0] = o.x;
+                O[j][1] = o.y;
+                O[j][2] = o.z;
+                O[j][3] = o.w;
+            }
             ok = warp_wait(&u_full[g], c & 1) && ok;
             Af<2> au[2];
             steps<8>(
@@ -767,15 +777,15 @@ __global__ void __launch_bounds__(Fwd<KD, G>::kWarps * 32) planes_chain_k(DArgs 
                 },
                 [&](int k, const uint32_t(*f)[4]) {
                     const Af<2>& af = au[(k / 2) & 1];
-                    if (k & 1) mma_step<T>(O[i], af, f, k / 2);
-                    else mma_step<T>(O[i], high(af), f, k / 2);
+                    if (k & 1) mma_step<T>(O, af, f, k / 2);
+                    else mma_step<T>(O, high(af), f, k / 2);
                 });
             warp_arrive(&u_empty[g]);
             // rows of 16 values through shared memory: 32 bytes a token, two lanes each
-            e16* sO = theirs + Sm::kO;
+            __syncwarp();
 #pragma unroll
             for (int p = 0; p < kC / 16; ++p) {
-                const Af<1> o = from_acc<T, 1>(O[i][2 * p], O[i][2 * p + 1]);
+                const Af<1> o = from_acc<T, 1>(O[2 * p], O[2 * p + 1]);
                 st_tile_t(sO, Sm::LDO, 16 * p, o.r[0]);
             }
             __syncwarp();
