@@ -115,21 +115,30 @@ __device__ __forceinline__ void from_acc_part(Af<P>& a, int i, float x, float y)
         a.r[1][i] = Num<T>::pack(x - h.x, y - h.y);
     }
 }
-// of a tile stored [m][k], and stored [k][m]
-__device__ __forceinline__ void ld_a(uint32_t* r, const e16* s, int ld, int m0, int k0) {
+// A tile in shared memory by its 32-bit address, in elements.  (With generic
+// pointers the address arithmetic of unrolled loads was most of the code.)
+struct Sh {
+    uint32_t a;
+    __device__ __forceinline__ Sh operator+(int n) const { return Sh{a + 2u * static_cast<uint32_t>(n)}; }
+};
+__device__ __forceinline__ Sh sh(const void* p) { return Sh{smem_u32(p)}; }
+
+// A operands of a tile stored [m][k], and stored [k][m]: the lane's part of the
+// address, then the tile's (a constant where loops are unrolled).
+__device__ __forceinline__ void ld_a(uint32_t* r, Sh s, int ld, int m0, int k0) {
     const int l = threadIdx.x & 31;
-    ldsm4(r, s + (m0 + (l & 15)) * ld + k0 + (l >> 4) * 8);
+    ldsm4(r, (s + ((l & 15) * ld + (l >> 4) * 8) + m0 * ld + k0).a);
 }
-__device__ __forceinline__ void ld_at(uint32_t* r, const e16* s, int ld, int m0, int k0) {
+__device__ __forceinline__ void ld_at(uint32_t* r, Sh s, int ld, int m0, int k0) {
     const int l = threadIdx.x & 31;
-    ldsm4t(r, s + (k0 + (l & 7) + ((l >> 4) & 1) * 8) * ld + m0 + ((l >> 3) & 1) * 8);
+    ldsm4t(r, (s + (((l & 7) + ((l >> 4) & 1) * 8) * ld + ((l >> 3) & 1) * 8) + m0 + k0 * ld).a);
 }
 // 16 columns of B by 16 of the summed index, stored [n][k], and (TR) [k][n]
 template <bool TR>
-__device__ __forceinline__ void ld_b(uint32_t* b, const e16* s, int ld, int n0, int k0) {
+__device__ __forceinline__ void ld_b(uint32_t* b, Sh s, int ld, int n0, int k0) {
     const int l = threadIdx.x & 31;
-    if constexpr (TR) ldsm4t(b, s + (k0 + (l & 7) + ((l >> 3) & 1) * 8) * ld + n0 + ((l >> 4) & 1) * 8);
-    else ldsm4(b, s + (n0 + (l & 7) + ((l >> 4) & 1) * 8) * ld + k0 + ((l >> 3) & 1) * 8);
+    if constexpr (TR) ldsm4t(b, (s + (((l & 7) + ((l >> 3) & 1) * 8) * ld + ((l >> 4) & 1) * 8) + n0 + k0 * ld).a);
+    else ldsm4(b, (s + (((l & 7) + ((l >> 4) & 1) * 8) * ld + ((l >> 3) & 1) * 8) + n0 * ld + k0).a);
 }
 // Tiles that tensor maps bring.  Rows of 64 columns in 128-byte swizzle, 64
 // rows a box, boxes one after another (queries, keys); rows of 16 columns in
@@ -137,22 +146,27 @@ __device__ __forceinline__ void ld_b(uint32_t* b, const e16* s, int ld, int n0, 
 __device__ __forceinline__ int at128(int row, int col) {
     return (col >> 6) * (kC * 64) + row * 64 + ((((col >> 3) & 7) ^ (row & 7)) << 3) + (col & 7);
 }
-__device__ __forceinline__ int at32(int row, int col) { return row * 16 + (((col >> 3) ^ ((row >> 2) & 1)) << 3); }
-
+// The swizzle is (16-byte column) xor (row mod 8), and a lane's row mod 8 is its
+// number mod 8: its own part of the address is made once, a tile's columns are
+// xored in (boxes start on 1024 bytes) and its rows added.
 template <bool TR>
-__device__ __forceinline__ void ld_b128(uint32_t* b, const e16* s, int n0, int k0) {
+__device__ __forceinline__ void ld_b128(uint32_t* b, Sh s, int n0, int k0) {
     const int l = threadIdx.x & 31;
-    if constexpr (TR) ldsm4t(b, s + at128(k0 + (l & 7) + ((l >> 3) & 1) * 8, n0 + ((l >> 4) & 1) * 8));
-    else ldsm4(b, s + at128(n0 + (l & 7) + ((l >> 4) & 1) * 8, k0 + ((l >> 3) & 1) * 8));
+    const int row = (l & 7) + ((TR ? l >> 3 : l >> 4) & 1) * 8, bit = (TR ? l >> 4 : l >> 3) & 1;
+    const uint32_t mine = s.a + row * 128 + ((bit ^ (l & 7)) << 4);
+    const int col = TR ? n0 : k0, r0 = TR ? k0 : n0;
+    const uint32_t at = (mine ^ static_cast<uint32_t>(((col >> 3) & 7) << 4)) + (col >> 6) * (kC * 128) + r0 * 128;
+    if constexpr (TR) ldsm4t(b, at);
+    else ldsm4(b, at);
 }
 // 16 rows of A: tokens m0.. of a group, and (at) its 16 columns by tokens k0..
-__device__ __forceinline__ void ld_a32(uint32_t* r, const e16* s, int m0) {
+__device__ __forceinline__ void ld_a32(uint32_t* r, Sh s, int m0) {
     const int l = threadIdx.x & 31;
-    ldsm4(r, s + at32(m0 + (l & 15), (l >> 4) * 8));
+    ldsm4(r, (s + ((l & 15) * 16 + (((l >> 4) ^ (l >> 2)) & 1) * 8) + m0 * 16).a);
 }
-__device__ __forceinline__ void ld_at32(uint32_t* r, const e16* s, int k0) {
+__device__ __forceinline__ void ld_at32(uint32_t* r, Sh s, int k0) {
     const int l = threadIdx.x & 31;
-    ldsm4t(r, s + at32(k0 + (l & 7) + ((l >> 4) & 1) * 8, ((l >> 3) & 1) * 8));
+    ldsm4t(r, (s + (((l & 7) + ((l >> 4) & 1) * 8) * 16 + (((l >> 3) ^ (l >> 2)) & 1) * 8) + k0 * 16).a);
 }
 template <typename T>
 __device__ __forceinline__ void mma_pair(float* c0, float* c1, const uint32_t* a, const uint32_t* b) {
@@ -161,14 +175,14 @@ __device__ __forceinline__ void mma_pair(float* c0, float* c1, const uint32_t* a
 }
 // A in P planes times one plane of B
 template <typename T, int P, bool TR>
-__device__ __forceinline__ void mm(float* c0, float* c1, const Af<P>& a, const e16* s, int ld, int n0, int k0) {
+__device__ __forceinline__ void mm(float* c0, float* c1, const Af<P>& a, Sh s, int ld, int n0, int k0) {
     uint32_t b[4];
     ld_b<TR>(b, s, ld, n0, k0);
 #pragma unroll
     for (int p = P - 1; p >= 0; --p) mma_pair<T>(c0, c1, a.r[p], b);
 }
 template <typename T, int P, bool TR>
-__device__ __forceinline__ void mm128(float* c0, float* c1, const Af<P>& a, const e16* s, int n0, int k0) {
+__device__ __forceinline__ void mm128(float* c0, float* c1, const Af<P>& a, Sh s, int n0, int k0) {
     uint32_t b[4];
     ld_b128<TR>(b, s, n0, k0);
 #pragma unroll
@@ -176,7 +190,7 @@ __device__ __forceinline__ void mm128(float* c0, float* c1, const Af<P>& a, cons
 }
 // A in P planes times B in two (the product of the low planes is left out)
 template <typename T, int P, bool TR>
-__device__ __forceinline__ void mm_hl(float* c0, float* c1, const Af<P>& a, const e16* hi, const e16* lo, int ld,
+__device__ __forceinline__ void mm_hl(float* c0, float* c1, const Af<P>& a, Sh hi, Sh lo, int ld,
                                       int n0, int k0) {
     uint32_t b[4];
     ld_b<TR>(b, lo, ld, n0, k0);
@@ -228,18 +242,18 @@ template <int P> __device__ __forceinline__ Af<1> high(const Af<P>& a) {
     return Af<1>{{{a.r[0][0], a.r[0][1], a.r[0][2], a.r[0][3]}}};
 }
 // accumulators of 16 rows by 16 columns to a tile [row][col] (as ld_a reads it)
-__device__ __forceinline__ void st_tile(e16* s, int ld, int c0, const uint32_t* r) {
+__device__ __forceinline__ void st_tile(Sh s, int ld, int c0, const uint32_t* r) {
     const int l = threadIdx.x & 31;
     asm volatile("stmatrix.sync.aligned.m8n8.x4.shared.b16 [%0], {%1,%2,%3,%4};" ::"r"(
-                     smem_u32(s + (l & 15) * ld + c0 + (l >> 4) * 8)),
+                     (s + ((l & 15) * ld + (l >> 4) * 8) + c0).a),
                  "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3])
                  : "memory");
 }
 // and to a tile [col][row]
-__device__ __forceinline__ void st_tile_t(e16* s, int ld, int c0, const uint32_t* r) {
+__device__ __forceinline__ void st_tile_t(Sh s, int ld, int c0, const uint32_t* r) {
     const int l = threadIdx.x & 31;
     asm volatile("stmatrix.sync.aligned.m8n8.x4.trans.shared.b16 [%0], {%1,%2,%3,%4};" ::"r"(
-                     smem_u32(s + (c0 + (l & 7) + (l >> 4) * 8) * ld + ((l >> 3) & 1) * 8)),
+                     (s + (((l & 7) + (l >> 4) * 8) * ld + ((l >> 3) & 1) * 8) + c0 * ld).a),
                  "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3])
                  : "memory");
 }
@@ -284,7 +298,7 @@ __device__ __forceinline__ float ratio(const float* G, int i, int j) {
 constexpr int kAld = kC + 8;  // float32 tiles
 
 template <typename T, int KD>
-__global__ void __launch_bounds__(128) planes_prep_k(DArgs a) {
+__global__ void __launch_bounds__(128) planes_prep_k(const __grid_constant__ DArgs a) {
     using F = FmtF<false>;
     const int c = blockIdx.x, h = blockIdx.y, b = blockIdx.z;
     const int len = row_length(a, b);
@@ -360,13 +374,13 @@ __global__ void __launch_bounds__(128) planes_prep_k(DArgs a) {
 #pragma unroll
         for (int k0 = 0; k0 < KD; k0 += 16) {
             Af<1> ak, aq;
-            ld_a(ak.r[0], sK, LD, m0, k0);
-            ld_a(aq.r[0], sQ, LD, m0, k0);
+            ld_a(ak.r[0], sh(sK), LD, m0, k0);
+            ld_a(aq.r[0], sh(sQ), LD, m0, k0);
 #pragma unroll
             for (int p = 0; p < kC / 16; ++p)
                 if (p <= warp) {
                     uint32_t bk[4];
-                    ld_b<false>(bk, sK, LD, 16 * p, k0);
+                    ld_b<false>(bk, sh(sK), LD, 16 * p, k0);
                     mma_pair<T>(kk[2 * p], kk[2 * p + 1], ak.r[0], bk);
                     mma_pair<T>(qk[2 * p], qk[2 * p + 1], aq.r[0], bk);
                 }
@@ -505,7 +519,7 @@ __device__ __forceinline__ void state_store(const float (*S)[4], float* p, int K
 
 // KEEP: S and U are written for a backward.
 template <typename T, int KD, int G, bool KEEP>
-__global__ void __launch_bounds__(Fwd<KD, G>::kWarps * 32) planes_chain_k(DArgs a, const __grid_constant__ Maps maps) {
+__global__ void __launch_bounds__(Fwd<KD, G>::kWarps * 32) planes_chain_k(const __grid_constant__ DArgs a, const __grid_constant__ Maps maps) {
     using Sm = Fwd<KD, G>;
     const int h = blockIdx.y, b = blockIdx.z, hk = h / (a.Hv / a.Hk);
     const int len = row_length(a, b), nc = (len + kC - 1) / kC;
@@ -571,6 +585,7 @@ __global__ void __launch_bounds__(Fwd<KD, G>::kWarps * 32) planes_chain_k(DArgs 
         for (int c = 0; c < nc && ok; ++c) {
             const unsigned char* st = smem + (c & 1) * Sm::kStage;
             const e16* e = reinterpret_cast<const e16*>(st);
+            const Sh es = sh(e);
             const float* ga = reinterpret_cast<const float*>(e + Sm::kGa);
             const float *gam = ga + 2 * kC, *dec = ga + 3 * kC;
             const int64_t id = head * a.n + c;
@@ -590,12 +605,12 @@ __global__ void __launch_bounds__(Fwd<KD, G>::kWarps * 32) planes_chain_k(DArgs 
                     steps<KD / 16>(
                         [&](int i, uint32_t(*f)[4]) {
 #pragma unroll
-                            for (int p = 0; p < 4; ++p) ld_b128<false>(f[p], e + Sm::kK, 16 * p, 16 * i);
+                            for (int p = 0; p < 4; ++p) ld_b128<false>(f[p], es + Sm::kK, 16 * p, 16 * i);
                         },
                         [&](int i, const uint32_t(*f)[4]) {
                             Af<2>& af = as[i & 1];
-                            st_tile(sS, Sm::LDK, 16 * i, af.r[0]);
-                            if constexpr (KEEP) st_tile(sS + 16 * Sm::LDK, Sm::LDK, 16 * i, af.r[1]);
+                            st_tile(sh(sS), Sm::LDK, 16 * i, af.r[0]);
+                            if constexpr (KEEP) st_tile(sh(sS) + 16 * Sm::LDK, Sm::LDK, 16 * i, af.r[1]);
                             mma_step_with<T>(X, af, f, [&](int q) {
                                 if (i + 1 < KD / 16) {
                                     const float* s = S[2 * i + 2 + q / 2];
@@ -617,7 +632,7 @@ __global__ void __launch_bounds__(Fwd<KD, G>::kWarps * 32) planes_chain_k(DArgs 
 #pragma unroll
                 for (int p = 0; p < kC / 16; ++p) {
                     uint32_t r[4];
-                    ld_at32(r, e + Sm::kV + warp * kC * 16, 16 * p);
+                    ld_at32(r, es + Sm::kV + warp * kC * 16, 16 * p);
 #pragma unroll
                     for (int i = 0; i < 2; ++i) {
                         const float2 f = *reinterpret_cast<const float2*>(gam + 16 * p + 8 * i + 2 * L.t);
@@ -650,7 +665,7 @@ __global__ void __launch_bounds__(Fwd<KD, G>::kWarps * 32) planes_chain_k(DArgs 
                         [&](int i, uint32_t(*f)[4]) {
 #pragma unroll
                             for (int p = 0; p < 4; ++p)
-                                if (p >= i / 2) ld_b<false>(f[p], e + Sm::kT + (i & 1 ? 0 : kCC), kTld, 16 * p, 16 * (i / 2));
+                                if (p >= i / 2) ld_b<false>(f[p], es + Sm::kT + (i & 1 ? 0 : kCC), kTld, 16 * p, 16 * (i / 2));
                         },
                         [&](int i, const uint32_t(*f)[4]) {
                             const int kk = i / 2;
@@ -679,13 +694,13 @@ __global__ void __launch_bounds__(Fwd<KD, G>::kWarps * 32) planes_chain_k(DArgs 
                     steps<4 * Q>(
                         [&](int i, uint32_t(*f)[4]) {
 #pragma unroll
-                            for (int p = 0; p < 4; ++p) ld_b128<true>(f[p], e + Sm::kK, 64 * (i % Q) + 16 * p, 16 * (i / Q));
+                            for (int p = 0; p < 4; ++p) ld_b128<true>(f[p], es + Sm::kK, 64 * (i % Q) + 16 * p, 16 * (i / Q));
                         },
                         [&](int i, const uint32_t(*f)[4]) {
                             const int kk = i / Q;
                             if (i % Q == 0) {
-                                st_tile(sU, kTld, 16 * kk, up[kk & 1].r[0]);
-                                st_tile(sU + 16 * kTld, kTld, 16 * kk, up[kk & 1].r[1]);
+                                st_tile(sh(sU), kTld, 16 * kk, up[kk & 1].r[0]);
+                                st_tile(sh(sU) + 16 * kTld, kTld, 16 * kk, up[kk & 1].r[1]);
                             }
                             mma_step_with<T>(S + 8 * (i % Q), ud[kk & 1], f, [&](int q) {
                                 if (kk + 1 < 4) {
@@ -717,6 +732,7 @@ __global__ void __launch_bounds__(Fwd<KD, G>::kWarps * 32) planes_chain_k(DArgs 
     for (int c = 0; c < nc && ok; ++c) {
         const unsigned char* st = smem + (c & 1) * Sm::kStage;
         const e16* e = reinterpret_cast<const e16*>(st);
+        const Sh es = sh(e);
         const float* sgam = reinterpret_cast<const float*>(e + Sm::kGa) + 4 * kC;
         const int rows = min(kC, len - c * kC), all = min(kC, a.L - c * kC);
         ok = warp_wait(&full[c & 1], (c >> 1) & 1);
@@ -736,9 +752,9 @@ __global__ void __launch_bounds__(Fwd<KD, G>::kWarps * 32) planes_chain_k(DArgs 
             Af<1> as[2];
             steps<KD / 16>(
                 [&](int k, uint32_t(*f)[4]) {
-                    ld_a(as[k & 1].r[0], sS, Sm::LDK, 0, 16 * k);
+                    ld_a(as[k & 1].r[0], sh(sS), Sm::LDK, 0, 16 * k);
 #pragma unroll
-                    for (int p = 0; p < 4; ++p) ld_b128<false>(f[p], e + Sm::kQ, 16 * p, 16 * k);
+                    for (int p = 0; p < 4; ++p) ld_b128<false>(f[p], es + Sm::kQ, 16 * p, 16 * k);
                 },
                 [&](int k, const uint32_t(*f)[4]) { mma_step<T>(O, as[k & 1], f); });
             warp_arrive(&s_empty[g]);
@@ -763,17 +779,18 @@ __global__ void __launch_bounds__(Fwd<KD, G>::kWarps * 32) planes_chain_k(DArgs 
                 O[j][2] = o.z;
                 O[j][3] = o.w;
             }
+            const Sh ts = sh(theirs);
             ok = warp_wait(&u_full[g], c & 1) && ok;
             Af<2> au[2];
             steps<8>(
                 [&](int k, uint32_t(*f)[4]) {
                     if (!(k & 1)) {
-                        ld_a(au[(k / 2) & 1].r[0], theirs + Sm::kU, kTld, 0, 8 * k);
-                        ld_a(au[(k / 2) & 1].r[1], theirs + Sm::kU + 16 * kTld, kTld, 0, 8 * k);
+                        ld_a(au[(k / 2) & 1].r[0], ts + Sm::kU, kTld, 0, 8 * k);
+                        ld_a(au[(k / 2) & 1].r[1], ts + Sm::kU + 16 * kTld, kTld, 0, 8 * k);
                     }
 #pragma unroll
                     for (int p = 0; p < 4; ++p)
-                        if (p >= k / 2) ld_b<false>(f[p], e + Sm::kM + (k & 1 ? 0 : kCC), kTld, 16 * p, 16 * (k / 2));
+                        if (p >= k / 2) ld_b<false>(f[p], es + Sm::kM + (k & 1 ? 0 : kCC), kTld, 16 * p, 16 * (k / 2));
                 },
                 [&](int k, const uint32_t(*f)[4]) {
                     const Af<2>& af = au[(k / 2) & 1];
@@ -786,7 +803,7 @@ __global__ void __launch_bounds__(Fwd<KD, G>::kWarps * 32) planes_chain_k(DArgs 
 #pragma unroll
             for (int p = 0; p < kC / 16; ++p) {
                 const Af<1> o = from_acc<T, 1>(O[2 * p], O[2 * p + 1]);
-                st_tile_t(sO, Sm::LDO, 16 * p, o.r[0]);
+                st_tile_t(sh(sO), Sm::LDO, 16 * p, o.r[0]);
             }
             __syncwarp();
 #pragma unroll
@@ -829,7 +846,7 @@ struct Rev {
 };
 
 template <typename T, int KD, int G>
-__global__ void __launch_bounds__(Rev<KD, G>::kWarps * 32) planes_rchain_k(DArgs a, const __grid_constant__ Maps maps) {
+__global__ void __launch_bounds__(Rev<KD, G>::kWarps * 32) planes_rchain_k(const __grid_constant__ DArgs a, const __grid_constant__ Maps maps) {
     using Sm = Rev<KD, G>;
     const int h = blockIdx.y, b = blockIdx.z, hk = h / (a.Hv / a.Hk);
     const int len = row_length(a, b), nc = (len + kC - 1) / kC;
@@ -896,6 +913,7 @@ __global__ void __launch_bounds__(Rev<KD, G>::kWarps * 32) planes_rchain_k(DArgs
         for (int i = 0; i < nc && ok; ++i) {
             const int c = nc - 1 - i;
             const e16* e = reinterpret_cast<const e16*>(smem + (i & 1) * Sm::kStage);
+            const Sh es = sh(e);
             const float* ga = reinterpret_cast<const float*>(e + Sm::kGa);
             const float *gam = ga + 2 * kC, *dec = ga + 3 * kC;
             const int64_t id = head * a.n + c;
@@ -910,12 +928,12 @@ __global__ void __launch_bounds__(Rev<KD, G>::kWarps * 32) planes_rchain_k(DArgs
                     steps<KD / 16>(
                         [&](int k, uint32_t(*f)[4]) {
 #pragma unroll
-                            for (int p = 0; p < 4; ++p) ld_b128<false>(f[p], e + Sm::kK, 16 * p, 16 * k);
+                            for (int p = 0; p < 4; ++p) ld_b128<false>(f[p], es + Sm::kK, 16 * p, 16 * k);
                         },
                         [&](int k, const uint32_t(*f)[4]) {
                             Af<2>& af = as[k & 1];
-                            st_tile(sS, Sm::LDK, 16 * k, af.r[0]);
-                            st_tile(sS + 16 * Sm::LDK, Sm::LDK, 16 * k, af.r[1]);
+                            st_tile(sh(sS), Sm::LDK, 16 * k, af.r[0]);
+                            st_tile(sh(sS) + 16 * Sm::LDK, Sm::LDK, 16 * k, af.r[1]);
                             mma_step_with<T>(U, af, f, [&](int q) {
                                 if (k + 1 < KD / 16) {
                                     const float* s = S[2 * k + 2 + q / 2];
@@ -945,10 +963,10 @@ __global__ void __launch_bounds__(Rev<KD, G>::kWarps * 32) planes_rchain_k(DArgs
                     Af<1> ad[2];
                     steps<8>(
                         [&](int k, uint32_t(*f)[4]) {
-                            if (!(k & 1)) ld_at32(ad[(k / 2) & 1].r[0], e + Sm::kD + warp * kC * 16, 8 * k);
+                            if (!(k & 1)) ld_at32(ad[(k / 2) & 1].r[0], es + Sm::kD + warp * kC * 16, 8 * k);
 #pragma unroll
                             for (int p = 0; p < 4; ++p)
-                                if (p <= k / 2) ld_b<true>(f[p], e + Sm::kM + (k & 1 ? 0 : kCC), kTld, 16 * p, 16 * (k / 2));
+                                if (p <= k / 2) ld_b<true>(f[p], es + Sm::kM + (k & 1 ? 0 : kCC), kTld, 16 * p, 16 * (k / 2));
                         },
                         [&](int k, const uint32_t(*f)[4]) { mma_step<T>(U, ad[(k / 2) & 1], f, 0, k / 2 + 1); });
                 }
@@ -976,7 +994,7 @@ __global__ void __launch_bounds__(Rev<KD, G>::kWarps * 32) planes_rchain_k(DArgs
                             const int kk = 3 - k / 2;
 #pragma unroll
                             for (int p = 0; p < 4; ++p)
-                                if (p <= kk) ld_b<true>(f[p], e + Sm::kT + (k & 1 ? 0 : kCC), kTld, 16 * p, 16 * kk);
+                                if (p <= kk) ld_b<true>(f[p], es + Sm::kT + (k & 1 ? 0 : kCC), kTld, 16 * p, 16 * kk);
                         },
                         [&](int k, const uint32_t(*f)[4]) {
                             const int kk = 3 - k / 2;
@@ -1012,13 +1030,13 @@ __global__ void __launch_bounds__(Rev<KD, G>::kWarps * 32) planes_rchain_k(DArgs
                         [&](int k, uint32_t(*f)[4]) {
 #pragma unroll
                             for (int p = 0; p < 4; ++p)
-                                ld_b128<true>(f[p], e + Sm::kK, 64 * (k % Q) + 16 * p, 16 * (3 - k / Q));
+                                ld_b128<true>(f[p], es + Sm::kK, 64 * (k % Q) + 16 * p, 16 * (3 - k / Q));
                         },
                         [&](int k, const uint32_t(*f)[4]) {
                             const int kk = 3 - k / Q;
                             if (k % Q == 0) {
-                                st_tile(sX, kTld, 16 * kk, xp[kk & 1].r[0]);
-                                st_tile(sX + 16 * kTld, kTld, 16 * kk, xp[kk & 1].r[1]);
+                                st_tile(sh(sX), kTld, 16 * kk, xp[kk & 1].r[0]);
+                                st_tile(sh(sX) + 16 * kTld, kTld, 16 * kk, xp[kk & 1].r[1]);
                             }
                             mma_step_with<T>(S + 8 * (k % Q), xd[kk & 1], f, [&](int q) {
                                 if (kk > 0) {
@@ -1046,6 +1064,7 @@ __global__ void __launch_bounds__(Rev<KD, G>::kWarps * 32) planes_rchain_k(DArgs
     // ---- (scale gam dO)^T Q of the groups ----
     for (int i = 0; i < nc && ok; ++i) {
         const e16* e = reinterpret_cast<const e16*>(smem + (i & 1) * Sm::kStage);
+        const Sh es = sh(e);
         const float* sgam = reinterpret_cast<const float*>(e + Sm::kGa) + 4 * kC;
         ok = warp_wait(&full[i & 1], (i >> 1) & 1);
         for (int g = warp - G; g < G; g += Sm::H) {
@@ -1056,13 +1075,13 @@ __global__ void __launch_bounds__(Rev<KD, G>::kWarps * 32) planes_rchain_k(DArgs
             steps<4 * Q>(
                 [&](int k, uint32_t(*f)[4]) {
 #pragma unroll
-                    for (int p = 0; p < 4; ++p) ld_b128<true>(f[p], e + Sm::kQ, 64 * (k % Q) + 16 * p, 16 * (k / Q));
+                    for (int p = 0; p < 4; ++p) ld_b128<true>(f[p], es + Sm::kQ, 64 * (k % Q) + 16 * p, 16 * (k / Q));
                 },
                 [&](int k, const uint32_t(*f)[4]) {
                     const int kk = k / Q;
                     if (k % Q == 0) {
                         uint32_t r[4];
-                        ld_at32(r, e + Sm::kD + g * kC * 16, 16 * kk);
+                        ld_at32(r, es + Sm::kD + g * kC * 16, 16 * kk);
                         float y[2][4];
 #pragma unroll
                         for (int x = 0; x < 2; ++x) {
@@ -1142,8 +1161,128 @@ __device__ __forceinline__ void rows_out(const float (*x)[4], e16* p, int64_t st
     }
 }
 
+// The loads of the next tile, by warp 0.  Where they are is kept in shared memory
+// (at: chunk, value head, first value column; tiles and chunks so far; waits for
+// `land` so far), as a lane has no registers for it.
+template <int KD>
+__device__ __forceinline__ bool grad_produce(const DArgs& a, const Maps& maps, unsigned char* smem) {
+    using Sm = Grad<KD>;
+    constexpr int VT = Sm::VT;
+    uint64_t* full = reinterpret_cast<uint64_t*>(smem + Sm::kBars);
+    uint64_t *empty = full + 2, *qfull = full + 4, *qempty = full + 6, *land = full + 8;
+    int* at = reinterpret_cast<int*>(land + 1);
+    const int rep = a.Hv / a.Hk, items = a.B * a.Hk * a.n;
+    const Lane L;
+    bool ok = true;
+            int it = at[0], h = at[1], v0 = at[2];
+            if (it >= items) return true;
+            const int bh = it / a.n, c = it - bh * a.n, b = bh / a.Hk, hk = bh - b * a.Hk, t0 = c * kC;
+            const int ptile = at[3], pseen = at[4];
+            int landed = at[5];
+            const int rows = min(kC, row_length(a, b) - t0);
+            const bool tail = rows < min(kC, a.L - t0);
+            if (h < 0) {  // a new chunk: its keys and queries
+                h = hk * rep;
+                e16* e = reinterpret_cast<e16*>(smem + 2 * Sm::kStage + (pseen & 1) * Sm::kKQ);
+                uint64_t* bar = tail ? land : &qfull[pseen & 1];
+                ok = warp_wait(&qempty[pseen & 1], ((pseen >> 1) & 1) ^ 1) && ok;
+                if (L.l == 0) {
+                    mbar_expect_tx(bar, Sm::kKQ);
+    #pragma unroll
+                    for (int x = 0; x < KD; x += 64) {
+                        tma_load(e + Sm::kK + x * kC, &maps.k, bar, x, t0, hk, b);
+                        tma_load(e + Sm::kQ + x * kC, &maps.q, bar, x, t0, hk, b);
+                    }
+                }
+                __syncwarp();
+                if (tail) {
+                    ok = warp_wait(land, landed++ & 1) && ok;
+                    zero_rows<64>(e + Sm::kK, 2 * (KD / 64), rows);
+                    fence_async();
+                    warp_arrive(&qfull[pseen & 1]);
+                }
+            }
+            const int vn = min(VT, a.Vp - v0);
+            e16* e = reinterpret_cast<e16*>(smem + (ptile & 1) * Sm::kStage);
+            uint64_t* bar = tail ? land : &full[ptile & 1];
+            ok = warp_wait(&empty[ptile & 1], ((ptile >> 1) & 1) ^ 1) && ok;
+            if (L.l == 0) {
+                const int64_t id = (static_cast<int64_t>(b) * a.Hv + h) * a.n + c;
+                mbar_expect_tx(bar, vn * (kC + 4 * kTld + 4 * Sm::LDK) * 2 + kGates * 4);
+                for (int v = 0; v < vn; v += 16) tma_load(e + Sm::kD + v * kC, &maps.d, bar, v0 + v, t0, h, b);
+                const e16* U = static_cast<const e16*>(a.U) + (id * 2 * a.Vp + v0) * kTld;
+                const e16* X = static_cast<const e16*>(a.dV) + (id * 2 * a.Vp + v0) * kTld;
+                const e16* S = static_cast<const e16*>(a.S) + (id * 2 * a.Vp + v0) * Sm::LDK;
+                const e16* R = static_cast<const e16*>(a.dS) + (id * 2 * a.Vp + v0) * Sm::LDK;
+                for (int p = 0; p < 2; ++p) {
+                    bulk_load(e + Sm::kS + p * VT * Sm::LDK, S + static_cast<int64_t>(p) * a.Vp * Sm::LDK, vn * Sm::LDK * 2, bar);
+                    bulk_load(e + Sm::kR + p * VT * Sm::LDK, R + static_cast<int64_t>(p) * a.Vp * Sm::LDK, vn * Sm::LDK * 2, bar);
+                    bulk_load(e + Sm::kU + p * VT * kTld, U + static_cast<int64_t>(p) * a.Vp * kTld, vn * kTld * 2, bar);
+                    bulk_load(e + Sm::kX + p * VT * kTld, X + static_cast<int64_t>(p) * a.Vp * kTld, vn * kTld * 2, bar);
+                }
+                bulk_load(e + Sm::kGa, a.gates + id * kGates, kGates * 4, bar);
+            }
+            __syncwarp();
+            if (tail) {
+                ok = warp_wait(land, landed++ & 1) && ok;
+                zero_rows<16>(e + Sm::kD, vn / 16, rows);
+                fence_async();
+                warp_arrive(&full[ptile & 1]);
+            }
+            // the next tile: of this head, of the next, or of the next chunk with a token
+            int seen_next = pseen;
+            v0 += VT;
+            if (v0 >= a.Vp) {
+                v0 = 0;
+                if (++h == (hk + 1) * rep) {
+                    h = -1;
+                    ++seen_next;
+                    for (it += gridDim.x; it < items; it += gridDim.x) {
+                        const int nbh = it / a.n;
+                        if (row_length(a, nbh / a.Hk) > (it - nbh * a.n) * kC) break;
+                    }
+                }
+            }
+            if (L.l == 0) {
+                at[0] = it;
+                at[1] = h;
+                at[2] = v0;
+                at[3] = ptile + 1;
+                at[4] = seen_next;
+                at[5] = landed;
+            }
+            __syncwarp();
+    return ok;
+}
+
+// Zeros for a chunk behind the sequence.
+__device__ __forceinline__ void grad_zero(const DArgs& a, int b, int hk, int c) {
+    const int rep = a.Hv / a.Hk, all = min(kC, a.L - c * kC), tid = threadIdx.x, n = blockDim.x;
+    const int64_t row0 = static_cast<int64_t>(b) * a.L + static_cast<int64_t>(c) * kC;
+    const int64_t qst = static_cast<int64_t>(a.Hk) * a.K, vst = static_cast<int64_t>(a.Hv) * a.V;
+    const uint4 z = make_uint4(0, 0, 0, 0);
+#pragma unroll 1
+    for (int i = tid; i < all * (a.K / 8); i += n) {
+        const int64_t o = (row0 + i / (a.K / 8)) * qst + static_cast<int64_t>(hk) * a.K + i % (a.K / 8) * 8;
+        *reinterpret_cast<uint4*>(static_cast<e16*>(a.dq) + o) = z;
+        *reinterpret_cast<uint4*>(static_cast<e16*>(a.dk) + o) = z;
+    }
+#pragma unroll 1
+    for (int h = hk * rep; h < (hk + 1) * rep; ++h) {
+#pragma unroll 1
+        for (int i = tid; i < all * (a.V / 8); i += n)
+            *reinterpret_cast<uint4*>(static_cast<e16*>(a.dv) + (row0 + i / (a.V / 8)) * vst + static_cast<int64_t>(h) * a.V +
+                                      i % (a.V / 8) * 8) = z;
+#pragma unroll 1
+        for (int i = tid; i < all; i += n) {
+            gate_store(a.dg, a.gate_dtype, (row0 + i) * a.Hv + h, 0.f);
+            gate_store(a.dbeta, a.gate_dtype, (row0 + i) * a.Hv + h, 0.f);
+        }
+    }
+}
+
 template <typename T, int KD>
-__global__ void __launch_bounds__(32 * kGradWarps, 1) planes_grad_k(DArgs a, float* group, const __grid_constant__ Maps maps) {
+__global__ void __launch_bounds__(32 * kGradWarps, 1) planes_grad_k(const __grid_constant__ DArgs a, float* group, const __grid_constant__ Maps maps) {
     using Sm = Grad<KD>;
     constexpr int VT = Sm::VT, NT = KD / 16;  // accumulator tiles of a half of the key columns
     extern __shared__ __align__(128) unsigned char smem_raw[];
@@ -1166,89 +1305,8 @@ __global__ void __launch_bounds__(32 * kGradWarps, 1) planes_grad_k(DArgs a, flo
     const int items = a.B * a.Hk * a.n;
     bool ok = true;
     int tile = 0, seen = 0;  // tiles and chunks so far
-    // Where the loads are (warp 0 alone; in shared memory, as a lane has no registers for it):
-    // chunk, value head, first value column; tiles and chunks so far; waits for `land` so far.
     int* at = reinterpret_cast<int*>(land + 1);
-    auto produce = [&]() {
-        int it = at[0], h = at[1], v0 = at[2];
-        if (it >= items) return;
-        const int bh = it / a.n, c = it - bh * a.n, b = bh / a.Hk, hk = bh - b * a.Hk, t0 = c * kC;
-        const int ptile = at[3], pseen = at[4];
-        int landed = at[5];
-        const int rows = min(kC, row_length(a, b) - t0);
-        const bool tail = rows < min(kC, a.L - t0);
-        if (h < 0) {  // a new chunk: its keys and queries
-            h = hk * rep;
-            e16* e = reinterpret_cast<e16*>(smem + 2 * Sm::kStage + (pseen & 1) * Sm::kKQ);
-            uint64_t* bar = tail ? land : &qfull[pseen & 1];
-            ok = warp_wait(&qempty[pseen & 1], ((pseen >> 1) & 1) ^ 1) && ok;
-            if (L.l == 0) {
-                mbar_expect_tx(bar, Sm::kKQ);
-#pragma unroll
-                for (int x = 0; x < KD; x += 64) {
-                    tma_load(e + Sm::kK + x * kC, &maps.k, bar, x, t0, hk, b);
-                    tma_load(e + Sm::kQ + x * kC, &maps.q, bar, x, t0, hk, b);
-                }
-            }
-            __syncwarp();
-            if (tail) {
-                ok = warp_wait(land, landed++ & 1) && ok;
-                zero_rows<64>(e + Sm::kK, 2 * (KD / 64), rows);
-                fence_async();
-                warp_arrive(&qfull[pseen & 1]);
-            }
-        }
-        const int vn = min(VT, a.Vp - v0);
-        e16* e = reinterpret_cast<e16*>(smem + (ptile & 1) * Sm::kStage);
-        uint64_t* bar = tail ? land : &full[ptile & 1];
-        ok = warp_wait(&empty[ptile & 1], ((ptile >> 1) & 1) ^ 1) && ok;
-        if (L.l == 0) {
-            const int64_t id = (static_cast<int64_t>(b) * a.Hv + h) * a.n + c;
-            mbar_expect_tx(bar, vn * (kC + 4 * kTld + 4 * Sm::LDK) * 2 + kGates * 4);
-            for (int v = 0; v < vn; v += 16) tma_load(e + Sm::kD + v * kC, &maps.d, bar, v0 + v, t0, h, b);
-            const e16* U = static_cast<const e16*>(a.U) + (id * 2 * a.Vp + v0) * kTld;
-            const e16* X = static_cast<const e16*>(a.dV) + (id * 2 * a.Vp + v0) * kTld;
-            const e16* S = static_cast<const e16*>(a.S) + (id * 2 * a.Vp + v0) * Sm::LDK;
-            const e16* R = static_cast<const e16*>(a.dS) + (id * 2 * a.Vp + v0) * Sm::LDK;
-            for (int p = 0; p < 2; ++p) {
-                bulk_load(e + Sm::kS + p * VT * Sm::LDK, S + static_cast<int64_t>(p) * a.Vp * Sm::LDK, vn * Sm::LDK * 2, bar);
-                bulk_load(e + Sm::kR + p * VT * Sm::LDK, R + static_cast<int64_t>(p) * a.Vp * Sm::LDK, vn * Sm::LDK * 2, bar);
-                bulk_load(e + Sm::kU + p * VT * kTld, U + static_cast<int64_t>(p) * a.Vp * kTld, vn * kTld * 2, bar);
-                bulk_load(e + Sm::kX + p * VT * kTld, X + static_cast<int64_t>(p) * a.Vp * kTld, vn * kTld * 2, bar);
-            }
-            bulk_load(e + Sm::kGa, a.gates + id * kGates, kGates * 4, bar);
-        }
-        __syncwarp();
-        if (tail) {
-            ok = warp_wait(land, landed++ & 1) && ok;
-            zero_rows<16>(e + Sm::kD, vn / 16, rows);
-            fence_async();
-            warp_arrive(&full[ptile & 1]);
-        }
-        // the next tile: of this head, of the next, or of the next chunk with a token
-        int seen_next = pseen;
-        v0 += VT;
-        if (v0 >= a.Vp) {
-            v0 = 0;
-            if (++h == (hk + 1) * rep) {
-                h = -1;
-                ++seen_next;
-                for (it += gridDim.x; it < items; it += gridDim.x) {
-                    const int nbh = it / a.n;
-                    if (row_length(a, nbh / a.Hk) > (it - nbh * a.n) * kC) break;
-                }
-            }
-        }
-        if (L.l == 0) {
-            at[0] = it;
-            at[1] = h;
-            at[2] = v0;
-            at[3] = ptile + 1;
-            at[4] = seen_next;
-            at[5] = landed;
-        }
-        __syncwarp();
-    };
+    bool first = true;
     if (warp == 0) {
         int it = blockIdx.x;
         for (; it < items; it += gridDim.x) {
@@ -1261,9 +1319,8 @@ __global__ void __launch_bounds__(32 * kGradWarps, 1) planes_grad_k(DArgs a, flo
             at[2] = at[3] = at[4] = at[5] = 0;
         }
         __syncwarp();
-        produce();
     }
-    const int rg = warp & 3, half = (warp >> 2) & 1, m0 = rg * 16, n0 = half * (KD / 2);
+    const int rg = (warp >> 1) & 3, half = warp & 1, m0 = rg * 16, n0 = half * (KD / 2);
     const bool writer = warp >= 8;
     const int r0 = m0 + L.g, r1 = r0 + 8;
     e16* sN = reinterpret_cast<e16*>(smem + Sm::kN);
@@ -1279,27 +1336,12 @@ __global__ void __launch_bounds__(32 * kGradWarps, 1) planes_grad_k(DArgs a, flo
         const int qst = a.Hk * a.K, vst = a.Hv * a.V;
         e16* dq = static_cast<e16*>(a.dq) + row0 * qst + hk * a.K;
         e16* dk = static_cast<e16*>(a.dk) + row0 * qst + hk * a.K;
-        if (rows <= 0) {  // behind the sequence
-            const uint4 z = make_uint4(0, 0, 0, 0);
-            for (int i = tid; i < all * (a.K / 8); i += 32 * kGradWarps) {
-                const int64_t o = static_cast<int64_t>(i / (a.K / 8)) * qst + i % (a.K / 8) * 8;
-                *reinterpret_cast<uint4*>(dq + o) = z;
-                *reinterpret_cast<uint4*>(dk + o) = z;
-            }
-            for (int h = hk * rep; h < (hk + 1) * rep; ++h) {
-                e16* dv = static_cast<e16*>(a.dv) + row0 * vst + static_cast<int64_t>(h) * a.V;
-                for (int i = tid; i < all * (a.V / 8); i += 32 * kGradWarps)
-                    *reinterpret_cast<uint4*>(dv + static_cast<int64_t>(i / (a.V / 8)) * vst + i % (a.V / 8) * 8) = z;
-                for (int i = tid; i < all; i += 32 * kGradWarps) {
-                    gate_store(a.dg, a.gate_dtype, (row0 + i) * a.Hv + h, 0.f);
-                    gate_store(a.dbeta, a.gate_dtype, (row0 + i) * a.Hv + h, 0.f);
-                }
-            }
+        if (rows <= 0) {
+            grad_zero(a, b, hk, c);
             continue;
         }
         const e16* kq = reinterpret_cast<const e16*>(smem + 2 * Sm::kStage + (seen & 1) * Sm::kKQ);
         const e16 *sK = kq + Sm::kK, *sQ = kq + Sm::kQ;
-        ok = warp_wait(&qfull[seen & 1], (seen >> 1) & 1);
         for (int h = hk * rep; h < (hk + 1) * rep; ++h) {
             e16* dv = static_cast<e16*>(a.dv) + row0 * vst + static_cast<int64_t>(h) * a.V;
             // readers: dQ and dK_read; writers: dK_write, and dO U^T (half 0) or dV U^T (half 1)
@@ -1309,21 +1351,26 @@ __global__ void __launch_bounds__(32 * kGradWarps, 1) planes_grad_k(DArgs a, flo
             for (int v0 = 0; v0 < a.Vp; v0 += VT, ++tile) {
                 const int vn = min(VT, a.Vp - v0);
                 const e16* e = reinterpret_cast<const e16*>(smem + (tile & 1) * Sm::kStage);
+                const Sh es = sh(e);
                 const float* ga = reinterpret_cast<const float*>(e + Sm::kGa);
-                if (warp == 0) produce();
+                if (warp == 0) {
+#pragma unroll 1
+                    for (int i = first ? 0 : 1; i < 2; ++i) ok = grad_produce<KD>(a, maps, smem) && ok;
+                    first = false;
+                }
                 ok = warp_wait(&full[tile & 1], (tile >> 1) & 1) && ok;
 #pragma unroll
                 for (int kk = 0; kk < VT / 16; ++kk) {
                     if (16 * kk >= vn) break;
                     if (!writer) {
                         Af<1> fd, fx;
-                        ld_a32(fd.r[0], e + Sm::kD + kk * kC * 16, m0);
-                        ld_at(fx.r[0], e + Sm::kX, kTld, m0, 16 * kk);
+                        ld_a32(fd.r[0], es + Sm::kD + kk * kC * 16, m0);
+                        ld_at(fx.r[0], es + Sm::kX, kTld, m0, 16 * kk);
 #pragma unroll
                         for (int p = 0; p < NT / 2; ++p) {
                             uint32_t sh[4], sl[4];
-                            ld_b<true>(sl, e + Sm::kS + VT * Sm::LDK, Sm::LDK, n0 + 16 * p, 16 * kk);
-                            ld_b<true>(sh, e + Sm::kS, Sm::LDK, n0 + 16 * p, 16 * kk);
+                            ld_b<true>(sl, es + Sm::kS + VT * Sm::LDK, Sm::LDK, n0 + 16 * p, 16 * kk);
+                            ld_b<true>(sh, es + Sm::kS, Sm::LDK, n0 + 16 * p, 16 * kk);
                             mma_pair<T>(x[2 * p], x[2 * p + 1], fd.r[0], sl);
                             mma_pair<T>(y[2 * p], y[2 * p + 1], fx.r[0], sl);
                             mma_pair<T>(x[2 * p], x[2 * p + 1], fd.r[0], sh);
@@ -1341,18 +1388,18 @@ __global__ void __launch_bounds__(32 * kGradWarps, 1) planes_grad_k(DArgs a, flo
                     } else {
                         Af<1> left;
                         Af<2> fu;
-                        ld_at(fu.r[0], e + Sm::kU, kTld, m0, 16 * kk);
-                        ld_at(fu.r[1], e + Sm::kU + VT * kTld, kTld, m0, 16 * kk);
-                        if (half) ld_at(left.r[0], e + Sm::kX, kTld, m0, 16 * kk);
-                        else ld_a32(left.r[0], e + Sm::kD + kk * kC * 16, m0);
+                        ld_at(fu.r[0], es + Sm::kU, kTld, m0, 16 * kk);
+                        ld_at(fu.r[1], es + Sm::kU + VT * kTld, kTld, m0, 16 * kk);
+                        if (half) ld_at(left.r[0], es + Sm::kX, kTld, m0, 16 * kk);
+                        else ld_a32(left.r[0], es + Sm::kD + kk * kC * 16, m0);
 #pragma unroll
                         for (int p = 0; p < NT / 2; ++p) {
                             uint32_t rh[4], rl[4];
-                            ld_b<true>(rl, e + Sm::kR + VT * Sm::LDK, Sm::LDK, n0 + 16 * p, 16 * kk);
-                            ld_b<true>(rh, e + Sm::kR, Sm::LDK, n0 + 16 * p, 16 * kk);
+                            ld_b<true>(rl, es + Sm::kR + VT * Sm::LDK, Sm::LDK, n0 + 16 * p, 16 * kk);
+                            ld_b<true>(rh, es + Sm::kR, Sm::LDK, n0 + 16 * p, 16 * kk);
                             mma_pair<T>(x[2 * p], x[2 * p + 1], fu.r[0], rl);
                             if (p <= rg)
-                                mm_hl<T, 1, true>(y[2 * p], y[2 * p + 1], left, e + Sm::kU, e + Sm::kU + VT * kTld, kTld, 16 * p,
+                                mm_hl<T, 1, true>(y[2 * p], y[2 * p + 1], left, es + Sm::kU, es + Sm::kU + VT * kTld, kTld, 16 * p,
                                                16 * kk);
                             mma_pair<T>(x[2 * p], x[2 * p + 1], fu.r[1], rh);
                             mma_pair<T>(x[2 * p], x[2 * p + 1], fu.r[0], rh);
@@ -1360,11 +1407,11 @@ __global__ void __launch_bounds__(32 * kGradWarps, 1) planes_grad_k(DArgs a, flo
 #pragma unroll
                         for (int p = NT / 2; p < kC / 16; ++p)
                             if (p <= rg)
-                                mm_hl<T, 1, true>(y[2 * p], y[2 * p + 1], left, e + Sm::kU, e + Sm::kU + VT * kTld, kTld, 16 * p,
+                                mm_hl<T, 1, true>(y[2 * p], y[2 * p + 1], left, es + Sm::kU, es + Sm::kU + VT * kTld, kTld, 16 * p,
                                                16 * kk);
                         if (half) {  // dbeta = (dV / beta).(U / beta)
                             uint32_t xl[4];
-                            ld_at(xl, e + Sm::kX + VT * kTld, kTld, m0, 16 * kk);
+                            ld_at(xl, es + Sm::kX + VT * kTld, kTld, m0, 16 * kk);
 #pragma unroll
                             for (int i = 0; i < 4; ++i) {
                                 const float2 p = Num<T>::unpack(left.r[0][i]), q = Num<T>::unpack(xl[i]);
@@ -1377,6 +1424,7 @@ __global__ void __launch_bounds__(32 * kGradWarps, 1) planes_grad_k(DArgs a, flo
                         }
                     }
                 }
+#pragma unroll 1
                 for (int i = tid; i < vn * (KD / 8); i += 32 * kGradWarps) {  // <S0, dS1>
                     const int o = i / (KD / 8) * Sm::LDK + i % (KD / 8) * 8;
                     const uint4 sh = *reinterpret_cast<const uint4*>(e + Sm::kS + o);
@@ -1416,6 +1464,7 @@ __global__ void __launch_bounds__(32 * kGradWarps, 1) planes_grad_k(DArgs a, flo
                 }
                 warp_arrive(&empty[tile & 1]);
             }
+            ok = warp_wait(&qfull[seen & 1], (seen >> 1) & 1) && ok;
             sd = warp_sum(sd);
             float tw = 0.f;  // writers: k.(d U dS1^T)
 #pragma unroll
@@ -1453,19 +1502,18 @@ __global__ void __launch_bounds__(32 * kGradWarps, 1) planes_grad_k(DArgs a, flo
             }
             sync_compute();  // N, E
             if (!writer) {
-#pragma unroll
-                for (int kk = 0; kk < kC / 16; ++kk) {
-                    if (kk > rg) break;  // rows of N and E
+#pragma unroll 1
+                for (int kk = 0; kk <= rg; ++kk) {  // rows of N and E
                     Af<2> fn, fe;
 #pragma unroll
                     for (int p = 0; p < 2; ++p) {
-                        ld_a(fn.r[p], sN + p * kCC, kTld, m0, 16 * kk);
-                        ld_a(fe.r[p], sE + p * kCC, kTld, m0, 16 * kk);
+                        ld_a(fn.r[p], sh(sN) + p * kCC, kTld, m0, 16 * kk);
+                        ld_a(fe.r[p], sh(sE) + p * kCC, kTld, m0, 16 * kk);
                     }
 #pragma unroll
                     for (int p = 0; p < NT / 2; ++p) {
                         uint32_t bk[4];
-                        ld_b128<true>(bk, sK, n0 + 16 * p, 16 * kk);
+                        ld_b128<true>(bk, sh(sK), n0 + 16 * p, 16 * kk);
                         mma_pair<T>(x[2 * p], x[2 * p + 1], fn.r[1], bk);
                         mma_pair<T>(y[2 * p], y[2 * p + 1], fe.r[1], bk);
                         mma_pair<T>(x[2 * p], x[2 * p + 1], fn.r[0], bk);
@@ -1473,19 +1521,18 @@ __global__ void __launch_bounds__(32 * kGradWarps, 1) planes_grad_k(DArgs a, flo
                     }
                 }
             } else {
-#pragma unroll
-                for (int kk = 0; kk < kC / 16; ++kk) {
-                    if (kk < rg) continue;  // columns of N and E
+#pragma unroll 1
+                for (int kk = rg; kk < kC / 16; ++kk) {  // columns of N and E
                     Af<2> fn, fe;
 #pragma unroll
                     for (int p = 0; p < 2; ++p) {
-                        ld_at(fn.r[p], sN + p * kCC, kTld, m0, 16 * kk);
-                        ld_at(fe.r[p], sE + p * kCC, kTld, m0, 16 * kk);
+                        ld_at(fn.r[p], sh(sN) + p * kCC, kTld, m0, 16 * kk);
+                        ld_at(fe.r[p], sh(sE) + p * kCC, kTld, m0, 16 * kk);
                     }
 #pragma unroll
                     for (int p = 0; p < NT / 2; ++p) {
-                        mm128<T, 2, true>(x[2 * p], x[2 * p + 1], fn, sQ, n0 + 16 * p, 16 * kk);
-                        mm128<T, 2, true>(x[2 * p], x[2 * p + 1], fe, sK, n0 + 16 * p, 16 * kk);
+                        mm128<T, 2, true>(x[2 * p], x[2 * p + 1], fn, sh(sQ), n0 + 16 * p, 16 * kk);
+                        mm128<T, 2, true>(x[2 * p], x[2 * p + 1], fe, sh(sK), n0 + 16 * p, 16 * kk);
                     }
                 }
             }
