@@ -12,7 +12,7 @@
 // warp that carries it.  A CTA holds G such warps, one or more helpers (the
 // forward's outputs; the reverse chain's Q^T dO) and a loading warp, which
 // copies each chunk's rows and tiles to shared memory with bulk copies, two
-// chunks deep: rows of the inputs by tensor maps (64 tokens by 64 or 16 columns,
+// chunks deep, and stores what a backward reads: rows of the inputs by tensor maps (64 tokens by 64 or 16 columns,
 // swizzled so that ldmatrix meets no bank twice; a bulk copy for each row of
 // 256 bytes took 67 cycles a row and bound the chains).  Tiles that kernels hand to each other (T', M, S, U, dS, dV) lie
 // in the workspace as they lie in shared memory, padding included, so that a
@@ -481,17 +481,22 @@ __global__ void __launch_bounds__(128) planes_prep_k(const __grid_constant__ DAr
 // ----------------------------------------------------------------------------
 // the forward chain and the outputs
 // ----------------------------------------------------------------------------
+constexpr int kChainGates = 5 * kC;  // (without 1 / beta)
+
 template <int KD, int G>
 struct Fwd {
     static constexpr int LDK = KD + 8, LDO = 24;
-    // helpers: warps 0..G-1 carry states; with three of them one helper has the fourth scheduler to itself
-    static constexpr int H = G == 3 ? 1 : G, kWarps = G + H + 1;
+    // Warps 0..G-1 carry states, then H helpers, then the loading warp.  (One helper for three
+    // groups was the slowest of them: 603 us where two take 510.)
+    static constexpr int H = G == 3 ? 2 : G, kWarps = G + H + 1;
     static constexpr int kK = 0, kQ = kK + kC * KD, kV = kQ + kC * KD, kT = kV + kC * 16 * G, kM = kT + 2 * kCC;
     static constexpr int kGa = kM + 2 * kCC;  // (elements) the gates, float32
-    static constexpr int kLoad = kGa * 2 + kGates * 4, kStage = up1024(kLoad);  // bytes
-    static constexpr int kS = 0, kU = 2 * 16 * LDK, kO = kU + 2 * 16 * kTld;  // a group's tiles (elements)
-    static constexpr int kGroup = kO * 2 + 16 * kC * 4;  // (O: float32 between its two products, then rows)
-    static constexpr int kBars = 2 * kStage + G * kGroup;
+    static constexpr int kLoad = kGa * 2 + kChainGates * 4, kStage = up1024(kLoad);  // bytes
+    // a group's (bytes): S in two planes, U and O in float32 (O's rows too)
+    static constexpr int kS = 0, kU = 4 * 16 * LDK, kO = kU + 16 * kC * 4, kGroup = kO + 16 * kC * 4;
+    static constexpr int kGroups = kStage + kLoad, kKeep = kGroups + G * kGroup;  // where U's planes are stored from
+    static constexpr int kStages = G < 4 ? G : 1;  // of U's planes, to be stored from
+    static constexpr int kBars = kKeep + kStages * 4 * 16 * kTld;
     static constexpr size_t bytes = 1024 + kBars + 8 * (5 + 4 * G);
 };
 
@@ -517,6 +522,79 @@ __device__ __forceinline__ void state_store(const float (*S)[4], float* p, int K
         }
 }
 
+// A group's accumulators (16 x 64) between warps: float32 as the lanes hold them.
+__device__ __forceinline__ void frag_put(float4* s, const float (*x)[4], const Lane& L) {
+#pragma unroll
+    for (int j = 0; j < kC / 8; ++j) s[j * 32 + L.l] = make_float4(x[j][0], x[j][1], x[j][2], x[j][3]);
+}
+__device__ __forceinline__ void frag_get(float (*x)[4], const float4* s, const Lane& L) {
+#pragma unroll
+    for (int j = 0; j < kC / 8; ++j) {
+        const float4 v = s[j * 32 + L.l];
+        x[j][0] = v.x;
+        x[j][1] = v.y;
+        x[j][2] = v.z;
+        x[j][3] = v.w;
+    }
+}
+// What the loading warp does for a backward, between two loads: group by group
+// the state's planes (from where its warp put them) and U or dV (split here)
+// go to the workspace.  (Done by the warps that carry the states, these stores
+// cost them 400 to 1500 cycles a chunk.)
+// `n` groups of a CTA, `step` bytes apart in shared memory; lane g stores group g
+// and waits for its own copies, so that the groups' copies run side by side.
+template <int LDK>
+__device__ __forceinline__ bool store_states(e16* to, const unsigned char* tile, int step, int n, int64_t Vp, uint64_t* there,
+                                             uint64_t* taken, uint32_t parity) {
+    const int l = threadIdx.x & 31;
+    bool ok = true;
+#pragma unroll 1
+    for (int g = 0; g < n; ++g) ok = warp_wait(&there[g], parity) && ok;
+    if (l < n) {
+        bulk_store(to + l * 16 * LDK, tile + l * step, 32 * LDK);
+        bulk_store(to + (Vp + l * 16) * LDK, tile + l * step + 32 * LDK, 32 * LDK);
+        bulk_commit();
+        bulk_wait_read();  // (and U's or dV's of the chunk before)
+        mbar_arrive(&taken[l]);
+    }
+    __syncwarp();
+    return ok;
+}
+// After store_states, which has seen the stages free.  One stage a group, or
+// (stages = 1) one for all, from which a group's copies then have to leave first.
+template <typename T>
+__device__ __forceinline__ bool store_values(e16* to, const unsigned char* frag, int step, int n, e16* stage, int stages,
+                                             int64_t Vp, uint64_t* there, uint64_t* taken, uint32_t parity) {
+    const Lane L;
+    bool ok = true;
+#pragma unroll 1
+    for (int g = 0; g < n; ++g) {
+        ok = warp_wait(&there[g], parity) && ok;
+        float x[kC / 8][4];
+        frag_get(x, reinterpret_cast<const float4*>(frag + g * step), L);
+        warp_arrive(&taken[g]);
+        e16* s = stage + (stages > 1 ? g * 2 * 16 * kTld : 0);
+        if (stages == 1 && g > 0) {
+            bulk_wait_read();
+            __syncwarp();
+        }
+#pragma unroll
+        for (int kk = 0; kk < kC / 16; ++kk) {
+            const Af<2> a = from_acc<T, 2>(x[2 * kk], x[2 * kk + 1]);
+            st_tile(sh(s), kTld, 16 * kk, a.r[0]);
+            st_tile(sh(s) + 16 * kTld, kTld, 16 * kk, a.r[1]);
+        }
+        fence_async();
+        __syncwarp();
+        if (L.l == g) {
+            bulk_store(to + g * 16 * kTld, s, 32 * kTld);
+            bulk_store(to + (Vp + g * 16) * kTld, s + 16 * kTld, 32 * kTld);
+            bulk_commit();
+        }
+    }
+    return ok;
+}
+
 // KEEP: S and U are written for a backward.
 template <typename T, int KD, int G, bool KEEP>
 __global__ void __launch_bounds__(Fwd<KD, G>::kWarps * 32) planes_chain_k(const __grid_constant__ DArgs a, const __grid_constant__ Maps maps) {
@@ -538,19 +616,24 @@ __global__ void __launch_bounds__(Fwd<KD, G>::kWarps * 32) planes_chain_k(const 
             mbar_init(&empty[s], G + Sm::H);
         }
         mbar_init(land, 1);
-        for (int i = 0; i < 4 * G; ++i) mbar_init(&s_full[i], 1);
+        for (int i = 0; i < G; ++i) {
+            mbar_init(&s_full[i], 1);
+            mbar_init(&s_empty[i], KEEP ? 2 : 1);
+            mbar_init(&u_full[i], 1);
+            mbar_init(&u_empty[i], KEEP ? 2 : 1);
+        }
         fence_mbar_init();
     }
     __syncthreads();
     bool ok = true;
     if (warp == Sm::kWarps - 1) {
         // ---- loads ----
-        for (int c = 0; c < nc && ok; ++c) {
+        auto load = [&](int c) {
             e16* e = reinterpret_cast<e16*>(smem + (c & 1) * Sm::kStage);
             const int t0 = c * kC, rows = min(kC, len - t0);
             const bool tail = rows < min(kC, a.L - t0);
             uint64_t* bar = tail ? land : &full[c & 1];
-            ok = warp_wait(&empty[c & 1], ((c >> 1) & 1) ^ 1);
+            ok = warp_wait(&empty[c & 1], ((c >> 1) & 1) ^ 1) && ok;
             if (L.l == 0) {
                 const int64_t id = head * a.n + c;
                 mbar_expect_tx(bar, Sm::kLoad);
@@ -559,7 +642,7 @@ __global__ void __launch_bounds__(Fwd<KD, G>::kWarps * 32) planes_chain_k(const 
                 bulk_load(e + Sm::kT, static_cast<const e16*>(a.T) + id * 2 * kCC, 4 * kCC, bar);
 #pragma unroll
                 for (int g = 0; g < G; ++g) tma_load(e + Sm::kV + g * kC * 16, &maps.v, bar, vb + 16 * g, t0, h, b);
-                bulk_load(e + Sm::kGa, a.gates + id * kGates, kGates * 4, bar);
+                bulk_load(e + Sm::kGa, a.gates + id * kGates, kChainGates * 4, bar);
 #pragma unroll
                 for (int x = 0; x < KD; x += 64) tma_load(e + Sm::kQ + x * kC, &maps.q, bar, x, t0, hk, b);
                 bulk_load(e + Sm::kM, static_cast<const e16*>(a.M) + id * 2 * kCC, 4 * kCC, bar);
@@ -571,15 +654,32 @@ __global__ void __launch_bounds__(Fwd<KD, G>::kWarps * 32) planes_chain_k(const 
                 zero_rows<16>(e + Sm::kV, G, rows);
                 warp_arrive(&full[c & 1]);
             }
+        };
+#pragma unroll 1
+        for (int c = KEEP ? -1 : 0; c < nc && ok; ++c) {
+            if constexpr (!KEEP) {
+                load(c);
+            } else {  // a load ahead of the stores
+                if (c + 1 < nc) load(c + 1);
+                if (c < 0) continue;
+                const int64_t id = (head * a.n + c) * 2 * a.Vp + vb;
+                const int n = min(G, (a.Vp - vb) / 16);
+                ok = store_states<Sm::LDK>(static_cast<e16*>(a.S) + id * Sm::LDK, smem + Sm::kGroups + Sm::kS, Sm::kGroup, n, a.Vp,
+                                           s_full, s_empty, c & 1) && ok;
+                ok = store_values<T>(static_cast<e16*>(a.U) + id * kTld, smem + Sm::kGroups + Sm::kU, Sm::kGroup, n,
+                                     reinterpret_cast<e16*>(smem + Sm::kKeep), Sm::kStages, a.Vp, u_full, u_empty, c & 1) && ok;
+            }
         }
+        if constexpr (KEEP) bulk_wait_all();
         return;
     }
     if (warp < G) {
         // ---- a state of 16 value columns ----
         const int v0 = vb + warp * 16;
         const bool on = v0 < a.Vp;
-        e16* mine = reinterpret_cast<e16*>(smem + 2 * Sm::kStage + warp * Sm::kGroup);
-        e16 *sS = mine + Sm::kS, *sU = mine + Sm::kU;
+        unsigned char* mine = smem + Sm::kGroups + warp * Sm::kGroup;
+        const Sh sS = sh(mine + Sm::kS);
+        float4* sU = reinterpret_cast<float4*>(mine + Sm::kU);
         float S[KD / 8][4];
         state_load<KD>(S, a.initial ? a.initial + head * a.K * a.V : nullptr, a.K, a.V, v0, L);
         for (int c = 0; c < nc && ok; ++c) {
@@ -593,10 +693,6 @@ __global__ void __launch_bounds__(Fwd<KD, G>::kWarps * 32) planes_chain_k(const 
                 ok = warp_wait(&full[c & 1], (c >> 1) & 1);
             } else {
                 ok = warp_wait2(&full[c & 1], (c >> 1) & 1, &s_empty[warp], (c & 1) ^ 1);
-                if constexpr (KEEP) {  // the last chunk's copies have left the tiles
-                    if (L.l == 0) bulk_wait_read();
-                    __syncwarp();
-                }
                 // (K S0)^T, S in two planes; the next 16 columns of S are split between the products
                 float X[kC / 8][4] = {};
                 {
@@ -609,8 +705,8 @@ __global__ void __launch_bounds__(Fwd<KD, G>::kWarps * 32) planes_chain_k(const 
                         },
                         [&](int i, const uint32_t(*f)[4]) {
                             Af<2>& af = as[i & 1];
-                            st_tile(sh(sS), Sm::LDK, 16 * i, af.r[0]);
-                            if constexpr (KEEP) st_tile(sh(sS) + 16 * Sm::LDK, Sm::LDK, 16 * i, af.r[1]);
+                            st_tile(sS, Sm::LDK, 16 * i, af.r[0]);
+                            if constexpr (KEEP) st_tile(sS + 16 * Sm::LDK, Sm::LDK, 16 * i, af.r[1]);
                             mma_step_with<T>(X, af, f, [&](int q) {
                                 if (i + 1 < KD / 16) {
                                     const float* s = S[2 * i + 2 + q / 2];
@@ -621,12 +717,6 @@ __global__ void __launch_bounds__(Fwd<KD, G>::kWarps * 32) planes_chain_k(const 
                 }
                 if constexpr (KEEP) fence_async();
                 warp_arrive(&s_full[warp]);
-                if (KEEP && L.l == 0) {
-                    e16* to = static_cast<e16*>(a.S) + (id * 2 * a.Vp + v0) * Sm::LDK;
-                    bulk_store(to, sS, 32 * Sm::LDK);
-                    bulk_store(to + static_cast<int64_t>(a.Vp) * Sm::LDK, sS + 16 * Sm::LDK, 32 * Sm::LDK);
-                    bulk_commit();
-                }
                 const bool u_free = mbar_try_wait(&u_empty[warp], (c & 1) ^ 1);
                 // X = V^T - gam (K S0)^T
 #pragma unroll
@@ -653,11 +743,7 @@ __global__ void __launch_bounds__(Fwd<KD, G>::kWarps * 32) planes_chain_k(const 
                     const float* u = U[2 * kk + q / 2];
                     from_acc_part<T>(to, q, u[2 * (q & 1)] * d.x, u[2 * (q & 1) + 1] * d.y);
                 };
-                auto plain = [&](Af<2>& to, int kk, int q) {
-                    const float* u = U[2 * kk + q / 2];
-                    from_acc_part<T>(to, q, u[2 * (q & 1)], u[2 * (q & 1) + 1]);
-                };
-                Af<2> ud[2], up[2];
+                Af<2> ud[2];
                 {
                     Af<2> ax[2];
                     ax[0] = from_acc<T, 2>(X[0], X[1]);
@@ -681,13 +767,14 @@ __global__ void __launch_bounds__(Fwd<KD, G>::kWarps * 32) planes_chain_k(const 
                                     from_acc_part<T>(ax[(kk + 1) & 1], q, x[2 * (q & 1)], x[2 * (q & 1) + 1]);
                                 }
                                 if (i == 4) decayed(ud[0], 0, q);
-                                if (i == 5) plain(up[0], 0, q);
                             };
                             if (i & 1) mma_step_with<T>(U, af, f, side, kk);
                             else mma_step_with<T>(U, high(af), f, side, kk);
                         });
                 }
                 ok = warp_wait_asked(u_free, &u_empty[warp], (c & 1) ^ 1) && ok;
+                frag_put(sU, U, L);
+                warp_arrive(&u_full[warp]);
                 // S^T = gam_63 S^T + (d U)^T K
                 {
                     constexpr int Q = KD / 64;
@@ -698,31 +785,15 @@ __global__ void __launch_bounds__(Fwd<KD, G>::kWarps * 32) planes_chain_k(const 
                         },
                         [&](int i, const uint32_t(*f)[4]) {
                             const int kk = i / Q;
-                            if (i % Q == 0) {
-                                st_tile(sh(sU), kTld, 16 * kk, up[kk & 1].r[0]);
-                                st_tile(sh(sU) + 16 * kTld, kTld, 16 * kk, up[kk & 1].r[1]);
-                            }
                             mma_step_with<T>(S + 8 * (i % Q), ud[kk & 1], f, [&](int q) {
-                                if (kk + 1 < 4) {
-                                    if (i % Q == 0) decayed(ud[(kk + 1) & 1], kk + 1, q);
-                                    if (i % Q == Q - 1) plain(up[(kk + 1) & 1], kk + 1, q);
-                                }
+                                if (kk + 1 < 4 && i % Q == 0) decayed(ud[(kk + 1) & 1], kk + 1, q);
                             });
                         });
-                }
-                if constexpr (KEEP) fence_async();
-                warp_arrive(&u_full[warp]);
-                if (KEEP && L.l == 0) {
-                    e16* to = static_cast<e16*>(a.U) + (id * 2 * a.Vp + v0) * kTld;
-                    bulk_store(to, sU, 32 * kTld);
-                    bulk_store(to + static_cast<int64_t>(a.Vp) * kTld, sU + 16 * kTld, 32 * kTld);
-                    bulk_commit();
                 }
             }
             warp_arrive(&empty[c & 1]);
         }
         if (on && a.final_state && ok) state_store<KD>(S, a.final_state + head * a.K * a.V, a.K, a.V, v0, L);
-        if (KEEP && L.l == 0) bulk_wait_all();
         return;
     }
     // ---- outputs of the groups g = helper, helper + H, .. ----
@@ -741,9 +812,9 @@ __global__ void __launch_bounds__(Fwd<KD, G>::kWarps * 32) planes_chain_k(const 
 #pragma unroll 1
         for (int g = helper; g < G; g += Sm::H) {
             if (vb + 16 * g >= a.Vp) break;
-            unsigned char* theirs = smem + 2 * Sm::kStage + g * Sm::kGroup;
-            const e16* sS = reinterpret_cast<const e16*>(theirs) + Sm::kS;
-            float4* sO = reinterpret_cast<float4*>(theirs + Sm::kO * 2);
+            unsigned char* theirs = smem + Sm::kGroups + g * Sm::kGroup;
+            const Sh sS = sh(theirs + Sm::kS);
+            float4* sO = reinterpret_cast<float4*>(theirs + Sm::kO);
             ok = warp_wait(&s_full[g], c & 1) && ok;
             // scale gam Q S0: S in one plane (its rounding, half a step of terms of any sign, against
             // the output's own: in bfloat16 y is off by 2.2e-3 in the norm instead of 1.7e-3, for half
@@ -752,7 +823,7 @@ __global__ void __launch_bounds__(Fwd<KD, G>::kWarps * 32) planes_chain_k(const 
             Af<1> as[2];
             steps<KD / 16>(
                 [&](int k, uint32_t(*f)[4]) {
-                    ld_a(as[k & 1].r[0], sh(sS), Sm::LDK, 0, 16 * k);
+                    ld_a(as[k & 1].r[0], sS, Sm::LDK, 0, 16 * k);
 #pragma unroll
                     for (int p = 0; p < 4; ++p) ld_b128<false>(f[p], es + Sm::kQ, 16 * p, 16 * k);
                 },
@@ -768,36 +839,28 @@ __global__ void __launch_bounds__(Fwd<KD, G>::kWarps * 32) planes_chain_k(const 
         for (int g = helper; g < G; g += Sm::H) {
             const int v0 = vb + 16 * g;
             if (v0 >= a.Vp) break;
-            e16* theirs = reinterpret_cast<e16*>(smem + 2 * Sm::kStage + g * Sm::kGroup);
-            e16* sO = theirs + Sm::kO;
-            float O[kC / 8][4];
-#pragma unroll
-            for (int j = 0; j < kC / 8; ++j) {
-                const float4 o = reinterpret_cast<const float4*>(sO)[j * 32 + L.l];
-                O[j][0] = o.x;
-                O[j][1] = o.y;
-                O[j][2] = o.z;
-                O[j][3] = o.w;
-            }
-            const Sh ts = sh(theirs);
+            unsigned char* theirs = smem + Sm::kGroups + g * Sm::kGroup;
+            e16* sO = reinterpret_cast<e16*>(theirs + Sm::kO);
+            float O[kC / 8][4], U[kC / 8][4];
+            frag_get(O, reinterpret_cast<const float4*>(sO), L);
             ok = warp_wait(&u_full[g], c & 1) && ok;
-            Af<2> au[2];
+            frag_get(U, reinterpret_cast<const float4*>(theirs + Sm::kU), L);
+            warp_arrive(&u_empty[g]);
+            Af<2> au;
             steps<8>(
                 [&](int k, uint32_t(*f)[4]) {
-                    if (!(k & 1)) {
-                        ld_a(au[(k / 2) & 1].r[0], ts + Sm::kU, kTld, 0, 8 * k);
-                        ld_a(au[(k / 2) & 1].r[1], ts + Sm::kU + 16 * kTld, kTld, 0, 8 * k);
-                    }
 #pragma unroll
                     for (int p = 0; p < 4; ++p)
                         if (p >= k / 2) ld_b<false>(f[p], es + Sm::kM + (k & 1 ? 0 : kCC), kTld, 16 * p, 16 * (k / 2));
                 },
                 [&](int k, const uint32_t(*f)[4]) {
-                    const Af<2>& af = au[(k / 2) & 1];
-                    if (k & 1) mma_step<T>(O, af, f, k / 2);
-                    else mma_step<T>(O, high(af), f, k / 2);
+                    if (k & 1) {
+                        mma_step<T>(O, au, f, k / 2);
+                    } else {
+                        au = from_acc<T, 2>(U[k], U[k + 1]);
+                        mma_step<T>(O, high(au), f, k / 2);
+                    }
                 });
-            warp_arrive(&u_empty[g]);
             // rows of 16 values through shared memory: 32 bytes a token, two lanes each
             __syncwarp();
 #pragma unroll
@@ -835,14 +898,16 @@ __global__ void __launch_bounds__(Fwd<KD, G>::kWarps * 32) planes_chain_k(const 
 template <int KD, int G>
 struct Rev {
     static constexpr int LDK = KD + 8;
-    static constexpr int H = G == 3 ? 1 : G, kWarps = G + H + 1;
+    static constexpr int H = G, kWarps = G + H + 1;
     static constexpr int kK = 0, kQ = kK + kC * KD, kD = kQ + kC * KD, kT = kD + kC * 16 * G, kM = kT + 2 * kCC;
     static constexpr int kGa = kM + 2 * kCC;
-    static constexpr int kLoad = kGa * 2 + kGates * 4, kStage = up1024(kLoad);
-    static constexpr int kS = 0, kX = 2 * 16 * LDK * 2, kZ = kX + 2 * 16 * kTld * 2;  // a group's tiles (bytes)
-    static constexpr int kGroup = kZ + 16 * KD * 4;
-    static constexpr int kBars = 2 * kStage + G * kGroup;
-    static constexpr size_t bytes = 1024 + kBars + 8 * (5 + 2 * G);
+    static constexpr int kLoad = kGa * 2 + kChainGates * 4, kStage = up1024(kLoad);
+    // a group's (bytes): dS in two planes, dV and (scale gam dO)^T Q in float32
+    static constexpr int kS = 0, kX = 4 * 16 * LDK, kZ = kX + 16 * kC * 4, kGroup = kZ + 16 * KD * 4;
+    static constexpr int kGroups = kStage + kLoad, kKeep = kGroups + G * kGroup;
+    static constexpr int kStages = G == 3 && KD == 128 ? 1 : G;
+    static constexpr int kBars = kKeep + kStages * 4 * 16 * kTld;
+    static constexpr size_t bytes = 1024 + kBars + 8 * (5 + 6 * G);
 };
 
 template <typename T, int KD, int G>
@@ -858,6 +923,7 @@ __global__ void __launch_bounds__(Rev<KD, G>::kWarps * 32) planes_rchain_k(const
     uint64_t* empty = full + 2;
     uint64_t* land = empty + 2;
     uint64_t *z_full = land + 1, *z_empty = z_full + G;
+    uint64_t *s_full = z_empty + G, *s_empty = s_full + G, *x_full = s_empty + G, *x_empty = x_full + G;
     const int64_t head = static_cast<int64_t>(b) * a.Hv + h;
     if (threadIdx.x == 0) {
         for (int s = 0; s < 2; ++s) {
@@ -865,19 +931,19 @@ __global__ void __launch_bounds__(Rev<KD, G>::kWarps * 32) planes_rchain_k(const
             mbar_init(&empty[s], G + Sm::H);
         }
         mbar_init(land, 1);
-        for (int i = 0; i < 2 * G; ++i) mbar_init(&z_full[i], 1);
+        for (int i = 0; i < 6 * G; ++i) mbar_init(&z_full[i], 1);
         fence_mbar_init();
     }
     __syncthreads();
     bool ok = true;
     if (warp == Sm::kWarps - 1) {
-        for (int i = 0; i < nc && ok; ++i) {
+        auto load = [&](int i) {
             const int c = nc - 1 - i;
             e16* e = reinterpret_cast<e16*>(smem + (i & 1) * Sm::kStage);
             const int t0 = c * kC, rows = min(kC, len - t0);
             const bool tail = rows < min(kC, a.L - t0);
             uint64_t* bar = tail ? land : &full[i & 1];
-            ok = warp_wait(&empty[i & 1], ((i >> 1) & 1) ^ 1);
+            ok = warp_wait(&empty[i & 1], ((i >> 1) & 1) ^ 1) && ok;
             if (L.l == 0) {
                 const int64_t id = head * a.n + c;
                 mbar_expect_tx(bar, Sm::kLoad);
@@ -886,7 +952,7 @@ __global__ void __launch_bounds__(Rev<KD, G>::kWarps * 32) planes_rchain_k(const
 #pragma unroll
                 for (int g = 0; g < G; ++g) tma_load(e + Sm::kD + g * kC * 16, &maps.d, bar, vb + 16 * g, t0, h, b);
                 bulk_load(e + Sm::kM, static_cast<const e16*>(a.M) + id * 2 * kCC, 4 * kCC, bar);
-                bulk_load(e + Sm::kGa, a.gates + id * kGates, kGates * 4, bar);
+                bulk_load(e + Sm::kGa, a.gates + id * kGates, kChainGates * 4, bar);
                 bulk_load(e + Sm::kT, static_cast<const e16*>(a.T) + id * 2 * kCC, 4 * kCC, bar);
 #pragma unroll
                 for (int x = 0; x < KD; x += 64) tma_load(e + Sm::kQ + x * kC, &maps.q, bar, x, t0, hk, b);
@@ -899,14 +965,27 @@ __global__ void __launch_bounds__(Rev<KD, G>::kWarps * 32) planes_rchain_k(const
                 fence_async();  // later chunks are copied over these rows
                 warp_arrive(&full[i & 1]);
             }
+        };
+#pragma unroll 1
+        for (int i = -1; i < nc && ok; ++i) {  // a load ahead of the stores
+            if (i + 1 < nc) load(i + 1);
+            if (i < 0) continue;
+            const int64_t id = (head * a.n + nc - 1 - i) * 2 * a.Vp + vb;
+            const int n = min(G, (a.Vp - vb) / 16);
+            ok = store_states<Sm::LDK>(static_cast<e16*>(a.dS) + id * Sm::LDK, smem + Sm::kGroups + Sm::kS, Sm::kGroup, n, a.Vp,
+                                       s_full, s_empty, i & 1) && ok;
+            ok = store_values<T>(static_cast<e16*>(a.dV) + id * kTld, smem + Sm::kGroups + Sm::kX, Sm::kGroup, n,
+                                 reinterpret_cast<e16*>(smem + Sm::kKeep), Sm::kStages, a.Vp, x_full, x_empty, i & 1) && ok;
         }
+        bulk_wait_all();
         return;
     }
     if (warp < G) {
         const int v0 = vb + warp * 16;
         const bool on = v0 < a.Vp;
-        unsigned char* mine = smem + 2 * Sm::kStage + warp * Sm::kGroup;
-        e16 *sS = reinterpret_cast<e16*>(mine + Sm::kS), *sX = reinterpret_cast<e16*>(mine + Sm::kX);
+        unsigned char* mine = smem + Sm::kGroups + warp * Sm::kGroup;
+        const Sh sS = sh(mine + Sm::kS);
+        float4* sX = reinterpret_cast<float4*>(mine + Sm::kX);
         const float4* sZ = reinterpret_cast<const float4*>(mine + Sm::kZ);
         float S[KD / 8][4];  // dS^T
         state_load<KD>(S, a.dfinal ? a.dfinal + head * a.K * a.V : nullptr, a.K, a.V, v0, L);
@@ -917,10 +996,10 @@ __global__ void __launch_bounds__(Rev<KD, G>::kWarps * 32) planes_rchain_k(const
             const float* ga = reinterpret_cast<const float*>(e + Sm::kGa);
             const float *gam = ga + 2 * kC, *dec = ga + 3 * kC;
             const int64_t id = head * a.n + c;
-            ok = warp_wait(&full[i & 1], (i >> 1) & 1);
-            if (on) {
-                if (L.l == 0) bulk_wait_read();  // the last chunk's copies have left the tiles
-                __syncwarp();
+            if (!on) {
+                ok = warp_wait(&full[i & 1], (i >> 1) & 1);
+            } else {
+                ok = warp_wait2(&full[i & 1], (i >> 1) & 1, &s_empty[warp], (i & 1) ^ 1);
                 float U[kC / 8][4] = {};  // dU^T = d (K dS1)^T + dO^T M
                 {
                     Af<2> as[2];
@@ -932,8 +1011,8 @@ __global__ void __launch_bounds__(Rev<KD, G>::kWarps * 32) planes_rchain_k(const
                         },
                         [&](int k, const uint32_t(*f)[4]) {
                             Af<2>& af = as[k & 1];
-                            st_tile(sh(sS), Sm::LDK, 16 * k, af.r[0]);
-                            st_tile(sh(sS) + 16 * Sm::LDK, Sm::LDK, 16 * k, af.r[1]);
+                            st_tile(sS, Sm::LDK, 16 * k, af.r[0]);
+                            st_tile(sS + 16 * Sm::LDK, Sm::LDK, 16 * k, af.r[1]);
                             mma_step_with<T>(U, af, f, [&](int q) {
                                 if (k + 1 < KD / 16) {
                                     const float* s = S[2 * k + 2 + q / 2];
@@ -943,14 +1022,8 @@ __global__ void __launch_bounds__(Rev<KD, G>::kWarps * 32) planes_rchain_k(const
                         });
                 }
                 fence_async();
-                __syncwarp();
-                if (L.l == 0) {
-                    e16* to = static_cast<e16*>(a.dS) + (id * 2 * a.Vp + v0) * Sm::LDK;
-                    bulk_store(to, sS, 32 * Sm::LDK);
-                    bulk_store(to + static_cast<int64_t>(a.Vp) * Sm::LDK, sS + 16 * Sm::LDK, 32 * Sm::LDK);
-                    bulk_commit();
-                }
-                const bool z_there = mbar_try_wait(&z_full[warp], i & 1);
+                warp_arrive(&s_full[warp]);
+                const bool z_there = mbar_try_wait(&z_full[warp], i & 1), x_free = mbar_try_wait(&x_empty[warp], (i & 1) ^ 1);
 #pragma unroll
                 for (int j = 0; j < kC / 8; ++j) {
                     const float2 f = *reinterpret_cast<const float2*>(dec + 8 * j + 2 * L.t);
@@ -980,12 +1053,7 @@ __global__ void __launch_bounds__(Rev<KD, G>::kWarps * 32) planes_rchain_k(const
                     const float* u = X[2 * kk + q / 2];
                     from_acc_part<T>(to, q, -u[2 * (q & 1)] * d.x, -u[2 * (q & 1) + 1] * d.y);
                 };
-                auto plain = [&](Af<2>& to, int kk, int q) {
-                    const float* u = X[2 * kk + q / 2];
-                    from_acc_part<T>(to, q, u[2 * (q & 1)], u[2 * (q & 1) + 1]);
-                };
                 Af<1> xd[2];
-                Af<2> xp[2];
                 {
                     Af<2> au[2];
                     au[1] = from_acc<T, 2>(U[6], U[7]);
@@ -1016,13 +1084,15 @@ __global__ void __launch_bounds__(Rev<KD, G>::kWarps * 32) planes_rchain_k(const
                                     from_acc_part<T>(au[(kk - 1) & 1], q, u[2 * (q & 1)], u[2 * (q & 1) + 1]);
                                 }
                                 if (k == 4) decayed(xd[1], 3, q);
-                                if (k == 5) plain(xp[1], 3, q);
                             };
                             if (k & 1) mma_step_with<T>(X, af, f, side, 0, kk + 1);
                             else mma_step_with<T>(X, high(af), f, side, 0, kk + 1);
                         });
                 }
                 warp_arrive(&z_empty[warp]);
+                ok = warp_wait_asked(x_free, &x_empty[warp], (i & 1) ^ 1) && ok;
+                frag_put(sX, X, L);
+                warp_arrive(&x_full[warp]);
                 // dS^T -= (gam dV)^T K
                 {
                     constexpr int Q = KD / 64;
@@ -1034,31 +1104,15 @@ __global__ void __launch_bounds__(Rev<KD, G>::kWarps * 32) planes_rchain_k(const
                         },
                         [&](int k, const uint32_t(*f)[4]) {
                             const int kk = 3 - k / Q;
-                            if (k % Q == 0) {
-                                st_tile(sh(sX), kTld, 16 * kk, xp[kk & 1].r[0]);
-                                st_tile(sh(sX) + 16 * kTld, kTld, 16 * kk, xp[kk & 1].r[1]);
-                            }
                             mma_step_with<T>(S + 8 * (k % Q), xd[kk & 1], f, [&](int q) {
-                                if (kk > 0) {
-                                    if (k % Q == 0) decayed(xd[(kk - 1) & 1], kk - 1, q);
-                                    if (k % Q == Q - 1) plain(xp[(kk - 1) & 1], kk - 1, q);
-                                }
+                                if (kk > 0 && k % Q == 0) decayed(xd[(kk - 1) & 1], kk - 1, q);
                             });
                         });
-                }
-                fence_async();
-                __syncwarp();
-                if (L.l == 0) {
-                    e16* to = static_cast<e16*>(a.dV) + (id * 2 * a.Vp + v0) * kTld;
-                    bulk_store(to, sX, 32 * kTld);
-                    bulk_store(to + static_cast<int64_t>(a.Vp) * kTld, sX + 16 * kTld, 32 * kTld);
-                    bulk_commit();
                 }
             }
             warp_arrive(&empty[i & 1]);
         }
         if (on && a.dinitial && ok) state_store<KD>(S, a.dinitial + head * a.K * a.V, a.K, a.V, v0, L);
-        if (L.l == 0) bulk_wait_all();
         return;
     }
     // ---- (scale gam dO)^T Q of the groups ----
@@ -1096,7 +1150,7 @@ __global__ void __launch_bounds__(Rev<KD, G>::kWarps * 32) planes_rchain_k(const
                     }
                     mma_step<T>(Z + 8 * (k % Q), af, f);
                 });
-            float4* sZ = reinterpret_cast<float4*>(smem + 2 * Sm::kStage + g * Sm::kGroup + Sm::kZ);
+            float4* sZ = reinterpret_cast<float4*>(smem + Sm::kGroups + g * Sm::kGroup + Sm::kZ);
             ok = warp_wait(&z_empty[g], (i & 1) ^ 1) && ok;
 #pragma unroll
             for (int j = 0; j < KD / 8; ++j) sZ[j * 32 + L.l] = make_float4(Z[j][0], Z[j][1], Z[j][2], Z[j][3]);
@@ -1652,13 +1706,15 @@ cudaError_t smem_limit(K kernel, size_t bytes) {
 
 constexpr int kSms = 148;
 
-// Groups of 16 value columns per CTA of a chain, one CTA on an SM at a time:
-// the fewest rounds of CTAs, weighed with the products that a chunk's busiest
-// scheduler has to do.  (Four groups do not fit the reverse chain's tiles.)
+// Groups of 16 value columns per CTA of a chain, one CTA on an SM at a time: the
+// fewest rounds of CTAs, weighed with what a chunk takes with G groups on an SM
+// (measured at K = V = 128, in units of 0.1 us: forward 28, 40, 44 with 2, 3, 4
+// groups, reverse 27, 35 with 2, 3; four do not fit the reverse chain's tiles).
+// 48 heads of 128 take 510 us of a forward with three groups, 710 with two.
 int chain_groups(const DArgs& a, bool reverse) {
     const int64_t heads = static_cast<int64_t>(a.B) * a.Hv, groups = a.Vp / 16;
     auto cost = [&](int64_t g, int64_t per) { return (heads * ((groups + g - 1) / g) + kSms - 1) / kSms * per; };
-    const int64_t x2 = cost(2, reverse ? 292 : 316), x3 = cost(3, reverse ? 384 : 372), x4 = cost(4, 440);
+    const int64_t x2 = cost(2, reverse ? 27 : 28), x3 = cost(3, reverse ? 35 : 40), x4 = cost(4, 44);
     if (reverse) return x2 <= x3 ? 2 : 3;
     return x2 <= x3 && x2 <= x4 ? 2 : x3 <= x4 ? 3 : 4;
 }
