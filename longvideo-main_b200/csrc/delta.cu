@@ -869,7 +869,9 @@ __global__ void __launch_bounds__(256) delta_grad_k(DArgs a, float* group) {
             const float behind = run - y0 + tot;
             const int64_t o = (row0 + i0) * a.Hv + h;
             if (i0 < all) {
-                gate_store(a.dg, a.gate_dtype, o, i0 < rows ? y0 + behind : 0.f);
+                // (the first token's decay meets an empty state: no rounding of the terms that cancel)
+                const bool none = i0 == 0 && c == 0 && !a.initial;
+                gate_store(a.dg, a.gate_dtype, o, i0 < rows && !none ? y0 + behind : 0.f);
                 gate_store(a.dbeta, a.gate_dtype, o, i0 < rows ? sDb[i0] : 0.f);
             }
             if (i0 + 1 < all) {

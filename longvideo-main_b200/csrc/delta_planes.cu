@@ -159,6 +159,11 @@ __device__ __forceinline__ void ld_b128(uint32_t* b, Sh s, int n0, int k0) {
     if constexpr (TR) ldsm4t(b, at);
     else ldsm4(b, at);
 }
+__device__ __forceinline__ void ld_a128(uint32_t* r, Sh s, int m0, int k0) {
+    const int l = threadIdx.x & 31;
+    const uint32_t mine = s.a + (l & 15) * 128 + (((l >> 4) ^ (l & 7)) << 4);
+    ldsm4(r, (mine ^ static_cast<uint32_t>(((k0 >> 3) & 7) << 4)) + (k0 >> 6) * (kC * 128) + m0 * 128);
+}
 // 16 rows of A: tokens m0.. of a group, and (at) its 16 columns by tokens k0..
 __device__ __forceinline__ void ld_a32(uint32_t* r, Sh s, int m0) {
     const int l = threadIdx.x & 31;
@@ -290,15 +295,28 @@ __device__ __forceinline__ float ratio(const float* G, int i, int j) {
 // ----------------------------------------------------------------------------
 // gates, T' and M of a chunk
 // ----------------------------------------------------------------------------
-// (I + A)^-1 by blocks, in float32: the 16 x 16 blocks on the diagonal by
-// forward substitution (a thread a column), then twice the step from blocks of
-// s to blocks of 2 s, [[P, 0], [R, Q]]^-1 = [[P^-1, 0], [-Q^-1 R P^-1, Q^-1]],
-// whose products run on the tensor cores with operands split in two tf32
-// parts.  (Forward substitution alone takes 2016 dependent multiply-adds.)
+// Two warps make M and two A, of each one block rows 3 and 0 (of 16 tokens), the
+// other 2 and 1: five 16 x 16 blocks each.  Blocks above the diagonal are neither
+// made nor written, as no product reads them.  The latter two then invert I + A by
+// blocks, in float32: the 16 x 16 blocks on the diagonal by forward substitution (a
+// thread a column), then twice the step from blocks of s to blocks of 2 s,
+// [[P, 0], [R, Q]]^-1 = [[P^-1, 0], [-Q^-1 R P^-1, Q^-1]], whose products run on the
+// tensor cores with operands split in two tf32 parts.  (Forward substitution alone
+// takes 2016 dependent multiply-adds.)  Bound by the instructions a chunk takes and
+// by what it moves, 32 KB in and 39 KB out; A and its inverse lie where K and Q
+// were, so that six CTAs share an SM.
 constexpr int kAld = kC + 8;  // float32 tiles
 
+__device__ __forceinline__ void sync_inverse() { asm volatile("bar.sync 1, 64;" ::: "memory"); }
+
+template <int KD>
+struct Prep {
+    static constexpr int kIn = 2 * kC * KD * 2, kTiles = 2 * kC * kAld * 4;
+    static constexpr size_t bytes = 1024 + (kIn > kTiles ? kIn : kTiles);
+};
+
 template <typename T, int KD>
-__global__ void __launch_bounds__(128) planes_prep_k(const __grid_constant__ DArgs a) {
+__global__ void __launch_bounds__(128) planes_prep_k(const __grid_constant__ DArgs a, const __grid_constant__ Maps maps) {
     using F = FmtF<false>;
     const int c = blockIdx.x, h = blockIdx.y, b = blockIdx.z;
     const int len = row_length(a, b);
@@ -307,29 +325,26 @@ __global__ void __launch_bounds__(128) planes_prep_k(const __grid_constant__ DAr
     const int hk = h / (a.Hv / a.Hk);
     const int64_t id = (static_cast<int64_t>(b) * a.Hv + h) * a.n + c, t0 = static_cast<int64_t>(c) * kC;
     extern __shared__ __align__(128) unsigned char smem_raw[];
-    unsigned char* smem = smem_raw;
-    constexpr int LD = KD + 8;
+    unsigned char* smem = align_smem(smem_raw);
     e16* sK = reinterpret_cast<e16*>(smem);
-    e16* sQ = sK + kC * LD;
-    float* sA = reinterpret_cast<float*>(sQ + kC * LD);  // A, lower triangle
-    float* sT = sA + kC * kAld;                          // its inverse
-    float* sY = reinterpret_cast<float*>(smem);          // a product (K and Q are done with by then)
+    e16* sQ = sK + kC * KD;
+    float* sA = reinterpret_cast<float*>(smem);  // A below the diagonal blocks, products above (after K and Q)
+    float* sT = sA + kC * kAld;                  // its inverse
     __shared__ float sG[2 * kC], sB[kC];
+    __shared__ uint64_t land;
     const int tid = threadIdx.x, warp = tid >> 5;
     const Lane L;
-    {
-        const e16* k = static_cast<const e16*>(a.k) + b * a.sk.b + t0 * a.sk.t + hk * a.sk.h;
-        const e16* q = static_cast<const e16*>(a.q) + b * a.sq.b + t0 * a.sq.t + hk * a.sq.h;
-        for (int i = tid; i < kC * (KD / 8); i += 128) {
-            const int r = i / (KD / 8), col = (i % (KD / 8)) * 8;
-            const bool in = r < rows && col < a.K;
-            cp_async16(sK + r * LD + col, in ? k + r * a.sk.t + col : k, in);
-            cp_async16(sQ + r * LD + col, in ? q + r * a.sq.t + col : q, in);
+    if (tid == 0) {
+        mbar_init(&land, 1);
+        fence_mbar_init();
+        mbar_expect_tx(&land, 4 * kC * KD);
+#pragma unroll
+        for (int x = 0; x < KD; x += 64) {
+            tma_load(sK + x * kC, &maps.k, &land, x, c * kC, hk, b);
+            tma_load(sQ + x * kC, &maps.q, &land, x, c * kC, hk, b);
         }
-        cp_async_commit();
     }
-    for (int i = tid; i < kC * kAld; i += 128) sT[i] = 0.f;
-    if (warp == 0) {
+    if (warp == 1) {
         double s[2];
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
@@ -366,112 +381,149 @@ __global__ void __launch_bounds__(128) planes_prep_k(const __grid_constant__ DAr
             ga[5 * kC + r] = r < rows ? 1.f / sB[r] : 0.f;
         }
     }
-    cp_async_wait_all();
     __syncthreads();
-    {  // a warp 16 rows of A and of M
-        float kk[kC / 8][4] = {}, qk[kC / 8][4] = {};
-        const int m0 = warp * 16;
+    if (!mbar_wait(&land, 0)) return;
+    if (rows < min(kC, a.L - c * kC)) {
+        if (warp == 0) zero_rows<64>(sK, 2 * (KD / 64), rows);
+        __syncthreads();
+    }
+    // block i of a warp: row block and column block
+    const int second = warp & 1, split = 4 - second;
+    const int rb0 = 3 - second, rb1 = second;
+    const bool left = warp >= 2;  // A
+    float x[5][2][4] = {};
+    {
+        const Sh s = sh(left ? sK : sQ);
 #pragma unroll
         for (int k0 = 0; k0 < KD; k0 += 16) {
-            Af<1> ak, aq;
-            ld_a(ak.r[0], sh(sK), LD, m0, k0);
-            ld_a(aq.r[0], sh(sQ), LD, m0, k0);
+            uint32_t a0[4], a1[4], bk[4];
+            ld_a128(a0, s, 16 * rb0, k0);
+            ld_a128(a1, s, 16 * rb1, k0);
 #pragma unroll
-            for (int p = 0; p < kC / 16; ++p)
-                if (p <= warp) {
-                    uint32_t bk[4];
-                    ld_b<false>(bk, sh(sK), LD, 16 * p, k0);
-                    mma_pair<T>(kk[2 * p], kk[2 * p + 1], ak.r[0], bk);
-                    mma_pair<T>(qk[2 * p], qk[2 * p + 1], aq.r[0], bk);
+            for (int p = 0; p < 4; ++p) {
+                if (p > rb0) break;
+                ld_b128<false>(bk, sh(sK), 16 * p, k0);
+                mma_pair<T>(x[p][0], x[p][1], a0, bk);
+                if (p <= rb1) {
+                    if (second) mma_pair<T>(x[3 + p > 4 ? 4 : 3 + p][0], x[3 + p > 4 ? 4 : 3 + p][1], a1, bk);
+                    else mma_pair<T>(x[4][0], x[4][1], a1, bk);
                 }
-        }
-        e16* M = static_cast<e16*>(a.M) + id * 2 * kCC;
-#pragma unroll
-        for (int j = 0; j < kC / 8; ++j) {
-            float m[4] = {};
-            if (j <= 2 * warp + 1)
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const int r = m0 + L.g + (e >> 1) * 8, col = 8 * j + 2 * L.t + (e & 1);
-                    const float w = col <= r ? ratio(sG, r, col) : 0.f;
-                    m[e] = a.scale * w * qk[j][e];
-                    sA[r * kAld + col] = col < r ? sB[r] * w * kk[j][e] : 0.f;
-                }
-#pragma unroll
-            for (int e = 0; e < 2; ++e) {
-                const uint32_t hi = Num<T>::pack(m[2 * e], m[2 * e + 1]);
-                const float2 f = Num<T>::unpack(hi);
-                const int o = (m0 + L.g + 8 * e) * kTld + 8 * j + 2 * L.t;
-                *reinterpret_cast<uint32_t*>(M + o) = hi;
-                *reinterpret_cast<uint32_t*>(M + kCC + o) = Num<T>::pack(m[2 * e] - f.x, m[2 * e + 1] - f.y);
             }
         }
     }
-    __syncthreads();
-    if (tid < kC) {  // column tid of its diagonal block
-        const int r0 = tid & ~15, col = tid & 15;
-        float x[16];
+    __syncthreads();  // K and Q are done with
+    e16* M = static_cast<e16*>(a.M) + id * 2 * kCC;
+#pragma unroll
+    for (int i = 0; i < 5; ++i) {
+        const int rb = i < split ? rb0 : rb1, cb = i < split ? i : i - split;
+        const int r0 = 16 * rb + L.g;
+        const float g0 = sG[r0], g1 = sG[r0 + 8], l0 = sG[kC + r0], l1 = sG[kC + r0 + 8];
+        const float f0 = left ? sB[r0] : a.scale, f1 = left ? sB[r0 + 8] : a.scale;
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+            const int col = 16 * cb + 8 * j + 2 * L.t;
+            const float2 gc = *reinterpret_cast<const float2*>(sG + col), lc = *reinterpret_cast<const float2*>(sG + kC + col);
+            const int last = left ? -1 : 0;  // A without the diagonal
+            float v[4];
+            v[0] = col <= r0 + last ? f0 * ex2_approx((g0 - gc.x) + (l0 - lc.x)) * x[i][j][0] : 0.f;
+            v[1] = col + 1 <= r0 + last ? f0 * ex2_approx((g0 - gc.y) + (l0 - lc.y)) * x[i][j][1] : 0.f;
+            v[2] = col <= r0 + 8 + last ? f1 * ex2_approx((g1 - gc.x) + (l1 - lc.x)) * x[i][j][2] : 0.f;
+            v[3] = col + 1 <= r0 + 8 + last ? f1 * ex2_approx((g1 - gc.y) + (l1 - lc.y)) * x[i][j][3] : 0.f;
+            if (left) {
+                *reinterpret_cast<float2*>(sA + r0 * kAld + col) = make_float2(v[0], v[1]);
+                *reinterpret_cast<float2*>(sA + (r0 + 8) * kAld + col) = make_float2(v[2], v[3]);
+            } else {
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    const uint32_t hi = Num<T>::pack(v[2 * e], v[2 * e + 1]);
+                    const float2 f = Num<T>::unpack(hi);
+                    const int o = (r0 + 8 * e) * kTld + col;
+                    *reinterpret_cast<uint32_t*>(M + o) = hi;
+                    *reinterpret_cast<uint32_t*>(M + kCC + o) = Num<T>::pack(v[2 * e] - f.x, v[2 * e + 1] - f.y);
+                }
+            }
+        }
+    }
+    if (!left) return;
+    sync_inverse();
+    const int u = tid - 64;
+    {  // column u of its diagonal block
+        const int r0 = u & ~15, col = u & 15;
+        float y[16];
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
-            float s0 = i == col ? 1.f : 0.f, s1 = 0.f;
+            float s[4] = {i == col ? 1.f : 0.f, 0.f, 0.f, 0.f};
             const float* ar = sA + (r0 + i) * kAld + r0;
 #pragma unroll
-            for (int m = 0; m < i; ++m) {
-                if (m & 1) s1 = fmaf(-ar[m], x[m], s1);
-                else s0 = fmaf(-ar[m], x[m], s0);
+            for (int m = 0; m < i; m += 4) {
+                const float4 f = *reinterpret_cast<const float4*>(ar + m);
+                s[0] = fmaf(-f.x, y[m], s[0]);
+                if (m + 1 < i) s[1] = fmaf(-f.y, y[m + 1], s[1]);
+                if (m + 2 < i) s[2] = fmaf(-f.z, y[m + 2], s[2]);
+                if (m + 3 < i) s[3] = fmaf(-f.w, y[m + 3], s[3]);
             }
-            x[i] = s0 + s1;
+            y[i] = (s[0] + s[1]) + (s[2] + s[3]);
         }
 #pragma unroll
-        for (int i = 0; i < 16; ++i) sT[(r0 + i) * kAld + tid] = x[i];
+        for (int i = 0; i < 16; ++i) sT[(r0 + i) * kAld + u] = y[i];
     }
-    __syncthreads();
-    // R P^-1 into sY, then -Q^-1 of it into the inverse; warps 0, 1: a pair of 16 x 16 blocks each
+    sync_inverse();
     auto put = [&](float* d, int r, int col, const float* x0, const float* x1, float sign) {
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            const int rr = r + L.g + (e >> 1) * 8, cc = col + 2 * L.t + (e & 1);
-            d[rr * kAld + cc] = sign * x0[e];
-            d[rr * kAld + cc + 8] = sign * x1[e];
+        for (int e = 0; e < 4; e += 2) {
+            float* p = d + (r + L.g + (e >> 1) * 8) * kAld + col + 2 * L.t;
+            *reinterpret_cast<float2*>(p) = make_float2(sign * x0[e], sign * x0[e + 1]);
+            *reinterpret_cast<float2*>(p + 8) = make_float2(sign * x1[e], sign * x1[e + 1]);
         }
     };
-    if (warp < 2) {
-        const int o = 32 * warp;
-        float x0[4] = {}, x1[4] = {};
+    {  // a pair of 16 x 16 blocks a warp: R P^-1 (kept above the diagonal of A), then -Q^-1 of it
+        const int o = 32 * second;
+        float* y = sA + o * kAld + o + 16;
+        float x0[4] = {}, x1[4] = {}, z0[4] = {}, z1[4] = {};
         F::template mma2<1, true>(x0, x1, F::from_smem(sA, kAld, o + 16, o), sT, kAld, o, o);
-        put(sY, o + 16, o, x0, x1, 1.f);
+        put(y, 0, 0, x0, x1, 1.f);
         __syncwarp();
-        float z0[4] = {}, z1[4] = {};
-        F::template mma2<1, true>(z0, z1, F::from_smem(sT, kAld, o + 16, o + 16), sY, kAld, o, o + 16);
+        F::template mma2<1, true>(z0, z1, F::from_smem(sT, kAld, o + 16, o + 16), y, kAld, 0, 0);
         put(sT, o + 16, o, z0, z1, -1.f);
     }
-    __syncthreads();
-    {  // blocks of 32: a warp one 16 x 16 tile of each product
-        const int r = 32 + 16 * (warp >> 1), col = 16 * (warp & 1);
-        float x0[4] = {}, x1[4] = {};
+    sync_inverse();
+    {  // the blocks of 32: 16 columns a warp
+        const int col = 16 * second;
+        float* y = sA + 32;
 #pragma unroll
-        for (int k = 0; k < 32; k += 16)
-            F::template mma2<1, true>(x0, x1, F::from_smem(sA, kAld, r, k), sT, kAld, col, k);
-        put(sY, r, col, x0, x1, 1.f);
-        __syncthreads();
-        float z0[4] = {}, z1[4] = {};
+        for (int r = 32; r < 64; r += 16) {
+            float x0[4] = {}, x1[4] = {};
 #pragma unroll
-        for (int k = 32; k < 64; k += 16)
-            F::template mma2<1, true>(z0, z1, F::from_smem(sT, kAld, r, k), sY, kAld, col, k);
-        put(sT, r, col, z0, z1, -1.f);
+            for (int k = 0; k < 32; k += 16)
+                if (k >= col) F::template mma2<1, true>(x0, x1, F::from_smem(sA, kAld, r, k), sT, kAld, col, k);
+            put(y, r - 32, col, x0, x1, 1.f);
+        }
+        __syncwarp();
+#pragma unroll
+        for (int r = 32; r < 64; r += 16) {
+            float z0[4] = {}, z1[4] = {};
+#pragma unroll
+            for (int k = 0; k < r - 16; k += 16)
+                F::template mma2<1, true>(z0, z1, F::from_smem(sT, kAld, r, 32 + k), y, kAld, col, k);
+            put(sT, r, col, z0, z1, -1.f);
+        }
     }
-    __syncthreads();
+    sync_inverse();
     e16* to = static_cast<e16*>(a.T) + id * 2 * kCC;
-    for (int i = tid; i < kC * 8; i += 128) {
-        const int r = i >> 3, c8 = (i & 7) * 8;
+#pragma unroll
+    for (int i = 0; i < 5; ++i) {  // ten blocks of 16 rows by two vectors of 8
+        const int at = i * 64 + u, blk = at >> 5, r16 = (at & 31) >> 1;
+        const int rb = blk >= 6 ? 3 : blk >= 3 ? 2 : blk >= 1 ? 1 : 0, cb = blk - rb * (rb + 1) / 2;
+        const int r = 16 * rb + r16, c8 = 16 * cb + (at & 1) * 8;
         uint32_t hi[4], lo[4];
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-            const float x = sT[r * kAld + c8 + 2 * e] * sB[c8 + 2 * e];
-            const float y = sT[r * kAld + c8 + 2 * e + 1] * sB[c8 + 2 * e + 1];
-            hi[e] = Num<T>::pack(x, y);
+            const float2 v = *reinterpret_cast<const float2*>(sT + r * kAld + c8 + 2 * e);
+            const float2 w = *reinterpret_cast<const float2*>(sB + c8 + 2 * e);
+            const float p = v.x * w.x, q = v.y * w.y;
+            hi[e] = Num<T>::pack(p, q);
             const float2 f = Num<T>::unpack(hi[e]);
-            lo[e] = Num<T>::pack(x - f.x, y - f.y);
+            lo[e] = Num<T>::pack(p - f.x, q - f.y);
         }
         *reinterpret_cast<uint4*>(to + r * kTld + c8) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
         *reinterpret_cast<uint4*>(to + kCC + r * kTld + c8) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
@@ -1675,7 +1727,9 @@ __global__ void __launch_bounds__(32 * kGradWarps, 1) planes_grad_k(const __grid
                 const float behind = run - y0 + tot;
                 const int64_t o = (row0 + i0) * a.Hv + h;
                 if (i0 < all) {
-                    gate_store(a.dg, a.gate_dtype, o, i0 < rows ? y0 + behind : 0.f);
+                    // (the first token's decay meets an empty state: no rounding of the terms that cancel)
+                    const bool none = i0 == 0 && c == 0 && !a.initial;
+                    gate_store(a.dg, a.gate_dtype, o, i0 < rows && !none ? y0 + behind : 0.f);
                     gate_store(a.dbeta, a.gate_dtype, o, i0 < rows ? sDb[i0] : 0.f);
                 }
                 if (i0 + 1 < all) {
@@ -1777,20 +1831,19 @@ bool make_maps(const DArgs& a, Maps& m) {
 
 template <typename T, int KD>
 cudaError_t fwd(const DArgs& a, cudaStream_t s) {
-    const size_t prep = 2 * kC * (KD + 8) * sizeof(e16) + 2 * kC * kAld * sizeof(float);
-    PLANES_TRY((smem_limit(planes_prep_k<T, KD>, prep)));
-    planes_prep_k<T, KD><<<dim3(a.n, a.Hv, a.B), 128, prep, s>>>(a);
-    note_launch();
-    PLANES_TRY(cudaGetLastError());
+    // a runtime call first: tensor maps are not made in a thread (autograd's, say) that
+    // has not met its device yet
+    PLANES_TRY((smem_limit(planes_prep_k<T, KD>, Prep<KD>::bytes)));
     Maps m{};
     if (!make_maps(a, m)) return cudaErrorInvalidValue;
+    planes_prep_k<T, KD><<<dim3(a.n, a.Hv, a.B), 128, Prep<KD>::bytes, s>>>(a, m);
+    note_launch();
+    PLANES_TRY(cudaGetLastError());
     return chain<T, KD>(a, m, false, s);
 }
 
 template <typename T, int KD>
 cudaError_t bwd(const DArgs& a, float* group, cudaStream_t s) {
-    // a runtime call first: tensor maps are not made in a thread (autograd's, say) that
-    // has not met its device yet
     PLANES_TRY((smem_limit(planes_grad_k<T, KD>, Grad<KD>::bytes)));
     Maps m{};
     if (!make_maps(a, m)) return cudaErrorInvalidValue;

@@ -123,6 +123,16 @@ def test_float32_gates_and_no_initial_state(dtype):
     compare(got, want)
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+def test_first_decay_of_an_empty_state_has_no_gradient(dtype):
+    d, do, dS = make(3, 5, 1, 2, 64, 32, dtype, seed=30, initial=False)
+    got, want = both(d, do, dS)
+    assert float(want["dg"][:, 0].abs().max()) == 0.0 and float(got["dg"][:, 0].abs().max()) == 0.0
+    compare(got, want)
+    one, _ = both({n: t[:, :1] for n, t in d.items()}, do[:, :1], dS)
+    assert float(one["dg"].abs().max()) == 0.0
+
+
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
 def test_lengths(dtype):
     """Rows of no token, one token, up to a chunk's border and over L (clamped); what lies behind holds NaN and infinities."""
