@@ -890,8 +890,12 @@ __global__ void __launch_bounds__(256) delta_grad_k(DArgs a, float* group) {
 // key row, in registers from the first token to the last.  k^T S' and q^T S'
 // are summed together, as o = q^T S' + (q.k) u; one token is one pass over the
 // state: read once, written once.
+// Bound by the state's bytes; what counts is how many of them are under way, so
+// eight CTAs share a multiprocessor (K = 128, 64 rows of 16 heads: 29.0 us, 4.6
+// TB/s, against 33.3 with the five that 82 registers a thread allow; 16 rows 6.7
+// us against 7.9; six or ten CTAs, 64 or 128 columns a CTA were no faster).
 template <typename T, int KD>
-__global__ void __launch_bounds__(128) delta_step_k(DArgs a, int vec_s) {
+__global__ void __launch_bounds__(128, 8) delta_step_k(const __grid_constant__ DArgs a, int vec_s) {
     constexpr int R = KD / 16;
     const int h = blockIdx.y, b = blockIdx.z, hk = h / (a.Hv / a.Hk);
     const int len = row_length(a, b);
@@ -907,7 +911,7 @@ __global__ void __launch_bounds__(128) delta_step_k(DArgs a, int vec_s) {
 #pragma unroll
         for (int e = 0; e < 4; ++e) S[i][e] = 0.f;
         if (a.initial && k < a.K && v < a.V) {
-            const float* p = a.initial + base + static_cast<int64_t>(k) * a.V + v;
+            const float* p = a.initial + base + (k * a.V + v);
             if (vec_s) {
                 const float4 x = *reinterpret_cast<const float4*>(p);
                 S[i][0] = x.x; S[i][1] = x.y; S[i][2] = x.z; S[i][3] = x.w;
@@ -930,9 +934,6 @@ __global__ void __launch_bounds__(128) delta_step_k(DArgs a, int vec_s) {
         }
         const float al = expf(gate_value(a.g, a.gate_dtype, b * a.sg.b + t * a.sg.t + h * a.sg.h));
         const float be = gate_value(a.beta, a.gate_dtype, b * a.sb.b + t * a.sb.t + h * a.sb.h);
-        float val[4];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) val[e] = v + e < a.V ? to_f32(vp[t * a.sv.t + v + e]) : 0.f;
         __syncthreads();
         float x[4] = {}, y[4] = {}, qk = 0.f;
 #pragma unroll
@@ -962,6 +963,9 @@ __global__ void __launch_bounds__(128) delta_step_k(DArgs a, int vec_s) {
             if (lane == 0) sqk[s][warp] = qk;
         }
         __syncthreads();
+        float val[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) val[e] = v + e < a.V ? to_f32(vp[t * a.sv.t + v + e]) : 0.f;
         float4 X = red[s][0][0][lane & 7], Y = red[s][1][0][lane & 7];
         qk = sqk[s][0];
 #pragma unroll
@@ -998,7 +1002,7 @@ __global__ void __launch_bounds__(128) delta_step_k(DArgs a, int vec_s) {
     for (int i = 0; i < R; ++i) {
         const int kr = kg + 16 * i;
         if (kr < a.K && v < a.V) {
-            float* p = a.final_state + base + static_cast<int64_t>(kr) * a.V + v;
+            float* p = a.final_state + base + (kr * a.V + v);
             if (vec_s) {
                 *reinterpret_cast<float4*>(p) = make_float4(S[i][0], S[i][1], S[i][2], S[i][3]);
             } else {
