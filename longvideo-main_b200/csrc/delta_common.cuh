@@ -134,6 +134,7 @@ struct FmtF {
 #pragma unroll
         for (int half = 0; half < 2; ++half) {
             float* c = half ? c1 : c0;
+            float x[4] = {};
             const int n = n0 + 8 * half + L.g;
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
@@ -144,10 +145,12 @@ struct FmtF {
                 uint32_t bh0, bl0, bh1, bl1;
                 split_tf32(v.x, bh0, bl0);
                 split_tf32(v.y, bh1, bl1);
-                mma_tf32(c, a.lo[h], bh0, bh1);
-                if constexpr (!(X && IN)) mma_tf32(c, a.h[h], bl0, bl1);
-                mma_tf32(c, a.h[h], bh0, bh1);
+                mma_tf32(x, a.lo[h], bh0, bh1);
+                if constexpr (!(X && IN)) mma_tf32(x, a.h[h], bl0, bl1);
+                mma_tf32(x, a.h[h], bh0, bh1);
             }
+#pragma unroll
+            for (int i = 0; i < 4; ++i) c[i] += x[i];
         }
     }
     static __device__ __forceinline__ void load_t(float* x0, float* x1, const E* s, int ld, int r0, int c0) {
