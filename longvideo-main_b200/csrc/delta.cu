@@ -58,7 +58,8 @@ __device__ __forceinline__ void mm(float* c0, float* c1, const typename F::templ
 
 // 64 rows of an input (row stride st, `rows` of them in the sequence, `cols`
 // columns that exist) into shared memory as [row][colp]; the rest is 0 and is
-// not read.
+// not read.  Aligned float32 rows are copied asynchronously (the caller commits
+// and waits).
 template <class F, typename T>
 __device__ __forceinline__ void load_rows(typename F::E* dst, int ld, const T* src, int64_t st, int rows, int cols,
                                           int colp, bool vec, int tid, int nthr) {
@@ -68,6 +69,13 @@ __device__ __forceinline__ void load_rows(typename F::E* dst, int ld, const T* s
         const bool in = r < rows && c < cols;
         const T* p = src + r * st + c;
         typename F::E* o = dst + r * ld + c;
+        if constexpr (sizeof(T) == sizeof(float)) {
+            if (vec) {
+                cp_async16(o, in ? p : src, in);
+                cp_async16(o + 4, in ? p + 4 : src, in);
+                continue;
+            }
+        }
         float v[8];
         if (in && vec) {
             load8<T>(p, v);
@@ -274,6 +282,24 @@ __device__ __forceinline__ void acc_store_t(const float (*x)[4], typename F::E* 
             p[static_cast<int64_t>(8 * j + 2 * L.t + (e & 1)) * ld + v0 + L.g + (e >> 1) * 8] = F::put(x[j][e]);
 }
 
+// Accumulators that a loop takes two tiles at a time go through shared memory,
+// each lane's own: with every tile in registers the loops over the summed index
+// would have to be unrolled, and a chunk's instructions (70 KB and more) would
+// be fetched anew for every chunk.
+template <int NT>
+__device__ __forceinline__ void lane_put(float4* s, const float (*x)[4]) {
+#pragma unroll
+    for (int j = 0; j < NT; ++j) s[j * 32] = make_float4(x[j][0], x[j][1], x[j][2], x[j][3]);
+}
+__device__ __forceinline__ void lane_get(float* x, const float4* s) {
+    const float4 v = *s;
+    x[0] = v.x;
+    x[1] = v.y;
+    x[2] = v.z;
+    x[3] = v.w;
+}
+template <int KD, int W> constexpr size_t kLaneBytes = size_t(W) * 16 * KD * sizeof(float);
+
 // W warps, 16 value columns each.
 template <class F, typename T, int KD, int W>
 __global__ void __launch_bounds__(W * 32) delta_chain_k(DArgs a) {
@@ -293,6 +319,7 @@ __global__ void __launch_bounds__(W * 32) delta_chain_k(DArgs a) {
         for (int j = 0; j < KD / 8; ++j) S[j][0] = S[j][1] = S[j][2] = S[j][3] = 0.f;
     }
     const bool on = v0 < a.Vp;
+    float4* mine = reinterpret_cast<float4*>(smem + 2 * St::bytes) + warp * 4 * KD + L.l;
     if (nc > 0) chain_load<F, T, KD, W>(a, smem, 0, b, h, hk, len, vb, W * 32);
     cp_async_commit();
     for (int c = 0; c < nc; ++c) {
@@ -311,9 +338,13 @@ __global__ void __launch_bounds__(W * 32) delta_chain_k(DArgs a) {
             if (a.S) acc_store<E, KD / 8>(S, static_cast<E*>(a.S) + (id * a.Vp + v0) * KD, KD, L);
             // P = (K S0)^T, then X = V^T - gam P in its place
             float X[kC / 8][4] = {};
-#pragma unroll
+            lane_put<KD / 8>(mine, S);
+#pragma unroll 1
             for (int k0 = 0; k0 < KD; k0 += 16) {
-                const auto af = F::template from_acc<2>(S[k0 / 8], S[k0 / 8 + 1]);
+                float x0[4], x1[4];
+                lane_get(x0, mine + k0 * 4);
+                lane_get(x1, mine + k0 * 4 + 32);
+                const auto af = F::template from_acc<2>(x0, x1);
 #pragma unroll
                 for (int p = 0; p < kC / 16; ++p)
                     mm_in<F, 2, false>(X[2 * p], X[2 * p + 1], af, sK, St::LDK, 16 * p, k0);
@@ -328,28 +359,34 @@ __global__ void __launch_bounds__(W * 32) delta_chain_k(DArgs a) {
                     X[2 * p + 1][e] = x1[e] - gam[16 * p + 8 + 2 * L.t + (e & 1)] * X[2 * p + 1][e];
                 }
             }
+            lane_put<kC / 8>(mine, X);
             float U[kC / 8][4] = {};
-#pragma unroll
+#pragma unroll 1
             for (int kk = 0; kk < kC / 16; ++kk) {
-                const auto af = F::template from_acc<2>(X[2 * kk], X[2 * kk + 1]);
+                float x0[4], x1[4];
+                lane_get(x0, mine + kk * 64);
+                lane_get(x1, mine + kk * 64 + 32);
+                const auto af = F::template from_acc<2>(x0, x1);
 #pragma unroll
-                for (int p = kk; p < kC / 16; ++p) {
-                    mm<F, 2, false>(U[2 * p], U[2 * p + 1], af, sT, kTld, 16 * p, 16 * kk);
-                }
+                for (int p = 0; p < kC / 16; ++p)
+                    if (p >= kk) mm<F, 2, false>(U[2 * p], U[2 * p + 1], af, sT, kTld, 16 * p, 16 * kk);
             }
+            lane_put<kC / 8>(mine, U);
             acc_store_t<F>(U, static_cast<E*>(a.U) + id * kC * a.Vp, a.Vp, v0, L);
             const float gc = gam[kC - 1];
 #pragma unroll
             for (int j = 0; j < KD / 8; ++j)
 #pragma unroll
                 for (int e = 0; e < 4; ++e) S[j][e] *= gc;
-#pragma unroll
+#pragma unroll 1
             for (int kk = 0; kk < kC / 16; ++kk) {
                 float y0[4], y1[4];
+                lane_get(y0, mine + kk * 64);
+                lane_get(y1, mine + kk * 64 + 32);
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
-                    y0[e] = U[2 * kk][e] * dec[16 * kk + 2 * L.t + (e & 1)];
-                    y1[e] = U[2 * kk + 1][e] * dec[16 * kk + 8 + 2 * L.t + (e & 1)];
+                    y0[e] *= dec[16 * kk + 2 * L.t + (e & 1)];
+                    y1[e] *= dec[16 * kk + 8 + 2 * L.t + (e & 1)];
                 }
                 const auto af = F::template from_acc<2>(y0, y1);
 #pragma unroll
@@ -546,6 +583,7 @@ __global__ void __launch_bounds__(W * 32) delta_rchain_k(DArgs a) {
     }
     const bool on = v0 < a.Vp;
     constexpr bool two = St::kStages == 2;
+    float4* mine = reinterpret_cast<float4*>(smem + St::kStages * St::bytes) + warp * 4 * KD + L.l;
     if (two && nc > 0) {
         rchain_load<F, T, KD, W>(a, smem + ((nc - 1) & 1) * St::bytes, nc - 1, b, h, hk, len, vb, W * 32);
         cp_async_commit();
@@ -569,9 +607,13 @@ __global__ void __launch_bounds__(W * 32) delta_rchain_k(DArgs a) {
             const int64_t id = head * a.n + c;
             acc_store<E, KD / 8>(S, static_cast<E*>(a.dS) + (id * a.Vp + v0) * KD, KD, L);
             float U[kC / 8][4] = {};  // dU^T
-#pragma unroll
+            lane_put<KD / 8>(mine, S);
+#pragma unroll 1
             for (int k0 = 0; k0 < KD; k0 += 16) {
-                const auto af = F::template from_acc<1>(S[k0 / 8], S[k0 / 8 + 1]);
+                float x0[4], x1[4];
+                lane_get(x0, mine + k0 * 4);
+                lane_get(x1, mine + k0 * 4 + 32);
+                const auto af = F::template from_acc<1>(x0, x1);
 #pragma unroll
                 for (int p = 0; p < kC / 16; ++p)
                     mm_in<F, 1, false>(U[2 * p], U[2 * p + 1], af, e + St::kK, St::LDK, 16 * p, k0);
@@ -580,36 +622,43 @@ __global__ void __launch_bounds__(W * 32) delta_rchain_k(DArgs a) {
             for (int j = 0; j < kC / 8; ++j)
 #pragma unroll
                 for (int x = 0; x < 4; ++x) U[j][x] *= dec[8 * j + 2 * L.t + (x & 1)];
-#pragma unroll
+#pragma unroll 1
             for (int kk = 0; kk < kC / 16; ++kk) {
                 const auto af = F::from_smem_t(e + St::kD, St::LDV, warp * 16, 16 * kk);
 #pragma unroll
-                for (int p = 0; p <= kk; ++p)
-                    mm<F, 1, true>(U[2 * p], U[2 * p + 1], af, e + St::kM, kTld, 16 * p, 16 * kk);
+                for (int p = 0; p < kC / 16; ++p)
+                    if (p <= kk) mm<F, 1, true>(U[2 * p], U[2 * p + 1], af, e + St::kM, kTld, 16 * p, 16 * kk);
             }
+            lane_put<kC / 8>(mine, U);
             float X[kC / 8][4] = {};  // dV^T
-#pragma unroll
+#pragma unroll 1
             for (int kk = 0; kk < kC / 16; ++kk) {
-                const auto af = F::template from_acc<2>(U[2 * kk], U[2 * kk + 1]);
+                float x0[4], x1[4];
+                lane_get(x0, mine + kk * 64);
+                lane_get(x1, mine + kk * 64 + 32);
+                const auto af = F::template from_acc<2>(x0, x1);
 #pragma unroll
-                for (int p = 0; p <= kk; ++p)
-                    mm<F, 2, true>(X[2 * p], X[2 * p + 1], af, e + St::kT, kTld, 16 * p, 16 * kk);
+                for (int p = 0; p < kC / 16; ++p)
+                    if (p <= kk) mm<F, 2, true>(X[2 * p], X[2 * p + 1], af, e + St::kT, kTld, 16 * p, 16 * kk);
             }
+            lane_put<kC / 8>(mine, X);
             acc_store_t<F>(X, static_cast<E*>(a.dV) + id * kC * a.Vp, a.Vp, v0, L);
             const float gc = gam[kC - 1];
 #pragma unroll
             for (int j = 0; j < KD / 8; ++j)
 #pragma unroll
                 for (int x = 0; x < 4; ++x) S[j][x] *= gc;
-#pragma unroll
+#pragma unroll 1
             for (int kk = 0; kk < kC / 16; ++kk) {
                 auto ad = F::from_smem_t(e + St::kD, St::LDV, warp * 16, 16 * kk);
                 F::scale_k(ad, gam + 2 * kC, 16 * kk);
                 float y0[4], y1[4];
+                lane_get(y0, mine + kk * 64);
+                lane_get(y1, mine + kk * 64 + 32);
 #pragma unroll
                 for (int x = 0; x < 4; ++x) {
-                    y0[x] = -gam[16 * kk + 2 * L.t + (x & 1)] * X[2 * kk][x];
-                    y1[x] = -gam[16 * kk + 8 + 2 * L.t + (x & 1)] * X[2 * kk + 1][x];
+                    y0[x] *= -gam[16 * kk + 2 * L.t + (x & 1)];
+                    y1[x] *= -gam[16 * kk + 8 + 2 * L.t + (x & 1)];
                 }
                 const auto av = F::template from_acc<1>(y0, y1);
 #pragma unroll
@@ -1033,12 +1082,14 @@ cudaError_t run_chain(const DArgs& a, bool reverse, cudaStream_t s) {
     const dim3 grid((a.Vp + 16 * W - 1) / (16 * W), a.Hv, a.B);
     if (reverse) {
         using St = RStage<F, KD, W>;
-        DELTA_TRY(smem_limit(delta_rchain_k<F, T, KD, W>, St::kStages * St::bytes));
-        delta_rchain_k<F, T, KD, W><<<grid, W * 32, St::kStages * St::bytes, s>>>(a);
+        constexpr size_t bytes = St::kStages * St::bytes + kLaneBytes<KD, W>;
+        DELTA_TRY(smem_limit(delta_rchain_k<F, T, KD, W>, bytes));
+        delta_rchain_k<F, T, KD, W><<<grid, W * 32, bytes, s>>>(a);
     } else {
         using St = ChainStage<F, KD, W>;
-        DELTA_TRY(smem_limit(delta_chain_k<F, T, KD, W>, 2 * St::bytes));
-        delta_chain_k<F, T, KD, W><<<grid, W * 32, 2 * St::bytes, s>>>(a);
+        constexpr size_t bytes = 2 * St::bytes + kLaneBytes<KD, W>;
+        DELTA_TRY(smem_limit(delta_chain_k<F, T, KD, W>, bytes));
+        delta_chain_k<F, T, KD, W><<<grid, W * 32, bytes, s>>>(a);
     }
     note_launch();
     return cudaGetLastError();

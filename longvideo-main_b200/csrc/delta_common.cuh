@@ -43,11 +43,16 @@ __device__ __forceinline__ void mma_f16(float* c, const uint32_t* a, uint32_t b0
                  : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
                  : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
+// (not volatile: the products of several tiles can be interleaved)
 __device__ __forceinline__ void mma_tf32(float* c, const uint32_t* a, uint32_t b0, uint32_t b1) {
-    asm volatile("mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
-                 "{%0,%1,%2,%3};"
-                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+    asm("mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void mma_tf32_first(float* c, const uint32_t* a, uint32_t b0, uint32_t b1) {  // c = a b
+    asm("mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+        : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.f));
 }
 __device__ __forceinline__ uint32_t to_tf32(float x) {
     uint32_t r;
@@ -126,31 +131,37 @@ struct FmtF {
                 split_tf32(v * f[k0 + 8 * h + 2 * t + (i >> 1)], a.h[h][i], a.lo[h][i]);
             }
     }
-    // IN: B is a tile of inputs
+    // IN: B is a tile of inputs.  The products of a step are summed apart, in four
+    // chains of three that hide each other's latency, and added in float32: the
+    // matrix instruction's own sum is cut off, not rounded, and a state that
+    // takes hundreds of steps drifted by it (6e-6 of its norm instead of 3e-7).
     template <int P, bool TR, bool IN = false>
     static __device__ __forceinline__ void mma2(float* c0, float* c1, const Af<P>& a, const E* s, int ld, int n0,
                                                 int k0) {
         const Lane L;
+        float x[4][4];
+        uint32_t hi[4][2], lo[4][2];
 #pragma unroll
-        for (int half = 0; half < 2; ++half) {
-            float* c = half ? c1 : c0;
-            float x[4] = {};
-            const int n = n0 + 8 * half + L.g;
+        for (int i = 0; i < 4; ++i) {  // i: 8 columns, 8 of the summed index
+            const int n = n0 + 8 * (i >> 1) + L.g, k = k0 + 8 * (i & 1) + 2 * L.t;
+            float2 v;
+            if constexpr (TR) v = make_float2(s[k * ld + n], s[(k + 1) * ld + n]);
+            else v = *reinterpret_cast<const float2*>(s + n * ld + k);
+            split_tf32(v.x, hi[i][0], lo[i][0]);
+            split_tf32(v.y, hi[i][1], lo[i][1]);
+        }
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                const int k = k0 + 8 * h + 2 * L.t;
-                float2 v;
-                if constexpr (TR) v = make_float2(s[k * ld + n], s[(k + 1) * ld + n]);
-                else v = *reinterpret_cast<const float2*>(s + n * ld + k);
-                uint32_t bh0, bl0, bh1, bl1;
-                split_tf32(v.x, bh0, bl0);
-                split_tf32(v.y, bh1, bl1);
-                mma_tf32(x, a.lo[h], bh0, bh1);
-                if constexpr (!(X && IN)) mma_tf32(x, a.h[h], bl0, bl1);
-                mma_tf32(x, a.h[h], bh0, bh1);
-            }
+        for (int i = 0; i < 4; ++i) mma_tf32_first(x[i], a.lo[i & 1], hi[i][0], hi[i][1]);
+        if constexpr (!(X && IN)) {
 #pragma unroll
-            for (int i = 0; i < 4; ++i) c[i] += x[i];
+            for (int i = 0; i < 4; ++i) mma_tf32(x[i], a.h[i & 1], lo[i][0], lo[i][1]);
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) mma_tf32(x[i], a.h[i & 1], hi[i][0], hi[i][1]);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            c0[e] += x[0][e] + x[1][e];
+            c1[e] += x[2][e] + x[3][e];
         }
     }
     static __device__ __forceinline__ void load_t(float* x0, float* x1, const E* s, int ld, int r0, int c0) {
