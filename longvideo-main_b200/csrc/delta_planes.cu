@@ -1,22 +1,32 @@
-// delta_planes.cu -- the gated delta rule on bfloat16 inputs (sm_100a).
+// delta_planes.cu -- the gated delta rule on bfloat16 and float16 inputs (sm_100a).
 //
-// The formulas are those of delta.cu.  Here every product runs on bf16
-// operands: the inputs are exact in bf16, and a float32 result that goes back
-// in as an operand is split into two bf16 planes, x = hi + lo (16 significant
-// bits), or rounded to one where a term's rounding stays far below the
-// output's own (said where it is done).
+// The formulas are those of delta.cu.  Here every product runs on 16-bit
+// operands of the inputs' type: the inputs are exact in it, and a float32
+// result that goes back in as an operand is split into two planes of it,
+// x = hi + lo (16 significant bits in bfloat16, 22 in float16), or rounded to
+// one where a term's rounding stays below the output's own (said where it is
+// done).  With one plane everywhere dg was off by 5e-3 of its norm.
 //
-// The two chains are bound by the length of one chunk's dependent products, as
-// only 16-column groups of a state run side by side (a warp each, 8 a head of
-// 128): so everything that does not depend on the state is taken out of the
-// warp that carries it.  A CTA holds G such warps, one or more helpers (the
-// forward's outputs; the reverse chain's Q^T dO) and a loading warp, which
-// copies each chunk's rows and tiles to shared memory with bulk copies, two
-// chunks deep, and stores what a backward reads: rows of the inputs by tensor maps (64 tokens by 64 or 16 columns,
-// swizzled so that ldmatrix meets no bank twice; a bulk copy for each row of
-// 256 bytes took 67 cycles a row and bound the chains).  Tiles that kernels hand to each other (T', M, S, U, dS, dV) lie
-// in the workspace as they lie in shared memory, padding included, so that a
-// tile is one copy.  Every wait is bounded.
+// The kernels, with times at B=4 L=16384 H=8 (forward) and B=8 L=8192 H=6
+// (training), K = V = 128, bfloat16:
+//   planes_prep_k    per chunk: gam, d, T' and M            145 us; 112 us
+//   planes_chain_k   the chunks in order: S, U and the outputs  598 us; 519 us
+//   planes_rchain_k  the chunks in reverse order: dV and dS     445 us
+//   planes_grad_k    per chunk: dQ, dK, dbeta, dg               797 us
+//
+// The two chains are bound by the length of one chunk's dependent products (2.3
+// us each; 256 chunks of a head follow one another), as only 16-column groups
+// of a state run side by side (a warp each, 8 a head of 128): so everything
+// that does not depend on the state is taken out of the warp that carries it.
+// A CTA holds G such warps, one or more helpers (the forward's outputs; the
+// reverse chain's Q^T dO) and a loading warp, which copies each chunk's rows
+// and tiles to shared memory, two chunks deep, and stores what a backward
+// reads.  Rows of the inputs come by tensor maps (64 tokens by 64 or 16
+// columns, swizzled so that ldmatrix meets no bank twice; a bulk copy for each
+// row of 256 bytes took 67 cycles a row and bound the chains).  Tiles that
+// kernels hand to each other (T', M, S, U, dS, dV) lie in the workspace as
+// they lie in shared memory, padding included, so that a tile is one copy.
+// Every wait is bounded.
 #include <cuda.h>
 #include <cudaTypedefs.h>
 

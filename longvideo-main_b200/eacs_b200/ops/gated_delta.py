@@ -14,7 +14,14 @@ per row and updates the state in place, for streaming.
 Layouts: q, k (B, L, Hk, K), v (B, L, Hv, V), g and beta (B, L, Hv), states
 (B, Hv, K, V) float32.  Hv is a multiple of Hk; value head h reads key head
 h // (Hv // Hk).  Views are taken with their strides (a slice of a fused
-projection needs no copy) as long as their last dimension is dense.
+projection needs no copy) as long as their last dimension is dense; 16-bit
+ones are fastest when their rows start on 16 bytes (K, V and all strides
+multiples of 8).  Sums and states are float32.  Operands of the products keep
+22 significant bits, 16 for bfloat16 inputs.  With float16 inputs states have
+to stay within float16's range.  The same inputs give the same bits.
+
+A backward that is captured into a graph must not share leaves with an eager
+graph that is still alive (autograd's own rule).
 """
 from __future__ import annotations
 
