@@ -392,7 +392,7 @@ __global__ void __launch_bounds__(128) planes_prep_k(const __grid_constant__ DAr
         }
     }
     __syncthreads();
-    if (!mbar_wait(&land, 0)) return;
+    mbar_wait(&land, 0);  // (one that runs out is recorded; nobody leaves the barriers below)
     if (rows < min(kC, a.L - c * kC)) {
         if (warp == 0) zero_rows<64>(sK, 2 * (KD / 64), rows);
         __syncthreads();
@@ -1747,7 +1747,8 @@ __global__ void __launch_bounds__(32 * kGradWarps, 1) planes_grad_k(const __grid
                     gate_store(a.dbeta, a.gate_dtype, o + a.Hv, i0 + 1 < rows ? sDb[i0 + 1] : 0.f);
                 }
             }
-            sync_compute();  // the sums and dK_write have been read
+            // the sums and dK_write have been read; all warps leave together where a wait ran out
+            ok = __syncthreads_and(ok);
         }
         warp_arrive(&qempty[seen & 1]);
         ++seen;
