@@ -160,8 +160,11 @@ def gated_delta_step(q: Tensor, k: Tensor, v: Tensor, g: Tensor, beta: Tensor, s
                      scale: float | None = None) -> Tensor:
     """One token per row: q, k (B, Hk, K), v (B, Hv, V), g and beta (B, Hv);
     `state` (B, Hv, K, V) float32, contiguous, is updated in place.  Returns
-    o (B, Hv, V) in q's dtype.  No gradient."""
+    o (B, Hv, V) in q's dtype.  No gradient: inputs that want one are refused
+    where gradients are enabled."""
     dev = _check("gated_delta_step", q, k, v, g, beta, None, state, 1)
+    if torch.is_grad_enabled() and any(t.requires_grad for t in (q, k, v, g, beta)):
+        raise RuntimeError("gated_delta_step: has no gradient; call it under torch.no_grad() or with detached tensors")
     if not state.is_contiguous() or state.requires_grad:
         raise RuntimeError("gated_delta_step: the state is updated in place: it must be contiguous and without a gradient")
     scale = q.shape[-1] ** -0.5 if scale is None else float(scale)

@@ -431,3 +431,71 @@ def test_refusals():
     gated_delta_step(*tok, leaf)
     with pytest.raises(RuntimeError, match="modified by an inplace operation"):
         y.backward()
+
+
+def test_step_refuses_inputs_that_want_a_gradient():
+    d, _, _ = make(2, 1, 1, 2, 16, 8, torch.float32, seed=31)
+    tok = [d[n][:, 0] for n in ("q", "k", "v", "g", "beta")]
+    before = d["initial"].clone()
+    for i in range(5):
+        bad = [t.clone().requires_grad_(j == i) for j, t in enumerate(tok)]
+        with pytest.raises(RuntimeError, match="no gradient"):
+            gated_delta_step(*bad, d["initial"])
+        assert torch.equal(d["initial"], before)
+        with torch.no_grad():
+            o = gated_delta_step(*bad, d["initial"].clone())
+        assert torch.equal(o, gated_delta_step(*tok, d["initial"].clone()))
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_backward_twice_and_two_calls_at_once(dtype):
+    """What a forward keeps serves every backward of it; calls on two streams share nothing."""
+    runs = []
+    for i in range(2):
+        d, do, dS = make(2, 300, 2, 4, 128, 64, dtype, seed=32 + i)
+        x = {n: t.detach().clone().requires_grad_(True) for n, t in d.items()}
+        runs.append((x, do, dS))
+
+    def forward(x):
+        return gated_delta_rule(*(x[n] for n in ("q", "k", "v", "g", "beta")), initial_state=x["initial"], output_final_state=True)
+    want = []
+    for x, do, dS in runs:
+        out = forward(x)
+        first = torch.autograd.grad(out, list(x.values()), [do, dS], retain_graph=True)
+        again = torch.autograd.grad(out, list(x.values()), [do, dS])
+        assert all(torch.equal(a, b) for a, b in zip(first, again))
+        want.append([t.detach() for t in out] + list(first))
+    torch.cuda.synchronize()
+    streams, got = [torch.cuda.Stream() for _ in runs], [[], []]
+    for _ in range(3):
+        for i, (x, do, dS) in enumerate(runs):
+            with torch.cuda.stream(streams[i]):
+                out = forward(x)
+                got[i].append([t.detach() for t in out] + list(torch.autograd.grad(out, list(x.values()), [do, dS])))
+    torch.cuda.synchronize()
+    for i in range(2):
+        for g in got[i]:
+            assert all(torch.equal(a, b) for a, b in zip(g, want[i]))
+
+
+def test_sequences_past_32_bit_offsets():
+    """The last row of a batch with over 2^31 values, forward and backward, against that row alone (each within the
+    tolerance of the truth)."""
+    B, L, H, K, V = 2, 66000, 128, 64, 128
+    gen = torch.Generator(DEV).manual_seed(34)
+    rnd = lambda *s: torch.empty(*s, dtype=torch.bfloat16, device=DEV).normal_(generator=gen)
+    x = dict(q=rnd(B, L, H, K).mul_(K ** -0.5), k=rnd(B, L, H, K).mul_(K ** -0.5), v=rnd(B, L, H, V),
+             g=-0.1 * torch.rand(B, L, H, generator=gen, device=DEV), beta=torch.rand(B, L, H, generator=gen, device=DEV))
+    do = rnd(B, L, H, V)
+    res = []
+    for rows in (slice(0, B), slice(B - 1, B)):
+        leaves = [t[rows].detach().requires_grad_(True) for t in x.values()]
+        o, S = gated_delta_rule(*leaves, output_final_state=True)
+        grads = torch.autograd.grad(o, leaves, do[rows])
+        res.append([t[-1].detach().clone() for t in (o, S, *grads)])
+        del o, S, grads, leaves
+    for n, a, b in zip(("o", "S", "dq", "dk", "dv", "dg", "dbeta"), *res):
+        err, ref = float((a.float() - b.float()).norm()), float(b.float().norm())
+        assert ref > 0 and err <= 2 * tol(a.dtype, torch.bfloat16) * ref, (n, err / ref)
+    del x, do, res
+    torch.cuda.empty_cache()
