@@ -41,10 +41,10 @@
 // These kernels take float32 inputs, and 16-bit ones that delta_planes.cu does
 // not (rows that do not start on 16 bytes, expanded dimensions).  Operands are
 // tf32 split in two (22 bits), three products each: errors are 3e-7 to 5e-7 of
-// the norm.  Times at B=4 L=9498 H=10 K=128 V=64, float32: delta_prep_k 193 us,
-// delta_chain_k 1958, delta_out_k 881, delta_rchain_k 3467, delta_grad_k 1314.
+// the norm.  Times at B=4 L=9498 H=10 K=128 V=64, float32: delta_prep_k 162 us,
+// delta_chain_k 1648, delta_out_k 446, delta_rchain_k 2986, delta_grad_k 1072.
 // The chains are bound by a chunk's dependent products on one warp of each
-// scheduler (13 and 23 us a chunk), the others by the products and the
+// scheduler (11 and 20 us a chunk), the others by the products and the
 // splitting of every tile as it is read.
 #include <algorithm>
 

@@ -54,14 +54,14 @@ __device__ __forceinline__ void mma_tf32_first(float* c, const uint32_t* a, uint
         : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.f));
 }
-__device__ __forceinline__ uint32_t to_tf32(float x) {
-    uint32_t r;
-    asm("cvt.rna.tf32.f32 %0, %1;" : "=r"(r) : "f"(x));
-    return r;
-}
+// x = hi + lo in tf32 (11 significant bits each): hi to the nearest, lo cut off,
+// of either sign, so x is off by at most 2^-22 of itself.  In integer operations:
+// the conversion instruction runs at a fraction of their rate (the chains took
+// a fifth longer, delta_out_k half).  A NaN whose bits the addition overflows is
+// still one in lo.
 __device__ __forceinline__ void split_tf32(float x, uint32_t& hi, uint32_t& lo) {
-    hi = to_tf32(x);
-    lo = to_tf32(x - __uint_as_float(hi));
+    hi = (__float_as_uint(x) + 0x1000u) & 0xffffe000u;
+    lo = __float_as_uint(x - __uint_as_float(hi)) & 0xffffe000u;
 }
 
 // Lane coordinates: an accumulator tile (16 x 8) holds rows g, g + 8 and
@@ -147,8 +147,13 @@ struct FmtF {
             float2 v;
             if constexpr (TR) v = make_float2(s[k * ld + n], s[(k + 1) * ld + n]);
             else v = *reinterpret_cast<const float2*>(s + n * ld + k);
-            split_tf32(v.x, hi[i][0], lo[i][0]);
-            split_tf32(v.y, hi[i][1], lo[i][1]);
+            if constexpr (X && IN) {
+                hi[i][0] = __float_as_uint(v.x);
+                hi[i][1] = __float_as_uint(v.y);
+            } else {
+                split_tf32(v.x, hi[i][0], lo[i][0]);
+                split_tf32(v.y, hi[i][1], lo[i][1]);
+            }
         }
 #pragma unroll
         for (int i = 0; i < 4; ++i) mma_tf32_first(x[i], a.lo[i & 1], hi[i][0], hi[i][1]);

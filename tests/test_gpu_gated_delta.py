@@ -499,3 +499,28 @@ def test_sequences_past_32_bit_offsets():
         assert ref > 0 and err <= 2 * tol(a.dtype, torch.bfloat16) * ref, (n, err / ref)
     del x, do, res
     torch.cuda.empty_cache()
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("pad", [0, 3])
+@pytest.mark.parametrize("bad", [float("nan"), float("inf")])
+def test_nan_and_infinity_of_a_token_reach_what_follows(dtype, pad, bad):
+    """Also NaN with every bit set; rows that start on 16 bytes and not.  The chunks before are as they were."""
+    d, _, _ = make(1, 200, 1, 2, 64, 64, dtype, seed=35)
+    clean = {n: t.clone() for n, t in d.items()}
+    d["k"][0, 70, 0, 5] = bad
+    if bad != bad:
+        bits = d["k"].view(torch.int16 if dtype.itemsize == 2 else torch.int32)
+        bits[0, 70, 0, 5] = torch.iinfo(bits.dtype).max
+    outs = []
+    for x in (clean, d):
+        args = []
+        for n in ("q", "k", "v"):
+            wide = torch.zeros(*x[n].shape[:-1], 64 + 8 + pad, dtype=dtype, device=DEV)
+            wide[..., pad:pad + 64].copy_(x[n])
+            args.append(wide[..., pad:pad + 64])
+        outs.append(gated_delta_rule(*args, x["g"], x["beta"], initial_state=x["initial"], output_final_state=True))
+    (o0, S0), (o1, S1) = outs
+    assert bool(torch.isfinite(o0).all() and torch.isfinite(S0).all())
+    assert torch.equal(o0[:, :64], o1[:, :64])
+    assert not bool(torch.isfinite(o1[:, 128:]).any()) and not bool(torch.isfinite(S1).any())
