@@ -136,7 +136,7 @@ typedef struct EacsDelta {
     int32_t gate_dtype;
 } EacsDelta;
 
-/* Chunked forward: o (B,L,Hv,V) dense of dtype; final_state (B,Hv,K,V)
+/* Chunked forward: o (B,L,Hv,V) dense of dtype, on 16 bytes; final_state (B,Hv,K,V)
  * float32 or NULL.  With training != 0 the workspace holds what
  * eacs_delta_bwd reads and is kept, unchanged, until then.  Products run on the
  * tensor cores with operands split in two: tf32, 22 significant bits, or, for
@@ -149,8 +149,8 @@ EACS_API int eacs_delta_fwd(const EacsDelta* p, void* o, float* final_state, voi
 EACS_API size_t eacs_delta_workspace_size(const EacsDelta* p, int training);
 
 /* Backward: dout (B,L,Hv,V) of dtype with its strides, dfinal (B,Hv,K,V)
- * float32 or NULL (the final state's gradient); dq, dk, dv dense of dtype
- * (dq and dk summed over the value heads of a key head), dg and dbeta dense
+ * float32 or NULL (the final state's gradient); dq, dk, dv dense of dtype, on
+ * 16 bytes (dq and dk summed over the value heads of a key head), dg and dbeta dense
  * of gate_dtype, dinitial (B,Hv,K,V) float32 or NULL.  `saved` is the
  * workspace of the training forward with the same arguments.  Where q, k and v
  * are 16-bit and read 16 bytes at a time, dout's rows have to start on 16

@@ -47,6 +47,7 @@
 // scheduler (11 and 20 us a chunk), the others by the products and the
 // splitting of every tile as it is read.
 #include <algorithm>
+#include <initializer_list>
 
 #include "delta_common.cuh"
 
@@ -1256,6 +1257,13 @@ void set_workspace(DArgs& a, const EacsDelta& p, void* ws, bool training) {
     a.U = w;
 }
 bool inputs_set(const EacsDelta& p) { return p.q && p.k && p.v && p.g && p.beta; }
+// Outputs and the gradients of tokens are stored in pairs, or 16 bytes at a time
+// where K and V are multiples of 8: every store is aligned if their starts are.
+bool on16(std::initializer_list<const void*> ps) {
+    uintptr_t bits = 0;
+    for (const void* p : ps) bits |= reinterpret_cast<uintptr_t>(p);
+    return (bits & 15u) == 0;
+}
 
 }  // namespace
 
@@ -1282,6 +1290,7 @@ int delta_fwd(const EacsDelta& p, void* o, float* final_state, void* ws, size_t 
                           fn);
     }
     if (!inputs_set(p) || !o) return fail(EACS_ERR_INVALID, "%s: null pointer argument", fn);
+    if (!on16({o})) return fail(EACS_ERR_INVALID, "%s: o must start on 16 bytes", fn);
     DArgs a = make_args(p);
     const size_t need = fwd_sizes(p, a, training).total;
     if (!ws || ws_bytes < need) return fail(EACS_ERR_WORKSPACE, "%s: workspace of %zu bytes, %zu needed", fn, ws_bytes, need);
@@ -1330,6 +1339,7 @@ int delta_bwd(const EacsDelta& p, const DeltaGrads& d, const void* saved, size_t
     }
     if (!inputs_set(p) || !d.dout || !d.dq || !d.dk || !d.dv || !d.dg || !d.dbeta)
         return fail(EACS_ERR_INVALID, "%s: null pointer argument", fn);
+    if (!on16({d.dq, d.dk, d.dv})) return fail(EACS_ERR_INVALID, "%s: dq, dk and dv must start on 16 bytes", fn);
     DArgs a = make_args(p);
     const size_t need_saved = fwd_sizes(p, a, true).total, need = bwd_sizes(p, a).total;
     if (!saved || saved_bytes < need_saved)

@@ -123,3 +123,19 @@ def test_install_norms(monkeypatch):
         assert cls + ".__init__" in patched
         assert type(getattr(mods[n], cls)(8).norm) is LayerNorm
         assert not hasattr(getattr(mods[n], cls).__init__.__wrapped__, "__wrapped__")
+
+
+@pytest.mark.parametrize("dtype", [0, 1, 2])
+def test_delta_rejects_outputs_off_16_bytes_without_device(dtype):
+    """Outputs and 16-bit gradients are written up to 16 bytes at a time."""
+    L = _lib.lib()
+    strides, big = (ctypes.c_int64 * 3)(1, 1, 1), 1 << 40
+    off = P + (4 if dtype == 0 else 2)
+    assert L.eacs_delta_fwd(delta(dtype=dtype, gate=dtype), off, None, P, big, 0, None) == _lib.EACS_ERR_INVALID
+    assert "16 bytes" in _lib.last_error()
+    for i in range(3):
+        grads = [P] * 5
+        grads[i] = off
+        assert L.eacs_delta_bwd(delta(dtype=dtype, gate=dtype), P, strides, None, *grads, None, P, big, P, big,
+                                None) == _lib.EACS_ERR_INVALID
+        assert "16 bytes" in _lib.last_error()
