@@ -114,9 +114,10 @@ EACS_API size_t eacs_layer_norm_bwd_workspace_size(int64_t rows, int64_t d);
  * initial_state (B,Hv,K,V) float32 dense or NULL (zeros).  K goes up to 128,
  * V to 1024.  Rows of q, k, v that start on 16 bytes, with K and V multiples
  * of 8, are read 16 bytes at a time; 16-bit inputs of that kind (no dimension
- * of more than one element having stride 0) take the fastest kernels.  Which
- * kernels run goes by the pointers' alignment and the strides, and so do the
- * workspace sizes: ask for them with the arguments of the call. */
+ * of more than one element having stride 0) take the fastest kernels, bfloat16
+ * always, float16 where no backward follows.  Which kernels run goes by the
+ * pointers' alignment and the strides, and so do the workspace sizes: ask for
+ * them with the arguments of the call. */
 typedef struct EacsDelta {
     const void* q;
     const void* k;
@@ -139,11 +140,11 @@ typedef struct EacsDelta {
 /* Chunked forward: o (B,L,Hv,V) dense of dtype, on 16 bytes; final_state (B,Hv,K,V)
  * float32 or NULL.  With training != 0 the workspace holds what
  * eacs_delta_bwd reads and is kept, unchanged, until then.  Products run on the
- * tensor cores with operands split in two: tf32, 22 significant bits, or, for
- * 16-bit inputs whose rows are read 16 bytes at a time, two values of their
- * type (bfloat16 16 bits; float16 22 bits, and what is split, states and
- * values corrected by them, has to stay within 65504 there); all sums and the
- * state are float32. */
+ * tensor cores with operands split in two: tf32, 22 significant bits, or, in
+ * the 16-bit kernels, two values of the inputs' type (bfloat16 16 bits; float16
+ * 22 bits of the largest value of a tile, which is brought into its range by a
+ * power of two); all sums and the state are float32.  With training, beta is
+ * held 2^-64 away from 0. */
 EACS_API int eacs_delta_fwd(const EacsDelta* p, void* o, float* final_state, void* workspace, size_t workspace_bytes,
                             int training, void* stream);
 EACS_API size_t eacs_delta_workspace_size(const EacsDelta* p, int training);
@@ -153,7 +154,7 @@ EACS_API size_t eacs_delta_workspace_size(const EacsDelta* p, int training);
  * 16 bytes (dq and dk summed over the value heads of a key head), dg and dbeta dense
  * of gate_dtype, dinitial (B,Hv,K,V) float32 or NULL.  `saved` is the
  * workspace of the training forward with the same arguments.  Where q, k and v
- * are 16-bit and read 16 bytes at a time, dout's rows have to start on 16
+ * are bfloat16 and read 16 bytes at a time, dout's rows have to start on 16
  * bytes too, without a stride of 0. */
 EACS_API int eacs_delta_bwd(const EacsDelta* p, const void* dout, const int64_t* dout_stride, const float* dfinal,
                             void* dq, void* dk, void* dv, void* dg, void* dbeta, float* dinitial, const void* saved,

@@ -21,8 +21,8 @@
 //   dG_i = q_i.dQ_i + k_i.(dK_read - dK_write)_i,
 //   dg_i = sum_{j >= i} dG_j + <S1, dS1>
 // (a decay reaches every product between a token at or behind it that reads
-// and one before it that wrote; beta is held 2^-64 away from 0 so that it can
-// be divided out).  Gam is formed from a sum of g kept in two floats, so that
+// and one before it that wrote; for a backward beta is held 2^-64 away from 0 so
+// that it can be divided out).  Gam is formed from a sum of g kept in two floats, so that
 // a decay of 0 in a chunk takes nothing from the precision behind it.
 //
 // Only S and dS go from chunk to chunk.  The kernels:
@@ -39,7 +39,8 @@
 // shuffle or a barrier between them.
 //
 // These kernels take float32 inputs, and 16-bit ones that delta_planes.cu does
-// not (rows that do not start on 16 bytes, expanded dimensions).  Operands are
+// not (rows that do not start on 16 bytes, expanded dimensions, float16 training:
+// B=2 L=4096 H=12 K=V=64 forward and backward 2.4 ms).  Operands are
 // tf32 split in two (22 bits), three products each: errors are 3e-7 to 5e-7 of
 // the norm.  Times at B=4 L=9498 H=10 K=128 V=64, float32: delta_prep_k 162 us,
 // delta_chain_k 1648, delta_out_k 446, delta_rchain_k 2986, delta_grad_k 1072.
@@ -140,7 +141,8 @@ __global__ void __launch_bounds__(128) delta_prep_k(DArgs a) {
             float gv = 0.f, bv = 0.f;
             if (r < rows) {
                 gv = gate_value(a.g, a.gate_dtype, b * a.sg.b + (t0 + r) * a.sg.t + h * a.sg.h);
-                bv = hold_beta(gate_value(a.beta, a.gate_dtype, b * a.sb.b + (t0 + r) * a.sb.t + h * a.sb.h));
+                bv = gate_value(a.beta, a.gate_dtype, b * a.sb.b + (t0 + r) * a.sb.t + h * a.sb.h);
+                if (a.M) bv = hold_beta(bv);  // a backward divides by it
                 gv = gv < -200.f ? -200.f : gv;  // e^-200 is 0 in float32
             }
             s[i] = gv;
@@ -1208,19 +1210,22 @@ bool mapped(int64_t B, int64_t L, int64_t H, const int64_t* st) {
         if (n[i] > 1 && (st[i] <= 0 || st[i] >= int64_t{1} << 39)) return false;
     return true;
 }
-// Whether the 16-bit kernels take these inputs.  The backward goes by the forward's inputs alone, as it
+// Whether the 16-bit kernels take these inputs: bfloat16, and float16 where no
+// backward follows.  float16's exponent is too short for what a backward keeps
+// and divides (a rate of 1e-4 left 8 bits of dbeta, one of 0 none), so its
+// training runs in tf32.  The backward goes by the forward's inputs alone, as it
 // reads what the forward left (an upstream gradient in another layout is
 // refused by delta_bwd then).
-bool planes(const EacsDelta& p, const DArgs& a) {
-    return p.dtype != EACS_DTYPE_F32 && a.vec_qk && a.vec_v && mapped(p.B, p.L, p.Hk, p.q_stride) &&
-           mapped(p.B, p.L, p.Hk, p.k_stride) && mapped(p.B, p.L, p.Hv, p.v_stride);
+bool planes(const EacsDelta& p, const DArgs& a, bool training) {
+    return (p.dtype == EACS_DTYPE_BF16 || (p.dtype == EACS_DTYPE_F16 && !training)) && a.vec_qk && a.vec_v &&
+           mapped(p.B, p.L, p.Hk, p.q_stride) && mapped(p.B, p.L, p.Hk, p.k_stride) && mapped(p.B, p.L, p.Hv, p.v_stride);
 }
 
 struct Sizes { size_t gates, T, M, S, U, total; };
 Sizes fwd_sizes(const EacsDelta& p, const DArgs& a, bool training) {
     const size_t ids = static_cast<size_t>(p.B) * p.Hv * chunks(p.L), e = sizeof(float);
     Sizes z{};
-    if (planes(p, a)) {
+    if (planes(p, a, training)) {
         z.total = planes_saved_size(a, training);
         return z;
     }
@@ -1236,7 +1241,7 @@ struct BSizes { size_t dS, dV, group, total; };
 BSizes bwd_sizes(const EacsDelta& p, const DArgs& a) {
     const size_t ids = static_cast<size_t>(p.B) * p.Hv * chunks(p.L), e = sizeof(float);
     BSizes z{};
-    if (planes(p, a)) {
+    if (planes(p, a, true)) {
         z.dS = align256(planes_bwd_size(a));
     } else {
         z.dS = align256(ids * pad16(p.V) * key_pad(p.K) * e);
@@ -1299,7 +1304,7 @@ int delta_fwd(const EacsDelta& p, void* o, float* final_state, void* ws, size_t 
     a.out = o;
     a.final_state = final_state;
     cudaError_t e;
-    if (planes(p, a))
+    if (planes(p, a, training))
         e = planes_fwd(a, ws, training, stream);
     else if (p.dtype == EACS_DTYPE_BF16)
         e = p.K <= 64 ? run_fwd<FmtF<true>, __nv_bfloat16, 64>(a, stream) : run_fwd<FmtF<true>, __nv_bfloat16, 128>(a, stream);
@@ -1354,7 +1359,7 @@ int delta_bwd(const EacsDelta& p, const DeltaGrads& d, const void* saved, size_t
     a.dq = d.dq; a.dk = d.dk; a.dv = d.dv; a.dg = d.dg; a.dbeta = d.dbeta;
     a.dfinal = d.dfinal;
     a.dinitial = d.dinitial;
-    if (planes(p, a) && !(a.vec_do && mapped(p.B, p.L, p.Hv, d.dout_stride)))
+    if (planes(p, a, true) && !(a.vec_do && mapped(p.B, p.L, p.Hv, d.dout_stride)))
         return fail(EACS_ERR_INVALID, "%s: rows of dout must start on 16 bytes, with strides above 0, where those of q, k and v do", fn);
     const BSizes z = bwd_sizes(p, a);
     char* w = static_cast<char*>(ws);
@@ -1362,7 +1367,7 @@ int delta_bwd(const EacsDelta& p, const DeltaGrads& d, const void* saved, size_t
     a.dV = w; w += z.dV;
     float* group = reinterpret_cast<float*>(w);
     cudaError_t e;
-    if (planes(p, a))
+    if (planes(p, a, true))
         e = planes_bwd(a, const_cast<void*>(saved), ws, group, stream);
     else if (p.dtype == EACS_DTYPE_BF16)
         e = p.K <= 64 ? run_bwd<FmtF<true>, __nv_bfloat16, 64>(a, group, stream) : run_bwd<FmtF<true>, __nv_bfloat16, 128>(a, group, stream);

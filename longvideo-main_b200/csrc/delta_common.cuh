@@ -201,7 +201,8 @@ struct DArgs {
     int vec_qk, vec_v, vec_do;  // rows can be read 16 bytes at a time
     float scale;
     // workspace, per chunk id ((b Hv + h) n + c)
-    float* gates;  // [id][6][64]: G (high), G (low), gam, d, scale gam, 1 / beta (delta_planes.cu)
+    float* gates;  // [id][6][64]: G (high), G (low), gam, d, scale gam, 1 / beta (delta_planes.cu; there with
+                   // float16: beta, what T' and M are to be multiplied by, gam, d, scale gam)
     void* T;       // [id][planes][64][64]
     void* M;       // [id][64][64] or null
     void* S;       // [id][Vp][KD]: S0^T or null

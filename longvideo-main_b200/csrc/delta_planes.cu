@@ -1,4 +1,5 @@
-// delta_planes.cu -- the gated delta rule on bfloat16 and float16 inputs (sm_100a).
+// delta_planes.cu -- the gated delta rule on bfloat16 inputs, and the forward pass
+// without a backward on float16 ones (sm_100a).
 //
 // The formulas are those of delta.cu.  Here every product runs on 16-bit
 // operands of the inputs' type: the inputs are exact in it, and a float32
@@ -6,6 +7,14 @@
 // x = hi + lo (16 significant bits in bfloat16, 22 in float16), or rounded to
 // one where a term's rounding stays below the output's own (said where it is
 // done).  With one plane everywhere dg was off by 5e-3 of its norm.
+//
+// float16's exponent is too short for this by itself: below 2^-3 the low plane
+// runs out.  There T' and M, S, X and U are scaled by powers of two (Scaled
+// below), and T' is made without beta: with Ahat_ij = Gam_ij k_i.k_j (j < i) and
+// D = diag(beta), e = (I + Ahat D)^-1 X and U = D e, so that a small beta meets
+// float32 only (B=3 L=1001 H=8 K=64 V=96: 51 us with it, 43 without).  What a
+// backward keeps and multiplies (S, U, dS and dV of all groups in one sum) would
+// need scales of its own, so float16 training runs on the kernels of delta.cu.
 //
 // The kernels, with times at B=4 L=16384 H=8 (forward) and B=8 L=8192 H=6
 // (training), K = V = 128, bfloat16:
@@ -99,6 +108,40 @@ template <> struct Num<__half> {
     static __device__ __forceinline__ float2 unpack(uint32_t v) { return __half22float2(*reinterpret_cast<const __half2*>(&v)); }
     static __device__ __forceinline__ void mma(float* c, const uint32_t* a, uint32_t b0, uint32_t b1) { mma_f16(c, a, b0, b1); }
 };
+
+// float16's exponent is short: two planes hold 22 bits of values from 2^-3 up,
+// and a step of 2^-25 below.  So its tiles are kept near 1 by powers of two
+// (Scaled): a tile whose largest value is between 2^-3 and 2^13 stays as it is,
+// any other is brought to 2^4, and is then off by at most 2^-22 of its largest value.
+// bfloat16 has float32's exponent and needs none of it.
+template <typename T> constexpr bool Scaled = false;
+template <> constexpr bool Scaled<__half> = true;
+
+constexpr int kMaxExp = 100;  // of a scale
+__device__ __forceinline__ float pow2(int e) { return __int_as_float((e + 127) << 23); }
+__device__ __forceinline__ uint32_t abs_bits(float v) { return __float_as_uint(v) & 0x7fffffffu; }  // ordered as |v| is
+template <int N>
+__device__ __forceinline__ uint32_t max_bits(const float (*x)[4]) {  // of a warp's tile
+    float m[4] = {};
+#pragma unroll
+    for (int j = 0; j < N; ++j)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) m[e] = fmaxf(m[e], fabsf(x[j][e]));
+    return __reduce_max_sync(0xffffffffu, abs_bits(fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3]))));
+}
+// The exponent to scale a tile by whose largest absolute value has these bits (0
+// for a tile of zeros, and for one that is infinite: nothing helps it)
+__device__ __forceinline__ int scale_exp(uint32_t bits) {
+    const int e = static_cast<int>(bits >> 23) - 127;
+    return bits == 0 || (e >= -3 && e < 13) || e == 128 ? 0 : max(-kMaxExp, min(kMaxExp, 4 - e));
+}
+template <int N>
+__device__ __forceinline__ void scale_tile(float (*x)[4], float f) {
+#pragma unroll
+    for (int j = 0; j < N; ++j)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) x[j][e] *= f;
+}
 
 template <int P> struct Af { uint32_t r[P][4]; };  // 16 x 16 of A in P planes
 
@@ -305,7 +348,7 @@ __device__ __forceinline__ float ratio(const float* G, int i, int j) {
 // ----------------------------------------------------------------------------
 // gates, T' and M of a chunk
 // ----------------------------------------------------------------------------
-// Two warps make M and two A, of each one block rows 3 and 0 (of 16 tokens), the
+// Two warps make M and two A (float16: Ahat D), of each one block rows 3 and 0 (of 16 tokens), the
 // other 2 and 1: five 16 x 16 blocks each.  Blocks above the diagonal are neither
 // made nor written, as no product reads them.  The latter two then invert I + A by
 // blocks, in float32: the 16 x 16 blocks on the diagonal by forward substitution (a
@@ -341,9 +384,11 @@ __global__ void __launch_bounds__(128) planes_prep_k(const __grid_constant__ DAr
     float* sA = reinterpret_cast<float*>(smem);  // A below the diagonal blocks, products above (after K and Q)
     float* sT = sA + kC * kAld;                  // its inverse
     __shared__ float sG[2 * kC], sB[kC];
+    __shared__ uint32_t sMax[4];
     __shared__ uint64_t land;
     const int tid = threadIdx.x, warp = tid >> 5;
     const Lane L;
+    float* ga = a.gates + id * kGates;
     if (tid == 0) {
         mbar_init(&land, 1);
         fence_mbar_init();
@@ -362,7 +407,8 @@ __global__ void __launch_bounds__(128) planes_prep_k(const __grid_constant__ DAr
             float gv = 0.f, bv = 0.f;
             if (r < rows) {
                 gv = gate_value(a.g, a.gate_dtype, b * a.sg.b + (t0 + r) * a.sg.t + h * a.sg.h);
-                bv = hold_beta(gate_value(a.beta, a.gate_dtype, b * a.sb.b + (t0 + r) * a.sb.t + h * a.sb.h));
+                bv = gate_value(a.beta, a.gate_dtype, b * a.sb.b + (t0 + r) * a.sb.t + h * a.sb.h);
+                if (a.S) bv = hold_beta(bv);  // a backward divides by it
                 gv = gv < -200.f ? -200.f : gv;  // e^-200 is 0 in float32
             }
             s[i] = gv * 1.4426950408889634;  // to powers of two
@@ -376,19 +422,24 @@ __global__ void __launch_bounds__(128) planes_prep_k(const __grid_constant__ DAr
             if (L.l >= o) run += up;
         }
         const double before = run - s[1], total = __shfl_sync(0xffffffffu, run, 31);
-        float* ga = a.gates + id * kGates;
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
             const int r = 2 * L.l + i;
             const double G = before + s[i];
             const float hi = static_cast<float>(G), lo = static_cast<float>(G - hi);
             const float gam = exp2f(static_cast<float>(G));
-            sG[r] = ga[r] = hi;
-            sG[kC + r] = ga[kC + r] = lo;
+            sG[r] = hi;
+            sG[kC + r] = lo;
+            if constexpr (Scaled<T>) {  // (no backward reads G)
+                ga[r] = sB[r];
+            } else {
+                ga[r] = hi;
+                ga[kC + r] = lo;
+                if (a.S) ga[5 * kC + r] = r < rows ? 1.f / sB[r] : 0.f;
+            }
             ga[2 * kC + r] = gam;
             ga[3 * kC + r] = exp2f(static_cast<float>(total - G));
             ga[4 * kC + r] = a.scale * gam;
-            ga[5 * kC + r] = r < rows ? 1.f / sB[r] : 0.f;
         }
     }
     __syncthreads();
@@ -423,35 +474,63 @@ __global__ void __launch_bounds__(128) planes_prep_k(const __grid_constant__ DAr
     }
     __syncthreads();  // K and Q are done with
     e16* M = static_cast<e16*>(a.M) + id * 2 * kCC;
+    auto put_m = [&](const float* v, int r0, int col) {
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+            const uint32_t hi = Num<T>::pack(v[2 * e], v[2 * e + 1]);
+            const float2 f = Num<T>::unpack(hi);
+            const int o = (r0 + 8 * e) * kTld + col;
+            *reinterpret_cast<uint32_t*>(M + o) = hi;
+            *reinterpret_cast<uint32_t*>(M + kCC + o) = Num<T>::pack(v[2 * e] - f.x, v[2 * e + 1] - f.y);
+        }
+    };
 #pragma unroll
     for (int i = 0; i < 5; ++i) {
         const int rb = i < split ? rb0 : rb1, cb = i < split ? i : i - split;
         const int r0 = 16 * rb + L.g;
         const float g0 = sG[r0], g1 = sG[r0 + 8], l0 = sG[kC + r0], l1 = sG[kC + r0 + 8];
-        const float f0 = left ? sB[r0] : a.scale, f1 = left ? sB[r0 + 8] : a.scale;
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
             const int col = 16 * cb + 8 * j + 2 * L.t;
             const float2 gc = *reinterpret_cast<const float2*>(sG + col), lc = *reinterpret_cast<const float2*>(sG + kC + col);
             const int last = left ? -1 : 0;  // A without the diagonal
-            float v[4];
-            v[0] = col <= r0 + last ? f0 * ex2_approx((g0 - gc.x) + (l0 - lc.x)) * x[i][j][0] : 0.f;
-            v[1] = col + 1 <= r0 + last ? f0 * ex2_approx((g0 - gc.y) + (l0 - lc.y)) * x[i][j][1] : 0.f;
-            v[2] = col <= r0 + 8 + last ? f1 * ex2_approx((g1 - gc.x) + (l1 - lc.x)) * x[i][j][2] : 0.f;
-            v[3] = col + 1 <= r0 + 8 + last ? f1 * ex2_approx((g1 - gc.y) + (l1 - lc.y)) * x[i][j][3] : 0.f;
+            // A has beta of its row, Ahat D of its column
+            float f[4] = {a.scale, a.scale, a.scale, a.scale};
+            if (left) {
+                f[0] = sB[Scaled<T> ? col : r0];
+                f[1] = sB[Scaled<T> ? col + 1 : r0];
+                f[2] = sB[Scaled<T> ? col : r0 + 8];
+                f[3] = sB[Scaled<T> ? col + 1 : r0 + 8];
+            }
+            float* v = x[i][j];
+            v[0] = col <= r0 + last ? f[0] * ex2_approx((g0 - gc.x) + (l0 - lc.x)) * v[0] : 0.f;
+            v[1] = col + 1 <= r0 + last ? f[1] * ex2_approx((g0 - gc.y) + (l0 - lc.y)) * v[1] : 0.f;
+            v[2] = col <= r0 + 8 + last ? f[2] * ex2_approx((g1 - gc.x) + (l1 - lc.x)) * v[2] : 0.f;
+            v[3] = col + 1 <= r0 + 8 + last ? f[3] * ex2_approx((g1 - gc.y) + (l1 - lc.y)) * v[3] : 0.f;
             if (left) {
                 *reinterpret_cast<float2*>(sA + r0 * kAld + col) = make_float2(v[0], v[1]);
                 *reinterpret_cast<float2*>(sA + (r0 + 8) * kAld + col) = make_float2(v[2], v[3]);
-            } else {
-#pragma unroll
-                for (int e = 0; e < 2; ++e) {
-                    const uint32_t hi = Num<T>::pack(v[2 * e], v[2 * e + 1]);
-                    const float2 f = Num<T>::unpack(hi);
-                    const int o = (r0 + 8 * e) * kTld + col;
-                    *reinterpret_cast<uint32_t*>(M + o) = hi;
-                    *reinterpret_cast<uint32_t*>(M + kCC + o) = Num<T>::pack(v[2 * e] - f.x, v[2 * e + 1] - f.y);
-                }
+            } else if (!Scaled<T>) {
+                put_m(v, r0, col);
             }
+        }
+    }
+    // The largest value of the two warps of a tile; `bar`: theirs
+    auto pair_scale = [&](uint32_t bits, int bar) {
+        if (L.l == 0) sMax[warp] = bits;
+        asm volatile("bar.sync %0, 64;" ::"r"(bar) : "memory");
+        return scale_exp(max(sMax[warp & 2], sMax[warp | 1]));
+    };
+    if constexpr (Scaled<T>) {
+        if (!left) {
+            const int e = pair_scale(max_bits<10>(&x[0][0]), 2);
+            scale_tile<10>(&x[0][0], pow2(e));
+            if (tid == 0) ga[kC + 1] = pow2(-e);
+#pragma unroll
+            for (int i = 0; i < 5; ++i)
+#pragma unroll
+                for (int j = 0; j < 2; ++j)
+                    put_m(x[i][j], 16 * (i < split ? rb0 : rb1) + L.g, 16 * (i < split ? i : i - split) + 8 * j + 2 * L.t);
         }
     }
     if (!left) return;
@@ -520,16 +599,35 @@ __global__ void __launch_bounds__(128) planes_prep_k(const __grid_constant__ DAr
     }
     sync_inverse();
     e16* to = static_cast<e16*>(a.T) + id * 2 * kCC;
-#pragma unroll
-    for (int i = 0; i < 5; ++i) {  // ten blocks of 16 rows by two vectors of 8
+    float ft = 1.f;
+    auto at_block = [&](int i, int& r, int& c8) {  // ten blocks of 16 rows by two vectors of 8
         const int at = i * 64 + u, blk = at >> 5, r16 = (at & 31) >> 1;
         const int rb = blk >= 6 ? 3 : blk >= 3 ? 2 : blk >= 1 ? 1 : 0, cb = blk - rb * (rb + 1) / 2;
-        const int r = 16 * rb + r16, c8 = 16 * cb + (at & 1) * 8;
+        r = 16 * rb + r16;
+        c8 = 16 * cb + (at & 1) * 8;
+    };
+    if constexpr (Scaled<T>) {
+        float m = 0.f;
+#pragma unroll
+        for (int i = 0; i < 5; ++i) {
+            int r, c8;
+            at_block(i, r, c8);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) m = fmaxf(m, fabsf(sT[r * kAld + c8 + e]));
+        }
+        const int e = pair_scale(__reduce_max_sync(0xffffffffu, abs_bits(m)), 1);
+        ft = pow2(e);
+        if (u == 0) ga[kC] = pow2(-e);
+    }
+#pragma unroll
+    for (int i = 0; i < 5; ++i) {
+        int r, c8;
+        at_block(i, r, c8);
         uint32_t hi[4], lo[4];
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
             const float2 v = *reinterpret_cast<const float2*>(sT + r * kAld + c8 + 2 * e);
-            const float2 w = *reinterpret_cast<const float2*>(sB + c8 + 2 * e);
+            const float2 w = Scaled<T> ? make_float2(ft, ft) : *reinterpret_cast<const float2*>(sB + c8 + 2 * e);
             const float p = v.x * w.x, q = v.y * w.y;
             hi[e] = Num<T>::pack(p, q);
             const float2 f = Num<T>::unpack(hi[e]);
@@ -559,7 +657,8 @@ struct Fwd {
     static constexpr int kGroups = kStage + kLoad, kKeep = kGroups + G * kGroup;  // where U's planes are stored from
     static constexpr int kStages = G < 4 ? G : 1;  // of U's planes, to be stored from
     static constexpr int kBars = kKeep + kStages * 4 * 16 * kTld;
-    static constexpr size_t bytes = 1024 + kBars + 8 * (5 + 4 * G);
+    static constexpr int kExp = kBars + 8 * (5 + 4 * G);  // (float16) the exponent of each group's S
+    static constexpr size_t bytes = 1024 + kExp + 4 * G;
 };
 
 // S^T (16 value rows v0.., K columns) of a (K, V) float32 state
@@ -671,6 +770,7 @@ __global__ void __launch_bounds__(Fwd<KD, G>::kWarps * 32) planes_chain_k(const 
     uint64_t* empty = full + 2;
     uint64_t* land = empty + 2;
     uint64_t *s_full = land + 1, *s_empty = s_full + G, *u_full = s_empty + G, *u_empty = u_full + G;
+    int* s_exp = reinterpret_cast<int*>(smem + Sm::kExp);
     const int64_t head = static_cast<int64_t>(b) * a.Hv + h;
     if (threadIdx.x == 0) {
         for (int s = 0; s < 2; ++s) {
@@ -744,6 +844,7 @@ __global__ void __launch_bounds__(Fwd<KD, G>::kWarps * 32) planes_chain_k(const 
         float4* sU = reinterpret_cast<float4*>(mine + Sm::kU);
         float S[KD / 8][4];
         state_load<KD>(S, a.initial ? a.initial + head * a.K * a.V : nullptr, a.K, a.V, v0, L);
+        int se = 0;  // (float16) S holds 2^se times the state
         for (int c = 0; c < nc && ok; ++c) {
             const unsigned char* st = smem + (c & 1) * Sm::kStage;
             const e16* e = reinterpret_cast<const e16*>(st);
@@ -755,6 +856,19 @@ __global__ void __launch_bounds__(Fwd<KD, G>::kWarps * 32) planes_chain_k(const 
                 ok = warp_wait(&full[c & 1], (c >> 1) & 1);
             } else {
                 ok = warp_wait2(&full[c & 1], (c >> 1) & 1, &s_empty[warp], (c & 1) ^ 1);
+                float s_max = 0.f;
+                auto scale_state = [&](float largest) {  // by the largest value of S and of what is added to it
+                    const int e = max(-kMaxExp, min(kMaxExp, se + scale_exp(__float_as_uint(largest)))) - se;
+                    if (e == 0) return 1.f;
+                    scale_tile<KD / 8>(S, pow2(e));
+                    se += e;
+                    return pow2(e);
+                };
+                if constexpr (Scaled<T>) {
+                    s_max = __uint_as_float(max_bits<KD / 8>(S));
+                    s_max *= scale_state(s_max);
+                    if (L.l == 0) s_exp[warp] = se;
+                }
                 // (K S0)^T, S in two planes; the next 16 columns of S are split between the products
                 float X[kC / 8][4] = {};
                 {
@@ -787,7 +901,11 @@ __global__ void __launch_bounds__(Fwd<KD, G>::kWarps * 32) planes_chain_k(const 
                     ld_at32(r, es + Sm::kV + warp * kC * 16, 16 * p);
 #pragma unroll
                     for (int i = 0; i < 2; ++i) {
-                        const float2 f = *reinterpret_cast<const float2*>(gam + 16 * p + 8 * i + 2 * L.t);
+                        float2 f = *reinterpret_cast<const float2*>(gam + 16 * p + 8 * i + 2 * L.t);
+                        if constexpr (Scaled<T>) {
+                            f.x *= pow2(-se);
+                            f.y *= pow2(-se);
+                        }
                         float* x = X[2 * p + i];
                         const float2 lo = Num<T>::unpack(r[2 * i]), hi = Num<T>::unpack(r[2 * i + 1]);
                         x[0] = fmaf(-f.x, x[0], lo.x);
@@ -797,11 +915,21 @@ __global__ void __launch_bounds__(Fwd<KD, G>::kWarps * 32) planes_chain_k(const 
                     }
                 }
                 // U^T = X T'^T, both in two planes; between the products S is scaled, and the first
-                // 16 tokens of U, which are done after theirs, are split for the update
+                // 16 tokens of U, which are done after theirs, are split for the update (float16: when
+                // all of U is known)
+                int xe = 0;
+                if constexpr (Scaled<T>) {
+                    xe = scale_exp(max_bits<kC / 8>(X));
+                    if (xe != 0) scale_tile<kC / 8>(X, pow2(xe));
+                }
                 float U[kC / 8][4] = {};
                 const float gc = gam[kC - 1];
                 auto decayed = [&](Af<2>& to, int kk, int q) {
-                    const float2 d = *reinterpret_cast<const float2*>(dec + 16 * kk + 8 * (q / 2) + 2 * L.t);
+                    float2 d = *reinterpret_cast<const float2*>(dec + 16 * kk + 8 * (q / 2) + 2 * L.t);
+                    if constexpr (Scaled<T>) {
+                        d.x *= pow2(se);
+                        d.y *= pow2(se);
+                    }
                     const float* u = U[2 * kk + q / 2];
                     from_acc_part<T>(to, q, u[2 * (q & 1)] * d.x, u[2 * (q & 1) + 1] * d.y);
                 };
@@ -828,11 +956,28 @@ __global__ void __launch_bounds__(Fwd<KD, G>::kWarps * 32) planes_chain_k(const 
                                     const float* x = X[2 * kk + 2 + q / 2];
                                     from_acc_part<T>(ax[(kk + 1) & 1], q, x[2 * (q & 1)], x[2 * (q & 1) + 1]);
                                 }
-                                if (i == 4) decayed(ud[0], 0, q);
+                                if (!Scaled<T> && i == 4) decayed(ud[0], 0, q);
                             };
                             if (i & 1) mma_step_with<T>(U, af, f, side, kk);
                             else mma_step_with<T>(U, high(af), f, side, kk);
                         });
+                }
+                if constexpr (Scaled<T>) {  // beta, which T' was made without
+                    float u_max = 0.f;
+#pragma unroll
+                    for (int j = 0; j < kC / 8; ++j) {
+                        const float2 r = *reinterpret_cast<const float2*>(ga + 8 * j + 2 * L.t);
+                        const float2 d = *reinterpret_cast<const float2*>(dec + 8 * j + 2 * L.t);
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            U[j][i] = U[j][i] * pow2(-xe) * ((i & 1 ? r.y : r.x) * ga[kC]);
+                            u_max = fmaxf(u_max, fabsf(U[j][i] * (i & 1 ? d.y : d.x)));
+                        }
+                    }
+                    u_max = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(u_max)));
+                    scale_state(fmaxf(s_max * gc, u_max * pow2(se)));
+#pragma unroll
+                    for (int q = 0; q < 4; ++q) decayed(ud[0], 0, q);
                 }
                 ok = warp_wait_asked(u_free, &u_empty[warp], (c & 1) ^ 1) && ok;
                 frag_put(sU, U, L);
@@ -855,6 +1000,7 @@ __global__ void __launch_bounds__(Fwd<KD, G>::kWarps * 32) planes_chain_k(const 
             }
             warp_arrive(&empty[c & 1]);
         }
+        if constexpr (Scaled<T>) scale_tile<KD / 8>(S, pow2(-se));
         if (on && a.final_state && ok) state_store<KD>(S, a.final_state + head * a.K * a.V, a.K, a.V, v0, L);
         return;
     }
@@ -890,10 +1036,15 @@ __global__ void __launch_bounds__(Fwd<KD, G>::kWarps * 32) planes_chain_k(const 
                     for (int p = 0; p < 4; ++p) ld_b128<false>(f[p], es + Sm::kQ, 16 * p, 16 * k);
                 },
                 [&](int k, const uint32_t(*f)[4]) { mma_step<T>(O, as[k & 1], f); });
+            const float unit = Scaled<T> ? pow2(-s_exp[g]) : 1.f;
             warp_arrive(&s_empty[g]);
 #pragma unroll
             for (int j = 0; j < kC / 8; ++j) {
-                const float2 f = *reinterpret_cast<const float2*>(sgam + 8 * j + 2 * L.t);
+                float2 f = *reinterpret_cast<const float2*>(sgam + 8 * j + 2 * L.t);
+                if constexpr (Scaled<T>) {
+                    f.x *= unit;
+                    f.y *= unit;
+                }
                 sO[j * 32 + L.l] = make_float4(O[j][0] * f.x, O[j][1] * f.y, O[j][2] * f.x, O[j][3] * f.y);
             }
         }
@@ -908,6 +1059,14 @@ __global__ void __launch_bounds__(Fwd<KD, G>::kWarps * 32) planes_chain_k(const 
             ok = warp_wait(&u_full[g], c & 1) && ok;
             frag_get(U, reinterpret_cast<const float4*>(theirs + Sm::kU), L);
             warp_arrive(&u_empty[g]);
+            // float16: M U by itself, as U and M are scaled
+            float Y[Scaled<T> ? kC / 8 : 1][4] = {};
+            int ue = 0;
+            if constexpr (Scaled<T>) {
+                ue = scale_exp(max_bits<kC / 8>(U));
+                scale_tile<kC / 8>(U, pow2(ue));
+            }
+            auto& sums = *[&]() { if constexpr (Scaled<T>) return &Y; else return &O; }();
             Af<2> au;
             steps<8>(
                 [&](int k, uint32_t(*f)[4]) {
@@ -917,12 +1076,19 @@ __global__ void __launch_bounds__(Fwd<KD, G>::kWarps * 32) planes_chain_k(const 
                 },
                 [&](int k, const uint32_t(*f)[4]) {
                     if (k & 1) {
-                        mma_step<T>(O, au, f, k / 2);
+                        mma_step<T>(sums, au, f, k / 2);
                     } else {
                         au = from_acc<T, 2>(U[k], U[k + 1]);
-                        mma_step<T>(O, high(au), f, k / 2);
+                        mma_step<T>(sums, high(au), f, k / 2);
                     }
                 });
+            if constexpr (Scaled<T>) {
+                const float fm = reinterpret_cast<const float*>(e + Sm::kGa)[kC + 1];
+#pragma unroll
+                for (int j = 0; j < kC / 8; ++j)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) O[j][i] = fmaf(Y[j][i] * pow2(-ue), fm, O[j][i]);
+            }
             // rows of 16 values through shared memory: 32 bytes a token, two lanes each
             __syncwarp();
 #pragma unroll
@@ -1786,7 +1952,10 @@ int chain_groups(const DArgs& a, bool reverse) {
 
 template <typename T, int KD, int G>
 cudaError_t chain_launch(const DArgs& a, const Maps& m, cudaStream_t s) {
-    const auto k = a.S ? planes_chain_k<T, KD, G, true> : planes_chain_k<T, KD, G, false>;
+    auto k = planes_chain_k<T, KD, G, false>;
+    if constexpr (!Scaled<T>) {
+        if (a.S) k = planes_chain_k<T, KD, G, true>;
+    }
     PLANES_TRY(smem_limit(k, Fwd<KD, G>::bytes));
     k<<<dim3((a.Vp / 16 + G - 1) / G, a.Hv, a.B), Fwd<KD, G>::kWarps * 32, Fwd<KD, G>::bytes, s>>>(a, m);
     note_launch();
@@ -1803,7 +1972,9 @@ cudaError_t rchain_launch(const DArgs& a, const Maps& m, cudaStream_t s) {
 template <typename T, int KD>
 cudaError_t chain(const DArgs& a, const Maps& m, bool reverse, cudaStream_t s) {
     const int g = chain_groups(a, reverse);
-    if (reverse) return g == 2 ? rchain_launch<T, KD, 2>(a, m, s) : rchain_launch<T, KD, 3>(a, m, s);
+    if constexpr (!Scaled<T>) {
+        if (reverse) return g == 2 ? rchain_launch<T, KD, 2>(a, m, s) : rchain_launch<T, KD, 3>(a, m, s);
+    }
     return g == 2 ? chain_launch<T, KD, 2>(a, m, s) : g == 3 ? chain_launch<T, KD, 3>(a, m, s) : chain_launch<T, KD, 4>(a, m, s);
 }
 
@@ -1900,7 +2071,6 @@ cudaError_t planes_bwd(DArgs a, void* saved, void* ws, float* group, cudaStream_
     char* w = static_cast<char*>(ws);
     a.dS = w;
     a.dV = w + state_bytes(a);
-    if (a.half) return a.K <= 64 ? bwd<__half, 64>(a, group, s) : bwd<__half, 128>(a, group, s);
     return a.K <= 64 ? bwd<__nv_bfloat16, 64>(a, group, s) : bwd<__nv_bfloat16, 128>(a, group, s);
 }
 

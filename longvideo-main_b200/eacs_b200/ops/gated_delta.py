@@ -17,8 +17,10 @@ h // (Hv // Hk).  Views are taken with their strides (a slice of a fused
 projection needs no copy) as long as their last dimension is dense; 16-bit
 ones are fastest when their rows start on 16 bytes (K, V and all strides
 multiples of 8).  Sums and states are float32.  Operands of the products keep
-22 significant bits, 16 for bfloat16 inputs.  With float16 inputs states have
-to stay within float16's range.  The same inputs give the same bits.
+22 significant bits, 16 for bfloat16 inputs; float16 ones may be of any size
+that float32 holds.  float16 training runs on the kernels of float32, at a
+fifth of bfloat16's speed.  The same inputs give the same bits (float16: with
+gradients, or without).
 
 A backward that is captured into a graph must not share leaves with an eager
 graph that is still alive (autograd's own rule).

@@ -524,3 +524,56 @@ def test_nan_and_infinity_of_a_token_reach_what_follows(dtype, pad, bad):
     assert bool(torch.isfinite(o0).all() and torch.isfinite(S0).all())
     assert torch.equal(o0[:, :64], o1[:, :64])
     assert not bool(torch.isfinite(o1[:, 128:]).any()) and not bool(torch.isfinite(S1).any())
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("size", [1e-6, 1e-3, 1.0, 1e4, 1e6])
+@pytest.mark.parametrize("K", [64, 128])
+def test_small_rates_and_gradients_of_any_size(dtype, size, K):
+    """Rates of 0, 1e-7 and 1e-4 among others, upstream gradients from 1e-6 to beyond float16's range (the final state's,
+    in float32; the outputs' as far as their type goes).  A 16-bit gradient that is not a normal number of its type is off by half a
+    step of the smallest (2^-25 in float16); one beyond its range is infinite.  Of a token whose rate is small, dbeta is
+    the product of two vectors of V values that are off by TOL of their norms: by 2 TOL |a| |b|, which is 2 TOL sqrt(V) of
+    the norm of the products' sums, as the vectors have nothing to do with each other."""
+    B, L, V = 1, 140, 64
+    d, do, dS = make(B, L, 1, 2, K, V, dtype, torch.float32, seed=40)
+    rates = {10: 0.0, 11: 0.0, 12: 1e-7, 13: 1e-4, 63: 0.0, 64: 1e-7, 90: 1e-4, 139: 0.0}
+    for t, x in rates.items():
+        d["beta"][0, t] = x
+    do = (do.float() * min(size, 1e4)).to(dtype)
+    got, want = both(d, do, dS * size)
+    step = 2.0 ** -25 if dtype == torch.float16 else 0.0
+    for n in want:
+        a, w = got[n].double().cpu(), want[n]
+        if got[n].dtype == torch.float16:
+            inside = w.abs() < torch.finfo(torch.float16).max
+            assert not bool(torch.isnan(a).any()), n
+            a, w = torch.where(inside, a, 0.0), torch.where(inside, w, 0.0)
+        assert bool(torch.isfinite(a).all()), n
+        err = float((a - w).norm())
+        assert err <= tol(got[n].dtype, dtype) * float(w.norm()) + step * a.numel() ** 0.5, (n, err / float(w.norm()))
+    at = sorted(rates)
+    a, w = got["dbeta"][0, at].double().cpu(), want["dbeta"][0, at]
+    assert float((a - w).norm()) <= 2 * TOL * V ** 0.5 * float(w.norm()), (a, w)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("shape", [(2, 200, 1, 2, 64, 40), (1, 150, 2, 2, 128, 128), (1, 130, 16, 64, 128, 104)])
+@pytest.mark.parametrize("rate,value,state,scale", [
+    (1.0, 1.0, 1.0, 1.0), (1e-4, 1.0, 0.0, 1.0), (0.0, 1.0, 1e-3, 1e3), (1.0, 1e-3, 1e-3, 1e2), (1.0, 1.0, 1e6, 1e-6), (1e-20, 1.0, 0.0, 1e20),
+    (1.0, 2e4, 1e9, 1e-9), (1e-30, 1.0, 1e-30, 1e30)])
+def test_forward_without_gradients_of_any_size(dtype, shape, rate, value, state, scale):
+    """Rates, values and states of very different sizes, with scales that bring the outputs near 1: the final state, which is
+    float32, keeps TOL of every head's norm."""
+    d, _, _ = make(*shape, dtype, torch.float32, seed=46)
+    d["beta"] *= rate
+    d["v"] = (d["v"].float() * value).clamp(-6e4, 6e4).to(dtype)  # (finite in float16)
+    d["initial"] *= state
+    x = [d[n] for n in ("q", "k", "v", "g", "beta")]
+    o, S = gated_delta_rule(*x, scale=scale, initial_state=d["initial"], output_final_state=True)
+    want, S64 = oracle(*(t.double().cpu() for t in x), scale, d["initial"].double().cpu())
+    assert bool(torch.isfinite(o).all()) and bool(torch.isfinite(S).all())
+    err, ref = (S.double().cpu() - S64).norm(dim=(2, 3)), S64.norm(dim=(2, 3))
+    assert bool((err <= TOL * ref).all()), float((err / ref).max())
+    err, ref = float((o.double().cpu() - want).norm()), float(want.norm())
+    assert err <= tol(dtype) * ref + (2.0 ** -25 * o.numel() ** 0.5 if dtype == torch.float16 else 0.0), err / ref
