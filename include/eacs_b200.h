@@ -115,9 +115,13 @@ EACS_API size_t eacs_layer_norm_bwd_workspace_size(int64_t rows, int64_t d);
  * V to 1024.  Rows of q, k, v that start on 16 bytes, with K and V multiples
  * of 8, are read 16 bytes at a time; 16-bit inputs of that kind (no dimension
  * of more than one element having stride 0) take the fastest kernels, bfloat16
- * always, float16 where no backward follows.  Which kernels run goes by the
- * pointers' alignment and the strides, and so do the workspace sizes: ask for
- * them with the arguments of the call. */
+ * always, float16 where no backward follows.  Which kernels run (`path` 0)
+ * goes by the pointers' alignment and the strides, and so do the workspace
+ * sizes and what a workspace holds: ask for the sizes with the arguments of the
+ * call.  A backward whose inputs may have moved since the forward names the
+ * forward's path. */
+#define EACS_DELTA_PATH_GENERAL 1 /* any inputs */
+#define EACS_DELTA_PATH_16 2      /* the 16-bit kernels; refused for inputs that they do not take */
 typedef struct EacsDelta {
     const void* q;
     const void* k;
@@ -135,7 +139,11 @@ typedef struct EacsDelta {
     float scale;
     int32_t dtype;
     int32_t gate_dtype;
+    int32_t path;
 } EacsDelta;
+
+/* The path that a forward with these arguments takes, or 0 if they are refused. */
+EACS_API int eacs_delta_path(const EacsDelta* p, int training);
 
 /* Chunked forward: o (B,L,Hv,V) dense of dtype, on 16 bytes; final_state (B,Hv,K,V)
  * float32 or NULL.  With training != 0 the workspace holds what

@@ -1156,7 +1156,7 @@ int64_t key_pad(int64_t K) { return K <= 64 ? 64 : 128; }
 size_t align256(size_t x) { return (x + 255) / 256 * 256; }
 
 // EACS_OK, or the error that these sizes and types are refused with
-int check_delta(const EacsDelta& p, const char* fn) {
+int check_sizes(const EacsDelta& p, const char* fn) {
     if (p.B < 0 || p.L < 0 || p.Hk <= 0 || p.Hv <= 0 || p.K <= 0 || p.V <= 0)
         return fail(EACS_ERR_INVALID, "%s: bad sizes", fn);
     if (p.Hv % p.Hk != 0)
@@ -1213,12 +1213,24 @@ bool mapped(int64_t B, int64_t L, int64_t H, const int64_t* st) {
 // Whether the 16-bit kernels take these inputs: bfloat16, and float16 where no
 // backward follows.  float16's exponent is too short for what a backward keeps
 // and divides (a rate of 1e-4 left 8 bits of dbeta, one of 0 none), so its
-// training runs in tf32.  The backward goes by the forward's inputs alone, as it
-// reads what the forward left (an upstream gradient in another layout is
+// training runs in tf32.  The backward goes by the forward's path, or by its inputs
+// alone, as it reads what the forward left (an upstream gradient in another layout is
 // refused by delta_bwd then).
-bool planes(const EacsDelta& p, const DArgs& a, bool training) {
+bool planes_take(const EacsDelta& p, const DArgs& a, bool training) {
     return (p.dtype == EACS_DTYPE_BF16 || (p.dtype == EACS_DTYPE_F16 && !training)) && a.vec_qk && a.vec_v &&
            mapped(p.B, p.L, p.Hk, p.q_stride) && mapped(p.B, p.L, p.Hk, p.k_stride) && mapped(p.B, p.L, p.Hv, p.v_stride);
+}
+// The path of a call: the caller's, or the one that its inputs lead to.
+bool planes(const EacsDelta& p, const DArgs& a, bool training) {
+    return p.path == 0 ? planes_take(p, a, training) : p.path == EACS_DELTA_PATH_16;
+}
+
+int check_delta(const EacsDelta& p, const char* fn, bool training) {
+    if (int rc = check_sizes(p, fn)) return rc;
+    if (p.path < 0 || p.path > EACS_DELTA_PATH_16) return fail(EACS_ERR_INVALID, "%s: unknown path %d", fn, p.path);
+    if (p.path == EACS_DELTA_PATH_16 && !planes_take(p, make_args(p), training))
+        return fail(EACS_ERR_INVALID, "%s: the 16-bit kernels do not take these inputs", fn);
+    return EACS_OK;
 }
 
 struct Sizes { size_t gates, T, M, S, U, total; };
@@ -1272,19 +1284,23 @@ bool on16(std::initializer_list<const void*> ps) {
 
 }  // namespace
 
+int delta_path(const EacsDelta& p, bool training) {
+    if (check_delta(p, "eacs_delta_path", training) != EACS_OK) return 0;
+    return planes(p, make_args(p), training) ? EACS_DELTA_PATH_16 : EACS_DELTA_PATH_GENERAL;
+}
 size_t delta_workspace_size(const EacsDelta& p, bool training) {
-    if (check_delta(p, "eacs_delta_workspace_size") != EACS_OK) return 0;
+    if (check_delta(p, "eacs_delta_workspace_size", training) != EACS_OK) return 0;
     return fwd_sizes(p, make_args(p), training).total;
 }
 size_t delta_bwd_workspace_size(const EacsDelta& p) {
-    if (check_delta(p, "eacs_delta_bwd_workspace_size") != EACS_OK) return 0;
+    if (check_delta(p, "eacs_delta_bwd_workspace_size", true) != EACS_OK) return 0;
     return bwd_sizes(p, make_args(p)).total;
 }
 
 int delta_fwd(const EacsDelta& p, void* o, float* final_state, void* ws, size_t ws_bytes, bool training,
               cudaStream_t stream) {
     const char* fn = "eacs_delta_fwd";
-    if (int rc = check_delta(p, fn)) return rc;
+    if (int rc = check_delta(p, fn, training)) return rc;
     const size_t state = static_cast<size_t>(p.B) * p.Hv * p.K * p.V * sizeof(float);
     if (p.B == 0) return EACS_OK;
     if (p.L == 0) {  // no token: the state stays
@@ -1317,7 +1333,7 @@ int delta_fwd(const EacsDelta& p, void* o, float* final_state, void* ws, size_t 
 
 int delta_step(const EacsDelta& p, void* o, float* final_state, cudaStream_t stream) {
     const char* fn = "eacs_delta_step";
-    if (int rc = check_delta(p, fn)) return rc;
+    if (int rc = check_sizes(p, fn)) return rc;
     if (p.B == 0) return EACS_OK;
     if ((!inputs_set(p) || !o) && p.L > 0) return fail(EACS_ERR_INVALID, "%s: null pointer argument", fn);
     DArgs a = make_args(p);
@@ -1333,7 +1349,7 @@ int delta_step(const EacsDelta& p, void* o, float* final_state, cudaStream_t str
 int delta_bwd(const EacsDelta& p, const DeltaGrads& d, const void* saved, size_t saved_bytes, void* ws, size_t ws_bytes,
               cudaStream_t stream) {
     const char* fn = "eacs_delta_bwd";
-    if (int rc = check_delta(p, fn)) return rc;
+    if (int rc = check_delta(p, fn, true)) return rc;
     const size_t state = static_cast<size_t>(p.B) * p.Hv * p.K * p.V * sizeof(float);
     if (p.B == 0) return EACS_OK;
     if (p.L == 0) {

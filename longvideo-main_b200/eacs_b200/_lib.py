@@ -37,6 +37,7 @@ _SZ = ctypes.c_size_t
 # (Packed in one call: a ctypes.Structure filled field by field takes as long as
 # a short launch.)
 DELTA = struct.Struct("=5Q15q2Q6qf2i4x")
+DELTA_PATH = struct.Struct("=5Q15q2Q6qf3i")  # with the path of the kernels named
 
 
 # name -> (restype, argtypes); mirrors include/eacs_b200.h
@@ -54,6 +55,7 @@ SIGNATURES = {
                                  _I64, _I64, _P]),
     "eacs_layer_norm_bwd_workspace_size": (_SZ, [_I64, _I64]),
     "eacs_delta_fwd": (_I, [_P, _P, _P, _P, _SZ, _I, _P]),
+    "eacs_delta_path": (_I, [_P, _I]),
     "eacs_delta_workspace_size": (_SZ, [_P, _I]),
     "eacs_delta_bwd": (_I, [_P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _SZ, _P, _SZ, _P]),
     "eacs_delta_bwd_workspace_size": (_SZ, [_P]),

@@ -72,7 +72,7 @@ def _check(name, q, k, v, g, beta, lengths, state, lead):
     return dev
 
 
-def _args(q, k, v, g, beta, scale, lengths, state) -> bytes:
+def _args(q, k, v, g, beta, scale, lengths, state, path=0) -> bytes:
     """EacsDelta of a sequence (B, L, H, D), or of one token a row (B, H, D)."""
     qs, vs = q.shape, v.shape
     if len(qs) == 4:
@@ -84,14 +84,14 @@ def _args(q, k, v, g, beta, scale, lengths, state) -> bytes:
         for t in (q, k, v, g, beta):
             s = t.stride()
             st += (s[0], 0, s[1])
-    return _lib.DELTA.pack(q.data_ptr(), k.data_ptr(), v.data_ptr(), g.data_ptr(), beta.data_ptr(), *st,
-                           0 if lengths is None else lengths.data_ptr(), 0 if state is None else state.data_ptr(),
-                           qs[0], L, qs[-2], vs[-2], qs[-1], vs[-1], scale, _lib.DTYPE_CODES[q.dtype],
-                           _lib.DTYPE_CODES[g.dtype])
+    return _lib.DELTA_PATH.pack(q.data_ptr(), k.data_ptr(), v.data_ptr(), g.data_ptr(), beta.data_ptr(), *st,
+                                0 if lengths is None else lengths.data_ptr(), 0 if state is None else state.data_ptr(),
+                                qs[0], L, qs[-2], vs[-2], qs[-1], vs[-1], scale, _lib.DTYPE_CODES[q.dtype],
+                                _lib.DTYPE_CODES[g.dtype], path)
 
 
 def _forward(args, out_state, training, dev):
-    """(o, final state or None, workspace) of (q, k, v, g, beta, scale, lengths, initial)."""
+    """(o, final state or None, workspace, its path) of (q, k, v, g, beta, scale, lengths, initial)."""
     q, k, v = args[:3]
     p = _args(*args)
     L_ = _lib.lib()
@@ -101,13 +101,14 @@ def _forward(args, out_state, training, dev):
     with on(dev):
         _lib.check(L_.eacs_delta_fwd(p, o.data_ptr(), _lib.ptr(final), ws.data_ptr(), ws.numel(),
                                      int(training), _lib.raw_stream(dev.index)), "eacs_delta_fwd")
-    return o, final, ws
+    return o, final, ws, L_.eacs_delta_path(p, 1) if training else 0
 
 
 class GatedDeltaFunction(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, g, beta, scale, lengths, initial, out_state, dev):
-        o, final, ws = _forward((q, k, v, g, beta, scale, lengths, initial), out_state, True, dev)
+        # what ws holds goes by where the inputs lie; hooks may give them back elsewhere
+        o, final, ws, ctx.path = _forward((q, k, v, g, beta, scale, lengths, initial), out_state, True, dev)
         ctx.save_for_backward(q, k, v, g, beta, lengths, initial, ws)
         ctx.scale, ctx.dev = scale, dev
         ctx.set_materialize_grads(False)
@@ -124,11 +125,18 @@ class GatedDeltaFunction(torch.autograd.Function):
         if do.data_ptr() % 16:  # a view that starts inside an allocation
             do = do.clone()
         dfinal = None if dfinal is None else dfinal.contiguous()
-        p = _args(q, k, v, g, beta, ctx.scale, lengths, initial)
+        q, k, v = _dense_last(q), _dense_last(k), _dense_last(v)
+        lengths, initial = (None if t is None else t.contiguous() for t in (lengths, initial))
         L_ = _lib.lib()
+        p = _args(q, k, v, g, beta, ctx.scale, lengths, initial, ctx.path)
+        need = int(L_.eacs_delta_bwd_workspace_size(p))
+        if need == 0 and do.numel():  # not as the path wants them
+            q, k, v = (t.clone(memory_format=torch.contiguous_format) for t in (q, k, v))
+            p = _args(q, k, v, g, beta, ctx.scale, lengths, initial, ctx.path)
+            need = int(L_.eacs_delta_bwd_workspace_size(p))
         dq, dk, dv, dg, db = (torch.empty(t.shape, dtype=t.dtype, device=dev) for t in (q, k, v, g, beta))
         di = torch.empty(initial.shape, dtype=torch.float32, device=dev) if ctx.needs_input_grad[7] else None
-        w2 = torch.empty(int(L_.eacs_delta_bwd_workspace_size(p)), dtype=torch.uint8, device=dev)
+        w2 = torch.empty(need, dtype=torch.uint8, device=dev)
         with on(dev):
             _lib.check(L_.eacs_delta_bwd(
                 p, do.data_ptr(), (ctypes.c_int64 * 3)(*do.stride()[:3]), _lib.ptr(dfinal), dq.data_ptr(),
@@ -154,7 +162,7 @@ def gated_delta_rule(q: Tensor, k: Tensor, v: Tensor, g: Tensor, beta: Tensor, s
     state = None if initial_state is None else initial_state.contiguous()
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (q, k, v, g, beta, state)):
         return GatedDeltaFunction.apply(q, k, v, g, beta, scale, lengths, state, output_final_state, dev)
-    o, final, _ = _forward((q, k, v, g, beta, scale, lengths, state), output_final_state, False, dev)
+    o, final, _, _ = _forward((q, k, v, g, beta, scale, lengths, state), output_final_state, False, dev)
     return (o, final) if output_final_state else o
 
 

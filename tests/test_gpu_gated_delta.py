@@ -577,3 +577,34 @@ def test_forward_without_gradients_of_any_size(dtype, shape, rate, value, state,
     assert bool((err <= TOL * ref).all()), float((err / ref).max())
     err, ref = float((o.double().cpu() - want).norm()), float(want.norm())
     assert err <= tol(dtype) * ref + (2.0 ** -25 * o.numel() ** 0.5 if dtype == torch.float16 else 0.0), err / ref
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("how", ["off a boundary", "expanded", "aligned"])
+def test_saved_tensors_that_come_back_in_another_layout(dtype, how):
+    """Hooks that move what is saved give dense, aligned copies (or ones that are neither); the backward reads what the
+    forward left all the same."""
+    B, L, H, K, V = 2, 100, 2, 64, 64
+    d, do, dS = make(B, L, H, H, K, V, dtype, seed=41)
+
+    def run():
+        leaves = {n: t.detach().clone().requires_grad_(True) for n, t in d.items()}
+        x = dict(leaves)
+        if how == "off a boundary":
+            x["v"] = torch.nn.functional.pad(leaves["v"], (3, 5))[..., 3:3 + V]
+        if how == "expanded":
+            leaves["k"] = d["k"][:, :, :1].detach().clone().requires_grad_(True)
+            x["k"] = leaves["k"].expand(B, L, H, K)
+        o, S = gated_delta_rule(*(x[n] for n in ("q", "k", "v", "g", "beta")), initial_state=x["initial"], output_final_state=True)
+        return o, S, list(leaves.values())
+
+    def odd(t):  # one element off its old alignment
+        flat = torch.empty(t.numel() + 1, dtype=t.dtype, device=t.device)[1:]
+        return flat.copy_(t.reshape(-1)).view(t.shape) if t.dtype == dtype else t
+    o, S, leaves = run()
+    want = torch.autograd.grad([o, S], leaves, [do, dS])
+    for hooks in (torch.autograd.graph.save_on_cpu(), torch.autograd.graph.saved_tensors_hooks(odd, lambda t: t)):
+        with hooks:
+            o, S, leaves = run()
+        for a, b in zip(torch.autograd.grad([o, S], leaves, [do, dS]), want):
+            assert torch.equal(a, b)
