@@ -5,6 +5,7 @@ from __future__ import annotations
 import contextlib
 
 import torch
+from torch.autograd import forward_ad
 
 
 def require(cond: bool, msg: str) -> None:
@@ -26,6 +27,24 @@ def cuda_tensors(name: str, *ts: torch.Tensor) -> torch.device:
 def on(dev: torch.device):
     """torch.cuda.device(dev) where dev is not the current device, else nothing."""
     return contextlib.nullcontext() if torch.cuda.current_device() == dev.index else torch.cuda.device(dev)
+
+
+def is_plain(*ts: torch.Tensor | None) -> bool:
+    """Whether these are tensors whose values alone are asked for: none has a
+    forward-mode tangent, none belongs to a torch.func transform, and nothing
+    is being traced.  Kernels called by pointer see the values only; what would
+    have to be carried along or recorded would be lost."""
+    if forward_ad._current_level >= 0 and any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in ts):
+        return False
+    if torch.compiler.is_compiling():  # (whose graph ends where the kernel is called)
+        return True
+    return not torch.jit.is_tracing() and torch._C._functorch.peek_interpreter_stack() is None
+
+
+def require_plain(name: str, *ts: torch.Tensor | None) -> None:
+    if not is_plain(*ts):
+        raise RuntimeError(f"{name}: has no forward-mode derivative and runs under no torch.func transform "
+                           "or torch.jit.trace")
 
 
 def one_device(name: str, first: torch.Tensor, *ts: torch.Tensor | None) -> torch.device:

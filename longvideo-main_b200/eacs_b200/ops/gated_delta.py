@@ -22,8 +22,9 @@ that float32 holds.  float16 training runs on the kernels of float32, at a
 fifth of bfloat16's speed.  The same inputs give the same bits (float16: with
 gradients, or without).
 
-A backward that is captured into a graph must not share leaves with an eager
-graph that is still alive (autograd's own rule).
+Gradients are reverse mode, once; forward-mode, torch.func or traced calls are
+refused.  A backward that is captured into a graph must not share
+leaves with an eager graph that is still alive (autograd's own rule).
 """
 from __future__ import annotations
 
@@ -33,7 +34,7 @@ import torch
 from torch import Tensor
 
 from .. import _lib
-from ._check import on, one_device
+from ._check import on, one_device, require_plain
 
 MAX_K = 128
 MAX_V = 1024
@@ -48,6 +49,7 @@ def _dense_last(t: Tensor) -> Tensor:
 def _check(name, q, k, v, g, beta, lengths, state, lead):
     """Device of the arguments; lead: the dimensions in front of the head's."""
     dev = one_device(name, q, k, v, g, beta, lengths, state)
+    require_plain(name, q, k, v, g, beta, state)
     qs, vs, dt = q.shape, v.shape, q.dtype
     if len(qs) != lead + 2 or k.shape != qs:
         raise RuntimeError(f"{name}: q and k must have one shape of {lead + 2} dimensions")

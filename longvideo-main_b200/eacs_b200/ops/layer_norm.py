@@ -20,7 +20,7 @@ import torch
 from torch import Tensor, nn
 
 from .. import _lib
-from ._check import on, one_device
+from ._check import is_plain, on, one_device, require_plain
 
 MAX_D = 8192
 
@@ -94,8 +94,10 @@ def layer_norm(x: Tensor, weight: Tensor | None = None, bias: Tensor | None = No
     """LayerNorm of x (+ residual) over the last dimension, in x's dtype.
 
     x (..., d) float32 / float16 / bfloat16, d up to 8192; residual like x;
-    weight and bias (d), both of one of those dtypes, or None."""
+    weight and bias (d), both of one of those dtypes, or None.  Gradients are
+    reverse mode only, and forward-mode or traced inputs are refused."""
     dev = one_device("layer_norm", x, residual, weight, bias)
+    require_plain("layer_norm", x, residual, weight, bias)
     dt = x.dtype
     if x.dim() < 1 or dt not in _lib.DTYPE_CODES:
         raise RuntimeError(f"layer_norm: unsupported x, {dt} of {x.dim()} dimensions")
@@ -127,11 +129,12 @@ class LayerNorm(nn.LayerNorm):
     In a float16 / bfloat16 autocast region the input is taken to float32
     first, as autocast runs layer norms.  CPU tensors and what `layer_norm`
     does not take (float64, several normalised dimensions, more than 8192
-    features) keep torch's own."""
+    features, forward-mode derivatives, torch.func and tracing) keep torch's
+    own."""
 
     def forward(self, x: Tensor) -> Tensor:
         if (not x.is_cuda or len(self.normalized_shape) != 1 or self.normalized_shape[0] > MAX_D
-                or x.dtype not in _lib.DTYPE_CODES or x.shape[-1:] != self.normalized_shape
+                or not is_plain(x, self.weight, self.bias) or x.dtype not in _lib.DTYPE_CODES or x.shape[-1:] != self.normalized_shape
                 or any(p is not None and p.dtype not in _lib.DTYPE_CODES for p in (self.weight, self.bias))):
             return super().forward(x)
         if x.dtype != torch.float32 and torch.is_autocast_enabled("cuda"):

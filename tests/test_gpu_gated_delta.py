@@ -608,3 +608,22 @@ def test_saved_tensors_that_come_back_in_another_layout(dtype, how):
             o, S, leaves = run()
         for a, b in zip(torch.autograd.grad([o, S], leaves, [do, dS]), want):
             assert torch.equal(a, b)
+
+
+def test_forward_mode_and_traced_inputs_are_refused():
+    from torch.autograd import forward_ad
+    d, _, _ = make(1, 3, 1, 2, 16, 8, torch.bfloat16, seed=47)
+    seq = [d[n] for n in ("q", "k", "v", "g", "beta")]
+    tok, state = [t[:, 0] for t in seq], d["initial"]
+    before = state.clone()
+    with forward_ad.dual_level():
+        for i in range(6):
+            a = [forward_ad.make_dual(t, torch.ones_like(t)) if j == i else t for j, t in enumerate([*seq, state])]
+            with pytest.raises(RuntimeError, match="forward-mode"):
+                gated_delta_rule(*a[:5], initial_state=a[5])
+            a = [forward_ad.make_dual(t, torch.ones_like(t)) if j == i else t for j, t in enumerate([*tok, state])]
+            with pytest.raises(RuntimeError, match="forward-mode"):
+                gated_delta_step(*a)
+    with torch.no_grad(), pytest.raises(RuntimeError, match="trace"):
+        torch.jit.trace(lambda *a: gated_delta_rule(*a), seq)
+    assert torch.equal(state, before)

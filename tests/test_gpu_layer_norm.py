@@ -207,3 +207,27 @@ def test_refusals():
                      ((x, w.cpu()), {}), ((torch.zeros(3, 0, device=DEV),), {})):
         with pytest.raises(RuntimeError):
             layer_norm(*args, **kw)
+
+
+def test_forward_mode_and_traced_inputs():
+    """The function refuses what it would drop a derivative of; the module runs torch's own norm there."""
+    from torch.autograd import forward_ad
+    g = torch.Generator(DEV).manual_seed(7)
+    x, t = (torch.randn(6, 48, generator=g, device=DEV) for _ in range(2))
+    ours, ref = LayerNorm(48).to(DEV), nn.LayerNorm(48).to(DEV)
+    with forward_ad.dual_level():
+        dual = forward_ad.make_dual(x, t)
+        for kw in (dict(), dict(residual=x)):
+            with pytest.raises(RuntimeError, match="forward-mode"):
+                layer_norm(dual, **kw)
+        with pytest.raises(RuntimeError, match="forward-mode"):
+            layer_norm(x, residual=dual)
+        got, want = (forward_ad.unpack_dual(m(dual)) for m in (ours, ref))
+        assert torch.equal(got.primal, want.primal) and torch.equal(got.tangent, want.tangent)
+        close(layer_norm(x), ref(x).double(), torch.float32)  # (a tensor without a tangent)
+    assert torch.equal(torch.func.jvp(ours, (x,), (t,))[1], torch.func.jvp(ref, (x,), (t,))[1])
+    with torch.no_grad():
+        with pytest.raises(RuntimeError, match="trace"):
+            torch.jit.trace(lambda a: layer_norm(a), x)
+        traced = torch.jit.trace(ours, x)
+        assert torch.equal(traced(t), ref(t))

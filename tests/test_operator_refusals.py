@@ -163,3 +163,24 @@ def test_delta_path_named_by_the_caller_without_device():
         assert L.eacs_delta_path(bad, 1) == 0 and L.eacs_delta_workspace_size(bad, 1) == 0
         assert L.eacs_delta_fwd(bad, P, None, P, big, 1, None) == _lib.EACS_ERR_INVALID
         assert L.eacs_delta_bwd(bad, P, strides, None, P, P, P, P, P, None, P, big, P, big, None) == _lib.EACS_ERR_INVALID
+
+
+def test_forward_mode_transforms_and_traces_are_seen():
+    """What a kernel called by pointer would drop: tangents, transforms' wrappers, records of a trace."""
+    from torch.autograd import forward_ad
+    from eacs_b200.ops._check import is_plain, require_plain
+    x, seen = torch.ones(3), []
+    assert is_plain(x, None) and is_plain(x.clone().requires_grad_(True))
+    with forward_ad.dual_level():
+        dual = forward_ad.make_dual(x, torch.ones(3))
+        assert is_plain(x) and not is_plain(x, None, dual)
+        with pytest.raises(RuntimeError, match="forward-mode"):
+            require_plain("op", dual)
+    note = lambda t: seen.append(is_plain(t)) or t * 1
+    torch.func.vmap(note)(torch.ones(2, 2))
+    torch.func.jvp(note, (x,), (x,))
+    torch.func.grad(lambda t: note(t).sum())(x)
+    assert seen == [False] * 3 and is_plain(x)
+    seen.clear()
+    torch.jit.trace(note, x, check_trace=False)
+    assert False in seen and is_plain(x)
