@@ -7,7 +7,8 @@ and, with the blended branches as the residual, MultiScaleEACS's
 out_norm(x + fused) (cst_ssm/modules/multiscale.py:176-179).  Statistics and
 sums are float32 and each output is rounded once, so x + residual is never
 rounded (or written) itself.  Differentiable in x, residual, weight and bias;
-the gradients of weight and bias are the same bits on every run.
+the gradients of weight and bias are the same bits on every run.  A backward
+with create_graph runs in torch operations, so that it can be differentiated.
 
 `LayerNorm` is the nn.LayerNorm module that runs it (same parameters and state
 dict), `use_norms(model)` turns the nn.LayerNorm modules of a model into it, and
@@ -54,6 +55,18 @@ def _forward(x, weight, bias, eps, residual, dev):
     return y
 
 
+def _recorded_gradients(x, weight, residual, dy, eps):
+    """The gradients (ds, dweight, dbias) in torch operations: for a backward that is itself to be differentiated."""
+    s = x.float() if residual is None else x.float() + residual.float()
+    c = s - s.mean(-1, keepdim=True)
+    rstd = (c.square().mean(-1, keepdim=True) + eps).rsqrt()
+    h, dy = c * rstd, dy.float()
+    p = dy if weight is None else dy * weight.float()
+    ds = rstd * (p - p.mean(-1, keepdim=True) - h * (p * h).mean(-1, keepdim=True))
+    d = x.shape[-1]
+    return ds.to(x.dtype), (dy * h).reshape(-1, d).sum(0), dy.reshape(-1, d).sum(0)
+
+
 class LayerNormFunction(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, eps, residual, dev):
@@ -63,12 +76,15 @@ class LayerNormFunction(torch.autograd.Function):
         return _forward(x, weight, bias, eps, residual, dev)
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, dy):
         x, weight, residual = ctx.saved_tensors
         need_x, need_w, need_b, _, need_r, _ = ctx.needs_input_grad
         dev, d = ctx.dev, x.shape[-1]
         wd = weight.dtype if weight is not None else ctx.bias_dtype
+        if torch.is_grad_enabled():  # create_graph
+            ds, dw, db = _recorded_gradients(x, weight, residual, dy, ctx.eps)
+            return (ds if need_x else None, dw.to(wd) if need_w else None, db.to(wd) if need_b else None, None,
+                    ds if need_r else None, None)
         dw = torch.empty(d, dtype=wd, device=dev) if need_w else None
         db = torch.empty(d, dtype=wd, device=dev) if need_b else None
         dx = torch.empty(x.shape, dtype=x.dtype, device=dev)

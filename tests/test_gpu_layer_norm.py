@@ -231,3 +231,23 @@ def test_forward_mode_and_traced_inputs():
             torch.jit.trace(lambda a: layer_norm(a), x)
         traced = torch.jit.trace(ours, x)
         assert torch.equal(traced(t), ref(t))
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_backward_of_the_backward(dtype):
+    """A gradient penalty through the module, against torch's norm in 64 bits: first gradients rounded to the type once, the
+    penalty's made of them and rounded again (half a step each, and 1e-5 for float32 sums)."""
+    g = torch.Generator(DEV).manual_seed(8)
+    x, dy = (torch.randn(5, 9, 64, generator=g, device=DEV).to(dtype) for _ in range(2))
+    m = LayerNorm(64).to(DEV)
+    nn.init.normal_(m.weight)
+    ref = nn.LayerNorm(64).double()
+    ref.load_state_dict({n: t.double().cpu() for n, t in m.state_dict().items()})
+    res = []
+    for norm, conv in ((m, lambda t: t.clone()), (ref, lambda t: t.double().cpu())):
+        xx = conv(x).requires_grad_(True)
+        dx, dw = torch.autograd.grad(norm(xx), (xx, norm.weight), conv(dy), create_graph=True)
+        res.append([dx, dw, *torch.autograd.grad(dx.square().sum() + dw.square().sum(), (xx, norm.weight))])
+    for a, c in zip(*res):
+        err = float((a.detach().double().cpu() - c.detach()).norm())
+        assert err <= (1e-5 + (torch.finfo(dtype).eps if dtype != torch.float32 else 0.0)) * float(c.detach().norm())
