@@ -758,7 +758,7 @@ __device__ __forceinline__ bool store_values(e16* to, const unsigned char* frag,
 
 // KEEP: S and U are written for a backward.
 template <typename T, int KD, int G, bool KEEP>
-__global__ void __launch_bounds__(Fwd<KD, G>::kWarps * 32) planes_chain_k(const __grid_constant__ DArgs a, const __grid_constant__ Maps maps) {
+__global__ void __launch_bounds__(Fwd<KD, G>::kWarps * 32, 1) planes_chain_k(const __grid_constant__ DArgs a, const __grid_constant__ Maps maps) {
     using Sm = Fwd<KD, G>;
     const int h = blockIdx.y, b = blockIdx.z, hk = h / (a.Hv / a.Hk);
     const int len = row_length(a, b), nc = (len + kC - 1) / kC;
@@ -882,7 +882,7 @@ __global__ void __launch_bounds__(Fwd<KD, G>::kWarps * 32) planes_chain_k(const 
                         [&](int i, const uint32_t(*f)[4]) {
                             Af<2>& af = as[i & 1];
                             st_tile(sS, Sm::LDK, 16 * i, af.r[0]);
-                            if constexpr (KEEP) st_tile(sS + 16 * Sm::LDK, Sm::LDK, 16 * i, af.r[1]);
+                            st_tile(sS + 16 * Sm::LDK, Sm::LDK, 16 * i, af.r[1]);
                             mma_step_with<T>(X, af, f, [&](int q) {
                                 if (i + 1 < KD / 16) {
                                     const float* s = S[2 * i + 2 + q / 2];
@@ -1024,14 +1024,14 @@ __global__ void __launch_bounds__(Fwd<KD, G>::kWarps * 32) planes_chain_k(const 
             const Sh sS = sh(theirs + Sm::kS);
             float4* sO = reinterpret_cast<float4*>(theirs + Sm::kO);
             ok = warp_wait(&s_full[g], c & 1) && ok;
-            // scale gam Q S0: S in one plane (its rounding, half a step of terms of any sign, against
-            // the output's own: in bfloat16 y is off by 2.2e-3 in the norm instead of 1.7e-3, for half
-            // the products)
+            // scale gam Q S0 (with S in one plane y is off by 2.2e-3 in the norm instead of 1.7e-3, and
+            // by 2^-9 |q| |S| where the terms cancel)
             float O[kC / 8][4] = {};
-            Af<1> as[2];
+            Af<2> as[2];
             steps<KD / 16>(
                 [&](int k, uint32_t(*f)[4]) {
                     ld_a(as[k & 1].r[0], sS, Sm::LDK, 0, 16 * k);
+                    ld_a(as[k & 1].r[1], sS + 16 * Sm::LDK, Sm::LDK, 0, 16 * k);
 #pragma unroll
                     for (int p = 0; p < 4; ++p) ld_b128<false>(f[p], es + Sm::kQ, 16 * p, 16 * k);
                 },
@@ -1139,7 +1139,7 @@ struct Rev {
 };
 
 template <typename T, int KD, int G>
-__global__ void __launch_bounds__(Rev<KD, G>::kWarps * 32) planes_rchain_k(const __grid_constant__ DArgs a, const __grid_constant__ Maps maps) {
+__global__ void __launch_bounds__(Rev<KD, G>::kWarps * 32, 1) planes_rchain_k(const __grid_constant__ DArgs a, const __grid_constant__ Maps maps) {
     using Sm = Rev<KD, G>;
     const int h = blockIdx.y, b = blockIdx.z, hk = h / (a.Hv / a.Hk);
     const int len = row_length(a, b), nc = (len + kC - 1) / kC;

@@ -627,3 +627,26 @@ def test_forward_mode_and_traced_inputs_are_refused():
     with torch.no_grad(), pytest.raises(RuntimeError, match="trace"):
         torch.jit.trace(lambda *a: gated_delta_rule(*a), seq)
     assert torch.equal(state, before)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("training", [False, True])
+@pytest.mark.parametrize("K,V", [(128, 128), (64, 40)])
+def test_outputs_of_a_large_state_that_cancels(dtype, training, K, V):
+    """A state whose columns sum to 0 under queries of equal elements: its operands' rounding (TOL of |q| |S|) shows, not
+    the outputs'.  beta = 0 and g = 0 keep the state."""
+    L = 130
+    d, _, _ = make(1, L, 1, 2, K, V, dtype, torch.float32, seed=42)
+    d["beta"].zero_()
+    d["g"].zero_()
+    d["q"] = (K ** -0.5 * (1 + 0.01 * d["q"].float())).to(dtype)
+    S0 = 64 * (d["initial"] - d["initial"].mean(2, keepdim=True))
+    x = [d[n] for n in ("q", "k", "v", "g", "beta")]
+    if training:
+        x[2] = x[2].clone().requires_grad_(True)
+    o, S = gated_delta_rule(*x, initial_state=S0, output_final_state=True)
+    want, _ = oracle(*(t.detach().double().cpu() for t in x), K ** -0.5, S0.double().cpu())
+    size = K ** -0.5 * L ** 0.5 * float(d["q"][0, 0].float().norm()) * float(S0.norm())
+    err = float((o.detach().double().cpu() - want).norm())
+    assert err <= TOL * size + torch.finfo(dtype).eps / 2 * float(want.norm()), err / size
+    assert torch.equal(S.detach(), S0)
