@@ -233,27 +233,11 @@ __device__ __forceinline__ void mma_pair(float* c0, float* c1, const uint32_t* a
 }
 // A in P planes times one plane of B
 template <typename T, int P, bool TR>
-__device__ __forceinline__ void mm(float* c0, float* c1, const Af<P>& a, Sh s, int ld, int n0, int k0) {
-    uint32_t b[4];
-    ld_b<TR>(b, s, ld, n0, k0);
-#pragma unroll
-    for (int p = P - 1; p >= 0; --p) mma_pair<T>(c0, c1, a.r[p], b);
-}
-template <typename T, int P, bool TR>
 __device__ __forceinline__ void mm128(float* c0, float* c1, const Af<P>& a, Sh s, int n0, int k0) {
     uint32_t b[4];
     ld_b128<TR>(b, s, n0, k0);
 #pragma unroll
     for (int p = P - 1; p >= 0; --p) mma_pair<T>(c0, c1, a.r[p], b);
-}
-// A in P planes times B in two (the product of the low planes is left out)
-template <typename T, int P, bool TR>
-__device__ __forceinline__ void mm_hl(float* c0, float* c1, const Af<P>& a, Sh hi, Sh lo, int ld,
-                                      int n0, int k0) {
-    uint32_t b[4];
-    ld_b<TR>(b, lo, ld, n0, k0);
-    mma_pair<T>(c0, c1, a.r[0], b);
-    mm<T, P, TR>(c0, c1, a, hi, ld, n0, k0);
 }
 // Steps 0..N-1 of a product: a step's tiles of B (up to four pairs) are read
 // while the step before is multiplied.
@@ -1120,9 +1104,8 @@ __global__ void __launch_bounds__(Fwd<KD, G>::kWarps * 32, 1) planes_chain_k(con
 // ----------------------------------------------------------------------------
 // the reverse chain
 // ----------------------------------------------------------------------------
-// All operands in two planes but for dV in K^T (gam dV), whose rounding stays
-// below the gradients' own (measured against 64 bits: 1.7e-3 of the norm of
-// every gradient, which is the outputs' rounding alone, with either).
+// All operands in two planes (with dV in one, float32 gradients of gates were off
+// by 1.2e-3 of their norm).
 template <int KD, int G>
 struct Rev {
     static constexpr int LDK = KD + 8;
@@ -1276,12 +1259,12 @@ __global__ void __launch_bounds__(Rev<KD, G>::kWarps * 32, 1) planes_rchain_k(co
                 // (scale gam dO)^T Q added, and the last tokens of dV, done first, are split for the update
                 float X[kC / 8][4] = {};
                 const float gc = gam[kC - 1];
-                auto decayed = [&](Af<1>& to, int kk, int q) {
+                auto decayed = [&](Af<2>& to, int kk, int q) {
                     const float2 d = *reinterpret_cast<const float2*>(gam + 16 * kk + 8 * (q / 2) + 2 * L.t);
                     const float* u = X[2 * kk + q / 2];
                     from_acc_part<T>(to, q, -u[2 * (q & 1)] * d.x, -u[2 * (q & 1) + 1] * d.y);
                 };
-                Af<1> xd[2];
+                Af<2> xd[2];
                 {
                     Af<2> au[2];
                     au[1] = from_acc<T, 2>(U[6], U[7]);
@@ -1399,9 +1382,7 @@ __global__ void __launch_bounds__(Rev<KD, G>::kWarps * 32, 1) planes_rchain_k(co
 // the L1 cache too small for it, and spilled sums went to L2 (1039 us for 393216
 // tokens of 128 x 128 with 16 warps of a quarter of all products each).  The value
 // columns come in tiles of 32, two deep, so that the two states of a chunk (in two
-// planes 139 KB of its 260 KB) never have to be in shared memory whole.  dV, whose
-// rounding does not show in the products, goes in as one plane (the output
-// itself); U, S, dS, N and E as two.
+// planes 139 KB of its 260 KB) never have to be in shared memory whole.
 constexpr int kGradWarps = 16;
 template <int KD>
 struct Grad {
@@ -1645,9 +1626,11 @@ __global__ void __launch_bounds__(32 * kGradWarps, 1) planes_grad_k(const __grid
                 for (int kk = 0; kk < VT / 16; ++kk) {
                     if (16 * kk >= vn) break;
                     if (!writer) {
-                        Af<1> fd, fx;
+                        Af<1> fd;
+                        Af<2> fx;
                         ld_a32(fd.r[0], es + Sm::kD + kk * kC * 16, m0);
                         ld_at(fx.r[0], es + Sm::kX, kTld, m0, 16 * kk);
+                        ld_at(fx.r[1], es + Sm::kX + VT * kTld, kTld, m0, 16 * kk);
 #pragma unroll
                         for (int p = 0; p < NT / 2; ++p) {
                             uint32_t sh[4], sl[4];
@@ -1656,6 +1639,7 @@ __global__ void __launch_bounds__(32 * kGradWarps, 1) planes_grad_k(const __grid
                             mma_pair<T>(x[2 * p], x[2 * p + 1], fd.r[0], sl);
                             mma_pair<T>(y[2 * p], y[2 * p + 1], fx.r[0], sl);
                             mma_pair<T>(x[2 * p], x[2 * p + 1], fd.r[0], sh);
+                            mma_pair<T>(y[2 * p], y[2 * p + 1], fx.r[1], sh);
                             mma_pair<T>(y[2 * p], y[2 * p + 1], fx.r[0], sh);
                         }
                         if ((kk & 1) == half) {  // dv
@@ -1668,35 +1652,40 @@ __global__ void __launch_bounds__(32 * kGradWarps, 1) planes_grad_k(const __grid
                             }
                         }
                     } else {
-                        Af<1> left;
-                        Af<2> fu;
+                        Af<2> left, fu;  // (dO has no low plane)
                         ld_at(fu.r[0], es + Sm::kU, kTld, m0, 16 * kk);
                         ld_at(fu.r[1], es + Sm::kU + VT * kTld, kTld, m0, 16 * kk);
-                        if (half) ld_at(left.r[0], es + Sm::kX, kTld, m0, 16 * kk);
-                        else ld_a32(left.r[0], es + Sm::kD + kk * kC * 16, m0);
+                        if (half) {
+                            ld_at(left.r[0], es + Sm::kX, kTld, m0, 16 * kk);
+                            ld_at(left.r[1], es + Sm::kX + VT * kTld, kTld, m0, 16 * kk);
+                        } else {
+                            ld_a32(left.r[0], es + Sm::kD + kk * kC * 16, m0);
+                        }
+                        auto triangle = [&](int p) {
+                            uint32_t uh[4], ul[4];
+                            ld_b<true>(ul, es + Sm::kU + VT * kTld, kTld, 16 * p, 16 * kk);
+                            ld_b<true>(uh, es + Sm::kU, kTld, 16 * p, 16 * kk);
+                            mma_pair<T>(y[2 * p], y[2 * p + 1], left.r[0], ul);
+                            if (half) mma_pair<T>(y[2 * p], y[2 * p + 1], left.r[1], uh);
+                            mma_pair<T>(y[2 * p], y[2 * p + 1], left.r[0], uh);
+                        };
 #pragma unroll
                         for (int p = 0; p < NT / 2; ++p) {
                             uint32_t rh[4], rl[4];
                             ld_b<true>(rl, es + Sm::kR + VT * Sm::LDK, Sm::LDK, n0 + 16 * p, 16 * kk);
                             ld_b<true>(rh, es + Sm::kR, Sm::LDK, n0 + 16 * p, 16 * kk);
                             mma_pair<T>(x[2 * p], x[2 * p + 1], fu.r[0], rl);
-                            if (p <= rg)
-                                mm_hl<T, 1, true>(y[2 * p], y[2 * p + 1], left, es + Sm::kU, es + Sm::kU + VT * kTld, kTld, 16 * p,
-                                               16 * kk);
+                            if (p <= rg) triangle(p);
                             mma_pair<T>(x[2 * p], x[2 * p + 1], fu.r[1], rh);
                             mma_pair<T>(x[2 * p], x[2 * p + 1], fu.r[0], rh);
                         }
 #pragma unroll
                         for (int p = NT / 2; p < kC / 16; ++p)
-                            if (p <= rg)
-                                mm_hl<T, 1, true>(y[2 * p], y[2 * p + 1], left, es + Sm::kU, es + Sm::kU + VT * kTld, kTld, 16 * p,
-                                               16 * kk);
+                            if (p <= rg) triangle(p);
                         if (half) {  // dbeta = (dV / beta).(U / beta)
-                            uint32_t xl[4];
-                            ld_at(xl, es + Sm::kX + VT * kTld, kTld, m0, 16 * kk);
 #pragma unroll
                             for (int i = 0; i < 4; ++i) {
-                                const float2 p = Num<T>::unpack(left.r[0][i]), q = Num<T>::unpack(xl[i]);
+                                const float2 p = Num<T>::unpack(left.r[0][i]), q = Num<T>::unpack(left.r[1][i]);
                                 const float2 u = Num<T>::unpack(fu.r[0][i]), w = Num<T>::unpack(fu.r[1][i]);
                                 const float f = ga[5 * kC + (i & 1 ? r1 : r0)];
                                 float& db = i & 1 ? db1 : db0;

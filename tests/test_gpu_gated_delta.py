@@ -650,3 +650,15 @@ def test_outputs_of_a_large_state_that_cancels(dtype, training, K, V):
     err = float((o.detach().double().cpu() - want).norm())
     assert err <= TOL * size + torch.finfo(dtype).eps / 2 * float(want.norm()), err / size
     assert torch.equal(S.detach(), S0)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("shape", [(2, 257, 2, 2, 128, 128), (1, 150, 1, 2, 64, 96), (1, 200, 2, 4, 128, 40)])
+def test_float32_gradients_of_16_bit_tokens(dtype, shape):
+    """The gradients of float32 gates and of the initial state are computed from operands of 16 bits or more, like the
+    outputs: within TOL, whatever the tokens' type."""
+    d, do, dS = make(*shape, dtype, torch.float32, seed=43)
+    got, want = both(d, do, dS)
+    for n in ("dg", "dbeta", "dinitial"):
+        err, ref = float((got[n].double().cpu() - want[n]).norm()), float(want[n].norm())
+        assert got[n].dtype == torch.float32 and err <= TOL * ref, (n, err / ref)
