@@ -252,27 +252,6 @@ __device__ __forceinline__ void chain_load(const DArgs& a, unsigned char* st, in
     load_ws(ga, 2 * kC, a.gates + id * kGates + 2 * kC, 2 * kC, 1, 2 * kC, tid, nthr);
 }
 
-// S^T (16 value rows v0.., K columns) of a (K, V) float32 state
-template <int KD>
-__device__ __forceinline__ void state_load(float (*S)[4], const float* p, int K, int V, int v0, const Lane& L) {
-#pragma unroll
-    for (int j = 0; j < KD / 8; ++j)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            const int k = 8 * j + 2 * L.t + (e & 1), v = v0 + L.g + (e >> 1) * 8;
-            S[j][e] = k < K && v < V ? p[static_cast<int64_t>(k) * V + v] : 0.f;
-        }
-}
-template <int KD>
-__device__ __forceinline__ void state_store(const float (*S)[4], float* p, int K, int V, int v0, const Lane& L) {
-#pragma unroll
-    for (int j = 0; j < KD / 8; ++j)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            const int k = 8 * j + 2 * L.t + (e & 1), v = v0 + L.g + (e >> 1) * 8;
-            if (k < K && v < V) p[static_cast<int64_t>(k) * V + v] = S[j][e];
-        }
-}
 // accumulators into a dense [row][ld] workspace tile, rows r0.., as pairs
 __device__ __forceinline__ void put2(float* p, float x, float y) { *reinterpret_cast<float2*>(p) = make_float2(x, y); }
 
@@ -324,12 +303,7 @@ __global__ void __launch_bounds__(W * 32) delta_chain_k(DArgs a) {
     extern __shared__ __align__(16) unsigned char smem[];
     const int64_t head = static_cast<int64_t>(b) * a.Hv + h;
     float S[KD / 8][4];
-    if (a.initial) {
-        state_load<KD>(S, a.initial + head * a.K * a.V, a.K, a.V, v0, L);
-    } else {
-#pragma unroll
-        for (int j = 0; j < KD / 8; ++j) S[j][0] = S[j][1] = S[j][2] = S[j][3] = 0.f;
-    }
+    state_load<KD>(S, a.initial ? a.initial + head * a.K * a.V : nullptr, a.K, a.V, v0, L);
     const bool on = v0 < a.Vp;
     float4* mine = reinterpret_cast<float4*>(smem + 2 * St::bytes) + warp * 4 * KD + L.l;
     if (nc > 0) chain_load<F, T, KD, W>(a, smem, 0, b, h, hk, len, vb, W * 32);
@@ -587,12 +561,7 @@ __global__ void __launch_bounds__(W * 32) delta_rchain_k(DArgs a) {
     extern __shared__ __align__(16) unsigned char smem[];
     const int64_t head = static_cast<int64_t>(b) * a.Hv + h;
     float S[KD / 8][4];  // dS^T
-    if (a.dfinal) {
-        state_load<KD>(S, a.dfinal + head * a.K * a.V, a.K, a.V, v0, L);
-    } else {
-#pragma unroll
-        for (int j = 0; j < KD / 8; ++j) S[j][0] = S[j][1] = S[j][2] = S[j][3] = 0.f;
-    }
+    state_load<KD>(S, a.dfinal ? a.dfinal + head * a.K * a.V : nullptr, a.K, a.V, v0, L);
     const bool on = v0 < a.Vp;
     constexpr bool two = St::kStages == 2;
     float4* mine = reinterpret_cast<float4*>(smem + St::kStages * St::bytes) + warp * 4 * KD + L.l;
@@ -1078,17 +1047,6 @@ __global__ void __launch_bounds__(128, 8) delta_step_k(const __grid_constant__ D
 // ----------------------------------------------------------------------------
 // launches
 // ----------------------------------------------------------------------------
-template <typename K>
-cudaError_t smem_limit(K kernel, size_t bytes) {
-    return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(bytes));
-}
-
-#define DELTA_TRY(x)                          \
-    do {                                      \
-        const cudaError_t e_ = (x);           \
-        if (e_ != cudaSuccess) return e_;     \
-    } while (0)
-
 template <class F, typename T, int KD, int W>
 cudaError_t run_chain(const DArgs& a, bool reverse, cudaStream_t s) {
     const dim3 grid((a.Vp + 16 * W - 1) / (16 * W), a.Hv, a.B);

@@ -262,9 +262,40 @@ template <> __device__ __forceinline__ void load8<__nv_bfloat16>(const __nv_bflo
     }
 }
 
+// S^T (16 value rows v0.., K columns) of a (K, V) float32 state, or zeros
+template <int KD>
+__device__ __forceinline__ void state_load(float (*S)[4], const float* p, int K, int V, int v0, const Lane& L) {
+#pragma unroll
+    for (int j = 0; j < KD / 8; ++j)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const int k = 8 * j + 2 * L.t + (e & 1), v = v0 + L.g + (e >> 1) * 8;
+            S[j][e] = p && k < K && v < V ? p[static_cast<int64_t>(k) * V + v] : 0.f;
+        }
+}
+template <int KD>
+__device__ __forceinline__ void state_store(const float (*S)[4], float* p, int K, int V, int v0, const Lane& L) {
+#pragma unroll
+    for (int j = 0; j < KD / 8; ++j)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const int k = 8 * j + 2 * L.t + (e & 1), v = v0 + L.g + (e >> 1) * 8;
+            if (k < K && v < V) p[static_cast<int64_t>(k) * V + v] = S[j][e];
+        }
+}
 
+template <typename K>
+cudaError_t smem_limit(K kernel, size_t bytes) {
+    return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(bytes));
+}
 
-// delta_planes.cu: bfloat16 and float16 inputs whose rows start on 16 bytes
+#define DELTA_TRY(x)                          \
+    do {                                      \
+        const cudaError_t e_ = (x);           \
+        if (e_ != cudaSuccess) return e_;     \
+    } while (0)
+
+// delta_planes.cu: bfloat16 inputs whose rows start on 16 bytes, and float16 ones without a backward
 size_t planes_saved_size(const DArgs& a, bool training);
 size_t planes_bwd_size(const DArgs& a);
 cudaError_t planes_fwd(DArgs a, void* ws, bool training, cudaStream_t s);

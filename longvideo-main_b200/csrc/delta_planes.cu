@@ -645,28 +645,6 @@ struct Fwd {
     static constexpr size_t bytes = 1024 + kExp + 4 * G;
 };
 
-// S^T (16 value rows v0.., K columns) of a (K, V) float32 state
-template <int KD>
-__device__ __forceinline__ void state_load(float (*S)[4], const float* p, int K, int V, int v0, const Lane& L) {
-#pragma unroll
-    for (int j = 0; j < KD / 8; ++j)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            const int k = 8 * j + 2 * L.t + (e & 1), v = v0 + L.g + (e >> 1) * 8;
-            S[j][e] = p && k < K && v < V ? p[static_cast<int64_t>(k) * V + v] : 0.f;
-        }
-}
-template <int KD>
-__device__ __forceinline__ void state_store(const float (*S)[4], float* p, int K, int V, int v0, const Lane& L) {
-#pragma unroll
-    for (int j = 0; j < KD / 8; ++j)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            const int k = 8 * j + 2 * L.t + (e & 1), v = v0 + L.g + (e >> 1) * 8;
-            if (k < K && v < V) p[static_cast<int64_t>(k) * V + v] = S[j][e];
-        }
-}
-
 // A group's accumulators (16 x 64) between warps: float32 as the lanes hold them.
 __device__ __forceinline__ void frag_put(float4* s, const float (*x)[4], const Lane& L) {
 #pragma unroll
@@ -1437,84 +1415,84 @@ __device__ __forceinline__ bool grad_produce(const DArgs& a, const Maps& maps, u
     const int rep = a.Hv / a.Hk, items = a.B * a.Hk * a.n;
     const Lane L;
     bool ok = true;
-            int it = at[0], h = at[1], v0 = at[2];
-            if (it >= items) return true;
-            const int bh = it / a.n, c = it - bh * a.n, b = bh / a.Hk, hk = bh - b * a.Hk, t0 = c * kC;
-            const int ptile = at[3], pseen = at[4];
-            int landed = at[5];
-            const int rows = min(kC, row_length(a, b) - t0);
-            const bool tail = rows < min(kC, a.L - t0);
-            if (h < 0) {  // a new chunk: its keys and queries
-                h = hk * rep;
-                e16* e = reinterpret_cast<e16*>(smem + 2 * Sm::kStage + (pseen & 1) * Sm::kKQ);
-                uint64_t* bar = tail ? land : &qfull[pseen & 1];
-                ok = warp_wait(&qempty[pseen & 1], ((pseen >> 1) & 1) ^ 1) && ok;
-                if (L.l == 0) {
-                    mbar_expect_tx(bar, Sm::kKQ);
-    #pragma unroll
-                    for (int x = 0; x < KD; x += 64) {
-                        tma_load(e + Sm::kK + x * kC, &maps.k, bar, x, t0, hk, b);
-                        tma_load(e + Sm::kQ + x * kC, &maps.q, bar, x, t0, hk, b);
-                    }
-                }
-                __syncwarp();
-                if (tail) {
-                    ok = warp_wait(land, landed++ & 1) && ok;
-                    zero_rows<64>(e + Sm::kK, 2 * (KD / 64), rows);
-                    fence_async();
-                    warp_arrive(&qfull[pseen & 1]);
-                }
+    int it = at[0], h = at[1], v0 = at[2];
+    if (it >= items) return true;
+    const int bh = it / a.n, c = it - bh * a.n, b = bh / a.Hk, hk = bh - b * a.Hk, t0 = c * kC;
+    const int ptile = at[3], pseen = at[4];
+    int landed = at[5];
+    const int rows = min(kC, row_length(a, b) - t0);
+    const bool tail = rows < min(kC, a.L - t0);
+    if (h < 0) {  // a new chunk: its keys and queries
+        h = hk * rep;
+        e16* e = reinterpret_cast<e16*>(smem + 2 * Sm::kStage + (pseen & 1) * Sm::kKQ);
+        uint64_t* bar = tail ? land : &qfull[pseen & 1];
+        ok = warp_wait(&qempty[pseen & 1], ((pseen >> 1) & 1) ^ 1) && ok;
+        if (L.l == 0) {
+            mbar_expect_tx(bar, Sm::kKQ);
+#pragma unroll
+            for (int x = 0; x < KD; x += 64) {
+                tma_load(e + Sm::kK + x * kC, &maps.k, bar, x, t0, hk, b);
+                tma_load(e + Sm::kQ + x * kC, &maps.q, bar, x, t0, hk, b);
             }
-            const int vn = min(VT, a.Vp - v0);
-            e16* e = reinterpret_cast<e16*>(smem + (ptile & 1) * Sm::kStage);
-            uint64_t* bar = tail ? land : &full[ptile & 1];
-            ok = warp_wait(&empty[ptile & 1], ((ptile >> 1) & 1) ^ 1) && ok;
-            if (L.l == 0) {
-                const int64_t id = (static_cast<int64_t>(b) * a.Hv + h) * a.n + c;
-                mbar_expect_tx(bar, vn * (kC + 4 * kTld + 4 * Sm::LDK) * 2 + kGates * 4);
-                for (int v = 0; v < vn; v += 16) tma_load(e + Sm::kD + v * kC, &maps.d, bar, v0 + v, t0, h, b);
-                const e16* U = static_cast<const e16*>(a.U) + (id * 2 * a.Vp + v0) * kTld;
-                const e16* X = static_cast<const e16*>(a.dV) + (id * 2 * a.Vp + v0) * kTld;
-                const e16* S = static_cast<const e16*>(a.S) + (id * 2 * a.Vp + v0) * Sm::LDK;
-                const e16* R = static_cast<const e16*>(a.dS) + (id * 2 * a.Vp + v0) * Sm::LDK;
-                for (int p = 0; p < 2; ++p) {
-                    bulk_load(e + Sm::kS + p * VT * Sm::LDK, S + static_cast<int64_t>(p) * a.Vp * Sm::LDK, vn * Sm::LDK * 2, bar);
-                    bulk_load(e + Sm::kR + p * VT * Sm::LDK, R + static_cast<int64_t>(p) * a.Vp * Sm::LDK, vn * Sm::LDK * 2, bar);
-                    bulk_load(e + Sm::kU + p * VT * kTld, U + static_cast<int64_t>(p) * a.Vp * kTld, vn * kTld * 2, bar);
-                    bulk_load(e + Sm::kX + p * VT * kTld, X + static_cast<int64_t>(p) * a.Vp * kTld, vn * kTld * 2, bar);
-                }
-                bulk_load(e + Sm::kGa, a.gates + id * kGates, kGates * 4, bar);
+        }
+        __syncwarp();
+        if (tail) {
+            ok = warp_wait(land, landed++ & 1) && ok;
+            zero_rows<64>(e + Sm::kK, 2 * (KD / 64), rows);
+            fence_async();
+            warp_arrive(&qfull[pseen & 1]);
+        }
+    }
+    const int vn = min(VT, a.Vp - v0);
+    e16* e = reinterpret_cast<e16*>(smem + (ptile & 1) * Sm::kStage);
+    uint64_t* bar = tail ? land : &full[ptile & 1];
+    ok = warp_wait(&empty[ptile & 1], ((ptile >> 1) & 1) ^ 1) && ok;
+    if (L.l == 0) {
+        const int64_t id = (static_cast<int64_t>(b) * a.Hv + h) * a.n + c;
+        mbar_expect_tx(bar, vn * (kC + 4 * kTld + 4 * Sm::LDK) * 2 + kGates * 4);
+        for (int v = 0; v < vn; v += 16) tma_load(e + Sm::kD + v * kC, &maps.d, bar, v0 + v, t0, h, b);
+        const e16* U = static_cast<const e16*>(a.U) + (id * 2 * a.Vp + v0) * kTld;
+        const e16* X = static_cast<const e16*>(a.dV) + (id * 2 * a.Vp + v0) * kTld;
+        const e16* S = static_cast<const e16*>(a.S) + (id * 2 * a.Vp + v0) * Sm::LDK;
+        const e16* R = static_cast<const e16*>(a.dS) + (id * 2 * a.Vp + v0) * Sm::LDK;
+        for (int p = 0; p < 2; ++p) {
+            bulk_load(e + Sm::kS + p * VT * Sm::LDK, S + static_cast<int64_t>(p) * a.Vp * Sm::LDK, vn * Sm::LDK * 2, bar);
+            bulk_load(e + Sm::kR + p * VT * Sm::LDK, R + static_cast<int64_t>(p) * a.Vp * Sm::LDK, vn * Sm::LDK * 2, bar);
+            bulk_load(e + Sm::kU + p * VT * kTld, U + static_cast<int64_t>(p) * a.Vp * kTld, vn * kTld * 2, bar);
+            bulk_load(e + Sm::kX + p * VT * kTld, X + static_cast<int64_t>(p) * a.Vp * kTld, vn * kTld * 2, bar);
+        }
+        bulk_load(e + Sm::kGa, a.gates + id * kGates, kGates * 4, bar);
+    }
+    __syncwarp();
+    if (tail) {
+        ok = warp_wait(land, landed++ & 1) && ok;
+        zero_rows<16>(e + Sm::kD, vn / 16, rows);
+        fence_async();
+        warp_arrive(&full[ptile & 1]);
+    }
+    // the next tile: of this head, of the next, or of the next chunk with a token
+    int seen_next = pseen;
+    v0 += VT;
+    if (v0 >= a.Vp) {
+        v0 = 0;
+        if (++h == (hk + 1) * rep) {
+            h = -1;
+            ++seen_next;
+            for (it += gridDim.x; it < items; it += gridDim.x) {
+                const int nbh = it / a.n;
+                if (row_length(a, nbh / a.Hk) > (it - nbh * a.n) * kC) break;
             }
-            __syncwarp();
-            if (tail) {
-                ok = warp_wait(land, landed++ & 1) && ok;
-                zero_rows<16>(e + Sm::kD, vn / 16, rows);
-                fence_async();
-                warp_arrive(&full[ptile & 1]);
-            }
-            // the next tile: of this head, of the next, or of the next chunk with a token
-            int seen_next = pseen;
-            v0 += VT;
-            if (v0 >= a.Vp) {
-                v0 = 0;
-                if (++h == (hk + 1) * rep) {
-                    h = -1;
-                    ++seen_next;
-                    for (it += gridDim.x; it < items; it += gridDim.x) {
-                        const int nbh = it / a.n;
-                        if (row_length(a, nbh / a.Hk) > (it - nbh * a.n) * kC) break;
-                    }
-                }
-            }
-            if (L.l == 0) {
-                at[0] = it;
-                at[1] = h;
-                at[2] = v0;
-                at[3] = ptile + 1;
-                at[4] = seen_next;
-                at[5] = landed;
-            }
-            __syncwarp();
+        }
+    }
+    if (L.l == 0) {
+        at[0] = it;
+        at[1] = h;
+        at[2] = v0;
+        at[3] = ptile + 1;
+        at[4] = seen_next;
+        at[5] = landed;
+    }
+    __syncwarp();
     return ok;
 }
 
@@ -1913,46 +1891,37 @@ __global__ void __launch_bounds__(32 * kGradWarps, 1) planes_grad_k(const __grid
 // ----------------------------------------------------------------------------
 // launches
 // ----------------------------------------------------------------------------
-template <typename K>
-cudaError_t smem_limit(K kernel, size_t bytes) {
-    return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(bytes));
-}
-
-#define PLANES_TRY(x)                         \
-    do {                                      \
-        const cudaError_t e_ = (x);           \
-        if (e_ != cudaSuccess) return e_;     \
-    } while (0)
-
 constexpr int kSms = 148;
 
 // Groups of 16 value columns per CTA of a chain, one CTA on an SM at a time: the
-// fewest rounds of CTAs, weighed with what a chunk takes with G groups on an SM
-// (measured at K = V = 128, in units of 0.1 us: forward 28, 40, 44 with 2, 3, 4
-// groups, reverse 27, 35 with 2, 3; four do not fit the reverse chain's tiles).
-// 48 heads of 128 take 510 us of a forward with three groups, 710 with two.
+// fewest rounds of CTAs, weighed with what a chunk takes with 2, 3 or 4 groups on
+// an SM.  Measured at V = 128, us:
+//                                       K = 128            K = 64
+//   forward                             2.43 3.36 3.27     1.73 2.75 2.38
+//   forward, float16                    2.98 3.62 3.77     2.12 2.99 2.77
+//   forward that keeps for a backward   2.74 3.54 4.37     2.36 2.93 3.82
+//   reverse                             2.80 3.40          2.34 2.93
+// (four groups do not fit the reverse chain's tiles).
 int chain_groups(const DArgs& a, bool reverse) {
     const int64_t heads = static_cast<int64_t>(a.B) * a.Hv, groups = a.Vp / 16;
     auto cost = [&](int64_t g, int64_t per) { return (heads * ((groups + g - 1) / g) + kSms - 1) / kSms * per; };
-    const int64_t x2 = cost(2, reverse ? 27 : 28), x3 = cost(3, reverse ? 35 : 40), x4 = cost(4, 44);
+    const int64_t x2 = cost(2, 27), x3 = cost(3, 34), x4 = cost(4, a.S ? 43 : 36);
     if (reverse) return x2 <= x3 ? 2 : 3;
+    if (!a.S) return x2 <= x4 ? 2 : 4;  // (three are no faster than four)
     return x2 <= x3 && x2 <= x4 ? 2 : x3 <= x4 ? 3 : 4;
 }
 
-template <typename T, int KD, int G>
+template <typename T, int KD, int G, bool KEEP>
 cudaError_t chain_launch(const DArgs& a, const Maps& m, cudaStream_t s) {
-    auto k = planes_chain_k<T, KD, G, false>;
-    if constexpr (!Scaled<T>) {
-        if (a.S) k = planes_chain_k<T, KD, G, true>;
-    }
-    PLANES_TRY(smem_limit(k, Fwd<KD, G>::bytes));
+    const auto k = planes_chain_k<T, KD, G, KEEP>;
+    DELTA_TRY(smem_limit(k, Fwd<KD, G>::bytes));
     k<<<dim3((a.Vp / 16 + G - 1) / G, a.Hv, a.B), Fwd<KD, G>::kWarps * 32, Fwd<KD, G>::bytes, s>>>(a, m);
     note_launch();
     return cudaGetLastError();
 }
 template <typename T, int KD, int G>
 cudaError_t rchain_launch(const DArgs& a, const Maps& m, cudaStream_t s) {
-    PLANES_TRY((smem_limit(planes_rchain_k<T, KD, G>, Rev<KD, G>::bytes)));
+    DELTA_TRY((smem_limit(planes_rchain_k<T, KD, G>, Rev<KD, G>::bytes)));
     planes_rchain_k<T, KD, G><<<dim3((a.Vp / 16 + G - 1) / G, a.Hv, a.B), Rev<KD, G>::kWarps * 32, Rev<KD, G>::bytes, s>>>(a, m);
     note_launch();
     return cudaGetLastError();
@@ -1963,8 +1932,12 @@ cudaError_t chain(const DArgs& a, const Maps& m, bool reverse, cudaStream_t s) {
     const int g = chain_groups(a, reverse);
     if constexpr (!Scaled<T>) {
         if (reverse) return g == 2 ? rchain_launch<T, KD, 2>(a, m, s) : rchain_launch<T, KD, 3>(a, m, s);
+        if (a.S)
+            return g == 2   ? chain_launch<T, KD, 2, true>(a, m, s)
+                   : g == 3 ? chain_launch<T, KD, 3, true>(a, m, s)
+                            : chain_launch<T, KD, 4, true>(a, m, s);
     }
-    return g == 2 ? chain_launch<T, KD, 2>(a, m, s) : g == 3 ? chain_launch<T, KD, 3>(a, m, s) : chain_launch<T, KD, 4>(a, m, s);
+    return g == 2 ? chain_launch<T, KD, 2, false>(a, m, s) : chain_launch<T, KD, 4, false>(a, m, s);
 }
 
 PFN_cuTensorMapEncodeTiled_v12000 encode_fn() {
@@ -2004,21 +1977,21 @@ template <typename T, int KD>
 cudaError_t fwd(const DArgs& a, cudaStream_t s) {
     // a runtime call first: tensor maps are not made in a thread (autograd's, say) that
     // has not met its device yet
-    PLANES_TRY((smem_limit(planes_prep_k<T, KD>, Prep<KD>::bytes)));
+    DELTA_TRY((smem_limit(planes_prep_k<T, KD>, Prep<KD>::bytes)));
     Maps m{};
     if (!make_maps(a, m)) return cudaErrorInvalidValue;
     planes_prep_k<T, KD><<<dim3(a.n, a.Hv, a.B), 128, Prep<KD>::bytes, s>>>(a, m);
     note_launch();
-    PLANES_TRY(cudaGetLastError());
+    DELTA_TRY(cudaGetLastError());
     return chain<T, KD>(a, m, false, s);
 }
 
 template <typename T, int KD>
 cudaError_t bwd(const DArgs& a, float* group, cudaStream_t s) {
-    PLANES_TRY((smem_limit(planes_grad_k<T, KD>, Grad<KD>::bytes)));
+    DELTA_TRY((smem_limit(planes_grad_k<T, KD>, Grad<KD>::bytes)));
     Maps m{};
     if (!make_maps(a, m)) return cudaErrorInvalidValue;
-    PLANES_TRY((chain<T, KD>(a, m, true, s)));
+    DELTA_TRY((chain<T, KD>(a, m, true, s)));
     const int items = a.B * a.Hk * a.n;
     planes_grad_k<T, KD><<<items < kSms ? items : kSms, 32 * kGradWarps, Grad<KD>::bytes, s>>>(a, group, m);
     note_launch();

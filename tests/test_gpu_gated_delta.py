@@ -662,3 +662,87 @@ def test_float32_gradients_of_16_bit_tokens(dtype, shape):
     for n in ("dg", "dbeta", "dinitial"):
         err, ref = float((got[n].double().cpu() - want[n]).norm()), float(want[n].norm())
         assert got[n].dtype == torch.float32 and err <= TOL * ref, (n, err / ref)
+
+
+def test_lengths_and_resets_in_float16():
+    test_lengths(torch.float16)
+    test_resets_zero_and_double_rates(torch.float16)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("K,V", [(64, 48), (128, 128)])
+def test_lengths_and_resets_without_gradients(dtype, K, V):
+    """The forward that keeps nothing: rows of any length with NaN and infinities behind them, resets, rates of 0 and 2."""
+    lengths = [0, 1, 64, 100, 130, 500, -3]
+    d, _, _ = make(len(lengths), 130, 1, 2, K, V, dtype, seed=48)
+    d["g"][:, 20], d["g"][:, 100, 0], d["g"][:, 30:60] = float("-inf"), -60.0, 0.0
+    d["beta"][:, 10:14], d["beta"][:, 50], d["beta"][:, 51] = 0.0, 2.0, -0.5
+    dev = torch.tensor(lengths, dtype=torch.int32, device=DEV)
+
+    def run():
+        return gated_delta_rule(*(d[n] for n in ("q", "k", "v", "g", "beta")), initial_state=d["initial"], output_final_state=True,
+                                lengths=dev)
+    o, S = run()
+    x = [d[n].double().cpu() for n in ("q", "k", "v", "g", "beta")]
+    o64, S64 = oracle(*x, K ** -0.5, d["initial"].double().cpu(), dev.cpu())
+    close(o, o64)
+    close(S, S64)
+    for i, n in enumerate(lengths):
+        n = min(max(n, 0), 130)
+        assert float(o[i, n:].abs().sum()) == 0.0
+        if n == 0:
+            assert torch.equal(S[i], d["initial"][i])
+        for name in ("q", "k", "v", "g", "beta"):
+            d[name][i, n:] = float("nan") if i % 2 else float("inf")
+    again = run()
+    assert torch.equal(o, again[0]) and torch.equal(S, again[1])
+
+
+def test_without_gradients_on_another_stream_and_in_a_graph():
+    d, _, _ = make(2, 200, 2, 4, 128, 128, torch.float16, seed=49)
+    call = lambda: gated_delta_rule(*(d[n] for n in ("q", "k", "v", "g", "beta")), initial_state=d["initial"], output_final_state=True)
+    want = call()
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        side = call()
+    s.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(side, want))
+    del side
+    gr = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(gr):
+        out = call()
+    d["v"].mul_(1e-4)
+    d["initial"].mul_(1e5)
+    want = call()
+    gr.replay()
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(out, want))
+    with torch.inference_mode():
+        got = call()
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+@pytest.mark.parametrize("name", ["q", "k", "v", "g", "beta", "initial"])
+def test_each_gradient_against_differences(name):
+    """Each input by itself, f = <o, do> + <S, dS>, fourth-order differences of the kernel's forward along the input's own
+    gradient, a tenth of the input's size.  float32 operands keep 22 bits and not 16, which leaves 2^-6 of TOL; with the
+    float32 sums 2^-4.  A forward off by that much of |o| |do| + |S| |dS| moves the slope by 18 / 12 of it over h = 2^-4.
+    Truncation is h^4 / 30 = 5e-7 of a fifth derivative, less than a tenth of that."""
+    d, do, dS = make(1, 80, 1, 2, 64, 64, torch.float32, seed=44)
+
+    def run(x):
+        return gated_delta_rule(*(x[n] for n in ("q", "k", "v", "g", "beta")), initial_state=x["initial"], output_final_state=True)
+    x = d[name].clone().requires_grad_(True)
+    o, S = run({**d, name: x})
+    grad = torch.autograd.grad([o, S], x, [do, dS])[0].double()
+    way = (0.1 * d[name].double().norm() / grad.norm() * grad).float()
+
+    def f(s):
+        o, S = run({**d, name: d[name] + s * way})
+        return float((o.double() * do.double()).sum() + (S.double() * dS.double()).sum())
+    slope, h = float((grad * way.double()).sum()), 2.0 ** -4
+    num = (8 * (f(h) - f(-h)) - (f(2 * h) - f(-2 * h))) / (12 * h)
+    size = float(o.detach().norm() * do.norm() + S.detach().norm() * dS.norm())
+    allowed = 1.5 * TOL / 16 * size / h
+    assert abs(num - slope) <= allowed and slope > 10 * allowed, (num, slope, allowed)
