@@ -265,13 +265,18 @@ template <> __device__ __forceinline__ void load8<__nv_bfloat16>(const __nv_bflo
 // S^T (16 value rows v0.., K columns) of a (K, V) float32 state, or zeros
 template <int KD>
 __device__ __forceinline__ void state_load(float (*S)[4], const float* p, int K, int V, int v0, const Lane& L) {
+    if (p) {
 #pragma unroll
-    for (int j = 0; j < KD / 8; ++j)
+        for (int j = 0; j < KD / 8; ++j)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            const int k = 8 * j + 2 * L.t + (e & 1), v = v0 + L.g + (e >> 1) * 8;
-            S[j][e] = p && k < K && v < V ? p[static_cast<int64_t>(k) * V + v] : 0.f;
-        }
+            for (int e = 0; e < 4; ++e) {
+                const int k = 8 * j + 2 * L.t + (e & 1), v = v0 + L.g + (e >> 1) * 8;
+                S[j][e] = k < K && v < V ? p[static_cast<int64_t>(k) * V + v] : 0.f;
+            }
+    } else {
+#pragma unroll
+        for (int j = 0; j < KD / 8; ++j) S[j][0] = S[j][1] = S[j][2] = S[j][3] = 0.f;
+    }
 }
 template <int KD>
 __device__ __forceinline__ void state_store(const float (*S)[4], float* p, int K, int V, int v0, const Lane& L) {
