@@ -152,7 +152,8 @@ EACS_API int eacs_delta_path(const EacsDelta* p, int training);
  * the 16-bit kernels, two values of the inputs' type (bfloat16 16 bits; float16
  * 22 bits of the largest value of a tile, which is brought into its range by a
  * power of two); all sums and the state are float32.  With training, beta is
- * held 2^-64 away from 0. */
+ * held 2^-64 away from 0.  A NaN or an infinity of a token also reaches the
+ * tokens before it in its block of 16. */
 EACS_API int eacs_delta_fwd(const EacsDelta* p, void* o, float* final_state, void* workspace, size_t workspace_bytes,
                             int training, void* stream);
 EACS_API size_t eacs_delta_workspace_size(const EacsDelta* p, int training);

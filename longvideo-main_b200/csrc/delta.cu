@@ -42,8 +42,8 @@
 // not (rows that do not start on 16 bytes, expanded dimensions, float16 training:
 // B=2 L=4096 H=12 K=V=64 forward and backward 2.4 ms).  Operands are
 // tf32 split in two (22 bits), three products each: errors are 3e-7 to 5e-7 of
-// the norm.  Times at B=4 L=9498 H=10 K=128 V=64, float32: delta_prep_k 162 us,
-// delta_chain_k 1648, delta_out_k 446, delta_rchain_k 2986, delta_grad_k 1072.
+// the norm.  Times at B=4 L=9498 H=10 K=128 V=64, float32: delta_prep_k 248 us,
+// delta_chain_k 1650, delta_out_k 662, delta_rchain_k 2980, delta_grad_k 1594.
 // The chains are bound by a chunk's dependent products on one warp of each
 // scheduler (11 and 20 us a chunk), the others by the products and the
 // splitting of every tile as it is read.
@@ -920,7 +920,8 @@ __global__ void __launch_bounds__(256) delta_grad_k(DArgs a, float* group) {
 // key row, in registers from the first token to the last.  k^T S' and q^T S'
 // are summed together, as o = q^T S' + (q.k) u; one token is one pass over the
 // state: read once, written once.
-// Bound by the state's bytes; what counts is how many of them are under way, so
+// Bound by the state's bytes, of which a CTA has none under way while it adds up,
+// and by the last round of CTAs (64 rows of 16 heads: 4096 on 1184 places): so
 // eight CTAs share a multiprocessor (K = 128, 64 rows of 16 heads: 29.0 us, 4.6
 // TB/s, against 33.3 with the five that 82 registers a thread allow; 16 rows 6.7
 // us against 7.9; six or ten CTAs, 64 or 128 columns a CTA were no faster).

@@ -4,9 +4,10 @@
 // The formulas are those of delta.cu.  Here every product runs on 16-bit
 // operands of the inputs' type: the inputs are exact in it, and a float32
 // result that goes back in as an operand is split into two planes of it,
-// x = hi + lo (16 significant bits in bfloat16, 22 in float16), or rounded to
-// one where a term's rounding stays below the output's own (said where it is
-// done).  With one plane everywhere dg was off by 5e-3 of its norm.
+// x = hi + lo (16 significant bits in bfloat16, 22 in float16).  With one plane
+// everywhere dg was off by 5e-3 of its norm.  A NaN or an infinity of a token
+// spreads over its block of 16 tokens, as what lies above a triangle's diagonal
+// there is multiplied by 0.
 //
 // float16's exponent is too short for this by itself: below 2^-3 the low plane
 // runs out.  There T' and M, S, X and U are scaled by powers of two (Scaled
@@ -18,13 +19,13 @@
 //
 // The kernels, with times at B=4 L=16384 H=8 (forward) and B=8 L=8192 H=6
 // (training), K = V = 128, bfloat16:
-//   planes_prep_k    per chunk: gam, d, T' and M            145 us; 112 us
-//   planes_chain_k   the chunks in order: S, U and the outputs  598 us; 519 us
-//   planes_rchain_k  the chunks in reverse order: dV and dS     445 us
-//   planes_grad_k    per chunk: dQ, dK, dbeta, dg               797 us
+//   planes_prep_k    per chunk: gam, d, T' and M            141 us; 112 us
+//   planes_chain_k   the chunks in order: S, U and the outputs  650 us; 568 us
+//   planes_rchain_k  the chunks in reverse order: dV and dS     471 us
+//   planes_grad_k    per chunk: dQ, dK, dbeta, dg               873 us
 //
-// The two chains are bound by the length of one chunk's dependent products (2.3
-// us each; 256 chunks of a head follow one another), as only 16-column groups
+// The two chains are bound by the length of one chunk's dependent products (2.4
+// to 2.8 us each; 256 chunks of a head follow one another), as only 16-column groups
 // of a state run side by side (a warp each, 8 a head of 128): so everything
 // that does not depend on the state is taken out of the warp that carries it.
 // A CTA holds G such warps, one or more helpers (the forward's outputs; the

@@ -29,16 +29,21 @@ def on(dev: torch.device):
     return contextlib.nullcontext() if torch.cuda.current_device() == dev.index else torch.cuda.device(dev)
 
 
+_tracing, _transforms = torch._C._get_tracing_state, torch._C._functorch.peek_interpreter_stack
+
+
 def is_plain(*ts: torch.Tensor | None) -> bool:
     """Whether these are tensors whose values alone are asked for: none has a
     forward-mode tangent, none belongs to a torch.func transform, and nothing
     is being traced.  Kernels called by pointer see the values only; what would
     have to be carried along or recorded would be lost."""
-    if forward_ad._current_level >= 0 and any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in ts):
+    if forward_ad._current_level < 0 and _tracing() is None and _transforms() is None:
+        return True
+    if any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in ts):
         return False
     if torch.compiler.is_compiling():  # (whose graph ends where the kernel is called)
         return True
-    return not torch.jit.is_tracing() and torch._C._functorch.peek_interpreter_stack() is None
+    return _tracing() is None and _transforms() is None
 
 
 def require_plain(name: str, *ts: torch.Tensor | None) -> None:
