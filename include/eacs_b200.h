@@ -114,9 +114,8 @@ EACS_API size_t eacs_layer_norm_bwd_workspace_size(int64_t rows, int64_t d);
  * initial_state (B,Hv,K,V) float32 dense or NULL (zeros).  K goes up to 128,
  * V to 1024.  Rows of q, k, v that start on 16 bytes, with K and V multiples
  * of 8, are read 16 bytes at a time; 16-bit inputs of that kind (no dimension
- * of more than one element having stride 0) take the fastest kernels, bfloat16
- * always, float16 where no backward follows.  Which kernels run (`path` 0)
- * goes by the pointers' alignment and the strides, and so do the workspace
+ * of more than one element having stride 0) take the fastest kernels.  Which
+ * kernels run (`path` 0) goes by the pointers' alignment and the strides, and so do the workspace
  * sizes and what a workspace holds: ask for the sizes with the arguments of the
  * call.  A backward whose inputs may have moved since the forward names the
  * forward's path. */
@@ -142,8 +141,8 @@ typedef struct EacsDelta {
     int32_t path;
 } EacsDelta;
 
-/* The path that a forward with these arguments takes, or 0 if they are refused. */
-EACS_API int eacs_delta_path(const EacsDelta* p, int training);
+/* The path that a call with these arguments takes, or 0 if they are refused. */
+EACS_API int eacs_delta_path(const EacsDelta* p);
 
 /* Chunked forward: o (B,L,Hv,V) dense of dtype, on 16 bytes; final_state (B,Hv,K,V)
  * float32 or NULL.  With training != 0 the workspace holds what
@@ -163,7 +162,7 @@ EACS_API size_t eacs_delta_workspace_size(const EacsDelta* p, int training);
  * 16 bytes (dq and dk summed over the value heads of a key head), dg and dbeta dense
  * of gate_dtype, dinitial (B,Hv,K,V) float32 or NULL.  `saved` is the
  * workspace of the training forward with the same arguments.  Where q, k and v
- * are bfloat16 and read 16 bytes at a time, dout's rows have to start on 16
+ * are 16-bit and read 16 bytes at a time, dout's rows have to start on 16
  * bytes too, without a stride of 0. */
 EACS_API int eacs_delta_bwd(const EacsDelta* p, const void* dout, const int64_t* dout_stride, const float* dfinal,
                             void* dq, void* dk, void* dv, void* dg, void* dbeta, float* dinitial, const void* saved,

@@ -105,7 +105,7 @@ int eacs_layer_norm_bwd(const void* x, int64_t x_stride, const void* residual, i
     return eacs::layer_norm(c, static_cast<cudaStream_t>(stream));
 }
 
-int eacs_delta_path(const EacsDelta* p, int training) { return p ? eacs::delta_path(*p, training != 0) : 0; }
+int eacs_delta_path(const EacsDelta* p) { return p ? eacs::delta_path(*p) : 0; }
 
 size_t eacs_delta_workspace_size(const EacsDelta* p, int training) {
     return p ? eacs::delta_workspace_size(*p, training != 0) : 0;

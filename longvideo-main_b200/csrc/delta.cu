@@ -39,10 +39,9 @@
 // shuffle or a barrier between them.
 //
 // These kernels take float32 inputs, and 16-bit ones that delta_planes.cu does
-// not (rows that do not start on 16 bytes, expanded dimensions, float16 training:
-// B=2 L=4096 H=12 K=V=64 forward and backward 2.4 ms).  Operands are
-// tf32 split in two (22 bits), three products each: errors are 3e-7 to 5e-7 of
-// the norm.  Times at B=4 L=9498 H=10 K=128 V=64, float32: delta_prep_k 248 us,
+// not (rows that do not start on 16 bytes, expanded dimensions); delta_grad_k
+// takes float16 from there too.  Operands are tf32 split in two (22 bits), three
+// products each: errors are 3e-7 to 5e-7 of the norm.  Times at B=4 L=9498 H=10 K=128 V=64, float32: delta_prep_k 248 us,
 // delta_chain_k 1650, delta_out_k 662, delta_rchain_k 2980, delta_grad_k 1594.
 // The chains are bound by a chunk's dependent products on one warp of each
 // scheduler (11 and 20 us a chunk), the others by the products and the
@@ -1090,12 +1089,17 @@ cudaError_t run_fwd(const DArgs& a, cudaStream_t s) {
 }
 
 template <class F, typename T, int KD>
-cudaError_t run_bwd(const DArgs& a, float* group, cudaStream_t s) {
-    DELTA_TRY((run_chain<F, T, KD>(a, true, s)));
+cudaError_t run_grad(const DArgs& a, float* group, cudaStream_t s) {
     DELTA_TRY(smem_limit(delta_grad_k<F, T, KD>, GradSmem<F, KD>::bytes));
     delta_grad_k<F, T, KD><<<dim3(a.n, a.Hk, a.B), 256, GradSmem<F, KD>::bytes, s>>>(a, group);
     note_launch();
     return cudaGetLastError();
+}
+
+template <class F, typename T, int KD>
+cudaError_t run_bwd(const DArgs& a, float* group, cudaStream_t s) {
+    DELTA_TRY((run_chain<F, T, KD>(a, true, s)));
+    return run_grad<F, T, KD>(a, group, s);
 }
 
 template <typename T>
@@ -1169,25 +1173,22 @@ bool mapped(int64_t B, int64_t L, int64_t H, const int64_t* st) {
         if (n[i] > 1 && (st[i] <= 0 || st[i] >= int64_t{1} << 39)) return false;
     return true;
 }
-// Whether the 16-bit kernels take these inputs: bfloat16, and float16 where no
-// backward follows.  float16's exponent is too short for what a backward keeps
-// and divides (a rate of 1e-4 left 8 bits of dbeta, one of 0 none), so its
-// training runs in tf32.  The backward goes by the forward's path, or by its inputs
-// alone, as it reads what the forward left (an upstream gradient in another layout is
-// refused by delta_bwd then).
-bool planes_take(const EacsDelta& p, const DArgs& a, bool training) {
-    return (p.dtype == EACS_DTYPE_BF16 || (p.dtype == EACS_DTYPE_F16 && !training)) && a.vec_qk && a.vec_v &&
-           mapped(p.B, p.L, p.Hk, p.q_stride) && mapped(p.B, p.L, p.Hk, p.k_stride) && mapped(p.B, p.L, p.Hv, p.v_stride);
+// Whether the 16-bit kernels take these inputs.  The backward goes by the
+// forward's path, or by its inputs alone, as it reads what the forward left (an
+// upstream gradient in another layout is refused by delta_bwd then).
+bool planes_take(const EacsDelta& p, const DArgs& a) {
+    return p.dtype != EACS_DTYPE_F32 && a.vec_qk && a.vec_v && mapped(p.B, p.L, p.Hk, p.q_stride) &&
+           mapped(p.B, p.L, p.Hk, p.k_stride) && mapped(p.B, p.L, p.Hv, p.v_stride);
 }
 // The path of a call: the caller's, or the one that its inputs lead to.
-bool planes(const EacsDelta& p, const DArgs& a, bool training) {
-    return p.path == 0 ? planes_take(p, a, training) : p.path == EACS_DELTA_PATH_16;
+bool planes(const EacsDelta& p, const DArgs& a) {
+    return p.path == 0 ? planes_take(p, a) : p.path == EACS_DELTA_PATH_16;
 }
 
-int check_delta(const EacsDelta& p, const char* fn, bool training) {
+int check_delta(const EacsDelta& p, const char* fn) {
     if (int rc = check_sizes(p, fn)) return rc;
     if (p.path < 0 || p.path > EACS_DELTA_PATH_16) return fail(EACS_ERR_INVALID, "%s: unknown path %d", fn, p.path);
-    if (p.path == EACS_DELTA_PATH_16 && !planes_take(p, make_args(p), training))
+    if (p.path == EACS_DELTA_PATH_16 && !planes_take(p, make_args(p)))
         return fail(EACS_ERR_INVALID, "%s: the 16-bit kernels do not take these inputs", fn);
     return EACS_OK;
 }
@@ -1196,7 +1197,7 @@ struct Sizes { size_t gates, T, M, S, U, total; };
 Sizes fwd_sizes(const EacsDelta& p, const DArgs& a, bool training) {
     const size_t ids = static_cast<size_t>(p.B) * p.Hv * chunks(p.L), e = sizeof(float);
     Sizes z{};
-    if (planes(p, a, training)) {
+    if (planes(p, a)) {
         z.total = planes_saved_size(a, training);
         return z;
     }
@@ -1212,7 +1213,7 @@ struct BSizes { size_t dS, dV, group, total; };
 BSizes bwd_sizes(const EacsDelta& p, const DArgs& a) {
     const size_t ids = static_cast<size_t>(p.B) * p.Hv * chunks(p.L), e = sizeof(float);
     BSizes z{};
-    if (planes(p, a, true)) {
+    if (planes(p, a)) {
         z.dS = align256(planes_bwd_size(a));
     } else {
         z.dS = align256(ids * pad16(p.V) * key_pad(p.K) * e);
@@ -1243,23 +1244,23 @@ bool on16(std::initializer_list<const void*> ps) {
 
 }  // namespace
 
-int delta_path(const EacsDelta& p, bool training) {
-    if (check_delta(p, "eacs_delta_path", training) != EACS_OK) return 0;
-    return planes(p, make_args(p), training) ? EACS_DELTA_PATH_16 : EACS_DELTA_PATH_GENERAL;
+int delta_path(const EacsDelta& p) {
+    if (check_delta(p, "eacs_delta_path") != EACS_OK) return 0;
+    return planes(p, make_args(p)) ? EACS_DELTA_PATH_16 : EACS_DELTA_PATH_GENERAL;
 }
 size_t delta_workspace_size(const EacsDelta& p, bool training) {
-    if (check_delta(p, "eacs_delta_workspace_size", training) != EACS_OK) return 0;
+    if (check_delta(p, "eacs_delta_workspace_size") != EACS_OK) return 0;
     return fwd_sizes(p, make_args(p), training).total;
 }
 size_t delta_bwd_workspace_size(const EacsDelta& p) {
-    if (check_delta(p, "eacs_delta_bwd_workspace_size", true) != EACS_OK) return 0;
+    if (check_delta(p, "eacs_delta_bwd_workspace_size") != EACS_OK) return 0;
     return bwd_sizes(p, make_args(p)).total;
 }
 
 int delta_fwd(const EacsDelta& p, void* o, float* final_state, void* ws, size_t ws_bytes, bool training,
               cudaStream_t stream) {
     const char* fn = "eacs_delta_fwd";
-    if (int rc = check_delta(p, fn, training)) return rc;
+    if (int rc = check_delta(p, fn)) return rc;
     const size_t state = static_cast<size_t>(p.B) * p.Hv * p.K * p.V * sizeof(float);
     if (p.B == 0) return EACS_OK;
     if (p.L == 0) {  // no token: the state stays
@@ -1279,7 +1280,7 @@ int delta_fwd(const EacsDelta& p, void* o, float* final_state, void* ws, size_t 
     a.out = o;
     a.final_state = final_state;
     cudaError_t e;
-    if (planes(p, a, training))
+    if (planes(p, a))
         e = planes_fwd(a, ws, training, stream);
     else if (p.dtype == EACS_DTYPE_BF16)
         e = p.K <= 64 ? run_fwd<FmtF<true>, __nv_bfloat16, 64>(a, stream) : run_fwd<FmtF<true>, __nv_bfloat16, 128>(a, stream);
@@ -1308,7 +1309,7 @@ int delta_step(const EacsDelta& p, void* o, float* final_state, cudaStream_t str
 int delta_bwd(const EacsDelta& p, const DeltaGrads& d, const void* saved, size_t saved_bytes, void* ws, size_t ws_bytes,
               cudaStream_t stream) {
     const char* fn = "eacs_delta_bwd";
-    if (int rc = check_delta(p, fn, true)) return rc;
+    if (int rc = check_delta(p, fn)) return rc;
     const size_t state = static_cast<size_t>(p.B) * p.Hv * p.K * p.V * sizeof(float);
     if (p.B == 0) return EACS_OK;
     if (p.L == 0) {
@@ -1334,7 +1335,7 @@ int delta_bwd(const EacsDelta& p, const DeltaGrads& d, const void* saved, size_t
     a.dq = d.dq; a.dk = d.dk; a.dv = d.dv; a.dg = d.dg; a.dbeta = d.dbeta;
     a.dfinal = d.dfinal;
     a.dinitial = d.dinitial;
-    if (planes(p, a, true) && !(a.vec_do && mapped(p.B, p.L, p.Hv, d.dout_stride)))
+    if (planes(p, a) && !(a.vec_do && mapped(p.B, p.L, p.Hv, d.dout_stride)))
         return fail(EACS_ERR_INVALID, "%s: rows of dout must start on 16 bytes, with strides above 0, where those of q, k and v do", fn);
     const BSizes z = bwd_sizes(p, a);
     char* w = static_cast<char*>(ws);
@@ -1342,9 +1343,11 @@ int delta_bwd(const EacsDelta& p, const DeltaGrads& d, const void* saved, size_t
     a.dV = w; w += z.dV;
     float* group = reinterpret_cast<float*>(w);
     cudaError_t e;
-    if (planes(p, a, true))
+    if (planes(p, a)) {
         e = planes_bwd(a, const_cast<void*>(saved), ws, group, stream);
-    else if (p.dtype == EACS_DTYPE_BF16)
+        if (e == cudaSuccess && a.half)
+            e = p.K <= 64 ? run_grad<FmtF<true>, __half, 64>(a, group, stream) : run_grad<FmtF<true>, __half, 128>(a, group, stream);
+    } else if (p.dtype == EACS_DTYPE_BF16)
         e = p.K <= 64 ? run_bwd<FmtF<true>, __nv_bfloat16, 64>(a, group, stream) : run_bwd<FmtF<true>, __nv_bfloat16, 128>(a, group, stream);
     else if (p.dtype == EACS_DTYPE_F16)
         e = p.K <= 64 ? run_bwd<FmtF<true>, __half, 64>(a, group, stream) : run_bwd<FmtF<true>, __half, 128>(a, group, stream);

@@ -197,13 +197,13 @@ struct DArgs {
     float* dinitial;       // or null
     int B, L, Hk, Hv, K, V, n, Vp;  // n chunks, Vp = V rounded up to 16
     int gate_dtype;
-    int half;  // q, k, v: float16 (delta_planes.cu)
+    int half;  // q, k, v: float16
     int vec_qk, vec_v, vec_do;  // rows can be read 16 bytes at a time
     float scale;
     // workspace, per chunk id ((b Hv + h) n + c)
-    float* gates;  // [id][6][64]: G (high), G (low), gam, d, scale gam, 1 / beta (delta_planes.cu; there with
-                   // float16: beta, what T' and M are to be multiplied by, gam, d, scale gam)
+    float* gates;  // [id][6][64]: G (high), G (low), gam, d, scale gam, 1 / beta (delta_planes.cu; with float16 beta)
     void* T;       // [id][planes][64][64]
+    void* Tr;      // (float16 training, delta_planes.cu) the reverse chain's
     void* M;       // [id][64][64] or null
     void* S;       // [id][Vp][KD]: S0^T or null
     void* U;       // [id][64][Vp]
@@ -300,11 +300,12 @@ cudaError_t smem_limit(K kernel, size_t bytes) {
         if (e_ != cudaSuccess) return e_;     \
     } while (0)
 
-// delta_planes.cu: bfloat16 inputs whose rows start on 16 bytes, and float16 ones without a backward
+// delta_planes.cu: 16-bit inputs whose rows start on 16 bytes
 size_t planes_saved_size(const DArgs& a, bool training);
 size_t planes_bwd_size(const DArgs& a);
 cudaError_t planes_fwd(DArgs a, void* ws, bool training, cudaStream_t s);
-cudaError_t planes_bwd(DArgs a, void* saved, void* ws, float* group, cudaStream_t s);
+// float16: up to dS and dV, which are set in `a` with what the forward kept
+cudaError_t planes_bwd(DArgs& a, void* saved, void* ws, float* group, cudaStream_t s);
 cudaError_t planes_read_status(int* out, cudaStream_t s);
 
 }  // namespace eacs

@@ -1,5 +1,4 @@
-// delta_planes.cu -- the gated delta rule on bfloat16 inputs, and the forward pass
-// without a backward on float16 ones (sm_100a).
+// delta_planes.cu -- the gated delta rule on bfloat16 and float16 inputs (sm_100a).
 //
 // The formulas are those of delta.cu.  Here every product runs on 16-bit
 // operands of the inputs' type: the inputs are exact in it, and a float32
@@ -10,12 +9,14 @@
 // there is multiplied by 0.
 //
 // float16's exponent is too short for this by itself: below 2^-3 the low plane
-// runs out.  There T' and M, S, X and U are scaled by powers of two (Scaled
-// below), and T' is made without beta: with Ahat_ij = Gam_ij k_i.k_j (j < i) and
-// D = diag(beta), e = (I + Ahat D)^-1 X and U = D e, so that a small beta meets
-// float32 only (B=3 L=1001 H=8 K=64 V=96: 51 us with it, 43 without).  What a
-// backward keeps and multiplies (S, U, dS and dV of all groups in one sum) would
-// need scales of its own, so float16 training runs on the kernels of delta.cu.
+// runs out.  There T' and M, S, X and U, dS and dU are scaled by powers of two
+// (Scaled below), and T' is made without beta: with Ahat_ij = Gam_ij k_i.k_j
+// (j < i) and D = diag(beta), e = (I + Ahat D)^-1 X and U = D e, and in reverse
+// dV = D (I + D Ahat)^-T dU, so that a small beta meets float32 only (forward at
+// B=3 L=1001 H=8 K=64 V=96: 49 us with it, 43 without).  What a backward keeps and
+// multiplies (S, U, dS and dV, of all groups in one sum) is stored in float32 and
+// goes to delta_grad_k of delta.cu (B=2 L=4096 H=12 K=V=64, forward and backward:
+// 52 + 166 + 171 + 263 us; 2400 with everything there).
 //
 // The kernels, with times at B=4 L=16384 H=8 (forward) and B=8 L=8192 H=6
 // (training), K = V = 128, bfloat16:
@@ -333,10 +334,10 @@ __device__ __forceinline__ float ratio(const float* G, int i, int j) {
 // ----------------------------------------------------------------------------
 // gates, T' and M of a chunk
 // ----------------------------------------------------------------------------
-// Two warps make M and two A (float16: Ahat D), of each one block rows 3 and 0 (of 16 tokens), the
-// other 2 and 1: five 16 x 16 blocks each.  Blocks above the diagonal are neither
-// made nor written, as no product reads them.  The latter two then invert I + A by
-// blocks, in float32: the 16 x 16 blocks on the diagonal by forward substitution (a
+// Two warps make M and two A (float16: Ahat D), of each one block rows 3 and 0 (of
+// 16 tokens), the other 2 and 1: five 16 x 16 blocks each.  Blocks above the
+// diagonal are neither made nor written, as no product reads them.  The latter two
+// then invert I + A by blocks, in float32: the 16 x 16 blocks on the diagonal by forward substitution (a
 // thread a column), then twice the step from blocks of s to blocks of 2 s,
 // [[P, 0], [R, Q]]^-1 = [[P^-1, 0], [-Q^-1 R P^-1, Q^-1]], whose products run on the
 // tensor cores with operands split in two tf32 parts.  (Forward substitution alone
@@ -346,6 +347,10 @@ __device__ __forceinline__ float ratio(const float* G, int i, int j) {
 constexpr int kAld = kC + 8;  // float32 tiles
 
 __device__ __forceinline__ void sync_inverse() { asm volatile("bar.sync 1, 64;" ::: "memory"); }
+
+// What a scaled tile is to be multiplied by lies behind its first row.
+__device__ __forceinline__ float tile_unit(const e16* tile) { return *reinterpret_cast<const float*>(tile + kC); }
+__device__ __forceinline__ void set_tile_unit(e16* tile, int e) { *reinterpret_cast<float*>(tile + kC) = pow2(-e); }
 
 template <int KD>
 struct Prep {
@@ -369,7 +374,7 @@ __global__ void __launch_bounds__(128) planes_prep_k(const __grid_constant__ DAr
     float* sA = reinterpret_cast<float*>(smem);  // A below the diagonal blocks, products above (after K and Q)
     float* sT = sA + kC * kAld;                  // its inverse
     __shared__ float sG[2 * kC], sB[kC];
-    __shared__ uint32_t sMax[4];
+    __shared__ uint32_t sMax[2][4];
     __shared__ uint64_t land;
     const int tid = threadIdx.x, warp = tid >> 5;
     const Lane L;
@@ -415,8 +420,12 @@ __global__ void __launch_bounds__(128) planes_prep_k(const __grid_constant__ DAr
             const float gam = exp2f(static_cast<float>(G));
             sG[r] = hi;
             sG[kC + r] = lo;
-            if constexpr (Scaled<T>) {  // (no backward reads G)
-                ga[r] = sB[r];
+            if constexpr (Scaled<T>) {
+                const double Ge = G * 0.6931471805599453;  // as the gradients' kernel takes it
+                const float h = static_cast<float>(Ge);
+                ga[r] = h;
+                ga[kC + r] = static_cast<float>(Ge - h);
+                ga[5 * kC + r] = sB[r];
             } else {
                 ga[r] = hi;
                 ga[kC + r] = lo;
@@ -500,17 +509,17 @@ __global__ void __launch_bounds__(128) planes_prep_k(const __grid_constant__ DAr
             }
         }
     }
-    // The largest value of the two warps of a tile; `bar`: theirs
-    auto pair_scale = [&](uint32_t bits, int bar) {
-        if (L.l == 0) sMax[warp] = bits;
+    // From the largest value of the two warps of a tile; `bar`: theirs, `slot`: of the tile
+    auto pair_scale = [&](uint32_t bits, int bar, int slot) {
+        if (L.l == 0) sMax[slot][warp] = bits;
         asm volatile("bar.sync %0, 64;" ::"r"(bar) : "memory");
-        return scale_exp(max(sMax[warp & 2], sMax[warp | 1]));
+        return scale_exp(max(sMax[slot][warp & 2], sMax[slot][warp | 1]));
     };
     if constexpr (Scaled<T>) {
         if (!left) {
-            const int e = pair_scale(max_bits<10>(&x[0][0]), 2);
+            const int e = pair_scale(max_bits<10>(&x[0][0]), 2, 0);
             scale_tile<10>(&x[0][0], pow2(e));
-            if (tid == 0) ga[kC + 1] = pow2(-e);
+            if (tid == 0) set_tile_unit(M, e);
 #pragma unroll
             for (int i = 0; i < 5; ++i)
 #pragma unroll
@@ -583,43 +592,67 @@ __global__ void __launch_bounds__(128) planes_prep_k(const __grid_constant__ DAr
         }
     }
     sync_inverse();
-    e16* to = static_cast<e16*>(a.T) + id * 2 * kCC;
-    float ft = 1.f;
     auto at_block = [&](int i, int& r, int& c8) {  // ten blocks of 16 rows by two vectors of 8
         const int at = i * 64 + u, blk = at >> 5, r16 = (at & 31) >> 1;
         const int rb = blk >= 6 ? 3 : blk >= 3 ? 2 : blk >= 1 ? 1 : 0, cb = blk - rb * (rb + 1) / 2;
         r = 16 * rb + r16;
         c8 = 16 * cb + (at & 1) * 8;
     };
-    if constexpr (Scaled<T>) {
-        float m = 0.f;
+    auto put_t = [&](e16* to, auto pair) {  // pair(row, column): of columns column, column + 1
 #pragma unroll
         for (int i = 0; i < 5; ++i) {
             int r, c8;
             at_block(i, r, c8);
+            uint32_t hi[4], lo[4];
 #pragma unroll
-            for (int e = 0; e < 8; ++e) m = fmaxf(m, fabsf(sT[r * kAld + c8 + e]));
+            for (int e = 0; e < 4; ++e) {
+                const float2 v = pair(r, c8 + 2 * e);
+                hi[e] = Num<T>::pack(v.x, v.y);
+                const float2 f = Num<T>::unpack(hi[e]);
+                lo[e] = Num<T>::pack(v.x - f.x, v.y - f.y);
+            }
+            *reinterpret_cast<uint4*>(to + r * kTld + c8) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+            *reinterpret_cast<uint4*>(to + kCC + r * kTld + c8) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
         }
-        const int e = pair_scale(__reduce_max_sync(0xffffffffu, abs_bits(m)), 1);
-        ft = pow2(e);
-        if (u == 0) ga[kC] = pow2(-e);
-    }
+    };
+    e16* to = static_cast<e16*>(a.T) + id * 2 * kCC;
+    auto inverse = [&](int r, int c) { return *reinterpret_cast<const float2*>(sT + r * kAld + c); };
+    if constexpr (Scaled<T>) {
+        auto put_scaled = [&](e16* t, int slot, auto pair) {
+            float m = 0.f;
 #pragma unroll
-    for (int i = 0; i < 5; ++i) {
-        int r, c8;
-        at_block(i, r, c8);
-        uint32_t hi[4], lo[4];
+            for (int i = 0; i < 5; ++i) {
+                int r, c8;
+                at_block(i, r, c8);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            const float2 v = *reinterpret_cast<const float2*>(sT + r * kAld + c8 + 2 * e);
-            const float2 w = Scaled<T> ? make_float2(ft, ft) : *reinterpret_cast<const float2*>(sB + c8 + 2 * e);
-            const float p = v.x * w.x, q = v.y * w.y;
-            hi[e] = Num<T>::pack(p, q);
-            const float2 f = Num<T>::unpack(hi[e]);
-            lo[e] = Num<T>::pack(p - f.x, q - f.y);
-        }
-        *reinterpret_cast<uint4*>(to + r * kTld + c8) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
-        *reinterpret_cast<uint4*>(to + kCC + r * kTld + c8) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+                for (int e = 0; e < 8; e += 2) {
+                    const float2 v = pair(r, c8 + e);
+                    m = fmaxf(m, fmaxf(fabsf(v.x), fabsf(v.y)));
+                }
+            }
+            const int e = pair_scale(__reduce_max_sync(0xffffffffu, abs_bits(m)), 1, slot);
+            const float f = pow2(e);
+            put_t(t, [&](int r, int c) {
+                const float2 v = pair(r, c);
+                return make_float2(v.x * f, v.y * f);
+            });
+            if (u == 0) set_tile_unit(t, e);
+        };
+        put_scaled(to, 0, inverse);
+        // (I + D Ahat)^-1 = D (I + Ahat D)^-1 D^-1 for the reverse chain (on the diagonal both have 1)
+        if (a.Tr)
+            put_scaled(static_cast<e16*>(a.Tr) + id * 2 * kCC, 1, [&](int r, int c) {
+                float2 v = inverse(r, c);
+                const float2 w = *reinterpret_cast<const float2*>(sB + c);
+                v.x = r > c && c < rows ? v.x * (sB[r] / w.x) : r == c ? 1.f : 0.f;
+                v.y = r > c + 1 && c + 1 < rows ? v.y * (sB[r] / w.y) : r == c + 1 ? 1.f : 0.f;
+                return v;
+            });
+    } else {
+        put_t(to, [&](int r, int c) {
+            const float2 v = inverse(r, c), w = *reinterpret_cast<const float2*>(sB + c);
+            return make_float2(v.x * w.x, v.y * w.y);
+        });
     }
 }
 
@@ -627,6 +660,13 @@ __global__ void __launch_bounds__(128) planes_prep_k(const __grid_constant__ DAr
 // the forward chain and the outputs
 // ----------------------------------------------------------------------------
 constexpr int kChainGates = 5 * kC;  // (without 1 / beta)
+// What of a chunk's gates a chain loads, and where it then finds them.
+template <typename T>
+struct Gates {
+    static constexpr int first = Scaled<T> ? 2 * kC : 0, n = Scaled<T> ? 4 * kC : kChainGates;
+    static constexpr int gam = 2 * kC - first, dec = 3 * kC - first, sgam = 4 * kC - first, beta = 5 * kC - first;
+    static constexpr uint32_t less = (kChainGates - n) * 4;  // bytes
+};
 
 template <int KD, int G>
 struct Fwd {
@@ -719,6 +759,54 @@ __device__ __forceinline__ bool store_values(e16* to, const unsigned char* frag,
     return ok;
 }
 
+// What the loading warp does with float16, whose backward reads float32 (laid out
+// as delta.cu's kernels have it): the states of `n` groups from their scaled
+// planes, [value][key], and U or dV, [token][value].
+template <int KD, int LDK>
+__device__ __forceinline__ bool store_states_f32(float* to, const unsigned char* tile, int step, int n, const int* exps,
+                                                 uint64_t* there, uint64_t* taken, uint32_t parity) {
+    using N = Num<__half>;
+    const int l = threadIdx.x & 31;
+    bool ok = true;
+#pragma unroll 1
+    for (int g = 0; g < n; ++g) {
+        ok = warp_wait(&there[g], parity) && ok;
+        const float unit = pow2(-exps[g]);
+        const e16* s = reinterpret_cast<const e16*>(tile + g * step);
+#pragma unroll 1
+        for (int i = l; i < 16 * KD / 8; i += 32) {
+            const int r = i / (KD / 8), k = i % (KD / 8) * 8;
+            const uint4 hi = *reinterpret_cast<const uint4*>(s + r * LDK + k), lo = *reinterpret_cast<const uint4*>(s + (16 + r) * LDK + k);
+            const uint32_t *h = &hi.x, *w = &lo.x;
+            float4* o = reinterpret_cast<float4*>(to + (g * 16 + r) * KD + k);
+#pragma unroll
+            for (int e = 0; e < 4; e += 2) {
+                const float2 a = N::unpack(h[e]), b = N::unpack(w[e]), c = N::unpack(h[e + 1]), d = N::unpack(w[e + 1]);
+                o[e / 2] = make_float4((a.x + b.x) * unit, (a.y + b.y) * unit, (c.x + d.x) * unit, (c.y + d.y) * unit);
+            }
+        }
+        warp_arrive(&taken[g]);
+    }
+    return ok;
+}
+__device__ __forceinline__ bool store_values_f32(float* to, int ld, const unsigned char* frag, int step, int n, uint64_t* there,
+                                                 uint64_t* taken, uint32_t parity) {
+    const Lane L;
+    bool ok = true;
+#pragma unroll 1
+    for (int g = 0; g < n; ++g) {
+        ok = warp_wait(&there[g], parity) && ok;
+        float x[kC / 8][4];
+        frag_get(x, reinterpret_cast<const float4*>(frag + g * step), L);
+        warp_arrive(&taken[g]);
+#pragma unroll
+        for (int j = 0; j < kC / 8; ++j)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) to[static_cast<int64_t>(8 * j + 2 * L.t + (e & 1)) * ld + 16 * g + L.g + (e >> 1) * 8] = x[j][e];
+    }
+    return ok;
+}
+
 // KEEP: S and U are written for a backward.
 template <typename T, int KD, int G, bool KEEP>
 __global__ void __launch_bounds__(Fwd<KD, G>::kWarps * 32, 1) planes_chain_k(const __grid_constant__ DArgs a, const __grid_constant__ Maps maps) {
@@ -761,13 +849,13 @@ __global__ void __launch_bounds__(Fwd<KD, G>::kWarps * 32, 1) planes_chain_k(con
             ok = warp_wait(&empty[c & 1], ((c >> 1) & 1) ^ 1) && ok;
             if (L.l == 0) {
                 const int64_t id = head * a.n + c;
-                mbar_expect_tx(bar, Sm::kLoad);
+                mbar_expect_tx(bar, Sm::kLoad - Gates<T>::less);
 #pragma unroll
                 for (int x = 0; x < KD; x += 64) tma_load(e + Sm::kK + x * kC, &maps.k, bar, x, t0, hk, b);
                 bulk_load(e + Sm::kT, static_cast<const e16*>(a.T) + id * 2 * kCC, 4 * kCC, bar);
 #pragma unroll
                 for (int g = 0; g < G; ++g) tma_load(e + Sm::kV + g * kC * 16, &maps.v, bar, vb + 16 * g, t0, h, b);
-                bulk_load(e + Sm::kGa, a.gates + id * kGates, kChainGates * 4, bar);
+                bulk_load(e + Sm::kGa, a.gates + id * kGates + Gates<T>::first, Gates<T>::n * 4, bar);
 #pragma unroll
                 for (int x = 0; x < KD; x += 64) tma_load(e + Sm::kQ + x * kC, &maps.q, bar, x, t0, hk, b);
                 bulk_load(e + Sm::kM, static_cast<const e16*>(a.M) + id * 2 * kCC, 4 * kCC, bar);
@@ -787,12 +875,20 @@ __global__ void __launch_bounds__(Fwd<KD, G>::kWarps * 32, 1) planes_chain_k(con
             } else {  // a load ahead of the stores
                 if (c + 1 < nc) load(c + 1);
                 if (c < 0) continue;
-                const int64_t id = (head * a.n + c) * 2 * a.Vp + vb;
                 const int n = min(G, (a.Vp - vb) / 16);
-                ok = store_states<Sm::LDK>(static_cast<e16*>(a.S) + id * Sm::LDK, smem + Sm::kGroups + Sm::kS, Sm::kGroup, n, a.Vp,
-                                           s_full, s_empty, c & 1) && ok;
-                ok = store_values<T>(static_cast<e16*>(a.U) + id * kTld, smem + Sm::kGroups + Sm::kU, Sm::kGroup, n,
-                                     reinterpret_cast<e16*>(smem + Sm::kKeep), Sm::kStages, a.Vp, u_full, u_empty, c & 1) && ok;
+                if constexpr (Scaled<T>) {
+                    const int64_t id = head * a.n + c;
+                    ok = store_states_f32<KD, Sm::LDK>(static_cast<float*>(a.S) + (id * a.Vp + vb) * KD, smem + Sm::kGroups + Sm::kS,
+                                                       Sm::kGroup, n, s_exp, s_full, s_empty, c & 1) && ok;
+                    ok = store_values_f32(static_cast<float*>(a.U) + id * kC * a.Vp + vb, a.Vp, smem + Sm::kGroups + Sm::kU, Sm::kGroup, n,
+                                          u_full, u_empty, c & 1) && ok;
+                } else {
+                    const int64_t id = (head * a.n + c) * 2 * a.Vp + vb;
+                    ok = store_states<Sm::LDK>(static_cast<e16*>(a.S) + id * Sm::LDK, smem + Sm::kGroups + Sm::kS, Sm::kGroup, n,
+                                               a.Vp, s_full, s_empty, c & 1) && ok;
+                    ok = store_values<T>(static_cast<e16*>(a.U) + id * kTld, smem + Sm::kGroups + Sm::kU, Sm::kGroup, n,
+                                         reinterpret_cast<e16*>(smem + Sm::kKeep), Sm::kStages, a.Vp, u_full, u_empty, c & 1) && ok;
+                }
             }
         }
         if constexpr (KEEP) bulk_wait_all();
@@ -813,7 +909,7 @@ __global__ void __launch_bounds__(Fwd<KD, G>::kWarps * 32, 1) planes_chain_k(con
             const e16* e = reinterpret_cast<const e16*>(st);
             const Sh es = sh(e);
             const float* ga = reinterpret_cast<const float*>(e + Sm::kGa);
-            const float *gam = ga + 2 * kC, *dec = ga + 3 * kC;
+            const float *gam = ga + Gates<T>::gam, *dec = ga + Gates<T>::dec;
             const int64_t id = head * a.n + c;
             if (!on) {
                 ok = warp_wait(&full[c & 1], (c >> 1) & 1);
@@ -926,14 +1022,15 @@ __global__ void __launch_bounds__(Fwd<KD, G>::kWarps * 32, 1) planes_chain_k(con
                         });
                 }
                 if constexpr (Scaled<T>) {  // beta, which T' was made without
+                    const float unit = tile_unit(e + Sm::kT);
                     float u_max = 0.f;
 #pragma unroll
                     for (int j = 0; j < kC / 8; ++j) {
-                        const float2 r = *reinterpret_cast<const float2*>(ga + 8 * j + 2 * L.t);
+                        const float2 r = *reinterpret_cast<const float2*>(ga + Gates<T>::beta + 8 * j + 2 * L.t);
                         const float2 d = *reinterpret_cast<const float2*>(dec + 8 * j + 2 * L.t);
 #pragma unroll
                         for (int i = 0; i < 4; ++i) {
-                            U[j][i] = U[j][i] * pow2(-xe) * ((i & 1 ? r.y : r.x) * ga[kC]);
+                            U[j][i] = U[j][i] * pow2(-xe) * ((i & 1 ? r.y : r.x) * unit);
                             u_max = fmaxf(u_max, fabsf(U[j][i] * (i & 1 ? d.y : d.x)));
                         }
                     }
@@ -975,7 +1072,7 @@ __global__ void __launch_bounds__(Fwd<KD, G>::kWarps * 32, 1) planes_chain_k(con
         const unsigned char* st = smem + (c & 1) * Sm::kStage;
         const e16* e = reinterpret_cast<const e16*>(st);
         const Sh es = sh(e);
-        const float* sgam = reinterpret_cast<const float*>(e + Sm::kGa) + 4 * kC;
+        const float* sgam = reinterpret_cast<const float*>(e + Sm::kGa) + Gates<T>::sgam;
         const int rows = min(kC, len - c * kC), all = min(kC, a.L - c * kC);
         ok = warp_wait(&full[c & 1], (c >> 1) & 1);
         // (Loops over the groups are not unrolled: what the warps of a CTA run in a chunk has to fit
@@ -1046,7 +1143,7 @@ __global__ void __launch_bounds__(Fwd<KD, G>::kWarps * 32, 1) planes_chain_k(con
                     }
                 });
             if constexpr (Scaled<T>) {
-                const float fm = reinterpret_cast<const float*>(e + Sm::kGa)[kC + 1];
+                const float fm = tile_unit(e + Sm::kM);
 #pragma unroll
                 for (int j = 0; j < kC / 8; ++j)
 #pragma unroll
@@ -1097,7 +1194,8 @@ struct Rev {
     static constexpr int kGroups = kStage + kLoad, kKeep = kGroups + G * kGroup;
     static constexpr int kStages = G == 3 && KD == 128 ? 1 : G;
     static constexpr int kBars = kKeep + kStages * 4 * 16 * kTld;
-    static constexpr size_t bytes = 1024 + kBars + 8 * (5 + 6 * G);
+    static constexpr int kExp = kBars + 8 * (5 + 6 * G);  // (float16) the exponent of each group's dS
+    static constexpr size_t bytes = 1024 + kExp + 4 * G;
 };
 
 template <typename T, int KD, int G>
@@ -1114,6 +1212,8 @@ __global__ void __launch_bounds__(Rev<KD, G>::kWarps * 32, 1) planes_rchain_k(co
     uint64_t* land = empty + 2;
     uint64_t *z_full = land + 1, *z_empty = z_full + G;
     uint64_t *s_full = z_empty + G, *s_empty = s_full + G, *x_full = s_empty + G, *x_empty = x_full + G;
+    int* s_exp = reinterpret_cast<int*>(smem + Sm::kExp);
+    const e16* tiles = static_cast<const e16*>(Scaled<T> ? a.Tr : a.T);
     const int64_t head = static_cast<int64_t>(b) * a.Hv + h;
     if (threadIdx.x == 0) {
         for (int s = 0; s < 2; ++s) {
@@ -1136,14 +1236,14 @@ __global__ void __launch_bounds__(Rev<KD, G>::kWarps * 32, 1) planes_rchain_k(co
             ok = warp_wait(&empty[i & 1], ((i >> 1) & 1) ^ 1) && ok;
             if (L.l == 0) {
                 const int64_t id = head * a.n + c;
-                mbar_expect_tx(bar, Sm::kLoad);
+                mbar_expect_tx(bar, Sm::kLoad - Gates<T>::less);
 #pragma unroll
                 for (int x = 0; x < KD; x += 64) tma_load(e + Sm::kK + x * kC, &maps.k, bar, x, t0, hk, b);
 #pragma unroll
                 for (int g = 0; g < G; ++g) tma_load(e + Sm::kD + g * kC * 16, &maps.d, bar, vb + 16 * g, t0, h, b);
                 bulk_load(e + Sm::kM, static_cast<const e16*>(a.M) + id * 2 * kCC, 4 * kCC, bar);
-                bulk_load(e + Sm::kGa, a.gates + id * kGates, kChainGates * 4, bar);
-                bulk_load(e + Sm::kT, static_cast<const e16*>(a.T) + id * 2 * kCC, 4 * kCC, bar);
+                bulk_load(e + Sm::kGa, a.gates + id * kGates + Gates<T>::first, Gates<T>::n * 4, bar);
+                bulk_load(e + Sm::kT, tiles + id * 2 * kCC, 4 * kCC, bar);
 #pragma unroll
                 for (int x = 0; x < KD; x += 64) tma_load(e + Sm::kQ + x * kC, &maps.q, bar, x, t0, hk, b);
             }
@@ -1160,12 +1260,20 @@ __global__ void __launch_bounds__(Rev<KD, G>::kWarps * 32, 1) planes_rchain_k(co
         for (int i = -1; i < nc && ok; ++i) {  // a load ahead of the stores
             if (i + 1 < nc) load(i + 1);
             if (i < 0) continue;
-            const int64_t id = (head * a.n + nc - 1 - i) * 2 * a.Vp + vb;
             const int n = min(G, (a.Vp - vb) / 16);
-            ok = store_states<Sm::LDK>(static_cast<e16*>(a.dS) + id * Sm::LDK, smem + Sm::kGroups + Sm::kS, Sm::kGroup, n, a.Vp,
-                                       s_full, s_empty, i & 1) && ok;
-            ok = store_values<T>(static_cast<e16*>(a.dV) + id * kTld, smem + Sm::kGroups + Sm::kX, Sm::kGroup, n,
-                                 reinterpret_cast<e16*>(smem + Sm::kKeep), Sm::kStages, a.Vp, x_full, x_empty, i & 1) && ok;
+            if constexpr (Scaled<T>) {
+                const int64_t id = head * a.n + nc - 1 - i;
+                ok = store_states_f32<KD, Sm::LDK>(static_cast<float*>(a.dS) + (id * a.Vp + vb) * KD, smem + Sm::kGroups + Sm::kS,
+                                                   Sm::kGroup, n, s_exp, s_full, s_empty, i & 1) && ok;
+                ok = store_values_f32(static_cast<float*>(a.dV) + id * kC * a.Vp + vb, a.Vp, smem + Sm::kGroups + Sm::kX, Sm::kGroup, n,
+                                      x_full, x_empty, i & 1) && ok;
+            } else {
+                const int64_t id = (head * a.n + nc - 1 - i) * 2 * a.Vp + vb;
+                ok = store_states<Sm::LDK>(static_cast<e16*>(a.dS) + id * Sm::LDK, smem + Sm::kGroups + Sm::kS, Sm::kGroup, n, a.Vp,
+                                           s_full, s_empty, i & 1) && ok;
+                ok = store_values<T>(static_cast<e16*>(a.dV) + id * kTld, smem + Sm::kGroups + Sm::kX, Sm::kGroup, n,
+                                     reinterpret_cast<e16*>(smem + Sm::kKeep), Sm::kStages, a.Vp, x_full, x_empty, i & 1) && ok;
+            }
         }
         bulk_wait_all();
         return;
@@ -1179,17 +1287,26 @@ __global__ void __launch_bounds__(Rev<KD, G>::kWarps * 32, 1) planes_rchain_k(co
         const float4* sZ = reinterpret_cast<const float4*>(mine + Sm::kZ);
         float S[KD / 8][4];  // dS^T
         state_load<KD>(S, a.dfinal ? a.dfinal + head * a.K * a.V : nullptr, a.K, a.V, v0, L);
+        int se = 0;  // (float16) S holds 2^se times dS
         for (int i = 0; i < nc && ok; ++i) {
-            const int c = nc - 1 - i;
             const e16* e = reinterpret_cast<const e16*>(smem + (i & 1) * Sm::kStage);
             const Sh es = sh(e);
             const float* ga = reinterpret_cast<const float*>(e + Sm::kGa);
-            const float *gam = ga + 2 * kC, *dec = ga + 3 * kC;
-            const int64_t id = head * a.n + c;
+            const float *gam = ga + Gates<T>::gam, *dec = ga + Gates<T>::dec;
             if (!on) {
                 ok = warp_wait(&full[i & 1], (i >> 1) & 1);
             } else {
                 ok = warp_wait2(&full[i & 1], (i >> 1) & 1, &s_empty[warp], (i & 1) ^ 1);
+                auto scale_state = [&](uint32_t bits) {
+                    const int e = max(-kMaxExp, min(kMaxExp, se + scale_exp(bits))) - se;
+                    if (e == 0) return;
+                    scale_tile<KD / 8>(S, pow2(e));
+                    se += e;
+                };
+                if constexpr (Scaled<T>) {
+                    scale_state(max_bits<KD / 8>(S));
+                    if (L.l == 0) s_exp[warp] = se;
+                }
                 float U[kC / 8][4] = {};  // dU^T = d (K dS1)^T + dO^T M
                 {
                     Af<2> as[2];
@@ -1216,13 +1333,20 @@ __global__ void __launch_bounds__(Rev<KD, G>::kWarps * 32, 1) planes_rchain_k(co
                 const bool z_there = mbar_try_wait(&z_full[warp], i & 1), x_free = mbar_try_wait(&x_empty[warp], (i & 1) ^ 1);
 #pragma unroll
                 for (int j = 0; j < kC / 8; ++j) {
-                    const float2 f = *reinterpret_cast<const float2*>(dec + 8 * j + 2 * L.t);
+                    float2 f = *reinterpret_cast<const float2*>(dec + 8 * j + 2 * L.t);
+                    if constexpr (Scaled<T>) {
+                        f.x *= pow2(-se);
+                        f.y *= pow2(-se);
+                    }
                     U[j][0] *= f.x;
                     U[j][1] *= f.y;
                     U[j][2] *= f.x;
                     U[j][3] *= f.y;
                 }
+                int ue = 0;  // (float16) U holds 2^ue dU
                 {
+                    float Y[Scaled<T> ? kC / 8 : 1][4] = {};  // float16: dO^T M by itself, as M is scaled
+                    auto& sums = *[&]() { if constexpr (Scaled<T>) return &Y; else return &U; }();
                     Af<1> ad[2];
                     steps<8>(
                         [&](int k, uint32_t(*f)[4]) {
@@ -1231,15 +1355,29 @@ __global__ void __launch_bounds__(Rev<KD, G>::kWarps * 32, 1) planes_rchain_k(co
                             for (int p = 0; p < 4; ++p)
                                 if (p <= k / 2) ld_b<true>(f[p], es + Sm::kM + (k & 1 ? 0 : kCC), kTld, 16 * p, 16 * (k / 2));
                         },
-                        [&](int k, const uint32_t(*f)[4]) { mma_step<T>(U, ad[(k / 2) & 1], f, 0, k / 2 + 1); });
+                        [&](int k, const uint32_t(*f)[4]) { mma_step<T>(sums, ad[(k / 2) & 1], f, 0, k / 2 + 1); });
+                    if constexpr (Scaled<T>) {
+                        const float fm = tile_unit(e + Sm::kM);
+#pragma unroll
+                        for (int j = 0; j < kC / 8; ++j)
+#pragma unroll
+                            for (int x = 0; x < 4; ++x) U[j][x] = fmaf(Y[j][x], fm, U[j][x]);
+                        ue = scale_exp(max_bits<kC / 8>(U));
+                        if (ue != 0) scale_tile<kC / 8>(U, pow2(ue));
+                    }
                 }
                 ok = warp_wait_asked(z_there, &z_full[warp], i & 1) && ok;
                 // dV^T = dU^T T', the last 16 tokens first; between the products dS is scaled and
                 // (scale gam dO)^T Q added, and the last tokens of dV, done first, are split for the update
+                // (float16: beta comes after the product, and then the split)
                 float X[kC / 8][4] = {};
                 const float gc = gam[kC - 1];
                 auto decayed = [&](Af<2>& to, int kk, int q) {
-                    const float2 d = *reinterpret_cast<const float2*>(gam + 16 * kk + 8 * (q / 2) + 2 * L.t);
+                    float2 d = *reinterpret_cast<const float2*>(gam + 16 * kk + 8 * (q / 2) + 2 * L.t);
+                    if constexpr (Scaled<T>) {
+                        d.x *= pow2(se);
+                        d.y *= pow2(se);
+                    }
                     const float* u = X[2 * kk + q / 2];
                     from_acc_part<T>(to, q, -u[2 * (q & 1)] * d.x, -u[2 * (q & 1) + 1] * d.y);
                 };
@@ -1262,7 +1400,8 @@ __global__ void __launch_bounds__(Rev<KD, G>::kWarps * 32, 1) planes_rchain_k(co
                                     constexpr int N = KD / 8;
                                     const int j = k * 2 + q / 2;
                                     if (j < N) {
-                                        const float4 z = sZ[j * 32 + L.l];
+                                        float4 z = sZ[j * 32 + L.l];
+                                        if constexpr (Scaled<T>) z = make_float4(z.x * pow2(se), z.y * pow2(se), z.z * pow2(se), z.w * pow2(se));
                                         S[j][0] = fmaf(gc, S[j][0], z.x);
                                         S[j][1] = fmaf(gc, S[j][1], z.y);
                                         S[j][2] = fmaf(gc, S[j][2], z.z);
@@ -1273,13 +1412,31 @@ __global__ void __launch_bounds__(Rev<KD, G>::kWarps * 32, 1) planes_rchain_k(co
                                     const float* u = U[2 * kk - 2 + q / 2];
                                     from_acc_part<T>(au[(kk - 1) & 1], q, u[2 * (q & 1)], u[2 * (q & 1) + 1]);
                                 }
-                                if (k == 4) decayed(xd[1], 3, q);
+                                if (!Scaled<T> && k == 4) decayed(xd[1], 3, q);
                             };
                             if (k & 1) mma_step_with<T>(X, af, f, side, 0, kk + 1);
                             else mma_step_with<T>(X, high(af), f, side, 0, kk + 1);
                         });
                 }
                 warp_arrive(&z_empty[warp]);
+                if constexpr (Scaled<T>) {
+                    const float unit = tile_unit(e + Sm::kT);
+                    float x_max = 0.f;
+#pragma unroll
+                    for (int j = 0; j < kC / 8; ++j) {
+                        const float2 r = *reinterpret_cast<const float2*>(ga + Gates<T>::beta + 8 * j + 2 * L.t);
+                        const float2 d = *reinterpret_cast<const float2*>(gam + 8 * j + 2 * L.t);
+#pragma unroll
+                        for (int x = 0; x < 4; ++x) {
+                            X[j][x] = X[j][x] * pow2(-ue) * ((x & 1 ? r.y : r.x) * unit);
+                            x_max = fmaxf(x_max, fabsf(X[j][x] * (x & 1 ? d.y : d.x)));
+                        }
+                    }
+                    x_max = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(x_max))) * pow2(se);
+                    scale_state(max(max_bits<KD / 8>(S), __float_as_uint(x_max)));
+#pragma unroll
+                    for (int q = 0; q < 4; ++q) decayed(xd[1], 3, q);
+                }
                 ok = warp_wait_asked(x_free, &x_empty[warp], (i & 1) ^ 1) && ok;
                 frag_put(sX, X, L);
                 warp_arrive(&x_full[warp]);
@@ -1302,6 +1459,7 @@ __global__ void __launch_bounds__(Rev<KD, G>::kWarps * 32, 1) planes_rchain_k(co
             }
             warp_arrive(&empty[i & 1]);
         }
+        if constexpr (Scaled<T>) scale_tile<KD / 8>(S, pow2(-se));
         if (on && a.dinitial && ok) state_store<KD>(S, a.dinitial + head * a.K * a.V, a.K, a.V, v0, L);
         return;
     }
@@ -1309,13 +1467,29 @@ __global__ void __launch_bounds__(Rev<KD, G>::kWarps * 32, 1) planes_rchain_k(co
     for (int i = 0; i < nc && ok; ++i) {
         const e16* e = reinterpret_cast<const e16*>(smem + (i & 1) * Sm::kStage);
         const Sh es = sh(e);
-        const float* sgam = reinterpret_cast<const float*>(e + Sm::kGa) + 4 * kC;
+        const float* sgam = reinterpret_cast<const float*>(e + Sm::kGa) + Gates<T>::sgam;
         ok = warp_wait(&full[i & 1], (i >> 1) & 1);
         for (int g = warp - G; g < G; g += Sm::H) {
             if (vb + 16 * g >= a.Vp) break;
             float Z[KD / 8][4] = {};
             Af<2> af;
             constexpr int Q = KD / 64;
+            int de = 0;  // (float16) of scale gam dO
+            if constexpr (Scaled<T>) {
+                float m = 0.f;
+#pragma unroll 1
+                for (int kk = 0; kk < kC / 16; ++kk) {
+                    uint32_t r[4];
+                    ld_at32(r, es + Sm::kD + g * kC * 16, 16 * kk);
+#pragma unroll
+                    for (int x = 0; x < 2; ++x) {
+                        const float2 d = *reinterpret_cast<const float2*>(sgam + 16 * kk + 8 * x + 2 * L.t);
+                        const float2 lo = Num<T>::unpack(r[2 * x]), hi = Num<T>::unpack(r[2 * x + 1]);
+                        m = fmaxf(m, fmaxf(fmaxf(fabsf(lo.x * d.x), fabsf(lo.y * d.y)), fmaxf(fabsf(hi.x * d.x), fabsf(hi.y * d.y))));
+                    }
+                }
+                de = scale_exp(__reduce_max_sync(0xffffffffu, __float_as_uint(m)));
+            }
             steps<4 * Q>(
                 [&](int k, uint32_t(*f)[4]) {
 #pragma unroll
@@ -1329,7 +1503,11 @@ __global__ void __launch_bounds__(Rev<KD, G>::kWarps * 32, 1) planes_rchain_k(co
                         float y[2][4];
 #pragma unroll
                         for (int x = 0; x < 2; ++x) {
-                            const float2 d = *reinterpret_cast<const float2*>(sgam + 16 * kk + 8 * x + 2 * L.t);
+                            float2 d = *reinterpret_cast<const float2*>(sgam + 16 * kk + 8 * x + 2 * L.t);
+                            if constexpr (Scaled<T>) {
+                                d.x *= pow2(de);
+                                d.y *= pow2(de);
+                            }
                             const float2 lo = Num<T>::unpack(r[2 * x]), hi = Num<T>::unpack(r[2 * x + 1]);
                             y[x][0] = lo.x * d.x;
                             y[x][1] = lo.y * d.y;
@@ -1342,6 +1520,7 @@ __global__ void __launch_bounds__(Rev<KD, G>::kWarps * 32, 1) planes_rchain_k(co
                 });
             float4* sZ = reinterpret_cast<float4*>(smem + Sm::kGroups + g * Sm::kGroup + Sm::kZ);
             ok = warp_wait(&z_empty[g], (i & 1) ^ 1) && ok;
+            if constexpr (Scaled<T>) scale_tile<KD / 8>(Z, pow2(-de));
 #pragma unroll
             for (int j = 0; j < KD / 8; ++j) sZ[j * 32 + L.l] = make_float4(Z[j][0], Z[j][1], Z[j][2], Z[j][3]);
             warp_arrive(&z_full[g]);
@@ -1931,13 +2110,11 @@ cudaError_t rchain_launch(const DArgs& a, const Maps& m, cudaStream_t s) {
 template <typename T, int KD>
 cudaError_t chain(const DArgs& a, const Maps& m, bool reverse, cudaStream_t s) {
     const int g = chain_groups(a, reverse);
-    if constexpr (!Scaled<T>) {
-        if (reverse) return g == 2 ? rchain_launch<T, KD, 2>(a, m, s) : rchain_launch<T, KD, 3>(a, m, s);
-        if (a.S)
-            return g == 2   ? chain_launch<T, KD, 2, true>(a, m, s)
-                   : g == 3 ? chain_launch<T, KD, 3, true>(a, m, s)
-                            : chain_launch<T, KD, 4, true>(a, m, s);
-    }
+    if (reverse) return g == 2 ? rchain_launch<T, KD, 2>(a, m, s) : rchain_launch<T, KD, 3>(a, m, s);
+    if (a.S)
+        return g == 2   ? chain_launch<T, KD, 2, true>(a, m, s)
+               : g == 3 ? chain_launch<T, KD, 3, true>(a, m, s)
+                        : chain_launch<T, KD, 4, true>(a, m, s);
     return g == 2 ? chain_launch<T, KD, 2, false>(a, m, s) : chain_launch<T, KD, 4, false>(a, m, s);
 }
 
@@ -1989,13 +2166,17 @@ cudaError_t fwd(const DArgs& a, cudaStream_t s) {
 
 template <typename T, int KD>
 cudaError_t bwd(const DArgs& a, float* group, cudaStream_t s) {
-    DELTA_TRY((smem_limit(planes_grad_k<T, KD>, Grad<KD>::bytes)));
+    // a runtime call first, as in fwd
+    if constexpr (Scaled<T>) DELTA_TRY((smem_limit(planes_rchain_k<T, KD, 2>, Rev<KD, 2>::bytes)));
+    else DELTA_TRY((smem_limit(planes_grad_k<T, KD>, Grad<KD>::bytes)));
     Maps m{};
     if (!make_maps(a, m)) return cudaErrorInvalidValue;
     DELTA_TRY((chain<T, KD>(a, m, true, s)));
-    const int items = a.B * a.Hk * a.n;
-    planes_grad_k<T, KD><<<items < kSms ? items : kSms, 32 * kGradWarps, Grad<KD>::bytes, s>>>(a, group, m);
-    note_launch();
+    if constexpr (!Scaled<T>) {  // (float16's gradients are delta.cu's)
+        const int items = a.B * a.Hk * a.n;
+        planes_grad_k<T, KD><<<items < kSms ? items : kSms, 32 * kGradWarps, Grad<KD>::bytes, s>>>(a, group, m);
+        note_launch();
+    }
     return cudaGetLastError();
 }
 
@@ -2004,8 +2185,11 @@ int key_dim(const DArgs& a) { return a.K <= 64 ? 64 : 128; }
 size_t ids(const DArgs& a) { return static_cast<size_t>(a.B) * a.Hv * a.n; }
 size_t gates_bytes(const DArgs& a) { return up256(ids(a) * kGates * sizeof(float)); }
 size_t square_bytes(const DArgs& a) { return up256(ids(a) * 2 * kCC * sizeof(e16)); }
-size_t state_bytes(const DArgs& a) { return up256(ids(a) * 2 * a.Vp * (key_dim(a) + 8) * sizeof(e16)); }
-size_t value_bytes(const DArgs& a, int planes) { return up256(ids(a) * planes * a.Vp * kTld * sizeof(e16)); }
+// float16: float32, without padding
+size_t state_bytes(const DArgs& a) {
+    return up256(ids(a) * a.Vp * (a.half ? key_dim(a) * sizeof(float) : 2 * (key_dim(a) + 8) * sizeof(e16)));
+}
+size_t value_bytes(const DArgs& a) { return up256(ids(a) * a.Vp * (a.half ? kC * sizeof(float) : 2 * kTld * sizeof(e16))); }
 
 void set_saved(DArgs& a, void* ws, bool training) {
     char* w = static_cast<char*>(ws);
@@ -2013,15 +2197,17 @@ void set_saved(DArgs& a, void* ws, bool training) {
     a.T = w; w += square_bytes(a);
     a.M = w; w += square_bytes(a);
     a.S = training ? w : nullptr; w += state_bytes(a);
-    a.U = training ? w : nullptr;
+    a.U = training ? w : nullptr; w += value_bytes(a);
+    a.Tr = training && a.half ? w : nullptr;
 }
 
 }  // namespace
 
 size_t planes_saved_size(const DArgs& a, bool training) {
-    return gates_bytes(a) + 2 * square_bytes(a) + (training ? state_bytes(a) + value_bytes(a, 2) : 0);
+    return gates_bytes(a) + 2 * square_bytes(a) +
+           (training ? state_bytes(a) + value_bytes(a) + (a.half ? square_bytes(a) : 0) : 0);
 }
-size_t planes_bwd_size(const DArgs& a) { return state_bytes(a) + value_bytes(a, 2); }
+size_t planes_bwd_size(const DArgs& a) { return state_bytes(a) + value_bytes(a); }
 
 cudaError_t planes_fwd(DArgs a, void* ws, bool training, cudaStream_t s) {
     set_saved(a, ws, training);
@@ -2029,11 +2215,12 @@ cudaError_t planes_fwd(DArgs a, void* ws, bool training, cudaStream_t s) {
     return a.K <= 64 ? fwd<__nv_bfloat16, 64>(a, s) : fwd<__nv_bfloat16, 128>(a, s);
 }
 
-cudaError_t planes_bwd(DArgs a, void* saved, void* ws, float* group, cudaStream_t s) {
+cudaError_t planes_bwd(DArgs& a, void* saved, void* ws, float* group, cudaStream_t s) {
     set_saved(a, saved, true);
     char* w = static_cast<char*>(ws);
     a.dS = w;
     a.dV = w + state_bytes(a);
+    if (a.half) return a.K <= 64 ? bwd<__half, 64>(a, group, s) : bwd<__half, 128>(a, group, s);
     return a.K <= 64 ? bwd<__nv_bfloat16, 64>(a, group, s) : bwd<__nv_bfloat16, 128>(a, group, s);
 }
 

@@ -357,7 +357,7 @@ struct DeltaGrads {
     void *dq, *dk, *dv, *dg, *dbeta;
     float* dinitial;      // or null
 };
-int delta_path(const EacsDelta& p, bool training);
+int delta_path(const EacsDelta& p);
 size_t delta_workspace_size(const EacsDelta& p, bool training);
 size_t delta_bwd_workspace_size(const EacsDelta& p);
 int delta_fwd(const EacsDelta& p, void* o, float* final_state, void* ws, size_t ws_bytes, bool training,

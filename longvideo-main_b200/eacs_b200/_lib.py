@@ -55,7 +55,7 @@ SIGNATURES = {
                                  _I64, _I64, _P]),
     "eacs_layer_norm_bwd_workspace_size": (_SZ, [_I64, _I64]),
     "eacs_delta_fwd": (_I, [_P, _P, _P, _P, _SZ, _I, _P]),
-    "eacs_delta_path": (_I, [_P, _I]),
+    "eacs_delta_path": (_I, [_P]),
     "eacs_delta_workspace_size": (_SZ, [_P, _I]),
     "eacs_delta_bwd": (_I, [_P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _SZ, _P, _SZ, _P]),
     "eacs_delta_bwd_workspace_size": (_SZ, [_P]),

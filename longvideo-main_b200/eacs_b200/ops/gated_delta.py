@@ -17,17 +17,17 @@ h // (Hv // Hk).  Views are taken with their strides (a slice of a fused
 projection needs no copy) as long as their last dimension is dense; 16-bit
 ones are fastest when their rows start on 16 bytes (K, V and all strides
 multiples of 8).  Sums and states are float32.  Operands of the products keep
-22 significant bits, 16 for bfloat16 inputs; float16 ones may be of any size
-that float32 holds.  float16 training runs on the kernels of float32, at a
-fifth of bfloat16's speed.  The same inputs give the same bits (float16: with
-gradients, or without).
+22 significant bits, 16 for bfloat16 inputs; float16's states, values corrected
+by them and gradients of them may be of any size that float32 holds.  The same
+inputs give the same bits.  Where gradients are wanted beta is held 2^-64 away
+from 0.
 
 A NaN or an infinity of a token reaches what follows it, and up to 15 tokens
 before it (the rest of its block of 16; in the backward pass, up to 15 behind an
 upstream gradient's).  A forward at K = V = 128 takes 38 KB of workspace for each
 chunk of 64 tokens of a head in the 16-bit kernels and 116 KB in the others;
-with gradients 145 KB (133) are kept until the backward, which takes 106 KB (98)
-more.  A device wait that runs out leaves outputs unwritten and is reported by
+with gradients 145 KB (float16 155, others 133) are kept until the backward,
+which takes 106 KB (98) more.  A device wait that runs out leaves outputs unwritten and is reported by
 eacs_device_status.
 
 Gradients are reverse mode, once; forward-mode, torch.func or traced calls are
@@ -111,7 +111,7 @@ def _forward(args, out_state, training, dev):
     with on(dev):
         _lib.check(L_.eacs_delta_fwd(p, o.data_ptr(), _lib.ptr(final), ws.data_ptr(), ws.numel(),
                                      int(training), _lib.raw_stream(dev.index)), "eacs_delta_fwd")
-    return o, final, ws, L_.eacs_delta_path(p, 1) if training else 0
+    return o, final, ws, L_.eacs_delta_path(p) if training else 0
 
 
 class GatedDeltaFunction(torch.autograd.Function):

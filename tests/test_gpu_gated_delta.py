@@ -746,3 +746,61 @@ def test_each_gradient_against_differences(name):
     size = float(o.detach().norm() * do.norm() + S.detach().norm() * dS.norm())
     allowed = 1.5 * TOL / 16 * size / h
     assert abs(num - slope) <= allowed and slope > 10 * allowed, (num, slope, allowed)
+
+
+@pytest.mark.parametrize("shape", [(1, 130, 12, 24, 64, 200), (3, 130, 4, 16, 128, 128), (1, 130, 16, 64, 128, 104), (2, 193, 4, 32, 64, 128)])
+def test_many_heads_in_float16(shape):
+    d, do, dS = make(*shape, torch.float16, torch.float32, seed=sum(shape))
+    lengths = torch.tensor([shape[1], 66, 1][:shape[0]], dtype=torch.int32)
+    compare(*both(d, do, dS, lengths.to(DEV)))
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("value,state,scale", [(1.0, 1.0, 1.0), (1e-3, 1e-3, 1e2), (1.0, 1e6, 1e-6), (1e4, 1e9, 1e-9), (1.0, 0.0, 1.0)])
+def test_forward_with_and_without_gradients_has_the_same_bits(dtype, value, state, scale):
+    d, _, _ = make(2, 200, 2, 4, 128, 72, dtype, torch.float32, seed=50)
+    d["v"] = (d["v"].float() * value).clamp(-6e4, 6e4).to(dtype)
+    d["initial"] *= state
+    call = lambda q: gated_delta_rule(q, *(d[n] for n in ("k", "v", "g", "beta")), scale=scale, initial_state=d["initial"],
+                                      output_final_state=True)
+    for a, b in zip(call(d["q"].clone().requires_grad_(True)), call(d["q"])):
+        assert bool(torch.isfinite(a).all()) and torch.equal(a, b)
+
+
+@pytest.mark.parametrize("K,V", [(64, 64), (128, 48)])
+def test_float16_gradients_of_groups_of_different_sizes(K, V):
+    """Value columns (and so the tiles of a state) from 1e-4 to 1e4 of one another, forward and backward."""
+    d, do, dS = make(1, 150, 1, 2, K, V, torch.float16, torch.float32, seed=51)
+    sizes = torch.logspace(-2, 2, V, device=DEV)
+    d["v"], d["initial"] = (d["v"].float() * sizes).half(), d["initial"] * sizes
+    do, dS = (do.float() / sizes).half(), dS / sizes
+    got, want = both(d, do, dS)
+    compare(got, want)
+    for n in ("S", "dinitial"):  # column by column
+        err, ref = (got[n].double().cpu() - want[n]).norm(dim=2), want[n].norm(dim=2)
+        assert bool((err <= TOL * ref).all()), (n, float((err / ref).max()))
+
+
+def test_float16_backward_twice_streams_and_graphs():
+    test_backward_twice_and_two_calls_at_once(torch.float16)
+    d, do, dS = make(2, 200, 2, 4, 64, 64, torch.float16, seed=52)
+    x = {n: t.detach().clone().requires_grad_(True) for n, t in d.items()}
+
+    def step():
+        o, S = gated_delta_rule(*(x[n] for n in ("q", "k", "v", "g", "beta")), initial_state=x["initial"], output_final_state=True)
+        return (o.detach(), S.detach(), *torch.autograd.grad([o, S], list(x.values()), [do, dS]))
+    graphs = []
+    for _ in range(2):
+        gr = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(gr):
+            out = step()
+        graphs.append((gr, out))
+    with torch.no_grad():
+        x["v"].mul_(0.01)
+        do.mul_(0.01)
+    want = step()
+    for gr, _ in graphs:
+        gr.replay()
+    torch.cuda.synchronize()
+    for _, out in graphs:
+        assert all(torch.equal(a, b) for a, b in zip(out, want))

@@ -152,15 +152,15 @@ def test_delta_path_named_by_the_caller_without_device():
             st += [640 * n, 64 * n, n]
         return _lib.DELTA_PATH.pack(q, P, P, P, P, *st, 0, 0, 2, 10, 4, 4, K, 8, 1.0, dtype, dtype, path)
     assert _lib.DELTA_PATH.size == _lib.DELTA.size
-    assert L.eacs_delta_path(args(0), 1) == 2 and L.eacs_delta_path(args(0, q=P + 2), 1) == 1
-    assert L.eacs_delta_path(args(0, K=12), 1) == 1 and L.eacs_delta_path(args(0, dtype=0), 0) == 1
-    assert L.eacs_delta_path(args(0, dtype=1), 0) == 2 and L.eacs_delta_path(args(0, dtype=1), 1) == 1
-    assert L.eacs_delta_path(args(1), 1) == 1 and L.eacs_delta_path(None, 1) == 0
+    assert L.eacs_delta_path(args(0)) == 2 and L.eacs_delta_path(args(0, q=P + 2)) == 1
+    assert L.eacs_delta_path(args(0, K=12)) == 1 and L.eacs_delta_path(args(0, dtype=0)) == 1
+    assert L.eacs_delta_path(args(0, dtype=1)) == 2 and L.eacs_delta_path(args(1)) == 1
+    assert L.eacs_delta_path(None) == 0
     for size in (lambda a: L.eacs_delta_workspace_size(a, 1), L.eacs_delta_bwd_workspace_size):
         assert size(args(0)) == size(args(2)) != size(args(1)) == size(args(0, q=P + 2))
     big = 1 << 40
-    for bad in (args(2, q=P + 2), args(2, dtype=0), args(2, dtype=1), args(3), args(-1)):
-        assert L.eacs_delta_path(bad, 1) == 0 and L.eacs_delta_workspace_size(bad, 1) == 0
+    for bad in (args(2, q=P + 2), args(2, dtype=0), args(3), args(-1)):
+        assert L.eacs_delta_path(bad) == 0 and L.eacs_delta_workspace_size(bad, 1) == 0
         assert L.eacs_delta_fwd(bad, P, None, P, big, 1, None) == _lib.EACS_ERR_INVALID
         assert L.eacs_delta_bwd(bad, P, strides, None, P, P, P, P, P, None, P, big, P, big, None) == _lib.EACS_ERR_INVALID
 
