@@ -2077,10 +2077,12 @@ constexpr int kSms = 148;
 // fewest rounds of CTAs, weighed with what a chunk takes with 2, 3 or 4 groups on
 // an SM.  Measured at V = 128, us:
 //                                       K = 128            K = 64
-//   forward                             2.43 3.36 3.27     1.73 2.75 2.38
-//   forward, float16                    2.98 3.62 3.77     2.12 2.99 2.77
-//   forward that keeps for a backward   2.74 3.54 4.37     2.36 2.93 3.82
-//   reverse                             2.80 3.40          2.34 2.93
+//   forward                             2.33 3.35 3.30     1.74 2.71 2.37
+//     float16                           2.91 3.59 3.75     2.12 3.01 2.62
+//   forward that keeps for a backward   2.72 3.54 4.24     2.31 2.89 3.84
+//     float16                           3.44 4.39 5.67     2.47 3.15 4.03
+//   reverse                             2.79 3.46          2.34 2.92
+//     float16                           3.48 4.50          2.66 3.15
 // (four groups do not fit the reverse chain's tiles).
 int chain_groups(const DArgs& a, bool reverse) {
     const int64_t heads = static_cast<int64_t>(a.B) * a.Hv, groups = a.Vp / 16;
