@@ -174,6 +174,138 @@ EACS_API size_t eacs_delta_bwd_workspace_size(const EacsDelta* p);
  * NULL. */
 EACS_API int eacs_delta_step(const EacsDelta* p, void* o, float* final_state, void* stream);
 
+/* The selective state space scan: a diagonal recurrence whose steps and whose
+ * input and output vectors go by the token, beside the scans above (one step
+ * per frame, rates that do not change).  Per row, channel d and state n, with
+ * s = softplus(dt + dt_bias) (softplus != 0) or dt + dt_bias,
+ *   h_t[n] = exp(s_t A[d,n]) h_{t-1}[n] + s_t x_t B_t[n]
+ *   y_t = (sum_n C_t[n] h_t[n] + skip[d] x_t) silu(z_t).
+ * x, dt, z (rows,L,D) and B, C (rows,L,N) of dtype, with strides of row and
+ * token in elements and a dense last dimension; z may be NULL (no gate).  A
+ * (D,N), skip (D) and dt_bias (D) float32 dense; skip and dt_bias may be NULL
+ * (0).  lengths (rows) int32 or NULL: a row has min(max(lengths[r], 0), L)
+ * tokens; what lies behind is not read, its outputs and gradients are 0 and
+ * the state stays.  initial_state (rows,D,N) float32 dense or NULL (zeros).
+ * N goes up to 64.  Sums and states are float32; A <= 0 and s >= 0 are meant
+ * (states that grow do so as float32 lets them).  Rows that start on 16 bytes
+ * are read several channels at a time. */
+typedef struct EacsSelective {
+    const void* x;
+    const void* dt;
+    const void* z;
+    const void* B;
+    const void* C;
+    int64_t x_stride[2];
+    int64_t dt_stride[2];
+    int64_t z_stride[2];
+    int64_t B_stride[2];
+    int64_t C_stride[2];
+    const float* A;
+    const float* skip;
+    const float* dt_bias;
+    const int32_t* lengths;
+    const float* initial_state;
+    int64_t rows, L, D, N;
+    int32_t dtype;
+    int32_t softplus;
+} EacsSelective;
+
+/* y (rows,L,D) dense of dtype; final_state (rows,D,N) float32 or NULL.
+ * checkpoints (16-byte aligned, or NULL) of eacs_selective_ckpt_size bytes
+ * receives the states that eacs_selective_bwd starts from. */
+EACS_API int eacs_selective_fwd(const EacsSelective* p, void* y, float* final_state, void* checkpoints,
+                                size_t checkpoint_bytes, void* stream);
+EACS_API size_t eacs_selective_ckpt_size(const EacsSelective* p);
+
+/* Backward: dy (rows,L,D) of dtype with its strides of row and token, dfinal
+ * (rows,D,N) float32 or NULL; dx, ddt, dz (rows,L,D) and dB, dC (rows,L,N)
+ * dense of dtype (dz NULL without z), dA (D,N) float32, dskip and ddt_bias (D)
+ * float32 or NULL, dinitial (rows,D,N) float32 or NULL.  Sums over rows, tokens
+ * and channels are added in a fixed order.  The workspace is 16-byte aligned. */
+EACS_API int eacs_selective_bwd(const EacsSelective* p, const void* dy, const int64_t* dy_stride, const float* dfinal,
+                                void* dx, void* ddt, void* dz, void* dB, void* dC, float* dA, float* dskip,
+                                float* ddt_bias, float* dinitial, const void* checkpoints, size_t checkpoint_bytes,
+                                void* workspace, size_t workspace_bytes, void* stream);
+EACS_API size_t eacs_selective_bwd_workspace_size(const EacsSelective* p);
+
+/* One token a row: x, dt, z, y (rows,D) and B, C (rows,N) (the token strides, L,
+ * lengths and initial_state are not used); state (rows,D,N) float32 dense is
+ * updated in place. */
+EACS_API int eacs_selective_step(const EacsSelective* p, void* y, float* state, void* stream);
+
+/* The short causal convolution of each channel, in front of a recurrence: with
+ * `width` taps (2 to 4) and x_t for t < 0 from the state,
+ *   p_t = bias + sum_w weight[d,w] x_{t-width+1+w},  y_t = silu(p_t)  (silu != 0) or p_t.
+ * x (rows,L,D) of dtype with strides of row and token in elements and a dense
+ * last dimension; weight (D,width) and bias (D, or NULL) of w_dtype.  A state is
+ * the last width - 1 inputs, (rows,width-1,D) of dtype, oldest first;
+ * initial_state may be NULL (zeros).  lengths as for EacsSelective.  Sums are
+ * float32.  Vectors of channels are moved at once where pointers and strides
+ * allow it. */
+typedef struct EacsConv {
+    const void* x;
+    const void* weight;
+    const void* bias;
+    const void* initial_state;
+    const int32_t* lengths;
+    int64_t x_stride[2];
+    int64_t rows, L, D;
+    int32_t width;
+    int32_t dtype;
+    int32_t w_dtype;
+    int32_t silu;
+} EacsConv;
+
+/* y (rows,L,D) dense of dtype; final_state or NULL. */
+EACS_API int eacs_conv_fwd(const EacsConv* p, void* y, void* final_state, void* stream);
+/* Backward: dy with its strides of row and token, dfinal or NULL; dx dense of
+ * dtype; dweight and dbias of w_dtype (either may be NULL), sums in float32
+ * added in a fixed order; dinitial or NULL.  The workspace (16-byte aligned) is
+ * needed when dweight or dbias is asked for. */
+EACS_API int eacs_conv_bwd(const EacsConv* p, const void* dy, const int64_t* dy_stride, const void* dfinal, void* dx,
+                           void* dweight, void* dbias, void* dinitial, void* workspace, size_t workspace_bytes,
+                           void* stream);
+EACS_API size_t eacs_conv_bwd_workspace_size(const EacsConv* p);
+/* One token a row: x, y (rows,D); the state is moved on in place. */
+EACS_API int eacs_conv_step(const EacsConv* p, void* y, void* state, void* stream);
+
+/* The norms before and after a block with its gate and its scaled residual,
+ * over rows of d values; r(v) = 1 / sqrt(mean(v^2) + eps):
+ *   residual NULL:  y = x r(x) weight silu(gate)
+ *   else:           u = x, or x r(x) post_weight (post_norm != 0);
+ *                   u = u silu(gate) where there is a gate;
+ *                   s = residual + scale u;  y = s r(s) weight.
+ * x, gate and residual of dtype with row strides in elements; gate may be NULL
+ * (no gate); weight, scale and post_weight (d) of w_dtype may be NULL (ones).
+ * y and s dense of dtype, each rounded once from float32.  d goes up to 8192;
+ * rows that start and end on 16 bytes are read 16 bytes at a time. */
+typedef struct EacsNorm {
+    const void* x;
+    const void* gate;
+    const void* residual;
+    const void* weight;
+    const void* scale;
+    const void* post_weight;
+    int64_t x_stride, gate_stride, residual_stride;
+    int64_t rows, d;
+    float eps;
+    int32_t dtype;
+    int32_t w_dtype;
+    int32_t post_norm;
+} EacsNorm;
+
+EACS_API int eacs_norm_fwd(const EacsNorm* p, void* y, void* s, void* stream);
+/* Backward: dy and ds (of y and s; either may be NULL) with row strides; dx,
+ * dgate, dresidual dense of dtype (dgate NULL without a gate; dresidual NULL
+ * without a residual, or where it equals dx: neither gate nor scale nor
+ * post_norm); dweight, dscale and dpost_weight of w_dtype, each or NULL, sums in
+ * float32 added in a fixed order, for which the workspace (16-byte aligned) is
+ * needed. */
+EACS_API int eacs_norm_bwd(const EacsNorm* p, const void* dy, int64_t dy_stride, const void* ds, int64_t ds_stride,
+                           void* dx, void* dgate, void* dresidual, void* dweight, void* dscale, void* dpost_weight,
+                           void* workspace, size_t workspace_bytes, void* stream);
+EACS_API size_t eacs_norm_bwd_workspace_size(const EacsNorm* p);
+
 /* Failure-path check (no counterpart in the reference): one CTA waits, with
  * the library's bounded waits (CTA scope and cluster scope) limited to
  * `polls` polls (1..65536), on an mbarrier phase that nothing completes.

@@ -69,7 +69,10 @@ int eacs_device_status(int* status, void* stream) {
     int e = 0;
     rc = eacs::cuda_check(eacs::planes_read_status(&e, s), "eacs_device_status");
     if (rc) return rc;
-    *status = a ? a : (b ? b : (c ? c : (d ? d : e)));
+    int f = 0;
+    rc = eacs::cuda_check(eacs::selective_read_status(&f, s), "eacs_device_status");
+    if (rc) return rc;
+    *status = a ? a : (b ? b : (c ? c : (d ? d : (e ? e : f))));
     return EACS_OK;
 }
 
@@ -131,6 +134,67 @@ int eacs_delta_bwd(const EacsDelta* p, const void* dout, const int64_t* dout_str
 int eacs_delta_step(const EacsDelta* p, void* o, float* final_state, void* stream) {
     if (!p) return eacs::fail(EACS_ERR_INVALID, "eacs_delta_step: null arguments");
     return eacs::delta_step(*p, o, final_state, static_cast<cudaStream_t>(stream));
+}
+
+size_t eacs_selective_ckpt_size(const EacsSelective* p) { return p ? eacs::selective_ckpt_size(*p) : 0; }
+
+int eacs_selective_fwd(const EacsSelective* p, void* y, float* final_state, void* checkpoints, size_t checkpoint_bytes,
+                       void* stream) {
+    if (!p) return eacs::fail(EACS_ERR_INVALID, "eacs_selective_fwd: null arguments");
+    return eacs::selective_fwd(*p, y, final_state, checkpoints, checkpoint_bytes, static_cast<cudaStream_t>(stream));
+}
+
+size_t eacs_selective_bwd_workspace_size(const EacsSelective* p) {
+    return p ? eacs::selective_bwd_workspace_size(*p) : 0;
+}
+
+int eacs_selective_bwd(const EacsSelective* p, const void* dy, const int64_t* dy_stride, const float* dfinal, void* dx,
+                       void* ddt, void* dz, void* dB, void* dC, float* dA, float* dskip, float* ddt_bias,
+                       float* dinitial, const void* checkpoints, size_t checkpoint_bytes, void* workspace,
+                       size_t workspace_bytes, void* stream) {
+    if (!p || !dy_stride) return eacs::fail(EACS_ERR_INVALID, "eacs_selective_bwd: null arguments");
+    eacs::SelectiveGrads g{dy, {dy_stride[0], dy_stride[1]}, dfinal, dx, ddt, dz, dB, dC, dA, dskip, ddt_bias, dinitial};
+    return eacs::selective_bwd(*p, g, checkpoints, checkpoint_bytes, workspace, workspace_bytes,
+                               static_cast<cudaStream_t>(stream));
+}
+
+int eacs_selective_step(const EacsSelective* p, void* y, float* state, void* stream) {
+    if (!p) return eacs::fail(EACS_ERR_INVALID, "eacs_selective_step: null arguments");
+    return eacs::selective_step(*p, y, state, static_cast<cudaStream_t>(stream));
+}
+
+int eacs_conv_fwd(const EacsConv* p, void* y, void* final_state, void* stream) {
+    if (!p) return eacs::fail(EACS_ERR_INVALID, "eacs_conv_fwd: null arguments");
+    return eacs::conv_fwd(*p, y, final_state, static_cast<cudaStream_t>(stream));
+}
+
+size_t eacs_conv_bwd_workspace_size(const EacsConv* p) { return p ? eacs::conv_bwd_workspace_size(*p) : 0; }
+
+int eacs_conv_bwd(const EacsConv* p, const void* dy, const int64_t* dy_stride, const void* dfinal, void* dx, void* dweight,
+                  void* dbias, void* dinitial, void* workspace, size_t workspace_bytes, void* stream) {
+    if (!p || !dy_stride) return eacs::fail(EACS_ERR_INVALID, "eacs_conv_bwd: null arguments");
+    eacs::ConvGrads g{dy, {dy_stride[0], dy_stride[1]}, dfinal, dx, dweight, dbias, dinitial};
+    return eacs::conv_bwd(*p, g, workspace, workspace_bytes, static_cast<cudaStream_t>(stream));
+}
+
+int eacs_conv_step(const EacsConv* p, void* y, void* state, void* stream) {
+    if (!p) return eacs::fail(EACS_ERR_INVALID, "eacs_conv_step: null arguments");
+    return eacs::conv_step(*p, y, state, static_cast<cudaStream_t>(stream));
+}
+
+int eacs_norm_fwd(const EacsNorm* p, void* y, void* s, void* stream) {
+    if (!p) return eacs::fail(EACS_ERR_INVALID, "eacs_norm_fwd: null arguments");
+    return eacs::norm_fwd(*p, y, s, static_cast<cudaStream_t>(stream));
+}
+
+size_t eacs_norm_bwd_workspace_size(const EacsNorm* p) { return p ? eacs::norm_bwd_workspace_size(*p) : 0; }
+
+int eacs_norm_bwd(const EacsNorm* p, const void* dy, int64_t dy_stride, const void* ds, int64_t ds_stride, void* dx,
+                  void* dgate, void* dresidual, void* dweight, void* dscale, void* dpost_weight, void* workspace,
+                  size_t workspace_bytes, void* stream) {
+    if (!p) return eacs::fail(EACS_ERR_INVALID, "eacs_norm_bwd: null arguments");
+    eacs::NormGrads g{dy, dy_stride, ds, ds_stride, dx, dgate, dresidual, dweight, dscale, dpost_weight};
+    return eacs::norm_bwd(*p, g, workspace, workspace_bytes, static_cast<cudaStream_t>(stream));
 }
 
 int eacs_wait_selftest(int polls, void* stream) {

@@ -227,10 +227,6 @@ __device__ __forceinline__ void gate_store(void* p, int dtype, int64_t i, float 
 }
 __device__ __forceinline__ float hold_beta(float b) { return fabsf(b) < kBetaMin ? kBetaMin : b; }
 
-__device__ __forceinline__ void cp_async16(void* smem, const void* gmem, bool valid) {
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(smem)), "l"(gmem), "r"(valid ? 16 : 0)
-                 : "memory");
-}
 template <int N>
 __device__ __forceinline__ void cp_async_wait_group() {
     asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");

@@ -202,6 +202,12 @@ template <typename T> __device__ __forceinline__ float to_f32(T v);
 template <> __device__ __forceinline__ float to_f32<float>(float v) { return v; }
 template <> __device__ __forceinline__ float to_f32<__half>(__half v) { return __half2float(v); }
 template <> __device__ __forceinline__ float to_f32<__nv_bfloat16>(__nv_bfloat16 v) { return __bfloat162float(v); }
+template <typename T> __device__ __forceinline__ T from_f32(float v);
+template <> __device__ __forceinline__ float from_f32<float>(float v) { return v; }
+template <> __device__ __forceinline__ __half from_f32<__half>(float v) { return __float2half_rn(v); }
+template <> __device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float v) {
+    return __float2bfloat16_rn(v);
+}
 
 // ----------------------------------------------------------------------------
 // mbarrier + TMA (cp.async.bulk[.tensor]) wrappers; every copy targets this
@@ -304,7 +310,7 @@ __device__ __forceinline__ void st_async_f32(uint32_t raddr, float v, uint32_t r
                  : "memory");
 }
 
-// Asynchronous global -> shared copies of 4 or 8 bytes (cp.async); with
+// Asynchronous global -> shared copies of 4, 8 or 16 bytes (cp.async); with
 // `valid` false nothing is read and the destination is zero-filled.
 __device__ __forceinline__ void cp_async4(void* smem, const void* gmem, bool valid) {
     asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(smem_u32(smem)), "l"(gmem),
@@ -314,6 +320,11 @@ __device__ __forceinline__ void cp_async4(void* smem, const void* gmem, bool val
 __device__ __forceinline__ void cp_async8(void* smem, const void* gmem, bool valid) {
     asm volatile("cp.async.ca.shared.global [%0], [%1], 8, %2;" ::"r"(smem_u32(smem)), "l"(gmem),
                  "r"(valid ? 8 : 0)
+                 : "memory");
+}
+__device__ __forceinline__ void cp_async16(void* smem, const void* gmem, bool valid) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(smem)), "l"(gmem),
+                 "r"(valid ? 16 : 0)
                  : "memory");
 }
 __device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }

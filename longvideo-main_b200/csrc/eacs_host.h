@@ -367,6 +367,46 @@ int delta_bwd(const EacsDelta& p, const DeltaGrads& d, const void* saved, size_t
 int delta_step(const EacsDelta& p, void* o, float* final_state, cudaStream_t stream);
 cudaError_t planes_read_status(int* out, cudaStream_t stream);
 
+// selective.cu: the selective state space scan
+struct SelectiveGrads {
+    const void* dy;
+    int64_t dy_stride[2];
+    const float* dfinal;  // or null
+    void *dx, *ddt, *dz, *dB, *dC;
+    float *dA, *dskip, *ddt_bias, *dinitial;  // the last three may be null
+};
+size_t selective_ckpt_size(const EacsSelective& p);
+size_t selective_bwd_workspace_size(const EacsSelective& p);
+int selective_fwd(const EacsSelective& p, void* y, float* final_state, void* ckpt, size_t ckpt_bytes, cudaStream_t stream);
+int selective_bwd(const EacsSelective& p, const SelectiveGrads& g, const void* ckpt, size_t ckpt_bytes, void* ws,
+                  size_t ws_bytes, cudaStream_t stream);
+int selective_step(const EacsSelective& p, void* y, float* state, cudaStream_t stream);
+cudaError_t selective_read_status(int* out, cudaStream_t stream);
+
+// conv.cu: the short causal convolution
+struct ConvGrads {
+    const void* dy;
+    int64_t dy_stride[2];
+    const void* dfinal;  // or null
+    void *dx, *dweight, *dbias, *dinitial;  // the last three may be null
+};
+size_t conv_bwd_workspace_size(const EacsConv& p);
+int conv_fwd(const EacsConv& p, void* y, void* final_state, cudaStream_t stream);
+int conv_bwd(const EacsConv& p, const ConvGrads& g, void* ws, size_t ws_bytes, cudaStream_t stream);
+int conv_step(const EacsConv& p, void* y, void* state, cudaStream_t stream);
+
+// block_norm.cu: norms before and after a block, its gate and its scaled residual
+struct NormGrads {
+    const void* dy;  // or null
+    int64_t dy_stride;
+    const void* ds;  // or null
+    int64_t ds_stride;
+    void *dx, *dgate, *dresidual, *dweight, *dscale, *dpost_weight;
+};
+size_t norm_bwd_workspace_size(const EacsNorm& p);
+int norm_fwd(const EacsNorm& p, void* y, void* s, cudaStream_t stream);
+int norm_bwd(const EacsNorm& p, const NormGrads& g, void* ws, size_t ws_bytes, cudaStream_t stream);
+
 // train.cu
 struct TrainBwdCall {
     const void* lam;

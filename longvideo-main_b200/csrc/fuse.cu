@@ -48,11 +48,6 @@ __device__ __forceinline__ void load_vec(const T* p, float* f) {
     for (int i = 0; i < Vec<T>::E; ++i) f[i] = to_f32(e[i]);
 }
 
-template <typename T> __device__ __forceinline__ T from_f32(float v);
-template <> __device__ __forceinline__ float from_f32<float>(float v) { return v; }
-template <> __device__ __forceinline__ __half from_f32<__half>(float v) { return __float2half_rn(v); }
-template <> __device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
-
 template <typename T>
 __device__ __forceinline__ void store_vec(T* p, const float* f) {
     uint4 raw;

@@ -21,16 +21,10 @@
 
 #include "eacs_common.cuh"
 #include "eacs_host.h"
+#include "row_common.cuh"
 
 namespace eacs {
 namespace {
-
-template <typename T> __device__ __forceinline__ T ln_from_f32(float v);
-template <> __device__ __forceinline__ float ln_from_f32<float>(float v) { return v; }
-template <> __device__ __forceinline__ __half ln_from_f32<__half>(float v) { return __float2half_rn(v); }
-template <> __device__ __forceinline__ __nv_bfloat16 ln_from_f32<__nv_bfloat16>(float v) {
-    return __float2bfloat16_rn(v);
-}
 
 struct LnArgs {
     const void* x;
@@ -44,43 +38,6 @@ struct LnArgs {
     int d, w_dtype;
     float eps;
 };
-
-__device__ __forceinline__ float ln_param(const void* p, int dtype, int i, float none) {
-    if (!p) return none;
-    if (dtype == EACS_DTYPE_F32) return static_cast<const float*>(p)[i];
-    if (dtype == EACS_DTYPE_F16) return __half2float(static_cast<const __half*>(p)[i]);
-    return __bfloat162float(static_cast<const __nv_bfloat16*>(p)[i]);
-}
-
-// VEC elements moved as one access (16 bytes, or a single element)
-template <typename T, int VEC> struct alignas(VEC * sizeof(T)) LnVec { T e[VEC]; };
-
-// The barrier of the TPR threads that share a row: the CTA's, or one of its own
-// for each group (their numbers of rows may differ).
-template <int TPR>
-__device__ __forceinline__ void row_barrier() {
-    if (TPR < static_cast<int>(blockDim.x))
-        asm volatile("bar.sync %0, %1;" ::"r"(1 + static_cast<int>(threadIdx.x) / TPR), "n"(TPR) : "memory");
-    else
-        __syncthreads();
-}
-// Sum over those threads; slot alternates so that one barrier a reduction is
-// enough.  `red` is the group's own.
-template <int TPR>
-__device__ __forceinline__ float row_sum(float v, float* red, int& slot) {
-    v = warp_sum(v);
-    if constexpr (TPR > 32) {
-        constexpr int W = TPR / 32;
-        float* r = red + slot * W;
-        slot ^= 1;
-        if ((threadIdx.x & 31) == 0) r[threadIdx.x / 32 % W] = v;
-        row_barrier<TPR>();
-        v = 0.f;
-#pragma unroll
-        for (int i = 0; i < W; ++i) v += r[i];
-    }
-    return v;
-}
 
 // Three sums at once.  `red` is read a barrier before it is written again: the
 // row's other sum lies between.
@@ -109,16 +66,16 @@ __device__ __forceinline__ void row_sums3(float* v, float* red) {
 // (16-bit values two to a register) and taken to float32 where they are used.
 template <typename T, int VEC, int VPL, int TPR>
 struct LnRow {
-    LnVec<T, VEC> raw[VPL];
+    RowVec<T, VEC> raw[VPL];
     __device__ __forceinline__ void read(const T* p, int d, int t) {
 #pragma unroll
         for (int k = 0; k < VPL; ++k) {
             const int i0 = (k * TPR + t) * VEC;
             if (i0 < d) {
-                raw[k] = *reinterpret_cast<const LnVec<T, VEC>*>(p + i0);
+                raw[k] = *reinterpret_cast<const RowVec<T, VEC>*>(p + i0);
             } else {
 #pragma unroll
-                for (int e = 0; e < VEC; ++e) raw[k].e[e] = ln_from_f32<T>(0.f);
+                for (int e = 0; e < VEC; ++e) raw[k].e[e] = from_f32<T>(0.f);
             }
         }
     }
@@ -145,64 +102,15 @@ struct LnSum {
     }
 };
 
-// Weight (or bias) as float32.  In shared memory a thread's values of one vector
-// are float4s that lie TPR apart: no two lanes meet in a bank.  With 512 threads
-// a row a thread's share (at most 16 values) stays in its registers instead.
-template <int VEC, int VPL, int TPR>
-struct LnParam {
-    static constexpr bool kShared = TPR < 512;
-    static constexpr int E = VEC < 4 ? 1 : 4, Q = VEC / E;
-    static constexpr int kFloats = kShared ? VPL * TPR * VEC : 4;
-    float* s;
-    float r[kShared ? 1 : VPL][VEC];
-    __device__ __forceinline__ void fill(float* smem, const void* p, int dtype, int d, float none) {
-        s = smem;
-        if constexpr (kShared) {
-            const int t = threadIdx.x % TPR;
-            for (int k = threadIdx.x / TPR; k < VPL; k += blockDim.x / TPR)  // dealt to the CTA's groups
-#pragma unroll
-                for (int e = 0; e < VEC; ++e) {
-                    const int i = (k * TPR + t) * VEC + e;
-                    s[((k * Q + e / E) * TPR + t) * E + e % E] = i < d ? ln_param(p, dtype, i, none) : 0.f;
-                }
-        } else {
-#pragma unroll
-            for (int k = 0; k < VPL; ++k)
-#pragma unroll
-                for (int e = 0; e < VEC; ++e) {
-                    const int i = (k * TPR + static_cast<int>(threadIdx.x)) * VEC + e;
-                    r[k][e] = i < d ? ln_param(p, dtype, i, none) : 0.f;
-                }
-        }
-    }
-    __device__ __forceinline__ void get(float* v, int k, int t) const {
-        if constexpr (!kShared) {
-#pragma unroll
-            for (int e = 0; e < VEC; ++e) v[e] = r[k][e];
-        } else if constexpr (E == 4) {
-#pragma unroll
-            for (int q = 0; q < Q; ++q) {
-                const float4 f = reinterpret_cast<const float4*>(s)[(k * Q + q) * TPR + t];
-                v[4 * q] = f.x;
-                v[4 * q + 1] = f.y;
-                v[4 * q + 2] = f.z;
-                v[4 * q + 3] = f.w;
-            }
-        } else {
-            v[0] = s[k * TPR + t];
-        }
-    }
-};
-
 // CTAs of RPC groups of TPR threads; a group takes every (grid RPC)th row.  Loads
 // are kept in flight by the number of warps, not by reading a row ahead: that
 // takes the registers of half the warps (measured on 65536 bf16 rows of 1024: 64
 // us ahead, 49 without; the backward at 768: 144 and 72).
 template <typename T, int VEC, int VPL, int TPR, int RPC, bool RES, int CTAS>
 __global__ void __launch_bounds__(TPR * RPC, CTAS) ln_fwd_k(LnArgs a) {
-    using V = LnVec<T, VEC>;
+    using V = RowVec<T, VEC>;
     using Row = LnRow<T, VEC, VPL, TPR>;
-    using Par = LnParam<VEC, VPL, TPR>;
+    using Par = RowParam<VEC, VPL, TPR>;
     __shared__ float reds[RPC][2 * (TPR / 32)];
     __shared__ __align__(16) float sw[Par::kFloats], sb[Par::kFloats];
     Par w, b;
@@ -251,7 +159,7 @@ __global__ void __launch_bounds__(TPR * RPC, CTAS) ln_fwd_k(LnArgs a) {
                 b.get(bv, k, t);
                 V o;
 #pragma unroll
-                for (int e = 0; e < VEC; ++e) o.e[e] = ln_from_f32<T>(fmaf((s.at(k, e) - mean) * rstd, wv[e], bv[e]));
+                for (int e = 0; e < VEC; ++e) o.e[e] = from_f32<T>(fmaf((s.at(k, e) - mean) * rstd, wv[e], bv[e]));
                 *reinterpret_cast<V*>(y + i0) = o;
             }
         }
@@ -270,15 +178,11 @@ struct LnStage {
     static constexpr size_t bytes = on ? static_cast<size_t>(RPC) * 2 * kRows * kRow : 0;
 };
 
-__device__ __forceinline__ void ln_cp16(void* smem, const void* gmem) {
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(smem)), "l"(gmem) : "memory");
-}
-
 template <typename T, int VEC, int VPL, int TPR, int RPC, bool RES, int CTAS>
 __global__ void __launch_bounds__(TPR * RPC, CTAS) ln_bwd_k(LnArgs a) {
-    using V = LnVec<T, VEC>;
+    using V = RowVec<T, VEC>;
     using Row = LnRow<T, VEC, VPL, TPR>;
-    using Par = LnParam<VEC, VPL, TPR>;
+    using Par = RowParam<VEC, VPL, TPR>;
     using St = LnStage<T, VEC, VPL, TPR, RPC, RES>;
     __shared__ float reds[RPC][5 * (TPR / 32)];
     __shared__ __align__(16) float sw[Par::kFloats];
@@ -303,9 +207,9 @@ __global__ void __launch_bounds__(TPR * RPC, CTAS) ln_bwd_k(LnArgs a) {
             for (int k = 0; k < VPL; ++k) {
                 const int i0 = (k * TPR + t) * VEC;
                 if (i < a.rows && i0 < a.d) {
-                    ln_cp16(at(s, 0, k), x + i * a.sx + i0);
-                    ln_cp16(at(s, 1, k), dy + i * a.sdy + i0);
-                    if constexpr (RES) ln_cp16(at(s, 2, k), r + i * a.sr + i0);
+                    row_cp16(at(s, 0, k), x + i * a.sx + i0);
+                    row_cp16(at(s, 1, k), dy + i * a.sdy + i0);
+                    if constexpr (RES) row_cp16(at(s, 2, k), r + i * a.sr + i0);
                 }
             }
             cp_async_commit();
@@ -396,7 +300,7 @@ __global__ void __launch_bounds__(TPR * RPC, CTAS) ln_bwd_k(LnArgs a) {
                     const float h = (v[e] - mean) * rstd;
                     dw[k][e] = fmaf(g[e], h, dw[k][e]);
                     db[k][e] += g[e];
-                    o.e[e] = ln_from_f32<T>((fmaf(g[e], wv[e], -s1) - h * s2) * rstd);
+                    o.e[e] = from_f32<T>((fmaf(g[e], wv[e], -s1) - h * s2) * rstd);
                 }
                 *reinterpret_cast<V*>(dx + i0) = o;
             }
@@ -436,32 +340,6 @@ __global__ void __launch_bounds__(TPR * RPC, CTAS) ln_bwd_k(LnArgs a) {
     }
 }
 
-// dweight and dbias: sums of `n` partial rows, 32 columns a CTA (one a lane),
-// the rows dealt to the 32 warps and their sums added in order.
-__global__ void __launch_bounds__(1024) ln_reduce_k(const float* __restrict__ part, int n, int d, void* dw, void* db,
-                                                    int w_dtype) {
-    __shared__ float s[32][33];
-    const int lane = threadIdx.x & 31, wid = threadIdx.x >> 5;
-    const int i = blockIdx.x * 32 + lane;
-    void* out = blockIdx.y ? db : dw;
-    if (!out) return;
-    const float* p = part + blockIdx.y * static_cast<int64_t>(d) + i;
-    float v = 0.f;
-    if (i < d) {
-#pragma unroll 8
-        for (int r = wid; r < n; r += 32) v += p[static_cast<int64_t>(r) * 2 * d];
-    }
-    s[wid][lane] = v;
-    __syncthreads();
-    v = warp_sum(s[lane][wid]);  // column wid of this CTA
-    const int c = blockIdx.x * 32 + wid;
-    if (lane == 0 && c < d) {
-        if (w_dtype == EACS_DTYPE_F32) static_cast<float*>(out)[c] = v;
-        else if (w_dtype == EACS_DTYPE_F16) static_cast<__half*>(out)[c] = __float2half_rn(v);
-        else static_cast<__nv_bfloat16*>(out)[c] = __float2bfloat16_rn(v);
-    }
-}
-
 constexpr int kLnMaxD = 8192;
 
 // The backward's CTAs an SM at most: its grid is also the number of partial rows
@@ -469,25 +347,12 @@ constexpr int kLnMaxD = 8192;
 constexpr int kLnBwdCtas = 6;
 constexpr int kLnMaxParts = 148 * kLnBwdCtas;
 
-// Grid: every row its group while the rows last, at most the CTAs that are
-// resident at once (each then loops over rows, so that the weight is read and the
-// sums are kept on the SM, and no second round of CTAs runs half empty).
-template <typename K>
-int ln_resident(K kernel, int threads, size_t smem) {
-    int n = 0;
-    if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, kernel, threads, smem) != cudaSuccess) n = 1;
-    return n < 1 ? 1 : n;
-}
-int ln_grid(int64_t rows, int rpc, int per_sm) {
-    return static_cast<int>(std::min<int64_t>((rows + rpc - 1) / rpc, int64_t{148} * per_sm));
-}
-
 template <typename T, int VEC, int VPL, int TPR, int RPC, bool RES>
 cudaError_t ln_fwd_launch(const LnArgs& a, cudaStream_t s) {
     // registers for three CTAs an SM where a lane keeps its sums of two rows in float32
     constexpr int ctas = RPC == 1 || !RES ? 1 : 3;
-    static const int per = ln_resident(ln_fwd_k<T, VEC, VPL, TPR, RPC, RES, ctas>, TPR * RPC, 0);
-    ln_fwd_k<T, VEC, VPL, TPR, RPC, RES, ctas><<<ln_grid(a.rows, RPC, per), TPR * RPC, 0, s>>>(a);
+    static const int per = row_resident(ln_fwd_k<T, VEC, VPL, TPR, RPC, RES, ctas>, TPR * RPC, 0);
+    ln_fwd_k<T, VEC, VPL, TPR, RPC, RES, ctas><<<row_grid(a.rows, RPC, per), TPR * RPC, 0, s>>>(a);
     note_launch();
     return cudaGetLastError();
 }
@@ -499,8 +364,8 @@ cudaError_t ln_bwd_launch(const LnArgs& a, int* parts, cudaStream_t s) {
     const auto k = ln_bwd_k<T, VEC, VPL, TPR, RPC, RES, ctas>;
     const cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
     if (e != cudaSuccess) return e;
-    static const int per = std::min(ln_resident(k, TPR * RPC, smem), kLnBwdCtas);
-    *parts = ln_grid(a.rows, RPC, per);
+    static const int per = std::min(row_resident(k, TPR * RPC, smem), kLnBwdCtas);
+    *parts = row_grid(a.rows, RPC, per);
     k<<<*parts, TPR * RPC, smem, s>>>(a);
     note_launch();
     return cudaGetLastError();
@@ -611,9 +476,10 @@ int layer_norm(const LayerNormCall& c, cudaStream_t stream) {
     else if (c.dtype == EACS_DTYPE_BF16) e = ln_dispatch<__nv_bfloat16>(a, vec, c.backward, &parts, stream);
     else e = ln_dispatch<float>(a, vec, c.backward, &parts, stream);
     if (e == cudaSuccess && want) {
-        ln_reduce_k<<<dim3((a.d + 31) / 32, 2), 1024, 0, stream>>>(a.part, parts, a.d, c.dweight, c.dbias, c.w_dtype);
-        note_launch();
-        e = cudaGetLastError();
+        RowSums r{};
+        r.part = a.part, r.rows = parts, r.stride = 2 * static_cast<int64_t>(a.d), r.dtype = c.w_dtype;
+        r.out[0] = c.dweight, r.out[1] = c.dbias, r.at[1] = a.d, r.n[0] = r.n[1] = a.d;
+        e = row_sums(r, 2, stream);
     }
     return cuda_check(e, fn);
 }

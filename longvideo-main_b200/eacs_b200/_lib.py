@@ -38,6 +38,15 @@ _SZ = ctypes.c_size_t
 # a short launch.)
 DELTA = struct.Struct("=5Q15q2Q6qf2i4x")
 DELTA_PATH = struct.Struct("=5Q15q2Q6qf3i")  # with the path of the kernels named
+# EacsSelective: 5 pointers, their strides over row and token, A, skip, dt_bias,
+# lengths and initial_state, rows, L, D, N, type, softplus
+SELECTIVE = struct.Struct("=5Q10q5Q4q2i")
+# EacsConv: x, weight, bias, initial_state and lengths, x's strides, rows, L, D,
+# width, type, the weight's type, silu
+CONV = struct.Struct("=5Q5q4i")
+# EacsNorm: x, gate, residual, weight, scale and post_weight, three row strides,
+# rows, d, eps, type, the weights' type, post_norm
+NORM = struct.Struct("=6Q5qf3i")
 
 
 # name -> (restype, argtypes); mirrors include/eacs_b200.h
@@ -60,6 +69,18 @@ SIGNATURES = {
     "eacs_delta_bwd": (_I, [_P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _SZ, _P, _SZ, _P]),
     "eacs_delta_bwd_workspace_size": (_SZ, [_P]),
     "eacs_delta_step": (_I, [_P, _P, _P, _P]),
+    "eacs_selective_fwd": (_I, [_P, _P, _P, _P, _SZ, _P]),
+    "eacs_selective_ckpt_size": (_SZ, [_P]),
+    "eacs_selective_bwd": (_I, [_P] * 14 + [_SZ, _P, _SZ, _P]),
+    "eacs_selective_bwd_workspace_size": (_SZ, [_P]),
+    "eacs_selective_step": (_I, [_P, _P, _P, _P]),
+    "eacs_conv_fwd": (_I, [_P, _P, _P, _P]),
+    "eacs_conv_bwd": (_I, [_P] * 9 + [_SZ, _P]),
+    "eacs_conv_bwd_workspace_size": (_SZ, [_P]),
+    "eacs_conv_step": (_I, [_P, _P, _P, _P]),
+    "eacs_norm_fwd": (_I, [_P, _P, _P, _P]),
+    "eacs_norm_bwd": (_I, [_P, _P, _I64, _P, _I64] + [_P] * 7 + [_SZ, _P]),
+    "eacs_norm_bwd_workspace_size": (_SZ, [_P]),
     "eacs_set_kernel_events": (_I, [_P, _P]),
     "eacs_scan_fwd": (_I, [_P, _P, _P, _I64, _I64, _I64, _I64, _P]),
     "eacs_scan_bwd": (_I, [_P, _P, _P, _P, _P, _I64, _I64, _I64, _I64, _P]),

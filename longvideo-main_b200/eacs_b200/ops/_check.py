@@ -59,3 +59,10 @@ def one_device(name: str, first: torch.Tensor, *ts: torch.Tensor | None) -> torc
                                                 for t in ts):
         return cuda_tensors(name, first, *(t for t in ts if t is not None))
     return dev
+
+
+def dense_last(t: torch.Tensor) -> torch.Tensor:
+    """t, copied if its last dimension is not dense."""
+    if t.stride(-1) == 1 or t.shape[-1] == 1:
+        return t
+    return t.contiguous()

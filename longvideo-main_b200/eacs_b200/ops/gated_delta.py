@@ -42,16 +42,10 @@ import torch
 from torch import Tensor
 
 from .. import _lib
-from ._check import on, one_device, require_plain
+from ._check import dense_last, on, one_device, require_plain
 
 MAX_K = 128
 MAX_V = 1024
-
-
-def _dense_last(t: Tensor) -> Tensor:
-    if t.stride(-1) == 1 or t.shape[-1] == 1:
-        return t
-    return t.contiguous()
 
 
 def _check(name, q, k, v, g, beta, lengths, state, lead):
@@ -135,7 +129,7 @@ class GatedDeltaFunction(torch.autograd.Function):
         if do.data_ptr() % 16:  # a view that starts inside an allocation
             do = do.clone()
         dfinal = None if dfinal is None else dfinal.contiguous()
-        q, k, v = _dense_last(q), _dense_last(k), _dense_last(v)
+        q, k, v = dense_last(q), dense_last(k), dense_last(v)
         lengths, initial = (None if t is None else t.contiguous() for t in (lengths, initial))
         L_ = _lib.lib()
         p = _args(q, k, v, g, beta, ctx.scale, lengths, initial, ctx.path)
@@ -167,7 +161,7 @@ def gated_delta_rule(q: Tensor, k: Tensor, v: Tensor, g: Tensor, beta: Tensor, s
     initial_state, through o and the final state."""
     dev = _check("gated_delta_rule", q, k, v, g, beta, lengths, initial_state, 2)
     scale = q.shape[-1] ** -0.5 if scale is None else float(scale)
-    q, k, v = _dense_last(q), _dense_last(k), _dense_last(v)
+    q, k, v = dense_last(q), dense_last(k), dense_last(v)
     lengths = None if lengths is None else lengths.contiguous()
     state = None if initial_state is None else initial_state.contiguous()
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (q, k, v, g, beta, state)):
@@ -188,7 +182,7 @@ def gated_delta_step(q: Tensor, k: Tensor, v: Tensor, g: Tensor, beta: Tensor, s
     if not state.is_contiguous() or state.requires_grad:
         raise RuntimeError("gated_delta_step: the state is updated in place: it must be contiguous and without a gradient")
     scale = q.shape[-1] ** -0.5 if scale is None else float(scale)
-    q, k, v = _dense_last(q), _dense_last(k), _dense_last(v)
+    q, k, v = dense_last(q), dense_last(k), dense_last(v)
     o = torch.empty(v.shape, dtype=q.dtype, device=dev)
     p = _args(q, k, v, g, beta, scale, None, state)
     with on(dev):
