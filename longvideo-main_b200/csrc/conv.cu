@@ -356,8 +356,8 @@ int conv_check(const char* fn, const EacsConv& p, bool single) {
         if (dt != EACS_DTYPE_F32 && dt != EACS_DTYPE_F16 && dt != EACS_DTYPE_BF16)
             return fail(EACS_ERR_INVALID, "%s: unknown dtype %d", fn, dt);
     if (p.width < 2 || p.width > kConvMaxWidth) return fail(EACS_ERR_UNSUPPORTED, "%s: %d taps, not 2 to %d", fn, p.width, kConvMaxWidth);
-    if (p.rows > 65535 || p.D > (int64_t{1} << 24) || p.L > (int64_t{1} << 31))
-        return fail(EACS_ERR_UNSUPPORTED, "%s: more than 65535 rows, 2^24 channels or 2^31 tokens", fn);
+    if (p.rows > 65535 || p.D > (int64_t{1} << 24) || p.L > (int64_t{1} << 30))
+        return fail(EACS_ERR_UNSUPPORTED, "%s: more than 65535 rows, 2^24 channels or 2^30 tokens", fn);
     if (p.rows > 0 && (!p.weight || ((p.L > 0 || single) && !p.x))) return fail(EACS_ERR_INVALID, "%s: null pointer argument", fn);
     return EACS_OK;
 }

@@ -29,7 +29,7 @@
 namespace eacs {
 namespace {
 
-constexpr float kLog2e = 1.44269504f, kLog2eLo = 1.92596303e-8f, kLn2 = 0.693147181f;
+constexpr float kLog2e = 1.44269504f, kLn2 = 0.693147181f;
 
 // ---- pairs of float32 ---------------------------------------------------------------------------------
 using f32x2 = unsigned long long;
@@ -64,35 +64,24 @@ __device__ __forceinline__ f32x2 ex2_pair(f32x2 v) {
 struct alignas(16) Quad { f32x2 lo, hi; };  // four states
 
 // ---- a token's step and gate ----------------------------------------------------------------------------
-// e^-|v|: the argument's rounding is put right to first order (without that it is off by |v| 2^-24).
-__device__ __forceinline__ float exp_neg_abs(float v) {
-    const float t = -fabsf(v);
-    const float p = t * kLog2e;
-    const float r = fmaf(t, kLog2eLo, fmaf(t, kLog2e, -p));
-    const float u = ex2_approx(p);
-    return p > -126.0f ? fmaf(u, r * kLn2, u) : u;  // (r has no value where p is infinite)
-}
-// softplus(v) = max(v, 0) + log(1 + u), u = e^-|v|, with log(1 + u) = 2 artanh(q), q = u / (2 + u) <= 1/3, from its series
-// to q^13 (the first term left out is 1.4e-8 of the sum): relatively exact for the small steps that v << 0 gives, where
-// log(1 + u) taken from the rounded 1 + u is not.  slope is its derivative.
+// softplus(v) = max(v, 0) + log(1 + u) with u = e^-|v| and log(1 + u) = 2 artanh(q), q = u / (2 + u) <= 1/3: relatively
+// exact for the small steps that v << 0 gives, where log(1 + u) taken from the rounded 1 + u is not.  2 artanh(q) / q is a
+// polynomial of degree 4 in q^2, fitted on [0, 1/9] at Chebyshev's points (8e-9 of the value).  u's argument is put right
+// for its rounding to first order (without that u is off by |v| 2^-24); below e^-87 u stays there.  slope is the derivative.
 __device__ __forceinline__ float softplus(float v, float& slope) {
-    const float u = exp_neg_abs(v);
+    const float t = fmaxf(-fabsf(v), -87.0f), p0 = t * kLog2e;
+    float u = ex2_approx(p0);
+    u = fmaf(u * fmaf(t, kLog2e, -p0), kLn2, u);
     const float q = __fdividef(u, 2.0f + u), q2 = q * q;
-    float p = fmaf(q2, 1.0f / 13, 1.0f / 11);
-    p = fmaf(q2, p, 1.0f / 9);
-    p = fmaf(q2, p, 1.0f / 7);
-    p = fmaf(q2, p, 1.0f / 5);
-    p = fmaf(q2, p, 1.0f / 3);
-    p = fmaf(q2, p, 1.0f);
+    float p = fmaf(q2, 0.2817465663f, 0.2796141803f);
+    p = fmaf(q2, p, 0.4002485275f);
+    p = fmaf(q2, p, 0.6666631699f);
+    p = fmaf(q2, p, 2.0f);
     const float inv = __fdividef(1.0f, 1.0f + u);
     slope = v >= 0.0f ? inv : u * inv;
-    return (v > 0.0f ? v : 0.0f) + 2.0f * q * p;
+    return fmaf(q, p, v < 0.0f ? 0.0f : v);  // (a NaN stays one)
 }
-__device__ __forceinline__ float sigmoid(float v) {
-    const float u = exp_neg_abs(v);
-    const float inv = __fdividef(1.0f, 1.0f + u);
-    return v >= 0.0f ? inv : u * inv;
-}
+__device__ __forceinline__ float sigmoid(float v) { return __fdividef(1.0f, 1.0f + ex2_approx(v * -kLog2e)); }
 
 struct SelArgs {
     const void *x, *dt, *z, *B, *C;      // z may be null
@@ -103,8 +92,7 @@ struct SelArgs {
     void* y;
     float* hN;                           // or null
     float* ckpt;                         // or null: states in front of every 8 tokens, (B, ceil(L / 8), D, 4 LN)
-    int64_t L;
-    int D, N;
+    int L, D, N;
     int softplus;
     int vec, vec_bc;                     // rows of x, dt, z (y, dy ...) / of B, C may be read as vectors
     // backward
@@ -120,35 +108,132 @@ struct SelArgs {
     int groups;                          // groups of channels a CTA
 };
 
-__device__ __forceinline__ int64_t sel_length(const SelArgs& a, int64_t b) {
+__device__ __forceinline__ int sel_length(const SelArgs& a, int64_t b) {
     if (!a.lengths) return a.L;
-    const int64_t n = a.lengths[b];
+    const int n = a.lengths[b];
     return n < 0 ? 0 : (n > a.L ? a.L : n);
 }
 
-// E neighbouring channels of one token as they lie in memory.
-template <typename T, int E> struct alignas(E * sizeof(T) < 16 ? E * sizeof(T) : 16) Run { T e[E]; };
+// E neighbouring channels of one token as they lie in memory, in whole registers: taken apart only where they are used, so
+// that asking for them does not wait for them.
+template <typename T> __device__ __forceinline__ void unpack(uint32_t w, float& a, float& b);
+template <> __device__ __forceinline__ void unpack<__nv_bfloat16>(uint32_t w, float& a, float& b) {
+    a = __uint_as_float(w << 16);
+    b = __uint_as_float(w & 0xffff0000u);
+}
+template <> __device__ __forceinline__ void unpack<__half>(uint32_t w, float& a, float& b) {
+    const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w));
+    a = f.x, b = f.y;
+}
+template <> __device__ __forceinline__ void unpack<float>(uint32_t w, float& a, float& b) { a = __uint_as_float(w), b = 0.f; }
+template <typename T> __device__ __forceinline__ uint32_t pack(float a, float b);
+template <> __device__ __forceinline__ uint32_t pack<__nv_bfloat16>(float a, float b) {
+    const __nv_bfloat162 v = __floats2bfloat162_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&v);
+}
+template <> __device__ __forceinline__ uint32_t pack<__half>(float a, float b) {
+    const __half2 v = __floats2half2_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&v);
+}
+template <> __device__ __forceinline__ uint32_t pack<float>(float a, float) { return __float_as_uint(a); }
 
 template <typename T, int E>
-__device__ __forceinline__ void read_run(Run<T, E>& r, const T* p, bool in, int d, int D, bool vec) {
-    if (in && vec && d + E <= D) {
-        r = *reinterpret_cast<const Run<T, E>*>(p);
-    } else {
+struct Run {
+    static constexpr int kBytes = E * sizeof(T), kWords = (kBytes + 3) / 4, kPer = 4 / sizeof(T);
+    uint32_t w[kWords];
+    // the channels d.. of D; FULL: all of them are there, and vectors may be read
+    template <bool FULL = false>
+    __device__ __forceinline__ void read(const T* p, bool in, int d, int D, bool vec) {
+        if (FULL) {
 #pragma unroll
-        for (int e = 0; e < E; ++e) r.e[e] = in && d + e < D ? p[e] : from_f32<T>(0.f);
+            for (int i = 0; i < kWords; ++i) w[i] = 0;
+        }
+        if (in && (FULL || (vec && d + E <= D))) {
+            if constexpr (kBytes >= 16) {
+#pragma unroll
+                for (int i = 0; i < kWords; i += 4) {
+                    const uint4 v = reinterpret_cast<const uint4*>(p)[i / 4];
+                    w[i] = v.x, w[i + 1] = v.y, w[i + 2] = v.z, w[i + 3] = v.w;
+                }
+            } else if constexpr (kBytes == 8) {
+                const uint2 v = *reinterpret_cast<const uint2*>(p);
+                w[0] = v.x, w[1] = v.y;
+            } else if constexpr (kBytes == 4) {
+                w[0] = *reinterpret_cast<const uint32_t*>(p);
+            } else {
+                w[0] = *reinterpret_cast<const uint16_t*>(p);
+            }
+        } else if (!FULL) {
+#pragma unroll
+            for (int i = 0; i < kWords; ++i) {
+                w[i] = 0;
+#pragma unroll
+                for (int k = 0; k < kPer; ++k) {
+                    const int e = i * kPer + k;
+                    if (e < E && in && d + e < D) {
+                        if constexpr (sizeof(T) == 4) w[i] = reinterpret_cast<const uint32_t*>(p)[e];
+                        else w[i] |= static_cast<uint32_t>(reinterpret_cast<const uint16_t*>(p)[e]) << (16 * k);
+                    }
+                }
+            }
+        }
     }
-}
-template <typename T, int E>
-__device__ __forceinline__ void write_run(const float* v, T* p, int d, int D, bool vec) {
-    if (vec && d + E <= D) {
-        Run<T, E> r;
+    __device__ __forceinline__ void floats(float* v) const {
 #pragma unroll
-        for (int e = 0; e < E; ++e) r.e[e] = from_f32<T>(v[e]);
-        *reinterpret_cast<Run<T, E>*>(p) = r;
+        for (int i = 0; i < kWords; ++i) {
+            float a, b;
+            unpack<T>(w[i], a, b);
+            v[i * kPer] = a;
+            if (kPer == 2 && i * kPer + 1 < E) v[i * kPer + 1] = b;
+        }
+    }
+};
+template <typename T, int E, bool FULL = false>
+__device__ __forceinline__ void write_run(const float* v, T* p, int d, int D, bool vec) {
+    using R = Run<T, E>;
+    if ((FULL || (vec && d + E <= D)) && R::kBytes >= 4) {
+        uint32_t w[R::kWords];
+#pragma unroll
+        for (int i = 0; i < R::kWords; ++i) w[i] = pack<T>(v[i * R::kPer], v[(i * R::kPer + 1) % E]);
+        if constexpr (R::kBytes >= 16) {
+#pragma unroll
+            for (int i = 0; i < R::kWords; i += 4) reinterpret_cast<uint4*>(p)[i / 4] = make_uint4(w[i], w[i + 1], w[i + 2], w[i + 3]);
+        } else if constexpr (R::kBytes == 8) {
+            *reinterpret_cast<uint2*>(p) = make_uint2(w[0], w[1]);
+        } else {
+            *reinterpret_cast<uint32_t*>(p) = w[0];
+        }
     } else {
 #pragma unroll
         for (int e = 0; e < E; ++e)
-            if (d + e < D) p[e] = from_f32<T>(v[e]);
+            if (FULL || d + e < D) p[e] = from_f32<T>(v[e]);
+    }
+}
+
+// E floats to shared memory
+template <int E>
+__device__ __forceinline__ void put_run(float* p, const float* v) {
+    if constexpr (E % 4 == 0) {
+#pragma unroll
+        for (int e = 0; e < E; e += 4) *reinterpret_cast<float4*>(p + e) = make_float4(v[e], v[e + 1], v[e + 2], v[e + 3]);
+    } else if constexpr (E == 2) {
+        *reinterpret_cast<float2*>(p) = make_float2(v[0], v[1]);
+    } else {
+        p[0] = v[0];
+    }
+}
+
+template <int E>
+__device__ __forceinline__ void get_run(float* v, const float* p) {
+    if constexpr (E % 4 == 0) {
+#pragma unroll
+        for (int e = 0; e < E; e += 4) {
+            const float4 q = *reinterpret_cast<const float4*>(p + e);
+            v[e] = q.x, v[e + 1] = q.y, v[e + 2] = q.z, v[e + 3] = q.w;
+        }
+    } else {
+#pragma unroll
+        for (int e = 0; e < E; ++e) v[e] = p[e];
     }
 }
 
@@ -171,7 +256,8 @@ __device__ __forceinline__ Quad quad(float4 v) { return Quad{pair(v.x, v.y), pai
 
 // B and C of a slice of S tokens, by one warp: asked for with cp.async as they lie (where rows allow it), then turned into
 // float32 rows of NP = 4 LN states, zeros behind the row's end and behind N.
-template <typename T, int LN, int S>
+// FULL: rows of NP states that vectors may be read from.
+template <typename T, int LN, int S, bool FULL>
 struct SliceBC {
     static constexpr int NP = 4 * LN, V = 16 / sizeof(T);
     static constexpr size_t kRawBytes = 2 * S * NP * sizeof(T), kBytes = 2 * S * NP * sizeof(float);
@@ -179,37 +265,51 @@ struct SliceBC {
     const T* C;
     T* raw;
     float* out;
-    __device__ __forceinline__ void ask(const SelArgs& a, int64_t t0, int64_t len, int lane) const {
-        if (!a.vec_bc) return;
-        const int per = a.N / V;
-        for (int i = lane; i < S * per; i += 32) {
-            const int r = i / per, c = i - r * per;
-            const bool in = t0 + r < len;
-            const int64_t t = in ? t0 + r : 0;
-            cp_async16(raw + r * NP + c * V, B + t * a.sB[1] + c * V, in);
-            cp_async16(raw + (S + r) * NP + c * V, C + t * a.sC[1] + c * V, in);
+    __device__ __forceinline__ void ask(const SelArgs& a, int t0, int len, int lane) const {
+        if (!FULL && !a.vec_bc) return;
+        constexpr int per = NP / V;  // 16-byte pieces a row, those behind N left out
+        const int64_t oB = t0 * a.sB[1], oC = t0 * a.sC[1];
+#pragma unroll
+        for (int i = 0; i < (S * per + 31) / 32; ++i) {
+            const int k = i * 32 + lane, r = k / per, c = k % per * V;
+            if (k < S * per && (FULL || c < a.N)) {
+                const bool in = t0 + r < len;
+                cp_async16(raw + r * NP + c, B + (in ? oB + r * a.sB[1] : 0) + c, in);
+                cp_async16(raw + (S + r) * NP + c, C + (in ? oC + r * a.sC[1] : 0) + c, in);
+            }
         }
         cp_async_commit();
     }
-    __device__ __forceinline__ void take(const SelArgs& a, int64_t t0, int64_t len, int lane) const {
-        if (a.vec_bc) cp_async_wait_all();
+    __device__ __forceinline__ void take(const SelArgs& a, int t0, int len, int lane) const {
+        if (FULL || a.vec_bc) cp_async_wait_all();
         __syncwarp();
 #pragma unroll
         for (int which = 0; which < 2; ++which) {
             const T* g = which ? C : B;
             const int64_t st = which ? a.sC[1] : a.sB[1];
 #pragma unroll
-            for (int i = lane; i < S * LN; i += 32) {
-                const int r = i / LN, n = i % LN * 4;
-                float v[4];
+            for (int i = 0; i < (S * LN + 31) / 32; ++i) {
+                const int k = i * 32 + lane, r = k / LN, n = k % LN * 4;
+                if (S * LN < 32 && k >= S * LN) break;
+                float v[4] = {};
+                if (FULL || a.vec_bc) {
+                    if (FULL || n < a.N) {
+                        Run<T, 4> q;
+                        q.template read<true>(raw + (which * S + r) * NP + n, true, 0, 4, true);
+                        q.floats(v);
+                    }
+                } else {
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    if (a.vec_bc) v[e] = n < a.N ? to_f32(raw[(which * S + r) * NP + n + e]) : 0.f;
-                    else v[e] = t0 + r < len && n + e < a.N ? to_f32(g[(t0 + r) * st + n + e]) : 0.f;
+                    for (int e = 0; e < 4; ++e)
+                        if (t0 + r < len && n + e < a.N) v[e] = to_f32(g[(t0 + r) * st + n + e]);
                 }
                 *reinterpret_cast<float4*>(out + (which * S + r) * NP + n) = make_float4(v[0], v[1], v[2], v[3]);
             }
         }
+    }
+    __device__ __forceinline__ void b(int t, int ln, float* v) const {
+        const float4 q = *reinterpret_cast<const float4*>(out + t * NP + ln * 4);
+        v[0] = q.x, v[1] = q.y, v[2] = q.z, v[3] = q.w;
     }
     __device__ __forceinline__ Quad b(int t, int ln) const { return *reinterpret_cast<const Quad*>(out + t * NP + ln * 4); }
     __device__ __forceinline__ Quad c(int t, int ln) const { return *reinterpret_cast<const Quad*>(out + (S + t) * NP + ln * 4); }
@@ -218,149 +318,191 @@ struct SliceBC {
 // ---------------------------------------------------------------------------------------------------------
 // forward
 // ---------------------------------------------------------------------------------------------------------
-// A slice is S tokens of CW channels.  Per-token values are worked out in the layout they are read in: lane = (token, half
-// of the channels), E channels a lane; the sweep over the states reads them as (token, channel).  kRot turns the places of a
-// row's channels so that neither side meets in a bank.
+// A slice is S tokens of CW channels, two channels a thread.  A token's values are worked out in the layout they are read
+// in (lane = token and a quarter of the channels, E of them) and handed to the sweep through shared memory.
+// The sweep starts from a state of zero, so that nothing in it waits for the warp before: it leaves the slice's own state,
+// the product P of its decays, its own part of the outputs, and C P of every token.  With the state h handed in, the state
+// handed on is own + P h (all that the ring waits for), and the outputs get (C P) . h.
+// What a thread reads from shared memory (128 bytes a clock and multiprocessor) is what bounds this next to the special
+// function pipe: two channels a thread halve what B and C cost.
 template <int LN>
 struct FwdShape {
-    static constexpr int S = 16, NP = 4 * LN, CW = 32 / LN, E = CW / 2;
-    static constexpr int YS = CW + (E > 1 ? 2 : 1);
-    static __device__ __forceinline__ int place(int t, int c) {
-        const int half = c / E, i = c % E;
-        return t * CW + half * E + ((i + t * CW / 8 + (E == 8 ? half : 0)) & (E - 1));
-    }
+    static constexpr int S = 8, NP = 4 * LN, CW = 64 / LN, E = CW / 4;
+    static constexpr int YS = CW + 4;
 };
 template <typename T, int LN>
 constexpr size_t sel_fwd_warp_bytes() {
     using Sh = FwdShape<LN>;
-    using BC = SliceBC<T, LN, Sh::S>;
-    return BC::kRawBytes + BC::kBytes + Sh::S * Sh::CW * 16 + (Sh::S * Sh::YS * 4 + 15) / 16 * 16 + 512;
+    using BC = SliceBC<T, LN, Sh::S, true>;
+    return BC::kRawBytes + BC::kBytes + 2 * Sh::S * Sh::CW * 4 + Sh::S * Sh::YS * 4;
 }
+// a CTA's own: the states handed on (two channels of 32 lanes a warp), dt_bias and skip of its channels
+template <int LN>
+constexpr size_t sel_fwd_cta_bytes(int W) {
+    return W * 1024 + 2 * FwdShape<LN>::CW * 4;
+}
+constexpr int kSelFwdWarps = 12;  // a multiprocessor's: the registers of one CTA of 12 warps, or of several smaller ones
 
-template <typename T, int LN, bool CKPT>
-__global__ void __launch_bounds__(128, 4) sel_fwd_k(const SelArgs a) {
+// FULL: groups of CW channels and rows of NP states, all of them on 16 bytes
+template <typename T, int LN, bool CKPT, bool FULL>
+__global__ void __launch_bounds__(kSelFwdWarps * 32, 1) sel_fwd_k(const SelArgs a) {
     using Sh = FwdShape<LN>;
-    using BC = SliceBC<T, LN, Sh::S>;
+    using BC = SliceBC<T, LN, Sh::S, FULL>;
     constexpr int S = Sh::S, NP = Sh::NP, CW = Sh::CW, E = Sh::E;
     extern __shared__ __align__(16) unsigned char smem[];
     const int lane = threadIdx.x & 31, w = threadIdx.x >> 5, W = blockDim.x >> 5;
-    unsigned char* mine = smem + static_cast<size_t>(W) * 512 + static_cast<size_t>(w) * (sel_fwd_warp_bytes<T, LN>() - 512);
-    Quad* hop = reinterpret_cast<Quad*>(smem);  // [W][32]: the state that each warp is handed
-    float4* sd = reinterpret_cast<float4*>(mine + BC::kRawBytes + BC::kBytes);  // (s log2 e) twice, (s x) twice
-    float* yb = reinterpret_cast<float*>(mine + BC::kRawBytes + BC::kBytes + S * CW * 16);
+    Quad* hop = reinterpret_cast<Quad*>(smem);  // [W][2][32]: the state that each warp is handed
+    float* pars = reinterpret_cast<float*>(smem + W * 1024);  // [2][CW]: dt_bias, skip
+    unsigned char* mine = smem + sel_fwd_cta_bytes<LN>(W) + static_cast<size_t>(w) * sel_fwd_warp_bytes<T, LN>();
+    float* ss = reinterpret_cast<float*>(mine + BC::kRawBytes + BC::kBytes);  // [S][CW]: s log2 e
+    float* sv = ss + S * CW;                                                  // [S][CW]: s x
+    float* yb = sv + S * CW;                                                  // [S][YS]: sums over the states
 
     const int64_t b = blockIdx.y;
     const int d0 = blockIdx.x * CW;
-    const int64_t len = sel_length(a, b);
-    const int64_t slices = (len + S - 1) / S;
-    const int ln = lane % LN, ch = lane / LN, d = d0 + ch, n0 = ln * 4;  // in the sweep
-    const int row = lane / 2, dr = d0 + (lane & 1) * E;                  // in memory's layout
-    const T* x = static_cast<const T*>(a.x) + b * a.sx[0] + dr;
-    const T* dt = static_cast<const T*>(a.dt) + b * a.sdt[0] + dr;
-    const T* z = a.z ? static_cast<const T*>(a.z) + b * a.sz[0] + dr : nullptr;
-    T* y = static_cast<T*>(a.y) + b * a.L * a.D + dr;
+    const int len = sel_length(a, b), slices = (len + S - 1) / S;
+    const int ln = lane % LN, ch = lane / LN * 2, d = d0 + ch, n0 = ln * 4;  // in the sweep
+    const int row = lane / 4, cr = (lane & 3) * E, dr = d0 + cr;             // in memory's layout
+    T* y = static_cast<T*>(a.y) + (b * a.L + row) * a.D + dr;
     const BC bc{static_cast<const T*>(a.B) + b * a.sB[0], static_cast<const T*>(a.C) + b * a.sC[0],
                 reinterpret_cast<T*>(mine), reinterpret_cast<float*>(mine + BC::kRawBytes)};
-    const bool vec = a.vec != 0;
+    const bool vec = a.vec != 0, gated = a.z != nullptr;
 
-    const Quad A = quad(read_states(a.A, d, a.D, n0, a.N));
-    float bias[E], skip[E];
-#pragma unroll
-    for (int e = 0; e < E; ++e) {
-        bias[e] = a.bias && dr + e < a.D ? a.bias[dr + e] : 0.f;
-        skip[e] = a.skip && dr + e < a.D ? a.skip[dr + e] : 0.f;
+    for (int i = threadIdx.x; i < 2 * CW; i += blockDim.x) {
+        const float* p = i < CW ? a.bias : a.skip;
+        const int c = d0 + i % CW;
+        pars[i] = p && c < a.D ? p[c] : 0.f;
     }
-    Quad h = quad(make_float4(0.f, 0.f, 0.f, 0.f));
-    if (w == 0 && a.h0) h = quad(read_states(a.h0 + b * a.D * a.N, d, a.D, n0, a.N));
+    __syncthreads();
+    float A[2][4];
+#pragma unroll
+    for (int c = 0; c < 2; ++c) {
+        const float4 q = read_states(a.A, d + c, a.D, n0, a.N);
+        A[c][0] = q.x, A[c][1] = q.y, A[c][2] = q.z, A[c][3] = q.w;
+    }
+    Quad h[2];
+#pragma unroll
+    for (int c = 0; c < 2; ++c) h[c] = quad(w == 0 && a.h0 ? read_states(a.h0 + b * a.D * a.N, d + c, a.D, n0, a.N) : make_float4(0.f, 0.f, 0.f, 0.f));
 
     Run<T, E> rx, rt, rz;
-    auto ask = [&](int64_t j) {
-        const int64_t t = j * S + row;
-        const bool in = t < len;
-        read_run<T, E>(rx, x + t * a.sx[1], in, dr, a.D, vec);
-        read_run<T, E>(rt, dt + t * a.sdt[1], in, dr, a.D, vec);
-        if (z) read_run<T, E>(rz, z + t * a.sz[1], in, dr, a.D, vec);
+    const int64_t t_first = w * S + row;
+    const T* x = static_cast<const T*>(a.x) + b * a.sx[0] + t_first * a.sx[1] + dr;
+    const T* dt = static_cast<const T*>(a.dt) + b * a.sdt[0] + t_first * a.sdt[1] + dr;
+    const T* z = gated ? static_cast<const T*>(a.z) + b * a.sz[0] + t_first * a.sz[1] + dr : nullptr;
+    auto ask = [&](int j) {  // of the warp's next slice
+        const bool in = j * S + row < len;
+        rx.template read<FULL>(x, in, dr, a.D, vec);
+        rt.template read<FULL>(dt, in, dr, a.D, vec);
+        if (gated) rz.template read<FULL>(z, in, dr, a.D, vec);
         bc.ask(a, j * S, len, lane);
+        x += W * S * a.sx[1];
+        dt += W * S * a.sdt[1];
+        if (gated) z += W * S * a.sz[1];
     };
     if (w < slices) ask(w);
-    for (int64_t j = w; j < slices; j += W) {
-        const int64_t t0 = j * S;
+    for (int j = w; j < slices; j += W) {
+        const int t0 = j * S;
         bc.take(a, t0, len, lane);
-        float xs[E], gain[E];
         const bool in = t0 + row < len;
+        const Run<T, E> kx = rx, kz = rz;  // for the outputs
+        {
+            float xs[E], s[E], bias[E];
+            rx.floats(xs);
+            rt.floats(s);
+            get_run<E>(bias, pars + cr);
 #pragma unroll
-        for (int e = 0; e < E; ++e) {
-            float slope;
-            const float raw = to_f32(rt.e[e]) + bias[e];
-            const float s = in ? (a.softplus ? softplus(raw, slope) : raw) : 0.f;
-            xs[e] = to_f32(rx.e[e]);
-            const float zv = z ? to_f32(rz.e[e]) : 0.f;
-            gain[e] = z ? zv * sigmoid(zv) : 1.f;
-            const float sl = s * kLog2e, v = s * xs[e];
-            sd[Sh::place(row, (lane & 1) * E + e)] = make_float4(sl, sl, v, v);
+            for (int e = 0; e < E; ++e) {
+                float slope;
+                s[e] += bias[e];
+                if (a.softplus) s[e] = softplus(s[e], slope);
+                s[e] = in ? s[e] : 0.f;
+                xs[e] *= s[e];
+                s[e] *= kLog2e;
+            }
+            put_run<E>(ss + row * CW + cr, s);
+            put_run<E>(sv + row * CW + cr, xs);
         }
         __syncwarp();
         if (j + W < slices) ask(j + W);
 
-        Quad ah[S];  // the decays, then the states
+        Quad own[2], P[2], CP[S][2];
+        float v[2 * S];
 #pragma unroll
         for (int t = 0; t < S; ++t) {
-            const f32x2 s2 = reinterpret_cast<const Quad*>(sd)[Sh::place(t, ch)].lo;
-            ah[t].lo = ex2_pair(mul2(s2, A.lo));
-            ah[t].hi = ex2_pair(mul2(s2, A.hi));
+            const float2 s2 = *reinterpret_cast<const float2*>(ss + t * CW + ch), v2 = *reinterpret_cast<const float2*>(sv + t * CW + ch);
+            const Quad Cq = bc.c(t, ln);
+            float Bv[4];
+            bc.b(t, ln, Bv);
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+                const float sc = c ? s2.y : s2.x, vc = c ? v2.y : v2.x;
+                const f32x2 a0 = pair(ex2_approx(sc * A[c][0]), ex2_approx(sc * A[c][1]));
+                const f32x2 a1 = pair(ex2_approx(sc * A[c][2]), ex2_approx(sc * A[c][3]));
+                const f32x2 b0 = pair(vc * Bv[0], vc * Bv[1]), b1 = pair(vc * Bv[2], vc * Bv[3]);
+                own[c].lo = t ? fma2(a0, own[c].lo, b0) : b0;
+                own[c].hi = t ? fma2(a1, own[c].hi, b1) : b1;
+                P[c].lo = t ? mul2(P[c].lo, a0) : a0;
+                P[c].hi = t ? mul2(P[c].hi, a1) : a1;
+                v[2 * t + c] = both(fma2(Cq.hi, own[c].hi, mul2(Cq.lo, own[c].lo)));
+                CP[t][c].lo = mul2(Cq.lo, P[c].lo);
+                CP[t][c].hi = mul2(Cq.hi, P[c].hi);
+            }
         }
         if (j > 0 && W > 1) {
             asm volatile("bar.sync %0, 64;" ::"r"(w) : "memory");
-            h = hop[w * 32 + lane];
+            h[0] = hop[(w * 2) * 32 + lane];
+            h[1] = hop[(w * 2 + 1) * 32 + lane];
         }
 #pragma unroll
-        for (int t = 0; t < S; ++t) {
-            if constexpr (CKPT) {
-                if (t % 8 == 0 && t0 + t < len && d < a.D) {
-                    const int64_t k = (b * ((a.L + 7) / 8) + (t0 + t) / 8) * a.D + d;
-                    *reinterpret_cast<Quad*>(a.ckpt + k * NP + n0) = h;
-                }
-            }
-            const f32x2 v2 = reinterpret_cast<const Quad*>(sd)[Sh::place(t, ch)].hi;
-            const Quad Bq = bc.b(t, ln);
-            h.lo = fma2(ah[t].lo, h.lo, mul2(v2, Bq.lo));
-            h.hi = fma2(ah[t].hi, h.hi, mul2(v2, Bq.hi));
-            ah[t] = h;
+        for (int c = 0; c < 2; ++c) {
+            own[c].lo = fma2(P[c].lo, h[c].lo, own[c].lo);
+            own[c].hi = fma2(P[c].hi, h[c].hi, own[c].hi);
         }
         if (j + 1 < slices) {
             if (W > 1) {
                 const int next = w + 1 == W ? 0 : w + 1;
-                hop[next * 32 + lane] = h;
+                hop[(next * 2) * 32 + lane] = own[0];
+                hop[(next * 2 + 1) * 32 + lane] = own[1];
                 asm volatile("bar.arrive %0, 64;" ::"r"(next) : "memory");
             }
         } else if (a.hN) {
-            write_states(a.hN + b * a.D * a.N, d, a.D, n0, a.N, h);
+            for (int c = 0; c < 2; ++c) write_states(a.hN + b * a.D * a.N, d + c, a.D, n0, a.N, own[c]);
         }
-        float v[S];
+        if constexpr (CKPT) {
 #pragma unroll
-        for (int t = 0; t < S; ++t) {
-            const Quad Cq = bc.c(t, ln);
-            v[t] = both(fma2(Cq.hi, ah[t].hi, mul2(Cq.lo, ah[t].lo)));
+            for (int c = 0; c < 2; ++c)
+                if (FULL || d + c < a.D) *reinterpret_cast<Quad*>(a.ckpt + ((b * ((a.L + 7) / 8) + j) * a.D + d + c) * NP + n0) = h[c];
         }
-        Fold<S, LN / 2, 1>::run(v, lane);
-        const int first = FoldShape<S, LN / 2, 1>::held(lane);
 #pragma unroll
-        for (int i = 0; i < S / LN; ++i) yb[(first + i) * Sh::YS + ch] = v[i];
+        for (int t = 0; t < S; ++t)
+#pragma unroll
+            for (int c = 0; c < 2; ++c) v[2 * t + c] += both(fma2(CP[t][c].hi, h[c].hi, mul2(CP[t][c].lo, h[c].lo)));
+        if (W == 1) h[0] = own[0], h[1] = own[1];
+        Fold<2 * S, LN / 2, 1>::run(v, lane);
+        const int first = FoldShape<2 * S, LN / 2, 1>::held(lane);
+#pragma unroll
+        for (int i = 0; i < 2 * S / LN; ++i) yb[((first + i) / 2) * Sh::YS + ch + ((first + i) & 1)] = v[i];
         __syncwarp();
         if (t0 + row < a.L) {
-            float o[E];
+            float o[E], xs[E], g[E], skip[E];
+            kx.floats(xs);
+            get_run<E>(skip, pars + CW + cr);
+            get_run<E>(o, yb + row * Sh::YS + cr);
+            if (gated) kz.floats(g);
 #pragma unroll
             for (int e = 0; e < E; ++e) {
-                const float q = yb[row * Sh::YS + (lane & 1) * E + e];
-                o[e] = in ? fmaf(skip[e], xs[e], q) * gain[e] : 0.f;
+                o[e] = fmaf(skip[e], xs[e], o[e]);
+                if (gated) o[e] *= g[e] * sigmoid(g[e]);
+                o[e] = in ? o[e] : 0.f;
             }
-            write_run<T, E>(o, y + (t0 + row) * a.D, dr, a.D, vec);
+            write_run<T, E, FULL>(o, y + static_cast<int64_t>(t0) * a.D, dr, a.D, vec);
         }
     }
     // behind the row's end, and a row without a token
     const float nil[E] = {};
-    for (int64_t t = (slices + w) * S + row; t < a.L; t += static_cast<int64_t>(W) * S) write_run<T, E>(nil, y + t * a.D, dr, a.D, vec);
-    if (slices == 0 && w == 0 && a.hN) write_states(a.hN + b * a.D * a.N, d, a.D, n0, a.N, h);
+    for (int64_t t = static_cast<int64_t>(slices + w) * S; t + row < a.L; t += W * S) write_run<T, E, FULL>(nil, y + t * a.D, dr, a.D, vec);
+    if (slices == 0 && w == 0 && a.hN)
+        for (int c = 0; c < 2; ++c) write_states(a.hN + b * a.D * a.N, d + c, a.D, n0, a.N, h[c]);
 }
 
 // ---------------------------------------------------------------------------------------------------------
@@ -447,7 +589,7 @@ struct BwdShape {
 template <typename T, int LN>
 constexpr size_t sel_bwd_warp_bytes() {
     using Sh = BwdShape<LN>;
-    using BC = SliceBC<T, LN, Sh::S>;
+    using BC = SliceBC<T, LN, Sh::S, false>;
     return BC::kRawBytes + BC::kBytes + Sh::S * Sh::CW * 24 + (3 * Sh::S * Sh::YS * 4 + 15) / 16 * 16;
 }
 // hop, dA and A of a group; per-lane sums of dskip and ddt_bias; a barrier a group
@@ -460,7 +602,7 @@ constexpr int kSelBwdWarps = 8, kSelBwdMaxGroups = 8;
 template <typename T, int LN>
 __global__ void __launch_bounds__(kSelBwdWarps * 32, 1) sel_bwd_k(const SelArgs a) {
     using Sh = BwdShape<LN>;
-    using BC = SliceBC<T, LN, Sh::S>;
+    using BC = SliceBC<T, LN, Sh::S, false>;
     constexpr int S = Sh::S, NP = Sh::NP, CW = Sh::CW, E = Sh::E, YS = Sh::YS, W = kSelBwdWarps;
     extern __shared__ __align__(16) unsigned char smem[];
     const int lane = threadIdx.x & 31, w = threadIdx.x >> 5, G = a.groups;
@@ -475,7 +617,7 @@ __global__ void __launch_bounds__(kSelBwdWarps * 32, 1) sel_bwd_k(const SelArgs 
     float* ob = reinterpret_cast<float*>(gd + S * CW);                      // [3][S][YS]: o, dv, sum_n A w
 
     const int64_t b = blockIdx.y;
-    const int64_t len = sel_length(a, b), slices = (len + S - 1) / S, n8 = (a.L + 7) / 8;
+    const int len = sel_length(a, b), slices = (len + S - 1) / S, n8 = (a.L + 7) / 8;
     const int base = blockIdx.x * G * CW;  // the CTA's first channel
     const int ln = lane % LN, ch = lane / LN, n0 = ln * 4;
     const int row = lane / 4, sub = (lane & 3) * E;  // in memory's layout; lanes past CW channels idle (LN = 16)
@@ -501,14 +643,14 @@ __global__ void __launch_bounds__(kSelBwdWarps * 32, 1) sel_bwd_k(const SelArgs 
 
     Run<T, E> rx, rt, rz, rg;
     Quad hn;  // the checkpoint
-    auto ask = [&](int64_t j, int g) {
-        const int64_t t = j * S + row;
+    auto ask = [&](int j, int g) {
+        const int t = j * S + row;
         const int d = base + g * CW + sub, dc = base + g * CW + ch;
         const bool in = t < len && reads;
-        read_run<T, E>(rx, x + t * a.sx[1] + d, in, d, a.D, vec);
-        read_run<T, E>(rt, dt + t * a.sdt[1] + d, in, d, a.D, vec);
-        if (z) read_run<T, E>(rz, z + t * a.sz[1] + d, in, d, a.D, vec);
-        read_run<T, E>(rg, dy + t * a.sdy[1] + d, in, d, a.D, vec);
+        rx.read(x + t * a.sx[1] + d, in, d, a.D, vec);
+        rt.read(dt + t * a.sdt[1] + d, in, d, a.D, vec);
+        if (z) rz.read(z + t * a.sz[1] + d, in, d, a.D, vec);
+        rg.read(dy + t * a.sdy[1] + d, in, d, a.D, vec);
         hn = dc < a.D ? *reinterpret_cast<const Quad*>(a.ckpt + ((b * n8 + j) * a.D + dc) * NP + n0)
                       : quad(make_float4(0.f, 0.f, 0.f, 0.f));
     };
@@ -518,8 +660,8 @@ __global__ void __launch_bounds__(kSelBwdWarps * 32, 1) sel_bwd_k(const SelArgs 
         bc.ask(a, (slices - 1 - w) * S, len, lane);
         ask(slices - 1 - w, 0);
     }
-    for (int64_t k = w; k < slices; k += W, ++turn) {  // k: from the row's end
-        const int64_t j = slices - 1 - k, t0 = j * S;
+    for (int k = w; k < slices; k += W, ++turn) {  // k: from the row's end
+        const int j = slices - 1 - k, t0 = j * S;
         bc.take(a, t0, len, lane);
         __syncwarp();
         if (k + W < slices) bc.ask(a, (j - W) * S, len, lane);
@@ -531,17 +673,18 @@ __global__ void __launch_bounds__(kSelBwdWarps * 32, 1) sel_bwd_k(const SelArgs 
             const int d = base + g * CW + sub, dc = base + g * CW + ch;
             const bool in = t0 + row < len && reads;
             float xs[E], ss[E], slope[E], dof[E], dzf[E];
+            rx.floats(xs);
+            rt.floats(ss);
+            rg.floats(dof);
+            if (z) rz.floats(dzf);
 #pragma unroll
             for (int e = 0; e < E; ++e) {
                 const bool on = in && d + e < a.D;
-                const float raw = to_f32(rt.e[e]) + (a.bias && on ? a.bias[d + e] : 0.f);
+                const float raw = ss[e] + (a.bias && on ? a.bias[d + e] : 0.f);
                 slope[e] = 1.f;
                 ss[e] = on ? (a.softplus ? softplus(raw, slope[e]) : raw) : 0.f;
-                xs[e] = to_f32(rx.e[e]);
-                const float g0 = to_f32(rg.e[e]);
-                dof[e] = g0;
                 if (z) {
-                    const float zv = to_f32(rz.e[e]), sg = sigmoid(zv);
+                    const float zv = dzf[e], sg = sigmoid(zv), g0 = dof[e];
                     dof[e] = g0 * (zv * sg);
                     dzf[e] = g0 * sg * fmaf(zv, 1.f - sg, 1.f);
                 }
@@ -639,7 +782,7 @@ __global__ void __launch_bounds__(kSelBwdWarps * 32, 1) sel_bwd_k(const SelArgs 
                     acc[(2 * e + 1) * 32] += ot[e];
                     if (z) oz[e] = in ? dzf[e] * fmaf(sk, xs[e], ob[row * YS + sub + e]) : 0.f;
                 }
-                const int64_t o = rowD + (t0 + row) * a.D + d;
+                const int64_t o = rowD + static_cast<int64_t>(t0 + row) * a.D + d;
                 write_run<T, E>(ox, static_cast<T*>(a.dx) + o, d, a.D, vec);
                 write_run<T, E>(ot, static_cast<T*>(a.ddt) + o, d, a.D, vec);
                 if (z) write_run<T, E>(oz, static_cast<T*>(a.dz) + o, d, a.D, vec);
@@ -670,7 +813,7 @@ __global__ void __launch_bounds__(kSelBwdWarps * 32, 1) sel_bwd_k(const SelArgs 
     // gradients of what lies behind the row's end
     if (reads) {
         const float nil[E] = {};
-        for (int64_t t = (slices + w) * S + row; t < a.L; t += W * S)
+        for (int64_t t = static_cast<int64_t>(slices + w) * S + row; t < a.L; t += W * S)
             for (int g = 0; g < G; ++g) {
                 const int d = base + g * CW + sub;
                 const int64_t o = rowD + t * a.D + d;
@@ -761,8 +904,8 @@ int sel_check(const char* fn, const EacsSelective& p, bool single) {
     if (p.dtype != EACS_DTYPE_F32 && p.dtype != EACS_DTYPE_F16 && p.dtype != EACS_DTYPE_BF16)
         return fail(EACS_ERR_INVALID, "%s: unknown dtype %d", fn, p.dtype);
     if (p.N > 64) return fail(EACS_ERR_UNSUPPORTED, "%s: N=%lld > 64", fn, (long long)p.N);
-    if (p.rows > 65535 || p.D > (int64_t{1} << 24) || p.L > (int64_t{1} << 31))
-        return fail(EACS_ERR_UNSUPPORTED, "%s: more than 65535 rows, 2^24 channels or 2^31 tokens", fn);
+    if (p.rows > 65535 || p.D > (int64_t{1} << 24) || p.L > (int64_t{1} << 30))
+        return fail(EACS_ERR_UNSUPPORTED, "%s: more than 65535 rows, 2^24 channels or 2^30 tokens", fn);
     if (p.rows > 0 && (p.L > 0 || single) && (!p.x || !p.dt || !p.A || !p.B || !p.C))
         return fail(EACS_ERR_INVALID, "%s: null pointer argument", fn);
     return EACS_OK;
@@ -774,7 +917,7 @@ SelArgs sel_args(const EacsSelective& p) {
     for (int i = 0; i < 2; ++i)
         a.sx[i] = p.x_stride[i], a.sdt[i] = p.dt_stride[i], a.sz[i] = p.z_stride[i], a.sB[i] = p.B_stride[i], a.sC[i] = p.C_stride[i];
     a.A = p.A, a.skip = p.skip, a.bias = p.dt_bias, a.lengths = p.lengths, a.h0 = p.initial_state;
-    a.L = p.L, a.D = static_cast<int>(p.D), a.N = static_cast<int>(p.N), a.Bn = p.rows, a.softplus = p.softplus;
+    a.L = static_cast<int>(p.L), a.D = static_cast<int>(p.D), a.N = static_cast<int>(p.N), a.Bn = p.rows, a.softplus = p.softplus;
     const int64_t esz = p.dtype == EACS_DTYPE_F32 ? 4 : 2;
     const int64_t dense[2] = {p.D, p.D};  // of what is written
     a.vec = sel_aligned(p.x, p.x_stride, esz) && sel_aligned(p.dt, p.dt_stride, esz) && sel_aligned(p.z, p.z_stride, esz) &&
@@ -783,15 +926,18 @@ SelArgs sel_args(const EacsSelective& p) {
     return a;
 }
 
-template <typename T, int LN, bool CKPT>
+// Twelve warps a multiprocessor: of one CTA where there are few, else of two or three.
+template <typename T, int LN, bool CKPT, bool FULL>
 cudaError_t sel_fwd_launch(const SelArgs& a, cudaStream_t s) {
-    constexpr int W = 4;
-    const size_t smem = W * sel_fwd_warp_bytes<T, LN>();
-    const auto k = sel_fwd_k<T, LN, CKPT>;
+    constexpr int CW = FwdShape<LN>::CW;
+    const dim3 grid((a.D + CW - 1) / CW, static_cast<unsigned>(a.Bn));
+    const int64_t ctas = static_cast<int64_t>(grid.x) * grid.y;
+    const int W = ctas <= 148 ? 12 : ctas <= 296 ? 6 : 4;
+    const size_t smem = sel_fwd_cta_bytes<LN>(W) + W * sel_fwd_warp_bytes<T, LN>();
+    const auto k = sel_fwd_k<T, LN, CKPT, FULL>;
     const cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
     if (e != cudaSuccess) return e;
-    constexpr int CW = FwdShape<LN>::CW;
-    k<<<dim3((a.D + CW - 1) / CW, static_cast<unsigned>(a.Bn)), W * 32, smem, s>>>(a);
+    k<<<grid, W * 32, smem, s>>>(a);
     note_launch();
     return cudaGetLastError();
 }
@@ -855,7 +1001,9 @@ cudaError_t sel_bwd_launch(const SelArgs& a, int parts, T* dB, T* dC, float* dA,
 
 template <typename T, int LN>
 cudaError_t sel_fwd_any(const SelArgs& a, cudaStream_t s) {
-    return a.ckpt ? sel_fwd_launch<T, LN, true>(a, s) : sel_fwd_launch<T, LN, false>(a, s);
+    const bool full = a.vec && a.vec_bc && a.D % FwdShape<LN>::CW == 0 && a.N == 4 * LN;
+    if (a.ckpt) return full ? sel_fwd_launch<T, LN, true, true>(a, s) : sel_fwd_launch<T, LN, true, false>(a, s);
+    return full ? sel_fwd_launch<T, LN, false, true>(a, s) : sel_fwd_launch<T, LN, false, false>(a, s);
 }
 
 size_t sel_up(size_t n) { return (n + 255) / 256 * 256; }
