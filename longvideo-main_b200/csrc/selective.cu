@@ -592,28 +592,30 @@ constexpr size_t sel_bwd_warp_bytes() {
     using BC = SliceBC<T, LN, Sh::S, false>;
     return BC::kRawBytes + BC::kBytes + Sh::S * Sh::CW * 24 + (3 * Sh::S * Sh::YS * 4 + 15) / 16 * 16;
 }
-// hop, dA and A of a group; per-lane sums of dskip and ddt_bias; a barrier a group
+// of a group of channels: g handed on, sums of dA, dskip and ddt_bias and a barrier a warp; A, dt_bias and skip
 template <int LN>
 constexpr size_t sel_bwd_group_bytes(int W) {
-    return static_cast<size_t>(W) * (512 + 512 + 2 * BwdShape<LN>::E * 128 + 8) + 512;
+    return static_cast<size_t>(W) * (512 + 512 + 2 * BwdShape<LN>::E * 128 + 8) + 512 + 2 * BwdShape<LN>::CW * 4;
 }
 constexpr int kSelBwdWarps = 8, kSelBwdMaxGroups = 8;
 
-template <typename T, int LN>
+// FULL: groups of CW channels and rows of NP states, all of them on 16 bytes
+template <typename T, int LN, bool FULL>
 __global__ void __launch_bounds__(kSelBwdWarps * 32, 1) sel_bwd_k(const SelArgs a) {
     using Sh = BwdShape<LN>;
-    using BC = SliceBC<T, LN, Sh::S, false>;
+    using BC = SliceBC<T, LN, Sh::S, FULL>;
     constexpr int S = Sh::S, NP = Sh::NP, CW = Sh::CW, E = Sh::E, YS = Sh::YS, W = kSelBwdWarps;
     extern __shared__ __align__(16) unsigned char smem[];
     const int lane = threadIdx.x & 31, w = threadIdx.x >> 5, G = a.groups;
     Quad* hop = reinterpret_cast<Quad*>(smem);             // [W][G][32]: the g that each warp is handed
     Quad* dAs = hop + W * G * 32;                          // [W][G][32]
     Quad* As = dAs + W * G * 32;                           // [G][32]
-    float* sums = reinterpret_cast<float*>(As + G * 32);   // [W][G][2 E][32]
-    uint64_t* bars = reinterpret_cast<uint64_t*>(sums + W * G * 2 * E * 32);  // [W][G]
+    float* sums = reinterpret_cast<float*>(As + G * 32);   // [W][G][32][2 E]: dskip and ddt_bias of a lane's tokens
+    float* pars = sums + W * G * 2 * E * 32;               // [2][G CW]: dt_bias, skip
+    uint64_t* bars = reinterpret_cast<uint64_t*>(pars + 2 * G * CW);  // [W][G]
     unsigned char* mine = smem + (sel_bwd_group_bytes<LN>(W) * G + 15) / 16 * 16 + static_cast<size_t>(w) * sel_bwd_warp_bytes<T, LN>();
-    Quad* sd = reinterpret_cast<Quad*>(mine + BC::kRawBytes + BC::kBytes);  // (s log2 e) twice, (s x) twice
-    f32x2* gd = reinterpret_cast<f32x2*>(sd + S * CW);                      // do twice
+    Quad* sd = reinterpret_cast<Quad*>(mine + BC::kRawBytes + BC::kBytes);  // [S][CW]: (s log2 e) twice, (s x) twice
+    f32x2* gd = reinterpret_cast<f32x2*>(sd + S * CW);                      // [S][CW]: do twice
     float* ob = reinterpret_cast<float*>(gd + S * CW);                      // [3][S][YS]: o, dv, sum_n A w
 
     const int64_t b = blockIdx.y;
@@ -621,21 +623,21 @@ __global__ void __launch_bounds__(kSelBwdWarps * 32, 1) sel_bwd_k(const SelArgs 
     const int base = blockIdx.x * G * CW;  // the CTA's first channel
     const int ln = lane % LN, ch = lane / LN, n0 = ln * 4;
     const int row = lane / 4, sub = (lane & 3) * E;  // in memory's layout; lanes past CW channels idle (LN = 16)
-    const bool reads = sub < CW;
-    const int64_t rowD = b * a.L * a.D;
-    const T* x = static_cast<const T*>(a.x) + b * a.sx[0];
-    const T* dt = static_cast<const T*>(a.dt) + b * a.sdt[0];
-    const T* z = a.z ? static_cast<const T*>(a.z) + b * a.sz[0] : nullptr;
-    const T* dy = static_cast<const T*>(a.dy) + b * a.sdy[0];
+    const bool reads = sub < CW, gated = a.z != nullptr;
     const BC bc{static_cast<const T*>(a.B) + b * a.sB[0], static_cast<const T*>(a.C) + b * a.sC[0],
                 reinterpret_cast<T*>(mine), reinterpret_cast<float*>(mine + BC::kRawBytes)};
     const bool vec = a.vec != 0;
 
     for (int g = w; g < G; g += W) As[g * 32 + lane] = quad(read_states(a.A, base + g * CW + ch, a.D, n0, a.N));
+    for (int i = threadIdx.x; i < 2 * G * CW; i += W * 32) {
+        const float* p = i < G * CW ? a.bias : a.skip;
+        const int c = base + i % (G * CW);
+        pars[i] = p && c < a.D ? p[c] : 0.f;
+    }
     for (int g = 0; g < G; ++g) {
         dAs[(w * G + g) * 32 + lane] = quad(make_float4(0.f, 0.f, 0.f, 0.f));
 #pragma unroll
-        for (int e = 0; e < 2 * E; ++e) sums[((w * G + g) * 2 * E + e) * 32 + lane] = 0.f;
+        for (int e = 0; e < 2 * E; ++e) sums[((w * G + g) * 32 + lane) * 2 * E + e] = 0.f;
         if (lane == 0) mbar_init(&bars[w * G + g], 1);
     }
     fence_mbar_init();
@@ -643,47 +645,65 @@ __global__ void __launch_bounds__(kSelBwdWarps * 32, 1) sel_bwd_k(const SelArgs 
 
     Run<T, E> rx, rt, rz, rg;
     Quad hn;  // the checkpoint
-    auto ask = [&](int j, int g) {
-        const int t = j * S + row;
-        const int d = base + g * CW + sub, dc = base + g * CW + ch;
-        const bool in = t < len && reads;
-        rx.read(x + t * a.sx[1] + d, in, d, a.D, vec);
-        rt.read(dt + t * a.sdt[1] + d, in, d, a.D, vec);
-        if (z) rz.read(z + t * a.sz[1] + d, in, d, a.D, vec);
-        rg.read(dy + t * a.sdy[1] + d, in, d, a.D, vec);
-        hn = dc < a.D ? *reinterpret_cast<const Quad*>(a.ckpt + ((b * n8 + j) * a.D + dc) * NP + n0)
-                      : quad(make_float4(0.f, 0.f, 0.f, 0.f));
+    const T *px, *pt, *pz = nullptr, *pg;  // the lane's token and channels of the slice and group asked for next
+    const float* pc;
+    int nj = slices - 1 - w, ng = 0;       // that slice and group
+    auto place = [&] {
+        const int64_t t = static_cast<int64_t>(nj) * S + row;
+        const int d = base + sub;
+        px = static_cast<const T*>(a.x) + b * a.sx[0] + t * a.sx[1] + d;
+        pt = static_cast<const T*>(a.dt) + b * a.sdt[0] + t * a.sdt[1] + d;
+        if (gated) pz = static_cast<const T*>(a.z) + b * a.sz[0] + t * a.sz[1] + d;
+        pg = static_cast<const T*>(a.dy) + b * a.sdy[0] + t * a.sdy[1] + d;
+        pc = a.ckpt + ((b * n8 + nj) * a.D + base + ch) * NP + n0;
+    };
+    auto ask = [&] {
+        const int o = ng * CW, d = base + o + sub;
+        const bool in = nj * S + row < len && reads;
+        rx.template read<FULL>(px + o, in, d, a.D, vec);
+        rt.template read<FULL>(pt + o, in, d, a.D, vec);
+        if (gated) rz.template read<FULL>(pz + o, in, d, a.D, vec);
+        rg.template read<FULL>(pg + o, in, d, a.D, vec);
+        hn = FULL || base + o + ch < a.D ? *reinterpret_cast<const Quad*>(pc + static_cast<int64_t>(o) * NP) : quad(make_float4(0.f, 0.f, 0.f, 0.f));
+        if (++ng == G) {
+            ng = 0;
+            nj -= W;
+            if (nj >= 0) place();
+        }
     };
     bool ok = true;
     uint32_t turn = 0;
-    if (w < slices) {
-        bc.ask(a, (slices - 1 - w) * S, len, lane);
-        ask(slices - 1 - w, 0);
+    if (nj >= 0) {
+        bc.ask(a, nj * S, len, lane);
+        place();
+        ask();
     }
     for (int k = w; k < slices; k += W, ++turn) {  // k: from the row's end
         const int j = slices - 1 - k, t0 = j * S;
         bc.take(a, t0, len, lane);
         __syncwarp();
-        if (k + W < slices) bc.ask(a, (j - W) * S, len, lane);
+        if (j >= W) bc.ask(a, (j - W) * S, len, lane);
         Quad accB[S], accC[S];
 #pragma unroll
         for (int t = 0; t < S; ++t) accB[t] = accC[t] = quad(make_float4(0.f, 0.f, 0.f, 0.f));
+        const bool in = t0 + row < len && reads;
+        const int64_t out = (b * a.L + t0 + row) * a.D + base + sub;
 
         for (int g = 0; g < G; ++g) {
-            const int d = base + g * CW + sub, dc = base + g * CW + ch;
-            const bool in = t0 + row < len && reads;
+            const int d = base + g * CW + sub, dc = base + g * CW + ch, wg = w * G + g;
             float xs[E], ss[E], slope[E], dof[E], dzf[E];
             rx.floats(xs);
             rt.floats(ss);
             rg.floats(dof);
-            if (z) rz.floats(dzf);
+            if (gated) rz.floats(dzf);
 #pragma unroll
             for (int e = 0; e < E; ++e) {
-                const bool on = in && d + e < a.D;
-                const float raw = ss[e] + (a.bias && on ? a.bias[d + e] : 0.f);
+                const float raw = ss[e] + pars[g * CW + (reads ? sub : 0) + e];
                 slope[e] = 1.f;
-                ss[e] = on ? (a.softplus ? softplus(raw, slope[e]) : raw) : 0.f;
-                if (z) {
+                ss[e] = raw;
+                if (a.softplus) ss[e] = softplus(raw, slope[e]);
+                ss[e] = in && (FULL || d + e < a.D) ? ss[e] : 0.f;
+                if (gated) {
                     const float zv = dzf[e], sg = sigmoid(zv), g0 = dof[e];
                     dof[e] = g0 * (zv * sg);
                     dzf[e] = g0 * sg * fmaf(zv, 1.f - sg, 1.f);
@@ -696,8 +716,7 @@ __global__ void __launch_bounds__(kSelBwdWarps * 32, 1) sel_bwd_k(const SelArgs 
             }
             Quad h = hn;
             __syncwarp();
-            if (g + 1 < G) ask(j, g + 1);
-            else if (k + W < slices) ask(j - W, 0);
+            if (g + 1 < G || j >= W) ask();
 
             const Quad A = As[g * 32 + lane];
             Quad dec[S], old[S];  // e^(s A), and e^(s A) h
@@ -719,7 +738,7 @@ __global__ void __launch_bounds__(kSelBwdWarps * 32, 1) sel_bwd_k(const SelArgs 
             }
             const int first = FoldShape<S, LN / 2, 1>::held(lane);
             constexpr int kept = FoldShape<S, LN / 2, 1>::kRem;
-            if (z) {
+            if (gated) {
                 Fold<S, LN / 2, 1>::run(v, lane);
 #pragma unroll
                 for (int i = 0; i < kept; ++i) ob[(first + i) * YS + ch] = v[i];
@@ -727,12 +746,12 @@ __global__ void __launch_bounds__(kSelBwdWarps * 32, 1) sel_bwd_k(const SelArgs 
             Quad gs = quad(make_float4(0.f, 0.f, 0.f, 0.f));
             if (k > 0) {
                 const uint32_t phase = (w == 0 ? turn - 1 : turn) & 1;
-                if (ok) ok = mbar_wait(&bars[w * G + g], phase);
-                gs = hop[(w * G + g) * 32 + lane];
+                if (ok) ok = mbar_wait(&bars[wg], phase);
+                gs = hop[wg * 32 + lane];
             } else if (a.dhN) {
                 gs = quad(read_states(a.dhN + b * a.D * a.N, dc, a.D, n0, a.N));
             }
-            Quad dA = dAs[(w * G + g) * 32 + lane];
+            Quad dA = dAs[wg * 32 + lane];
             float dv[S], aw[S];
 #pragma unroll
             for (int t = S - 1; t >= 0; --t) {
@@ -752,15 +771,15 @@ __global__ void __launch_bounds__(kSelBwdWarps * 32, 1) sel_bwd_k(const SelArgs 
                 gs.hi = mul2(gs.hi, dec[t].hi);
             }
             if (j > 0) {
-                const int next = w + 1 == W ? 0 : w + 1;
-                hop[(next * G + g) * 32 + lane] = gs;
+                const int next = (w + 1 == W ? 0 : w + 1) * G + g;
+                hop[next * 32 + lane] = gs;
                 __syncwarp();
                 if (lane == 0)
-                    asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(&bars[next * G + g])) : "memory");
+                    asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(&bars[next])) : "memory");
             } else if (a.dh0) {
                 write_states(a.dh0 + b * a.D * a.N, dc, a.D, n0, a.N, gs);
             }
-            dAs[(w * G + g) * 32 + lane] = dA;
+            dAs[wg * 32 + lane] = dA;
             Fold<S, LN / 2, 1>::run(dv, lane);
             Fold<S, LN / 2, 1>::run(aw, lane);
 #pragma unroll
@@ -770,26 +789,26 @@ __global__ void __launch_bounds__(kSelBwdWarps * 32, 1) sel_bwd_k(const SelArgs 
             }
             __syncwarp();
             if (t0 + row < a.L && reads) {
-                float ox[E], ot[E], oz[E];
-                float* acc = sums + (w * G + g) * 2 * E * 32 + lane;
+                float ox[E], ot[E], oz[E], acc[2 * E];
+                get_run<2 * E>(acc, sums + (wg * 32 + lane) * 2 * E);
 #pragma unroll
                 for (int e = 0; e < E; ++e) {
-                    const float sk = a.skip && d + e < a.D ? a.skip[d + e] : 0.f;
+                    const float sk = pars[(G + g) * CW + sub + e];
                     const float dvv = ob[(S + row) * YS + sub + e];
                     ox[e] = in ? fmaf(dvv, ss[e], dof[e] * sk) : 0.f;
                     ot[e] = in ? fmaf(dvv, xs[e], ob[(2 * S + row) * YS + sub + e]) * slope[e] : 0.f;
-                    acc[2 * e * 32] = fmaf(dof[e], xs[e], acc[2 * e * 32]);
-                    acc[(2 * e + 1) * 32] += ot[e];
-                    if (z) oz[e] = in ? dzf[e] * fmaf(sk, xs[e], ob[row * YS + sub + e]) : 0.f;
+                    acc[2 * e] = fmaf(dof[e], xs[e], acc[2 * e]);
+                    acc[2 * e + 1] += ot[e];
+                    if (gated) oz[e] = in ? dzf[e] * fmaf(sk, xs[e], ob[row * YS + sub + e]) : 0.f;
                 }
-                const int64_t o = rowD + static_cast<int64_t>(t0 + row) * a.D + d;
-                write_run<T, E>(ox, static_cast<T*>(a.dx) + o, d, a.D, vec);
-                write_run<T, E>(ot, static_cast<T*>(a.ddt) + o, d, a.D, vec);
-                if (z) write_run<T, E>(oz, static_cast<T*>(a.dz) + o, d, a.D, vec);
+                put_run<2 * E>(sums + (wg * 32 + lane) * 2 * E, acc);
+                write_run<T, E, FULL>(ox, static_cast<T*>(a.dx) + out + g * CW, d, a.D, vec);
+                write_run<T, E, FULL>(ot, static_cast<T*>(a.ddt) + out + g * CW, d, a.D, vec);
+                if (gated) write_run<T, E, FULL>(oz, static_cast<T*>(a.dz) + out + g * CW, d, a.D, vec);
             }
             __syncwarp();  // ob and sd are written again
         }
-        // the slice's sums over the CTA's channels: a lane ends with NP / CW ... of its tokens' four states
+        // the slice's sums over the CTA's channels, folded over the lanes of a warp that hold the same states
 #pragma unroll
         for (int which = 0; which < 2; ++which) {
             float v[S * 4];
@@ -801,7 +820,7 @@ __global__ void __launch_bounds__(kSelBwdWarps * 32, 1) sel_bwd_k(const SelArgs 
             }
             Fold<S * 4, 16, LN>::run(v, lane);
             const int first = FoldShape<S * 4, 16, LN>::held(lane);
-            constexpr int kept = FoldShape<S * 4, 16, LN>::kRem;  // 2 LN / ...: at least 2
+            constexpr int kept = FoldShape<S * 4, 16, LN>::kRem;  // at least 2
             float* part = (which ? a.partC : a.partB) + ((static_cast<int64_t>(blockIdx.x) * a.Bn + b) * a.L + t0) * NP + n0;
 #pragma unroll
             for (int i = 0; i < kept; i += 2) {
@@ -816,10 +835,10 @@ __global__ void __launch_bounds__(kSelBwdWarps * 32, 1) sel_bwd_k(const SelArgs 
         for (int64_t t = static_cast<int64_t>(slices + w) * S + row; t < a.L; t += W * S)
             for (int g = 0; g < G; ++g) {
                 const int d = base + g * CW + sub;
-                const int64_t o = rowD + t * a.D + d;
-                write_run<T, E>(nil, static_cast<T*>(a.dx) + o, d, a.D, vec);
-                write_run<T, E>(nil, static_cast<T*>(a.ddt) + o, d, a.D, vec);
-                if (z) write_run<T, E>(nil, static_cast<T*>(a.dz) + o, d, a.D, vec);
+                const int64_t o = (b * a.L + t) * a.D + d;
+                write_run<T, E, FULL>(nil, static_cast<T*>(a.dx) + o, d, a.D, vec);
+                write_run<T, E, FULL>(nil, static_cast<T*>(a.ddt) + o, d, a.D, vec);
+                if (gated) write_run<T, E, FULL>(nil, static_cast<T*>(a.dz) + o, d, a.D, vec);
             }
     }
     __syncthreads();
@@ -844,7 +863,7 @@ __global__ void __launch_bounds__(kSelBwdWarps * 32, 1) sel_bwd_k(const SelArgs 
         if (d >= a.D) continue;
         float s = 0.f;
         for (int v = 0; v < W; ++v)
-            for (int r = 0; r < S; ++r) s += sums[((v * G + g) * 2 * E + 2 * (c % E) + which) * 32 + r * 4 + c / E];
+            for (int r = 0; r < S; ++r) s += sums[((v * G + g) * 32 + r * 4 + c / E) * 2 * E + 2 * (c % E) + which];
         a.partS[(b * 2 + which) * a.D + d] = s;
     }
 }
@@ -977,7 +996,9 @@ template <typename T, int LN>
 cudaError_t sel_bwd_launch(const SelArgs& a, int parts, T* dB, T* dC, float* dA, float* dskip, float* dbias, cudaStream_t s) {
     constexpr int W = kSelBwdWarps;
     const size_t smem = (sel_bwd_group_bytes<LN>(W) * a.groups + 15) / 16 * 16 + W * sel_bwd_warp_bytes<T, LN>();
-    const auto k = sel_bwd_k<T, LN>;
+    // (a group of channels may start past D only where they are not FULL)
+    const bool full = a.vec && a.vec_bc && a.N == 4 * LN && a.D % (a.groups * BwdShape<LN>::CW) == 0;
+    const auto k = full ? sel_bwd_k<T, LN, true> : sel_bwd_k<T, LN, false>;
     cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
     if (e != cudaSuccess) return e;
     k<<<dim3(parts, static_cast<unsigned>(a.Bn)), W * 32, smem, s>>>(a);
