@@ -99,7 +99,9 @@ struct ConvCols {
     }
 };
 
-// U tokens are read before the first is used, so that many bytes are under way.
+// U tokens are read before the first is used, so that many bytes are under way.  Vectors of 4 values: with 16 bytes of a
+// 16-bit type a thread's taps and window leave registers for a third of the threads (79 us instead of what stands at
+// conv_fwd_launch).
 template <typename T, int VEC, int W, int U>
 __global__ void __launch_bounds__(128) conv_fwd_k(const ConvArgs a) {
     const int nv = a.D / VEC;
@@ -118,29 +120,33 @@ __global__ void __launch_bounds__(128) conv_fwd_k(const ConvArgs a) {
     if (t0 < tl)
 #pragma unroll
         for (int k = 1; k < W; ++k) Cols::input(win[k], a, x, b, t0 - W + k, c);
+    const T* px = x + t0 * a.sx[1];
+    T* py = y + t0 * a.D;
+    auto token = [&](const RowVec<T, VEC>& v) {
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) {
+#pragma unroll
+            for (int k = 0; k + 1 < W; ++k) win[k][e] = win[k + 1][e];
+            win[W - 1][e] = to_f32(v.e[e]);
+        }
+        float p[VEC];
+        cols.dot(p, win);
+        if (a.silu)
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) p[e] *= conv_sigmoid(p[e]);
+        conv_write<T, VEC>(py, p);
+        py += a.D;
+    };
     int64_t t = t0;
-    for (; t < tl; t += U) {
+    for (; t + U <= tl; t += U) {
         RowVec<T, VEC> raw[U];
 #pragma unroll
-        for (int u = 0; u < U; ++u)
-            if (t + u < tl) raw[u] = *reinterpret_cast<const RowVec<T, VEC>*>(x + (t + u) * a.sx[1]);
+        for (int u = 0; u < U; ++u) raw[u] = *reinterpret_cast<const RowVec<T, VEC>*>(px + u * a.sx[1]);
+        px += U * a.sx[1];
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
-            if (t + u >= tl) break;
-#pragma unroll
-            for (int e = 0; e < VEC; ++e) {
-#pragma unroll
-                for (int k = 0; k + 1 < W; ++k) win[k][e] = win[k + 1][e];
-                win[W - 1][e] = to_f32(raw[u].e[e]);
-            }
-            float p[VEC];
-            cols.dot(p, win);
-            if (a.silu)
-#pragma unroll
-                for (int e = 0; e < VEC; ++e) p[e] *= conv_sigmoid(p[e]);
-            conv_write<T, VEC>(y + (t + u) * a.D, p);
-        }
+        for (int u = 0; u < U; ++u) token(raw[u]);
     }
+    for (; t < tl; ++t, px += a.sx[1]) token(*reinterpret_cast<const RowVec<T, VEC>*>(px));
     const float nil[VEC] = {};
     for (t = max(t0, tl); t < t1; ++t) conv_write<T, VEC>(y + t * a.D, nil);
     if (a.hN && t0 == 0) {
@@ -153,7 +159,8 @@ __global__ void __launch_bounds__(128) conv_fwd_k(const ConvArgs a) {
     }
 }
 
-// CTAs of 32 columns (VEC channels each) times R runs.
+// CTAs of 32 columns (VEC channels each) times R runs.  A token gives dp; the gradient of the input W - 1 tokens before it
+// is then whole.
 template <typename T, int VEC, int W, int R, int U>
 __global__ void __launch_bounds__(32 * R) conv_bwd_k(const ConvArgs a) {
     __shared__ float comb[R][32];
@@ -170,75 +177,101 @@ __global__ void __launch_bounds__(32 * R) conv_bwd_k(const ConvArgs a) {
         T* dx = static_cast<T*>(a.dx) + b * a.L * a.D + c;
         const T* dhN = static_cast<const T*>(a.dhN);
         using Cols = ConvCols<T, VEC, W>;
+        using V = RowVec<T, VEC>;
         Cols cols;
         cols.taps(a, c);
         float win[W][VEC], dp[W][VEC] = {};  // dp of the token and of the W - 1 before it
         if (t0 < tl)
 #pragma unroll
             for (int k = 1; k < W; ++k) Cols::input(win[k], a, x, b, t0 - W + k, c);
+        auto shift = [&] {
+#pragma unroll
+            for (int k = 0; k + 1 < W; ++k)
+#pragma unroll
+                for (int e = 0; e < VEC; ++e) dp[k][e] = dp[k + 1][e], win[k][e] = win[k + 1][e];
+        };
+        auto token = [&](const V& vx, const V& vg, bool mine) {  // mine: one of the run's own
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) win[W - 1][e] = to_f32(vx.e[e]);
+            float p[VEC];
+            cols.dot(p, win);
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) {
+                float g = to_f32(vg.e[e]);
+                if (a.silu) {
+                    const float s = conv_sigmoid(p[e]);
+                    g *= s * fmaf(p[e], 1.f - s, 1.f);
+                }
+                dp[W - 1][e] = g;
+            }
+            if (mine)
+#pragma unroll
+                for (int e = 0; e < VEC; ++e) {
+                    db[e] += dp[W - 1][e];
+#pragma unroll
+                    for (int k = 0; k < W; ++k) dw[k][e] = fmaf(dp[W - 1][e], win[k][e], dw[k][e]);
+                }
+        };
+        auto gradient = [&](float* g) {
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) {
+                g[e] = cols.w[0][e] * dp[W - 1][e];
+#pragma unroll
+                for (int k = 1; k < W; ++k) g[e] = fmaf(cols.w[k][e], dp[W - 1 - k][e], g[e]);
+            }
+        };
         // the inputs of a row's first run reach back to the state
         const int64_t first = t0 == 0 ? -(W - 1) : t0;
         const int64_t stop = t0 < len || t0 == 0 ? tl + W - 1 : t0;
-        for (int64_t t = t0; t < stop; t += U) {
-            RowVec<T, VEC> rx[U], rg[U];
+        auto any = [&](int64_t tt) {  // a token near either end of the run
+            const int64_t o = tt - (W - 1);
+            shift();
+            if (tt < len) {
+                token(*reinterpret_cast<const V*>(x + tt * a.sx[1]), *reinterpret_cast<const V*>(dy + tt * a.sdy[1]), tt < tl);
+            } else {
 #pragma unroll
-            for (int u = 0; u < U; ++u)
-                if (t + u < min(stop, len)) {
-                    rx[u] = *reinterpret_cast<const RowVec<T, VEC>*>(x + (t + u) * a.sx[1]);
-                    rg[u] = *reinterpret_cast<const RowVec<T, VEC>*>(dy + (t + u) * a.sdy[1]);
-                }
+                for (int e = 0; e < VEC; ++e) dp[W - 1][e] = 0.f;
+            }
+            if (o < first || o >= len) return;
+            float g[VEC];
+            gradient(g);
+            const int64_t f = o - (len - (W - 1));  // its place in the final state
+            if (dhN && f >= 0) {
+                float v[VEC];
+                conv_read<T, VEC>(v, dhN + (b * (W - 1) + f) * a.D + c);
+#pragma unroll
+                for (int e = 0; e < VEC; ++e) g[e] += v[e];
+            }
+            if (o >= 0) conv_write<T, VEC>(dx + o * a.D, g);
+            else if (a.dh0) conv_write<T, VEC>(static_cast<T*>(a.dh0) + (b * (W - 1) + o + W - 1) * a.D + c, g);
+        };
+        int64_t t = t0;
+        for (; t < min(t0 + W - 1, stop); ++t) any(t);
+        // between them every token is the run's own and completes an input of the run; none of those is in the final state
+        const T *px = x + t * a.sx[1], *pg = dy + t * a.sdy[1];
+        T* pd = dx + (t - (W - 1)) * a.D;
+        for (; t + U <= tl; t += U) {
+            V rx[U], rg[U];
 #pragma unroll
             for (int u = 0; u < U; ++u) {
-                const int64_t tt = t + u, o = tt - (W - 1);  // the input whose gradient is now whole
-                if (tt >= stop) break;
+                rx[u] = *reinterpret_cast<const V*>(px + u * a.sx[1]);
+                rg[u] = *reinterpret_cast<const V*>(pg + u * a.sdy[1]);
+            }
+            px += U * a.sx[1];
+            pg += U * a.sdy[1];
 #pragma unroll
-                for (int k = 0; k + 1 < W; ++k)
-#pragma unroll
-                    for (int e = 0; e < VEC; ++e) dp[k][e] = dp[k + 1][e], win[k][e] = win[k + 1][e];
-                if (tt < len) {
-#pragma unroll
-                    for (int e = 0; e < VEC; ++e) win[W - 1][e] = to_f32(rx[u].e[e]);
-                    float p[VEC];
-                    cols.dot(p, win);
-#pragma unroll
-                    for (int e = 0; e < VEC; ++e) {
-                        float g = to_f32(rg[u].e[e]);
-                        if (a.silu) {
-                            const float s = conv_sigmoid(p[e]);
-                            g *= s * fmaf(p[e], 1.f - s, 1.f);
-                        }
-                        dp[W - 1][e] = g;
-                    }
-                    if (tt < tl)
-#pragma unroll
-                        for (int e = 0; e < VEC; ++e) {
-                            db[e] += dp[W - 1][e];
-#pragma unroll
-                            for (int k = 0; k < W; ++k) dw[k][e] = fmaf(dp[W - 1][e], win[k][e], dw[k][e]);
-                        }
-                } else {
-#pragma unroll
-                    for (int e = 0; e < VEC; ++e) dp[W - 1][e] = 0.f;
-                }
-                if (o < first || o >= len) continue;
-                float g[VEC] = {};
-#pragma unroll
-                for (int k = 0; k < W; ++k)
-#pragma unroll
-                    for (int e = 0; e < VEC; ++e) g[e] = fmaf(cols.w[k][e], dp[W - 1 - k][e], g[e]);
-                const int64_t f = o - (len - (W - 1));  // its place in the final state
-                if (dhN && f >= 0) {
-                    float v[VEC];
-                    conv_read<T, VEC>(v, dhN + (b * (W - 1) + f) * a.D + c);
-#pragma unroll
-                    for (int e = 0; e < VEC; ++e) g[e] += v[e];
-                }
-                if (o >= 0) conv_write<T, VEC>(dx + o * a.D, g);
-                else if (a.dh0) conv_write<T, VEC>(static_cast<T*>(a.dh0) + (b * (W - 1) + o + W - 1) * a.D + c, g);
+            for (int u = 0; u < U; ++u) {
+                shift();
+                token(rx[u], rg[u], true);
+                float g[VEC];
+                gradient(g);
+                conv_write<T, VEC>(pd, g);
+                pd += a.D;
             }
         }
+        for (; t < stop; ++t) any(t);
         const float nil[VEC] = {};
-        for (int64_t t = max(t0, tl); t < t1; ++t) conv_write<T, VEC>(dx + t * a.D, nil);
+        for (t = max(t0, tl); t < t1; ++t) conv_write<T, VEC>(dx + t * a.D, nil);
     }
     if (!a.part) return;
     float* part = a.part + static_cast<int64_t>(blockIdx.y) * a.D * (W + 1);
@@ -338,8 +371,7 @@ cudaError_t conv_step_launch(ConvArgs& a, cudaStream_t s) {
 
 template <typename T>
 cudaError_t conv_fwd_any(ConvArgs& a, int width, bool vec, cudaStream_t s) {
-    constexpr int E = 16 / sizeof(T);
-    return vec ? EACS_CONV_W(T, E, conv_fwd_launch, a, s) : EACS_CONV_W(T, 1, conv_fwd_launch, a, s);
+    return vec ? EACS_CONV_W(T, 4, conv_fwd_launch, a, s) : EACS_CONV_W(T, 1, conv_fwd_launch, a, s);
 }
 template <typename T>
 cudaError_t conv_step_any(ConvArgs& a, int width, bool vec, cudaStream_t s) {
@@ -402,7 +434,7 @@ int conv_fwd(const EacsConv& p, void* y, void* final_state, cudaStream_t stream)
     a.y = y;
     a.hN = final_state;
     if (p.L == 0 && !final_state) return EACS_OK;
-    const bool vec = conv_vec(p, p.dtype == EACS_DTYPE_F32 ? 4 : 8, {p.x, y, p.initial_state, final_state}, {p.x_stride[0], p.x_stride[1]});
+    const bool vec = conv_vec(p, 4, {p.x, y, p.initial_state, final_state}, {p.x_stride[0], p.x_stride[1]});
     const cudaError_t e = p.dtype == EACS_DTYPE_F32   ? conv_fwd_any<float>(a, p.width, vec, stream)
                           : p.dtype == EACS_DTYPE_F16 ? conv_fwd_any<__half>(a, p.width, vec, stream)
                                                       : conv_fwd_any<__nv_bfloat16>(a, p.width, vec, stream);

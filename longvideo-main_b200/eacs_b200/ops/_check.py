@@ -53,16 +53,46 @@ def require_plain(name: str, *ts: torch.Tensor | None) -> None:
 
 
 def one_device(name: str, first: torch.Tensor, *ts: torch.Tensor | None) -> torch.device:
-    """cuda_tensors for tensors of which some may be None, without a loop's cost on the way that passes."""
-    dev = first.device if isinstance(first, torch.Tensor) else None
-    if dev is None or dev.type != "cuda" or any(t is not None and (not isinstance(t, torch.Tensor) or t.device != dev)
-                                                for t in ts):
-        return cuda_tensors(name, first, *(t for t in ts if t is not None))
-    return dev
+    """cuda_tensors for tensors of which some may be None, without its cost on the way that passes."""
+    if isinstance(first, torch.Tensor) and first.is_cuda:
+        index = first.get_device()
+        for t in ts:
+            if t is not None and (not isinstance(t, torch.Tensor) or t.get_device() != index):
+                break
+        else:
+            return first.device
+    return cuda_tensors(name, first, *(t for t in ts if t is not None))
 
 
-def dense_last(t: torch.Tensor) -> torch.Tensor:
+def wants_grad(*ts: torch.Tensor | None) -> bool:
+    """Whether gradients are enabled and one of these wants one."""
+    if torch.is_grad_enabled():
+        for t in ts:
+            if t is not None and t.requires_grad:
+                return True
+    return False
+
+
+def dense(t: torch.Tensor | None) -> torch.Tensor | None:
+    return None if t is None else t.contiguous()
+
+
+def new_like(t: torch.Tensor | None) -> torch.Tensor | None:
+    """An uninitialised dense tensor of t's shape, dtype and device."""
+    return None if t is None else torch.empty_like(t, memory_format=torch.contiguous_format)
+
+
+def once(backward):
+    """torch's once_differentiable, whose cost only a backward with create_graph pays."""
+    recorded = torch.autograd.function.once_differentiable(backward)
+
+    def run(ctx, *grads):
+        return recorded(ctx, *grads) if torch.is_grad_enabled() else backward(ctx, *grads)
+    return run
+
+
+def dense_last(t: torch.Tensor | None) -> torch.Tensor | None:
     """t, copied if its last dimension is not dense."""
-    if t.stride(-1) == 1 or t.shape[-1] == 1:
+    if t is None or t.stride(-1) == 1 or t.shape[-1] == 1:
         return t
     return t.contiguous()

@@ -24,23 +24,26 @@ import torch
 from torch import Tensor
 
 from .. import _lib
-from ._check import on, one_device, require_plain
+from ._check import dense, new_like, on, once, one_device, require_plain, wants_grad
 from .layer_norm import MAX_D, _rows
 
 
 def _args(x, gate, residual, weight, scale, post, post_norm, eps):
     """EacsNorm, and the tensors that it points into."""
     d = x.shape[-1]
-    (xr, xs), (gr, gs), (rr, rs) = ((None, 0) if t is None else _rows(t, d) for t in (x, gate, residual))
-    p = lambda t: 0 if t is None else t.data_ptr()
-    w = next((t for t in (weight, scale, post) if t is not None), None)
-    return _lib.NORM.pack(xr.data_ptr(), p(gr), p(rr), p(weight), p(scale), p(post), xs, gs, rs, x.numel() // d, d, eps,
-                          _lib.DTYPE_CODES[x.dtype], 0 if w is None else _lib.DTYPE_CODES[w.dtype], int(post_norm)), (xr, gr, rr)
+    xr, xs = _rows(x, d)
+    gr, gs = (None, 0) if gate is None else _rows(gate, d)
+    rr, rs = (None, 0) if residual is None else _rows(residual, d)
+    w = weight if weight is not None else scale if scale is not None else post
+    return _lib.NORM.pack(xr.data_ptr(), 0 if gr is None else gr.data_ptr(), 0 if rr is None else rr.data_ptr(),
+                          0 if weight is None else weight.data_ptr(), 0 if scale is None else scale.data_ptr(),
+                          0 if post is None else post.data_ptr(), xs, gs, rs, x.numel() // d, d, eps,
+                          _lib.DTYPE_CODES[x.dtype], 0 if w is None else _lib.DTYPE_CODES[w.dtype], post_norm), (xr, gr, rr)
 
 
 def _forward(x, gate, residual, weight, scale, post, post_norm, eps, dev):
-    y = torch.empty(x.shape, dtype=x.dtype, device=dev)
-    s = None if residual is None else torch.empty(x.shape, dtype=x.dtype, device=dev)
+    y = new_like(x)
+    s = None if residual is None else new_like(x)
     if y.numel():
         p, held = _args(x, gate, residual, weight, scale, post, post_norm, eps)
         with on(dev):
@@ -58,28 +61,29 @@ class BlockNormFunction(torch.autograd.Function):
         return y if s is None else (y, s)
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
+    @once
     def backward(ctx, dy, ds=None):
         x, gate, residual, weight, scale, post = ctx.saved_tensors
         if dy is None and ds is None:
             return (None,) * 9
         need, dev, d = ctx.needs_input_grad, ctx.dev, x.shape[-1]
-        weight, scale, post = (None if t is None else t.contiguous() for t in (weight, scale, post))
-        like = lambda t: torch.empty(t.shape, dtype=t.dtype, device=dev)
-        dw, dc, dp = (like(t) if need[i] else None for i, t in ((3, weight), (4, scale), (5, post)))
+        weight, scale, post = dense(weight), dense(scale), dense(post)
+        dw = new_like(weight) if need[3] else None
+        dc = new_like(scale) if need[4] else None
+        dp = new_like(post) if need[5] else None
+        same = residual is not None and gate is None and scale is None and not ctx.post_norm  # as a sum's backward gives it
+        dx, dg = new_like(x), new_like(gate)
+        dr = None if same else new_like(residual)
         if x.numel() == 0:
             zero = lambda t: None if t is None else t.zero_()
-            return like(x), None if gate is None else like(gate), None if residual is None else like(residual), zero(dw), zero(dc), \
-                zero(dp), None, None, None
+            return dx, dg, dx if same else dr, zero(dw), zero(dc), zero(dp), None, None, None
         p, held = _args(x, gate, residual, weight, scale, post, ctx.post_norm, ctx.eps)
-        dx, dg = like(x), None if gate is None else like(gate)
-        same = residual is not None and gate is None and scale is None and not ctx.post_norm  # as a sum's backward gives it
-        dr = None if residual is None or same else like(residual)
-        (gr, gs), (sr, ss) = ((None, 0) if t is None else _rows(t, d) for t in (dy, ds))
+        gr, gs = (None, 0) if dy is None else _rows(dy, d)
+        sr, ss = (None, 0) if ds is None else _rows(ds, d)
         L_ = _lib.lib()
         ws = None
         if dw is not None or dc is not None or dp is not None:
-            ws = torch.empty(int(L_.eacs_norm_bwd_workspace_size(p)), dtype=torch.uint8, device=dev)
+            ws = x.new_empty(L_.eacs_norm_bwd_workspace_size(p), dtype=torch.uint8)
         with on(dev):
             _lib.check(L_.eacs_norm_bwd(p, _lib.ptr(gr), gs, _lib.ptr(sr), ss, dx.data_ptr(), _lib.ptr(dg), _lib.ptr(dr),
                                         _lib.ptr(dw), _lib.ptr(dc), _lib.ptr(dp), _lib.ptr(ws), 0 if ws is None else ws.numel(),
@@ -95,19 +99,19 @@ def _run(name, x, gate, residual, weight, scale, post, post_norm, eps):
     d = x.shape[-1]
     if not 1 <= d <= MAX_D:
         raise RuntimeError(f"{name}: d={d} must be 1 to {MAX_D}")
-    for n, t in (("gate", gate), ("residual", residual)):
+    for t in (gate, residual):
         if t is not None and (t.shape != x.shape or t.dtype != x.dtype):
-            raise RuntimeError(f"{name}: {n} must have x's shape and dtype")
-    dtypes = set()
+            raise RuntimeError(f"{name}: {'gate' if t is gate else 'residual'} must have x's shape and dtype")
+    w = None
     for t in (weight, scale, post):
         if t is not None:
             if t.dim() != 1 or t.shape[0] != d or t.dtype not in _lib.DTYPE_CODES:
                 raise RuntimeError(f"{name}: weight, scale and post_weight must be ({d},), float32, float16 or bfloat16")
-            dtypes.add(t.dtype)
-    if len(dtypes) > 1:
-        raise RuntimeError(f"{name}: weight, scale and post_weight must have one dtype")
-    weight, scale, post = (None if t is None else t.contiguous() for t in (weight, scale, post))
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, gate, residual, weight, scale, post)):
+            if w is not None and t.dtype != w:
+                raise RuntimeError(f"{name}: weight, scale and post_weight must have one dtype")
+            w = t.dtype
+    weight, scale, post = dense(weight), dense(scale), dense(post)
+    if wants_grad(x, gate, residual, weight, scale, post):
         out = BlockNormFunction.apply(x, gate, residual, weight, scale, post, post_norm, float(eps), dev)
         return out if residual is not None else (out, None)
     return _forward(x, gate, residual, weight, scale, post, post_norm, float(eps), dev)

@@ -27,7 +27,7 @@ import torch
 from torch import Tensor
 
 from .. import _lib
-from ._check import dense_last, on, one_device, require_plain
+from ._check import dense, dense_last, new_like, on, once, one_device, require_plain, wants_grad
 
 MIN_WIDTH, MAX_WIDTH = 2, 4
 
@@ -65,8 +65,8 @@ def _args(x, weight, bias, activation, lengths, state) -> bytes:
 
 
 def _forward(x, weight, bias, activation, lengths, state, out_state, dev):
-    y = torch.empty(x.shape, dtype=x.dtype, device=dev)
-    final = torch.empty(x.shape[0], weight.shape[1] - 1, x.shape[2], dtype=x.dtype, device=dev) if out_state else None
+    y = new_like(x)
+    final = x.new_empty((x.shape[0], weight.shape[1] - 1, x.shape[2])) if out_state else None
     with on(dev):
         _lib.check(_lib.lib().eacs_conv_fwd(_args(x, weight, bias, activation, lengths, state), y.data_ptr(),
                                             _lib.ptr(final), _lib.raw_stream(dev.index)), "eacs_conv_fwd")
@@ -83,27 +83,24 @@ class CausalConvFunction(torch.autograd.Function):
         return (y, final) if out_state else y
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
+    @once
     def backward(ctx, dy, dfinal=None):
         x, weight, bias, lengths, initial = ctx.saved_tensors
         dev = ctx.dev
         if dy is None and dfinal is None:
             return (None,) * 8
         # hooks may give saved tensors back in another layout
-        x = dense_last(x)
-        weight, bias, lengths, initial = (None if t is None else t.contiguous() for t in (weight, bias, lengths, initial))
+        x, weight, bias, lengths, initial = dense_last(x), dense(weight), dense(bias), dense(lengths), dense(initial)
         dy = torch.zeros(x.shape, dtype=x.dtype, device=dev) if dy is None else dense_last(dy)
-        dfinal = None if dfinal is None else dfinal.contiguous()
+        dfinal = dense(dfinal)
         p = _args(x, weight, bias, ctx.activation, lengths, initial)
-        need = ctx.needs_input_grad
-        dx = torch.empty(x.shape, dtype=x.dtype, device=dev)
-        dw = torch.empty(weight.shape, dtype=weight.dtype, device=dev) if need[1] else None
-        db = torch.empty(bias.shape, dtype=bias.dtype, device=dev) if need[2] else None
-        di = torch.empty(initial.shape, dtype=initial.dtype, device=dev) if need[5] else None
+        _, need_w, need_b, _, _, need_i, _, _ = ctx.needs_input_grad
+        dx = new_like(x)
+        dw = new_like(weight) if need_w else None
+        db = new_like(bias) if need_b else None
+        di = new_like(initial) if need_i else None
         L_ = _lib.lib()
-        ws = None
-        if dw is not None or db is not None:
-            ws = torch.empty(int(L_.eacs_conv_bwd_workspace_size(p)), dtype=torch.uint8, device=dev)
+        ws = x.new_empty(L_.eacs_conv_bwd_workspace_size(p), dtype=torch.uint8) if need_w or need_b else None
         with on(dev):
             _lib.check(L_.eacs_conv_bwd(p, dy.data_ptr(), (ctypes.c_int64 * 2)(*dy.stride()[:2]), _lib.ptr(dfinal),
                                         dx.data_ptr(), _lib.ptr(dw), _lib.ptr(db), _lib.ptr(di), _lib.ptr(ws),
@@ -121,9 +118,8 @@ def causal_conv(x: Tensor, weight: Tensor, bias: Tensor | None = None, activatio
     Differentiable in x, weight, bias and initial_state, through y and the
     final state."""
     dev = _check("causal_conv", x, weight, bias, activation, lengths, initial_state, 2)
-    x, weight = dense_last(x), weight.contiguous()
-    bias, lengths, state = (None if t is None else t.contiguous() for t in (bias, lengths, initial_state))
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, bias, state)):
+    x, weight, bias, lengths, state = dense_last(x), dense(weight), dense(bias), dense(lengths), dense(initial_state)
+    if wants_grad(x, weight, bias, state):
         return CausalConvFunction.apply(x, weight, bias, activation, lengths, state, output_final_state, dev)
     y, final = _forward(x, weight, bias, activation, lengths, state, output_final_state, dev)
     return (y, final) if output_final_state else y
@@ -134,13 +130,12 @@ def causal_conv_step(x: Tensor, weight: Tensor, bias: Tensor | None, state: Tens
     on in place.  Returns y (B, D).  No gradient: inputs that want one are
     refused where gradients are enabled."""
     dev = _check("causal_conv_step", x, weight, bias, activation, None, state, 1)
-    if torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad or (bias is not None and bias.requires_grad)):
+    if wants_grad(x, weight, bias):
         raise RuntimeError("causal_conv_step: has no gradient; call it under torch.no_grad() or with detached tensors")
     if not state.is_contiguous() or state.requires_grad:
         raise RuntimeError("causal_conv_step: the state is updated in place: it must be contiguous and without a gradient")
-    x, weight = dense_last(x), weight.contiguous()
-    bias = None if bias is None else bias.contiguous()
-    y = torch.empty(x.shape, dtype=x.dtype, device=dev)
+    x, weight, bias = dense_last(x), dense(weight), dense(bias)
+    y = new_like(x)
     with on(dev):
         _lib.check(_lib.lib().eacs_conv_step(_args(x, weight, bias, activation, None, None), y.data_ptr(), state.data_ptr(),
                                              _lib.raw_stream(dev.index)), "eacs_conv_step")

@@ -35,7 +35,7 @@ import torch
 from torch import Tensor
 
 from .. import _lib
-from ._check import dense_last, on, one_device, require_plain
+from ._check import dense, dense_last, new_like, on, once, one_device, require_plain, wants_grad
 
 MAX_N = 64
 
@@ -85,9 +85,9 @@ def _forward(args, out_state, training, dev):
     x, A = args[0], args[2]
     p = _args(*args)
     L_ = _lib.lib()
-    y = torch.empty(x.shape, dtype=x.dtype, device=dev)
-    final = torch.empty(x.shape[0], *A.shape, dtype=torch.float32, device=dev) if out_state else None
-    ck = torch.empty(int(L_.eacs_selective_ckpt_size(p)), dtype=torch.uint8, device=dev) if training else None
+    y = new_like(x)
+    final = A.new_empty((x.shape[0], *A.shape)) if out_state else None
+    ck = x.new_empty(L_.eacs_selective_ckpt_size(p), dtype=torch.uint8) if training else None
     with on(dev):
         _lib.check(L_.eacs_selective_fwd(p, y.data_ptr(), _lib.ptr(final), _lib.ptr(ck), 0 if ck is None else ck.numel(),
                                          _lib.raw_stream(dev.index)), "eacs_selective_fwd")
@@ -104,23 +104,23 @@ class SelectiveSSMFunction(torch.autograd.Function):
         return (y, final) if out_state else y
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
+    @once
     def backward(ctx, dy, dfinal=None):
         x, dt, A, B, C, skip, z, dt_bias, lengths, initial, ck = ctx.saved_tensors
         dev = ctx.dev
         if dy is None and dfinal is None:
             return (None,) * 13
         # hooks may give saved tensors back in another layout
-        x, dt, B, C, z = (None if t is None else dense_last(t) for t in (x, dt, B, C, z))
-        A, skip, dt_bias, lengths, initial = (None if t is None else t.contiguous() for t in (A, skip, dt_bias, lengths, initial))
+        x, dt, B, C, z = dense_last(x), dense_last(dt), dense_last(B), dense_last(C), dense_last(z)
+        A, skip, dt_bias, lengths, initial = dense(A), dense(skip), dense(dt_bias), dense(lengths), dense(initial)
         dy = torch.zeros(x.shape, dtype=x.dtype, device=dev) if dy is None else dense_last(dy)
-        dfinal = None if dfinal is None else dfinal.contiguous()
+        dfinal = dense(dfinal)
         p = _args(x, dt, A, B, C, skip, z, dt_bias, ctx.softplus, lengths, initial)
-        like = lambda t: None if t is None else torch.empty(t.shape, dtype=t.dtype, device=dev)
-        dx, ddt, dA, dB, dC, dskip, dz, dbias = (like(t) for t in (x, dt, A, B, C, skip, z, dt_bias))
-        di = like(initial) if ctx.needs_input_grad[10] else None
+        dx, ddt, dA, dB, dC = new_like(x), new_like(dt), new_like(A), new_like(B), new_like(C)
+        dskip, dz, dbias = new_like(skip), new_like(z), new_like(dt_bias)
+        di = new_like(initial) if ctx.needs_input_grad[10] else None
         L_ = _lib.lib()
-        ws = torch.empty(int(L_.eacs_selective_bwd_workspace_size(p)), dtype=torch.uint8, device=dev)
+        ws = x.new_empty(L_.eacs_selective_bwd_workspace_size(p), dtype=torch.uint8)
         with on(dev):
             _lib.check(L_.eacs_selective_bwd(
                 p, dy.data_ptr(), (ctypes.c_int64 * 2)(*dy.stride()[:2]), _lib.ptr(dfinal), dx.data_ptr(), ddt.data_ptr(),
@@ -141,11 +141,9 @@ def selective_ssm(x: Tensor, dt: Tensor, A: Tensor, B: Tensor, C: Tensor, skip: 
     behind is not read, its outputs and gradients are 0.  Differentiable in
     every floating point input, through y and the final state."""
     dev = _check("selective_ssm", x, dt, A, B, C, skip, z, dt_bias, lengths, initial_state)
-    x, dt, B, C = dense_last(x), dense_last(dt), dense_last(B), dense_last(C)
-    z = None if z is None else dense_last(z)
-    A = A.contiguous()
-    skip, dt_bias, lengths, state = (None if t is None else t.contiguous() for t in (skip, dt_bias, lengths, initial_state))
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, dt, A, B, C, skip, z, dt_bias, state)):
+    x, dt, B, C, z = dense_last(x), dense_last(dt), dense_last(B), dense_last(C), dense_last(z)
+    A, skip, dt_bias, lengths, state = dense(A), dense(skip), dense(dt_bias), dense(lengths), dense(initial_state)
+    if wants_grad(x, dt, A, B, C, skip, z, dt_bias, state):
         return SelectiveSSMFunction.apply(x, dt, A, B, C, skip, z, dt_bias, bool(softplus), lengths, state,
                                           output_final_state, dev)
     y, final, _ = _forward((x, dt, A, B, C, skip, z, dt_bias, softplus, lengths, state), output_final_state, False, dev)
@@ -158,15 +156,13 @@ def selective_ssm_step(x: Tensor, dt: Tensor, A: Tensor, B: Tensor, C: Tensor, s
     float32, contiguous, is updated in place.  Returns y (B, D) in x's dtype.
     No gradient: inputs that want one are refused where gradients are enabled."""
     dev = _check("selective_ssm_step", x, dt, A, B, C, skip, z, dt_bias, None, state)
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, dt, A, B, C, skip, z, dt_bias)):
+    if wants_grad(x, dt, A, B, C, skip, z, dt_bias):
         raise RuntimeError("selective_ssm_step: has no gradient; call it under torch.no_grad() or with detached tensors")
     if not state.is_contiguous() or state.requires_grad:
         raise RuntimeError("selective_ssm_step: the state is updated in place: it must be contiguous and without a gradient")
-    x, dt, B, C = dense_last(x), dense_last(dt), dense_last(B), dense_last(C)
-    z = None if z is None else dense_last(z)
-    A = A.contiguous()
-    skip, dt_bias = (None if t is None else t.contiguous() for t in (skip, dt_bias))
-    y = torch.empty(x.shape, dtype=x.dtype, device=dev)
+    x, dt, B, C, z = dense_last(x), dense_last(dt), dense_last(B), dense_last(C), dense_last(z)
+    A, skip, dt_bias = dense(A), dense(skip), dense(dt_bias)
+    y = new_like(x)
     p = _args(x, dt, A, B, C, skip, z, dt_bias, softplus, None, None)
     with on(dev):
         _lib.check(_lib.lib().eacs_selective_step(p, y.data_ptr(), state.data_ptr(), _lib.raw_stream(dev.index)),
