@@ -6,12 +6,15 @@
 //   dx_t = sum_w weight[w] dp_{t+W-1-w},   dweight[w] = sum_t dp_t x_{t-W+1+w},   dbias = sum_t dp_t,
 // and what the final state's gradient adds to the last W - 1 inputs.
 //
-// Bound by memory both ways: each value is read once (but for the W - 1 tokens in front of a run) and written once.  A
-// thread takes VEC channels of a run of tokens; the W inputs that a token sees move through its registers.  Runs are as
-// long as leaves every multiprocessor full of threads once, so that the tokens read twice are few and no round of CTAs
-// runs half empty.  The backward takes p again from x (the forward saves nothing) and keeps dweight and dbias of its run in
-// registers; the runs of a CTA are added in shared memory, and a second kernel adds the CTAs' partial rows in order (no
-// atomics: the same inputs give the same bits).
+// Bound by memory both ways: each value is read once (but for the W - 1 tokens around a run) and written once.  A warp takes
+// 64 channels, two a lane, of a run of tokens; rows of 128 (float32: 256) bytes come through shared memory, asked for two
+// stages of 16 tokens ahead (cp.async, its own, so without a barrier between warps), and the W inputs that a token sees
+// move through the lanes' registers as pairs.  Through registers the same loads left too few threads: 67 us against 50 at
+// B=4 L=16384 D=1024 forward, 127 against 70 the backward at B=8 L=8192 D=768.  Runs are as long as leaves every
+// multiprocessor full of warps once.  Rows that do not start on 16 bytes take kernels of one channel a thread.
+// The backward takes p again from x (the forward saves nothing) and keeps dweight and dbias of its run in registers; the
+// runs of a CTA are added in shared memory, and a second kernel adds the CTAs' partial rows in order (no atomics: the same
+// inputs give the same bits).
 #include <algorithm>
 
 #include "eacs_common.cuh"
@@ -66,17 +69,52 @@ __device__ __forceinline__ void conv_write(T* p, const float* v) {
     *reinterpret_cast<RowVec<T, VEC>*>(p) = r;
 }
 
+// A thread's VEC channels as float32, two to a register pair where there are two.
+__device__ __forceinline__ float vfma(float a, float b, float c) { return fmaf(a, b, c); }
+__device__ __forceinline__ f32x2 vfma(f32x2 a, f32x2 b, f32x2 c) { return fma2(a, b, c); }
+__device__ __forceinline__ float vmul(float a, float b) { return a * b; }
+__device__ __forceinline__ f32x2 vmul(f32x2 a, f32x2 b) { return mul2(a, b); }
+__device__ __forceinline__ float vadd(float a, float b) { return a + b; }
+__device__ __forceinline__ f32x2 vadd(f32x2 a, f32x2 b) { return add2(a, b); }
+template <int VEC>
+struct ConvVal {
+    using P = f32x2;
+    static constexpr int N = VEC / 2;
+    P v[N];
+    __device__ __forceinline__ void set(const float* f) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) v[i] = pair(f[2 * i], f[2 * i + 1]);
+    }
+    __device__ __forceinline__ void get(float* f) const {
+#pragma unroll
+        for (int i = 0; i < N; ++i) halves(v[i], f[2 * i], f[2 * i + 1]);
+    }
+};
+template <>
+struct ConvVal<1> {
+    using P = float;
+    static constexpr int N = 1;
+    P v[1];
+    __device__ __forceinline__ void set(const float* f) { v[0] = f[0]; }
+    __device__ __forceinline__ void get(float* f) const { f[0] = v[0]; }
+};
+
 // One thread's channels: taps, and the inputs in front of token t0.
 template <typename T, int VEC, int W>
 struct ConvCols {
-    float w[W][VEC], bias[VEC];
+    using Val = ConvVal<VEC>;
+    Val w[W], bias;
     __device__ __forceinline__ void taps(const ConvArgs& a, int c) {
+        float f[VEC];
 #pragma unroll
-        for (int e = 0; e < VEC; ++e) {
+        for (int k = 0; k < W; ++k) {
 #pragma unroll
-            for (int k = 0; k < W; ++k) w[k][e] = read_param(a.weight, a.w_dtype, (c + e) * W + k, 0.f);
-            bias[e] = read_param(a.bias, a.w_dtype, c + e, 0.f);
+            for (int e = 0; e < VEC; ++e) f[e] = read_param(a.weight, a.w_dtype, (c + e) * W + k, 0.f);
+            w[k].set(f);
         }
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) f[e] = read_param(a.bias, a.w_dtype, c + e, 0.f);
+        bias.set(f);
     }
     // input number t of row b (t >= -(W - 1)): the row's, or the state's
     static __device__ __forceinline__ void input(float* v, const ConvArgs& a, const T* x, int64_t b, int64_t t, int c) {
@@ -89,206 +127,353 @@ struct ConvCols {
             for (int e = 0; e < VEC; ++e) v[e] = 0.f;
         }
     }
-    __device__ __forceinline__ void dot(float* p, const float (&win)[W][VEC]) const {
+    // the window in front of token t0, one place behind (a token moves it on)
+    static __device__ __forceinline__ void window(Val* win, const ConvArgs& a, const T* x, int64_t b, int64_t t0, int c) {
+        float v[VEC];
 #pragma unroll
-        for (int e = 0; e < VEC; ++e) {
-            p[e] = bias[e];
+        for (int k = 1; k < W; ++k) {
+            input(v, a, x, b, t0 - W + k, c);
+            win[k].set(v);
+        }
+    }
+    __device__ __forceinline__ void dot(float* p, const Val* win) const {
+        Val q = bias;
 #pragma unroll
-            for (int k = 0; k < W; ++k) p[e] = fmaf(w[k][e], win[k][e], p[e]);
+        for (int k = 0; k < W; ++k)
+#pragma unroll
+            for (int i = 0; i < Val::N; ++i) q.v[i] = vfma(w[k].v[i], win[k].v[i], q.v[i]);
+        q.get(p);
+    }
+};
+
+// One run of one thread's channels, forward: a token's input comes in, its output goes out.
+template <typename T, int VEC, int W>
+struct ConvFwd {
+    using Cols = ConvCols<T, VEC, W>;
+    using V = RowVec<T, VEC>;
+    Cols cols;
+    typename Cols::Val win[W];  // the inputs a token sees, its own last
+    __device__ __forceinline__ void token(const V& v, T* y, bool silu) {
+#pragma unroll
+        for (int k = 0; k + 1 < W; ++k) win[k] = win[k + 1];
+        float p[VEC];
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) p[e] = to_f32(v.e[e]);
+        win[W - 1].set(p);
+        cols.dot(p, win);
+        if (silu)
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) p[e] *= conv_sigmoid(p[e]);
+        conv_write<T, VEC>(y, p);
+    }
+};
+// The state behind row b, by the threads of its first run.
+template <typename T, int VEC, int W>
+__device__ __forceinline__ void conv_final(const ConvArgs& a, const T* x, int64_t b, int64_t len, int c) {
+    float v[VEC];
+#pragma unroll
+    for (int k = 0; k < W - 1; ++k) {
+        ConvCols<T, VEC, W>::input(v, a, x, b, len - (W - 1) + k, c);
+        conv_write<T, VEC>(static_cast<T*>(a.hN) + (b * (W - 1) + k) * a.D + c, v);
+    }
+}
+
+// ... and backward: a token gives dp; the gradient of the input W - 1 tokens before it is then whole.
+template <typename T, int VEC, int W>
+struct ConvBwd {
+    using Cols = ConvCols<T, VEC, W>;
+    using Val = typename Cols::Val;
+    using V = RowVec<T, VEC>;
+    Cols cols;
+    Val win[W], dp[W];  // dp of the token and of the W - 1 before it
+    Val dw[W + 1];      // the taps' sums, the bias's last
+    __device__ __forceinline__ void clear() {
+        const float nil[VEC] = {};
+#pragma unroll
+        for (int k = 0; k < W; ++k) dp[k].set(nil);
+#pragma unroll
+        for (int k = 0; k <= W; ++k) dw[k].set(nil);
+    }
+    __device__ __forceinline__ void shift() {
+#pragma unroll
+        for (int k = 0; k + 1 < W; ++k) dp[k] = dp[k + 1], win[k] = win[k + 1];
+    }
+    __device__ __forceinline__ void token(const V& vx, const V& vg, bool mine, bool silu) {  // mine: one of the run's own
+        float p[VEC], g[VEC];
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) p[e] = to_f32(vx.e[e]), g[e] = to_f32(vg.e[e]);
+        win[W - 1].set(p);
+        if (silu) {
+            cols.dot(p, win);
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) {
+                const float s = conv_sigmoid(p[e]);
+                g[e] *= s * fmaf(p[e], 1.f - s, 1.f);
+            }
+        }
+        dp[W - 1].set(g);
+        if (mine)
+#pragma unroll
+            for (int i = 0; i < Val::N; ++i) {
+                dw[W].v[i] = vadd(dw[W].v[i], dp[W - 1].v[i]);
+#pragma unroll
+                for (int k = 0; k < W; ++k) dw[k].v[i] = vfma(dp[W - 1].v[i], win[k].v[i], dw[k].v[i]);
+            }
+    }
+    __device__ __forceinline__ void gradient(float* f) const {
+        Val g;
+#pragma unroll
+        for (int i = 0; i < Val::N; ++i) {
+            g.v[i] = vmul(cols.w[0].v[i], dp[W - 1].v[i]);
+#pragma unroll
+            for (int k = 1; k < W; ++k) g.v[i] = vfma(cols.w[k].v[i], dp[W - 1 - k].v[i], g.v[i]);
+        }
+        g.get(f);
+    }
+    // Token tt of row b near either end of the run t0.., whose own tokens end at tl; dx: the row's first token.
+    __device__ __forceinline__ void any(const ConvArgs& a, T* dx, const V& vx, const V& vg, int64_t b, int c, int64_t tt, int64_t t0, int64_t tl,
+                                        int64_t len) {
+        const int64_t o = tt - (W - 1), first = t0 == 0 ? -(W - 1) : t0;  // a row's first run reaches back to the state
+        const float nil[VEC] = {};
+        shift();
+        if (tt < len) token(vx, vg, tt < tl, a.silu);
+        else dp[W - 1].set(nil);
+        if (o < first || o >= len) return;
+        float g[VEC];
+        gradient(g);
+        const int64_t f = o - (len - (W - 1));  // its place in the final state
+        if (a.dhN && f >= 0) {
+            float v[VEC];
+            conv_read<T, VEC>(v, static_cast<const T*>(a.dhN) + (b * (W - 1) + f) * a.D + c);
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) g[e] += v[e];
+        }
+        if (o >= 0) conv_write<T, VEC>(dx + o * a.D, g);
+        else if (a.dh0) conv_write<T, VEC>(static_cast<T*>(a.dh0) + (b * (W - 1) + o + W - 1) * a.D + c, g);
+    }
+    // The sums of the CTA's R runs, added in order: one partial row.
+    template <int R>
+    __device__ __forceinline__ void sums(const ConvArgs& a, int c, bool live) const {
+        __shared__ float comb[R][32];
+        if (!a.part) return;
+        const int lane = threadIdx.x & 31, run = threadIdx.x >> 5;
+        float* part = a.part + static_cast<int64_t>(blockIdx.y) * a.D * (W + 1);
+#pragma unroll
+        for (int k = 0; k <= W; ++k) {
+            float v[VEC];
+            dw[k].get(v);
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) {
+                __syncthreads();
+                comb[run][lane] = v[e];
+                __syncthreads();
+                if (run == 0 && live) {
+                    float s = comb[0][lane];
+#pragma unroll
+                    for (int j = 1; j < R; ++j) s += comb[j][lane];
+                    part[k < W ? (c + e) * W + k : a.D * W + c + e] = s;
+                }
+            }
         }
     }
 };
 
-// U tokens are read before the first is used, so that many bytes are under way.  Vectors of 4 values: with 16 bytes of a
-// 16-bit type a thread's taps and window leave registers for a third of the threads (79 us instead of what stands at
-// conv_fwd_launch).
-template <typename T, int VEC, int W, int U>
-__global__ void __launch_bounds__(128) conv_fwd_k(const ConvArgs a) {
-    const int nv = a.D / VEC;
-    const int64_t i = static_cast<int64_t>(blockIdx.x) * 128 + threadIdx.x;
-    const int64_t r = i / nv;
-    if (r >= a.rows * a.runs) return;
-    const int c = static_cast<int>(i - r * nv) * VEC;
+constexpr int kConvRuns = 4;  // runs a CTA, one a warp
+
+// ---- one channel a thread: any strides --------------------------------------------------------------------
+template <typename T, int W, int U>
+__global__ void __launch_bounds__(32 * kConvRuns) conv_fwd_any_k(const ConvArgs a) {
+    const int c = blockIdx.x * 32 + (threadIdx.x & 31);
+    const int64_t r = static_cast<int64_t>(blockIdx.y) * kConvRuns + (threadIdx.x >> 5);
+    if (c >= a.D || r >= a.rows * a.runs) return;
     const int64_t b = r / a.runs, len = conv_length(a, b);
     const int64_t t0 = (r - b * a.runs) * a.run, t1 = min(t0 + a.run, a.L), tl = min(t1, len);
     const T* x = static_cast<const T*>(a.x) + b * a.sx[0] + c;
     T* y = static_cast<T*>(a.y) + b * a.L * a.D + c;
-    using Cols = ConvCols<T, VEC, W>;
-    Cols cols;
-    cols.taps(a, c);
-    float win[W][VEC];  // the inputs a token sees, its own last
-    if (t0 < tl)
+    ConvFwd<T, 1, W> f;
+    f.cols.taps(a, c);
+    if (t0 < tl) ConvCols<T, 1, W>::window(f.win, a, x, b, t0, c);
+    for (int64_t t = t0; t < tl; t += U) {
+        RowVec<T, 1> raw[U];
 #pragma unroll
-        for (int k = 1; k < W; ++k) Cols::input(win[k], a, x, b, t0 - W + k, c);
-    const T* px = x + t0 * a.sx[1];
-    T* py = y + t0 * a.D;
-    auto token = [&](const RowVec<T, VEC>& v) {
+        for (int u = 0; u < U; ++u)
+            if (t + u < tl) raw[u].e[0] = x[(t + u) * a.sx[1]];
 #pragma unroll
-        for (int e = 0; e < VEC; ++e) {
-#pragma unroll
-            for (int k = 0; k + 1 < W; ++k) win[k][e] = win[k + 1][e];
-            win[W - 1][e] = to_f32(v.e[e]);
-        }
-        float p[VEC];
-        cols.dot(p, win);
-        if (a.silu)
-#pragma unroll
-            for (int e = 0; e < VEC; ++e) p[e] *= conv_sigmoid(p[e]);
-        conv_write<T, VEC>(py, p);
-        py += a.D;
-    };
-    int64_t t = t0;
-    for (; t + U <= tl; t += U) {
-        RowVec<T, VEC> raw[U];
-#pragma unroll
-        for (int u = 0; u < U; ++u) raw[u] = *reinterpret_cast<const RowVec<T, VEC>*>(px + u * a.sx[1]);
-        px += U * a.sx[1];
-#pragma unroll
-        for (int u = 0; u < U; ++u) token(raw[u]);
+        for (int u = 0; u < U; ++u)
+            if (t + u < tl) f.token(raw[u], y + (t + u) * a.D, a.silu);
     }
-    for (; t < tl; ++t, px += a.sx[1]) token(*reinterpret_cast<const RowVec<T, VEC>*>(px));
-    const float nil[VEC] = {};
-    for (t = max(t0, tl); t < t1; ++t) conv_write<T, VEC>(y + t * a.D, nil);
-    if (a.hN && t0 == 0) {
-        float v[VEC];
-#pragma unroll
-        for (int k = 0; k < W - 1; ++k) {
-            Cols::input(v, a, x, b, len - (W - 1) + k, c);
-            conv_write<T, VEC>(static_cast<T*>(a.hN) + (b * (W - 1) + k) * a.D + c, v);
-        }
-    }
+    for (int64_t t = max(t0, tl); t < t1; ++t) y[t * a.D] = from_f32<T>(0.f);
+    if (a.hN && t0 == 0) conv_final<T, 1, W>(a, x, b, len, c);
 }
 
-// CTAs of 32 columns (VEC channels each) times R runs.  A token gives dp; the gradient of the input W - 1 tokens before it
-// is then whole.
-template <typename T, int VEC, int W, int R, int U>
-__global__ void __launch_bounds__(32 * R) conv_bwd_k(const ConvArgs a) {
-    __shared__ float comb[R][32];
-    const int nv = a.D / VEC, col = blockIdx.x * 32 + threadIdx.x;
-    const int64_t r = static_cast<int64_t>(blockIdx.y) * R + threadIdx.y;
-    const bool live = col < nv && r < a.rows * a.runs;
-    const int c = col * VEC;
-    float dw[W][VEC] = {}, db[VEC] = {};
-    if (live) {
+template <typename T, int W, int U>
+__global__ void __launch_bounds__(32 * kConvRuns) conv_bwd_any_k(const ConvArgs a) {
+    const int c = blockIdx.x * 32 + (threadIdx.x & 31);
+    const int64_t r = static_cast<int64_t>(blockIdx.y) * kConvRuns + (threadIdx.x >> 5);
+    ConvBwd<T, 1, W> f;
+    f.clear();
+    if (c < a.D && r < a.rows * a.runs) {
         const int64_t b = r / a.runs, len = conv_length(a, b);
         const int64_t t0 = (r - b * a.runs) * a.run, t1 = min(t0 + a.run, a.L), tl = min(t1, len);
         const T* x = static_cast<const T*>(a.x) + b * a.sx[0] + c;
         const T* dy = static_cast<const T*>(a.dy) + b * a.sdy[0] + c;
         T* dx = static_cast<T*>(a.dx) + b * a.L * a.D + c;
-        const T* dhN = static_cast<const T*>(a.dhN);
-        using Cols = ConvCols<T, VEC, W>;
-        using V = RowVec<T, VEC>;
-        Cols cols;
-        cols.taps(a, c);
-        float win[W][VEC], dp[W][VEC] = {};  // dp of the token and of the W - 1 before it
-        if (t0 < tl)
-#pragma unroll
-            for (int k = 1; k < W; ++k) Cols::input(win[k], a, x, b, t0 - W + k, c);
-        auto shift = [&] {
-#pragma unroll
-            for (int k = 0; k + 1 < W; ++k)
-#pragma unroll
-                for (int e = 0; e < VEC; ++e) dp[k][e] = dp[k + 1][e], win[k][e] = win[k + 1][e];
-        };
-        auto token = [&](const V& vx, const V& vg, bool mine) {  // mine: one of the run's own
-#pragma unroll
-            for (int e = 0; e < VEC; ++e) win[W - 1][e] = to_f32(vx.e[e]);
-            float p[VEC];
-            cols.dot(p, win);
-#pragma unroll
-            for (int e = 0; e < VEC; ++e) {
-                float g = to_f32(vg.e[e]);
-                if (a.silu) {
-                    const float s = conv_sigmoid(p[e]);
-                    g *= s * fmaf(p[e], 1.f - s, 1.f);
-                }
-                dp[W - 1][e] = g;
-            }
-            if (mine)
-#pragma unroll
-                for (int e = 0; e < VEC; ++e) {
-                    db[e] += dp[W - 1][e];
-#pragma unroll
-                    for (int k = 0; k < W; ++k) dw[k][e] = fmaf(dp[W - 1][e], win[k][e], dw[k][e]);
-                }
-        };
-        auto gradient = [&](float* g) {
-#pragma unroll
-            for (int e = 0; e < VEC; ++e) {
-                g[e] = cols.w[0][e] * dp[W - 1][e];
-#pragma unroll
-                for (int k = 1; k < W; ++k) g[e] = fmaf(cols.w[k][e], dp[W - 1 - k][e], g[e]);
-            }
-        };
-        // the inputs of a row's first run reach back to the state
-        const int64_t first = t0 == 0 ? -(W - 1) : t0;
+        f.cols.taps(a, c);
+        if (t0 < tl) ConvCols<T, 1, W>::window(f.win, a, x, b, t0, c);
         const int64_t stop = t0 < len || t0 == 0 ? tl + W - 1 : t0;
-        auto any = [&](int64_t tt) {  // a token near either end of the run
-            const int64_t o = tt - (W - 1);
-            shift();
-            if (tt < len) {
-                token(*reinterpret_cast<const V*>(x + tt * a.sx[1]), *reinterpret_cast<const V*>(dy + tt * a.sdy[1]), tt < tl);
-            } else {
+        for (int64_t t = t0; t < stop; t += U) {
+            RowVec<T, 1> rx[U], rg[U];
 #pragma unroll
-                for (int e = 0; e < VEC; ++e) dp[W - 1][e] = 0.f;
-            }
-            if (o < first || o >= len) return;
-            float g[VEC];
-            gradient(g);
-            const int64_t f = o - (len - (W - 1));  // its place in the final state
-            if (dhN && f >= 0) {
-                float v[VEC];
-                conv_read<T, VEC>(v, dhN + (b * (W - 1) + f) * a.D + c);
+            for (int u = 0; u < U; ++u)
+                if (t + u < min(stop, len)) rx[u].e[0] = x[(t + u) * a.sx[1]], rg[u].e[0] = dy[(t + u) * a.sdy[1]];
 #pragma unroll
-                for (int e = 0; e < VEC; ++e) g[e] += v[e];
-            }
-            if (o >= 0) conv_write<T, VEC>(dx + o * a.D, g);
-            else if (a.dh0) conv_write<T, VEC>(static_cast<T*>(a.dh0) + (b * (W - 1) + o + W - 1) * a.D + c, g);
-        };
-        int64_t t = t0;
-        for (; t < min(t0 + W - 1, stop); ++t) any(t);
-        // between them every token is the run's own and completes an input of the run; none of those is in the final state
-        const T *px = x + t * a.sx[1], *pg = dy + t * a.sdy[1];
-        T* pd = dx + (t - (W - 1)) * a.D;
-        for (; t + U <= tl; t += U) {
-            V rx[U], rg[U];
-#pragma unroll
-            for (int u = 0; u < U; ++u) {
-                rx[u] = *reinterpret_cast<const V*>(px + u * a.sx[1]);
-                rg[u] = *reinterpret_cast<const V*>(pg + u * a.sdy[1]);
-            }
-            px += U * a.sx[1];
-            pg += U * a.sdy[1];
-#pragma unroll
-            for (int u = 0; u < U; ++u) {
-                shift();
-                token(rx[u], rg[u], true);
-                float g[VEC];
-                gradient(g);
-                conv_write<T, VEC>(pd, g);
-                pd += a.D;
-            }
+            for (int u = 0; u < U; ++u)
+                if (t + u < stop) f.any(a, dx, rx[u], rg[u], b, c, t + u, t0, tl, len);
         }
-        for (; t < stop; ++t) any(t);
-        const float nil[VEC] = {};
-        for (t = max(t0, tl); t < t1; ++t) conv_write<T, VEC>(dx + t * a.D, nil);
+        for (int64_t t = max(t0, tl); t < t1; ++t) dx[t * a.D] = from_f32<T>(0.f);
     }
-    if (!a.part) return;
-    float* part = a.part + static_cast<int64_t>(blockIdx.y) * a.D * (W + 1);
+    f.template sums<kConvRuns>(a, c, c < a.D);
+}
+
+// ---- two channels a lane, rows through shared memory -------------------------------------------------------
+constexpr int kConvU = 16, kConvStages = 3;  // tokens a stage; stages a warp
+
+// A warp's stages of N inputs: rows of 64 channels, copied 16 bytes a lane; what lies behind `end` is not read.
+template <typename T, int N>
+struct ConvStages {
+    static constexpr int kRow = 64, kPieces = kRow * sizeof(T) / 16;  // 16-byte pieces a row
+    static constexpr size_t kBytes = static_cast<size_t>(kConvStages) * N * kConvU * kRow * sizeof(T);
+    T* mem;
+    __device__ __forceinline__ T* row(int stage, int n, int u) const { return mem + ((stage * N + n) * kConvU + u) * kRow; }
+    // src[n]: token t, the tile's first channel
+    __device__ __forceinline__ void ask(int stage, const T* const (&src)[N], const int64_t (&stride)[N], int64_t left, int width, int lane) const {
 #pragma unroll
-    for (int k = 0; k <= W; ++k)
+        for (int n = 0; n < N; ++n)
 #pragma unroll
-        for (int e = 0; e < VEC; ++e) {
-            __syncthreads();
-            comb[threadIdx.y][threadIdx.x] = k < W ? dw[k < W ? k : 0][e] : db[e];
-            __syncthreads();
-            if (threadIdx.y == 0 && col < nv) {
-                float s = comb[0][threadIdx.x];
+            for (int i = 0; i < kConvU * kPieces / 32; ++i) {
+                const int u = (i * 32 + lane) / kPieces, q = (i * 32 + lane) % kPieces * (16 / static_cast<int>(sizeof(T)));
+                if (u < left && q < width) cp_async16(row(stage, n, u) + q, src[n] + u * stride[n] + q, true);
+            }
+        cp_async_commit();
+    }
+    // the stage asked for longest ago is there (one a turn is asked for, if of nothing)
+    __device__ __forceinline__ void wait() const {
+        asm volatile("cp.async.wait_group %0;" ::"n"(kConvStages - 2) : "memory");
+        __syncwarp();
+    }
+};
+
+template <typename T, int W>
+__global__ void __launch_bounds__(32 * kConvRuns) conv_fwd_k(const ConvArgs a) {
+    using V = RowVec<T, 2>;
+    extern __shared__ __align__(16) unsigned char smem[];
+    const int lane = threadIdx.x & 31, wid = threadIdx.x >> 5, c0 = blockIdx.x * 64, c = c0 + lane * 2;
+    const ConvStages<T, 1> st{reinterpret_cast<T*>(smem + wid * ConvStages<T, 1>::kBytes)};
+    const int64_t r = static_cast<int64_t>(blockIdx.y) * kConvRuns + wid;
+    if (r >= a.rows * a.runs) return;
+    const int64_t b = r / a.runs, len = conv_length(a, b);
+    const int64_t t0 = (r - b * a.runs) * a.run, t1 = min(t0 + a.run, a.L), tl = min(t1, len);
+    const bool live = c < a.D;
+    const T* x = static_cast<const T*>(a.x) + b * a.sx[0] + c0;
+    T* y = static_cast<T*>(a.y) + b * a.L * a.D + c;
+    const T* src[1] = {x + t0 * a.sx[1]};
+    const int64_t stride[1] = {a.sx[1]};
+    int64_t asked = t0;
+    int slot = 0;
+    auto ask = [&] {
+        st.ask(slot, src, stride, tl - asked, a.D - c0, lane);
+        slot = slot + 1 == kConvStages ? 0 : slot + 1;
+        src[0] += kConvU * a.sx[1];
+        asked += kConvU;
+    };
+    for (int i = 0; i + 1 < kConvStages; ++i) ask();
+    ConvFwd<T, 2, W> f;
+    f.cols.taps(a, live ? c : 0);
+    if (t0 < tl && live) ConvCols<T, 2, W>::window(f.win, a, x + lane * 2, b, t0, c);
+    T* py = y + t0 * a.D;
+    int now = 0;
+    for (int64_t t = t0; t < tl; t += kConvU, py += kConvU * static_cast<int64_t>(a.D)) {
+        st.wait();
+        ask();
+        const T* p = st.row(now, 0, 0) + lane * 2;
+        now = now + 1 == kConvStages ? 0 : now + 1;
+        if (!live) continue;
+        if (t + kConvU <= tl) {
 #pragma unroll
-                for (int j = 1; j < R; ++j) s += comb[j][threadIdx.x];
-                part[k < W ? (c + e) * W + k : a.D * W + c + e] = s;
+            for (int u = 0; u < kConvU; ++u) f.token(*reinterpret_cast<const V*>(p + u * 64), py + u * static_cast<int64_t>(a.D), a.silu);
+        } else {
+#pragma unroll 1
+            for (int u = 0; t + u < tl; ++u) f.token(*reinterpret_cast<const V*>(p + u * 64), py + u * static_cast<int64_t>(a.D), a.silu);
+        }
+    }
+    cp_async_wait_all();
+    if (!live) return;
+    const float nil[2] = {};
+    for (int64_t t = max(t0, tl); t < t1; ++t) conv_write<T, 2>(y + t * a.D, nil);
+    if (a.hN && t0 == 0) conv_final<T, 2, W>(a, x + lane * 2, b, len, c);
+}
+
+template <typename T, int W>
+__global__ void __launch_bounds__(32 * kConvRuns) conv_bwd_k(const ConvArgs a) {
+    using V = RowVec<T, 2>;
+    extern __shared__ __align__(16) unsigned char smem[];
+    const int lane = threadIdx.x & 31, wid = threadIdx.x >> 5, c0 = blockIdx.x * 64, c = c0 + lane * 2;
+    const ConvStages<T, 2> st{reinterpret_cast<T*>(smem + wid * ConvStages<T, 2>::kBytes)};
+    const int64_t r = static_cast<int64_t>(blockIdx.y) * kConvRuns + wid;
+    const bool live = c < a.D;
+    ConvBwd<T, 2, W> f;
+    f.clear();
+    if (r < a.rows * a.runs) {
+        const int64_t b = r / a.runs, len = conv_length(a, b);
+        const int64_t t0 = (r - b * a.runs) * a.run, t1 = min(t0 + a.run, a.L), tl = min(t1, len);
+        const T* x = static_cast<const T*>(a.x) + b * a.sx[0] + c0;
+        const T* dy = static_cast<const T*>(a.dy) + b * a.sdy[0] + c0;
+        T* dx = static_cast<T*>(a.dx) + b * a.L * a.D + c;
+        const int64_t stop = t0 < len || t0 == 0 ? tl + W - 1 : t0;
+        const T* src[2] = {x + t0 * a.sx[1], dy + t0 * a.sdy[1]};
+        const int64_t stride[2] = {a.sx[1], a.sdy[1]};
+        int64_t asked = t0;
+        int slot = 0;
+        auto ask = [&] {
+            st.ask(slot, src, stride, min(stop, len) - asked, a.D - c0, lane);
+            slot = slot + 1 == kConvStages ? 0 : slot + 1;
+            src[0] += kConvU * a.sx[1];
+            src[1] += kConvU * a.sdy[1];
+            asked += kConvU;
+        };
+        for (int i = 0; i + 1 < kConvStages; ++i) ask();
+        f.cols.taps(a, live ? c : 0);
+        if (t0 < tl && live) ConvCols<T, 2, W>::window(f.win, a, x + lane * 2, b, t0, c);
+        T* pd = dx + (t0 - (W - 1)) * a.D;
+        int now = 0;
+        for (int64_t t = t0; t < stop; t += kConvU, pd += kConvU * static_cast<int64_t>(a.D)) {
+            st.wait();
+            ask();
+            const T *px = st.row(now, 0, 0) + lane * 2, *pg = st.row(now, 1, 0) + lane * 2;
+            now = now + 1 == kConvStages ? 0 : now + 1;
+            if (!live) continue;
+            // inside the run every token is its own and completes an input of the run, none of which is in the final state
+            if (t > t0 && t + kConvU <= tl) {
+#pragma unroll 8
+                for (int u = 0; u < kConvU; ++u) {
+                    f.shift();
+                    f.token(*reinterpret_cast<const V*>(px + u * 64), *reinterpret_cast<const V*>(pg + u * 64), true, a.silu);
+                    float g[2];
+                    f.gradient(g);
+                    conv_write<T, 2>(pd + u * static_cast<int64_t>(a.D), g);
+                }
+            } else {
+#pragma unroll 1
+                for (int u = 0; u < kConvU && t + u < stop; ++u)
+                    f.any(a, dx, *reinterpret_cast<const V*>(px + u * 64), *reinterpret_cast<const V*>(pg + u * 64), b, c, t + u, t0, tl, len);
             }
         }
+        cp_async_wait_all();
+        const float nil[2] = {};
+        if (live)
+            for (int64_t t = max(t0, tl); t < t1; ++t) conv_write<T, 2>(dx + t * a.D, nil);
+    }
+    f.template sums<kConvRuns>(a, c, live);
 }
 
 template <typename T, int VEC, int W>
@@ -305,11 +490,14 @@ __global__ void __launch_bounds__(128) conv_step_k(const ConvArgs a) {
     raw[W - 1] = *reinterpret_cast<const RowVec<T, VEC>*>(static_cast<const T*>(a.x) + b * a.sx[0] + c);
     ConvCols<T, VEC, W> cols;
     cols.taps(a, c);
-    float win[W][VEC], p[VEC];
+    ConvVal<VEC> win[W];
+    float p[VEC];
 #pragma unroll
-    for (int k = 0; k < W; ++k)
+    for (int k = 0; k < W; ++k) {
 #pragma unroll
-        for (int e = 0; e < VEC; ++e) win[k][e] = to_f32(raw[k].e[e]);
+        for (int e = 0; e < VEC; ++e) p[e] = to_f32(raw[k].e[e]);
+        win[k].set(p);
+    }
     cols.dot(p, win);
     if (a.silu)
 #pragma unroll
@@ -320,34 +508,51 @@ __global__ void __launch_bounds__(128) conv_step_k(const ConvArgs a) {
 }
 
 // ---------------------------------------------------------------------------------------------------------
-constexpr int kConvBwdRuns = 4;  // runs a CTA of the backward
-
-// Runs that fill `threads` threads a multiprocessor once with `cols` columns a run; none shorter than 8 tokens.
-void conv_runs(ConvArgs& a, int64_t cols, int threads) {
-    const int64_t want = std::max<int64_t>(1, int64_t{148} * threads / (cols * std::max<int64_t>(a.rows, 1)));
-    a.run = std::max<int64_t>(8, (a.L + want - 1) / want);
+// Runs that give every multiprocessor its `warps` once, with `tiles` warps side by side a run; whole stages.
+void conv_runs(ConvArgs& a, int64_t tiles, int warps) {
+    const int64_t want = std::max<int64_t>(1, int64_t{148} * warps / (tiles * std::max<int64_t>(a.rows, 1)));
+    a.run = ((a.L + want - 1) / want + kConvU - 1) / kConvU * kConvU;
+    a.run = std::max<int64_t>(a.run, kConvU);
     a.runs = static_cast<int>(std::max<int64_t>(1, (a.L + a.run - 1) / a.run));
 }
-int64_t conv_bwd_cols(int64_t D, int vec) { return ((D + vec - 1) / vec + 31) / 32 * 32; }
-int conv_bwd_vec(bool vec) { return vec ? 4 : 1; }
-int64_t conv_bwd_rows(const ConvArgs& a) { return (a.rows * a.runs + kConvBwdRuns - 1) / kConvBwdRuns; }
+// The backward's: warps that are resident whatever the kernel, as its number of partial rows is part of the workspace.
+constexpr int kConvBwdWarps = 16;
+int64_t conv_bwd_rows(ConvArgs& a, bool staged) {
+    conv_runs(a, (a.D + (staged ? 63 : 31)) / (staged ? 64 : 32), kConvBwdWarps);
+    return (a.rows * a.runs + kConvRuns - 1) / kConvRuns;
+}
+dim3 conv_grid(const ConvArgs& a, int cols) {
+    return dim3((a.D + cols - 1) / cols, static_cast<unsigned>((a.rows * a.runs + kConvRuns - 1) / kConvRuns));
+}
 
-template <typename T, int VEC, int W>
-cudaError_t conv_fwd_launch(ConvArgs& a, cudaStream_t s) {
-    constexpr int U = VEC > 1 ? 8 : 16;
-    static const int per = row_resident(conv_fwd_k<T, VEC, W, U>, 128, 0);
-    const int64_t nv = a.D / VEC;
-    conv_runs(a, nv, per * 128);
-    const int64_t n = a.rows * a.runs * nv;
-    conv_fwd_k<T, VEC, W, U><<<static_cast<unsigned>((n + 127) / 128), 128, 0, s>>>(a);
+template <typename T, int W>
+cudaError_t conv_fwd_launch(ConvArgs& a, bool staged, cudaStream_t s) {
+    constexpr int threads = 32 * kConvRuns;
+    if (staged) {
+        constexpr size_t smem = kConvRuns * ConvStages<T, 1>::kBytes;
+        static const int per = row_resident(conv_fwd_k<T, W>, threads, smem);
+        conv_runs(a, (a.D + 63) / 64, per * kConvRuns);
+        conv_fwd_k<T, W><<<conv_grid(a, 64), threads, smem, s>>>(a);
+    } else {
+        static const int per = row_resident(conv_fwd_any_k<T, W, 8>, threads, 0);
+        conv_runs(a, (a.D + 31) / 32, per * kConvRuns);
+        conv_fwd_any_k<T, W, 8><<<conv_grid(a, 32), threads, 0, s>>>(a);
+    }
     note_launch();
     return cudaGetLastError();
 }
-template <typename T, int VEC, int W>
-cudaError_t conv_bwd_launch(ConvArgs& a, void* dweight, void* dbias, cudaStream_t s) {
-    constexpr int R = kConvBwdRuns;
-    const int64_t nv = a.D / VEC, rows = conv_bwd_rows(a);
-    conv_bwd_k<T, VEC, W, R, 4><<<dim3(static_cast<unsigned>((nv + 31) / 32), static_cast<unsigned>(rows)), dim3(32, R), 0, s>>>(a);
+template <typename T, int W>
+cudaError_t conv_bwd_launch(ConvArgs& a, bool staged, void* dweight, void* dbias, cudaStream_t s) {
+    constexpr int threads = 32 * kConvRuns;
+    const int64_t rows = conv_bwd_rows(a, staged);
+    if (staged) {
+        constexpr size_t smem = kConvRuns * ConvStages<T, 2>::kBytes;
+        const cudaError_t e = cudaFuncSetAttribute(conv_bwd_k<T, W>, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
+        if (e != cudaSuccess) return e;
+        conv_bwd_k<T, W><<<conv_grid(a, 64), threads, smem, s>>>(a);
+    } else {
+        conv_bwd_any_k<T, W, 4><<<conv_grid(a, 32), threads, 0, s>>>(a);
+    }
     note_launch();
     cudaError_t e = cudaGetLastError();
     if (e != cudaSuccess || !a.part) return e;
@@ -364,22 +569,23 @@ cudaError_t conv_step_launch(ConvArgs& a, cudaStream_t s) {
     return cudaGetLastError();
 }
 
-#define EACS_CONV_W(T, VEC, F, ...)             \
-    (width == 2   ? F<T, VEC, 2>(__VA_ARGS__)   \
-     : width == 3 ? F<T, VEC, 3>(__VA_ARGS__)   \
-                  : F<T, VEC, 4>(__VA_ARGS__))
-
 template <typename T>
-cudaError_t conv_fwd_any(ConvArgs& a, int width, bool vec, cudaStream_t s) {
-    return vec ? EACS_CONV_W(T, 4, conv_fwd_launch, a, s) : EACS_CONV_W(T, 1, conv_fwd_launch, a, s);
+cudaError_t conv_fwd_any(ConvArgs& a, int width, bool staged, cudaStream_t s) {
+    return width == 2 ? conv_fwd_launch<T, 2>(a, staged, s) : width == 3 ? conv_fwd_launch<T, 3>(a, staged, s) : conv_fwd_launch<T, 4>(a, staged, s);
+}
+template <typename T, int VEC>
+cudaError_t conv_step_width(ConvArgs& a, int width, cudaStream_t s) {
+    return width == 2 ? conv_step_launch<T, VEC, 2>(a, s) : width == 3 ? conv_step_launch<T, VEC, 3>(a, s) : conv_step_launch<T, VEC, 4>(a, s);
 }
 template <typename T>
 cudaError_t conv_step_any(ConvArgs& a, int width, bool vec, cudaStream_t s) {
-    return vec ? EACS_CONV_W(T, 4, conv_step_launch, a, s) : EACS_CONV_W(T, 1, conv_step_launch, a, s);
+    return vec ? conv_step_width<T, 4>(a, width, s) : conv_step_width<T, 1>(a, width, s);
 }
 template <typename T>
-cudaError_t conv_bwd_any(ConvArgs& a, int width, bool vec, void* dw, void* db, cudaStream_t s) {
-    return vec ? EACS_CONV_W(T, 4, conv_bwd_launch, a, dw, db, s) : EACS_CONV_W(T, 1, conv_bwd_launch, a, dw, db, s);
+cudaError_t conv_bwd_any(ConvArgs& a, int width, bool staged, void* dw, void* db, cudaStream_t s) {
+    return width == 2   ? conv_bwd_launch<T, 2>(a, staged, dw, db, s)
+           : width == 3 ? conv_bwd_launch<T, 3>(a, staged, dw, db, s)
+                        : conv_bwd_launch<T, 4>(a, staged, dw, db, s);
 }
 
 int conv_check(const char* fn, const EacsConv& p, bool single) {
@@ -400,6 +606,7 @@ ConvArgs conv_args(const EacsConv& p) {
     a.rows = p.rows, a.L = p.L, a.D = static_cast<int>(p.D), a.w_dtype = p.w_dtype, a.silu = p.silu;
     return a;
 }
+int conv_piece(const EacsConv& p) { return p.dtype == EACS_DTYPE_F32 ? 4 : 8; }  // elements of 16 bytes
 // Whether vectors of `n` elements may be moved at p and its strides (D of them a row).
 bool conv_vec(const EacsConv& p, int n, std::initializer_list<const void*> ptrs, std::initializer_list<int64_t> strides) {
     const uintptr_t bytes = static_cast<uintptr_t>(n) * (p.dtype == EACS_DTYPE_F32 ? 4 : 2);
@@ -413,15 +620,11 @@ bool conv_vec(const EacsConv& p, int n, std::initializer_list<const void*> ptrs,
 
 }  // namespace
 
-// The partial rows of a backward, for vectors or single elements, whichever has more.
+// The partial rows of a backward, whichever of its kernels has more.
 size_t conv_bwd_workspace_size(const EacsConv& p) {
     if (conv_check("eacs_conv_bwd_workspace_size", p, false) != EACS_OK || p.rows == 0) return 0;
     ConvArgs a = conv_args(p);
-    int64_t rows = 0;
-    for (int vec : {1, 4}) {
-        conv_runs(a, conv_bwd_cols(p.D, vec), 512);
-        rows = std::max(rows, conv_bwd_rows(a));
-    }
+    const int64_t rows = std::max(conv_bwd_rows(a, false), conv_bwd_rows(a, true));
     return static_cast<size_t>(rows) * p.D * (p.width + 1) * sizeof(float);
 }
 
@@ -434,7 +637,7 @@ int conv_fwd(const EacsConv& p, void* y, void* final_state, cudaStream_t stream)
     a.y = y;
     a.hN = final_state;
     if (p.L == 0 && !final_state) return EACS_OK;
-    const bool vec = conv_vec(p, 4, {p.x, y, p.initial_state, final_state}, {p.x_stride[0], p.x_stride[1]});
+    const bool vec = conv_vec(p, conv_piece(p), {p.x, y, p.initial_state, final_state}, {p.x_stride[0], p.x_stride[1]});
     const cudaError_t e = p.dtype == EACS_DTYPE_F32   ? conv_fwd_any<float>(a, p.width, vec, stream)
                           : p.dtype == EACS_DTYPE_F16 ? conv_fwd_any<__half>(a, p.width, vec, stream)
                                                       : conv_fwd_any<__nv_bfloat16>(a, p.width, vec, stream);
@@ -475,9 +678,8 @@ int conv_bwd(const EacsConv& p, const ConvGrads& g, void* ws, size_t ws_bytes, c
     a.dy = g.dy, a.dhN = g.dfinal, a.dx = g.dx, a.dh0 = g.dinitial;
     a.sdy[0] = g.dy_stride[0], a.sdy[1] = g.dy_stride[1];
     a.part = want ? static_cast<float*>(ws) : nullptr;
-    const bool vec = conv_vec(p, 4, {p.x, p.initial_state, g.dy, g.dfinal, g.dx, g.dinitial},
+    const bool vec = conv_vec(p, conv_piece(p), {p.x, p.initial_state, g.dy, g.dfinal, g.dx, g.dinitial},
                               {p.x_stride[0], p.x_stride[1], g.dy_stride[0], g.dy_stride[1]});
-    conv_runs(a, conv_bwd_cols(p.D, conv_bwd_vec(vec)), 512);
     const cudaError_t e = p.dtype == EACS_DTYPE_F32   ? conv_bwd_any<float>(a, p.width, vec, g.dweight, g.dbias, stream)
                           : p.dtype == EACS_DTYPE_F16 ? conv_bwd_any<__half>(a, p.width, vec, g.dweight, g.dbias, stream)
                                                       : conv_bwd_any<__nv_bfloat16>(a, p.width, vec, g.dweight, g.dbias, stream);
