@@ -37,42 +37,62 @@ struct BnArgs {
 
 __device__ __forceinline__ float bn_sigmoid(float v) { return __fdividef(1.0f, 1.0f + ex2_approx(v * -1.44269504f)); }
 
-// One row of an input: VPL vectors a thread, as they lie in memory.
+// One row of an input: VPL vectors a thread, as they lie in memory (whole registers), taken apart where they are used.
 template <typename T, int VEC, int VPL, int TPR>
 struct BnRow {
-    RowVec<T, VEC> raw[VPL];
+    static constexpr int kPer = VEC > 1 ? 4 / sizeof(T) : 1, kWords = VEC / kPer;  // elements a word; words a vector
+    uint32_t raw[VPL][kWords];
+    __device__ __forceinline__ void load(int k, const void* p) {
+        if constexpr (VEC > 1) {
+            const uint4 q = *static_cast<const uint4*>(p);
+            raw[k][0] = q.x, raw[k][1] = q.y, raw[k][2] = q.z, raw[k][3] = q.w;
+        } else if constexpr (sizeof(T) == 4) {
+            raw[k][0] = *static_cast<const uint32_t*>(p);
+        } else {
+            raw[k][0] = *static_cast<const uint16_t*>(p);
+        }
+    }
+    __device__ __forceinline__ void zero(int k) {
+#pragma unroll
+        for (int i = 0; i < kWords; ++i) raw[k][i] = 0;
+    }
     __device__ __forceinline__ void read(const T* p, int d, int t) {
 #pragma unroll
         for (int k = 0; k < VPL; ++k) {
             const int i0 = (k * TPR + t) * VEC;
-            if (i0 < d) {
-                raw[k] = *reinterpret_cast<const RowVec<T, VEC>*>(p + i0);
-            } else {
-#pragma unroll
-                for (int e = 0; e < VEC; ++e) raw[k].e[e] = from_f32<T>(0.f);
-            }
+            if (i0 < d) load(k, p + i0);
+            else zero(k);
         }
     }
     __device__ __forceinline__ void zero() {
 #pragma unroll
-        for (int k = 0; k < VPL; ++k)
-#pragma unroll
-            for (int e = 0; e < VEC; ++e) raw[k].e[e] = from_f32<T>(0.f);
+        for (int k = 0; k < VPL; ++k) zero(k);
     }
-    __device__ __forceinline__ float at(int k, int e) const { return to_f32(raw[k].e[e]); }
+    __device__ __forceinline__ float at(int k, int e) const {
+        float a, b;
+        unpack<T>(raw[k][e / kPer], a, b);
+        return e % kPer ? b : a;
+    }
 };
 template <typename T, int VEC>
 __device__ __forceinline__ void bn_write(T* p, const float* v) {
-    RowVec<T, VEC> o;
+    if constexpr (VEC > 1) {
+        constexpr int per = 4 / sizeof(T);
+        uint32_t w[4];
 #pragma unroll
-    for (int e = 0; e < VEC; ++e) o.e[e] = from_f32<T>(v[e]);
-    *reinterpret_cast<RowVec<T, VEC>*>(p) = o;
+        for (int i = 0; i < 4; ++i) w[i] = pack<T>(v[i * per], v[i * per + per - 1]);
+        *reinterpret_cast<uint4*>(p) = make_uint4(w[0], w[1], w[2], w[3]);
+    } else {
+        p[0] = from_f32<T>(v[0]);
+    }
 }
 
 // CTAs of RPC groups of TPR threads; a group takes every (grid RPC)th row.  Groups smaller than a warp go through their
 // rows together (their sums are the warp's shuffles): a group without a row reads and writes nothing.
-template <typename T, int VEC, int VPL, int TPR, int RPC, bool RES>
+// HOW: what there is of gate (1) and post norm (2); 4: the arguments say (rows read element by element).
+template <typename T, int VEC, int VPL, int TPR, int RPC, bool RES, int HOW>
 __global__ void __launch_bounds__(TPR * RPC) bn_fwd_k(const BnArgs a) {
+    const bool gated = HOW == 4 ? a.gate != nullptr : (HOW & 1) != 0, normed = HOW == 4 ? a.has_post != 0 : (HOW & 2) != 0;
     using Row = BnRow<T, VEC, VPL, TPR>;
     using Par = RowParam<VEC, VPL, TPR>;
     __shared__ float reds[RPC][2 * (TPR / 32) + 1];
@@ -85,7 +105,7 @@ __global__ void __launch_bounds__(TPR * RPC) bn_fwd_k(const BnArgs a) {
         w.fill(sw, a.weight, a.w_dtype, a.d, 1.f);
         scale.fill(sc, a.scale, a.w_dtype, a.d, 1.f);
     }
-    if (a.has_post) post.fill(sp, a.post, a.w_dtype, a.d, 1.f);
+    if (normed) post.fill(sp, a.post, a.w_dtype, a.d, 1.f);
     __syncthreads();
     const float inv = 1.0f / static_cast<float>(a.d);
     const int64_t step = static_cast<int64_t>(gridDim.x) * RPC;
@@ -95,14 +115,14 @@ __global__ void __launch_bounds__(TPR * RPC) bn_fwd_k(const BnArgs a) {
         const int dl = live ? a.d : 0;
         Row x, g, r;
         x.read(static_cast<const T*>(a.x) + row * a.sx, dl, t);
-        if (a.gate) g.read(static_cast<const T*>(a.gate) + row * a.sg, dl, t);
+        if (gated) g.read(static_cast<const T*>(a.gate) + row * a.sg, dl, t);
         if constexpr (RES) r.read(static_cast<const T*>(a.res) + row * a.sr, dl, t);
         float u[VPL][VEC];
 #pragma unroll
         for (int k = 0; k < VPL; ++k)
 #pragma unroll
             for (int e = 0; e < VEC; ++e) u[k][e] = x.at(k, e);
-        if (a.has_post) {
+        if (normed) {
             float sq = 0.f;
 #pragma unroll
             for (int k = 0; k < VPL; ++k)
@@ -117,7 +137,7 @@ __global__ void __launch_bounds__(TPR * RPC) bn_fwd_k(const BnArgs a) {
                 for (int e = 0; e < VEC; ++e) u[k][e] = u[k][e] * rs * p[e];
             }
         }
-        if (a.gate)
+        if (gated)
 #pragma unroll
             for (int k = 0; k < VPL; ++k)
 #pragma unroll
@@ -161,6 +181,27 @@ __global__ void __launch_bounds__(TPR * RPC) bn_fwd_k(const BnArgs a) {
     }
 }
 
+// The backward's inputs of a thread's next row on their way to shared memory (its own 16-byte vectors, so without a
+// barrier) while it works on this one: 18 warps that each waited for their row left memory idle (199 us of 65536 rows of
+// 768 with a scale; what it takes now stands at bn_bwd_launch).
+template <int VEC, int VPL, int TPR, int RPC, bool RES, int HOW>
+struct BnStage {
+    static constexpr int kInputs = 2 + (HOW & 1) + (RES ? 2 : 0);
+    static constexpr size_t kTwo = static_cast<size_t>(2) * kInputs * VPL * TPR * RPC * 16;
+    static constexpr bool on = VEC > 1 && kTwo <= 168 * 1024;  // (float32 rows above 4096 values are read as they are needed)
+    static constexpr size_t bytes = on ? kTwo : 0;
+    unsigned char* mem;
+    __device__ __forceinline__ unsigned char* at(int stage, int input, int k) const {
+        return mem + (((stage * kInputs + input) * VPL + k) * static_cast<size_t>(TPR * RPC) + threadIdx.x) * 16;
+    }
+};
+
+// CTAs a multiprocessor that a backward keeps registers for: 18 warps or more without gate and post norm, else 12 to 16.
+constexpr int bn_bwd_min(int threads, int how) {
+    const int n = (how == 0 ? 640 : 512) / threads;
+    return n < 1 ? 1 : n;
+}
+
 // Two sums over a row's threads at once.
 template <int TPR>
 __device__ __forceinline__ void row_sum2(float& p, float& q, float* red, int& slot) {
@@ -181,8 +222,9 @@ __device__ __forceinline__ void row_sum2(float& p, float& q, float* red, int& sl
     }
 }
 
-template <typename T, int VEC, int VPL, int TPR, int RPC, bool RES>
-__global__ void __launch_bounds__(TPR * RPC) bn_bwd_k(const BnArgs a) {
+template <typename T, int VEC, int VPL, int TPR, int RPC, bool RES, int HOW>
+__global__ void __launch_bounds__(TPR * RPC, bn_bwd_min(TPR * RPC, HOW)) bn_bwd_k(const BnArgs a) {
+    const bool gated = HOW == 4 ? a.gate != nullptr : (HOW & 1) != 0, normed = HOW == 4 ? a.has_post != 0 : (HOW & 2) != 0;
     using Row = BnRow<T, VEC, VPL, TPR>;
     using Par = RowParam<VEC, VPL, TPR>;
     __shared__ __align__(8) float reds[RPC][4 * (TPR / 32) + 2];
@@ -196,27 +238,69 @@ __global__ void __launch_bounds__(TPR * RPC) bn_bwd_k(const BnArgs a) {
         w.fill(sw, a.weight, a.w_dtype, a.d, 1.f);
         scale.fill(sc, a.scale, a.w_dtype, a.d, 1.f);
     }
-    if (a.has_post) post.fill(sp, a.post, a.w_dtype, a.d, 1.f);
+    if (normed) post.fill(sp, a.post, a.w_dtype, a.d, 1.f);
     __syncthreads();
     float dw[RES ? VPL : 1][VEC] = {}, dc[RES ? VPL : 1][VEC] = {}, dp[VPL][VEC] = {};
     const float inv = 1.0f / static_cast<float>(a.d);
     const int64_t step = static_cast<int64_t>(gridDim.x) * RPC;
-    for (int64_t row = static_cast<int64_t>(blockIdx.x) * RPC + grp;; row += step) {
+    extern __shared__ __align__(16) unsigned char stage_mem[];
+    using Stage = BnStage<VEC, VPL, TPR, RPC, RES, HOW>;
+    const Stage st{stage_mem};
+    // the inputs in order: x, dy, residual, ds, gate
+    auto input = [&](int i, int64_t row) -> const T* {
+        if (i == 0) return static_cast<const T*>(a.x) + row * a.sx;
+        if (i == 1) return a.dy ? static_cast<const T*>(a.dy) + row * a.sdy : nullptr;
+        if (RES && i == 2) return static_cast<const T*>(a.res) + row * a.sr;
+        if (RES && i == 3) return a.ds ? static_cast<const T*>(a.ds) + row * a.sds : nullptr;
+        return static_cast<const T*>(a.gate) + row * a.sg;
+    };
+    auto fetch = [&](int stage, int64_t row) {
+        if constexpr (Stage::on) {
+            if (row < a.rows)
+#pragma unroll
+                for (int i = 0; i < Stage::kInputs; ++i) {
+                    const T* p = input(i, row);
+#pragma unroll
+                    for (int k = 0; k < VPL; ++k) {
+                        const int i0 = (k * TPR + t) * VEC;
+                        if (p && i0 < a.d) row_cp16(st.at(stage, i, k), p + i0);
+                    }
+                }
+            cp_async_commit();
+        }
+    };
+    int stage = 0;
+    int64_t row = static_cast<int64_t>(blockIdx.x) * RPC + grp;
+    fetch(0, row);
+    for (;; row += step, stage ^= 1) {
         const bool live = row < a.rows;
         if (TPR < 32 ? !__any_sync(0xffffffffu, live) : !live) break;
         const int dl = live ? a.d : 0;
         Row x, g, r, gy, gs;
-        x.read(static_cast<const T*>(a.x) + row * a.sx, dl, t);
-        if (a.gate) g.read(static_cast<const T*>(a.gate) + row * a.sg, dl, t);
-        if constexpr (RES) r.read(static_cast<const T*>(a.res) + row * a.sr, dl, t);
-        if (a.dy) gy.read(static_cast<const T*>(a.dy) + row * a.sdy, dl, t);
-        else gy.zero();
-        if constexpr (RES) {
-            if (a.ds) gs.read(static_cast<const T*>(a.ds) + row * a.sds, dl, t);
-            else gs.zero();
+        if constexpr (Stage::on) {
+            fetch(stage ^ 1, row + step);
+            asm volatile("cp.async.wait_group 1;" ::: "memory");
         }
+        auto take = [&](Row& to, int i) {
+            const T* p = input(i, row);
+            if constexpr (Stage::on) {
+#pragma unroll
+                for (int k = 0; k < VPL; ++k) {
+                    if (p && (k * TPR + t) * VEC < dl) to.load(k, st.at(stage, i, k));
+                    else to.zero(k);
+                }
+            } else if (p) {
+                to.read(p, dl, t);
+            } else {
+                to.zero();
+            }
+        };
+        take(x, 0);
+        take(gy, 1);
+        if constexpr (RES) take(r, 2), take(gs, 3);
+        if (gated) take(g, RES ? 4 : 2);
         float r1 = 1.f;
-        if (a.has_post) {
+        if (normed) {
             float sq = 0.f, none = 0.f;
 #pragma unroll
             for (int k = 0; k < VPL; ++k)
@@ -226,9 +310,9 @@ __global__ void __launch_bounds__(TPR * RPC) bn_bwd_k(const BnArgs a) {
             r1 = 1.0f / sqrtf(sq * inv + a.eps);
         }
         // v: the gradient of u; before: u before the gate
-        auto before = [&](int k, int e, const float* p) { return a.has_post ? x.at(k, e) * r1 * p[e] : x.at(k, e); };
+        auto before = [&](int k, int e, const float* p) { return normed ? x.at(k, e) * r1 * p[e] : x.at(k, e); };
         auto gain = [&](int k, int e) {
-            if (!a.gate) return 1.f;
+            if (!gated) return 1.f;
             const float q = g.at(k, e);
             return q * bn_sigmoid(q);
         };
@@ -240,7 +324,7 @@ __global__ void __launch_bounds__(TPR * RPC) bn_bwd_k(const BnArgs a) {
                 float c[VEC], p[VEC], q[VEC];
                 scale.get(c, k, t);
                 w.get(q, k, t);
-                if (a.has_post) post.get(p, k, t);
+                if (normed) post.get(p, k, t);
 #pragma unroll
                 for (int e = 0; e < VEC; ++e) {
                     s[k][e] = fmaf(c[e], before(k, e, p) * gain(k, e), r.at(k, e));
@@ -256,7 +340,7 @@ __global__ void __launch_bounds__(TPR * RPC) bn_bwd_k(const BnArgs a) {
                 float c[VEC], p[VEC], q[VEC], o[VEC];
                 scale.get(c, k, t);
                 w.get(q, k, t);
-                if (a.has_post) post.get(p, k, t);
+                if (normed) post.get(p, k, t);
 #pragma unroll
                 for (int e = 0; e < VEC; ++e) {
                     const float dyv = gy.at(k, e);
@@ -273,12 +357,12 @@ __global__ void __launch_bounds__(TPR * RPC) bn_bwd_k(const BnArgs a) {
 #pragma unroll
                 for (int e = 0; e < VEC; ++e) v[k][e] = gy.at(k, e);
         }
-        if (a.gate)
+        if (gated)
 #pragma unroll
             for (int k = 0; k < VPL; ++k) {
                 const int i0 = (k * TPR + t) * VEC;
                 float p[VEC], o[VEC];
-                if (a.has_post) post.get(p, k, t);
+                if (normed) post.get(p, k, t);
 #pragma unroll
                 for (int e = 0; e < VEC; ++e) {
                     const float q = g.at(k, e), sg = bn_sigmoid(q);
@@ -287,7 +371,7 @@ __global__ void __launch_bounds__(TPR * RPC) bn_bwd_k(const BnArgs a) {
                 }
                 if (i0 < dl) bn_write<T, VEC>(static_cast<T*>(a.dgate) + row * a.d + i0, o);
             }
-        if (a.has_post) {
+        if (normed) {
             float sm = 0.f, none = 0.f;
 #pragma unroll
             for (int k = 0; k < VPL; ++k) {
@@ -318,7 +402,7 @@ __global__ void __launch_bounds__(TPR * RPC) bn_bwd_k(const BnArgs a) {
     float* part = a.part + static_cast<int64_t>(blockIdx.x) * 3 * a.d;
 #pragma unroll
     for (int which = RES ? 0 : 2; which < 3; ++which) {
-        if (which == 2 && !a.has_post) break;
+        if (which == 2 && !normed) break;
         float(*acc)[VEC] = which == 0 ? dw : which == 1 ? dc : dp;
         if constexpr (RPC > 1) {  // the CTA's groups one after another (a fixed order)
             for (int gi = 0; gi < RPC; ++gi) {
@@ -353,69 +437,84 @@ __global__ void __launch_bounds__(TPR * RPC) bn_bwd_k(const BnArgs a) {
 constexpr int kBnBwdCtas = 4;  // a backward's CTAs an SM at most: also its partial rows
 constexpr int kBnMaxParts = 148 * kBnBwdCtas;
 
-template <typename T, int VEC, int VPL, int TPR, int RPC, bool RES>
+template <typename T, int VEC, int VPL, int TPR, int RPC, bool RES, int HOW>
 cudaError_t bn_fwd_launch(const BnArgs& a, cudaStream_t s) {
-    static const int per = row_resident(bn_fwd_k<T, VEC, VPL, TPR, RPC, RES>, TPR * RPC, 0);
-    bn_fwd_k<T, VEC, VPL, TPR, RPC, RES><<<row_grid(a.rows, RPC, per), TPR * RPC, 0, s>>>(a);
+    const auto k = bn_fwd_k<T, VEC, VPL, TPR, RPC, RES, HOW>;
+    static const int per = row_resident(k, TPR * RPC, 0);
+    k<<<row_grid(a.rows, RPC, per), TPR * RPC, 0, s>>>(a);
     note_launch();
     return cudaGetLastError();
 }
-template <typename T, int VEC, int VPL, int TPR, int RPC, bool RES>
+template <typename T, int VEC, int VPL, int TPR, int RPC, bool RES, int HOW>
 cudaError_t bn_bwd_launch(const BnArgs& a, int* parts, cudaStream_t s) {
-    static const int per = std::min(row_resident(bn_bwd_k<T, VEC, VPL, TPR, RPC, RES>, TPR * RPC, 0), kBnBwdCtas);
+    const auto k = bn_bwd_k<T, VEC, VPL, TPR, RPC, RES, HOW>;
+    constexpr size_t smem = BnStage<VEC, VPL, TPR, RPC, RES, HOW>::bytes;
+    const cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
+    if (e != cudaSuccess) return e;
+    static const int per = std::min(row_resident(k, TPR * RPC, smem), kBnBwdCtas);
     *parts = row_grid(a.rows, RPC, per);
-    bn_bwd_k<T, VEC, VPL, TPR, RPC, RES><<<*parts, TPR * RPC, 0, s>>>(a);
+    k<<<*parts, TPR * RPC, smem, s>>>(a);
     note_launch();
     return cudaGetLastError();
 }
 
 // As few threads a row as hold it: forward up to four vectors a thread, backward (with three sums a column) up to two.
 // Rows whose start or length is not a multiple of 16 bytes are read element by element.
-template <typename T, bool RES>
-cudaError_t bn_fwd_any(const BnArgs& a, bool vec, cudaStream_t s) {
+template <typename T, bool RES, int HOW>
+cudaError_t bn_fwd_vec(const BnArgs& a, cudaStream_t s) {
     constexpr int E = 16 / sizeof(T);
-#define EACS_BN(VEC, VPL, TPR, RPC) return bn_fwd_launch<T, VEC, VPL, TPR, RPC, RES>(a, s)
+#define EACS_BN(VPL, TPR, RPC) return bn_fwd_launch<T, E, VPL, TPR, RPC, RES, HOW>(a, s)
     const int n = (a.d + E - 1) / E;
-    if (vec) {
-        if (n <= 8) EACS_BN(E, 1, 8, 32);
-        if (n <= 16) EACS_BN(E, 1, 16, 16);
-        if (n <= 32) EACS_BN(E, 1, 32, 8);
-        if (n <= 64) EACS_BN(E, 2, 32, 8);
-        if (n <= 96) EACS_BN(E, 3, 32, 8);
-        if (n <= 128) EACS_BN(E, 4, 32, 8);
-        if (n <= 256) EACS_BN(E, 2, 128, 2);
-        if (n <= 512) EACS_BN(E, 1, 512, 1);
-        if (n <= 1024) EACS_BN(E, 2, 512, 1);
-        if constexpr (E == 4) EACS_BN(E, 4, 512, 1);  // (16-bit rows of 8192 values have 1024 vectors)
-    }
-    if (a.d <= 256) EACS_BN(1, 8, 32, 8);
-    if (a.d <= 1024) EACS_BN(1, 8, 128, 2);
-    if (a.d <= 4096) EACS_BN(1, 8, 512, 1);
-    EACS_BN(1, 16, 512, 1);
+    if (n <= 8) EACS_BN(1, 8, 32);
+    if (n <= 16) EACS_BN(1, 16, 16);
+    if (n <= 32) EACS_BN(1, 32, 8);
+    if (n <= 64) EACS_BN(2, 32, 8);
+    if (n <= 96) EACS_BN(3, 32, 8);
+    if (n <= 128) EACS_BN(4, 32, 8);
+    if (n <= 256) EACS_BN(2, 128, 2);
+    if (n <= 512) EACS_BN(1, 512, 1);
+    if (n <= 1024) EACS_BN(2, 512, 1);
+    if constexpr (E == 4) EACS_BN(4, 512, 1);  // (16-bit rows of 8192 values have 1024 vectors)
+    return cudaErrorInvalidValue;
+#undef EACS_BN
+}
+template <typename T, bool RES, int HOW>
+cudaError_t bn_bwd_vec(const BnArgs& a, int* parts, cudaStream_t s) {
+    constexpr int E = 16 / sizeof(T);
+#define EACS_BN(VPL, TPR, RPC) return bn_bwd_launch<T, E, VPL, TPR, RPC, RES, HOW>(a, parts, s)
+    const int n = (a.d + E - 1) / E;
+    if (n <= 8) EACS_BN(1, 8, 32);
+    if (n <= 16) EACS_BN(1, 16, 16);
+    if (n <= 32) EACS_BN(1, 32, 8);
+    if (n <= 64) EACS_BN(1, 64, 4);
+    if (n <= 96) EACS_BN(1, 96, 2);
+    if (n <= 128) EACS_BN(1, 128, 2);
+    if (n <= 256) EACS_BN(1, 256, 1);
+    if (n <= 512) EACS_BN(1, 512, 1);
+    if (n <= 1024) EACS_BN(2, 512, 1);
+    if constexpr (E == 4) EACS_BN(4, 512, 1);
+    return cudaErrorInvalidValue;
 #undef EACS_BN
 }
 template <typename T, bool RES>
+cudaError_t bn_fwd_any(const BnArgs& a, bool vec, cudaStream_t s) {
+    if constexpr (RES)
+        if (vec && !a.has_post) return a.gate ? bn_fwd_vec<T, RES, 1>(a, s) : bn_fwd_vec<T, RES, 0>(a, s);
+    if (vec) return a.gate ? bn_fwd_vec<T, RES, 3>(a, s) : bn_fwd_vec<T, RES, 2>(a, s);
+    if (a.d <= 256) return bn_fwd_launch<T, 1, 8, 32, 8, RES, 4>(a, s);
+    if (a.d <= 1024) return bn_fwd_launch<T, 1, 8, 128, 2, RES, 4>(a, s);
+    if (a.d <= 4096) return bn_fwd_launch<T, 1, 8, 512, 1, RES, 4>(a, s);
+    return bn_fwd_launch<T, 1, 16, 512, 1, RES, 4>(a, s);
+}
+template <typename T, bool RES>
 cudaError_t bn_bwd_any(const BnArgs& a, bool vec, int* parts, cudaStream_t s) {
-    constexpr int E = 16 / sizeof(T);
-#define EACS_BN(VEC, VPL, TPR, RPC) return bn_bwd_launch<T, VEC, VPL, TPR, RPC, RES>(a, parts, s)
-    const int n = (a.d + E - 1) / E;
-    if (vec) {
-        if (n <= 8) EACS_BN(E, 1, 8, 32);
-        if (n <= 16) EACS_BN(E, 1, 16, 16);
-        if (n <= 32) EACS_BN(E, 1, 32, 8);
-        if (n <= 64) EACS_BN(E, 1, 64, 4);
-        if (n <= 96) EACS_BN(E, 1, 96, 2);
-        if (n <= 128) EACS_BN(E, 1, 128, 2);
-        if (n <= 256) EACS_BN(E, 1, 256, 1);
-        if (n <= 512) EACS_BN(E, 1, 512, 1);
-        if (n <= 1024) EACS_BN(E, 2, 512, 1);
-        if constexpr (E == 4) EACS_BN(E, 4, 512, 1);
-    }
-    if (a.d <= 128) EACS_BN(1, 4, 32, 8);
-    if (a.d <= 1024) EACS_BN(1, 8, 128, 2);
-    if (a.d <= 4096) EACS_BN(1, 8, 512, 1);
-    EACS_BN(1, 16, 512, 1);
-#undef EACS_BN
+    if constexpr (RES)
+        if (vec && !a.has_post) return a.gate ? bn_bwd_vec<T, RES, 1>(a, parts, s) : bn_bwd_vec<T, RES, 0>(a, parts, s);
+    if (vec) return a.gate ? bn_bwd_vec<T, RES, 3>(a, parts, s) : bn_bwd_vec<T, RES, 2>(a, parts, s);
+    if (a.d <= 128) return bn_bwd_launch<T, 1, 4, 32, 8, RES, 4>(a, parts, s);
+    if (a.d <= 1024) return bn_bwd_launch<T, 1, 8, 128, 2, RES, 4>(a, parts, s);
+    if (a.d <= 4096) return bn_bwd_launch<T, 1, 8, 512, 1, RES, 4>(a, parts, s);
+    return bn_bwd_launch<T, 1, 16, 512, 1, RES, 4>(a, parts, s);
 }
 
 int bn_check(const char* fn, const EacsNorm& p) {

@@ -7,8 +7,8 @@
 // and what the final state's gradient adds to the last W - 1 inputs.
 //
 // Bound by memory both ways: each value is read once (but for the W - 1 tokens around a run) and written once.  A warp takes
-// 64 channels, two a lane, of a run of tokens; rows of 128 (float32: 256) bytes come through shared memory, asked for two
-// stages of 16 tokens ahead (cp.async, its own, so without a barrier between warps), and the W inputs that a token sees
+// 64 channels, two a lane, of a run of tokens; rows of 128 (float32: 256) bytes come through shared memory, asked for three
+// stages of 8 tokens ahead (cp.async, its own, so without a barrier between warps), and the W inputs that a token sees
 // move through the lanes' registers as pairs.  Through registers the same loads left too few threads: 67 us against 50 at
 // B=4 L=16384 D=1024 forward, 127 against 70 the backward at B=8 L=8192 D=768.  Runs are as long as leaves every
 // multiprocessor full of warps once.  Rows that do not start on 16 bytes take kernels of one channel a thread.
@@ -336,7 +336,7 @@ __global__ void __launch_bounds__(32 * kConvRuns) conv_bwd_any_k(const ConvArgs 
 }
 
 // ---- two channels a lane, rows through shared memory -------------------------------------------------------
-constexpr int kConvU = 16, kConvStages = 3;  // tokens a stage; stages a warp
+constexpr int kConvU = 8, kConvStages = 4;  // tokens a stage; stages a warp
 
 // A warp's stages of N inputs: rows of 64 channels, copied 16 bytes a lane; what lies behind `end` is not read.
 template <typename T, int N>
@@ -454,7 +454,7 @@ __global__ void __launch_bounds__(32 * kConvRuns) conv_bwd_k(const ConvArgs a) {
             if (!live) continue;
             // inside the run every token is its own and completes an input of the run, none of which is in the final state
             if (t > t0 && t + kConvU <= tl) {
-#pragma unroll 8
+#pragma unroll
                 for (int u = 0; u < kConvU; ++u) {
                     f.shift();
                     f.token(*reinterpret_cast<const V*>(px + u * 64), *reinterpret_cast<const V*>(pg + u * 64), true, a.silu);

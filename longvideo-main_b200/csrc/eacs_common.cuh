@@ -238,6 +238,28 @@ template <> __device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(flo
     return __float2bfloat16_rn(v);
 }
 
+// Two 16-bit values of a register (or one float32) as float32, and back.
+template <typename T> __device__ __forceinline__ void unpack(uint32_t w, float& a, float& b);
+template <> __device__ __forceinline__ void unpack<__nv_bfloat16>(uint32_t w, float& a, float& b) {
+    a = __uint_as_float(w << 16);
+    b = __uint_as_float(w & 0xffff0000u);
+}
+template <> __device__ __forceinline__ void unpack<__half>(uint32_t w, float& a, float& b) {
+    const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w));
+    a = f.x, b = f.y;
+}
+template <> __device__ __forceinline__ void unpack<float>(uint32_t w, float& a, float& b) { a = __uint_as_float(w), b = 0.f; }
+template <typename T> __device__ __forceinline__ uint32_t pack(float a, float b);
+template <> __device__ __forceinline__ uint32_t pack<__nv_bfloat16>(float a, float b) {
+    const __nv_bfloat162 v = __floats2bfloat162_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&v);
+}
+template <> __device__ __forceinline__ uint32_t pack<__half>(float a, float b) {
+    const __half2 v = __floats2half2_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&v);
+}
+template <> __device__ __forceinline__ uint32_t pack<float>(float a, float) { return __float_as_uint(a); }
+
 // ----------------------------------------------------------------------------
 // mbarrier + TMA (cp.async.bulk[.tensor]) wrappers; every copy targets this
 // CTA's own shared memory from this GPU's memory.

@@ -96,27 +96,6 @@ __device__ __forceinline__ int sel_length(const SelArgs& a, int64_t b) {
 
 // E neighbouring channels of one token as they lie in memory, in whole registers: taken apart only where they are used, so
 // that asking for them does not wait for them.
-template <typename T> __device__ __forceinline__ void unpack(uint32_t w, float& a, float& b);
-template <> __device__ __forceinline__ void unpack<__nv_bfloat16>(uint32_t w, float& a, float& b) {
-    a = __uint_as_float(w << 16);
-    b = __uint_as_float(w & 0xffff0000u);
-}
-template <> __device__ __forceinline__ void unpack<__half>(uint32_t w, float& a, float& b) {
-    const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w));
-    a = f.x, b = f.y;
-}
-template <> __device__ __forceinline__ void unpack<float>(uint32_t w, float& a, float& b) { a = __uint_as_float(w), b = 0.f; }
-template <typename T> __device__ __forceinline__ uint32_t pack(float a, float b);
-template <> __device__ __forceinline__ uint32_t pack<__nv_bfloat16>(float a, float b) {
-    const __nv_bfloat162 v = __floats2bfloat162_rn(a, b);
-    return *reinterpret_cast<const uint32_t*>(&v);
-}
-template <> __device__ __forceinline__ uint32_t pack<__half>(float a, float b) {
-    const __half2 v = __floats2half2_rn(a, b);
-    return *reinterpret_cast<const uint32_t*>(&v);
-}
-template <> __device__ __forceinline__ uint32_t pack<float>(float a, float) { return __float_as_uint(a); }
-
 template <typename T, int E>
 struct Run {
     static constexpr int kBytes = E * sizeof(T), kWords = (kBytes + 3) / 4, kPer = 4 / sizeof(T);
