@@ -56,16 +56,31 @@ __device__ __forceinline__ int64_t conv_length(const ConvArgs& a, int64_t b) {
 __device__ __forceinline__ float conv_sigmoid(float v) { return __fdividef(1.0f, 1.0f + ex2_approx(v * -1.44269504f)); }
 
 template <typename T, int VEC>
-__device__ __forceinline__ void conv_read(float* v, const T* p) {
-    const RowVec<T, VEC> r = *reinterpret_cast<const RowVec<T, VEC>*>(p);
+__device__ __forceinline__ void conv_floats(float* v, const RowVec<T, VEC>& r) {
+    if constexpr (VEC > 1 && sizeof(T) == 2) {  // two to a register
+        const uint32_t* w = reinterpret_cast<const uint32_t*>(&r);
 #pragma unroll
-    for (int e = 0; e < VEC; ++e) v[e] = to_f32(r.e[e]);
+        for (int e = 0; e < VEC; e += 2) unpack<T>(w[e / 2], v[e], v[e + 1]);
+    } else {
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) v[e] = to_f32(r.e[e]);
+    }
+}
+template <typename T, int VEC>
+__device__ __forceinline__ void conv_read(float* v, const T* p) {
+    conv_floats<T, VEC>(v, *reinterpret_cast<const RowVec<T, VEC>*>(p));
 }
 template <typename T, int VEC>
 __device__ __forceinline__ void conv_write(T* p, const float* v) {
     RowVec<T, VEC> r;
+    if constexpr (VEC > 1 && sizeof(T) == 2) {
+        uint32_t* w = reinterpret_cast<uint32_t*>(&r);
 #pragma unroll
-    for (int e = 0; e < VEC; ++e) r.e[e] = from_f32<T>(v[e]);
+        for (int e = 0; e < VEC; e += 2) w[e / 2] = pack<T>(v[e], v[e + 1]);
+    } else {
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) r.e[e] = from_f32<T>(v[e]);
+    }
     *reinterpret_cast<RowVec<T, VEC>*>(p) = r;
 }
 
@@ -157,8 +172,7 @@ struct ConvFwd {
 #pragma unroll
         for (int k = 0; k + 1 < W; ++k) win[k] = win[k + 1];
         float p[VEC];
-#pragma unroll
-        for (int e = 0; e < VEC; ++e) p[e] = to_f32(v.e[e]);
+        conv_floats<T, VEC>(p, v);
         win[W - 1].set(p);
         cols.dot(p, win);
         if (silu)
@@ -200,8 +214,8 @@ struct ConvBwd {
     }
     __device__ __forceinline__ void token(const V& vx, const V& vg, bool mine, bool silu) {  // mine: one of the run's own
         float p[VEC], g[VEC];
-#pragma unroll
-        for (int e = 0; e < VEC; ++e) p[e] = to_f32(vx.e[e]), g[e] = to_f32(vg.e[e]);
+        conv_floats<T, VEC>(p, vx);
+        conv_floats<T, VEC>(g, vg);
         win[W - 1].set(p);
         if (silu) {
             cols.dot(p, win);
@@ -250,6 +264,18 @@ struct ConvBwd {
         }
         if (o >= 0) conv_write<T, VEC>(dx + o * a.D, g);
         else if (a.dh0) conv_write<T, VEC>(static_cast<T*>(a.dh0) + (b * (W - 1) + o + W - 1) * a.D + c, g);
+    }
+    // The run's sums: one partial row.
+    __device__ __forceinline__ void whole(const ConvArgs& a, int c, bool live) const {
+        if (!a.part || !live) return;
+        float* part = a.part + static_cast<int64_t>(blockIdx.y) * a.D * (W + 1);
+#pragma unroll
+        for (int k = 0; k <= W; ++k) {
+            float v[VEC];
+            dw[k].get(v);
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) part[k < W ? (c + e) * W + k : a.D * W + c + e] = v[e];
+        }
     }
     // The sums of the CTA's R runs, added in order: one partial row.
     template <int R>
@@ -337,6 +363,7 @@ __global__ void __launch_bounds__(32 * kConvRuns) conv_bwd_any_k(const ConvArgs 
 
 // ---- two channels a lane, rows through shared memory -------------------------------------------------------
 constexpr int kConvU = 8, kConvStages = 4;  // tokens a stage; stages a warp
+constexpr int kConvTiles = 4;               // warps of a CTA, side by side: rows of 512 bytes (float32: 1024) at a time
 
 // A warp's stages of N inputs: rows of 64 channels, copied 16 bytes a lane; what lies behind `end` is not read.
 template <typename T, int N>
@@ -364,13 +391,13 @@ struct ConvStages {
 };
 
 template <typename T, int W>
-__global__ void __launch_bounds__(32 * kConvRuns) conv_fwd_k(const ConvArgs a) {
+__global__ void __launch_bounds__(32 * kConvTiles) conv_fwd_k(const ConvArgs a) {
     using V = RowVec<T, 2>;
     extern __shared__ __align__(16) unsigned char smem[];
-    const int lane = threadIdx.x & 31, wid = threadIdx.x >> 5, c0 = blockIdx.x * 64, c = c0 + lane * 2;
+    const int lane = threadIdx.x & 31, wid = threadIdx.x >> 5, c0 = (blockIdx.x * kConvTiles + wid) * 64, c = c0 + lane * 2;
     const ConvStages<T, 1> st{reinterpret_cast<T*>(smem + wid * ConvStages<T, 1>::kBytes)};
-    const int64_t r = static_cast<int64_t>(blockIdx.y) * kConvRuns + wid;
-    if (r >= a.rows * a.runs) return;
+    const int64_t r = blockIdx.y;
+    if (c0 >= a.D) return;
     const int64_t b = r / a.runs, len = conv_length(a, b);
     const int64_t t0 = (r - b * a.runs) * a.run, t1 = min(t0 + a.run, a.L), tl = min(t1, len);
     const bool live = c < a.D;
@@ -414,16 +441,16 @@ __global__ void __launch_bounds__(32 * kConvRuns) conv_fwd_k(const ConvArgs a) {
 }
 
 template <typename T, int W>
-__global__ void __launch_bounds__(32 * kConvRuns) conv_bwd_k(const ConvArgs a) {
+__global__ void __launch_bounds__(32 * kConvTiles) conv_bwd_k(const ConvArgs a) {
     using V = RowVec<T, 2>;
     extern __shared__ __align__(16) unsigned char smem[];
-    const int lane = threadIdx.x & 31, wid = threadIdx.x >> 5, c0 = blockIdx.x * 64, c = c0 + lane * 2;
+    const int lane = threadIdx.x & 31, wid = threadIdx.x >> 5, c0 = (blockIdx.x * kConvTiles + wid) * 64, c = c0 + lane * 2;
     const ConvStages<T, 2> st{reinterpret_cast<T*>(smem + wid * ConvStages<T, 2>::kBytes)};
-    const int64_t r = static_cast<int64_t>(blockIdx.y) * kConvRuns + wid;
+    const int64_t r = blockIdx.y;
     const bool live = c < a.D;
     ConvBwd<T, 2, W> f;
     f.clear();
-    if (r < a.rows * a.runs) {
+    if (c0 < a.D) {
         const int64_t b = r / a.runs, len = conv_length(a, b);
         const int64_t t0 = (r - b * a.runs) * a.run, t1 = min(t0 + a.run, a.L), tl = min(t1, len);
         const T* x = static_cast<const T*>(a.x) + b * a.sx[0] + c0;
@@ -473,7 +500,7 @@ __global__ void __launch_bounds__(32 * kConvRuns) conv_bwd_k(const ConvArgs a) {
         if (live)
             for (int64_t t = max(t0, tl); t < t1; ++t) conv_write<T, 2>(dx + t * a.D, nil);
     }
-    f.template sums<kConvRuns>(a, c, live);
+    f.whole(a, c, live);
 }
 
 template <typename T, int VEC, int W>
@@ -494,8 +521,7 @@ __global__ void __launch_bounds__(128) conv_step_k(const ConvArgs a) {
     float p[VEC];
 #pragma unroll
     for (int k = 0; k < W; ++k) {
-#pragma unroll
-        for (int e = 0; e < VEC; ++e) p[e] = to_f32(raw[k].e[e]);
+        conv_floats<T, VEC>(p, raw[k]);
         win[k].set(p);
     }
     cols.dot(p, win);
@@ -519,39 +545,41 @@ void conv_runs(ConvArgs& a, int64_t tiles, int warps) {
 constexpr int kConvBwdWarps = 16;
 int64_t conv_bwd_rows(ConvArgs& a, bool staged) {
     conv_runs(a, (a.D + (staged ? 63 : 31)) / (staged ? 64 : 32), kConvBwdWarps);
-    return (a.rows * a.runs + kConvRuns - 1) / kConvRuns;
+    return staged ? a.rows * a.runs : (a.rows * a.runs + kConvRuns - 1) / kConvRuns;
 }
-dim3 conv_grid(const ConvArgs& a, int cols) {
-    return dim3((a.D + cols - 1) / cols, static_cast<unsigned>((a.rows * a.runs + kConvRuns - 1) / kConvRuns));
+dim3 conv_grid(const ConvArgs& a) {
+    return dim3((a.D + 64 * kConvTiles - 1) / (64 * kConvTiles), static_cast<unsigned>(a.rows * a.runs));
+}
+dim3 conv_grid_any(const ConvArgs& a) {
+    return dim3((a.D + 31) / 32, static_cast<unsigned>((a.rows * a.runs + kConvRuns - 1) / kConvRuns));
 }
 
 template <typename T, int W>
 cudaError_t conv_fwd_launch(ConvArgs& a, bool staged, cudaStream_t s) {
-    constexpr int threads = 32 * kConvRuns;
     if (staged) {
-        constexpr size_t smem = kConvRuns * ConvStages<T, 1>::kBytes;
-        static const int per = row_resident(conv_fwd_k<T, W>, threads, smem);
-        conv_runs(a, (a.D + 63) / 64, per * kConvRuns);
-        conv_fwd_k<T, W><<<conv_grid(a, 64), threads, smem, s>>>(a);
+        constexpr size_t smem = kConvTiles * ConvStages<T, 1>::kBytes;
+        static const int per = row_resident(conv_fwd_k<T, W>, 32 * kConvTiles, smem);
+        conv_runs(a, (a.D + 63) / 64, per * kConvTiles);
+        conv_fwd_k<T, W><<<conv_grid(a), 32 * kConvTiles, smem, s>>>(a);
     } else {
+        constexpr int threads = 32 * kConvRuns;
         static const int per = row_resident(conv_fwd_any_k<T, W, 8>, threads, 0);
         conv_runs(a, (a.D + 31) / 32, per * kConvRuns);
-        conv_fwd_any_k<T, W, 8><<<conv_grid(a, 32), threads, 0, s>>>(a);
+        conv_fwd_any_k<T, W, 8><<<conv_grid_any(a), threads, 0, s>>>(a);
     }
     note_launch();
     return cudaGetLastError();
 }
 template <typename T, int W>
 cudaError_t conv_bwd_launch(ConvArgs& a, bool staged, void* dweight, void* dbias, cudaStream_t s) {
-    constexpr int threads = 32 * kConvRuns;
     const int64_t rows = conv_bwd_rows(a, staged);
     if (staged) {
-        constexpr size_t smem = kConvRuns * ConvStages<T, 2>::kBytes;
+        constexpr size_t smem = kConvTiles * ConvStages<T, 2>::kBytes;
         const cudaError_t e = cudaFuncSetAttribute(conv_bwd_k<T, W>, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
         if (e != cudaSuccess) return e;
-        conv_bwd_k<T, W><<<conv_grid(a, 64), threads, smem, s>>>(a);
+        conv_bwd_k<T, W><<<conv_grid(a), 32 * kConvTiles, smem, s>>>(a);
     } else {
-        conv_bwd_any_k<T, W, 4><<<conv_grid(a, 32), threads, 0, s>>>(a);
+        conv_bwd_any_k<T, W, 4><<<conv_grid_any(a), 32 * kConvRuns, 0, s>>>(a);
     }
     note_launch();
     cudaError_t e = cudaGetLastError();
