@@ -266,10 +266,6 @@ struct SliceBC {
             }
         }
     }
-    __device__ __forceinline__ void b(int t, int ln, float* v) const {
-        const float4 q = *reinterpret_cast<const float4*>(out + t * NP + ln * 4);
-        v[0] = q.x, v[1] = q.y, v[2] = q.z, v[3] = q.w;
-    }
     __device__ __forceinline__ Quad b(int t, int ln) const { return *reinterpret_cast<const Quad*>(out + t * NP + ln * 4); }
     __device__ __forceinline__ Quad c(int t, int ln) const { return *reinterpret_cast<const Quad*>(out + (S + t) * NP + ln * 4); }
 };
@@ -277,16 +273,14 @@ struct SliceBC {
 // ---------------------------------------------------------------------------------------------------------
 // forward
 // ---------------------------------------------------------------------------------------------------------
-// A slice is S tokens of CW channels, two channels a thread.  A token's values are worked out in the layout they are read
-// in (lane = token and a quarter of the channels, E of them) and handed to the sweep through shared memory.
-// The sweep starts from a state of zero, so that nothing in it waits for the warp before: it leaves the slice's own state,
-// the product P of its decays, its own part of the outputs, and C P of every token.  With the state h handed in, the state
-// handed on is own + P h (all that the ring waits for), and the outputs get (C P) . h.
-// What a thread reads from shared memory (128 bytes a clock and multiprocessor) is what bounds this next to the special
-// function pipe: two channels a thread halve what B and C cost.
+// A slice is S tokens of CW channels; a thread holds eight states of a channel.  A token's values are worked out in the
+// layout they are read in (lane = token and a quarter of the channels, E of them) and handed to the sweep through shared
+// memory.  The sweep starts from a state of zero, so that nothing in it waits for the warp before: it leaves the slice's
+// own state, the product P of its decays, its own part of the outputs, and C P of every token.  With the state h handed in,
+// the state handed on is own + P h (all that the ring waits for), and the outputs get (C P) . h.
 template <int LN>
 struct FwdShape {
-    static constexpr int S = 8, NP = 4 * LN, CW = 64 / LN, E = CW / 4;
+    static constexpr int S = 8, NP = 4 * LN, L8 = LN / 2, CW = 32 / L8, E = CW / 4;  // L8: threads a channel
     static constexpr int YS = CW + 4;
 };
 template <typename T, int LN>
@@ -295,7 +289,7 @@ constexpr size_t sel_fwd_warp_bytes() {
     using BC = SliceBC<T, LN, Sh::S, true>;
     return BC::kRawBytes + BC::kBytes + 2 * Sh::S * Sh::CW * 4 + Sh::S * Sh::YS * 4;
 }
-// a CTA's own: the states handed on (two channels of 32 lanes a warp), dt_bias and skip of its channels
+// a CTA's own: the states handed on (eight of 32 lanes a warp), dt_bias and skip of its channels
 template <int LN>
 constexpr size_t sel_fwd_cta_bytes(int W) {
     return W * 1024 + 2 * FwdShape<LN>::CW * 4;
@@ -313,14 +307,13 @@ __global__ void __launch_bounds__(kSelFwdWarps * 32, 1) sel_fwd_k(const SelArgs 
     Quad* hop = reinterpret_cast<Quad*>(smem);  // [W][2][32]: the state that each warp is handed
     float* pars = reinterpret_cast<float*>(smem + W * 1024);  // [2][CW]: dt_bias, skip
     unsigned char* mine = smem + sel_fwd_cta_bytes<LN>(W) + static_cast<size_t>(w) * sel_fwd_warp_bytes<T, LN>();
-    float* ss = reinterpret_cast<float*>(mine + BC::kRawBytes + BC::kBytes);  // [S][CW]: s log2 e
-    float* sv = ss + S * CW;                                                  // [S][CW]: s x
-    float* yb = sv + S * CW;                                                  // [S][YS]: sums over the states
+    float2* sd = reinterpret_cast<float2*>(mine + BC::kRawBytes + BC::kBytes);  // [S][CW]: s log2 e, s x
+    float* yb = reinterpret_cast<float*>(sd + S * CW);                          // [S][YS]: sums over the states
 
     const int64_t b = blockIdx.y;
     const int d0 = blockIdx.x * CW;
     const int len = sel_length(a, b), slices = (len + S - 1) / S;
-    const int ln = lane % LN, ch = lane / LN * 2, d = d0 + ch, n0 = ln * 4;  // in the sweep
+    const int ln = lane % Sh::L8, ch = lane / Sh::L8, d = d0 + ch, n0 = ln * 8;  // in the sweep
     const int row = lane / 4, cr = (lane & 3) * E, dr = d0 + cr;             // in memory's layout
     T* y = static_cast<T*>(a.y) + (b * a.L + row) * a.D + dr;
     const BC bc{static_cast<const T*>(a.B) + b * a.sB[0], static_cast<const T*>(a.C) + b * a.sC[0],
@@ -333,15 +326,12 @@ __global__ void __launch_bounds__(kSelFwdWarps * 32, 1) sel_fwd_k(const SelArgs 
         pars[i] = p && c < a.D ? p[c] : 0.f;
     }
     __syncthreads();
-    float A[2][4];
+    Quad A[2], h[2];
 #pragma unroll
     for (int c = 0; c < 2; ++c) {
-        const float4 q = read_states(a.A, d + c, a.D, n0, a.N);
-        A[c][0] = q.x, A[c][1] = q.y, A[c][2] = q.z, A[c][3] = q.w;
+        A[c] = quad(read_states(a.A, d, a.D, n0 + 4 * c, a.N));
+        h[c] = quad(w == 0 && a.h0 ? read_states(a.h0 + b * a.D * a.N, d, a.D, n0 + 4 * c, a.N) : make_float4(0.f, 0.f, 0.f, 0.f));
     }
-    Quad h[2];
-#pragma unroll
-    for (int c = 0; c < 2; ++c) h[c] = quad(w == 0 && a.h0 ? read_states(a.h0 + b * a.D * a.N, d + c, a.D, n0, a.N) : make_float4(0.f, 0.f, 0.f, 0.f));
 
     Run<T, E> rx, rt, rz;
     const int64_t t_first = w * S + row;
@@ -378,34 +368,36 @@ __global__ void __launch_bounds__(kSelFwdWarps * 32, 1) sel_fwd_k(const SelArgs 
                 xs[e] *= s[e];
                 s[e] *= kLog2e;
             }
-            put_run<E>(ss + row * CW + cr, s);
-            put_run<E>(sv + row * CW + cr, xs);
+            float both_of[2 * E];
+#pragma unroll
+            for (int e = 0; e < E; ++e) both_of[2 * e] = s[e], both_of[2 * e + 1] = xs[e];
+            put_run<2 * E>(reinterpret_cast<float*>(sd + row * CW + cr), both_of);
         }
         __syncwarp();
         if (j + W < slices) ask(j + W);
 
         Quad own[2], P[2], CP[S][2];
-        float v[2 * S];
+        float v[S];
 #pragma unroll
         for (int t = 0; t < S; ++t) {
-            const float2 s2 = *reinterpret_cast<const float2*>(ss + t * CW + ch), v2 = *reinterpret_cast<const float2*>(sv + t * CW + ch);
-            const Quad Cq = bc.c(t, ln);
-            float Bv[4];
-            bc.b(t, ln, Bv);
+            const float2 q = sd[t * CW + ch];
+            const f32x2 s2 = pair(q.x, q.x), v2 = pair(q.y, q.y);
+            f32x2 sum;
 #pragma unroll
             for (int c = 0; c < 2; ++c) {
-                const float sc = c ? s2.y : s2.x, vc = c ? v2.y : v2.x;
-                const f32x2 a0 = pair(ex2_approx(sc * A[c][0]), ex2_approx(sc * A[c][1]));
-                const f32x2 a1 = pair(ex2_approx(sc * A[c][2]), ex2_approx(sc * A[c][3]));
-                const f32x2 b0 = pair(vc * Bv[0], vc * Bv[1]), b1 = pair(vc * Bv[2], vc * Bv[3]);
+                const Quad Bq = bc.b(t, 2 * ln + c), Cq = bc.c(t, 2 * ln + c);
+                const f32x2 a0 = ex2_pair(mul2(s2, A[c].lo)), a1 = ex2_pair(mul2(s2, A[c].hi));
+                const f32x2 b0 = mul2(v2, Bq.lo), b1 = mul2(v2, Bq.hi);
                 own[c].lo = t ? fma2(a0, own[c].lo, b0) : b0;
                 own[c].hi = t ? fma2(a1, own[c].hi, b1) : b1;
                 P[c].lo = t ? mul2(P[c].lo, a0) : a0;
                 P[c].hi = t ? mul2(P[c].hi, a1) : a1;
-                v[2 * t + c] = both(fma2(Cq.hi, own[c].hi, mul2(Cq.lo, own[c].lo)));
+                sum = c ? fma2(Cq.lo, own[c].lo, sum) : mul2(Cq.lo, own[c].lo);
+                sum = fma2(Cq.hi, own[c].hi, sum);
                 CP[t][c].lo = mul2(Cq.lo, P[c].lo);
                 CP[t][c].hi = mul2(Cq.hi, P[c].hi);
             }
+            v[t] = both(sum);
         }
         if (j > 0 && W > 1) {
             asm volatile("bar.sync %0, 64;" ::"r"(w) : "memory");
@@ -425,22 +417,26 @@ __global__ void __launch_bounds__(kSelFwdWarps * 32, 1) sel_fwd_k(const SelArgs 
                 asm volatile("bar.arrive %0, 64;" ::"r"(next) : "memory");
             }
         } else if (a.hN) {
-            for (int c = 0; c < 2; ++c) write_states(a.hN + b * a.D * a.N, d + c, a.D, n0, a.N, own[c]);
+            for (int c = 0; c < 2; ++c) write_states(a.hN + b * a.D * a.N, d, a.D, n0 + 4 * c, a.N, own[c]);
         }
         if constexpr (CKPT) {
+            float* k = a.ckpt + ((b * ((a.L + 7) / 8) + j) * a.D + d) * NP + n0;
 #pragma unroll
             for (int c = 0; c < 2; ++c)
-                if (FULL || d + c < a.D) *reinterpret_cast<Quad*>(a.ckpt + ((b * ((a.L + 7) / 8) + j) * a.D + d + c) * NP + n0) = h[c];
+                if (FULL || d < a.D) *reinterpret_cast<Quad*>(k + 4 * c) = h[c];
         }
 #pragma unroll
-        for (int t = 0; t < S; ++t)
-#pragma unroll
-            for (int c = 0; c < 2; ++c) v[2 * t + c] += both(fma2(CP[t][c].hi, h[c].hi, mul2(CP[t][c].lo, h[c].lo)));
+        for (int t = 0; t < S; ++t) {
+            f32x2 sum = mul2(CP[t][0].lo, h[0].lo);
+            sum = fma2(CP[t][0].hi, h[0].hi, sum);
+            sum = fma2(CP[t][1].lo, h[1].lo, sum);
+            v[t] += both(fma2(CP[t][1].hi, h[1].hi, sum));
+        }
         if (W == 1) h[0] = own[0], h[1] = own[1];
-        Fold<2 * S, LN / 2, 1>::run(v, lane);
-        const int first = FoldShape<2 * S, LN / 2, 1>::held(lane);
+        Fold<S, Sh::L8 / 2, 1>::run(v, lane);
+        const int first = FoldShape<S, Sh::L8 / 2, 1>::held(lane);
 #pragma unroll
-        for (int i = 0; i < 2 * S / LN; ++i) yb[((first + i) / 2) * Sh::YS + ch + ((first + i) & 1)] = v[i];
+        for (int i = 0; i < S / Sh::L8; ++i) yb[(first + i) * Sh::YS + ch] = v[i];
         __syncwarp();
         if (t0 + row < a.L) {
             float o[E], xs[E], g[E], skip[E];
@@ -461,7 +457,7 @@ __global__ void __launch_bounds__(kSelFwdWarps * 32, 1) sel_fwd_k(const SelArgs 
     const float nil[E] = {};
     for (int64_t t = static_cast<int64_t>(slices + w) * S; t + row < a.L; t += W * S) write_run<T, E, FULL>(nil, y + t * a.D, dr, a.D, vec);
     if (slices == 0 && w == 0 && a.hN)
-        for (int c = 0; c < 2; ++c) write_states(a.hN + b * a.D * a.N, d + c, a.D, n0, a.N, h[c]);
+        for (int c = 0; c < 2; ++c) write_states(a.hN + b * a.D * a.N, d, a.D, n0 + 4 * c, a.N, h[c]);
 }
 
 // ---------------------------------------------------------------------------------------------------------
@@ -904,13 +900,15 @@ SelArgs sel_args(const EacsSelective& p) {
     return a;
 }
 
-// Twelve warps a multiprocessor: of one CTA where there are few, else of two or three.
+// A CTA of the twelve warps that a multiprocessor has registers for, so that each ring has all of them: two rounds of 148
+// such CTAs took 644 us where rings of six warps, two at once, took 699 (B=4 L=16384 D=1024 N=16: 256 groups of channels).
+// Rows of few slices take as many warps as they have slices, and a multiprocessor several CTAs.
 template <typename T, int LN, bool CKPT, bool FULL>
 cudaError_t sel_fwd_launch(const SelArgs& a, cudaStream_t s) {
-    constexpr int CW = FwdShape<LN>::CW;
+    constexpr int CW = FwdShape<LN>::CW, S = FwdShape<LN>::S;
     const dim3 grid((a.D + CW - 1) / CW, static_cast<unsigned>(a.Bn));
-    const int64_t ctas = static_cast<int64_t>(grid.x) * grid.y;
-    const int W = ctas <= 148 ? 12 : ctas <= 296 ? 6 : 4;
+    const int slices = (a.L + S - 1) / S;
+    const int W = slices >= 12 ? kSelFwdWarps : slices >= 6 ? 6 : slices >= 4 ? 4 : slices;
     const size_t smem = sel_fwd_cta_bytes<LN>(W) + W * sel_fwd_warp_bytes<T, LN>();
     const auto k = sel_fwd_k<T, LN, CKPT, FULL>;
     const cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
