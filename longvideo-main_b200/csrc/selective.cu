@@ -562,8 +562,11 @@ constexpr size_t sel_bwd_group_bytes(int W) {
 }
 constexpr int kSelBwdWarps = 8, kSelBwdMaxGroups = 8;
 
-// FULL: groups of CW channels and rows of NP states, all of them on 16 bytes
-template <typename T, int LN, bool FULL>
+// FULL: groups of CW channels and rows of NP states, all of them on 16 bytes.  AHEAD: what is handed on is worked out
+// before the sweep that needs what is handed in (the slice's own end and the product of its decays, as in the forward): with
+// one group a CTA nothing else fills the ring's wait (B=1 L=8192 D=768 training step 643 to 546 us); with more the other
+// groups do, and the extra products cost (B=8: 1900 us without, 2003 with; two groups, B=2: 741 and 765).
+template <typename T, int LN, bool FULL, bool AHEAD>
 __global__ void __launch_bounds__(kSelBwdWarps * 32, 1) sel_bwd_k(const SelArgs a) {
     using Sh = BwdShape<LN>;
     using BC = SliceBC<T, LN, Sh::S, FULL>;
@@ -706,7 +709,29 @@ __global__ void __launch_bounds__(kSelBwdWarps * 32, 1) sel_bwd_k(const SelArgs 
 #pragma unroll
                 for (int i = 0; i < kept; ++i) ob[(first + i) * YS + ch] = v[i];
             }
-            Quad gs = quad(make_float4(0.f, 0.f, 0.f, 0.f));
+            Quad gs = quad(make_float4(0.f, 0.f, 0.f, 0.f)), own = gs, P = gs;
+            if constexpr (AHEAD) {
+#pragma unroll
+                for (int t = S - 1; t >= 0; --t) {
+                    const f32x2 do2 = gd[Sh::place(t, ch)];
+                    const Quad Cq = bc.c(t, ln);
+                    own.lo = mul2(dec[t].lo, t == S - 1 ? mul2(Cq.lo, do2) : fma2(Cq.lo, do2, own.lo));
+                    own.hi = mul2(dec[t].hi, t == S - 1 ? mul2(Cq.hi, do2) : fma2(Cq.hi, do2, own.hi));
+                    P.lo = t == S - 1 ? dec[t].lo : mul2(P.lo, dec[t].lo);
+                    P.hi = t == S - 1 ? dec[t].hi : mul2(P.hi, dec[t].hi);
+                }
+            }
+            auto hand_on = [&](const Quad& q) {
+                if (j > 0) {
+                    const int next = (w + 1 == W ? 0 : w + 1) * G + g;
+                    hop[next * 32 + lane] = q;
+                    __syncwarp();
+                    if (lane == 0)
+                        asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(&bars[next])) : "memory");
+                } else if (a.dh0) {
+                    write_states(a.dh0 + b * a.D * a.N, dc, a.D, n0, a.N, q);
+                }
+            };
             if (k > 0) {
                 const uint32_t phase = (w == 0 ? turn - 1 : turn) & 1;
                 if (ok) ok = mbar_wait(&bars[wg], phase);
@@ -714,6 +739,7 @@ __global__ void __launch_bounds__(kSelBwdWarps * 32, 1) sel_bwd_k(const SelArgs 
             } else if (a.dhN) {
                 gs = quad(read_states(a.dhN + b * a.D * a.N, dc, a.D, n0, a.N));
             }
+            if constexpr (AHEAD) hand_on(Quad{fma2(P.lo, gs.lo, own.lo), fma2(P.hi, gs.hi, own.hi)});
             Quad dA = dAs[wg * 32 + lane];
             float dv[S], aw[S];
 #pragma unroll
@@ -733,15 +759,7 @@ __global__ void __launch_bounds__(kSelBwdWarps * 32, 1) sel_bwd_k(const SelArgs 
                 gs.lo = mul2(gs.lo, dec[t].lo);
                 gs.hi = mul2(gs.hi, dec[t].hi);
             }
-            if (j > 0) {
-                const int next = (w + 1 == W ? 0 : w + 1) * G + g;
-                hop[next * 32 + lane] = gs;
-                __syncwarp();
-                if (lane == 0)
-                    asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(&bars[next])) : "memory");
-            } else if (a.dh0) {
-                write_states(a.dh0 + b * a.D * a.N, dc, a.D, n0, a.N, gs);
-            }
+            if constexpr (!AHEAD) hand_on(gs);
             dAs[wg * 32 + lane] = dA;
             Fold<S, LN / 2, 1>::run(dv, lane);
             Fold<S, LN / 2, 1>::run(aw, lane);
@@ -963,7 +981,9 @@ cudaError_t sel_bwd_launch(const SelArgs& a, int parts, T* dB, T* dC, float* dA,
     const size_t smem = (sel_bwd_group_bytes<LN>(W) * a.groups + 15) / 16 * 16 + W * sel_bwd_warp_bytes<T, LN>();
     // (a group of channels may start past D only where they are not FULL)
     const bool full = a.vec && a.vec_bc && a.N == 4 * LN && a.D % (a.groups * BwdShape<LN>::CW) == 0;
-    const auto k = full ? sel_bwd_k<T, LN, true> : sel_bwd_k<T, LN, false>;
+    const bool ahead = a.groups == 1;
+    const auto k = full ? (ahead ? sel_bwd_k<T, LN, true, true> : sel_bwd_k<T, LN, true, false>)
+                        : (ahead ? sel_bwd_k<T, LN, false, true> : sel_bwd_k<T, LN, false, false>);
     cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
     if (e != cudaSuccess) return e;
     k<<<dim3(parts, static_cast<unsigned>(a.Bn)), W * 32, smem, s>>>(a);
