@@ -12,6 +12,9 @@
 // once; s is never rounded before its norm.  The backward takes everything again from the forward's inputs, so the forward
 // saves nothing.  Sums over rows are kept in float32 registers, a thread's own columns; a CTA writes one partial row and a
 // second kernel adds them in order (no atomics: the same inputs give the same bits).
+// Measured, us (bytes' time in brackets): 65536 x 768 bfloat16 with a scale, forward 62 (62), backward 104 (92) + 8 for the
+// sums; heads of 128, 131072 of them, gated 20 (15).  Float32 rows above 4096 values and 16-bit ones above 4096 spill
+// registers in the backward.
 #include <algorithm>
 
 #include "eacs_common.cuh"
@@ -182,8 +185,8 @@ __global__ void __launch_bounds__(TPR * RPC) bn_fwd_k(const BnArgs a) {
 }
 
 // The backward's inputs of a thread's next row on their way to shared memory (its own 16-byte vectors, so without a
-// barrier) while it works on this one: 18 warps that each waited for their row left memory idle (199 us of 65536 rows of
-// 768 with a scale; what it takes now stands at bn_bwd_launch).
+// barrier) while it works on this one: 18 warps that each waited for their row left memory idle (65536 bfloat16 rows of 768
+// with a scale: 199 us without, 104 with it and values unpacked from whole registers; the bytes alone take 92).
 template <int VEC, int VPL, int TPR, int RPC, bool RES, int HOW>
 struct BnStage {
     static constexpr int kInputs = 2 + (HOW & 1) + (RES ? 2 : 0);

@@ -11,16 +11,23 @@
 //   dA[n]   = sum_t s_t w_t[n],   dskip = sum_t do_t x_t,   dz = dy o silu'(z),   ddt = ds softplus'.
 //
 // One exponential per token, channel and state is what it cannot do without: 16 a clock and multiprocessor, which is
-// 230 us for the 1.07e9 of B=4 L=16384 D=1024 N=16 against 82 us of memory traffic.  So the kernels are built around the
-// special function pipe.  A thread holds four states of a channel (LN threads a channel), a warp 32 / LN channels, and a
-// slice of tokens at a time, whose exponentials it takes before it needs the state: the warps of a CTA take consecutive
-// slices of the same channels and hand the state around a ring, so that the only thing in sequence is a slice's
-// multiply-adds.  (One warp for all of a row's tokens would leave a scheduler with less than one warp at the size above.)
-// Pairs of states are multiplied and added by the two-wide float32 instructions, which take half the issue slots.
+// 230 us for the 1.07e9 of B=4 L=16384 D=1024 N=16 (with those of softplus and silu 290) against 82 us of memory traffic.
+// A warp takes a slice of 8 tokens of a few channels at a time; the warps of a CTA take consecutive slices of the same
+// channels and hand the state around a ring, so that the only thing in sequence is a few multiply-adds a slice.  (One warp
+// for all of a row's tokens would leave a scheduler with less than one warp at that size.)  Pairs of states are multiplied
+// and added by the two-wide float32 instructions, which take half the issue slots.
 //
-// The forward for training writes the state in front of every 8 tokens; the backward starts a slice of 8 from it.  Sums
-// over channels stay in registers while a warp goes through its CTA's channels, are then folded over its lanes, and a CTA
-// writes one partial row of dB and dC that a second kernel adds in order (no atomics: the same inputs give the same bits).
+// Measured, us: forward B=4 L=16384 D=1024 N=16 bfloat16 637; B=1 322; B=8 L=8192 D=768 485 (528 with checkpoints), the
+// backward of that 1364 and 28 for the sums of dB and dC.  What holds it off the exponentials' time is latency: 12 warps a
+// multiprocessor (backward 8) with the registers that a slice's decays and sums take, at 12 (backward 26) instructions for
+// 32 updates; the special function pipe is 45 percent busy, issue slots 52 percent (backward 18 and 47).  Tried and slower:
+// slices of 4 tokens with 16 or 20 warps (813 and 894 us where 8 with 12 took 745), in the backward slices of 4 with two
+// channels a thread and 12 warps (half the shared memory reads, but half again as many instructions: 2477 us a training step
+// where 1971 was), and the tokens' values of all of a CTA's groups worked out at once (2180 where 1900 was).
+//
+// The forward for training writes the state in front of every 8 tokens; the backward starts a slice from it.  Sums over
+// channels stay in registers while a warp goes through its CTA's channels, are then folded over its lanes, and a CTA writes
+// one partial row of dB and dC that a second kernel adds in order (no atomics: the same inputs give the same bits).
 #include <algorithm>
 
 #include "eacs_common.cuh"
@@ -541,7 +548,8 @@ __global__ void __launch_bounds__(256) sel_step_k(const SelArgs a) {
 // ---------------------------------------------------------------------------------------------------------
 // Slices of 8 tokens from the last to the first, one a warp; a warp takes its slice through the CTA's groups of CW channels
 // and hands each group's g on.  Per slice and group: decays and states from the checkpoint, with dC on the way, then
-// backwards with dB, dv, w and dA.  dB and dC of the slice stay in 64 registers a lane over all groups.
+// backwards with dB, dv, w and dA.  A thread holds four states of a channel (LN threads a channel); dB and dC of the slice
+// stay in 64 registers a lane over all groups, so that they are folded over the lanes once a slice.
 template <int LN>
 struct BwdShape {
     static constexpr int S = 8, NP = 4 * LN, CW = 32 / LN;
