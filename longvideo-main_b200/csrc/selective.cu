@@ -111,21 +111,22 @@ __device__ __forceinline__ int sel_length(const SelArgs& a, int64_t b) {
 
 // E neighbouring channels of one token as they lie in memory, in whole registers: taken apart only where they are used, so
 // that asking for them does not wait for them.
-template <typename T, int E>
+// FULL: all of the channels are there, and vectors may be read.  Else a lane whose channels may not be read as a vector keeps
+// each in a register of its own.
+template <typename T, int E, bool FULL>
 struct Run {
-    static constexpr int kBytes = E * sizeof(T), kWords = (kBytes + 3) / 4, kPer = 4 / sizeof(T);
+    static constexpr int kBytes = E * sizeof(T), kPacked = (kBytes + 3) / 4, kPer = 4 / sizeof(T), kWords = FULL ? kPacked : E;
     uint32_t w[kWords];
-    // the channels d.. of D; FULL: all of them are there, and vectors may be read
-    template <bool FULL = false>
+    // the channels d.. of D
+    static __device__ __forceinline__ bool packed(int d, int D, bool vec) { return FULL || (vec && d + E <= D); }
     __device__ __forceinline__ void read(const T* p, bool in, int d, int D, bool vec) {
-        if (FULL) {
 #pragma unroll
-            for (int i = 0; i < kWords; ++i) w[i] = 0;
-        }
-        if (in && (FULL || (vec && d + E <= D))) {
+        for (int i = 0; i < kWords; ++i) w[i] = 0;
+        if (!in) return;
+        if (packed(d, D, vec)) {
             if constexpr (kBytes >= 16) {
 #pragma unroll
-                for (int i = 0; i < kWords; i += 4) {
+                for (int i = 0; i < kPacked; i += 4) {
                     const uint4 v = reinterpret_cast<const uint4*>(p)[i / 4];
                     w[i] = v.x, w[i + 1] = v.y, w[i + 2] = v.z, w[i + 3] = v.w;
                 }
@@ -137,34 +138,33 @@ struct Run {
             } else {
                 w[0] = *reinterpret_cast<const uint16_t*>(p);
             }
-        } else if (!FULL) {
+        } else if constexpr (!FULL) {
 #pragma unroll
-            for (int i = 0; i < kWords; ++i) {
-                w[i] = 0;
-#pragma unroll
-                for (int k = 0; k < kPer; ++k) {
-                    const int e = i * kPer + k;
-                    if (e < E && in && d + e < D) {
-                        if constexpr (sizeof(T) == 4) w[i] = reinterpret_cast<const uint32_t*>(p)[e];
-                        else w[i] |= static_cast<uint32_t>(reinterpret_cast<const uint16_t*>(p)[e]) << (16 * k);
-                    }
+            for (int e = 0; e < E; ++e)
+                if (d + e < D) {
+                    if constexpr (sizeof(T) == 4) w[e] = reinterpret_cast<const uint32_t*>(p)[e];
+                    else w[e] = reinterpret_cast<const uint16_t*>(p)[e];
                 }
-            }
         }
     }
-    __device__ __forceinline__ void floats(float* v) const {
+    __device__ __forceinline__ void floats(float* v, bool is_packed) const {
+        float a, b;
+        if (FULL || sizeof(T) == 4 || is_packed) {
 #pragma unroll
-        for (int i = 0; i < kWords; ++i) {
-            float a, b;
-            unpack<T>(w[i], a, b);
-            v[i * kPer] = a;
-            if (kPer == 2 && i * kPer + 1 < E) v[i * kPer + 1] = b;
+            for (int i = 0; i < kPacked; ++i) {
+                unpack<T>(w[i], a, b);
+                v[i * kPer] = a;
+                if (kPer == 2 && i * kPer + 1 < E) v[i * kPer + 1] = b;
+            }
+        } else {
+#pragma unroll
+            for (int e = 0; e < E; ++e) unpack<T>(w[e < kWords ? e : 0], v[e], b);
         }
     }
 };
 template <typename T, int E, bool FULL = false>
 __device__ __forceinline__ void write_run(const float* v, T* p, int d, int D, bool vec) {
-    using R = Run<T, E>;
+    using R = Run<T, E, true>;
     if ((FULL || (vec && d + E <= D)) && R::kBytes >= 4) {
         uint32_t w[R::kWords];
 #pragma unroll
@@ -268,9 +268,9 @@ struct SliceBC {
                 float v[4] = {};
                 if (FULL || a.vec_bc) {
                     if (FULL || n < a.N) {
-                        Run<T, 4> q;
-                        q.template read<true>(raw + (which * S + r) * NP + n, true, 0, 4, true);
-                        q.floats(v);
+                        Run<T, 4, true> q;
+                        q.read(raw + (which * S + r) * NP + n, true, 0, 4, true);
+                        q.floats(v, true);
                     }
                 } else {
 #pragma unroll
@@ -348,16 +348,18 @@ __global__ void __launch_bounds__(kSelFwdWarps * 32, 1) sel_fwd_k(const SelArgs 
         h[c] = quad(w == 0 && a.h0 ? read_states(a.h0 + b * a.D * a.N, d, a.D, n0 + 4 * c, a.N) : make_float4(0.f, 0.f, 0.f, 0.f));
     }
 
-    Run<T, E> rx, rt, rz;
+    using R = Run<T, E, FULL>;
+    R rx, rt, rz;
+    const bool packed = R::packed(dr, a.D, vec);
     const int64_t t_first = w * S + row;
     const T* x = static_cast<const T*>(a.x) + b * a.sx[0] + t_first * a.sx[1] + dr;
     const T* dt = static_cast<const T*>(a.dt) + b * a.sdt[0] + t_first * a.sdt[1] + dr;
     const T* z = gated ? static_cast<const T*>(a.z) + b * a.sz[0] + t_first * a.sz[1] + dr : nullptr;
     auto ask = [&](int j) {  // of the warp's next slice
         const bool in = j * S + row < len;
-        rx.template read<FULL>(x, in, dr, a.D, vec);
-        rt.template read<FULL>(dt, in, dr, a.D, vec);
-        if (gated) rz.template read<FULL>(z, in, dr, a.D, vec);
+        rx.read(x, in, dr, a.D, vec);
+        rt.read(dt, in, dr, a.D, vec);
+        if (gated) rz.read(z, in, dr, a.D, vec);
         bc.ask(a, j * S, len, lane);
         x += W * S * a.sx[1];
         dt += W * S * a.sdt[1];
@@ -368,11 +370,11 @@ __global__ void __launch_bounds__(kSelFwdWarps * 32, 1) sel_fwd_k(const SelArgs 
         const int t0 = j * S;
         bc.take(a, t0, len, lane);
         const bool in = t0 + row < len;
-        const Run<T, E> kx = rx, kz = rz;  // for the outputs
+        const R kx = rx, kz = rz;  // for the outputs
         {
             float xs[E], s[E], bias[E];
-            rx.floats(xs);
-            rt.floats(s);
+            rx.floats(xs, packed);
+            rt.floats(s, packed);
             get_run<E>(bias, pars + cr);
 #pragma unroll
             for (int e = 0; e < E; ++e) {
@@ -455,10 +457,10 @@ __global__ void __launch_bounds__(kSelFwdWarps * 32, 1) sel_fwd_k(const SelArgs 
         __syncwarp();
         if (t0 + row < a.L) {
             float o[E], xs[E], g[E], skip[E];
-            kx.floats(xs);
+            kx.floats(xs, packed);
             get_run<E>(skip, pars + CW + cr);
             get_run<E>(o, yb + row * Sh::YS + cr);
-            if (gated) kz.floats(g);
+            if (gated) kz.floats(g, packed);
 #pragma unroll
             for (int e = 0; e < E; ++e) {
                 o[e] = fmaf(skip[e], xs[e], o[e]);
@@ -617,7 +619,8 @@ __global__ void __launch_bounds__(kSelBwdWarps * 32, 1) sel_bwd_k(const SelArgs 
     fence_mbar_init();
     __syncthreads();
 
-    Run<T, E> rx, rt, rz, rg;
+    using R = Run<T, E, FULL>;
+    R rx, rt, rz, rg;
     Quad hn;  // the checkpoint
     const T *px, *pt, *pz = nullptr, *pg;  // the lane's token and channels of the slice and group asked for next
     const float* pc;
@@ -634,10 +637,10 @@ __global__ void __launch_bounds__(kSelBwdWarps * 32, 1) sel_bwd_k(const SelArgs 
     auto ask = [&] {
         const int o = ng * CW, d = base + o + sub;
         const bool in = nj * S + row < len && reads;
-        rx.template read<FULL>(px + o, in, d, a.D, vec);
-        rt.template read<FULL>(pt + o, in, d, a.D, vec);
-        if (gated) rz.template read<FULL>(pz + o, in, d, a.D, vec);
-        rg.template read<FULL>(pg + o, in, d, a.D, vec);
+        rx.read(px + o, in, d, a.D, vec);
+        rt.read(pt + o, in, d, a.D, vec);
+        if (gated) rz.read(pz + o, in, d, a.D, vec);
+        rg.read(pg + o, in, d, a.D, vec);
         hn = FULL || base + o + ch < a.D ? *reinterpret_cast<const Quad*>(pc + static_cast<int64_t>(o) * NP) : quad(make_float4(0.f, 0.f, 0.f, 0.f));
         if (++ng == G) {
             ng = 0;
@@ -666,10 +669,11 @@ __global__ void __launch_bounds__(kSelBwdWarps * 32, 1) sel_bwd_k(const SelArgs 
         for (int g = 0; g < G; ++g) {
             const int d = base + g * CW + sub, dc = base + g * CW + ch, wg = w * G + g;
             float xs[E], ss[E], slope[E], dof[E], dzf[E];
-            rx.floats(xs);
-            rt.floats(ss);
-            rg.floats(dof);
-            if (gated) rz.floats(dzf);
+            const bool packed = R::packed(d, a.D, vec);
+            rx.floats(xs, packed);
+            rt.floats(ss, packed);
+            rg.floats(dof, packed);
+            if (gated) rz.floats(dzf, packed);
 #pragma unroll
             for (int e = 0; e < E; ++e) {
                 const float raw = ss[e] + pars[g * CW + (reads ? sub : 0) + e];
