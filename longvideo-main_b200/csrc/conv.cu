@@ -12,8 +12,8 @@
 // registers as pairs.  A CTA's four warps lie side by side.  Through registers the same loads left too few threads: the
 // forward took 67 us at B=4 L=16384 D=1024 bfloat16 and takes 55 (41 for its bytes), the backward at B=8 L=8192 D=768 127
 // and 75 (46).  What is left is latency and issue: two special functions and 15 instructions a value forward, 30 backward,
-// at half of the issue slots.  Runs are as long as gives every multiprocessor its warps once.  Rows that do not start on
-// 16 bytes take kernels of one channel a thread.
+// at half of the issue slots.  Runs are as long as gives every multiprocessor its warps once.  Rows of an even number of
+// channels that do not start on 16 bytes are copied 4 bytes at a time; odd ones take kernels of one channel a thread.
 // The backward takes p again from x (the forward saves nothing) and keeps dweight and dbias of its run in registers: a run's
 // is one partial row, and a second kernel adds them in order (no atomics: the same inputs give the same bits).
 #include <algorithm>
@@ -366,10 +366,11 @@ __global__ void __launch_bounds__(32 * kConvRuns) conv_bwd_any_k(const ConvArgs 
 constexpr int kConvU = 8, kConvStages = 4;  // tokens a stage; stages a warp
 constexpr int kConvTiles = 4;               // warps of a CTA, side by side: rows of 512 bytes (float32: 1024) at a time
 
-// A warp's stages of N inputs: rows of 64 channels, copied 16 bytes a lane; what lies behind `end` is not read.
-template <typename T, int N>
+// A warp's stages of N inputs: rows of 64 channels, copied in pieces of PIECE bytes (16, or 4 where rows are only so
+// aligned); tokens from `left` on and channels from `width` on are not read.
+template <typename T, int N, int PIECE>
 struct ConvStages {
-    static constexpr int kRow = 64, kPieces = kRow * sizeof(T) / 16;  // 16-byte pieces a row
+    static constexpr int kRow = 64, kEach = PIECE / sizeof(T), kPieces = kRow / kEach;  // elements a piece, pieces a row
     static constexpr size_t kBytes = static_cast<size_t>(kConvStages) * N * kConvU * kRow * sizeof(T);
     T* mem;
     __device__ __forceinline__ T* row(int stage, int n, int u) const { return mem + ((stage * N + n) * kConvU + u) * kRow; }
@@ -379,8 +380,11 @@ struct ConvStages {
         for (int n = 0; n < N; ++n)
 #pragma unroll
             for (int i = 0; i < kConvU * kPieces / 32; ++i) {
-                const int u = (i * 32 + lane) / kPieces, q = (i * 32 + lane) % kPieces * (16 / static_cast<int>(sizeof(T)));
-                if (u < left && q < width) cp_async16(row(stage, n, u) + q, src[n] + u * stride[n] + q, true);
+                const int u = (i * 32 + lane) / kPieces, q = (i * 32 + lane) % kPieces * kEach;
+                if (u < left && q < width) {
+                    if constexpr (PIECE == 16) cp_async16(row(stage, n, u) + q, src[n] + u * stride[n] + q, true);
+                    else cp_async4(row(stage, n, u) + q, src[n] + u * stride[n] + q, true);
+                }
             }
         cp_async_commit();
     }
@@ -391,12 +395,12 @@ struct ConvStages {
     }
 };
 
-template <typename T, int W>
+template <typename T, int W, int PIECE>
 __global__ void __launch_bounds__(32 * kConvTiles) conv_fwd_k(const ConvArgs a) {
     using V = RowVec<T, 2>;
     extern __shared__ __align__(16) unsigned char smem[];
     const int lane = threadIdx.x & 31, wid = threadIdx.x >> 5, c0 = (blockIdx.x * kConvTiles + wid) * 64, c = c0 + lane * 2;
-    const ConvStages<T, 1> st{reinterpret_cast<T*>(smem + wid * ConvStages<T, 1>::kBytes)};
+    const ConvStages<T, 1, PIECE> st{reinterpret_cast<T*>(smem + wid * ConvStages<T, 1, PIECE>::kBytes)};
     const int64_t r = blockIdx.y;
     if (c0 >= a.D) return;
     const int64_t b = r / a.runs, len = conv_length(a, b);
@@ -441,12 +445,12 @@ __global__ void __launch_bounds__(32 * kConvTiles) conv_fwd_k(const ConvArgs a) 
     if (a.hN && t0 == 0) conv_final<T, 2, W>(a, x + lane * 2, b, len, c);
 }
 
-template <typename T, int W>
+template <typename T, int W, int PIECE>
 __global__ void __launch_bounds__(32 * kConvTiles) conv_bwd_k(const ConvArgs a) {
     using V = RowVec<T, 2>;
     extern __shared__ __align__(16) unsigned char smem[];
     const int lane = threadIdx.x & 31, wid = threadIdx.x >> 5, c0 = (blockIdx.x * kConvTiles + wid) * 64, c = c0 + lane * 2;
-    const ConvStages<T, 2> st{reinterpret_cast<T*>(smem + wid * ConvStages<T, 2>::kBytes)};
+    const ConvStages<T, 2, PIECE> st{reinterpret_cast<T*>(smem + wid * ConvStages<T, 2, PIECE>::kBytes)};
     const int64_t r = blockIdx.y;
     const bool live = c < a.D;
     ConvBwd<T, 2, W> f;
@@ -555,35 +559,47 @@ dim3 conv_grid_any(const ConvArgs& a) {
     return dim3((a.D + 31) / 32, static_cast<unsigned>((a.rows * a.runs + kConvRuns - 1) / kConvRuns));
 }
 
+template <typename T, int W, int PIECE>
+cudaError_t conv_fwd_staged(ConvArgs& a, cudaStream_t s) {
+    constexpr size_t smem = kConvTiles * ConvStages<T, 1, PIECE>::kBytes;
+    static const int per = row_resident(conv_fwd_k<T, W, PIECE>, 32 * kConvTiles, smem);
+    conv_runs(a, (a.D + 63) / 64, per * kConvTiles);
+    conv_fwd_k<T, W, PIECE><<<conv_grid(a), 32 * kConvTiles, smem, s>>>(a);
+    note_launch();
+    return cudaGetLastError();
+}
+template <typename T, int W, int PIECE>
+cudaError_t conv_bwd_staged(const ConvArgs& a, cudaStream_t s) {
+    constexpr size_t smem = kConvTiles * ConvStages<T, 2, PIECE>::kBytes;
+    const cudaError_t e = cudaFuncSetAttribute(conv_bwd_k<T, W, PIECE>, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
+    if (e != cudaSuccess) return e;
+    conv_bwd_k<T, W, PIECE><<<conv_grid(a), 32 * kConvTiles, smem, s>>>(a);
+    note_launch();
+    return cudaGetLastError();
+}
+// piece: the bytes that the staged kernels may copy at once, or 0
 template <typename T, int W>
-cudaError_t conv_fwd_launch(ConvArgs& a, bool staged, cudaStream_t s) {
-    if (staged) {
-        constexpr size_t smem = kConvTiles * ConvStages<T, 1>::kBytes;
-        static const int per = row_resident(conv_fwd_k<T, W>, 32 * kConvTiles, smem);
-        conv_runs(a, (a.D + 63) / 64, per * kConvTiles);
-        conv_fwd_k<T, W><<<conv_grid(a), 32 * kConvTiles, smem, s>>>(a);
-    } else {
-        constexpr int threads = 32 * kConvRuns;
-        static const int per = row_resident(conv_fwd_any_k<T, W, 8>, threads, 0);
-        conv_runs(a, (a.D + 31) / 32, per * kConvRuns);
-        conv_fwd_any_k<T, W, 8><<<conv_grid_any(a), threads, 0, s>>>(a);
-    }
+cudaError_t conv_fwd_launch(ConvArgs& a, int piece, cudaStream_t s) {
+    if (piece == 16) return conv_fwd_staged<T, W, 16>(a, s);
+    if (piece == 4) return conv_fwd_staged<T, W, 4>(a, s);
+    constexpr int threads = 32 * kConvRuns;
+    static const int per = row_resident(conv_fwd_any_k<T, W, 8>, threads, 0);
+    conv_runs(a, (a.D + 31) / 32, per * kConvRuns);
+    conv_fwd_any_k<T, W, 8><<<conv_grid_any(a), threads, 0, s>>>(a);
     note_launch();
     return cudaGetLastError();
 }
 template <typename T, int W>
-cudaError_t conv_bwd_launch(ConvArgs& a, bool staged, void* dweight, void* dbias, cudaStream_t s) {
-    const int64_t rows = conv_bwd_rows(a, staged);
-    if (staged) {
-        constexpr size_t smem = kConvTiles * ConvStages<T, 2>::kBytes;
-        const cudaError_t e = cudaFuncSetAttribute(conv_bwd_k<T, W>, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
-        if (e != cudaSuccess) return e;
-        conv_bwd_k<T, W><<<conv_grid(a), 32 * kConvTiles, smem, s>>>(a);
+cudaError_t conv_bwd_launch(ConvArgs& a, int piece, void* dweight, void* dbias, cudaStream_t s) {
+    const int64_t rows = conv_bwd_rows(a, piece != 0);
+    cudaError_t e;
+    if (piece) {
+        e = piece == 16 ? conv_bwd_staged<T, W, 16>(a, s) : conv_bwd_staged<T, W, 4>(a, s);
     } else {
         conv_bwd_any_k<T, W, 4><<<conv_grid_any(a), 32 * kConvRuns, 0, s>>>(a);
+        note_launch();
+        e = cudaGetLastError();
     }
-    note_launch();
-    cudaError_t e = cudaGetLastError();
     if (e != cudaSuccess || !a.part) return e;
     RowSums r{};
     r.part = a.part, r.rows = static_cast<int>(rows), r.stride = static_cast<int64_t>(a.D) * (W + 1), r.dtype = a.w_dtype;
@@ -599,8 +615,8 @@ cudaError_t conv_step_launch(ConvArgs& a, cudaStream_t s) {
 }
 
 template <typename T>
-cudaError_t conv_fwd_any(ConvArgs& a, int width, bool staged, cudaStream_t s) {
-    return width == 2 ? conv_fwd_launch<T, 2>(a, staged, s) : width == 3 ? conv_fwd_launch<T, 3>(a, staged, s) : conv_fwd_launch<T, 4>(a, staged, s);
+cudaError_t conv_fwd_any(ConvArgs& a, int width, int piece, cudaStream_t s) {
+    return width == 2 ? conv_fwd_launch<T, 2>(a, piece, s) : width == 3 ? conv_fwd_launch<T, 3>(a, piece, s) : conv_fwd_launch<T, 4>(a, piece, s);
 }
 template <typename T, int VEC>
 cudaError_t conv_step_width(ConvArgs& a, int width, cudaStream_t s) {
@@ -611,10 +627,10 @@ cudaError_t conv_step_any(ConvArgs& a, int width, bool vec, cudaStream_t s) {
     return vec ? conv_step_width<T, 4>(a, width, s) : conv_step_width<T, 1>(a, width, s);
 }
 template <typename T>
-cudaError_t conv_bwd_any(ConvArgs& a, int width, bool staged, void* dw, void* db, cudaStream_t s) {
-    return width == 2   ? conv_bwd_launch<T, 2>(a, staged, dw, db, s)
-           : width == 3 ? conv_bwd_launch<T, 3>(a, staged, dw, db, s)
-                        : conv_bwd_launch<T, 4>(a, staged, dw, db, s);
+cudaError_t conv_bwd_any(ConvArgs& a, int width, int piece, void* dw, void* db, cudaStream_t s) {
+    return width == 2   ? conv_bwd_launch<T, 2>(a, piece, dw, db, s)
+           : width == 3 ? conv_bwd_launch<T, 3>(a, piece, dw, db, s)
+                        : conv_bwd_launch<T, 4>(a, piece, dw, db, s);
 }
 
 int conv_check(const char* fn, const EacsConv& p, bool single) {
@@ -635,7 +651,6 @@ ConvArgs conv_args(const EacsConv& p) {
     a.rows = p.rows, a.L = p.L, a.D = static_cast<int>(p.D), a.w_dtype = p.w_dtype, a.silu = p.silu;
     return a;
 }
-int conv_piece(const EacsConv& p) { return p.dtype == EACS_DTYPE_F32 ? 4 : 8; }  // elements of 16 bytes
 // Whether vectors of `n` elements may be moved at p and its strides (D of them a row).
 bool conv_vec(const EacsConv& p, int n, std::initializer_list<const void*> ptrs, std::initializer_list<int64_t> strides) {
     const uintptr_t bytes = static_cast<uintptr_t>(n) * (p.dtype == EACS_DTYPE_F32 ? 4 : 2);
@@ -645,6 +660,12 @@ bool conv_vec(const EacsConv& p, int n, std::initializer_list<const void*> ptrs,
     for (int64_t st : strides)
         if (st % n) return false;
     return true;
+}
+
+// What the staged kernels may copy at once: 16 bytes, or 4 where pairs of channels (which they write) are aligned at least.
+int conv_piece(const EacsConv& p, std::initializer_list<const void*> ptrs, std::initializer_list<int64_t> strides) {
+    if (conv_vec(p, p.dtype == EACS_DTYPE_F32 ? 4 : 8, ptrs, strides)) return 16;
+    return conv_vec(p, 2, ptrs, strides) ? 4 : 0;
 }
 
 }  // namespace
@@ -666,10 +687,10 @@ int conv_fwd(const EacsConv& p, void* y, void* final_state, cudaStream_t stream)
     a.y = y;
     a.hN = final_state;
     if (p.L == 0 && !final_state) return EACS_OK;
-    const bool vec = conv_vec(p, conv_piece(p), {p.x, y, p.initial_state, final_state}, {p.x_stride[0], p.x_stride[1]});
-    const cudaError_t e = p.dtype == EACS_DTYPE_F32   ? conv_fwd_any<float>(a, p.width, vec, stream)
-                          : p.dtype == EACS_DTYPE_F16 ? conv_fwd_any<__half>(a, p.width, vec, stream)
-                                                      : conv_fwd_any<__nv_bfloat16>(a, p.width, vec, stream);
+    const int piece = conv_piece(p, {p.x, y, p.initial_state, final_state}, {p.x_stride[0], p.x_stride[1]});
+    const cudaError_t e = p.dtype == EACS_DTYPE_F32   ? conv_fwd_any<float>(a, p.width, piece, stream)
+                          : p.dtype == EACS_DTYPE_F16 ? conv_fwd_any<__half>(a, p.width, piece, stream)
+                                                      : conv_fwd_any<__nv_bfloat16>(a, p.width, piece, stream);
     return cuda_check(e, fn);
 }
 
@@ -707,11 +728,11 @@ int conv_bwd(const EacsConv& p, const ConvGrads& g, void* ws, size_t ws_bytes, c
     a.dy = g.dy, a.dhN = g.dfinal, a.dx = g.dx, a.dh0 = g.dinitial;
     a.sdy[0] = g.dy_stride[0], a.sdy[1] = g.dy_stride[1];
     a.part = want ? static_cast<float*>(ws) : nullptr;
-    const bool vec = conv_vec(p, conv_piece(p), {p.x, p.initial_state, g.dy, g.dfinal, g.dx, g.dinitial},
-                              {p.x_stride[0], p.x_stride[1], g.dy_stride[0], g.dy_stride[1]});
-    const cudaError_t e = p.dtype == EACS_DTYPE_F32   ? conv_bwd_any<float>(a, p.width, vec, g.dweight, g.dbias, stream)
-                          : p.dtype == EACS_DTYPE_F16 ? conv_bwd_any<__half>(a, p.width, vec, g.dweight, g.dbias, stream)
-                                                      : conv_bwd_any<__nv_bfloat16>(a, p.width, vec, g.dweight, g.dbias, stream);
+    const int piece = conv_piece(p, {p.x, p.initial_state, g.dy, g.dfinal, g.dx, g.dinitial},
+                                 {p.x_stride[0], p.x_stride[1], g.dy_stride[0], g.dy_stride[1]});
+    const cudaError_t e = p.dtype == EACS_DTYPE_F32   ? conv_bwd_any<float>(a, p.width, piece, g.dweight, g.dbias, stream)
+                          : p.dtype == EACS_DTYPE_F16 ? conv_bwd_any<__half>(a, p.width, piece, g.dweight, g.dbias, stream)
+                                                      : conv_bwd_any<__nv_bfloat16>(a, p.width, piece, g.dweight, g.dbias, stream);
     return cuda_check(e, fn);
 }
 
