@@ -504,7 +504,10 @@ cudaError_t bn_fwd_any(const BnArgs& a, bool vec, cudaStream_t s) {
     if constexpr (RES)
         if (vec && !a.has_post) return a.gate ? bn_fwd_vec<T, RES, 1>(a, s) : bn_fwd_vec<T, RES, 0>(a, s);
     if (vec) return a.gate ? bn_fwd_vec<T, RES, 3>(a, s) : bn_fwd_vec<T, RES, 2>(a, s);
+    if (a.d <= 64) return bn_fwd_launch<T, 1, 8, 8, 32, RES, 4>(a, s);
+    if (a.d <= 128) return bn_fwd_launch<T, 1, 8, 16, 16, RES, 4>(a, s);
     if (a.d <= 256) return bn_fwd_launch<T, 1, 8, 32, 8, RES, 4>(a, s);
+    if (a.d <= 512) return bn_fwd_launch<T, 1, 8, 64, 4, RES, 4>(a, s);
     if (a.d <= 1024) return bn_fwd_launch<T, 1, 8, 128, 2, RES, 4>(a, s);
     if (a.d <= 4096) return bn_fwd_launch<T, 1, 8, 512, 1, RES, 4>(a, s);
     return bn_fwd_launch<T, 1, 16, 512, 1, RES, 4>(a, s);
@@ -514,7 +517,11 @@ cudaError_t bn_bwd_any(const BnArgs& a, bool vec, int* parts, cudaStream_t s) {
     if constexpr (RES)
         if (vec && !a.has_post) return a.gate ? bn_bwd_vec<T, RES, 1>(a, parts, s) : bn_bwd_vec<T, RES, 0>(a, parts, s);
     if (vec) return a.gate ? bn_bwd_vec<T, RES, 3>(a, parts, s) : bn_bwd_vec<T, RES, 2>(a, parts, s);
+    if (a.d <= 32) return bn_bwd_launch<T, 1, 4, 8, 32, RES, 4>(a, parts, s);
+    if (a.d <= 64) return bn_bwd_launch<T, 1, 4, 16, 16, RES, 4>(a, parts, s);
     if (a.d <= 128) return bn_bwd_launch<T, 1, 4, 32, 8, RES, 4>(a, parts, s);
+    if (a.d <= 256) return bn_bwd_launch<T, 1, 4, 64, 4, RES, 4>(a, parts, s);
+    if (a.d <= 512) return bn_bwd_launch<T, 1, 4, 128, 2, RES, 4>(a, parts, s);
     if (a.d <= 1024) return bn_bwd_launch<T, 1, 8, 128, 2, RES, 4>(a, parts, s);
     if (a.d <= 4096) return bn_bwd_launch<T, 1, 8, 512, 1, RES, 4>(a, parts, s);
     return bn_bwd_launch<T, 1, 16, 512, 1, RES, 4>(a, parts, s);
