@@ -127,6 +127,15 @@ def test_norms(rows, d, dtype, wdtype):
         check(i, rnd(rows, d).to(dtype), rnd(rows, d).to(dtype))
 
 
+@pytest.mark.parametrize("rows,d", [(1, 7), (300, 31), (33, 50), (1301, 63), (65, 127), (40, 190), (700, 255), (9, 411), (301, 509)])
+def test_narrow_rows_element_by_element(rows, d):
+    for k, kw in enumerate([dict(gate=True, scale=True, post=True), dict(scale=True)]):
+        i, rnd = inputs((rows, d), F16, F32, "residual", k, **kw)
+        check(i, rnd(rows, d).half(), rnd(rows, d).half())
+    i, rnd = inputs((rows, d), BF16, BF16, "gated", 3, gate=True)
+    check(i, rnd(rows, d).bfloat16(), None)
+
+
 def test_heads_views_and_broadcast():
     i, rnd = inputs((2, 7, 3, 96), BF16, BF16, "gated", 1, gate=True)  # (B, L, heads, V): each head by itself
     check(i, rnd(2, 7, 3, 96).bfloat16(), None)

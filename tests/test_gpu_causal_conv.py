@@ -116,6 +116,16 @@ def test_forward_and_gradients(b, L, D, W, dtype, wdtype):
         check(i, rnd(b, L, D).to(dtype), rnd(b, W - 1, D).to(dtype) if k else None)
 
 
+@pytest.mark.parametrize("L,D,W", [(70, 50, 4), (40, 98, 3), (300, 6, 4), (33, 202, 2), (9, 2, 4)])
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+def test_even_rows_and_offsets(L, D, W, dtype):
+    i, rnd = inputs(3, L, D, W, dtype, F32, 7, ragged=True, initial=True)  # rows aligned to pairs of channels only
+    check(i, rnd(3, L, D).to(dtype), rnd(3, W - 1, D).to(dtype))
+    wide = rnd(3, L, 2 * D + 6).to(dtype)
+    for at in (2, 1, 4, D + 6):  # aligned to pairs, and not
+        check({**i, "x": wide[..., at:at + D]}, wide.flip(1)[..., at:at + D])
+
+
 @pytest.mark.parametrize("b,D,W,dtype", [(1, 1, 2, F32), (3, 40, 4, BF16), (2, 33, 3, F16), (300, 512, 4, BF16), (2, 6, 4, F32)])
 def test_step(b, D, W, dtype):
     for kw in (dict(), dict(bias=False, activation=None)):
