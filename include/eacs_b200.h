@@ -188,7 +188,8 @@ EACS_API int eacs_delta_step(const EacsDelta* p, void* o, float* final_state, vo
  * the state stays.  initial_state (rows,D,N) float32 dense or NULL (zeros).
  * N goes up to 64.  Sums and states are float32; A <= 0 and s >= 0 are meant
  * (states that grow do so as float32 lets them).  Rows that start on 16 bytes
- * are read several channels at a time. */
+ * are read several channels at a time.  Outputs overlap neither one another nor
+ * the inputs (a step's state apart; EacsConv and EacsNorm likewise). */
 typedef struct EacsSelective {
     const void* x;
     const void* dt;
