@@ -36,7 +36,7 @@
 namespace eacs {
 namespace {
 
-constexpr float kLog2e = 1.44269504f, kLn2 = 0.693147181f;
+constexpr float kLog2e = 1.44269504f, kLog2eLow = 1.92596303e-8f, kLn2 = 0.693147181f;  // (log2(e) is the first two's sum)
 
 __device__ __forceinline__ float both(f32x2 v) {
     float a, b;
@@ -61,12 +61,15 @@ __device__ __forceinline__ f32x2 decays(f32x2 s2, f32x2 A) { return ex2_pair(fma
 // ---- a token's step and gate ----------------------------------------------------------------------------
 // softplus(v) = max(v, 0) + log(1 + u) with u = e^-|v| and log(1 + u) = 2 artanh(q), q = u / (2 + u) <= 1/3: relatively
 // exact for the small steps that v << 0 gives, where log(1 + u) taken from the rounded 1 + u is not.  2 artanh(q) / q is a
-// polynomial of degree 4 in q^2, fitted on [0, 1/9] at Chebyshev's points (8e-9 of the value).  u's argument is put right
-// for its rounding to first order (without that u is off by |v| 2^-24); below e^-87 u stays there.  slope is the derivative.
+// polynomial of degree 4 in q^2, fitted on [0, 1/9] at Chebyshev's points (8e-9 of the value).  What u's argument lost, the
+// product's rounding and that of log2(e), is put back to first order (without the first u is off by |v| 2^-24, without the
+// second by |v| 2^-26): 2^-20 of the step in all.  Behind e^-87, where float32's normal numbers end, u is 0, so that -inf or
+// the lowest value in dt masks a token: it takes no step.  slope is the derivative.
 __device__ __forceinline__ float softplus(float v, float& slope) {
-    const float t = fmaxf(-fabsf(v), -87.0f), p0 = t * kLog2e;
+    const float t = -fabsf(v), p0 = t * kLog2e;
     float u = ex2_approx(p0);
-    u = fmaf(u * fmaf(t, kLog2e, -p0), kLn2, u);
+    u = fmaf(u * fmaf(t, kLog2eLow, fmaf(t, kLog2e, -p0)), kLn2, u);
+    u = t < -87.0f ? 0.0f : u;
     const float q = __fdividef(u, 2.0f + u), q2 = q * q;
     float p = fmaf(q2, 0.2817465663f, 0.2796141803f);
     p = fmaf(q2, p, 0.4002485275f);

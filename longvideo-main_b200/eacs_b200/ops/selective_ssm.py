@@ -136,7 +136,9 @@ def selective_ssm(x: Tensor, dt: Tensor, A: Tensor, B: Tensor, C: Tensor, skip: 
     """y (B, L, D) in x's dtype; with output_final_state also the state
     (B, D, N) float32 behind the last token.
 
-    softplus=False takes dt (+ dt_bias) itself as the step.  lengths (B) int32
+    softplus=False takes dt (+ dt_bias) itself as the step; a softplus below
+    e^-87 is 0, so that -inf or the dtype's lowest value in dt masks a token (its
+    channel keeps its state).  lengths (B) int32
     on the device: row b has lengths[b] tokens (clamped to 0..L); what lies
     behind is not read, its outputs and gradients are 0.  Differentiable in
     every floating point input, through y and the final state."""
