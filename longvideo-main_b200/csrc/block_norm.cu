@@ -38,8 +38,6 @@ struct BnArgs {
     float eps;
 };
 
-__device__ __forceinline__ float bn_sigmoid(float v) { return __fdividef(1.0f, 1.0f + ex2_approx(v * -1.44269504f)); }
-
 // One row of an input: VPL vectors a thread, as they lie in memory (whole registers), taken apart where they are used.
 template <typename T, int VEC, int VPL, int TPR>
 struct BnRow {
@@ -146,7 +144,7 @@ __global__ void __launch_bounds__(TPR * RPC) bn_fwd_k(const BnArgs a) {
 #pragma unroll
                 for (int e = 0; e < VEC; ++e) {
                     const float v = g.at(k, e);
-                    u[k][e] *= v * bn_sigmoid(v);
+                    u[k][e] *= v * sigmoid(v);
                 }
         T* y = static_cast<T*>(a.y) + row * a.d;
         if constexpr (!RES) {
@@ -317,7 +315,7 @@ __global__ void __launch_bounds__(TPR * RPC, bn_bwd_min(TPR * RPC, HOW)) bn_bwd_
         auto gain = [&](int k, int e) {
             if (!gated) return 1.f;
             const float q = g.at(k, e);
-            return q * bn_sigmoid(q);
+            return q * sigmoid(q);
         };
         float v[VPL][VEC];
         if constexpr (RES) {
@@ -368,8 +366,8 @@ __global__ void __launch_bounds__(TPR * RPC, bn_bwd_min(TPR * RPC, HOW)) bn_bwd_
                 if (normed) post.get(p, k, t);
 #pragma unroll
                 for (int e = 0; e < VEC; ++e) {
-                    const float q = g.at(k, e), sg = bn_sigmoid(q);
-                    o[e] = v[k][e] * before(k, e, p) * (sg * fmaf(q, 1.f - sg, 1.f));
+                    const float q = g.at(k, e), sg = sigmoid(q);
+                    o[e] = v[k][e] * before(k, e, p) * silu_slope(q, sg);
                     v[k][e] *= q * sg;
                 }
                 if (i0 < dl) bn_write<T, VEC>(static_cast<T*>(a.dgate) + row * a.d + i0, o);

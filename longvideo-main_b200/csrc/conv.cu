@@ -53,9 +53,6 @@ __device__ __forceinline__ int64_t conv_length(const ConvArgs& a, int64_t b) {
     return n < 0 ? 0 : (n > a.L ? a.L : n);
 }
 
-// sigmoid(v) = 1 / (1 + e^-v)
-__device__ __forceinline__ float conv_sigmoid(float v) { return __fdividef(1.0f, 1.0f + ex2_approx(v * -1.44269504f)); }
-
 template <typename T, int VEC>
 __device__ __forceinline__ void conv_floats(float* v, const RowVec<T, VEC>& r) {
     if constexpr (VEC > 1 && sizeof(T) == 2) {  // two to a register
@@ -178,7 +175,7 @@ struct ConvFwd {
         cols.dot(p, win);
         if (silu)
 #pragma unroll
-            for (int e = 0; e < VEC; ++e) p[e] *= conv_sigmoid(p[e]);
+            for (int e = 0; e < VEC; ++e) p[e] *= sigmoid(p[e]);
         conv_write<T, VEC>(y, p);
     }
 };
@@ -221,10 +218,7 @@ struct ConvBwd {
         if (silu) {
             cols.dot(p, win);
 #pragma unroll
-            for (int e = 0; e < VEC; ++e) {
-                const float s = conv_sigmoid(p[e]);
-                g[e] *= s * fmaf(p[e], 1.f - s, 1.f);
-            }
+            for (int e = 0; e < VEC; ++e) g[e] *= silu_slope(p[e], sigmoid(p[e]));
         }
         dp[W - 1].set(g);
         if (mine)
@@ -532,7 +526,7 @@ __global__ void __launch_bounds__(128) conv_step_k(const ConvArgs a) {
     cols.dot(p, win);
     if (a.silu)
 #pragma unroll
-        for (int e = 0; e < VEC; ++e) p[e] *= conv_sigmoid(p[e]);
+        for (int e = 0; e < VEC; ++e) p[e] *= sigmoid(p[e]);
     conv_write<T, VEC>(static_cast<T*>(a.y) + b * a.D + c, p);
 #pragma unroll
     for (int k = 0; k < W - 1; ++k) *reinterpret_cast<RowVec<T, VEC>*>(h + static_cast<int64_t>(k) * a.D) = raw[k + 1];

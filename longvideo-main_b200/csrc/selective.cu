@@ -36,8 +36,6 @@
 namespace eacs {
 namespace {
 
-constexpr float kLog2e = 1.44269504f, kLog2eLow = 1.92596303e-8f, kLn2 = 0.693147181f;  // (log2(e) is the first two's sum)
-
 __device__ __forceinline__ float both(f32x2 v) {
     float a, b;
     halves(v, a, b);
@@ -79,7 +77,6 @@ __device__ __forceinline__ float softplus(float v, float& slope) {
     slope = v >= 0.0f ? inv : u * inv;
     return fmaf(q, p, v < 0.0f ? 0.0f : v);  // (a NaN stays one)
 }
-__device__ __forceinline__ float sigmoid(float v) { return __fdividef(1.0f, 1.0f + ex2_approx(v * -kLog2e)); }
 
 struct SelArgs {
     const void *x, *dt, *z, *B, *C;      // z may be null
@@ -687,7 +684,7 @@ __global__ void __launch_bounds__(kSelBwdWarps * 32, 1) sel_bwd_k(const SelArgs 
                 if (gated) {
                     const float zv = dzf[e], sg = sigmoid(zv), g0 = dof[e];
                     dof[e] = g0 * (zv * sg);
-                    dzf[e] = g0 * sg * fmaf(zv, 1.f - sg, 1.f);
+                    dzf[e] = g0 * silu_slope(zv, sg);
                 }
                 if (reads) {
                     const float sl = ss[e] * kLog2e, v = ss[e] * xs[e];
