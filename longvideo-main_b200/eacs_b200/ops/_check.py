@@ -77,6 +77,15 @@ def dense(t: torch.Tensor | None) -> torch.Tensor | None:
     return None if t is None else t.contiguous()
 
 
+def packed(t: torch.Tensor | None) -> torch.Tensor | None:
+    """A saved tensor as a kernel that reads it by its pointer alone expects it: dense and on 16 bytes.  (Saved-tensor hooks
+    may give back a copy that is neither.)"""
+    if t is None:
+        return None
+    t = t.contiguous()
+    return t.clone() if t.data_ptr() % 16 else t
+
+
 def new_like(t: torch.Tensor | None) -> torch.Tensor | None:
     """An uninitialised dense tensor of t's shape, dtype and device."""
     return None if t is None else torch.empty_like(t, memory_format=torch.contiguous_format)

@@ -28,7 +28,7 @@ import torch
 from torch import Tensor
 
 from .. import _lib
-from ._check import cuda_tensors, require
+from ._check import cuda_tensors, packed, require
 from .eacs_gated_scan import prepare, workspace_bytes
 
 
@@ -173,7 +173,7 @@ class CellCommitsFunction(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, g_ys, g_gs, g_rs, g_ch, g_ct, g_cu, g_cB, g_cC):
-        gs, rs, stats = ctx.saved_tensors
+        gs, rs, stats = map(packed, ctx.saved_tensors)
         lam_c, log_c, u_c, B_c, C_c, t_c, D_c, m_c, v_c = ctx.prep
         eps_v, T, eta, var_eps, dt_init, dt_max = ctx.hp
         dev = u_c.device

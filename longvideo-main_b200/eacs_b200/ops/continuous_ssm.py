@@ -18,7 +18,7 @@ import torch
 from torch import Tensor
 
 from .. import _lib
-from ._check import cuda_tensors, require
+from ._check import cuda_tensors, packed, require
 
 DT_MIN = 1e-3  # effective_dt defaults (ops/discretization.py:67-68)
 DT_MAX = 1e3
@@ -111,7 +111,7 @@ class SSMCoreFunction(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, gy):
-        saved = ctx.saved_tensors
+        saved = [packed(t) for t in ctx.saved_tensors]
         prep = saved[:7]
         if not ctx.has_ckpt:  # empty input
             return (None,) * 9

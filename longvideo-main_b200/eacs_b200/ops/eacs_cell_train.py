@@ -16,7 +16,7 @@ import torch
 from torch import Tensor
 
 from .. import _lib
-from ._check import cuda_tensors, require
+from ._check import cuda_tensors, packed, require
 from .eacs_gated_scan import prepare, workspace_bytes
 
 
@@ -118,7 +118,7 @@ class GatedEACSCellFunction(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, g_ys, g_gs, g_rs, g_ns):
-        gs, rs, stats = ctx.saved_tensors
+        gs, rs, stats = map(packed, ctx.saved_tensors)
         eps_v, T, eta, var_eps, dt_init, dt_max = ctx.hp
         du, dBc, dCc, dt, dlam, dlog, dD, deps = _train_bwd(
             ctx.prep, gs, rs, stats, eps_v, T, eta, var_eps, dt_init, dt_max, g_ys, g_gs, g_rs, g_ns,

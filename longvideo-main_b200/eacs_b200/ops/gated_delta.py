@@ -42,7 +42,7 @@ import torch
 from torch import Tensor
 
 from .. import _lib
-from ._check import dense_last, on, one_device, require_plain
+from ._check import dense_last, on, one_device, packed, require_plain
 
 MAX_K = 128
 MAX_V = 1024
@@ -130,7 +130,7 @@ class GatedDeltaFunction(torch.autograd.Function):
             do = do.clone()
         dfinal = None if dfinal is None else dfinal.contiguous()
         q, k, v = dense_last(q), dense_last(k), dense_last(v)
-        lengths, initial = (None if t is None else t.contiguous() for t in (lengths, initial))
+        lengths, initial, ws = packed(lengths), packed(initial), packed(ws)
         L_ = _lib.lib()
         p = _args(q, k, v, g, beta, ctx.scale, lengths, initial, ctx.path)
         need = int(L_.eacs_delta_bwd_workspace_size(p))

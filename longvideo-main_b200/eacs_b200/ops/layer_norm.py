@@ -21,7 +21,7 @@ import torch
 from torch import Tensor, nn
 
 from .. import _lib
-from ._check import is_plain, on, one_device, require_plain
+from ._check import is_plain, on, one_device, packed, require_plain
 
 MAX_D = 8192
 
@@ -85,6 +85,7 @@ class LayerNormFunction(torch.autograd.Function):
             ds, dw, db = _recorded_gradients(x, weight, residual, dy, ctx.eps)
             return (ds if need_x else None, dw.to(wd) if need_w else None, db.to(wd) if need_b else None, None,
                     ds if need_r else None, None)
+        weight = packed(weight)
         dw = torch.empty(d, dtype=wd, device=dev) if need_w else None
         db = torch.empty(d, dtype=wd, device=dev) if need_b else None
         dx = torch.empty(x.shape, dtype=x.dtype, device=dev)

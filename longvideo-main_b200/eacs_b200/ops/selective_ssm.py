@@ -35,7 +35,7 @@ import torch
 from torch import Tensor
 
 from .. import _lib
-from ._check import dense, dense_last, new_like, on, once, one_device, require_plain, wants_grad
+from ._check import dense, dense_last, new_like, on, once, one_device, packed, require_plain, wants_grad
 
 MAX_N = 64
 
@@ -113,6 +113,7 @@ class SelectiveSSMFunction(torch.autograd.Function):
         # hooks may give saved tensors back in another layout
         x, dt, B, C, z = dense_last(x), dense_last(dt), dense_last(B), dense_last(C), dense_last(z)
         A, skip, dt_bias, lengths, initial = dense(A), dense(skip), dense(dt_bias), dense(lengths), dense(initial)
+        ck = packed(ck)
         dy = torch.zeros(x.shape, dtype=x.dtype, device=dev) if dy is None else dense_last(dy)
         dfinal = dense(dfinal)
         p = _args(x, dt, A, B, C, skip, z, dt_bias, ctx.softplus, lengths, initial)
