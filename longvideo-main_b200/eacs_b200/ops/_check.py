@@ -91,12 +91,29 @@ def new_like(t: torch.Tensor | None) -> torch.Tensor | None:
     return None if t is None else torch.empty_like(t, memory_format=torch.contiguous_format)
 
 
-def once(backward):
-    """torch's once_differentiable, whose cost only a backward with create_graph pays."""
-    recorded = torch.autograd.function.once_differentiable(backward)
+class _Once(torch.autograd.Function):
+    """Gradients as they are, behind the n tensors that they depend on, which may not be differentiated."""
 
+    @staticmethod
+    def forward(ctx, n, *tensors):
+        return tuple(None if g is None else g.view_as(g) for g in tensors[n:])
+
+    @staticmethod
+    def backward(ctx, *_):
+        raise RuntimeError("these gradients can be differentiated once only (create_graph is not supported here)")
+
+
+def once(backward):
+    """For a backward that cannot be differentiated itself: with create_graph its gradients are those of a plain backward, and
+    a backward through any of them raises.  (Left without a graph they would count as constants, and a penalty on them among
+    other terms would lose its gradient without a word.)  All inputs that may want a gradient have to be saved tensors."""
     def run(ctx, *grads):
-        return recorded(ctx, *grads) if torch.is_grad_enabled() else backward(ctx, *grads)
+        if not torch.is_grad_enabled():
+            return backward(ctx, *grads)
+        with torch.no_grad():
+            out = backward(ctx, *grads)
+        roots = [t for t in (*ctx.saved_tensors, *grads) if t is not None and t.requires_grad]
+        return _Once.apply(len(roots), *roots, *out)
     return run
 
 

@@ -42,7 +42,7 @@ import torch
 from torch import Tensor
 
 from .. import _lib
-from ._check import dense_last, on, one_device, packed, require_plain
+from ._check import dense_last, on, once, one_device, packed, require_plain
 
 MAX_K = 128
 MAX_V = 1024
@@ -119,7 +119,7 @@ class GatedDeltaFunction(torch.autograd.Function):
         return (o, final) if out_state else o
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
+    @once
     def backward(ctx, do, dfinal=None):
         q, k, v, g, beta, lengths, initial, ws = ctx.saved_tensors
         dev = ctx.dev
