@@ -34,6 +34,8 @@ MIN_WIDTH, MAX_WIDTH = 2, 4
 
 def _check(name, x, weight, bias, activation, lengths, state, lead):
     """Device of the arguments; lead: the dimensions in front of the channels."""
+    if weight is None or (lead == 1 and state is None):
+        raise RuntimeError(f"{name}: expects tensors for x{' and the weight' if lead == 2 else ', the weight and the state'}")
     dev = one_device(name, x, weight, bias, lengths, state)
     require_plain(name, x, weight, bias, state)
     xs = x.shape

@@ -50,6 +50,8 @@ MAX_V = 1024
 
 def _check(name, q, k, v, g, beta, lengths, state, lead):
     """Device of the arguments; lead: the dimensions in front of the head's."""
+    if k is None or v is None or g is None or beta is None or (lead == 1 and state is None):
+        raise RuntimeError(f"{name}: expects tensors for q, k, v, g{' and beta' if lead == 2 else ', beta and the state'}")
     dev = one_device(name, q, k, v, g, beta, lengths, state)
     require_plain(name, q, k, v, g, beta, state)
     qs, vs, dt = q.shape, v.shape, q.dtype

@@ -41,12 +41,14 @@ MAX_N = 64
 
 
 def _check(name, x, dt, A, B, C, skip, z, dt_bias, lengths, state):
+    lead = 1 if name.endswith("step") else 2
+    if dt is None or A is None or B is None or C is None or (lead == 1 and state is None):
+        raise RuntimeError(f"{name}: expects tensors for x, dt, A, B{' and C' if lead == 2 else ', C and the state'}")
     dev = one_device(name, x, dt, A, B, C, skip, z, dt_bias, lengths, state)
     require_plain(name, x, dt, A, B, C, skip, z, dt_bias, state)
     xs, ty = x.shape, x.dtype
     if ty not in _lib.DTYPE_CODES or dt.dtype != ty or B.dtype != ty or C.dtype != ty or (z is not None and z.dtype != ty):
         raise RuntimeError(f"{name}: x, dt, B, C and z must have one dtype, float32, float16 or bfloat16")
-    lead = 1 if name.endswith("step") else 2
     if len(xs) != lead + 1 or dt.shape != xs or (z is not None and z.shape != xs):
         raise RuntimeError(f"{name}: x, dt and z must have one shape of {lead + 1} dimensions")
     if A.dim() != 2 or A.shape[0] != xs[-1] or A.dtype != torch.float32:
