@@ -20,7 +20,8 @@
 // Measured, us: forward B=4 L=16384 D=1024 N=16 bfloat16 637; B=1 322; B=8 L=8192 D=768 485 (528 with checkpoints), the
 // backward of that 1364 and 28 for the sums of dB and dC.  What holds it off the exponentials' time is latency: 12 warps a
 // multiprocessor (backward 8) with the registers that a slice's decays and sums take, at 12 (backward 26) instructions for
-// 32 updates; the special function pipe is 45 percent busy, issue slots 52 percent (backward 18 and 47).  Tried and slower:
+// 32 updates; the special function pipe is 45 percent busy, issue slots 59 percent (backward 18 and 47).  The backward's kernels for one
+// group a CTA spill registers for N <= 8 (116 to 168 bytes a thread; others at most 72, the forward's at most 24).  Tried and slower:
 // slices of 4 tokens with 16 or 20 warps (813 and 894 us where 8 with 12 took 745), in the backward slices of 4 with two
 // channels a thread and 12 warps (half the shared memory reads, but half again as many instructions: 2477 us a training step
 // where 1971 was), and the tokens' values of all of a CTA's groups worked out at once (2180 where 1900 was).
@@ -61,13 +62,13 @@ __device__ __forceinline__ f32x2 decays(f32x2 s2, f32x2 A) { return ex2_pair(fma
 // exact for the small steps that v << 0 gives, where log(1 + u) taken from the rounded 1 + u is not.  2 artanh(q) / q is a
 // polynomial of degree 4 in q^2, fitted on [0, 1/9] at Chebyshev's points (8e-9 of the value).  What u's argument lost, the
 // product's rounding and that of log2(e), is put back to first order (without the first u is off by |v| 2^-24, without the
-// second by |v| 2^-26): 2^-20 of the step in all.  Behind e^-87, where float32's normal numbers end, u is 0, so that -inf or
-// the lowest value in dt masks a token: it takes no step.  slope is the derivative.
+// second by |v| 2^-26): 2^-20 of the step in all.  Behind e^-87, where float32's normal numbers end, the hardware's 2^v is 0
+// (v is held to where the argument's rest is a number), so that -inf or the lowest value in dt masks a token: it takes no step.
+// slope is the derivative.
 __device__ __forceinline__ float softplus(float v, float& slope) {
-    const float t = -fabsf(v), p0 = t * kLog2e;
+    const float t = fmaxf(-fabsf(v), -200.0f), p0 = t * kLog2e;
     float u = ex2_approx(p0);
     u = fmaf(u * fmaf(t, kLog2eLow, fmaf(t, kLog2e, -p0)), kLn2, u);
-    u = t < -87.0f ? 0.0f : u;
     const float q = __fdividef(u, 2.0f + u), q2 = q * q;
     float p = fmaf(q2, 0.2817465663f, 0.2796141803f);
     p = fmaf(q2, p, 0.4002485275f);
@@ -480,7 +481,9 @@ __global__ void __launch_bounds__(kSelFwdWarps * 32, 1) sel_fwd_k(const SelArgs 
 // ---------------------------------------------------------------------------------------------------------
 // single tokens
 // ---------------------------------------------------------------------------------------------------------
-// LN threads a channel with four states each, R rows a thread (A is read once for them).
+// LN threads a channel with four states each, R rows a thread (A is read once for them).  64 rows of 2048 channels with N=16:
+// 8.9 us where the bytes take 2.8.  A thread moves one vector of states and for it reads A, B, C and the channel's values
+// element by element: 17 loads in all, whose issue and latency is the difference.
 template <typename T, int LN, int R>
 __global__ void __launch_bounds__(256) sel_step_k(const SelArgs a) {
     const int i = blockIdx.x * 256 + threadIdx.x;
@@ -575,7 +578,8 @@ constexpr int kSelBwdWarps = 8, kSelBwdMaxGroups = 8;
 // FULL: groups of CW channels and rows of NP states, all of them on 16 bytes.  AHEAD: what is handed on is worked out
 // before the sweep that needs what is handed in (the slice's own end and the product of its decays, as in the forward): with
 // one group a CTA nothing else fills the ring's wait (B=1 L=8192 D=768 training step 643 to 546 us); with more the other
-// groups do, and the extra products cost (B=8: 1900 us without, 2003 with; two groups, B=2: 741 and 765).
+// groups do, and the extra products cost (B=8: 1900 us without, 2003 with; two groups, B=2: 741 and 765).  It goes by the
+// groups alone: one group is also what the rounds give some sizes with many CTAs (8 rows of 1024 or 1536 channels, N=16).
 template <typename T, int LN, bool FULL, bool AHEAD>
 __global__ void __launch_bounds__(kSelBwdWarps * 32, 1) sel_bwd_k(const SelArgs a) {
     using Sh = BwdShape<LN>;
@@ -967,7 +971,10 @@ cudaError_t sel_step_launch(const SelArgs& a, cudaStream_t s) {
 }
 
 // Groups of channels that a backward's CTA takes: as many as leave the fewest rounds of CTAs (one a multiprocessor) times
-// groups; of equals the most, for fewer partial rows.
+// groups; of equals the most, for fewer partial rows.  Neither the partial rows (8 bytes a padded state, token and CTA of a
+// row) nor whether the groups divide D (else every CTA takes the kernel with bounds checks, about 10 percent) is weighed:
+// B=8 L=8192 N=16 training steps take 1908 us for D=768 (6 groups, 134 MB of partial rows), 3188 for 1024 (1, 1074 MB),
+// 4915 for 1536 (1, 1611 MB) and 4755 for 2048 (7, not dividing, 310 MB).
 template <int LN>
 int sel_bwd_groups(int64_t rows, int64_t D) {
     constexpr int CW = BwdShape<LN>::CW;
