@@ -187,10 +187,12 @@ EACS_API int eacs_delta_step(const EacsDelta* p, void* o, float* final_state, vo
  * (0).  lengths (rows) int32 or NULL: a row has min(max(lengths[r], 0), L)
  * tokens; what lies behind is not read, its outputs and gradients are 0 and
  * the state stays.  initial_state (rows,D,N) float32 dense or NULL (zeros).
- * N goes up to 64.  Sums and states are float32; A <= 0 and s >= 0 are meant
- * (states that grow do so as float32 lets them).  Rows that start on 16 bytes
- * are read several channels at a time.  Outputs overlap neither one another nor
- * the inputs (a step's state apart; EacsConv and EacsNorm likewise). */
+ * N goes up to 64, rows to 65535.  Sums and states are float32; A finite and
+ * <= 0 and s >= 0 are meant (states that grow do so as float32 lets them).  Rows
+ * that start on 16 bytes are read several channels at a time, and rows of B and
+ * C whose N elements fill 16-byte pieces are copied ahead.  Outputs overlap
+ * neither one another nor the inputs (a step's state apart; EacsConv and
+ * EacsNorm likewise). */
 typedef struct EacsSelective {
     const void* x;
     const void* dt;
@@ -223,7 +225,10 @@ EACS_API size_t eacs_selective_ckpt_size(const EacsSelective* p);
  * (rows,D,N) float32 or NULL; dx, ddt, dz (rows,L,D) and dB, dC (rows,L,N)
  * dense of dtype (dz NULL without z), dA (D,N) float32, dskip and ddt_bias (D)
  * float32 or NULL, dinitial (rows,D,N) float32 or NULL.  Sums over rows, tokens
- * and channels are added in a fixed order.  The workspace is 16-byte aligned. */
+ * and channels are added in a fixed order.  The workspace is 16-byte aligned; it
+ * holds dB and dC of the CTAs of a row, 8 N' P bytes a token with N' = N rounded
+ * up to 8, 16, 32 or 64 and P = N' D / 128 / G rounded up, for the 1 to 8 groups
+ * of channels G that leave the fewest rounds of CTAs. */
 EACS_API int eacs_selective_bwd(const EacsSelective* p, const void* dy, const int64_t* dy_stride, const float* dfinal,
                                 void* dx, void* ddt, void* dz, void* dB, void* dC, float* dA, float* dskip,
                                 float* ddt_bias, float* dinitial, const void* checkpoints, size_t checkpoint_bytes,
@@ -241,8 +246,8 @@ EACS_API int eacs_selective_step(const EacsSelective* p, void* y, float* state, 
  * x (rows,L,D) of dtype with strides of row and token in elements and a dense
  * last dimension; weight (D,width) and bias (D, or NULL) of w_dtype.  A state is
  * the last width - 1 inputs, (rows,width-1,D) of dtype, oldest first;
- * initial_state may be NULL (zeros).  lengths as for EacsSelective.  Sums are
- * float32.  Vectors of channels are moved at once where pointers and strides
+ * initial_state may be NULL (zeros).  lengths and rows as for EacsSelective.
+ * Sums are float32.  Vectors of channels are moved at once where pointers and strides
  * allow it. */
 typedef struct EacsConv {
     const void* x;

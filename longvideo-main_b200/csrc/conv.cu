@@ -11,8 +11,8 @@
 // (cp.async, its own, so without a barrier between warps), and the W inputs that a token sees move through the lanes'
 // registers as pairs.  A CTA's four warps lie side by side.  Through registers the same loads left too few threads: the
 // forward took 67 us at B=4 L=16384 D=1024 bfloat16 and takes 55 (41 for its bytes), the backward at B=8 L=8192 D=768 127
-// and 75 (46).  What is left is latency and issue: two special functions and 15 instructions a value forward, 30 backward,
-// at half of the issue slots.  Runs are as long as gives every multiprocessor its warps once.  Rows of an even number of
+// and 75 (46).  What is left is latency and issue: 17 instructions of a warp for 32 values forward, 28 backward, two of them
+// special functions, at 61 and 57 percent of the issue slots.  Runs are as long as gives every multiprocessor its warps once.  Rows of an even number of
 // channels that do not start on 16 bytes are copied 4 bytes at a time; odd ones take kernels of one channel a thread.
 // The backward takes p again from x (the forward saves nothing) and keeps dweight and dbias of its run in registers: a run's
 // is one partial row, and a second kernel adds them in order (no atomics: the same inputs give the same bits).
