@@ -177,7 +177,7 @@ EACS_API int eacs_delta_step(const EacsDelta* p, void* o, float* final_state, vo
 /* The selective state space scan: a diagonal recurrence whose steps and whose
  * input and output vectors go by the token, beside the scans above (one step
  * per frame, rates that do not change).  Per row, channel d and state n, with
- * s = softplus(dt + dt_bias) (softplus != 0; 0 below e^-87, so that a dt of
+ * s = softplus(dt + dt_bias) (softplus != 0; 0 below e^-87.3, so that a dt of
  * -inf takes no step) or dt + dt_bias,
  *   h_t[n] = exp(s_t A[d,n]) h_{t-1}[n] + s_t x_t B_t[n]
  *   y_t = (sum_n C_t[n] h_t[n] + skip[d] x_t) silu(z_t).

@@ -6,16 +6,18 @@
 //   dx_t = sum_w weight[w] dp_{t+W-1-w},   dweight[w] = sum_t dp_t x_{t-W+1+w},   dbias = sum_t dp_t,
 // and what the final state's gradient adds to the last W - 1 inputs.
 //
-// Each value is read once (but for the W - 1 tokens around a run) and written once.  A warp takes 64 channels, two a lane,
-// of a run of tokens; rows of 128 (float32: 256) bytes come through shared memory, asked for three stages of 8 tokens ahead
-// (cp.async, its own, so without a barrier between warps), and the W inputs that a token sees move through the lanes'
-// registers as pairs.  A CTA's four warps lie side by side.  Through registers the same loads left too few threads: the
-// forward took 67 us at B=4 L=16384 D=1024 bfloat16 and takes 55 (41 for its bytes), the backward at B=8 L=8192 D=768 127
-// and 75 (46).  What is left is latency and issue: 17 instructions of a warp for 32 values forward, 28 backward, two of them
-// special functions, at 61 and 57 percent of the issue slots.  Runs are as long as gives every multiprocessor its warps once.  Rows of an even number of
-// channels that do not start on 16 bytes are copied 4 bytes at a time; odd ones take kernels of one channel a thread.
-// The backward takes p again from x (the forward saves nothing) and keeps dweight and dbias of its run in registers: a run's
-// is one partial row, and a second kernel adds them in order (no atomics: the same inputs give the same bits).
+// Each value is read once (but for the W - 1 tokens around a run) and written once.  A warp takes 64 channels, two a
+// lane, of a run of tokens; rows of 128 (float32: 256) bytes come through shared memory, asked for three stages of 8
+// tokens ahead (cp.async, its own, so without a barrier between warps), and the W inputs that a token sees move
+// through the lanes' registers as pairs.  A CTA's four warps lie side by side.  Through registers the same loads left
+// too few threads: the forward took 67 us at B=4 L=16384 D=1024 bfloat16 and takes 55 (41 for its bytes), the
+// backward at B=8 L=8192 D=768 127 and 75 (46).  What is left is latency and issue: 17 instructions of a warp for 32
+// values forward, 28 backward, two of them special functions, at 61 and 57 percent of the issue slots.  Runs are as
+// long as gives every multiprocessor its warps once.  Rows of an even number of channels that do not start on 16
+// bytes are copied 4 bytes at a time; odd ones take kernels of one channel a thread.
+// The backward takes p again from x (the forward saves nothing) and keeps dweight and dbias of its run in registers:
+// a run's is one partial row, and a second kernel adds them in order (no atomics: the same inputs give the same
+// bits).
 #include <algorithm>
 
 #include "eacs_common.cuh"

@@ -18,13 +18,14 @@
 // and added by the two-wide float32 instructions, which take half the issue slots.
 //
 // Measured, us: forward B=4 L=16384 D=1024 N=16 bfloat16 637; B=1 322; B=8 L=8192 D=768 485 (528 with checkpoints), the
-// backward of that 1364 and 28 for the sums of dB and dC.  What holds it off the exponentials' time is latency: 12 warps a
-// multiprocessor (backward 8) with the registers that a slice's decays and sums take, at 12 (backward 26) instructions for
-// 32 updates; the special function pipe is 45 percent busy, issue slots 59 percent (backward 18 and 47).  The backward's kernels for one
-// group a CTA spill registers for N <= 8 (116 to 168 bytes a thread; others at most 72, the forward's at most 24).  Tried and slower:
-// slices of 4 tokens with 16 or 20 warps (813 and 894 us where 8 with 12 took 745), in the backward slices of 4 with two
-// channels a thread and 12 warps (half the shared memory reads, but half again as many instructions: 2477 us a training step
-// where 1971 was), and the tokens' values of all of a CTA's groups worked out at once (2180 where 1900 was).
+// backward of that 1364 and 28 for the sums of dB and dC.  What holds it off the exponentials' time is latency: 12 warps
+// a multiprocessor (backward 8) with the registers that a slice's decays and sums take, at 12 (backward 26) instructions
+// for 32 updates; the special function pipe is 45 percent busy, issue slots 59 percent (backward 18 and 47).  The
+// backward's kernels for one group a CTA spill registers for N <= 8 (116 to 168 bytes a thread; others at most 72, the
+// forward's at most 24).  Tried and slower: slices of 4 tokens with 16 or 20 warps (813 and 894 us where 8 with 12 took
+// 745), in the backward slices of 4 with two channels a thread and 12 warps (half the shared memory reads, but half again
+// as many instructions: 2477 us a training step where 1971 was), and the tokens' values of all of a CTA's groups worked
+// out at once (2180 where 1900 was).
 //
 // The forward for training writes the state in front of every 8 tokens; the backward starts a slice from it.  Sums over
 // channels stay in registers while a warp goes through its CTA's channels, are then folded over its lanes, and a CTA writes
@@ -62,7 +63,7 @@ __device__ __forceinline__ f32x2 decays(f32x2 s2, f32x2 A) { return ex2_pair(fma
 // exact for the small steps that v << 0 gives, where log(1 + u) taken from the rounded 1 + u is not.  2 artanh(q) / q is a
 // polynomial of degree 4 in q^2, fitted on [0, 1/9] at Chebyshev's points (8e-9 of the value).  What u's argument lost, the
 // product's rounding and that of log2(e), is put back to first order (without the first u is off by |v| 2^-24, without the
-// second by |v| 2^-26): 2^-20 of the step in all.  Behind e^-87, where float32's normal numbers end, the hardware's 2^v is 0
+// second by |v| 2^-26): 2^-20 of the step in all.  Behind e^-87.3, where float32's normal numbers end, the hardware's 2^v is 0
 // (v is held to where the argument's rest is a number), so that -inf or the lowest value in dt masks a token: it takes no step.
 // slope is the derivative.
 __device__ __forceinline__ float softplus(float v, float& slope) {

@@ -10,10 +10,11 @@ on in place, for streaming.
 
 Layouts: x and y (B, L, D) of one dtype, weight (D, W) and bias (D) of one
 dtype (an nn.Conv1d's weight with its middle dimension squeezed), up to 65535
-rows (B), states (B, W - 1, D) of x's dtype: the last inputs, oldest first.  x may be a view with
-a dense last dimension (a slice of a fused projection needs no copy); rows that
-start on 16 bytes are fastest, then rows of an even number of channels.  Sums
-are float32, an output is rounded once.  The same inputs give the same bits.
+rows (B), states (B, W - 1, D) of x's dtype: the last inputs, oldest first.  x
+may be a view with a dense last dimension (a slice of a fused projection needs
+no copy); rows that start on 16 bytes are fastest, then rows of an even number of
+channels.  Sums are float32, an output is rounded once.  The same inputs give the
+same bits.
 
 Gradients are reverse mode, once; forward-mode, torch.func or traced calls are
 refused.  A backward captured into a CUDA graph must not share its leaves with

@@ -27,8 +27,8 @@ N rounded up to 8, 16, 32 or 64) until the backward, and the backward takes
 8 N P bytes a token of partial sums while it runs (N rounded up too): P, the
 CTAs of a row, is N D / (128 G) rounded up, for the 1 to 8 groups of channels G
 that leave the fewest rounds of CTAs.  One row of D=256, N=64 takes 64 KB a
-token, eight of D=768, N=16 2 KB.  A NaN or an infinity of a
-token reaches what follows it, never what lies before.
+token, eight of D=768, N=16 2 KB.  A NaN or an infinity of a token reaches what
+follows it, never what lies before.
 
 Gradients are reverse mode, once; forward-mode, torch.func or traced calls are
 refused.  A backward captured into a CUDA graph must not share its leaves with
@@ -147,8 +147,8 @@ def selective_ssm(x: Tensor, dt: Tensor, A: Tensor, B: Tensor, C: Tensor, skip: 
     (B, D, N) float32 behind the last token.
 
     softplus=False takes dt (+ dt_bias) itself as the step; a softplus below
-    e^-87 is 0, so that -inf or the dtype's lowest value in dt masks a token (its
-    channel keeps its state).  lengths (B) int32
+    e^-87.3 is 0, so that -inf or the dtype's lowest value in dt masks a token
+    (its channel keeps its state).  lengths (B) int32
     on the device: row b has lengths[b] tokens (clamped to 0..L); what lies
     behind is not read, its outputs and gradients are 0.  Differentiable in
     every floating point input, through y and the final state."""
